@@ -45,6 +45,9 @@ CUDA_SOURCES = [
     "attn_bwd3.cu",
     "attn_decode.cu",
     "decode_layer.cu",
+    "paged_cache.cu",
+    "attn_paged.cu",
+    "logits.cu",
     "transformer_block.cu",
     "comm_kernels.cu",
     "moe_kernels.cu",

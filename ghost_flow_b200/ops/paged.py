@@ -1,0 +1,254 @@
+"""A KV cache in pages: appending the keys and values of new tokens with the rotation on the way, and attention of new tokens
+(one of each sequence, chunks of prompts, whole prompts, any mix of them) over it.
+
+``kpages`` and ``vpages`` are pools ``[pages, page, Hk, D]``; row ``b`` of ``page_table`` (int32 ``[B, width]``) names the pages of
+sequence ``b`` in their order. New tokens of all sequences lie one behind the other: those of sequence ``b`` are rows ``cu[b] .. cu[b + 1] - 1``
+(``cu`` int32 ``[B + 1]``; without it every sequence has one), and ``lens[b]`` (int32) counts its keys with the new ones, so that new token
+``i`` of ``n`` stands at position ``lens[b] - n + i``. All of these stay on the device and nothing here waits for them: a captured call goes by
+what they hold when it is replayed. A sequence of no new tokens, or of no keys (an empty slot of a batch), is allowed.
+
+bf16 CUDA tensors take the kernels of ``csrc/paged_cache.cu`` and ``csrc/attn_paged.cu``; other types, layouts and CPU tensors, and calls that
+something follows (a gradient, tracing, transforms, modes), plain PyTorch. The reference has no cache (ghostflow-nn/src/gpt.rs:402-422).
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+from .fused import _observed, _rc, _rope_tables_fit_kernel, _rows_apart
+
+_INT32, _BF16 = torch.int32, torch.bfloat16
+
+
+def _check_batch(what, x, kpages, vpages, page_table, lens, cu) -> None:
+    """Raises for arguments that no batch has, whatever path it takes."""
+    if kpages.dim() != 4 or kpages.shape != vpages.shape or kpages.dtype != x.dtype or vpages.dtype != x.dtype:
+        raise ValueError(f"{what}: kpages and vpages are [pages, page, KV heads, head size] of {x.dtype}, not {list(kpages.shape)} of "
+                         f"{kpages.dtype} and {list(vpages.shape)} of {vpages.dtype}")
+    if kpages.shape[1] < 1:
+        raise ValueError(f"{what}: pages of {kpages.shape[1]} rows")
+    B = lens.shape[0] if lens.dim() == 1 else -1
+    if B < 0 or page_table.dim() != 2 or page_table.shape[0] != B or lens.dtype is not _INT32 or page_table.dtype is not _INT32:
+        raise ValueError(f"{what}: page_table is int32 [sequences, pages of each] and lens int32 [sequences], not {page_table.dtype} "
+                         f"{list(page_table.shape)} and {lens.dtype} {list(lens.shape)}")
+    if cu is not None and (cu.dtype is not _INT32 or cu.shape != (B + 1,)):
+        raise ValueError(f"{what}: cu is int32 [{B + 1}], the first token of each of {B} sequences and the end, not {cu.dtype} {list(cu.shape)}")
+    if cu is None and x.shape[0] != B:
+        raise ValueError(f"{what}: {x.shape[0]} tokens of {B} sequences need cu, the first token of each")
+    dev = x.device
+    if not (kpages.device == vpages.device == page_table.device == lens.device == dev and (cu is None or cu.device == dev)):
+        raise ValueError(f"{what}: tensors on different devices")
+
+
+def _ints_fit_kernel(page_table, lens, cu) -> bool:
+    return page_table.stride(1) == 1 and lens.is_contiguous() and (cu is None or cu.is_contiguous())
+
+
+def _pages_fit_kernel(kpages, vpages) -> bool:
+    P, page, Hk, D = kpages.shape
+    a, b = kpages.stride(), vpages.stride()
+    return (P > 0 and Hk > 0 and page >= 16 and page & (page - 1) == 0 and P * page < 2 ** 31 and a[3] == 1 and b[3] == 1
+            and not (a[0] | a[1] | a[2] | b[0] | b[1] | b[2]) & 7 and not (kpages.data_ptr() | vpages.data_ptr()) & 15)
+
+
+def _pages_apart(kpages, vpages) -> bool:
+    """Whether no two rows of the pools share memory."""
+    between = abs(kpages.data_ptr() - vpages.data_ptr()) // kpages.element_size()
+    if between >= kpages.numel() and kpages.is_contiguous() and vpages.is_contiguous():
+        return True
+    D = kpages.shape[3]
+    dims = [[*zip(t.stride()[:3], t.shape[:3])] for t in (kpages, vpages)]
+    if dims[0] == dims[1]:                 # the pools themselves are one more dimension
+        return _rows_apart(D, [*dims[0], (between, 2)])
+    ends = sorted((t.data_ptr(), t.data_ptr() + t.element_size() * (D + sum(st * (n - 1) for st, n in d)))
+                  for t, d in zip((kpages, vpages), dims))
+    return all(_rows_apart(D, d) for d in dims) and ends[0][1] <= ends[1][0]
+
+
+def _strides(kpages, vpages):
+    return (ctypes.c_longlong * 6)(*kpages.stride()[:3], *vpages.stride()[:3])
+
+
+def _wants_grad(*ts) -> bool:
+    return torch.is_grad_enabled() and any(t.requires_grad for t in ts)
+
+
+def _report(device, bad, what: str) -> None:
+    """A batch that names pages or positions that are not there: an error on the CPU, else the status word's (see ``_lib.check_status``)."""
+    if device.type != "cuda":
+        if bool(bad):
+            raise ValueError(f"{what}: a page or a position that is not there")
+        return
+    w = _lib.status_word(device)
+    w[0] = torch.where(bad & (w[0] == 0), 7, w[0])
+
+
+def _places(T, lens, cu):
+    """Sequence (that of the last one behind it), position, and whether it belongs to a sequence, of every token."""
+    B = lens.shape[0]
+    t = torch.arange(T, device=lens.device)
+    if cu is None:
+        return t, lens.long() - 1, torch.ones_like(t, dtype=torch.bool)
+    c = cu.long().clamp(0, T)
+    b = torch.searchsorted(c[1:].contiguous(), t, right=True)
+    inside = (b < B) & (t >= c[0])
+    b = b.clamp(max=max(B - 1, 0))
+    return b, lens.long()[b] - c[b + 1] + t, inside
+
+
+# ------------------------------------------------------------------------------------------ append
+def _append_ref(qkv, H, Hk, cos, sin, kpages, vpages, page_table, lens, cu, interleaved):
+    (P, page, _, D), T, dev = kpages.shape, qkv.shape[0], qkv.device
+    up = torch.promote_types(qkv.dtype, torch.float32)
+    b, pos, inside = _places(T, lens, cu)
+    here = inside & (pos >= 0)
+    fits = here & (pos < page_table.shape[1] * page) & (pos < cos.shape[0])
+    at = torch.where(fits, pos, 0)
+    stored = fits
+    if page_table.shape[1]:
+        pages = page_table.long()[b, at // page]
+        stored = fits & (pages >= 0) & (pages < P)
+    _report(dev, (here & ~stored).any(), "rope_qkv_to_pages")
+    if cos.shape[0]:
+        c, s = (t[at].to(up).unsqueeze(1) for t in (cos, sin))
+    else:
+        c = s = torch.zeros(T, 1, D // 2, dtype=up, device=dev)
+    x = qkv[:, :H + Hk].to(up)
+    lo, hi = (x[..., 0::2], x[..., 1::2]) if interleaved else x.chunk(2, -1)
+    lo, hi = lo * c - hi * s, hi * c + lo * s
+    x = torch.stack((lo, hi), -1).flatten(-2) if interleaved else torch.cat((lo, hi), -1)
+    x = x.masked_fill(~fits[:, None, None], 0).to(qkv.dtype)
+    if bool(stored.any()):
+        where = pages[stored], at[stored] % page
+        kpages[where] = x[stored, H:]
+        vpages[where] = qkv[stored, H + Hk:]
+    return x[:, :H].contiguous()
+
+
+def rope_qkv_to_pages(qkv, num_heads: int, num_kv_heads: int, cos, sin, kpages, vpages, page_table, lens, cu=None,
+                      interleaved: bool = False):
+    """Rotated q ``[T, H, D]`` of a packed projection output ``[T, H + 2 Hk, D]`` of new tokens; rotated k and v go to the rows of their
+    positions in the pages (see the module). ``cos`` and ``sin`` as for :func:`rope`, a row for each position. Two sequences may share
+    pages, but not rows that are written here. Tokens behind the last sequence are left out, and their rows of q are not written; those of
+    a sequence that holds fewer keys than new tokens give zeros where their position is below 0. A page that is not in the pools,
+    or a position that is not in the tables or behind the page table, is left out too, and ``_lib.check_status`` raises.
+    Inference only: a call with a gradient to record takes PyTorch's operations."""
+    H, Hk = num_heads, num_kv_heads
+    what = "rope_qkv_to_pages"
+    if qkv.dim() != 3 or qkv.shape[1] != H + 2 * Hk or H < 1 or Hk < 1:
+        raise ValueError(f"{what}: a packed projection of {H} + 2 x {Hk} heads is [tokens, {H + 2 * Hk}, head size], not {list(qkv.shape)}")
+    _check_batch(what, qkv, kpages, vpages, page_table, lens, cu)
+    T, _, D = qkv.shape
+    dev = qkv.device
+    if kpages.shape[2] != Hk or kpages.shape[3] != D:
+        raise ValueError(f"{what}: pages of {kpages.shape[2]} heads of {kpages.shape[3]} for {Hk} heads of {D}")
+    if not (cos.dim() == 2 and cos.shape == sin.shape and 2 * cos.shape[1] == D and cos.device == sin.device == dev):
+        raise ValueError(f"{what}: rope tables must be [positions, {D // 2}] on {dev}, got {list(cos.shape)} on {cos.device} and "
+                         f"{list(sin.shape)} on {sin.device}")
+    if T == 0:
+        return qkv.new_empty(0, H, D)
+    if not (qkv.is_cuda and qkv.dtype is _BF16) or _wants_grad(qkv, kpages, vpages) or _observed() or D % 16 or D > 4096 \
+            or not _ints_fit_kernel(page_table, lens, cu) or not _pages_fit_kernel(kpages, vpages) or not _pages_apart(kpages, vpages) \
+            or not _rope_tables_fit_kernel(cos, sin):
+        return _append_ref(qkv, H, Hk, cos, sin, kpages, vpages, page_table, lens, cu, interleaved)
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return rope_qkv_to_pages(qkv, H, Hk, cos, sin, kpages, vpages, page_table, lens, cu, interleaved)
+    if qkv.stride(2) != 1 or qkv.stride(1) != D or qkv.stride(0) % 8 or qkv.data_ptr() % 16:
+        qkv = qkv.clone(memory_format=torch.contiguous_format)
+    q = torch.empty((T, H, D), dtype=_BF16, device=dev)
+    _rc(_lib.cuda_lib().gf_paged_append(
+        qkv.data_ptr(), qkv.stride(0), q.data_ptr(), kpages.data_ptr(), vpages.data_ptr(), _strides(kpages, vpages),
+        page_table.data_ptr(), page_table.stride(0), page_table.shape[1], lens.data_ptr(), None if cu is None else cu.data_ptr(),
+        lens.shape[0], T, H, Hk, D, kpages.shape[1], kpages.shape[0], cos.data_ptr(), sin.data_ptr(), cos.shape[0],
+        1 if interleaved else 0, _lib.status_word(dev).data_ptr(), _lib.stream_ptr()), "gf_paged_append")
+    torch.autograd.graph.increment_version((kpages, vpages))     # a graph that saved the pools has to notice the write
+    return q
+
+
+# ------------------------------------------------------------------------------------------ attention
+def _attention_ref(q, kpages, vpages, page_table, lens, cu, scale, out):
+    (P, page, Hk, D), (T, H, _), dev, B = kpages.shape, q.shape, q.device, lens.shape[0]
+    up = torch.promote_types(q.dtype, torch.float32)
+    ends = list(range(B + 1)) if cu is None else cu.clamp(0, T).tolist()
+    bad, at, pieces = torch.zeros((), dtype=torch.bool, device=dev), 0, []
+    for b, length in enumerate(lens.tolist()):
+        n = max(0, min(length, page_table.shape[1] * page))
+        s, e = ends[b], ends[b + 1]
+        if n != length:
+            bad = bad | True
+        if e <= s:
+            continue
+        pages = page_table[b, :(n + page - 1) // page].long()
+        there = (pages >= 0) & (pages < P)
+        bad = bad | ~there.all()
+        k, v = (x[pages.clamp(0, max(P - 1, 0))].to(up).masked_fill(~there[:, None, None, None], 0).flatten(0, 1)[:n] if P else
+                torch.zeros(n, Hk, D, dtype=up, device=dev) for x in (kpages, vpages))
+        x = torch.einsum("thgd,nhd->hgtn", q[s:e].to(up).unflatten(1, (Hk, H // Hk)), k) * scale
+        last = length - (e - s) + torch.arange(e - s, device=dev)
+        hidden = torch.arange(n, device=dev) > last[:, None]
+        x = torch.softmax(x.masked_fill(hidden, float("-inf")), -1).masked_fill(hidden, 0)     # rows without a key: zeros
+        o = torch.einsum("hgtn,nhd->thgd", x, v).flatten(1, 2).to(q.dtype)
+        if out is not None:
+            out[s:e] = o
+        else:
+            pieces += [q.new_zeros(s - at, H, D), o] if s > at else [o]
+            at = e
+    _report(dev, bad, "paged_attention")
+    if out is not None:
+        return out
+    return torch.cat([*pieces, q.new_zeros(T - at, H, D)])
+
+
+def _ranges_overlap(a, b) -> bool:
+    def span(t):
+        return t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum(s * (n - 1) for s, n in zip(t.stride(), t.shape)))
+
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
+def paged_attention(q, kpages, vpages, page_table, lens, cu=None, scale: float | None = None, out=None):
+    """Causal attention of new tokens ``q [T, Hq, D]`` over the keys of their sequences in the pages (see the module), which hold the new
+    tokens' own already: a token at position ``p`` sees the keys ``0 .. p``. A token that sees none gives zeros; tokens behind
+    the last sequence are not written. What the pages hold behind a sequence's last key does not matter. ``out [T, Hq, D]``, where given, is
+    written and returned. A page that is not in the pools reads as zeros, keys behind the page table do not exist, and
+    ``_lib.check_status`` raises for both. Head sizes 64 and 128 with pages of a power of two from 16 rows take the kernels.
+    Inference only: a call with a gradient to record takes PyTorch's operations."""
+    what = "paged_attention"
+    if q.dim() != 3:
+        raise ValueError(f"{what}: q is [tokens, heads, head size], not {list(q.shape)}")
+    _check_batch(what, q, kpages, vpages, page_table, lens, cu)
+    T, H, D = q.shape
+    Hk, dev = kpages.shape[2], q.device
+    if kpages.shape[3] != D or Hk < 1 or H < 1 or H % Hk:
+        raise ValueError(f"{what}: {H} heads of {D} over pages of {Hk} heads of {kpages.shape[3]}")
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != dev):
+        raise ValueError(f"{what}: out is {list(q.shape)} of {q.dtype} on {dev}, not {list(out.shape)} of {out.dtype} on {out.device}")
+    if T == 0:
+        return torch.empty_like(q) if out is None else out
+    if out is not None and (_ranges_overlap(out, q) or _ranges_overlap(out, kpages) or _ranges_overlap(out, vpages)):
+        raise ValueError(f"{what}: out shares memory with q or the pages")
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    if not (q.is_cuda and q.dtype is _BF16) or D not in (64, 128) or _wants_grad(q, kpages, vpages) or _observed() \
+            or not _ints_fit_kernel(page_table, lens, cu) or not _pages_fit_kernel(kpages, vpages) \
+            or (out is not None and (out.stride(2) != 1 or out.stride(1) != D or out.stride(0) % 8 or out.stride(0) < H * D
+                                     or out.data_ptr() % 16)):
+        return _attention_ref(q, kpages, vpages, page_table, lens, cu, scale, out)
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return paged_attention(q, kpages, vpages, page_table, lens, cu, scale, out)
+    if q.stride(2) != 1 or q.stride(1) != D or q.stride(0) % 8 or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
+    o = torch.empty((T, H, D), dtype=_BF16, device=dev) if out is None else out
+    _rc(_lib.cuda_lib().gf_paged_attn(
+        q.data_ptr(), q.stride(0), kpages.data_ptr(), vpages.data_ptr(), _strides(kpages, vpages), page_table.data_ptr(),
+        page_table.stride(0), page_table.shape[1], lens.data_ptr(), None if cu is None else cu.data_ptr(), o.data_ptr(), o.stride(0),
+        lens.shape[0], T, H, Hk, D, kpages.shape[1], kpages.shape[0], scale, _lib.status_word(dev).data_ptr(), _lib.stream_ptr()),
+        "gf_paged_attn")
+    if out is not None:
+        torch.autograd.graph.increment_version(out)
+    return o

@@ -1,0 +1,131 @@
+"""What stands between a model's logits and the choice of a token: penalties for tokens that are there already, biases, and masks of the
+tokens that a grammar allows. The reference picks the largest logit (ghostflow-nn/src/gpt.rs:402-422).
+
+CUDA logits of fp32, bf16 or fp16 take the kernel of ``csrc/logits.cu``; CPU tensors, other layouts, and calls that something follows (a
+gradient, tracing, transforms, modes) plain PyTorch."""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from .fused import _observed, _rc
+from .paged import _ranges_overlap
+
+_KINDS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def pack_allowed(mask):
+    """Bits of a truth-valued mask ``[..., V]`` for :func:`process_logits`: int32 ``[..., ceil(V / 32)]``, entry ``v`` is bit ``v % 32`` of word
+    ``v // 32``."""
+    V = mask.shape[-1]
+    m = torch.nn.functional.pad(mask.to(torch.int64), (0, -V % 32)).unflatten(-1, (-1, 32))
+    words = (m << torch.arange(32, device=mask.device)).sum(-1)
+    return torch.where(words >= 2 ** 31, words - 2 ** 32, words).to(torch.int32)
+
+
+def _logits_ref(x, tokens, token_lens, generated_from, repetition, presence, frequency, bias, allowed):
+    B, V = x.shape
+    y = x.to(torch.promote_types(x.dtype, torch.float32))
+
+    def column(a):
+        return a[:, None] if torch.is_tensor(a) else a
+
+    if tokens is not None and tokens.shape[1] > 0:
+        t, j = tokens.long(), torch.arange(tokens.shape[1], device=x.device)
+        there = (t >= 0) & (t < V)
+        if token_lens is not None:
+            there = there & (j < token_lens[:, None])
+        new = there if generated_from is None else there & (j >= generated_from[:, None])
+        t = torch.where(there, t, 0)
+        seen, count = (torch.zeros(B, V, dtype=torch.int32, device=x.device).scatter_add_(1, t, m.int()) for m in (there, new))
+        r = column(repetition)
+        y = torch.where(seen > 0, torch.where(y > 0, y / r, y * r), y)
+        change = count * column(frequency) + torch.where(count > 0, column(presence), 0.0)
+        y = torch.where(seen > 0, y - change, y)
+    if bias is not None:
+        y = y + bias
+    if allowed is not None:
+        v = torch.arange(V, device=x.device)
+        y = y.masked_fill((allowed[..., v // 32] >> (v % 32)) & 1 == 0, float("-inf"))
+    return y.to(x.dtype)
+
+
+def process_logits(logits, tokens=None, token_lens=None, generated_from=None, repetition=1.0, presence=0.0, frequency=0.0, bias=None,
+                   allowed=None, out=None):
+    """Logits ``[B, V]`` ready for the choice of a token. For an entry that stands ``c`` times among the row's generated tokens, in this order:
+    if the row's ``tokens`` hold it at all, ``x / repetition`` where ``x > 0`` and ``x * repetition`` elsewhere, and then
+    ``x - (c * frequency + presence where c > 0)``; ``x + bias``; ``-inf`` unless ``allowed``. Computed in 32 bits and rounded once.
+
+    ``tokens [B, L]``, int32 or int64, holds ``token_lens[b]`` tokens (int32 ``[B]``; all ``L``) of which those from ``generated_from[b]``
+    (int32 ``[B]``; 0) are generated ones, those before them the prompt; a token outside the vocabulary (padding) is passed over. The
+    three penalties are numbers or fp32 ``[B]``. ``bias``: fp32 ``[V]`` or ``[B, V]``. ``allowed``: int32 bits ``[words]`` or ``[B, words]``
+    (:func:`pack_allowed`). ``out`` may be ``logits`` itself. A row of which nothing is allowed is all ``-inf``."""
+    what = "process_logits"
+    if logits.dim() != 2 or not logits.is_floating_point():
+        raise ValueError(f"{what}: logits are [rows, vocabulary], not {logits.dtype} {list(logits.shape)}")
+    (B, V), dev = logits.shape, logits.device
+    if tokens is not None:
+        if tokens.dim() != 2 or tokens.shape[0] != B or tokens.dtype not in (torch.int32, torch.int64) or tokens.device != dev:
+            raise ValueError(f"{what}: tokens are int32 or int64 [{B}, most of a row] on {dev}, not {tokens.dtype} {list(tokens.shape)} on "
+                             f"{tokens.device}")
+        for name, t in (("token_lens", token_lens), ("generated_from", generated_from)):
+            if t is not None and (t.shape != (B,) or t.dtype is not torch.int32 or t.device != dev):
+                raise ValueError(f"{what}: {name} is int32 [{B}] on {dev}, not {t.dtype} {list(t.shape)} on {t.device}")
+    elif token_lens is not None or generated_from is not None:
+        raise ValueError(f"{what}: token_lens and generated_from go with tokens")
+    for name, t in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
+        if torch.is_tensor(t):
+            if t.shape != (B,) or t.dtype is not torch.float32 or t.device != dev:
+                raise ValueError(f"{what}: {name} is a number or fp32 [{B}] on {dev}, not {t.dtype} {list(t.shape)} on {t.device}")
+    if not torch.is_tensor(repetition) and not repetition > 0:
+        raise ValueError(f"{what}: repetition is above 0, not {repetition}")
+    if bias is not None and (bias.shape not in ((V,), (B, V)) or bias.dtype is not torch.float32 or bias.device != dev):
+        raise ValueError(f"{what}: bias is fp32 [{V}] or [{B}, {V}] on {dev}, not {bias.dtype} {list(bias.shape)} on {bias.device}")
+    words = (V + 31) // 32
+    if allowed is not None and (allowed.dtype is not torch.int32 or allowed.shape not in ((words,), (B, words)) or allowed.device != dev):
+        raise ValueError(f"{what}: allowed is int32 [{words}] or [{B}, {words}] on {dev}, not {allowed.dtype} {list(allowed.shape)} on "
+                         f"{allowed.device}")
+    inplace = False
+    if out is not None:
+        if out.shape != logits.shape or out.dtype != logits.dtype or out.device != dev:
+            raise ValueError(f"{what}: out is {list(logits.shape)} of {logits.dtype} on {dev}, not {list(out.shape)} of {out.dtype} on "
+                             f"{out.device}")
+        inplace = out is logits or (out.data_ptr() == logits.data_ptr() and out.stride() == logits.stride())
+        if not inplace and logits.numel() and _ranges_overlap(out, logits):
+            raise ValueError(f"{what}: out shares memory with logits and is not logits")
+    if B == 0 or V == 0:
+        return torch.empty_like(logits) if out is None else out
+    tensors = [t for t in (logits, bias, repetition, presence, frequency, out) if torch.is_tensor(t)]
+    y = out
+    if not logits.is_cuda or logits.dtype not in _KINDS or _observed() or logits.stride(1) != 1 \
+            or (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)) \
+            or (out is not None and (out.stride(1) != 1 or (B > 1 and out.stride(0) < V))) \
+            or any(t is not None and t.stride(-1) != 1 for t in (tokens, bias, allowed)) \
+            or any(torch.is_tensor(t) and not t.is_contiguous() for t in (token_lens, generated_from, repetition, presence, frequency)):
+        y = _logits_ref(logits, tokens, token_lens, generated_from, repetition, presence, frequency, bias, allowed)
+        return y if out is None else out.copy_(y)
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return process_logits(logits, tokens, token_lens, generated_from, repetition, presence, frequency, bias, allowed, out)
+    if y is None:
+        # rows as far apart as they are, where they are apart: they then begin on the same boundaries
+        ld = logits.stride(0)
+        y = torch.empty((B, ld), dtype=logits.dtype, device=dev)[:, :V] if V <= ld < V + 64 else torch.empty_like(
+            logits, memory_format=torch.contiguous_format)
+
+    def pointer(t):
+        return t.data_ptr() if torch.is_tensor(t) else None
+
+    def number(t, otherwise):
+        return otherwise if torch.is_tensor(t) else float(t)
+
+    _rc(_lib.cuda_lib().gf_process_logits(
+        logits.data_ptr(), logits.stride(0), y.data_ptr(), y.stride(0), _KINDS[logits.dtype], B, V, pointer(tokens),
+        0 if tokens is None else tokens.stride(0), 0 if tokens is None else int(tokens.dtype is torch.int64),
+        0 if tokens is None else tokens.shape[1], pointer(token_lens), pointer(generated_from), pointer(repetition), pointer(presence),
+        pointer(frequency), number(repetition, 1.0), number(presence, 0.0), number(frequency, 0.0), pointer(bias),
+        0 if bias is None or bias.dim() == 1 else bias.stride(0), pointer(allowed),
+        0 if allowed is None or allowed.dim() == 1 else allowed.stride(0), _lib.stream_ptr()), "gf_process_logits")
+    if out is not None:
+        torch.autograd.graph.increment_version(out)
+    return y

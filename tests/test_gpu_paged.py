@@ -1,0 +1,248 @@
+"""Kernels over a paged cache against the definitions in 64 bits: lengths, heads, pages, layouts, empty sequences, what lies around."""
+import pytest
+import torch
+
+import _paged_oracle as oracle
+
+pytestmark = pytest.mark.gpu
+
+BATCHES = {"one": ([1], [1]), "two keys": ([2], [1]), "one each": ([1, 63, 64, 65, 128, 129, 300], [1] * 7),
+           "empty slots": ([0, 17, 0, 130], [1, 1, 0, 1]), "prompt": ([130], [130]), "prompts": ([5, 128, 257, 31], [5, 128, 257, 31]),
+           "chunk": ([385], [100]), "chunk behind a page": ([272], [16]), "mixed": ([300, 1, 77, 400, 0, 200], [1, 1, 30, 129, 0, 1]),
+           "fewer keys than tokens": ([3, 20, 0], [9, 4, 2]), "more than 32 sequences": ([*range(1, 40)], [1 + b % 3 for b in range(39)])}
+HEADS = [(1, 1, 64), (4, 2, 64), (6, 2, 128), (5, 1, 128), (8, 1, 64), (16, 1, 128), (12, 12, 64), (3, 1, 128)]
+
+
+def _attend(s, cu=True, **kw):
+    from ghost_flow_b200 import ops
+
+    return ops.paged_attention(s["q"], s["kp"], s["vp"], s["table"], s["lens"], s["cu"] if cu else None, **kw)
+
+
+@pytest.mark.parametrize("name", BATCHES)
+@pytest.mark.parametrize("H,Hk,D", HEADS)
+def test_attention(name, H, Hk, D, kernel_status):
+    lens, new = BATCHES[name]
+    lens = [max(n, 0) for n in lens]
+    s = oracle.batch(lens, new, H, Hk, D, 16 if D == 64 else 32, device="cuda", behind=3)
+    want, off = oracle.attention(s)
+    out = torch.full_like(s["q"], 7.0)
+    _attend(s, out=out)
+    n = sum(new)
+    oracle.close(out[:n], want[:n], off[:n], name)
+    assert (out[n:] == 7).all()                          # behind the last sequence
+    assert torch.equal(_attend(s)[:n], out[:n])
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("layout", ["dense", "heads first", "together"])
+@pytest.mark.parametrize("H,Hk,D", [(4, 2, 64), (8, 2, 128)])
+def test_attention_pages_and_layouts(page, layout, H, Hk, D, kernel_status):
+    lens, new = [page - 1, page, page + 1, 3 * page + 5, 300], [1, 2, page + 1, 40, 1]
+    s = oracle.batch(lens, new, H, Hk, D, page, device="cuda", layout=layout)
+    want, off = oracle.attention(s)
+    oracle.close(_attend(s), want, off)
+
+
+@pytest.mark.parametrize("H,Hk,D", [(4, 2, 64), (8, 1, 128), (16, 1, 64)])
+@pytest.mark.parametrize("scale", [None, 0.02, -0.3])
+def test_attention_of_one_token_each(H, Hk, D, scale, kernel_status):
+    lens = [1, 16, 17, 0, 64, 1000, 515]
+    s = oracle.batch(lens, [1] * len(lens), H, Hk, D, 16, device="cuda")
+    want, off = oracle.attention(s, scale)
+    oracle.close(_attend(s, cu=False, scale=scale), want, off)
+
+
+@pytest.mark.parametrize("lens,new", [([9000], [1]), ([5000, 3], [1, 1]), ([4000, 700], [40, 300]), ([20000], [3])])
+@pytest.mark.parametrize("H,Hk,D", [(4, 1, 128), (4, 4, 64)])
+def test_attention_over_long_sequences(lens, new, H, Hk, D, kernel_status):
+    s = oracle.batch(lens, new, H, Hk, D, 64, device="cuda")
+    want, off = oracle.attention(s)
+    oracle.close(_attend(s), want, off)
+
+
+def test_attention_with_scores_far_apart(kernel_status):
+    """Maxima that move by a lot, upwards and downwards along the keys, and scores of the type's size."""
+    for sizes in ((0.01, 40), (40, 0.01)):
+        s = oracle.batch([700, 300], [130, 1], 4, 2, 64, 32, device="cuda")
+        rows = torch.arange(700, device="cuda")
+        at = s["table"][0, rows // 32].long(), rows % 32
+        s["kp"][at] = (s["kp"][at].float() * torch.linspace(*sizes, 700, device="cuda")[:, None, None]).bfloat16()
+        want, off = oracle.attention(s)
+        oracle.close(_attend(s), want, off)
+
+
+def test_attention_of_views(kernel_status):
+    """q as a part of a packed projection, out with rows further apart."""
+    s = oracle.batch([40, 300], [7, 33], 6, 2, 64, 16, device="cuda")
+    packed = torch.randn(40, 10, 64, device="cuda").bfloat16()
+    packed[:, :6] = s["q"]
+    wide = torch.full((40, 8, 64), 7.0, device="cuda", dtype=torch.bfloat16)
+    want, off = oracle.attention(s)
+    from ghost_flow_b200 import ops
+    got = ops.paged_attention(packed[:, :6], s["kp"], s["vp"], s["table"], s["lens"], s["cu"], out=wide[:, 1:7])
+    oracle.close(got, want, off)
+    assert (wide[:, 0] == 7).all() and (wide[:, 7] == 7).all()
+    odd = s["q"].transpose(1, 2).contiguous().transpose(1, 2)        # a layout that is copied first
+    oracle.close(ops.paged_attention(odd, s["kp"], s["vp"], s["table"], s["lens"], s["cu"]), want, off)
+
+
+def test_attention_without_kernels_for_it(kernel_status):
+    """Types, head sizes and pages that PyTorch's operations take."""
+    for D, page, dtype in [(32, 16, torch.bfloat16), (64, 24, torch.bfloat16), (64, 16, torch.float32), (64, 16, torch.float16)]:
+        s = oracle.batch([40, 300, 0], [7, 33, 1], 6, 2, D, page, dtype, device="cuda")
+        want, off = oracle.attention(s)
+        oracle.close(_attend(s), want, off + 2 ** -20)
+
+
+@pytest.mark.parametrize("name", BATCHES)
+@pytest.mark.parametrize("H,Hk,D,layout", [(1, 1, 16, "dense"), (4, 2, 64, "together"), (25, 25, 64, "dense"), (32, 8, 128, "heads first"),
+                                           (5, 1, 80, "dense"), (40, 40, 128, "dense"), (2, 1, 256, "dense")])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_append(name, H, Hk, D, layout, interleaved, kernel_status):
+    from ghost_flow_b200 import ops
+
+    lens, new = BATCHES[name]
+    s = oracle.batch(lens, new, H, Hk, D, 16 if D == 64 else 32, device="cuda", layout=layout, behind=2)
+    cos, sin = ops.rope_tables(512, D, 1e4, "cuda")
+    q, qo, k, ko, v = oracle.append(s, H, Hk, cos, sin, interleaved)
+    with torch.no_grad():
+        got = ops.rope_qkv_to_pages(s["qkv"], H, Hk, cos, sin, s["kp"], s["vp"], s["table"], s["lens"], s["cu"], interleaved)
+    n = sum(new)
+    oracle.close(got[:n], q[:n], qo[:n])
+    oracle.close(s["kp"], k, ko)
+    oracle.close(s["vp"], v, 0.0)
+
+
+def test_append_then_attend_is_attention_of_the_whole(kernel_status):
+    """A prompt in chunks and token by token, against the whole prompt through the dense operators."""
+    from ghost_flow_b200 import ops
+
+    H, Hk, D, page, S = 8, 2, 64, 16, 200
+    cos, sin = ops.rope_tables(256, D, 1e4, "cuda")
+    x = torch.randn(2, S, H + 2 * Hk, D, device="cuda").bfloat16()
+    with torch.no_grad():
+        q, k, v = ops.rope_qkv(x, H, Hk, cos, sin)
+        whole = ops.flash_attention(q, k, v)
+        kp, vp = (torch.full((40, page, Hk, D), float("nan"), device="cuda", dtype=torch.bfloat16) for _ in range(2))
+        table = torch.randperm(40, device="cuda").int()[:26].view(2, 13)
+        at, got = [0, 0], [[], []]
+        for step in [(100, 1), (1, 60), (0, 17), (50, 50), (1, 1), (47, 71), (1, 0)]:
+            lens = [a + n for a, n in zip(at, step)]
+            cu = torch.tensor([0, step[0], sum(step)], dtype=torch.int32, device="cuda")
+            new = torch.cat([x[b, at[b]:lens[b]] for b in range(2)])
+            n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+            o = ops.paged_attention(ops.rope_qkv_to_pages(new, H, Hk, cos, sin, kp, vp, table, n, cu), kp, vp, table, n, cu)
+            for b in range(2):
+                got[b].append(o[int(cu[b]):int(cu[b + 1])])
+            at = lens
+    assert at == [S, S]
+    got = torch.stack([torch.cat(g) for g in got])
+    # both round probabilities and results to bf16: half a step each, of sums of |v| (below 4) at most twice
+    assert (got.float() - whole.float()).abs().max() < 4 * 4 * 2 ** -8
+    assert (got.float() - whole.float()).norm() / whole.float().norm() < 2 * 2 ** -8
+
+
+def test_pages_and_positions_that_are_not_there():
+    """Left out, and reported: nothing around them changes."""
+    from ghost_flow_b200 import ops
+    from ghost_flow_b200.ops import _lib
+
+    cos, sin = ops.rope_tables(64, 64, 1e4, "cuda")
+    for change, raises in [(lambda s: s["table"].__setitem__((1, 1), 10 ** 6), True), (lambda s: s["table"].__setitem__((1, 1), -5), True),
+                           (lambda s: s["lens"].__setitem__(1, 10 ** 6), True), (lambda s: None, False)]:
+        for new in ([1, 1], [1, 20]):
+            s = oracle.batch([7, 20], new, 4, 2, 64, 16, device="cuda")
+            before = s["kp"].clone(), s["vp"].clone()
+            change(s)
+            _lib.check_status()
+            a = _attend(s)
+            assert torch.isfinite(a[:1]).all()
+            if raises:
+                with pytest.raises(_lib.KernelStatusError):
+                    _lib.check_status()
+            ops.rope_qkv_to_pages(s["qkv"], 4, 2, cos, sin, s["kp"], s["vp"], s["table"], s["lens"], s["cu"])
+            if raises:
+                with pytest.raises(_lib.KernelStatusError):
+                    _lib.check_status()
+                page = s["table"][1, 0]                      # other rows keep what they held
+                rest = torch.ones(s["kp"].shape[0], dtype=torch.bool, device="cuda")
+                rest[page], rest[s["table"][0, 0]] = False, False
+                for x, y in zip((s["kp"], s["vp"]), before):
+                    assert torch.equal(x[rest].nan_to_num(3), y[rest].nan_to_num(3))
+            _lib.check_status()
+
+
+def test_replayed_calls_go_by_what_the_lengths_hold(kernel_status):
+    from ghost_flow_b200 import ops
+
+    H, Hk, D = 8, 2, 64
+    s = oracle.batch([200, 330, 5], [1, 1, 1], H, Hk, D, 16, device="cuda")
+    cos, sin = ops.rope_tables(512, D, 1e4, "cuda")
+    pools = s["kp"].clone(), s["vp"].clone()
+
+    def step(kp, vp):
+        q = ops.rope_qkv_to_pages(s["qkv"], H, Hk, cos, sin, kp, vp, s["table"], s["lens"])
+        return ops.paged_attention(q, kp, vp, s["table"], s["lens"])
+
+    with torch.no_grad():
+        step(s["kp"], s["vp"])
+        graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+        for g in graphs:                                    # two of them, that could share a workspace
+            with torch.cuda.graph(g):
+                outs.append(step(s["kp"], s["vp"]))
+        for lens in ([200, 330, 5], [17, 0, 1], [199, 64, 3]):
+            s["lens"].copy_(torch.tensor(lens, dtype=torch.int32))
+            for x, y in zip((s["kp"], s["vp"]), pools):
+                x.copy_(y)
+            want = step(s["kp"], s["vp"])
+            for x, y in zip((s["kp"], s["vp"]), pools):
+                x.copy_(y)
+            for g, o in zip(graphs, outs):
+                g.replay()
+            for o in outs:
+                assert torch.equal(o, want)
+
+
+def test_two_streams_at_once(kernel_status):
+    batches = [oracle.batch([3000 + 7 * i, 40], [1, 33], 8, 2, 128, 32, device="cuda", seed=i) for i in range(4)]
+    want = [_attend(s) for s in batches]
+    streams = [torch.cuda.Stream() for _ in batches]
+    torch.cuda.synchronize()
+    got = [None] * len(batches)
+    for _ in range(3):
+        for i, (s, st) in enumerate(zip(batches, streams)):
+            with torch.cuda.stream(st):
+                got[i] = _attend(s)
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+def test_writes_are_visible_to_autograd_and_to_dispatch_modes():
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    from ghost_flow_b200 import ops
+
+    s = oracle.batch([7, 20], [1, 2], 4, 2, 64, 16, device="cuda")
+    kp, vp = s["kp"].nan_to_num(0, 0, 0), s["vp"].nan_to_num(0, 0, 0)
+    cos, sin = ops.rope_tables(64, 64, 1e4, "cuda")
+    args = s["table"], s["lens"], s["cu"]
+    w = torch.ones_like(kp, requires_grad=True)
+    for saved in (kp, vp):
+        y = (saved * w).sum()
+        with torch.no_grad():
+            ops.rope_qkv_to_pages(s["qkv"], 4, 2, cos, sin, kp, vp, *args)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    seen = []
+
+    class Mode(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, a=(), kw=None):
+            seen.append(func._schema.name)
+            return func(*a, **(kw or {}))
+
+    want = ops.paged_attention(s["q"], kp, vp, *args)
+    with torch.no_grad(), Mode():
+        got = ops.paged_attention(s["q"], kp, vp, *args)
+    assert "aten::_softmax" in seen and (got.float() - want.float()).abs().max() < 2 ** -4
