@@ -1,88 +1,781 @@
 // Attention of new tokens over a paged KV cache (see paged.cuh), grouped-query aware.
 //
-// o = sum_j softmax_j(scale q . k_j) v_j over the keys j <= p of the token's sequence, p its position. One warp has one token and one query
-// head, goes through the keys one by one and keeps the running maximum and sum.
+// o = sum_j softmax_j(scale q . k_j) v_j over the keys j <= p of the token's sequence, p its position.
+//
+// A CTA works on one KV head and a block of new tokens of one sequence, over all keys or a part of them. The G = Hq / Hkv query heads of the KV head
+// are packed with the tokens into the 128 rows of a tile (row = token * G + head), so that keys and values are read once for all of them
+// whatever G is. The dataflow is that of attn_fwd3.cu: S = Q K^T in tensor memory, a softmax thread to a row, P back into tensor memory as the
+// A operand of O += P V, the output rescaled only when a row's maximum has grown by 2^8; tiles of 128 keys, assembled by TMA from the
+// sequence's pages (one box for a page's rows, or a part of a longer page) into the same swizzled layout. What is different:
+//
+//  * Two tiles to a CTA. With more than 128 rows they are two tiles of rows that share the keys; with 128 or less (single tokens, short
+//    chunks) they are the same rows at every other 128 keys, added up at the end: one tile alone would wait for its own softmax.
+//  * Work is dealt out on the device, from the lengths as they are at that time: a warp of every CTA scans them. Where the blocks do not fill the
+//    machine, the keys of every block are cut into pieces whose results a second kernel joins (see paged_plan).
+//  * Rows behind a sequence's last key may hold anything. Scores there are set to -inf, but a product takes 0 * V too, so an idle warp clears those
+//    rows of V in shared memory before the tile is handed on. Pages that are not there, and those behind the last, are zeros from TMA (a
+//    coordinate outside of the pool).
 #include "paged.cuh"
 
 namespace gf {
 
+constexpr int PG_TILE = 128;      // rows of a tile, keys of a step
+constexpr int PG_THREADS = 384;   // warpgroup 0: TMA warp, MMA warp, warp that clears rows, an idle one; warpgroups 1 and 2: softmax of tile 0 / 1
+constexpr int PG_REGS_CTRL = 104; // 128 x 104 + 256 x 200 = 64512, the block's own at launch (384 x 168)
+constexpr int PG_REGS_SOFTMAX = 200;
+constexpr int PG_PARTS = 2;       // P V of a tile is issued in this many parts of the keys
+constexpr float PG_RESCALE = 8.0f;  // log2 units
+constexpr int PG_WHOLE = 1 << 30;   // steps of a piece where no block is cut
+
 struct PagedAttn {
   PagedBatch seqs;
-  const __nv_bfloat16* q;        // [T, Hq, D], rows ldq apart
-  long long ldq;
-  const __nv_bfloat16 *kp, *vp;
-  long long kpage, krow, khead, vpage, vrow, vhead;
+  int Hq, Hkv, G, tq;            // G = Hq / Hkv, tq = 128 / G tokens of a tile
+  int slots;                     // CTAs that run at a time; 0: no block is cut
+  float scale;
   __nv_bfloat16* out;            // [T, Hq, D], rows ldo apart
   long long ldo;
-  int Hq, Hkv;
-  float scale_log2;
+  int* plan;                     // keys (in steps) of a piece, for the kernel that joins pieces
+  float* part;                   // [item][rows][D], then [item][rows][maximum, sum]
+  float* part_ml;
+  int rows, items;               // rows of an item in `part`, and CTAs
 };
 
-template <int D>
-__global__ void __launch_bounds__(128) paged_attn_kernel(const __grid_constant__ PagedAttn p) {
-  constexpr int E = D / 32;      // elements of a lane
-  const PagedBatch& S = p.seqs;
-  const int t = blockIdx.x, h = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int b = paged_seq_of(S, t);
-  if (b >= S.B || h >= p.Hq) return;
-  const int first = S.first(b), end = S.end(b);
-  if (t < first || t >= end) return;
-  const int len = S.lens[b], keys = (int)min((long long)max(len, 0), S.capacity());
-  if (len != keys && lane == 0) S.bad();
-  const int n = min(len - (end - first) + (t - first) + 1, keys), hk = h / (p.Hq / p.Hkv);
-  float q[E], o[E], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    q[e] = __bfloat162float(p.q[t * p.ldq + h * D + lane * E + e]);
-    o[e] = 0.f;
-  }
-  for (int j = 0; j < n; ++j) {
-    const int page = S.table[(long long)b * S.ld + (j >> S.page_shift)], r = j & ((1 << S.page_shift) - 1);
-    const bool there = page >= 0 && page < S.pages;
-    if (!there && lane == 0) S.bad();
-    float x = 0.f, v[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      x += there ? q[e] * __bfloat162float(p.kp[page * p.kpage + r * p.krow + hk * p.khead + lane * E + e]) : 0.f;
-      v[e] = there ? __bfloat162float(p.vp[page * p.vpage + r * p.vrow + hk * p.vhead + lane * E + e]) : 0.f;
+struct PgShape {                 // what a sequence is cut into
+  int n, len, keys, blocks, steps;
+};
+__device__ __forceinline__ PgShape pg_shape(const PagedAttn& p, int b) {
+  PgShape s;
+  s.n = max(0, p.seqs.end(b) - p.seqs.first(b));
+  s.len = p.seqs.lens[b];
+  s.keys = (int)min((long long)max(s.len, 0), p.seqs.capacity());
+  s.blocks = (s.n + 2 * p.tq - 1) / (2 * p.tq);
+  s.steps = max(1, (s.keys + PG_TILE - 1) / PG_TILE);
+  return s;
+}
+
+// Whole warp: steps of a piece. All blocks uncut where they fill the machine; else the shortest pieces that run at one time, or, of cuts in 2, 3
+// and 4, the one whose waves of CTAs take the least (a piece costs about 3 steps of its own).
+__device__ __forceinline__ int paged_plan(const PagedAttn& p) {
+  constexpr int OWN = 3;
+  if (p.slots == 0) return PG_WHOLE;
+  const int lane = threadIdx.x & 31;
+  auto items = [&](int U) {
+    int n = 0;
+    for (int b = lane; b < p.seqs.B; b += 32) {
+      const PgShape s = pg_shape(p, b);
+      n += s.blocks * ((s.steps + U - 1) / U);
     }
-#pragma unroll
-    for (int i = 16; i; i >>= 1) x += __shfl_xor_sync(0xffffffffu, x, i);
-    x *= p.scale_log2;
-    const float mn = fmaxf(m, x), ref = mn == -INFINITY ? 0.f : mn, a = ex2_approx(m - ref), w = ex2_approx(x - ref);
-    m = mn;
-    l = l * a + w;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = o[e] * a + w * v[e];
+    return __reduce_add_sync(0xffffffffu, n) * p.Hkv;
+  };
+  int most = 0;
+  for (int b = lane; b < p.seqs.B; b += 32) {
+    const PgShape s = pg_shape(p, b);
+    if (s.n > 0) most = max(most, s.steps);
   }
+  most = __reduce_max_sync(0xffffffffu, most);
+  const int whole = items(PG_WHOLE);
+  if (2 * whole <= p.slots) {
+    int lo = 1, hi = max(1, most);                 // the least U with items(U) <= slots
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (items(mid) <= p.slots) hi = mid; else lo = mid + 1;
+    }
+    return lo;
+  }
+  int best = PG_WHOLE, cost = (whole + p.slots - 1) / p.slots * (most + OWN);
+  for (int k = 2; k <= 4; ++k) {
+    const int U = (most + k - 1) / k, n = items(U);
+    const int c = (n + p.slots - 1) / p.slots * (U + OWN);
+    if (U > 0 && n <= 2 * p.slots && c < cost) {
+      cost = c;
+      best = U;
+    }
+  }
+  return best;
+}
+
+// A block of a sequence, and the keys of a piece of it.
+struct PgItem {
+  int b, hk, token, tokens, pos, keys, pieces, j0, j1;     // first token (row of q), how many, position of the first; steps j0 .. j1 - 1
+  __device__ __forceinline__ int visible(int upto) const {   // keys that the last of the first `upto` tokens sees
+    return max(0, min(pos + min(upto, tokens), keys));
+  }
+  __device__ __forceinline__ int steps(int upto) const { return (visible(upto) + PG_TILE - 1) / PG_TILE; }
+};
+__device__ __forceinline__ void pg_block(const PagedAttn& p, PgItem& it, const PgShape& s, int b, int blk) {
+  it.b = b;
+  it.token = p.seqs.first(b) + blk * 2 * p.tq;
+  it.tokens = min(2 * p.tq, s.n - blk * 2 * p.tq);
+  it.pos = s.len - s.n + blk * 2 * p.tq;
+  it.keys = s.keys;
+}
+
+// Whole warp: the item of a CTA; false behind the last. Inside a sequence the last block (the most keys) comes first, its heads and pieces
+// next to each other.
+__device__ __forceinline__ bool pg_find(const PagedAttn& p, int x, int U, PgItem& it) {
+  const int lane = threadIdx.x & 31;
+  for (int base = 0, before = 0; base < p.seqs.B; base += 32) {
+    PgShape s{};
+    int pieces = 1, n = 0;
+    if (base + lane < p.seqs.B) {
+      s = pg_shape(p, base + lane);
+      pieces = (s.steps + U - 1) / U;
+      n = s.blocks * pieces * p.Hkv;
+    }
+    int incl = n;
 #pragma unroll
-  for (int e = 0; e < E; ++e) p.out[t * p.ldo + h * D + lane * E + e] = __float2bfloat16(l > 0.f ? o[e] / l : 0.f);
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, before + incl > x);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      const int rem = x - before - (__shfl_sync(0xffffffffu, incl, l) - __shfl_sync(0xffffffffu, n, l));
+      s.n = __shfl_sync(0xffffffffu, s.n, l);
+      s.len = __shfl_sync(0xffffffffu, s.len, l);
+      s.keys = __shfl_sync(0xffffffffu, s.keys, l);
+      s.blocks = __shfl_sync(0xffffffffu, s.blocks, l);
+      it.pieces = __shfl_sync(0xffffffffu, pieces, l);
+      const int per = p.Hkv * it.pieces, blk = s.blocks - 1 - rem / per, in = rem % per;
+      it.hk = in / it.pieces;
+      pg_block(p, it, s, base + l, blk);
+      const int piece = in - it.hk * it.pieces, steps = it.steps(2 * p.tq);
+      it.j0 = (int)((long long)steps * piece / it.pieces);
+      it.j1 = (int)((long long)steps * (piece + 1) / it.pieces);
+      return true;
+    }
+    before += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  return false;
+}
+
+template <int HD>
+struct PgCfg {
+  static constexpr int CH = HD / 64;
+  static constexpr int TILE_BYTES = PG_TILE * HD * 2;
+  static constexpr int OFF_Q = 0;                                   // 2 tiles
+  static constexpr int OFF_K = OFF_Q + 2 * TILE_BYTES;              // 2 stages; at the end the sums of tile 1's keys
+  static constexpr int OFF_V = OFF_K + 2 * TILE_BYTES;              // 2 stages
+  static constexpr int OFF_BAR = OFF_V + 2 * TILE_BYTES;
+  static constexpr int OFF_ML = OFF_BAR + 256;                      // maxima and sums of tile 1's keys
+  static constexpr int SMEM_BYTES = OFF_ML + 2 * PG_TILE * 4 + 1024;
+  static constexpr int TM_S = 0;      // + t * 128; P (bf16 pairs) occupies the first 64 columns of the same region
+  static constexpr int TM_O = 256;    // + t * 128
+  static constexpr int TMEM_COLS = 512;
+  static_assert(PG_TILE * HD * 4 <= 2 * TILE_BYTES, "sums fit in the stages of K");
+};
+
+__device__ __forceinline__ float pg_max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// 4-D tile load global -> shared
+__device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* m, uint64_t* bar, int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+
+template <int HD>
+__global__ void __launch_bounds__(PG_THREADS, 1)
+paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ PagedAttn p) {
+  using Cfg = PgCfg<HD>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem + Cfg::OFF_Q;
+  uint8_t* sK = smem + Cfg::OFF_K;
+  uint8_t* sV = smem + Cfg::OFF_V;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::OFF_BAR);
+  uint64_t* q_full = bars + 0;
+  uint64_t* k_full = bars + 1;    // [2]
+  uint64_t* k_empty = bars + 3;   // [2]
+  uint64_t* v_full = bars + 5;    // [2]
+  uint64_t* v_empty = bars + 7;   // [2]
+  uint64_t* s_full = bars + 9;    // [2] per tile
+  uint64_t* o_done = bars + 11;   // [2] per tile
+  uint64_t* v_tail = bars + 13;   // the last V tile before its rows behind the sequence are cleared
+  uint64_t* p_full = bars + 14;   // [2][PG_PARTS]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 14 + 2 * PG_PARTS);
+  __shared__ PgItem shared_item;
+  __shared__ int shared_there;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (warp == 0) {
+    const int U = paged_plan(p);
+    if (p.plan && blockIdx.x == 0 && lane == 0) *p.plan = U;
+    PgItem it;
+    const bool there = pg_find(p, blockIdx.x, U, it);
+    if (lane == 0) {
+      shared_there = there;
+      if (there) shared_item = it;
+    }
+  } else if (threadIdx.x == 32) {
+    mbar_init(q_full, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
+      mbar_init(&s_full[i], 1);
+      for (int c = 0; c < PG_PARTS; ++c) mbar_init(&p_full[i * PG_PARTS + c], 4);
+      mbar_init(&o_done[i], 1);
+    }
+    mbar_init(v_tail, 1);
+    mbar_fence_init();
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  __syncthreads();
+  if (!shared_there) return;
+  const PgItem it = shared_item;
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, Cfg::TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  // steps of the piece, and of each tile: one behind the other over its own keys (two tiles of rows), or every other (one)
+  const bool alternate = it.tokens <= p.tq;
+  const int n_j = it.j1 - it.j0;
+  int cnt[2];
+  cnt[0] = alternate ? (n_j + 1) >> 1 : max(0, min(it.j1, it.steps(p.tq)) - it.j0);
+  cnt[1] = alternate ? n_j >> 1 : n_j;
+  // the last step's V has rows behind the sequence inside a page
+  const int box = min(PG_TILE, 1 << p.seqs.page_shift);
+  const int tail = it.keys - (it.j1 - 1) * PG_TILE;                  // rows of the last step that are keys
+  const bool clears = n_j > 0 && tail < PG_TILE && (tail & (box - 1)) != 0;
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PG_REGS_CTRL));
+  if (warp == 0) {
+    // ---------------------------------------------------------------- TMA producer: a lane has one box of a step
+    const int qtiles = alternate ? 1 : 2, qbox = p.tq * p.G * HD * 2;
+    if (lane == 0) {
+      mbar_expect_tx(q_full, qtiles * qbox);
+      for (int t = 0; t < qtiles; ++t)
+#pragma unroll
+        for (int c = 0; c < Cfg::CH; ++c)
+          tma_load_3d(sQ + t * Cfg::TILE_BYTES + c * (PG_TILE * 128), &tmQ, q_full, c * 64, it.hk * p.G, it.token + t * p.tq);
+      if (it.keys != p.seqs.lens[it.b]) p.seqs.bad();
+    }
+    const int boxes = PG_TILE / box;
+    const int* table = p.seqs.table + (long long)it.b * p.seqs.ld;
+    auto page_of = [&](int j) {
+      const int key = j * PG_TILE + lane * box;
+      if (lane >= boxes || j >= it.j1 || key >= it.keys) return p.seqs.pages;           // zeros
+      const int page = table[key >> p.seqs.page_shift];
+      if (page >= 0 && page < p.seqs.pages) return page;
+      p.seqs.bad();
+      return p.seqs.pages;
+    };
+    auto boxes_to = [&](uint8_t* dst, const CUtensorMap* m, uint64_t* bar, int j, int page) {
+      if (lane == 0) mbar_expect_tx(bar, Cfg::TILE_BYTES);
+      __syncwarp();
+      if (lane < boxes) {
+        const int y = (j * PG_TILE + lane * box) & ((1 << p.seqs.page_shift) - 1);
+#pragma unroll
+        for (int c = 0; c < Cfg::CH; ++c)
+          tma_load_4d(dst + c * (PG_TILE * 128) + lane * box * 128, m, bar, c * 64, y, it.hk, page);
+      }
+      __syncwarp();
+    };
+    int next = page_of(it.j0);
+    for (int i = 0; i < n_j; ++i) {
+      const int j = it.j0 + i, st = i & 1, page = next;
+      const uint32_t ph = (i >> 1) & 1;
+      next = page_of(j + 1);
+      if (!mbar_wait_warp(&k_empty[st], ph ^ 1)) {
+        if (p.seqs.status && lane == 0) atomicCAS(p.seqs.status, 0, GF_ERR_WAIT_EMPTY);
+        break;
+      }
+      boxes_to(sK + st * Cfg::TILE_BYTES, &tmK, &k_full[st], j, page);
+      if (!mbar_wait_warp(&v_empty[st], ph ^ 1)) {
+        if (p.seqs.status && lane == 0) atomicCAS(p.seqs.status, 0, GF_ERR_WAIT_EMPTY);
+        break;
+      }
+      boxes_to(sV + st * Cfg::TILE_BYTES, &tmV, clears && i == n_j - 1 ? v_tail : &v_full[st], j, page);
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMA issuer
+    const bool leader = elect_one();
+    constexpr uint32_t idesc_qk = umma_idesc_bf16(PG_TILE, PG_TILE, 0, 0);
+    constexpr uint32_t idesc_pv = umma_idesc_bf16(PG_TILE, HD, 0, 1);
+    const uint64_t dq0 = umma_desc_sw128(smem_u32(sQ), 16, 1024);
+    const uint64_t dk0 = umma_desc_sw128(smem_u32(sK), 16, 1024);
+    const uint64_t dv0 = umma_desc_sw128(smem_u32(sV), PG_TILE * 128, 1024);
+    constexpr uint64_t TILE_D = Cfg::TILE_BYTES >> 4;
+    bool ok = mbar_wait_warp_tight(q_full, 0);
+    if (!ok && p.seqs.status && leader) atomicCAS(p.seqs.status, 0, GF_ERR_WAIT_FULL);
+    const uint64_t second = alternate ? 0 : TILE_D;        // Q of tile 1
+    // S_t = Q_t K(stage)^T, announced on s_full[t]
+    auto issue_qk = [&](int t, int st) {
+      const uint64_t qa = dq0 + (t ? second : 0), ka = dk0 + (st ? TILE_D : 0);
+#pragma unroll
+      for (int kk = 0; kk < HD / 16; ++kk) {
+        const uint64_t off = ((kk >> 2) * (PG_TILE * 128) + (kk & 3) * 32) >> 4;
+        umma_bf16_ss_u(leader, tmem_base + Cfg::TM_S + t * 128, qa + off, ka + off, idesc_qk, kk > 0 ? 1u : 0u);
+      }
+      umma_commit_u(leader, &s_full[t]);
+    };
+    // O_t += P_t V(stage), n-th of the tile
+    auto issue_pv = [&](int t, int st, int n) {
+      const uint64_t va = dv0 + (st ? TILE_D : 0);
+#pragma unroll
+      for (int c = 0; c < PG_PARTS; ++c) {
+        if (ok && !mbar_wait_warp_tight(&p_full[t * PG_PARTS + c], n & 1)) {
+          if (p.seqs.status && leader) atomicCAS(p.seqs.status, 0, GF_ERR_WAIT_SOFTMAX);
+          ok = false;
+        }
+        if (ok) {
+          tc_fence_after();
+#pragma unroll
+          for (int kk = c * (PG_TILE / 16 / PG_PARTS); kk < (c + 1) * (PG_TILE / 16 / PG_PARTS); ++kk)
+            umma_bf16_ts_u(leader, tmem_base + Cfg::TM_O + t * 128, tmem_base + Cfg::TM_S + t * 128 + kk * 8,
+                           va + ((kk * 2048) >> 4), idesc_pv, (n > 0 || kk > 0) ? 1u : 0u);
+        }
+      }
+      if (ok && n == (t ? cnt[1] : cnt[0]) - 1) umma_commit_u(leader, &o_done[t]);
+    };
+    auto full = [&](uint64_t* bar, int i) {
+      if (ok && !mbar_wait_warp_tight(&bar[i & 1], (i >> 1) & 1)) {
+        if (p.seqs.status && leader) atomicCAS(p.seqs.status, 0, GF_ERR_WAIT_FULL);
+        ok = false;
+      }
+    };
+    if (alternate) {
+      // step i belongs to tile i % 2 and lies in stage i % 2
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (i < n_j) full(k_full, i);
+        if (ok && i < n_j) {
+          tc_fence_after();
+          issue_qk(i, i);
+          umma_commit_u(leader, &k_empty[i]);
+        }
+      }
+      for (int i = 0; i < n_j && ok; ++i) {
+        const int t = i & 1;
+        full(v_full, i);
+        if (!ok) break;
+        issue_pv(t, t, i >> 1);
+        if (!ok) break;
+        umma_commit_u(leader, &v_empty[t]);
+        if (i + 2 < n_j) {
+          full(k_full, i + 2);
+          if (!ok) break;
+          tc_fence_after();
+          issue_qk(t, t);
+          umma_commit_u(leader, &k_empty[t]);
+        }
+      }
+    } else {
+      if (n_j > 0) full(k_full, 0);
+      if (ok && n_j > 0) {
+        tc_fence_after();
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (cnt[t] > 0) issue_qk(t, 0);
+        umma_commit_u(leader, &k_empty[0]);
+      }
+      for (int i = 0; i < n_j && ok; ++i) {
+        full(v_full, i);
+        if (i + 1 < n_j) full(k_full, i + 1);
+        if (!ok) break;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (ok && i < cnt[t]) issue_pv(t, i & 1, i);
+          if (ok && i + 1 < cnt[t]) issue_qk(t, (i + 1) & 1);
+        }
+        if (!ok) break;
+        umma_commit_u(leader, &v_empty[i & 1]);
+        if (i + 1 < n_j) umma_commit_u(leader, &k_empty[(i + 1) & 1]);
+      }
+    }
+  } else if (warp == 2 && clears) {
+    // ---------------------------------------------------------------- rows of the last V behind the sequence: zeros
+    if (!mbar_wait_warp(v_tail, 0)) {
+      if (p.seqs.status && lane == 0) atomicCAS(p.seqs.status, 0, GF_ERR_WAIT_FULL);
+    } else {
+      const int st = (n_j - 1) & 1, end = (tail + box - 1) & ~(box - 1);       // what lies behind `end` came as zeros
+      for (int c = 0; c < Cfg::CH; ++c) {
+        uint4* rows = reinterpret_cast<uint4*>(sV + st * Cfg::TILE_BYTES + c * (PG_TILE * 128));
+        for (int i = tail * 8 + lane; i < end * 8; i += 32) rows[i] = make_uint4(0, 0, 0, 0);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&v_full[st]);
+    }
+  }
+  } else {
+    // ---------------------------------------------------------------- softmax warps: tile t = warp / 4 - 1
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PG_REGS_SOFTMAX));
+    const int t = (warp >> 2) - 1;
+    const int lane_grp = warp & 3;
+    const int r = lane_grp * 32 + lane;
+    const int tile_token = alternate ? 0 : t * p.tq;                   // first token of the tile in the block
+    const int tile_rows = max(0, min(p.tq, it.tokens - tile_token)) * p.G;
+    const int tok = tile_token + r / p.G, head = it.hk * p.G + r % p.G;
+    const bool mine = r < tile_rows;                                   // the row is a token's
+    const bool idle = lane_grp * 32 >= tile_rows;                      // no row of the warp is
+    const int lim = mine ? min(it.pos + tok, it.keys - 1) : -1;        // last key that the row sees
+    const int tile_lim = min(it.pos + tile_token, it.keys - 1);        // ... that all of them see
+    const uint32_t tlane = (uint32_t)(lane_grp * 32) << 16;
+    const uint32_t ts = tmem_base + Cfg::TM_S + t * 128 + tlane;
+    const uint32_t to = tmem_base + Cfg::TM_O + t * 128 + tlane;
+    const float sl2 = p.scale * 1.4426950408889634f;
+    float m_ref = -INFINITY, l = 0.f;
+    bool ok = true;
+    const int my_n = t ? cnt[1] : cnt[0];
+    for (int j = 0; j < my_n && ok; ++j) {
+      if (!mbar_wait_warp_tight(&s_full[t], j & 1)) {
+        if (p.seqs.status) atomicCAS(p.seqs.status, 0, GF_ERR_WAIT_TMEM_FULL);
+        ok = false;
+        break;
+      }
+      if (idle) {
+        if (lane == 0)
+          for (int c = 0; c < PG_PARTS; ++c) mbar_arrive(&p_full[t * PG_PARTS + c]);
+        continue;
+      }
+      tc_fence_after();
+      const int kv0 = (it.j0 + (alternate ? 2 * j + t : j)) * PG_TILE;
+      const bool need_mask = kv0 + PG_TILE - 1 > tile_lim;
+      // ---- row maximum, 64 scores at a time (the exponential pass reads them from tensor memory again)
+      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c2 = 0; c2 < 2; ++c2) {
+        uint32_t sa[32], sb[32];
+        tmem_ld32(ts + c2 * 64, sa);
+        tmem_ld32(ts + c2 * 64 + 32, sb);
+        tmem_ld_wait();
+        if (need_mask) {
+          const int last = lim - kv0 - c2 * 64;                          // last visible column here
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            if (i > last) sa[i] = 0xff800000u;  // -inf
+            if (32 + i > last) sb[i] = 0xff800000u;
+          }
+          tmem_st32(ts + c2 * 64, sa);
+          tmem_st32(ts + c2 * 64 + 32, sb);
+          tmem_st_wait();
+        }
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx4[e] = pg_max3(mx4[e], __uint_as_float(sa[i + e]), __uint_as_float(sb[i + e]));
+        }
+      }
+      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+      // ---- reference maximum: moved (and O, l rescaled) only when the row's maximum grew a lot. The commit behind s_full also covered
+      // the last P V, so O is quiescent here.
+      if (j == 0) {
+        m_ref = mx;
+      } else {
+        const bool grow = (mx - m_ref) * sl2 > PG_RESCALE;
+        if (__any_sync(0xffffffffu, grow)) {
+          const float alpha = grow ? ex2_approx((m_ref - mx) * sl2) : 1.f;
+#pragma unroll
+          for (int c = 0; c < HD / 32; ++c) {
+            uint32_t rr[32];
+            tmem_ld32(to + c * 32, rr);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) rr[i] = __float_as_uint(__uint_as_float(rr[i]) * alpha);
+            tmem_st32(to + c * 32, rr);
+          }
+          l *= alpha;
+          if (grow) m_ref = mx;
+        }
+      }
+      const float mref_use = (m_ref == -INFINITY) ? 0.f : m_ref;  // row with no visible key yet
+      const float mneg = -mref_use * sl2;
+      const uint64_t sl2x = pk2f(sl2, sl2), mnegx = pk2f(mneg, mneg);
+      uint64_t rsa = 0, rsb = 0;
+      uint32_t sa[32], sb[32];
+      auto chunk = [&](const uint32_t (&sv)[32], uint32_t dst) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          const uint64_t x = f2_fma(pk2(sv[i], sv[i + 1]), sl2x, mnegx);
+          const float p0 = ex2_approx(lo2(x)), p1 = ex2_approx(hi2(x));
+          if (i & 2) rsa = f2_add(rsa, pk2f(p0, p1)); else rsb = f2_add(rsb, pk2f(p0, p1));
+          pk[i >> 1] = pack_bf16x2(p0, p1);
+        }
+        tmem_st16(dst, pk);
+      };
+      tmem_ld32(ts, sa);
+#pragma unroll
+      for (int c2 = 0; c2 < 2; ++c2) {
+        tmem_ld_wait();
+        tmem_ld32(ts + c2 * 64 + 32, sb);
+        chunk(sa, ts + c2 * 32);
+        tmem_ld_wait();
+        if (c2 == 0) tmem_ld32(ts + 64, sa);
+        chunk(sb, ts + c2 * 32 + 16);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[t * PG_PARTS + c2]);
+      }
+      const uint64_t rs = f2_add(rsa, rsb);
+      l += lo2(rs) + hi2(rs);
+    }
+    // ---- end: all products into O have been done
+    auto done = [&](int tile) {
+      if (ok && (tile ? cnt[1] : cnt[0]) > 0 && !mbar_wait_warp_tight(&o_done[tile], 0)) {
+        if (p.seqs.status) atomicCAS(p.seqs.status, 0, GF_ERR_WAIT_TMEM_FULL);
+        ok = false;
+      }
+    };
+    done(t);
+    if (alternate) {
+      // both tiles have sums of the same rows: tile 1 leaves its own in shared memory, column by column
+      float* sums = reinterpret_cast<float*>(sK);
+      float* ml = reinterpret_cast<float*>(smem + Cfg::OFF_ML);
+      done(0);
+      if (t == 1 && !idle) {
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < HD / 32; ++c) {
+          uint32_t rr[32];
+          tmem_ld32(to + c * 32, rr);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) sums[(c * 32 + i) * PG_TILE + r] = my_n > 0 ? __uint_as_float(rr[i]) : 0.f;
+        }
+        ml[r] = m_ref;
+        ml[PG_TILE + r] = l;
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+    }
+    if (ok && !idle && !(alternate && t == 1)) {
+      tc_fence_after();
+      float a0 = 1.f, a1 = 0.f;
+      const float* sums = reinterpret_cast<const float*>(sK);
+      if (alternate) {
+        const float* ml = reinterpret_cast<const float*>(smem + Cfg::OFF_ML);
+        const float m1 = ml[r], mm = fmaxf(m_ref, m1), use = mm == -INFINITY ? 0.f : mm;
+        a0 = ex2_approx((m_ref - use) * sl2);
+        a1 = ex2_approx((m1 - use) * sl2);
+        l = l * a0 + ml[PG_TILE + r] * a1;
+        m_ref = mm;
+      }
+      const bool whole = it.pieces == 1;
+      const float inv = !whole ? 1.f : l > 0.f ? 1.f / l : 0.f;
+      a0 *= inv;
+      a1 *= inv;
+      __nv_bfloat16* orow = p.out + (long long)(it.token + tok) * p.ldo + head * HD;
+      const long long row = (long long)blockIdx.x * p.rows + (alternate ? r : t * PG_TILE + r);
+      float* prow = p.part + row * HD;
+#pragma unroll
+      for (int c = 0; c < HD / 32; ++c) {
+        uint32_t rr[32];
+        tmem_ld32(to + c * 32, rr);
+        tmem_ld_wait();
+        float o[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          o[i] = my_n > 0 ? __uint_as_float(rr[i]) * a0 : 0.f;       // tensor memory that nothing wrote may hold anything
+          if (alternate) o[i] += sums[(c * 32 + i) * PG_TILE + r] * a1;
+        }
+        if (!mine) continue;
+        if (whole) {
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4) {
+            uint4 u;
+            uint32_t* pu = reinterpret_cast<uint32_t*>(&u);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) pu[e] = pack_bf16x2(o[q4 * 8 + e * 2], o[q4 * 8 + e * 2 + 1]);
+            *reinterpret_cast<uint4*>(orow + c * 32 + q4 * 8) = u;
+          }
+        } else if (n_j > 0) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(prow + c * 32 + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        }
+      }
+      if (mine && !whole && n_j > 0) *reinterpret_cast<float2*>(p.part_ml + 2 * row) = make_float2(m_ref * sl2, l);
+    }
+  }
+
+  if (p.seqs.status && *reinterpret_cast<volatile int*>(p.seqs.status) != 0) error_drain_pause();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem_base, Cfg::TMEM_COLS);
+  }
+}
+
+// Adds up the pieces of blocks that were cut: a CTA takes one token and KV head after the other, a thread a column of a row.
+template <int HD>
+__global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ PagedAttn p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int U = *p.plan, lane = threadIdx.x & 31;
+  if (U == PG_WHOLE) return;
+  for (long long x = blockIdx.x; x < (long long)p.seqs.T * p.Hkv; x += gridDim.x) {
+    const int t = (int)(x / p.Hkv), hk = (int)(x % p.Hkv);
+    const int b = paged_seq_of(p.seqs, t);
+    if (b >= p.seqs.B) return;
+    const PgShape s = pg_shape(p, b);
+    const int first = p.seqs.first(b), pieces = (s.steps + U - 1) / U;
+    if (pieces == 1 || t < first || t >= first + s.n) continue;
+    int before = 0;                // items of the sequences in front
+    for (int i = lane; i < b; i += 32) {
+      const PgShape o = pg_shape(p, i);
+      before += o.blocks * ((o.steps + U - 1) / U);
+    }
+    before = __reduce_add_sync(0xffffffffu, before) * p.Hkv;
+    const int blk = (t - first) / (2 * p.tq);
+    PgItem it;
+    pg_block(p, it, s, b, blk);
+    const int in = t - it.token, steps = it.steps(2 * p.tq);
+    const long long item = before + ((long long)(s.blocks - 1 - blk) * p.Hkv + hk) * pieces;
+    if (item + pieces > p.items) return;                   // sequences that overlap in `cu`: not all items were run
+    const int d = threadIdx.x % HD;
+    for (int g = threadIdx.x / HD; g < p.G; g += blockDim.x / HD) {
+      const int r = (in / p.tq) * PG_TILE + (in % p.tq) * p.G + g;
+      float m = -INFINITY, l = 0.f, o = 0.f;
+      auto there = [&](int k) { return (long long)steps * k / pieces < (long long)steps * (k + 1) / pieces; };
+#pragma unroll 4
+      for (int k = 0; k < pieces; ++k)
+        if (there(k)) m = fmaxf(m, p.part_ml[2 * ((item + k) * p.rows + r)]);
+      const float use = m == -INFINITY ? 0.f : m;
+#pragma unroll 4
+      for (int k = 0; k < pieces; ++k) {
+        if (!there(k)) continue;
+        const long long row = (item + k) * p.rows + r;
+        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * row);
+        const float w = ex2_approx(ml.x - use);
+        l += ml.y * w;
+        o += ml.y > 0.f ? p.part[row * HD + d] * w : 0.f;
+      }
+      p.out[(long long)t * p.ldo + (hk * p.G + g) * HD + d] = __float2bfloat16(l > 0.f ? o / l : 0.f);
+    }
+  }
+}
+
+static int pg_map(CUtensorMap* out, const void* base, int rank, const cuuint64_t* dims, const long long* strides, const cuuint32_t* box) {
+  EncodeTiledFn fn = get_encode_fn();
+  if (!fn) return GFH_TMAP;
+  cuuint64_t bytes[3];
+  for (int i = 0; i < rank - 1; ++i) bytes[i] = dims[i + 1] > 1 ? (cuuint64_t)strides[i] * 2 : dims[0] * 2;   // a stride that nothing goes by
+  const cuuint32_t ones[4] = {1, 1, 1, 1};
+  const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, bytes, box, ones,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? GFH_OK : GFH_TMAP;
+}
+
+template <int HD>
+static int launch_paged(PagedAttn& p, const void* q, long long ldq, const void* kp, const void* vp, const long long* strides, int items,
+                        cudaStream_t st) {
+  using Cfg = PgCfg<HD>;
+  static gf::DeviceOnce configured;
+  auto kern = paged_attn_kernel<HD>;
+  if (configured.todo()) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES) != cudaSuccess) return GFH_CUDA;
+    configured.mark();
+  }
+  const PagedBatch& S = p.seqs;
+  CUtensorMap tq, tk, tv;
+  const cuuint64_t qdims[3] = {HD, (cuuint64_t)p.Hq, (cuuint64_t)S.T};
+  const long long qstrides[2] = {HD, ldq};
+  const cuuint32_t qbox[3] = {64, (cuuint32_t)p.G, (cuuint32_t)p.tq};
+  const int page = 1 << S.page_shift;
+  const cuuint64_t dims[4] = {HD, (cuuint64_t)page, (cuuint64_t)p.Hkv, (cuuint64_t)S.pages};
+  const cuuint32_t box[4] = {64, (cuuint32_t)(page < PG_TILE ? page : PG_TILE), 1, 1};
+  const long long ks[3] = {strides[1], strides[2], strides[0]}, vs[3] = {strides[4], strides[5], strides[3]};
+  int rc = pg_map(&tq, q, 3, qdims, qstrides, qbox);
+  if (!rc) rc = pg_map(&tk, kp, 4, dims, ks, box);
+  if (!rc) rc = pg_map(&tv, vp, 4, dims, vs, box);
+  if (rc) return rc;
+  kern<<<items, PG_THREADS, Cfg::SMEM_BYTES, st>>>(tq, tk, tv, p);
+  if (cudaGetLastError() != cudaSuccess) return GFH_CUDA;
+  if (p.slots == 0) return GFH_OK;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)min((long long)S.T * p.Hkv, 8ll * p.slots));
+  cfg.blockDim = dim3(p.G > 1 ? 256 : HD);
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, paged_join_kernel<HD>, p) != cudaSuccess) return GFH_CUDA;
+  note_extra_launches(1);
+  return GFH_OK;
+}
+
+// Items of a call at most, rows of one that are tokens' at most, and whether blocks may be cut: what decides the grid and the workspace.
+struct PgCall {
+  int items, rows, slots;
+  long long ws;
+};
+static bool pg_call(PgCall& c, int B, int T, bool one_each, int Hq, int Hkv, int D, int sms) {
+  const int G = Hq / Hkv, w = 2 * (PG_TILE / G);
+  const long long blocks = one_each ? B : min((long long)T, ((long long)T + (long long)B * (w - 1)) / w);
+  const long long items = blocks * Hkv;
+  if (items > 0x7fffffffll) return false;
+  c.slots = items < 2 * sms ? sms : 0;
+  c.items = c.slots ? 2 * sms : (int)items;
+  c.rows = one_each || T <= PG_TILE / G ? PG_TILE : 2 * PG_TILE;       // blocks of one tile, or of two
+  c.ws = c.slots ? 256 + 4ll * c.items * c.rows * (D + 2) : 0;
+  return true;
 }
 
 }  // namespace gf
 
 using namespace gf;
 
-// q [T, Hq, D] and out alike, rows ldq and ldo elements apart; strides: pages, rows and heads of kpages, then of vpages, in elements.
+static bool paged_sizes(int B, int T, int Hq, int Hkv, int D) {
+  return B > 0 && T > 0 && Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && Hq / Hkv <= PG_TILE && (D == 64 || D == 128) && Hkv <= 65535;
+}
+
+// Bytes of workspace of a call, -1 for sizes that are not taken.
+GF_API long long gf_paged_attn_workspace(int B, int T, int one_each, int Hq, int Hkv, int D) {
+  gf::bind();
+  PgCall c;
+  if (!paged_sizes(B, T, Hq, Hkv, D) || !pg_call(c, B, T, one_each != 0, Hq, Hkv, D, sm_count())) return -1;
+  return c.ws;
+}
+
+// q [T, Hq, D] and out alike, rows ldq and ldo elements apart; strides: pages, rows and heads of kpages, then of vpages, in elements; ws: as
+// many bytes as gf_paged_attn_workspace says, on a 256-byte boundary. scale > 0.
 GF_API int gf_paged_attn(const void* q, long long ldq, const void* kpages, const void* vpages, const long long* strides, const int* table,
                          int ld_table, int width, const int* lens, const int* cu, void* out, long long ldo, int B, int T, int Hq, int Hkv,
-                         int D, int page, int pages, float scale, int* status, void* stream) {
-  PagedAttn p;
-  if (!paged_batch(p.seqs, table, ld_table, width, lens, cu, B, T, page, pages, status)) return GFH_BAD_ARG;
-  if (Hq <= 0 || Hkv <= 0 || Hq % Hkv || (D != 64 && D != 128) || ldq % 8 || ldo % 8 || !strides) return GFH_BAD_ARG;
-  for (const void* x : {q, kpages, vpages, (const void*)out})
-    if (!x || (reinterpret_cast<uintptr_t>(x) & 15)) return GFH_BAD_ARG;
+                         int D, int page, int pages, float scale, void* ws, long long ws_bytes, int* status, void* stream) {
+  PagedAttn p{};
+  if (!paged_batch(p.seqs, table, ld_table, width, lens, cu, B, T, page, pages, status) || pages == 0) return GFH_BAD_ARG;
+  if (!paged_sizes(B, T, Hq, Hkv, D) || ldq % 8 || ldo % 8 || !strides || !(scale > 0.f)) return GFH_BAD_ARG;
+  for (const void* x : {q, kpages, vpages, (const void*)out, (const void*)ws})
+    if (reinterpret_cast<uintptr_t>(x) & 15) return GFH_BAD_ARG;
+  if (!q || !kpages || !vpages || !out) return GFH_BAD_ARG;
   for (int i = 0; i < 6; ++i)
-    if (strides[i] % 8) return GFH_BAD_ARG;
+    if (strides[i] % 8 || strides[i] < 0) return GFH_BAD_ARG;
+  gf::bind();
+  PgCall c;
+  if (!pg_call(c, B, T, cu == nullptr, Hq, Hkv, D, sm_count())) return GFH_TOO_LARGE;
+  if (ws_bytes < c.ws || (c.ws && !ws)) return GFH_BAD_ARG;
   gf::enter();
-  p.q = (const __nv_bfloat16*)q; p.ldq = ldq;
-  p.kp = (const __nv_bfloat16*)kpages; p.vp = (const __nv_bfloat16*)vpages;
-  p.kpage = strides[0]; p.krow = strides[1]; p.khead = strides[2];
-  p.vpage = strides[3]; p.vrow = strides[4]; p.vhead = strides[5];
+  p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.tq = PG_TILE / p.G;
+  p.slots = c.slots; p.scale = scale; p.rows = c.rows; p.items = c.items;
   p.out = (__nv_bfloat16*)out; p.ldo = ldo;
-  p.Hq = Hq; p.Hkv = Hkv; p.scale_log2 = scale * 1.4426950408889634f;
-  const dim3 grid(T, (Hq + 3) / 4);
-  if (D == 128) paged_attn_kernel<128><<<grid, 128, 0, (cudaStream_t)stream>>>(p);
-  else paged_attn_kernel<64><<<grid, 128, 0, (cudaStream_t)stream>>>(p);
-  return cudaGetLastError() == cudaSuccess ? GFH_OK : GFH_CUDA;
+  if (c.slots) {
+    p.plan = (int*)ws;
+    p.part = (float*)((char*)ws + 256);
+    p.part_ml = p.part + (long long)c.items * c.rows * D;
+  }
+  cudaStream_t st = (cudaStream_t)stream;
+  return D == 128 ? launch_paged<128>(p, q, ldq, kpages, vpages, strides, c.items, st)
+                  : launch_paged<64>(p, q, ldq, kpages, vpages, strides, c.items, st);
 }

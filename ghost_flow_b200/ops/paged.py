@@ -13,6 +13,7 @@ something follows (a gradient, tracing, transforms, modes), plain PyTorch. The r
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -170,6 +171,12 @@ def rope_qkv_to_pages(qkv, num_heads: int, num_kv_heads: int, cos, sin, kpages, 
 
 
 # ------------------------------------------------------------------------------------------ attention
+@functools.lru_cache(maxsize=4096)
+def _attention_workspace(device: int, B: int, T: int, one_each: bool, H: int, Hk: int, D: int) -> int:
+    """Bytes that a call leaves the results of pieces in (the number of SMs decides whether keys are cut)."""
+    return _lib.cuda_lib().gf_paged_attn_workspace(B, T, 1 if one_each else 0, H, Hk, D)
+
+
 def _attention_ref(q, kpages, vpages, page_table, lens, cu, scale, out):
     (P, page, Hk, D), (T, H, _), dev, B = kpages.shape, q.shape, q.device, lens.shape[0]
     up = torch.promote_types(q.dtype, torch.float32)
@@ -233,22 +240,28 @@ def paged_attention(q, kpages, vpages, page_table, lens, cu=None, scale: float |
     if out is not None and (_ranges_overlap(out, q) or _ranges_overlap(out, kpages) or _ranges_overlap(out, vpages)):
         raise ValueError(f"{what}: out shares memory with q or the pages")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if not (q.is_cuda and q.dtype is _BF16) or D not in (64, 128) or _wants_grad(q, kpages, vpages) or _observed() \
-            or not _ints_fit_kernel(page_table, lens, cu) or not _pages_fit_kernel(kpages, vpages) \
+    if not math.isfinite(scale):
+        raise ValueError(f"{what}: a scale of {scale}")
+    if not (q.is_cuda and q.dtype is _BF16) or D not in (64, 128) or H // Hk > 128 or _wants_grad(q, kpages, vpages) or _observed() \
+            or not _ints_fit_kernel(page_table, lens, cu) or not _pages_fit_kernel(kpages, vpages) or 0 in kpages.stride() + vpages.stride() \
             or (out is not None and (out.stride(2) != 1 or out.stride(1) != D or out.stride(0) % 8 or out.stride(0) < H * D
                                      or out.data_ptr() % 16)):
         return _attention_ref(q, kpages, vpages, page_table, lens, cu, scale, out)
     if dev.index != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return paged_attention(q, kpages, vpages, page_table, lens, cu, scale, out)
-    if q.stride(2) != 1 or q.stride(1) != D or q.stride(0) % 8 or q.data_ptr() % 16:
+    if not scale > 0:                        # the kernel takes the largest score before it scales
+        q, scale = q * (-1 if scale < 0 else 0), -scale if scale < 0 else 1.0
+    if q.stride(2) != 1 or q.stride(1) != D or q.stride(0) % 8 or q.data_ptr() % 16 or (T > 1 and q.stride(0) < H * D):
         q = q.clone(memory_format=torch.contiguous_format)
     o = torch.empty((T, H, D), dtype=_BF16, device=dev) if out is None else out
+    nbytes = _attention_workspace(dev.index, lens.shape[0], T, cu is None, H, Hk, D)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _rc(_lib.cuda_lib().gf_paged_attn(
         q.data_ptr(), q.stride(0), kpages.data_ptr(), vpages.data_ptr(), _strides(kpages, vpages), page_table.data_ptr(),
         page_table.stride(0), page_table.shape[1], lens.data_ptr(), None if cu is None else cu.data_ptr(), o.data_ptr(), o.stride(0),
-        lens.shape[0], T, H, Hk, D, kpages.shape[1], kpages.shape[0], scale, _lib.status_word(dev).data_ptr(), _lib.stream_ptr()),
-        "gf_paged_attn")
+        lens.shape[0], T, H, Hk, D, kpages.shape[1], kpages.shape[0], scale, None if ws is None else ws.data_ptr(),
+        nbytes, _lib.status_word(dev).data_ptr(), _lib.stream_ptr()), "gf_paged_attn")
     if out is not None:
         torch.autograd.graph.increment_version(out)
     return o
