@@ -28,6 +28,7 @@
 
 #include "gf_host.h"
 #include "gf_ptx.cuh"
+#include "paged.cuh"
 
 namespace gf {
 
@@ -162,6 +163,9 @@ struct DecParams {
   // append (gf_llama_decode): the new token's k and v are row len - 1; q and k are rotated here with these rows of the tables
   const float *cos_row, *sin_row;
   int interleaved;
+  // pages (gf_paged_attn_one): kc and vc are pools, a block of 16 keys lies in one page. Strides of pages, rows and heads, in elements
+  PagedBatch pages;
+  long long kpage, krow, khead, vpage, vrow, vhead;
 };
 
 // Rotates packed pairs: lo holds dims d, d + 1 and hi their partners (half-split), or each word is a pair (interleaved); the
@@ -183,16 +187,19 @@ enum DecKind : int {
   DEC_SLICES = 0,    // splits > 0
   DEC_APPEND = 1,    // the same, with the new token's row
   DEC_SHARES = 2,    // splits == 0
+  DEC_PAGES = 3,     // splits > 0, keys in pages
+  DEC_PAGES_SHARES = 4,
 };
+__host__ __device__ constexpr bool dec_shares(int kind) { return kind == DEC_SHARES || kind == DEC_PAGES_SHARES; }
 
 // Kinds of one piece to a CTA are compiled without what goes from one sequence to the next. With it, calls that the memory does
 // not bound took 5 to 25 % longer: us with / without it, 4 sequences of 64 keys, 64 / 8 heads of 64 3.8 / 3.1, 32 of 800, 32 /
 // 8 heads of 64 13.7 / 11.4, 32 of 200, 32 / 32 heads of 128 32.7 / 26.5. (Padded rows instead of the exchange of chunks are 10
 // % slower where memory bounds it: 32 of 4096 keys, 32 / 8 heads of 128 93 / 82: cp.async then fills lines in two parts.)
 template <int D, int KIND>
-__global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, KIND == DEC_SHARES>::CTAS)
+__global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, dec_shares(KIND)>::CTAS)
 attn_decode_kernel(const __grid_constant__ DecParams p) {
-  constexpr bool SHARES = KIND == DEC_SHARES, APPEND = KIND == DEC_APPEND;
+  constexpr bool SHARES = dec_shares(KIND), APPEND = KIND == DEC_APPEND, PAGED = KIND == DEC_PAGES || KIND == DEC_PAGES_SHARES;
   using Cfg = DecCfg<D, SHARES>;
   extern __shared__ __align__(128) uint8_t ring[];
   const DecWork& w = p.work;
@@ -230,14 +237,38 @@ attn_decode_kernel(const __grid_constant__ DecParams p) {
   DecAt ahead = at;
   int ahead_units = left_units;
   long long head = at.b * batch_stride + (long long)hk * D;      // of the sequence ahead
+  // paged: the page of this warp's keys in the unit ahead, and in the one behind it, on their way before the unit's keys are asked for
+  auto page_of = [&](const DecAt& a, int blk) {
+    const int k0 = blk * 64 + warp * DEC_KEYS;
+    return k0 < a.len ? p.pages.table[(long long)a.b * p.pages.ld + (k0 >> p.pages.page_shift)] : 0;
+  };
+  int page_ahead = 0, page_next = 0;
+  if constexpr (PAGED) {
+    page_ahead = page_of(ahead, ahead.blk);
+    if constexpr (!SHARES) page_next = page_of(ahead, ahead.blk + 1);
+  }
   // keys of this warp's next unit into stage `st`; one commit group per unit, empty ones behind the part
   auto load = [&](int st) {
     const int k0 = ahead.blk * 64 + warp * DEC_KEYS;
     if (ahead_units > 0 && k0 < ahead.len) {
       const uint32_t dst = my + st * (2 * Cfg::TILE);
+      if constexpr (PAGED) {
+        const bool there = page_ahead >= 0 && page_ahead < p.pages.pages;
+        if (!there && lane == 0) p.pages.bad();
+        const int r0 = k0 & ((1 << p.pages.page_shift) - 1);
+        const __nv_bfloat16* kb = p.kc + (there ? page_ahead * p.kpage : 0) + r0 * p.krow + hk * p.khead;
+        const __nv_bfloat16* vb = p.vc + (there ? page_ahead * p.vpage : 0) + r0 * p.vrow + hk * p.vhead;
+#pragma unroll
+        for (int n = 0; n < DEC_KEYS * D / 8 / 32; ++n) {
+          const int id = lane + n * 32, row = id / (D / 8), col = id % (D / 8);
+          const uint32_t to = dst + row * Cfg::ROW + Cfg::chunk(row, col), bytes = there && k0 + row < ahead.len ? 16u : 0u;
+          cp_async_16(to, kb + row * p.krow + col * 8, bytes);
+          cp_async_16(to + Cfg::TILE, vb + row * p.vrow + col * 8, bytes);
+        }
+      }
       const int lim = ahead.len - (APPEND ? 1 : 0);              // rows to read: the new token's comes from registers
 #pragma unroll
-      for (int n = 0; n < DEC_KEYS * D / 8 / 32; ++n) {
+      for (int n = 0; n < (PAGED ? 0 : DEC_KEYS * D / 8 / 32); ++n) {
         const int id = lane + n * 32, row = id / (D / 8), col = id % (D / 8);
         const int key = k0 + row;
         const long long off = head + (long long)max(0, min(key, lim - 1)) * row_stride + col * 8;
@@ -261,9 +292,14 @@ attn_decode_kernel(const __grid_constant__ DecParams p) {
       if (ahead_units > 0) {
         ahead.next(w);
         head = ahead.b * batch_stride + (long long)hk * D;
+        if constexpr (PAGED) page_ahead = page_of(ahead, ahead.blk);
       }
     } else {
       ++ahead.blk;
+      if constexpr (PAGED) {
+        page_ahead = page_next;
+        page_next = page_of(ahead, ahead.blk + 1);
+      }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -277,6 +313,7 @@ attn_decode_kernel(const __grid_constant__ DecParams p) {
   uint4 k_new, v_new;              // append: chunk `lane` of the new token's rows, in the warp whose keys it belongs to
   // ---- start of a piece
   auto begin = [&] {
+    if (PAGED && threadIdx.x == 0 && hk == 0 && w.lens[at.b] != at.len) p.pages.bad();
     const unsigned short* qp = reinterpret_cast<const unsigned short*>(
         p.q + at.b * p.ldq + (long long)(hk * G + min(r, G - 1)) * D + 2 * c);
 #pragma unroll
@@ -594,7 +631,7 @@ __global__ void __launch_bounds__(D) attn_decode_merge_kernel(const __grid_const
 template <int D, int KIND>
 static int launch_decode(const DecParams& p, int chained, cudaStream_t st) {
   static gf::DeviceOnce configured;
-  constexpr int SMEM = DecCfg<D, KIND == DEC_SHARES>::SMEM;
+  constexpr int SMEM = DecCfg<D, dec_shares(KIND)>::SMEM;
   auto kern = attn_decode_kernel<D, KIND>;
   if (configured.todo()) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess)
@@ -656,4 +693,28 @@ GF_API int gf_attn_decode(const void* q, long long ldq, const void* kcache, cons
   cudaStream_t st = (cudaStream_t)stream;
   if (splits < 0) return D == 128 ? launch_decode<128, DEC_SHARES>(p, 0, st) : launch_decode<64, DEC_SHARES>(p, 0, st);
   return D == 128 ? launch_decode<128, DEC_SLICES>(p, 0, st) : launch_decode<64, DEC_SLICES>(p, 0, st);
+}
+
+// One new token of each sequence over pages (see paged.cuh): x [B, Hq, D] and y alike; splits and scratch as above, with at most
+// width * page keys. At most 8 query heads to a KV head.
+GF_API int gf_paged_attn_one(const PagedCall* c, float scale, int splits, float* scratch, void* stream) {
+  DecParams p{};
+  if (!c || c->cu || !paged_batch(p.pages, *c) || c->H <= 0 || c->Hk <= 0 || c->H % c->Hk || c->H / c->Hk > DEC_MAX_G ||
+      (c->D != 64 && c->D != 128) || splits == 0 || !scratch || c->pages == 0)
+    return GFH_BAD_ARG;
+  if (splits > 65535) splits = 65535;
+  gf::enter();
+  const int D = (int)c->D;
+  p.work = {p.pages.lens, 0, (int)p.pages.capacity(), p.pages.B, (int)c->Hk, splits < 0 ? -splits : 0, splits > 0 ? splits : 0};
+  p.q = (const __nv_bfloat16*)c->x; p.ldq = c->ldx;
+  p.kc = (__nv_bfloat16*)c->kpages; p.vc = (__nv_bfloat16*)c->vpages;
+  p.Hq = (int)c->H; p.G = (int)(c->H / c->Hk);
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.part = scratch;
+  p.out = (__nv_bfloat16*)c->y; p.ldo = c->ldy;
+  p.kpage = c->strides[0]; p.krow = c->strides[1]; p.khead = c->strides[2];
+  p.vpage = c->strides[3]; p.vrow = c->strides[4]; p.vhead = c->strides[5];
+  cudaStream_t st = (cudaStream_t)stream;
+  if (splits < 0) return D == 128 ? launch_decode<128, DEC_PAGES_SHARES>(p, 0, st) : launch_decode<64, DEC_PAGES_SHARES>(p, 0, st);
+  return D == 128 ? launch_decode<128, DEC_PAGES>(p, 0, st) : launch_decode<64, DEC_PAGES>(p, 0, st);
 }

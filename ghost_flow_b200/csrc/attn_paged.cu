@@ -749,33 +749,26 @@ GF_API long long gf_paged_attn_workspace(int B, int T, int one_each, int Hq, int
   return c.ws;
 }
 
-// q [T, Hq, D] and out alike, rows ldq and ldo elements apart; strides: pages, rows and heads of kpages, then of vpages, in elements; ws: as
-// many bytes as gf_paged_attn_workspace says, on a 256-byte boundary. scale > 0.
-GF_API int gf_paged_attn(const void* q, long long ldq, const void* kpages, const void* vpages, const long long* strides, const int* table,
-                         int ld_table, int width, const int* lens, const int* cu, void* out, long long ldo, int B, int T, int Hq, int Hkv,
-                         int D, int page, int pages, float scale, void* ws, long long ws_bytes, int* status, void* stream) {
+// x [T, Hq, D] and y alike; ws: as many bytes as gf_paged_attn_workspace says, on a 16-byte boundary. scale > 0.
+GF_API int gf_paged_attn(const PagedCall* c, float scale, void* ws, long long ws_bytes, void* stream) {
   PagedAttn p{};
-  if (!paged_batch(p.seqs, table, ld_table, width, lens, cu, B, T, page, pages, status) || pages == 0) return GFH_BAD_ARG;
-  if (!paged_sizes(B, T, Hq, Hkv, D) || ldq % 8 || ldo % 8 || !strides || !(scale > 0.f)) return GFH_BAD_ARG;
-  for (const void* x : {q, kpages, vpages, (const void*)out, (const void*)ws})
-    if (reinterpret_cast<uintptr_t>(x) & 15) return GFH_BAD_ARG;
-  if (!q || !kpages || !vpages || !out) return GFH_BAD_ARG;
-  for (int i = 0; i < 6; ++i)
-    if (strides[i] % 8 || strides[i] < 0) return GFH_BAD_ARG;
+  if (!c || !paged_batch(p.seqs, *c) || c->pages == 0 || c->H > 0x7fffffff || c->Hk > 65535) return GFH_BAD_ARG;
+  const int B = p.seqs.B, T = p.seqs.T, Hq = (int)c->H, Hkv = (int)c->Hk, D = (int)c->D;
+  if (!paged_sizes(B, T, Hq, Hkv, D) || !(scale > 0.f) || (reinterpret_cast<uintptr_t>(ws) & 15)) return GFH_BAD_ARG;
   gf::bind();
-  PgCall c;
-  if (!pg_call(c, B, T, cu == nullptr, Hq, Hkv, D, sm_count())) return GFH_TOO_LARGE;
-  if (ws_bytes < c.ws || (c.ws && !ws)) return GFH_BAD_ARG;
+  PgCall n;
+  if (!pg_call(n, B, T, !p.seqs.cu, Hq, Hkv, D, sm_count())) return GFH_TOO_LARGE;
+  if (ws_bytes < n.ws || (n.ws && !ws)) return GFH_BAD_ARG;
   gf::enter();
   p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.tq = PG_TILE / p.G;
-  p.slots = c.slots; p.scale = scale; p.rows = c.rows; p.items = c.items;
-  p.out = (__nv_bfloat16*)out; p.ldo = ldo;
-  if (c.slots) {
+  p.slots = n.slots; p.scale = scale; p.rows = n.rows; p.items = n.items;
+  p.out = (__nv_bfloat16*)c->y; p.ldo = c->ldy;
+  if (n.slots) {
     p.plan = (int*)ws;
     p.part = (float*)((char*)ws + 256);
-    p.part_ml = p.part + (long long)c.items * c.rows * D;
+    p.part_ml = p.part + (long long)n.items * n.rows * D;
   }
   cudaStream_t st = (cudaStream_t)stream;
-  return D == 128 ? launch_paged<128>(p, q, ldq, kpages, vpages, strides, c.items, st)
-                  : launch_paged<64>(p, q, ldq, kpages, vpages, strides, c.items, st);
+  return D == 128 ? launch_paged<128>(p, c->x, c->ldx, c->kpages, c->vpages, c->strides, n.items, st)
+                  : launch_paged<64>(p, c->x, c->ldx, c->kpages, c->vpages, c->strides, n.items, st);
 }

@@ -91,19 +91,36 @@ __global__ void __launch_bounds__(LG_THREADS) logits_kernel(const __grid_constan
 
 using namespace gf;
 
-// x, y [B, V] of dtype (0 fp32, 1 bf16, 2 fp16), rows ldx and ldy elements apart; y may be x.
-GF_API int gf_process_logits(const void* x, long long ldx, void* y, long long ldy, int dtype, int B, int V, const void* tokens,
-                             long long ldt, int tokens64, int L, const int* token_lens, const int* generated_from, const float* repetition,
-                             const float* presence, const float* frequency, float repetition0, float presence0, float frequency0,
-                             const float* bias, long long ldb, const void* allowed, long long lda, void* stream) {
-  if (!x || !y || B <= 0 || V <= 0 || L < 0 || dtype < 0 || dtype > 2 || B > 65535) return GFH_BAD_ARG;
+// 8 bytes each, as in PagedCall.
+struct LogitsCall {
+  const void* x;                 // [B, V] of dtype (0 fp32, 1 bf16, 2 fp16), rows ldx apart
+  long long ldx;
+  void* y;                       // alike; may be x
+  long long ldy, dtype, B, V;
+  const void* tokens;
+  long long ldt, tokens64, L;
+  const int *token_lens, *generated_from;
+  const float *repetition, *presence, *frequency;
+  double repetition0, presence0, frequency0;
+  const float* bias;
+  long long ldb;
+  const unsigned* allowed;
+  long long lda;
+};
+
+GF_API int gf_process_logits(const LogitsCall* c, void* stream) {
+  constexpr long long MOST = 0x7fffffff;
+  if (!c || !c->x || !c->y || c->B <= 0 || c->V <= 0 || c->V > MOST || c->L < 0 || c->L > MOST || c->dtype < 0 || c->dtype > 2 ||
+      c->B > 65535)
+    return GFH_BAD_ARG;
   gf::enter();
-  LogitsParams p{x, y, ldx, ldy, L > 0 ? tokens : nullptr, ldt, token_lens, generated_from, repetition, presence, frequency, repetition0,
-                 presence0, frequency0, bias, ldb, (const unsigned*)allowed, lda, V, L, tokens64};
-  const dim3 grid((V + LG_SLICE - 1) / LG_SLICE, B);
+  const LogitsParams p{c->x, c->y, c->ldx, c->ldy, c->L > 0 ? c->tokens : nullptr, c->ldt, c->token_lens, c->generated_from,
+                       c->repetition, c->presence, c->frequency, (float)c->repetition0, (float)c->presence0, (float)c->frequency0,
+                       c->bias, c->ldb, c->allowed, c->lda, (int)c->V, (int)c->L, (int)c->tokens64};
+  const dim3 grid((unsigned)((c->V + LG_SLICE - 1) / LG_SLICE), (unsigned)c->B);
   cudaStream_t st = (cudaStream_t)stream;
-  if (dtype == 0) logits_kernel<float><<<grid, LG_THREADS, 0, st>>>(p);
-  else if (dtype == 1) logits_kernel<__nv_bfloat16><<<grid, LG_THREADS, 0, st>>>(p);
+  if (c->dtype == 0) logits_kernel<float><<<grid, LG_THREADS, 0, st>>>(p);
+  else if (c->dtype == 1) logits_kernel<__nv_bfloat16><<<grid, LG_THREADS, 0, st>>>(p);
   else logits_kernel<__half><<<grid, LG_THREADS, 0, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? GFH_OK : GFH_CUDA;
 }

@@ -17,7 +17,7 @@ struct PagedBatch {
   int* status;
   int ld, width, page_shift, pages, B, T;
 
-  __device__ __forceinline__ long long capacity() const { return (long long)width << page_shift; }
+  __host__ __device__ __forceinline__ long long capacity() const { return (long long)width << page_shift; }
   __device__ __forceinline__ int first(int b) const { return cu ? max(0, min(cu[b], T)) : b; }
   __device__ __forceinline__ int end(int b) const { return cu ? max(0, min(cu[b + 1], T)) : b + 1; }
   __device__ __forceinline__ void bad() const {
@@ -38,13 +38,34 @@ __device__ __forceinline__ int paged_seq_of(const PagedBatch& s, int t) {
   return b;
 }
 
-// Host: fills `s` from what a caller gives; false where the kernels do not take it.
-inline bool paged_batch(PagedBatch& s, const int* table, int ld, int width, const int* lens, const int* cu, int B, int T, int page,
-                        int pages, int* status) {
-  if (B <= 0 || T <= 0 || width < 0 || ld < 0 || page < 16 || (page & (page - 1)) || pages < 0 || !lens || (width > 0 && !table) ||
-      (!cu && T != B) || (long long)pages * page > 0x7fffffffll || (long long)width * page > 0x7fffffffll)
+// What the entry points take: tensors as addresses, sizes and strides in elements, 8 bytes each so that a caller in any language can pack them.
+struct PagedCall {
+  const void* x;                 // new tokens: [T, heads, D], heads packed, rows ldx apart
+  long long ldx;
+  void* y;                       // result: [T, H, D], rows ldy apart
+  long long ldy;
+  void *kpages, *vpages;         // [pages, page, Hk, D]
+  long long strides[6];          // pages, rows and heads of kpages, then of vpages
+  const int* table;
+  long long ld_table, width;
+  const int *lens, *cu;
+  long long B, T, H, Hk, D, page, pages;
+  int* status;
+};
+
+// Host: the batch of a call; false where the kernels do not take it: sizes, pages of other than a power of two from 16 rows, and rows of x, y
+// and the pools that are not on 16-byte boundaries.
+inline bool paged_batch(PagedBatch& s, const PagedCall& c) {
+  constexpr long long MOST = 0x7fffffff;
+  if (c.B <= 0 || c.B >= MOST || c.T <= 0 || c.T >= MOST || c.width < 0 || c.ld_table < 0 || c.ld_table > MOST || c.page < 16 ||
+      (c.page & (c.page - 1)) || c.page > MOST || c.pages < 0 || c.pages * c.page > MOST || c.width > MOST / c.page || !c.lens ||
+      (c.width > 0 && !c.table) || (!c.cu && c.T != c.B) || c.ldx % 8 || c.ldy % 8 || c.ldx < 0 || c.ldy < 0)
     return false;
-  s = {table, lens, cu, status, ld, width, __builtin_ctz((unsigned)page), pages, B, T};
+  for (const void* p : {c.x, (const void*)c.y, (const void*)c.kpages, (const void*)c.vpages})
+    if (!p || (reinterpret_cast<uintptr_t>(p) & 15)) return false;
+  for (long long st : c.strides)
+    if (st % 8 || st < 0) return false;
+  s = {c.table, c.lens, c.cu, c.status, (int)c.ld_table, (int)c.width, __builtin_ctzll((unsigned long long)c.page), (int)c.pages, (int)c.B, (int)c.T};
   return true;
 }
 

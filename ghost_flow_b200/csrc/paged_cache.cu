@@ -117,25 +117,21 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const __grid_c
 
 using namespace gf;
 
-// qkv [T, H + 2 Hk, D] bf16, rows ldx elements apart; q [T, H, D] dense; strides: pages, rows and heads of kpages, then of vpages, in elements.
-// Tables fp32 [positions, D / 2] dense. All rows on 16-byte boundaries.
-GF_API int gf_paged_append(const void* qkv, long long ldx, void* q, void* kpages, void* vpages, const long long* strides, const int* table,
-                           int ld_table, int width, const int* lens, const int* cu, int B, int T, int H, int Hk, int D, int page, int pages,
-                           const float* cos, const float* sin, int positions, int interleaved, int* status, void* stream) {
+// x [T, H + 2 Hk, D], y [T, H, D] dense. Tables fp32 [positions, D / 2] dense, on 16-byte boundaries.
+GF_API int gf_paged_append(const PagedCall* c, const float* cos, const float* sin, int positions, int interleaved, void* stream) {
   PagedAppend p;
-  if (!paged_batch(p.seqs, table, ld_table, width, lens, cu, B, T, page, pages, status)) return GFH_BAD_ARG;
-  if (H <= 0 || Hk <= 0 || D < 16 || D % 16 || D / 16 > PA_THREADS || positions < 0 || ldx % 8 || !strides) return GFH_BAD_ARG;
-  for (const void* x : {qkv, (const void*)q, (const void*)kpages, (const void*)vpages, (const void*)cos, (const void*)sin})
-    if (!x || (reinterpret_cast<uintptr_t>(x) & 15)) return GFH_BAD_ARG;
-  for (int i = 0; i < 6; ++i)
-    if (strides[i] % 8) return GFH_BAD_ARG;
+  if (!c || !paged_batch(p.seqs, *c)) return GFH_BAD_ARG;
+  const long long H = c->H, Hk = c->Hk, D = c->D;
+  if (H <= 0 || Hk <= 0 || H > 65535 || Hk > 65535 || D < 16 || D % 16 || D / 16 > PA_THREADS || positions < 0 || c->ldy != H * D ||
+      !cos || !sin || ((reinterpret_cast<uintptr_t>(cos) | reinterpret_cast<uintptr_t>(sin)) & 15))
+    return GFH_BAD_ARG;
   gf::enter();
-  p.qkv = (const __nv_bfloat16*)qkv; p.ldx = ldx;
-  p.q = (__nv_bfloat16*)q; p.kp = (__nv_bfloat16*)kpages; p.vp = (__nv_bfloat16*)vpages;
-  p.kpage = strides[0]; p.krow = strides[1]; p.khead = strides[2];
-  p.vpage = strides[3]; p.vrow = strides[4]; p.vhead = strides[5];
+  p.qkv = (const __nv_bfloat16*)c->x; p.ldx = c->ldx;
+  p.q = (__nv_bfloat16*)c->y; p.kp = (__nv_bfloat16*)c->kpages; p.vp = (__nv_bfloat16*)c->vpages;
+  p.kpage = c->strides[0]; p.krow = c->strides[1]; p.khead = c->strides[2];
+  p.vpage = c->strides[3]; p.vrow = c->strides[4]; p.vhead = c->strides[5];
   p.cos = cos; p.sin = sin;
-  p.H = H; p.Hk = Hk; p.D = D; p.positions = positions; p.interleaved = interleaved;
-  paged_append_kernel<<<T, PA_THREADS, 0, (cudaStream_t)stream>>>(p);
+  p.H = (int)H; p.Hk = (int)Hk; p.D = (int)D; p.positions = positions; p.interleaved = interleaved;
+  paged_append_kernel<<<p.seqs.T, PA_THREADS, 0, (cudaStream_t)stream>>>(p);
   return cudaGetLastError() == cudaSuccess ? GFH_OK : GFH_CUDA;
 }

@@ -72,10 +72,11 @@ _SIGS = {
     "gf_flash_attn_backward": [P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, P, F, I, P, P],
     "gf_llama_decode_layer": [P, P, F, P, P, P, F, P, P, P, P, P, P, I, P, P, I, I, I, I, I, I, I, I, I, P, P],
     "gf_attn_decode": [P, L, P, P, I, P, I, P, L, I, I, I, I, F, I, P, P],
-    "gf_paged_append": [P, L, P, P, P, P, P, I, I, P, P, I, I, I, I, I, I, I, P, P, I, I, P, P],
+    "gf_paged_append": [P, P, P, I, I, P],
     "gf_paged_attn_workspace": [I, I, I, I, I, I],
-    "gf_paged_attn": [P, L, P, P, P, P, I, I, P, P, P, L, I, I, I, I, I, I, I, F, P, L, P, P],
-    "gf_process_logits": [P, L, P, L, I, I, I, P, L, I, I, P, P, P, P, P, F, F, F, P, L, P, L, P],
+    "gf_paged_attn": [P, F, P, L, P],
+    "gf_paged_attn_one": [P, F, I, P, P],
+    "gf_process_logits": [P, P],
     "gf_flash_attn_bwd": [P, P, P, P, P, P, P, P, P, I, I, I, I, I, L, L, L, L, L, L, F, I, P, P],
     "gf_attn_bwd_prep": [P, P, P, P, I, I, I, I, L, L, P],
     "gf_flash_attn_bwd3": [P, P, P, P, P, P, P, P, P, I, I, I, I, I, L, L, L, L, L, L, F, I, P, P],

@@ -12,16 +12,19 @@ something follows (a gradient, tracing, transforms, modes), plain PyTorch. The r
 """
 from __future__ import annotations
 
-import ctypes
 import functools
 import math
+import struct
 
 import torch
 
 from . import _lib
 from .fused import _observed, _rc, _rope_tables_fit_kernel, _rows_apart
+from .gemm import _sm_count
+from .raw import _decode_parts
 
 _INT32, _BF16 = torch.int32, torch.bfloat16
+_MOST = 2 ** 31 - 1
 
 
 def _check_batch(what, x, kpages, vpages, page_table, lens, cu) -> None:
@@ -44,22 +47,11 @@ def _check_batch(what, x, kpages, vpages, page_table, lens, cu) -> None:
         raise ValueError(f"{what}: tensors on different devices")
 
 
-def _ints_fit_kernel(page_table, lens, cu) -> bool:
-    return page_table.stride(1) == 1 and lens.is_contiguous() and (cu is None or cu.is_contiguous())
-
-
-def _pages_fit_kernel(kpages, vpages) -> bool:
-    P, page, Hk, D = kpages.shape
-    a, b = kpages.stride(), vpages.stride()
-    return (P > 0 and Hk > 0 and page >= 16 and page & (page - 1) == 0 and P * page < 2 ** 31 and a[3] == 1 and b[3] == 1
-            and not (a[0] | a[1] | a[2] | b[0] | b[1] | b[2]) & 7 and not (kpages.data_ptr() | vpages.data_ptr()) & 15)
-
-
 def _pages_apart(kpages, vpages) -> bool:
     """Whether no two rows of the pools share memory."""
     between = abs(kpages.data_ptr() - vpages.data_ptr()) // kpages.element_size()
-    if between >= kpages.numel() and kpages.is_contiguous() and vpages.is_contiguous():
-        return True
+    if kpages.is_contiguous() and vpages.is_contiguous():
+        return between >= kpages.numel()
     D = kpages.shape[3]
     dims = [[*zip(t.stride()[:3], t.shape[:3])] for t in (kpages, vpages)]
     if dims[0] == dims[1]:                 # the pools themselves are one more dimension
@@ -69,12 +61,35 @@ def _pages_apart(kpages, vpages) -> bool:
     return all(_rows_apart(D, d) for d in dims) and ends[0][1] <= ends[1][0]
 
 
-def _strides(kpages, vpages):
-    return (ctypes.c_longlong * 6)(*kpages.stride()[:3], *vpages.stride()[:3])
+# the PagedCall of csrc/paged.cuh
+_CALL = struct.Struct("25q").pack
 
 
-def _wants_grad(*ts) -> bool:
-    return torch.is_grad_enabled() and any(t.requires_grad for t in ts)
+def _for_kernels(x, kpages, vpages, page_table, lens, cu):
+    """What a kernel call needs to know of a batch that the kernels take, in few looks at the tensors (a call for one token of a small
+    model is all host time): its device index, and the pools' strides and shape. ``None``: see :func:`_check_batch` for why."""
+    dev = x.device
+    if x.dtype is not _BF16 or dev.type != "cuda" or not (kpages.device == dev == vpages.device) or kpages.dtype is not _BF16 \
+            or vpages.dtype is not _BF16 or not (page_table.device == dev == lens.device) or page_table.dtype is not _INT32 \
+            or lens.dtype is not _INT32 or x.dim() != 3 or lens.dim() != 1 or page_table.dim() != 2:
+        return None
+    shape, (B,), (Bt, width) = kpages.shape, lens.shape, page_table.shape
+    if len(shape) != 4 or vpages.shape != shape or Bt != B or B == 0 or not page_table.stride(1) == 1 == lens.stride(0):
+        return None
+    if cu is None:
+        if x.shape[0] != B:
+            return None
+    elif cu.dtype is not _INT32 or cu.device != dev or cu.dim() != 1 or cu.shape[0] != B + 1 or cu.stride(0) != 1:
+        return None
+    P, page, Hk, D = shape
+    a0, a1, a2, a3 = kpages.stride()
+    b0, b1, b2, b3 = vpages.stride()
+    if P == 0 or Hk == 0 or page < 16 or page & (page - 1) or P * page > _MOST or width > _MOST // page or not a3 == 1 == b3 \
+            or (a0 | a1 | a2 | b0 | b1 | b2) & 7 or (kpages.data_ptr() | vpages.data_ptr()) & 15:
+        return None
+    if torch.is_grad_enabled() and (x.requires_grad or kpages.requires_grad or vpages.requires_grad) or _observed():
+        return None
+    return dev.index, B, width, P, page, Hk, D, (a0, a1, a2, b0, b1, b2)
 
 
 def _report(device, bad, what: str) -> None:
@@ -138,34 +153,40 @@ def rope_qkv_to_pages(qkv, num_heads: int, num_kv_heads: int, cos, sin, kpages, 
     or a position that is not in the tables or behind the page table, is left out too, and ``_lib.check_status`` raises.
     Inference only: a call with a gradient to record takes PyTorch's operations."""
     H, Hk = num_heads, num_kv_heads
-    what = "rope_qkv_to_pages"
-    if qkv.dim() != 3 or qkv.shape[1] != H + 2 * Hk or H < 1 or Hk < 1:
-        raise ValueError(f"{what}: a packed projection of {H} + 2 x {Hk} heads is [tokens, {H + 2 * Hk}, head size], not {list(qkv.shape)}")
-    _check_batch(what, qkv, kpages, vpages, page_table, lens, cu)
-    T, _, D = qkv.shape
-    dev = qkv.device
-    if kpages.shape[2] != Hk or kpages.shape[3] != D:
-        raise ValueError(f"{what}: pages of {kpages.shape[2]} heads of {kpages.shape[3]} for {Hk} heads of {D}")
-    if not (cos.dim() == 2 and cos.shape == sin.shape and 2 * cos.shape[1] == D and cos.device == sin.device == dev):
-        raise ValueError(f"{what}: rope tables must be [positions, {D // 2}] on {dev}, got {list(cos.shape)} on {cos.device} and "
-                         f"{list(sin.shape)} on {sin.device}")
-    if T == 0:
-        return qkv.new_empty(0, H, D)
-    if not (qkv.is_cuda and qkv.dtype is _BF16) or _wants_grad(qkv, kpages, vpages) or _observed() or D % 16 or D > 4096 \
-            or not _ints_fit_kernel(page_table, lens, cu) or not _pages_fit_kernel(kpages, vpages) or not _pages_apart(kpages, vpages) \
-            or not _rope_tables_fit_kernel(cos, sin):
+    fits = _for_kernels(qkv, kpages, vpages, page_table, lens, cu)
+    if fits is not None:
+        device, B, width, P, page, heads, D, strides = fits
+        T, G, Dx = qkv.shape
+        n = cos.shape[0]
+        if not (heads == Hk > 0 < H and G == H + 2 * Hk and Dx == D and D % 16 == 0 and D <= 4096 and T > 0 and cos.shape == sin.shape == (n, D // 2)
+                and cos.device == sin.device == qkv.device and _rope_tables_fit_kernel(cos, sin) and _pages_apart(kpages, vpages)):
+            fits = None
+    if fits is None:
+        what = "rope_qkv_to_pages"
+        if qkv.dim() != 3 or qkv.shape[1] != H + 2 * Hk or H < 1 or Hk < 1:
+            raise ValueError(f"{what}: a packed projection of {H} + 2 x {Hk} heads is [tokens, {H + 2 * Hk}, head size], not {list(qkv.shape)}")
+        _check_batch(what, qkv, kpages, vpages, page_table, lens, cu)
+        T, _, D = qkv.shape
+        if kpages.shape[2] != Hk or kpages.shape[3] != D or D % 2:
+            raise ValueError(f"{what}: pages of {kpages.shape[2]} heads of {kpages.shape[3]} for {Hk} heads of {D}")
+        if not (cos.dim() == 2 and cos.shape == sin.shape and 2 * cos.shape[1] == D and cos.device == sin.device == qkv.device):
+            raise ValueError(f"{what}: rope tables must be [positions, {D // 2}] on {qkv.device}, got {list(cos.shape)} on {cos.device} and "
+                             f"{list(sin.shape)} on {sin.device}")
+        if T == 0:
+            return qkv.new_empty(0, H, D)
         return _append_ref(qkv, H, Hk, cos, sin, kpages, vpages, page_table, lens, cu, interleaved)
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
+    if device != torch.cuda.current_device():
+        with torch.cuda.device(device):
             return rope_qkv_to_pages(qkv, H, Hk, cos, sin, kpages, vpages, page_table, lens, cu, interleaved)
-    if qkv.stride(2) != 1 or qkv.stride(1) != D or qkv.stride(0) % 8 or qkv.data_ptr() % 16:
-        qkv = qkv.clone(memory_format=torch.contiguous_format)
-    q = torch.empty((T, H, D), dtype=_BF16, device=dev)
+    x, (ld, sh, se) = qkv, qkv.stride()
+    if se != 1 or sh != D or ld % 8 or x.data_ptr() % 16:
+        x, ld = qkv.clone(memory_format=torch.contiguous_format), G * D
+    q = qkv.new_empty((T, H, D))
     _rc(_lib.cuda_lib().gf_paged_append(
-        qkv.data_ptr(), qkv.stride(0), q.data_ptr(), kpages.data_ptr(), vpages.data_ptr(), _strides(kpages, vpages),
-        page_table.data_ptr(), page_table.stride(0), page_table.shape[1], lens.data_ptr(), None if cu is None else cu.data_ptr(),
-        lens.shape[0], T, H, Hk, D, kpages.shape[1], kpages.shape[0], cos.data_ptr(), sin.data_ptr(), cos.shape[0],
-        1 if interleaved else 0, _lib.status_word(dev).data_ptr(), _lib.stream_ptr()), "gf_paged_append")
+        _CALL(x.data_ptr(), ld, q.data_ptr(), H * D, kpages.data_ptr(), vpages.data_ptr(), *strides, page_table.data_ptr(),
+              page_table.stride(0), width, lens.data_ptr(), 0 if cu is None else cu.data_ptr(), B, T, H, Hk, D, page, P,
+              _lib.status_word(qkv.device).data_ptr()),
+        cos.data_ptr(), sin.data_ptr(), n, 1 if interleaved else 0, _lib.stream_ptr()), "gf_paged_append")
     torch.autograd.graph.increment_version((kpages, vpages))     # a graph that saved the pools has to notice the write
     return q
 
@@ -225,43 +246,60 @@ def paged_attention(q, kpages, vpages, page_table, lens, cu=None, scale: float |
     written and returned. A page that is not in the pools reads as zeros, keys behind the page table do not exist, and
     ``_lib.check_status`` raises for both. Head sizes 64 and 128 with pages of a power of two from 16 rows take the kernels.
     Inference only: a call with a gradient to record takes PyTorch's operations."""
+    fits = _for_kernels(q, kpages, vpages, page_table, lens, cu)
+    if fits is not None:
+        device, B, width, P, page, Hk, D, strides = fits
+        T, H, Dx = q.shape
+        if not (T > 0 and Dx == D and (D == 128 or D == 64) and H > 0 and H % Hk == 0 and H // Hk <= 128 and 0 not in strides):
+            fits = None
+        elif out is not None:
+            st = out.stride()
+            if out.shape != q.shape or out.dtype is not _BF16 or out.device != q.device or st[2] != 1 or st[1] != D or st[0] % 8 \
+                    or st[0] < H * D or out.data_ptr() % 16:
+                fits = None
     what = "paged_attention"
-    if q.dim() != 3:
-        raise ValueError(f"{what}: q is [tokens, heads, head size], not {list(q.shape)}")
-    _check_batch(what, q, kpages, vpages, page_table, lens, cu)
-    T, H, D = q.shape
-    Hk, dev = kpages.shape[2], q.device
-    if kpages.shape[3] != D or Hk < 1 or H < 1 or H % Hk:
-        raise ValueError(f"{what}: {H} heads of {D} over pages of {Hk} heads of {kpages.shape[3]}")
-    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != dev):
-        raise ValueError(f"{what}: out is {list(q.shape)} of {q.dtype} on {dev}, not {list(out.shape)} of {out.dtype} on {out.device}")
-    if T == 0:
-        return torch.empty_like(q) if out is None else out
+    if fits is None:
+        if q.dim() != 3:
+            raise ValueError(f"{what}: q is [tokens, heads, head size], not {list(q.shape)}")
+        _check_batch(what, q, kpages, vpages, page_table, lens, cu)
+        T, H, D = q.shape
+        Hk = kpages.shape[2]
+        if kpages.shape[3] != D or Hk < 1 or H < 1 or H % Hk:
+            raise ValueError(f"{what}: {H} heads of {D} over pages of {Hk} heads of {kpages.shape[3]}")
+        if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device):
+            raise ValueError(f"{what}: out is {list(q.shape)} of {q.dtype} on {q.device}, not {list(out.shape)} of {out.dtype} on {out.device}")
+        if T == 0:
+            return torch.empty_like(q) if out is None else out
     if out is not None and (_ranges_overlap(out, q) or _ranges_overlap(out, kpages) or _ranges_overlap(out, vpages)):
         raise ValueError(f"{what}: out shares memory with q or the pages")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not math.isfinite(scale):
         raise ValueError(f"{what}: a scale of {scale}")
-    if not (q.is_cuda and q.dtype is _BF16) or D not in (64, 128) or H // Hk > 128 or _wants_grad(q, kpages, vpages) or _observed() \
-            or not _ints_fit_kernel(page_table, lens, cu) or not _pages_fit_kernel(kpages, vpages) or 0 in kpages.stride() + vpages.stride() \
-            or (out is not None and (out.stride(2) != 1 or out.stride(1) != D or out.stride(0) % 8 or out.stride(0) < H * D
-                                     or out.data_ptr() % 16)):
+    if fits is None:
         return _attention_ref(q, kpages, vpages, page_table, lens, cu, scale, out)
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
+    if device != torch.cuda.current_device():
+        with torch.cuda.device(device):
             return paged_attention(q, kpages, vpages, page_table, lens, cu, scale, out)
-    if not scale > 0:                        # the kernel takes the largest score before it scales
-        q, scale = q * (-1 if scale < 0 else 0), -scale if scale < 0 else 1.0
-    if q.stride(2) != 1 or q.stride(1) != D or q.stride(0) % 8 or q.data_ptr() % 16 or (T > 1 and q.stride(0) < H * D):
-        q = q.clone(memory_format=torch.contiguous_format)
-    o = torch.empty((T, H, D), dtype=_BF16, device=dev) if out is None else out
-    nbytes = _attention_workspace(dev.index, lens.shape[0], T, cu is None, H, Hk, D)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    _rc(_lib.cuda_lib().gf_paged_attn(
-        q.data_ptr(), q.stride(0), kpages.data_ptr(), vpages.data_ptr(), _strides(kpages, vpages), page_table.data_ptr(),
-        page_table.stride(0), page_table.shape[1], lens.data_ptr(), None if cu is None else cu.data_ptr(), o.data_ptr(), o.stride(0),
-        lens.shape[0], T, H, Hk, D, kpages.shape[1], kpages.shape[0], scale, None if ws is None else ws.data_ptr(),
-        nbytes, _lib.status_word(dev).data_ptr(), _lib.stream_ptr()), "gf_paged_attn")
+    one = cu is None and H // Hk <= 8
+    x = q
+    if not scale > 0 and not one:            # this kernel takes the largest score before it scales
+        x, scale = q * (-1 if scale < 0 else 0), -scale if scale < 0 else 1.0
+    ld, sh, se = x.stride()
+    if se != 1 or sh != D or ld % 8 or x.data_ptr() % 16 or ld < H * D:
+        x, ld = x.clone(memory_format=torch.contiguous_format), H * D
+    o = q.new_empty((T, H, D)) if out is None else out
+    lib = _lib.cuda_lib()
+    call = (x.data_ptr(), ld, o.data_ptr(), o.stride(0), kpages.data_ptr(), vpages.data_ptr(), *strides, page_table.data_ptr(),
+            page_table.stride(0), width, lens.data_ptr(), 0 if cu is None else cu.data_ptr(), B, T, H, Hk, D, page, P,
+            _lib.status_word(q.device).data_ptr())
+    if one:
+        parts = _decode_parts(B, Hk, width * page, D, _sm_count(q.device), True)
+        ws = torch.empty((B * parts if parts > 0 else -2 * parts) * H * (D + 2), dtype=torch.float32, device=q.device)
+        _rc(lib.gf_paged_attn_one(_CALL(*call), scale, parts, ws.data_ptr(), _lib.stream_ptr()), "gf_paged_attn_one")
+    else:
+        nbytes = _attention_workspace(device, B, T, cu is None, H, Hk, D)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+        _rc(lib.gf_paged_attn(_CALL(*call), scale, None if ws is None else ws.data_ptr(), nbytes, _lib.stream_ptr()), "gf_paged_attn")
     if out is not None:
         torch.autograd.graph.increment_version(out)
     return o

@@ -5,12 +5,15 @@ CUDA logits of fp32, bf16 or fp16 take the kernel of ``csrc/logits.cu``; CPU ten
 gradient, tracing, transforms, modes) plain PyTorch."""
 from __future__ import annotations
 
+import struct
+
 import torch
 
 from . import _lib
 from .fused import _observed, _rc
 from .paged import _ranges_overlap
 
+_CALL = struct.Struct("16q3d4q").pack      # the LogitsCall of csrc/logits.cu
 _KINDS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -114,18 +117,18 @@ def process_logits(logits, tokens=None, token_lens=None, generated_from=None, re
             logits, memory_format=torch.contiguous_format)
 
     def pointer(t):
-        return t.data_ptr() if torch.is_tensor(t) else None
+        return t.data_ptr() if torch.is_tensor(t) else 0
 
-    def number(t, otherwise):
-        return otherwise if torch.is_tensor(t) else float(t)
+    def number(t):
+        return 0.0 if torch.is_tensor(t) else float(t)
 
-    _rc(_lib.cuda_lib().gf_process_logits(
+    _rc(_lib.cuda_lib().gf_process_logits(_CALL(
         logits.data_ptr(), logits.stride(0), y.data_ptr(), y.stride(0), _KINDS[logits.dtype], B, V, pointer(tokens),
         0 if tokens is None else tokens.stride(0), 0 if tokens is None else int(tokens.dtype is torch.int64),
         0 if tokens is None else tokens.shape[1], pointer(token_lens), pointer(generated_from), pointer(repetition), pointer(presence),
-        pointer(frequency), number(repetition, 1.0), number(presence, 0.0), number(frequency, 0.0), pointer(bias),
+        pointer(frequency), number(repetition), number(presence), number(frequency), pointer(bias),
         0 if bias is None or bias.dim() == 1 else bias.stride(0), pointer(allowed),
-        0 if allowed is None or allowed.dim() == 1 else allowed.stride(0), _lib.stream_ptr()), "gf_process_logits")
+        0 if allowed is None or allowed.dim() == 1 else allowed.stride(0)), _lib.stream_ptr()), "gf_process_logits")
     if out is not None:
         torch.autograd.graph.increment_version(out)
     return y
