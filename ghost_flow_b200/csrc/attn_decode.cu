@@ -700,7 +700,7 @@ GF_API int gf_attn_decode(const void* q, long long ldq, const void* kcache, cons
 GF_API int gf_paged_attn_one(const PagedCall* c, float scale, int splits, float* scratch, void* stream) {
   DecParams p{};
   if (!c || c->cu || !paged_batch(p.pages, *c) || c->H <= 0 || c->Hk <= 0 || c->H % c->Hk || c->H / c->Hk > DEC_MAX_G ||
-      (c->D != 64 && c->D != 128) || splits == 0 || !scratch || c->pages == 0)
+      (c->D != 64 && c->D != 128) || splits == 0 || (!scratch && splits != 1) || c->pages == 0)
     return GFH_BAD_ARG;
   if (splits > 65535) splits = 65535;
   gf::enter();

@@ -167,7 +167,26 @@ def stream_ptr() -> int:
     return _RAW_STREAM(dev) if _RAW_STREAM is not None else torch.cuda.current_stream().cuda_stream
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def stream_on(device: int):
+    """:func:`stream_ptr` where ``device`` (an index) is the current one, else ``None``: launches go to the current device. For a tensor's
+    device: CUDA is there."""
+    if _current_device() != device:
+        return None
+    if device != getattr(_BOUND, "device", -1) or _RAW_STREAM is None:
+        return stream_ptr()
+    return _RAW_STREAM(device)
+
+
 _STATUS = {}
+
+
+def status_ptr(device: int) -> int:
+    """Address of :func:`status_word` of a device's index."""
+    t = _STATUS.get(device)
+    return (status_word(torch.device("cuda", device)) if t is None else t).data_ptr()
 
 
 def status_word(device=None) -> torch.Tensor:

@@ -25,6 +25,7 @@ from .raw import _decode_parts
 
 _INT32, _BF16 = torch.int32, torch.bfloat16
 _MOST = 2 ** 31 - 1
+_increment_version = torch.autograd.graph.increment_version
 
 
 def _check_batch(what, x, kpages, vpages, page_table, lens, cu) -> None:
@@ -47,17 +48,16 @@ def _check_batch(what, x, kpages, vpages, page_table, lens, cu) -> None:
         raise ValueError(f"{what}: tensors on different devices")
 
 
-def _pages_apart(kpages, vpages) -> bool:
-    """Whether no two rows of the pools share memory."""
-    between = abs(kpages.data_ptr() - vpages.data_ptr()) // kpages.element_size()
-    if kpages.is_contiguous() and vpages.is_contiguous():
-        return between >= kpages.numel()
-    D = kpages.shape[3]
-    dims = [[*zip(t.stride()[:3], t.shape[:3])] for t in (kpages, vpages)]
+def _pages_apart(P, page, Hk, D, pools) -> bool:
+    """Whether no two rows of the pools share memory (addresses of bf16, strides of pages, rows and heads of each)."""
+    k, v, a0, a1, a2, b0, b1, b2 = pools
+    between = abs(k - v) // 2
+    if a2 == b2 == D and a1 == b1 == Hk * D and a0 == b0 == page * a1:         # two dense pools
+        return between >= P * a0
+    dims = ((a0, P), (a1, page), (a2, Hk)), ((b0, P), (b1, page), (b2, Hk))
     if dims[0] == dims[1]:                 # the pools themselves are one more dimension
         return _rows_apart(D, [*dims[0], (between, 2)])
-    ends = sorted((t.data_ptr(), t.data_ptr() + t.element_size() * (D + sum(st * (n - 1) for st, n in d)))
-                  for t, d in zip((kpages, vpages), dims))
+    ends = sorted((at, at + 2 * (D + sum(st * (n - 1) for st, n in d))) for at, d in zip((k, v), dims))
     return all(_rows_apart(D, d) for d in dims) and ends[0][1] <= ends[1][0]
 
 
@@ -67,29 +67,32 @@ _CALL = struct.Struct("25q").pack
 
 def _for_kernels(x, kpages, vpages, page_table, lens, cu):
     """What a kernel call needs to know of a batch that the kernels take, in few looks at the tensors (a call for one token of a small
-    model is all host time): its device index, and the pools' strides and shape. ``None``: see :func:`_check_batch` for why."""
-    dev = x.device
-    if x.dtype is not _BF16 or dev.type != "cuda" or not (kpages.device == dev == vpages.device) or kpages.dtype is not _BF16 \
-            or vpages.dtype is not _BF16 or not (page_table.device == dev == lens.device) or page_table.dtype is not _INT32 \
-            or lens.dtype is not _INT32 or x.dim() != 3 or lens.dim() != 1 or page_table.dim() != 2:
+    model is all host time): its device, the sizes of the batch and the pools, and the pools' addresses and strides. ``None``:
+    see :func:`_check_batch` for why."""
+    dev = x.get_device()
+    if dev < 0 or x.dtype is not _BF16 or kpages.dtype is not _BF16 or vpages.dtype is not _BF16 or page_table.dtype is not _INT32 \
+            or lens.dtype is not _INT32 or not dev == kpages.get_device() == vpages.get_device() == page_table.get_device() == lens.get_device() \
+            or x.dim() != 3 or lens.dim() != 1 or page_table.dim() != 2 or kpages.dim() != 4:
         return None
-    shape, (B,), (Bt, width) = kpages.shape, lens.shape, page_table.shape
-    if len(shape) != 4 or vpages.shape != shape or Bt != B or B == 0 or not page_table.stride(1) == 1 == lens.stride(0):
+    shape, B, (Bt, width) = kpages.shape, lens.shape[0], page_table.shape
+    if vpages.shape != shape or Bt != B or B == 0 or not page_table.stride(1) == 1 == lens.stride(0):
         return None
     if cu is None:
         if x.shape[0] != B:
             return None
-    elif cu.dtype is not _INT32 or cu.device != dev or cu.dim() != 1 or cu.shape[0] != B + 1 or cu.stride(0) != 1:
+    elif cu.dtype is not _INT32 or cu.get_device() != dev or cu.dim() != 1 or cu.shape[0] != B + 1 or cu.stride(0) != 1:
         return None
     P, page, Hk, D = shape
     a0, a1, a2, a3 = kpages.stride()
     b0, b1, b2, b3 = vpages.stride()
     if P == 0 or Hk == 0 or page < 16 or page & (page - 1) or P * page > _MOST or width > _MOST // page or not a3 == 1 == b3 \
-            or (a0 | a1 | a2 | b0 | b1 | b2) & 7 or (kpages.data_ptr() | vpages.data_ptr()) & 15:
+            or (a0 | a1 | a2 | b0 | b1 | b2) & 7 or _observed() \
+            or (torch.is_grad_enabled() and (x.requires_grad or kpages.requires_grad or vpages.requires_grad)):
         return None
-    if torch.is_grad_enabled() and (x.requires_grad or kpages.requires_grad or vpages.requires_grad) or _observed():
+    k, v = kpages.data_ptr(), vpages.data_ptr()        # behind _observed: transformed tensors have no memory
+    if (k | v) & 15:
         return None
-    return dev.index, B, width, P, page, Hk, D, (a0, a1, a2, b0, b1, b2)
+    return dev, B, width, P, page, Hk, D, (k, v, a0, a1, a2, b0, b1, b2)
 
 
 def _report(device, bad, what: str) -> None:
@@ -155,11 +158,12 @@ def rope_qkv_to_pages(qkv, num_heads: int, num_kv_heads: int, cos, sin, kpages, 
     H, Hk = num_heads, num_kv_heads
     fits = _for_kernels(qkv, kpages, vpages, page_table, lens, cu)
     if fits is not None:
-        device, B, width, P, page, heads, D, strides = fits
+        device, B, width, P, page, heads, D, pools = fits
         T, G, Dx = qkv.shape
-        n = cos.shape[0]
-        if not (heads == Hk > 0 < H and G == H + 2 * Hk and Dx == D and D % 16 == 0 and D <= 4096 and T > 0 and cos.shape == sin.shape == (n, D // 2)
-                and cos.device == sin.device == qkv.device and _rope_tables_fit_kernel(cos, sin) and _pages_apart(kpages, vpages)):
+        tables = cos.shape
+        n = tables[0] if len(tables) == 2 and tables[1] * 2 == D and sin.shape == tables and device == cos.get_device() == sin.get_device() else -1
+        if not (heads == Hk > 0 < H and G == H + 2 * Hk and Dx == D and D % 16 == 0 and D <= 4096 and T > 0 and n >= 0
+                and _rope_tables_fit_kernel(cos, sin) and _pages_apart(P, page, Hk, D, pools)):
             fits = None
     if fits is None:
         what = "rope_qkv_to_pages"
@@ -175,19 +179,20 @@ def rope_qkv_to_pages(qkv, num_heads: int, num_kv_heads: int, cos, sin, kpages, 
         if T == 0:
             return qkv.new_empty(0, H, D)
         return _append_ref(qkv, H, Hk, cos, sin, kpages, vpages, page_table, lens, cu, interleaved)
-    if device != torch.cuda.current_device():
+    stream = _lib.stream_on(device)
+    if stream is None:
         with torch.cuda.device(device):
             return rope_qkv_to_pages(qkv, H, Hk, cos, sin, kpages, vpages, page_table, lens, cu, interleaved)
-    x, (ld, sh, se) = qkv, qkv.stride()
-    if se != 1 or sh != D or ld % 8 or x.data_ptr() % 16:
-        x, ld = qkv.clone(memory_format=torch.contiguous_format), G * D
+    x, (ld, sh, se), at = qkv, qkv.stride(), qkv.data_ptr()
+    if se != 1 or sh != D or ld % 8 or at % 16:
+        x = qkv.clone(memory_format=torch.contiguous_format)
+        ld, at = G * D, x.data_ptr()
     q = qkv.new_empty((T, H, D))
     _rc(_lib.cuda_lib().gf_paged_append(
-        _CALL(x.data_ptr(), ld, q.data_ptr(), H * D, kpages.data_ptr(), vpages.data_ptr(), *strides, page_table.data_ptr(),
-              page_table.stride(0), width, lens.data_ptr(), 0 if cu is None else cu.data_ptr(), B, T, H, Hk, D, page, P,
-              _lib.status_word(qkv.device).data_ptr()),
-        cos.data_ptr(), sin.data_ptr(), n, 1 if interleaved else 0, _lib.stream_ptr()), "gf_paged_append")
-    torch.autograd.graph.increment_version((kpages, vpages))     # a graph that saved the pools has to notice the write
+        _CALL(at, ld, q.data_ptr(), H * D, *pools, page_table.data_ptr(), page_table.stride(0), width, lens.data_ptr(),
+              0 if cu is None else cu.data_ptr(), B, T, H, Hk, D, page, P, _lib.status_ptr(device)),
+        cos.data_ptr(), sin.data_ptr(), n, 1 if interleaved else 0, stream), "gf_paged_append")
+    _increment_version((kpages, vpages))     # a graph that saved the pools has to notice the write
     return q
 
 
@@ -248,9 +253,9 @@ def paged_attention(q, kpages, vpages, page_table, lens, cu=None, scale: float |
     Inference only: a call with a gradient to record takes PyTorch's operations."""
     fits = _for_kernels(q, kpages, vpages, page_table, lens, cu)
     if fits is not None:
-        device, B, width, P, page, Hk, D, strides = fits
+        device, B, width, P, page, Hk, D, pools = fits
         T, H, Dx = q.shape
-        if not (T > 0 and Dx == D and (D == 128 or D == 64) and H > 0 and H % Hk == 0 and H // Hk <= 128 and 0 not in strides):
+        if not (T > 0 and Dx == D and (D == 128 or D == 64) and H > 0 and H % Hk == 0 and H // Hk <= 128 and 0 not in pools[2:]):
             fits = None
         elif out is not None:
             st = out.stride()
@@ -277,29 +282,32 @@ def paged_attention(q, kpages, vpages, page_table, lens, cu=None, scale: float |
         raise ValueError(f"{what}: a scale of {scale}")
     if fits is None:
         return _attention_ref(q, kpages, vpages, page_table, lens, cu, scale, out)
-    if device != torch.cuda.current_device():
+    stream = _lib.stream_on(device)
+    if stream is None:
         with torch.cuda.device(device):
             return paged_attention(q, kpages, vpages, page_table, lens, cu, scale, out)
     one = cu is None and H // Hk <= 8
     x = q
     if not scale > 0 and not one:            # this kernel takes the largest score before it scales
         x, scale = q * (-1 if scale < 0 else 0), -scale if scale < 0 else 1.0
-    ld, sh, se = x.stride()
-    if se != 1 or sh != D or ld % 8 or x.data_ptr() % 16 or ld < H * D:
-        x, ld = x.clone(memory_format=torch.contiguous_format), H * D
-    o = q.new_empty((T, H, D)) if out is None else out
-    lib = _lib.cuda_lib()
-    call = (x.data_ptr(), ld, o.data_ptr(), o.stride(0), kpages.data_ptr(), vpages.data_ptr(), *strides, page_table.data_ptr(),
-            page_table.stride(0), width, lens.data_ptr(), 0 if cu is None else cu.data_ptr(), B, T, H, Hk, D, page, P,
-            _lib.status_word(q.device).data_ptr())
+    (ld, sh, se), at = x.stride(), x.data_ptr()
+    if se != 1 or sh != D or ld % 8 or at % 16 or ld < H * D:
+        x = x.clone(memory_format=torch.contiguous_format)
+        ld, at = H * D, x.data_ptr()
+    if out is not None:
+        o, ldo = out, out.stride(0)
+    else:
+        o, ldo = torch.empty_like(x) if ld == H * D else q.new_empty((T, H, D)), H * D
+    call = _CALL(at, ld, o.data_ptr(), ldo, *pools, page_table.data_ptr(), page_table.stride(0), width, lens.data_ptr(),
+                 0 if cu is None else cu.data_ptr(), B, T, H, Hk, D, page, P, _lib.status_ptr(device))
     if one:
         parts = _decode_parts(B, Hk, width * page, D, _sm_count(q.device), True)
-        ws = torch.empty((B * parts if parts > 0 else -2 * parts) * H * (D + 2), dtype=torch.float32, device=q.device)
-        _rc(lib.gf_paged_attn_one(_CALL(*call), scale, parts, ws.data_ptr(), _lib.stream_ptr()), "gf_paged_attn_one")
+        ws = None if parts == 1 else torch.empty((B * parts if parts > 0 else -2 * parts) * H * (D + 2), dtype=torch.float32, device=q.device)
+        _rc(_lib.cuda_lib().gf_paged_attn_one(call, scale, parts, None if ws is None else ws.data_ptr(), stream), "gf_paged_attn_one")
     else:
         nbytes = _attention_workspace(device, B, T, cu is None, H, Hk, D)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-        _rc(lib.gf_paged_attn(_CALL(*call), scale, None if ws is None else ws.data_ptr(), nbytes, _lib.stream_ptr()), "gf_paged_attn")
+        _rc(_lib.cuda_lib().gf_paged_attn(call, scale, None if ws is None else ws.data_ptr(), nbytes, stream), "gf_paged_attn")
     if out is not None:
-        torch.autograd.graph.increment_version(out)
+        _increment_version(out)
     return o
