@@ -15,6 +15,8 @@
 //  * Rows behind a sequence's last key may hold anything. Scores there are set to -inf, but a product takes 0 * V too, so an idle warp clears those
 //    rows of V in shared memory before the tile is handed on. Pages that are not there, and those behind the last, are zeros from TMA (a
 //    coordinate outside of the pool).
+#include <type_traits>
+
 #include "paged.cuh"
 
 namespace gf {
@@ -616,18 +618,30 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   }
 }
 
-// Adds up the pieces of blocks that were cut: a CTA takes one token and KV head after the other, a thread a column of a row.
+// Adds up the pieces of blocks that were cut: a warp takes one token's row (a query head) after the other, a lane D / 32 columns of it. What the
+// rows belong to is found before the first kernel has ended.
 template <int HD>
 __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ PagedAttn p) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int U = *p.plan, lane = threadIdx.x & 31;
-  if (U == PG_WHOLE) return;
-  for (long long x = blockIdx.x; x < (long long)p.seqs.T * p.Hkv; x += gridDim.x) {
-    const int t = (int)(x / p.Hkv), hk = (int)(x % p.Hkv);
+  constexpr int E = HD / 32;
+  using Vec = typename std::conditional<E == 4, float4, float2>::type;
+  const int lane = threadIdx.x & 31;
+  const long long rows = (long long)p.seqs.T * p.Hq;
+  int U = 0;
+  for (long long x = blockIdx.x * 8ll + (threadIdx.x >> 5); x < rows; x += gridDim.x * 8ll) {
+    const int t = (int)(x / p.Hq), h = (int)(x - (long long)t * p.Hq), hk = h / p.G;
     const int b = paged_seq_of(p.seqs, t);
-    if (b >= p.seqs.B) return;
-    const PgShape s = pg_shape(p, b);
-    const int first = p.seqs.first(b), pieces = (s.steps + U - 1) / U;
+    PgShape s{};
+    int first = 0;
+    if (b < p.seqs.B) {
+      s = pg_shape(p, b);
+      first = p.seqs.first(b);
+    }
+    if (U == 0) {
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      U = *p.plan;
+    }
+    if (U == PG_WHOLE || b >= p.seqs.B) return;
+    const int pieces = (s.steps + U - 1) / U;
     if (pieces == 1 || t < first || t >= first + s.n) continue;
     int before = 0;                // items of the sequences in front
     for (int i = lane; i < b; i += 32) {
@@ -641,26 +655,44 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
     const int in = t - it.token, steps = it.steps(2 * p.tq);
     const long long item = before + ((long long)(s.blocks - 1 - blk) * p.Hkv + hk) * pieces;
     if (item + pieces > p.items) return;                   // sequences that overlap in `cu`: not all items were run
-    const int d = threadIdx.x % HD;
-    for (int g = threadIdx.x / HD; g < p.G; g += blockDim.x / HD) {
-      const int r = (in / p.tq) * PG_TILE + (in % p.tq) * p.G + g;
-      float m = -INFINITY, l = 0.f, o = 0.f;
-      auto there = [&](int k) { return (long long)steps * k / pieces < (long long)steps * (k + 1) / pieces; };
+    const long long row = item * p.rows + (in / p.tq) * PG_TILE + (in % p.tq) * p.G + (h - hk * p.G);
+    float m = -INFINITY, l = 0.f, o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = 0.f;
+    for (int k0 = 0; k0 < pieces; k0 += 32) {              // a lane has a piece's maximum and sum
+      const int k = k0 + lane;
+      const bool there = k < pieces && (long long)steps * k / pieces < (long long)steps * (k + 1) / pieces;
+      const float2 ml = there ? *reinterpret_cast<const float2*>(p.part_ml + 2 * (row + (long long)k * p.rows)) : make_float2(-INFINITY, 0.f);
+      float mm = ml.x;
+#pragma unroll
+      for (int i = 16; i; i >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, i));
+      mm = fmaxf(mm, m);
+      const float use = mm == -INFINITY ? 0.f : mm, old = ex2_approx(m - use), w = ml.y > 0.f ? ex2_approx(ml.x - use) : 0.f;
+      m = mm;
+      float sum = ml.y * w;
+#pragma unroll
+      for (int i = 16; i; i >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
+      l = l * old + sum;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] *= old;
+      const int n = min(32, pieces - k0);
+      const float* part = p.part + (row + (long long)k0 * p.rows) * HD + lane * E;
 #pragma unroll 4
-      for (int k = 0; k < pieces; ++k)
-        if (there(k)) m = fmaxf(m, p.part_ml[2 * ((item + k) * p.rows + r)]);
-      const float use = m == -INFINITY ? 0.f : m;
-#pragma unroll 4
-      for (int k = 0; k < pieces; ++k) {
-        if (!there(k)) continue;
-        const long long row = (item + k) * p.rows + r;
-        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * row);
-        const float w = ex2_approx(ml.x - use);
-        l += ml.y * w;
-        o += ml.y > 0.f ? p.part[row * HD + d] * w : 0.f;
+      for (int i = 0; i < n; ++i) {
+        const float wi = __shfl_sync(0xffffffffu, w, i);
+        const Vec v = *reinterpret_cast<const Vec*>(part + (long long)i * p.rows * HD);
+        const float* f = reinterpret_cast<const float*>(&v);
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] += wi > 0.f ? f[e] * wi : 0.f;      // what no piece has written may be anything
       }
-      p.out[(long long)t * p.ldo + (hk * p.G + g) * HD + d] = __float2bfloat16(l > 0.f ? o / l : 0.f);
     }
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    uint32_t u[E / 2];
+#pragma unroll
+    for (int e = 0; e < E; e += 2) u[e / 2] = pack_bf16x2(o[e] * inv, o[e + 1] * inv);
+    uint32_t* to = reinterpret_cast<uint32_t*>(p.out + t * p.ldo + h * HD + lane * E);
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) to[e] = u[e];
   }
 }
 
@@ -706,8 +738,8 @@ static int launch_paged(PagedAttn& p, const void* q, long long ldq, const void* 
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)min((long long)S.T * p.Hkv, 8ll * p.slots));
-  cfg.blockDim = dim3(p.G > 1 ? 256 : HD);
+  cfg.gridDim = dim3((unsigned)min(((long long)S.T * p.Hq + 7) / 8, 8ll * p.slots));
+  cfg.blockDim = dim3(256);
   cfg.stream = st;
   cfg.attrs = at;
   cfg.numAttrs = 1;

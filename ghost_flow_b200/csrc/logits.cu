@@ -10,10 +10,12 @@
 //   x = allowed ? x : -inf                                   all in 32 bits, rounded once
 //
 // One CTA has a slice of one row, which it reads and writes once, 16 bytes at a time. Which of its entries the row's tokens hold is a bit each in
-// shared memory; the entries whose bit is set have a counter each, in their order (an entry's counter is its rank among the set bits: those
-// of the words in front, counted once, and of its own word), so that there are no more of them than tokens and a slice may be long: a CTA reads
-// all tokens of its row, twice, whatever its slice is. Counters are whole numbers: the order of their atomics does not matter. The
-// first logits are on their way while the tokens are counted.
+// shared memory; an entry whose bit is set has a counter and a value, at its rank among the set bits (those of the words in front, counted
+// once, and of its own word), so that there are no more of them than tokens and a slice may be long: a CTA looks at all tokens of its
+// row, whatever its slice is. The penalties are worked out before the pass over the slice, a token to a thread; the pass itself only picks the
+// values up where a bit is set (with the arithmetic in the pass, whose warps nearly all meet a set bit, 512 rows of 50257 in fp32 took 95 us).
+// Counters are whole numbers, and a value is the same whichever of its tokens writes it: the order of the threads does not matter. The first
+// logits are on their way all the while.
 #include <cuda_fp16.h>
 
 #include "gf_host.h"
@@ -23,6 +25,7 @@ namespace gf {
 
 constexpr int LG_THREADS = 256;
 constexpr int LG_AHEAD = 4;      // vectors of a thread on their way together
+constexpr int LG_TOKENS = 8;     // tokens of a thread that it looks up once
 constexpr int LG_SLICE_MIN = 2048, LG_SLICE_MAX = 25600;
 
 struct LogitsParams {
@@ -65,6 +68,7 @@ __global__ void __launch_bounds__(LG_THREADS) logits_kernel(const __grid_constan
   unsigned* seen = shared;                         // [n_words]
   int* before = (int*)(shared + n_words);          // [n_words]: set bits of the words in front
   int* count = before + n_words;                   // [min(L, slice)]
+  float* value = (float*)(count + min(p.L, p.slice));
   const T* x = (const T*)p.x + row * p.ldx;
   T* y = (T*)p.y + row * p.ldy;
   // vector k has the entries from v0 - lead + k VEC on
@@ -84,28 +88,40 @@ __global__ void __launch_bounds__(LG_THREADS) logits_kernel(const __grid_constan
     }
   };
   load(threadIdx.x);
+  const float rep = p.repetition ? p.repetition[row] : p.repetition0, pres = p.presence ? p.presence[row] : p.presence0;
+  const float freq = p.frequency ? p.frequency[row] : p.frequency0;
   int n = 0;
   if (p.tokens) n = p.token_lens ? max(0, min(p.token_lens[row], p.L)) : p.L;
+  auto rank = [&](int v) { return before[v >> 5] + __popc(seen[v >> 5] & ((1u << (v & 31)) - 1)); };
   if (n > 0) {
     const int from = p.generated_from ? p.generated_from[row] : 0;
-    // f(entry of the slice, token) for the row's tokens in it
-    auto tokens = [&](auto f) {
-      for (int i0 = threadIdx.x; i0 < n; i0 += 4 * LG_THREADS) {
-        long long t[4];
+    // LG_TOKENS tokens of a thread from i0 on: their entries in the slice, -1 for one that is not in it
+    auto tokens = [&](int i0, int (&v)[LG_TOKENS]) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int i = i0 + j * LG_THREADS;
-          t[j] = i >= n ? -1ll : p.tokens64 ? ((const long long*)p.tokens)[row * p.ldt + i] : ((const int*)p.tokens)[row * p.ldt + i];
-        }
+      for (int j = 0; j < LG_TOKENS; ++j) {
+        const int i = i0 + j * LG_THREADS;
+        const long long t = i >= n ? -1ll : p.tokens64 ? ((const long long*)p.tokens)[row * p.ldt + i] : ((const int*)p.tokens)[row * p.ldt + i];
+        v[j] = t >= v0 && t < v1 ? (int)(t - v0) : -1;
+      }
+    };
+    int mine[LG_TOKENS];                           // the first of them, for every round
+    tokens(threadIdx.x, mine);
+    auto each = [&](auto f) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (t[j] >= v0 && t[j] < v1) f((int)(t[j] - v0), i0 + j * LG_THREADS);
+      for (int j = 0; j < LG_TOKENS; ++j)
+        if (mine[j] >= 0) f(mine[j], (int)threadIdx.x + j * LG_THREADS);
+      for (int i0 = threadIdx.x + LG_TOKENS * LG_THREADS; i0 < n; i0 += LG_TOKENS * LG_THREADS) {
+        int v[LG_TOKENS];
+        tokens(i0, v);
+#pragma unroll
+        for (int j = 0; j < LG_TOKENS; ++j)
+          if (v[j] >= 0) f(v[j], i0 + j * LG_THREADS);
       }
     };
     for (int i = threadIdx.x; i < n_words; i += LG_THREADS) seen[i] = 0;
-    for (int i = threadIdx.x; i < min(p.L, p.slice); i += LG_THREADS) count[i] = 0;
+    for (int i = threadIdx.x; i < min(n, p.slice); i += LG_THREADS) count[i] = 0;
     __syncthreads();
-    tokens([&](int v, int) { atomicOr(&seen[v >> 5], 1u << (v & 31)); });
+    each([&](int v, int) { atomicOr(&seen[v >> 5], 1u << (v & 31)); });
     __syncthreads();
     // ranks: a thread sums up the words that are its own, one behind the other, then the threads' sums
     const int per = (n_words + LG_THREADS - 1) / LG_THREADS, w0 = min(threadIdx.x * per, n_words), w1 = min(w0 + per, n_words);
@@ -128,20 +144,19 @@ __global__ void __launch_bounds__(LG_THREADS) logits_kernel(const __grid_constan
       at += __popc(seen[i]);
     }
     __syncthreads();
-    tokens([&](int v, int i) {
-      if (i >= from) atomicAdd(&count[before[v >> 5] + __popc(seen[v >> 5] & ((1u << (v & 31)) - 1))], 1);
+    each([&](int v, int i) {
+      if (i >= from) atomicAdd(&count[rank(v)], 1);
+    });
+    __syncthreads();
+    each([&](int v, int) {
+      const int r = rank(v), c = count[r];
+      const float a = to_f(x[v0 + v]);
+      value[r] = (a > 0.f ? a / rep : a * rep) - (c * freq + (c > 0 ? pres : 0.f));
     });
     __syncthreads();
   }
-  const float rep = p.repetition ? p.repetition[row] : p.repetition0, pres = p.presence ? p.presence[row] : p.presence0;
-  const float freq = p.frequency ? p.frequency[row] : p.frequency0;
   const float* bias = p.bias ? p.bias + row * p.ldb : nullptr;
   const unsigned* allowed = p.allowed ? p.allowed + row * p.lda : nullptr;
-  auto penalty = [&](float a, int l) {             // entry l of the slice, which the tokens hold
-    const int c = count[before[l >> 5] + __popc(seen[l >> 5] & ((1u << (l & 31)) - 1))];
-    a = a > 0.f ? a / rep : a * rep;
-    return a - (c * freq + (c > 0 ? pres : 0.f));
-  };
   for (int k0 = threadIdx.x; k0 < vectors; k0 += LG_AHEAD * LG_THREADS) {
     if (k0 != threadIdx.x) load(k0);
 #pragma unroll
@@ -158,7 +173,7 @@ __global__ void __launch_bounds__(LG_THREADS) logits_kernel(const __grid_constan
           if (hit) {
 #pragma unroll
             for (int j = 0; j < VEC; ++j)
-              if ((hit >> j) & 1) a[j] = penalty(a[j], e - v0 + j);
+              if ((hit >> j) & 1) a[j] = value[rank(e - v0 + j)];
           }
         }
         if (bias) {
@@ -187,7 +202,7 @@ __global__ void __launch_bounds__(LG_THREADS) logits_kernel(const __grid_constan
       } else {
         for (int v = max(e, v0); v < min(e + VEC, v1); ++v) {
           float a = to_f(x[v]);
-          if (n > 0 && ((seen[(v - v0) >> 5] >> ((v - v0) & 31)) & 1)) a = penalty(a, v - v0);
+          if (n > 0 && ((seen[(v - v0) >> 5] >> ((v - v0) & 31)) & 1)) a = value[rank(v - v0)];
           if (bias) a += bias[v];
           if (allowed && !((allowed[v >> 5] >> (v & 31)) & 1)) a = -INFINITY;
           from_f(y[v], a);
@@ -205,7 +220,7 @@ static int launch_logits(LogitsParams& p, long long B, cudaStream_t st) {
   p.slice = (int)(((p.V + slices - 1) / slices + 63) / 64 * 64);
   p.slices = (p.V + p.slice - 1) / p.slice;
   if (B * p.slices > 0x7fffffffll) return GFH_TOO_LARGE;
-  const size_t smem = p.tokens ? p.slice / 4 + 4ll * min(p.L, p.slice) : 0;
+  const size_t smem = p.tokens ? p.slice / 4 + 8ll * min(p.L, p.slice) : 0;
   static gf::DeviceMax granted;
   auto kern = logits_kernel<T>;
   if (smem > 48 * 1024 && granted.get() < smem) {
