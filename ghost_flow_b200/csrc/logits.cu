@@ -9,13 +9,11 @@
 //   x = x + bias[v]
 //   x = allowed ? x : -inf                                   all in 32 bits, rounded once
 //
-// One CTA has a slice of one row, which it reads and writes once, 16 bytes at a time. Which of its entries the row's tokens hold is a bit each in
-// shared memory; an entry whose bit is set has a counter and a value, at its rank among the set bits (those of the words in front, counted
-// once, and of its own word), so that there are no more of them than tokens and a slice may be long: a CTA looks at all tokens of its
-// row, whatever its slice is. The penalties are worked out before the pass over the slice, a token to a thread; the pass itself only picks the
-// values up where a bit is set (with the arithmetic in the pass, whose warps nearly all meet a set bit, 512 rows of 50257 in fp32 took 95 us).
-// Counters are whole numbers, and a value is the same whichever of its tokens writes it: the order of the threads does not matter. The first
-// logits are on their way all the while.
+// One CTA has a slice of one row. The row's tokens, each with a thread, set a bit for the entry that they hold and count themselves; then a pass
+// over the slice, 16 bytes at a time, does the arithmetic, whose first vectors were asked for before the tokens were looked at. An
+// entry's counter, later what is taken off it, lies at its rank among the set bits (those of the words in front, counted once, and of its own word):
+// there are no more of them than tokens, so that a slice may be long, and a CTA looks at all tokens of its row whatever its slice is; entries
+// of one vector have ranks one behind the other. Counters are whole numbers: the order of the threads does not matter.
 #include <cuda_fp16.h>
 
 #include "gf_host.h"
@@ -23,10 +21,11 @@
 
 namespace gf {
 
-constexpr int LG_THREADS = 256;
-constexpr int LG_AHEAD = 4;      // vectors of a thread on their way together
+constexpr int LG_THREADS = 512;
+constexpr int LG_CTAS = 3;       // on an SM
+constexpr int LG_STAGES = 4;     // vectors of a thread on their way together
 constexpr int LG_TOKENS = 8;     // tokens of a thread that it looks up once
-constexpr int LG_SLICE_MIN = 2048, LG_SLICE_MAX = 25600;
+constexpr int LG_SLICE_MIN = 4096, LG_SLICE_MAX = 25600;
 
 struct LogitsParams {
   const void* x;
@@ -51,61 +50,64 @@ __device__ __forceinline__ void from_f(float& y, float x) { y = x; }
 __device__ __forceinline__ void from_f(__nv_bfloat16& y, float x) { y = __float2bfloat16(x); }
 __device__ __forceinline__ void from_f(__half& y, float x) { y = __float2half(x); }
 
-// 32 bits from bit `at` on; `more`: whether the bits that are wanted go on into the next word
-__device__ __forceinline__ unsigned bits_at(const unsigned* words, int at, bool more) {
-  const int s = at & 31;
-  unsigned w = words[at >> 5] >> s;
-  if (more && s) w |= words[(at >> 5) + 1] << (32 - s);
-  return w;
-}
-
 template <typename T>
-__global__ void __launch_bounds__(LG_THREADS) logits_kernel(const __grid_constant__ LogitsParams p) {
+__global__ void __launch_bounds__(LG_THREADS, LG_CTAS) logits_kernel(const __grid_constant__ LogitsParams p) {
   constexpr int VEC = 16 / sizeof(T);
-  extern __shared__ unsigned shared[];
+  extern __shared__ __align__(16) unsigned shared[];
   __shared__ int warp_sum[LG_THREADS / 32];
-  const int row = blockIdx.x / p.slices, v0 = (blockIdx.x - row * p.slices) * p.slice, v1 = min(v0 + p.slice, p.V), n_words = p.slice / 32;
-  unsigned* seen = shared;                         // [n_words]
-  int* before = (int*)(shared + n_words);          // [n_words]: set bits of the words in front
-  int* count = before + n_words;                   // [min(L, slice)]
-  float* value = (float*)(count + min(p.L, p.slice));
-  const T* x = (const T*)p.x + row * p.ldx;
-  T* y = (T*)p.y + row * p.ldy;
-  // vector k has the entries from v0 - lead + k VEC on
-  const int lead = (int)((reinterpret_cast<uintptr_t>(x + v0) & 15) / sizeof(T));
-  const bool wide = (int)((reinterpret_cast<uintptr_t>(y + v0) & 15) / sizeof(T)) == lead;
-  const int vectors = (v1 - v0 + lead + VEC - 1) / VEC;
-  auto inside = [&](int k) {
-    const int e = v0 - lead + k * VEC;
-    return wide && e >= v0 && e + VEC <= v1;
+  const int row = blockIdx.x / p.slices, v0 = (blockIdx.x - row * p.slices) * p.slice, size = min(p.slice, p.V - v0), n_words = p.slice / 32;
+  uint4* ring = reinterpret_cast<uint4*>(shared);  // [LG_STAGES][LG_THREADS]: a thread reads what it asked for itself
+  unsigned* open = shared + 4 * LG_STAGES * LG_THREADS;          // [n_words]: allowed
+  uint2* seen = reinterpret_cast<uint2*>(open + n_words);        // [n_words]: bits, and set bits of the words in front
+  int* count = (int*)(seen + n_words);             // [min(L, slice)]
+  const T* x = (const T*)p.x + row * p.ldx + v0;   // entry 0 of the slice
+  T* y = (T*)p.y + row * p.ldy + v0;
+  // whole vectors: `vectors` from entry `head` on, on 16-byte boundaries of x and y; none where the two begin on different ones
+  const int head = min((int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) % 16 / sizeof(T)), size);
+  const int vectors = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(y)) & 15) ? 0 : (size - head) / VEC;
+  const T* xv = x + head + threadIdx.x * VEC;
+  const uint32_t slot = smem_u32(ring + threadIdx.x);
+  auto ask = [&](int k, int st) {                  // vector k of the slice; one group each, empty ones behind the last
+    if (k < vectors)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot + st * (LG_THREADS * 16)), "l"(xv + (k - (int)threadIdx.x) * VEC)
+                   : "memory");
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  uint4 in[LG_AHEAD];
-  auto load = [&](int k0) {
+  const float* bias = p.bias ? p.bias + row * p.ldb + v0 : nullptr;
+  auto begin = [&] {                               // what the pass needs first, on its way while the tokens are counted
 #pragma unroll
-    for (int i = 0; i < LG_AHEAD; ++i) {
-      const int k = k0 + i * LG_THREADS;
-      if (inside(k)) in[i] = *reinterpret_cast<const uint4*>(x + (v0 - lead + k * VEC));
-    }
+    for (int i = 0; i < LG_STAGES; ++i) ask(threadIdx.x + i * LG_THREADS, i);
+    if (p.allowed)
+      for (int i = threadIdx.x; i < (size + 31) / 32; i += LG_THREADS) open[i] = __ldg(p.allowed + row * p.lda + (v0 >> 5) + i);
   };
-  load(threadIdx.x);
-  const float rep = p.repetition ? p.repetition[row] : p.repetition0, pres = p.presence ? p.presence[row] : p.presence0;
-  const float freq = p.frequency ? p.frequency[row] : p.frequency0;
+  auto rank = [&](int v) {                         // of entry v if its bit is set, else of the next one whose is
+    const uint2 w = seen[v >> 5];
+    return (int)w.y + __popc(w.x & ~(0xffffffffu << (v & 31)));
+  };
   int n = 0;
-  if (p.tokens) n = p.token_lens ? max(0, min(p.token_lens[row], p.L)) : p.L;
-  auto rank = [&](int v) { return before[v >> 5] + __popc(seen[v >> 5] & ((1u << (v & 31)) - 1)); };
-  if (n > 0) {
+  const float rep = p.repetition ? p.repetition[row] : p.repetition0, less = 1.f / rep;
+  auto penalised = [&](float a, int r) { return (a > 0.f ? a * less : a * rep) - __int_as_float(count[r]); };
+  if (p.tokens) {
+    const float pres = p.presence ? p.presence[row] : p.presence0, freq = p.frequency ? p.frequency[row] : p.frequency0;
     const int from = p.generated_from ? p.generated_from[row] : 0;
-    // LG_TOKENS tokens of a thread from i0 on: their entries in the slice, -1 for one that is not in it
+    n = p.token_lens ? max(0, min(p.token_lens[row], p.L)) : p.L;
+    // LG_TOKENS tokens of a thread from i0 on: their entries, -1 for one that is not in the slice (or not there)
     auto tokens = [&](int i0, int (&v)[LG_TOKENS]) {
 #pragma unroll
       for (int j = 0; j < LG_TOKENS; ++j) {
         const int i = i0 + j * LG_THREADS;
-        const long long t = i >= n ? -1ll : p.tokens64 ? ((const long long*)p.tokens)[row * p.ldt + i] : ((const int*)p.tokens)[row * p.ldt + i];
-        v[j] = t >= v0 && t < v1 ? (int)(t - v0) : -1;
+        long long t = -1;
+        if (i < p.L) t = p.tokens64 ? ((const long long*)p.tokens)[row * p.ldt + i] : ((const int*)p.tokens)[row * p.ldt + i];
+        t -= v0;
+        v[j] = t >= 0 && t < size ? (int)t : -1;
       }
+#pragma unroll
+      for (int j = 0; j < LG_TOKENS; ++j)
+        if (i0 + j * LG_THREADS >= n) v[j] = -1;
     };
     int mine[LG_TOKENS];                           // the first of them, for every round
     tokens(threadIdx.x, mine);
+    begin();                                       // behind the tokens, which everything waits for
     auto each = [&](auto f) {
 #pragma unroll
       for (int j = 0; j < LG_TOKENS; ++j)
@@ -118,15 +120,14 @@ __global__ void __launch_bounds__(LG_THREADS) logits_kernel(const __grid_constan
           if (v[j] >= 0) f(v[j], i0 + j * LG_THREADS);
       }
     };
-    for (int i = threadIdx.x; i < n_words; i += LG_THREADS) seen[i] = 0;
-    for (int i = threadIdx.x; i < min(n, p.slice); i += LG_THREADS) count[i] = 0;
+    for (int i = threadIdx.x; i < n_words; i += LG_THREADS) seen[i].x = 0;
     __syncthreads();
-    each([&](int v, int) { atomicOr(&seen[v >> 5], 1u << (v & 31)); });
+    each([&](int v, int) { atomicOr(&seen[v >> 5].x, 1u << (v & 31)); });
     __syncthreads();
     // ranks: a thread sums up the words that are its own, one behind the other, then the threads' sums
     const int per = (n_words + LG_THREADS - 1) / LG_THREADS, w0 = min(threadIdx.x * per, n_words), w1 = min(w0 + per, n_words);
     int own = 0;
-    for (int i = w0; i < w1; ++i) own += __popc(seen[i]);
+    for (int i = w0; i < w1; ++i) own += __popc(seen[i].x);
     int incl = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -135,92 +136,119 @@ __global__ void __launch_bounds__(LG_THREADS) logits_kernel(const __grid_constan
     }
     if ((threadIdx.x & 31) == 31) warp_sum[threadIdx.x >> 5] = incl;
     __syncthreads();
-    int at = incl - own;
+    int at = incl - own, held = 0;                 // entries that the tokens hold
 #pragma unroll
-    for (int i = 0; i < LG_THREADS / 32; ++i)
+    for (int i = 0; i < LG_THREADS / 32; ++i) {
       if (i < (threadIdx.x >> 5)) at += warp_sum[i];
+      held += warp_sum[i];
+    }
+    for (int i = threadIdx.x; i < held; i += LG_THREADS) count[i] = 0;
     for (int i = w0; i < w1; ++i) {
-      before[i] = at;
-      at += __popc(seen[i]);
+      seen[i].y = at;
+      at += __popc(seen[i].x);
     }
     __syncthreads();
     each([&](int v, int i) {
       if (i >= from) atomicAdd(&count[rank(v)], 1);
     });
     __syncthreads();
-    each([&](int v, int) {
-      const int r = rank(v), c = count[r];
-      const float a = to_f(x[v0 + v]);
-      value[r] = (a > 0.f ? a / rep : a * rep) - (c * freq + (c > 0 ? pres : 0.f));
-    });
-    __syncthreads();
+    for (int i = threadIdx.x; i < held; i += LG_THREADS) {
+      const int c = count[i];
+      count[i] = __float_as_int(c * freq + (c > 0 ? pres : 0.f));
+    }
+  } else {
+    begin();
   }
-  const float* bias = p.bias ? p.bias + row * p.ldb : nullptr;
-  const unsigned* allowed = p.allowed ? p.allowed + row * p.lda : nullptr;
-  for (int k0 = threadIdx.x; k0 < vectors; k0 += LG_AHEAD * LG_THREADS) {
-    if (k0 != threadIdx.x) load(k0);
+  __syncthreads();                                 // `open` and what is taken off
+  // ---- the entries in front of the vectors and behind them, or all
+  const int behind = head + vectors * VEC;
+  for (int i = threadIdx.x; i < head + size - behind; i += LG_THREADS) {
+    const int v = i < head ? i : i - head + behind;
+    float a = to_f(x[v]);
+    if (n > 0 && ((seen[v >> 5].x >> (v & 31)) & 1)) a = penalised(a, rank(v));
+    if (bias) a += bias[v];
+    if (p.allowed && !((open[v >> 5] >> (v & 31)) & 1)) a = -INFINITY;
+    from_f(y[v], a);
+  }
+  // ---- the vectors
+  const float* bv = bias ? bias + head + threadIdx.x * VEC : nullptr;
+  const bool bias4 = (reinterpret_cast<uintptr_t>(bv) & 15) == 0;
+  float add[VEC];
+  auto bias_of = [&](int k) {                      // asked for a vector ahead
+    if (!bias || k >= vectors) return;
+    const float* from = bv + (k - (int)threadIdx.x) * VEC;
+    if (bias4) {
 #pragma unroll
-    for (int i = 0; i < LG_AHEAD; ++i) {
-      const int k = k0 + i * LG_THREADS, e = v0 - lead + k * VEC;
+      for (int j = 0; j < VEC; j += 4) {
+        const float4 u = __ldg(reinterpret_cast<const float4*>(from + j));
+        add[j] = u.x; add[j + 1] = u.y; add[j + 2] = u.z; add[j + 3] = u.w;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) add[j] = __ldg(from + j);
+    }
+  };
+  const bool apart = head % VEC != 0;              // the bits of a vector may go on into the next word
+  auto bits = [&](int l, auto word) {              // of the VEC entries from l on
+    unsigned w = word(l >> 5) >> (l & 31);
+    if (apart && (l & 31) + VEC > 32) w |= word((l >> 5) + 1) << (32 - (l & 31));
+    return w & ((1u << VEC) - 1);
+  };
+  bias_of(threadIdx.x);
+  T* to = y + head + threadIdx.x * VEC;
+  for (int k0 = threadIdx.x; k0 < vectors; k0 += LG_STAGES * LG_THREADS) {
+#pragma unroll
+    for (int st = 0; st < LG_STAGES; ++st) {
+      const int k = k0 + st * LG_THREADS;
       if (k >= vectors) break;
-      if (inside(k)) {
-        const T* have = reinterpret_cast<const T*>(&in[i]);
-        float a[VEC];
+      asm volatile("cp.async.wait_group %0;" ::"n"(LG_STAGES - 1) : "memory");
+      const uint4 in = ring[st * LG_THREADS + threadIdx.x];
+      const T* have = reinterpret_cast<const T*>(&in);
+      const int l = head + k * VEC;
+      float a[VEC];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) a[j] = to_f(have[j]);
-        if (n > 0) {
-          const unsigned hit = bits_at(seen, e - v0, ((e - v0) & 31) + VEC > 32) & ((1u << VEC) - 1);
-          if (hit) {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j)
-              if ((hit >> j) & 1) a[j] = value[rank(e - v0 + j)];
-          }
-        }
-        if (bias) {
-          if ((reinterpret_cast<uintptr_t>(bias + e) & 15) == 0) {
-#pragma unroll
-            for (int j = 0; j < VEC; j += 4) {
-              const float4 u = *reinterpret_cast<const float4*>(bias + e + j);
-              a[j] += u.x; a[j + 1] += u.y; a[j + 2] += u.z; a[j + 3] += u.w;
-            }
-          } else {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) a[j] += bias[e + j];
-          }
-        }
-        if (allowed) {
-          const unsigned ok = bits_at(allowed, e, (e & 31) + VEC > 32);
+      for (int j = 0; j < VEC; ++j) a[j] = to_f(have[j]);
+      if (n > 0) {
+        const unsigned hit = bits(l, [&](int w) { return seen[w].x; });
+        if (hit) {
+          int r = rank(l);
 #pragma unroll
           for (int j = 0; j < VEC; ++j)
-            if (!((ok >> j) & 1)) a[j] = -INFINITY;
-        }
-        uint4 u;
-        T* left = reinterpret_cast<T*>(&u);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) from_f(left[j], a[j]);
-        *reinterpret_cast<uint4*>(y + e) = u;
-      } else {
-        for (int v = max(e, v0); v < min(e + VEC, v1); ++v) {
-          float a = to_f(x[v]);
-          if (n > 0 && ((seen[(v - v0) >> 5] >> ((v - v0) & 31)) & 1)) a = value[rank(v - v0)];
-          if (bias) a += bias[v];
-          if (allowed && !((allowed[v >> 5] >> (v & 31)) & 1)) a = -INFINITY;
-          from_f(y[v], a);
+            if ((hit >> j) & 1) a[j] = penalised(a[j], r++);
         }
       }
+      if (bias) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) a[j] += add[j];
+        bias_of(k + LG_THREADS);
+      }
+      if (p.allowed) {
+        const unsigned ok = bits(l, [&](int w) { return open[w]; });
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          if (!((ok >> j) & 1)) a[j] = -INFINITY;
+      }
+      uint4 u;
+      T* left = reinterpret_cast<T*>(&u);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) from_f(left[j], a[j]);
+      *reinterpret_cast<uint4*>(to + (k - (int)threadIdx.x) * VEC) = u;
+      ask(k + LG_STAGES * LG_THREADS, st);
     }
   }
 }
 
-// A slice is as long as leaves about four CTAs to an SM, and at most LG_SLICE_MAX.
+// Rows are cut into as many slices as run at one time, of LG_SLICE_MIN entries or more; more rows than that into slices of at most LG_SLICE_MAX (a CTA
+// spends about half as long on its row's tokens as on such a slice: half as long ones took 62 us for 512 rows instead of 52, whole rows 61, because
+// a fourth round of CTAs then has little to do).
 template <typename T>
 static int launch_logits(LogitsParams& p, long long B, cudaStream_t st) {
-  const long long want = ((long long)p.V * B + 4 * sm_count() - 1) / (4 * sm_count());
-  long long slices = (p.V + max((long long)LG_SLICE_MIN, min(want, (long long)LG_SLICE_MAX)) - 1) / max((long long)LG_SLICE_MIN, min(want, (long long)LG_SLICE_MAX));
+  const long long most = (p.V + LG_SLICE_MIN - 1) / LG_SLICE_MIN, least = (p.V + LG_SLICE_MAX - 1) / LG_SLICE_MAX;
+  const long long slices = max(least, min(most, (long long)LG_CTAS * sm_count() / B));
   p.slice = (int)(((p.V + slices - 1) / slices + 63) / 64 * 64);
   p.slices = (p.V + p.slice - 1) / p.slice;
   if (B * p.slices > 0x7fffffffll) return GFH_TOO_LARGE;
-  const size_t smem = p.tokens ? p.slice / 4 + 8ll * min(p.L, p.slice) : 0;
+  const size_t smem = 16 * LG_STAGES * LG_THREADS + p.slice / 8 + (p.tokens ? p.slice / 4 + 4ll * min(p.L, p.slice) : 0);
   static gf::DeviceMax granted;
   auto kern = logits_kernel<T>;
   if (smem > 48 * 1024 && granted.get() < smem) {
