@@ -87,8 +87,35 @@ struct DecWork {
   __device__ __forceinline__ static int part_of(long long u, int n, int total) { return (int)(((u + 1) * n - 1) / total); }
 };
 
+struct DecParams {
+  DecWork work;
+  const __nv_bfloat16* q;       // [B, Hq * D], pitch ldq; with append: packed rows [Hq + 2 Hkv heads of D]
+  long long ldq;
+  __nv_bfloat16 *kc, *vc;       // [B, s_max, Hkv * D]
+  int Hq, G;                    // G = Hq / Hkv
+  float scale_log2;
+  float* part;                  // [slots][G heads][D sums, maximum, total]
+  __nv_bfloat16* out;
+  long long ldo;
+  // append (gf_llama_decode): the new token's k and v are row len - 1; q and k are rotated here with these rows of the tables
+  const float *cos_row, *sin_row;
+  int interleaved;
+  // pages (gf_paged_attn_one): kc and vc are pools, a block of 16 keys lies in one page. Strides of pages, rows and heads, in elements
+  PagedBatch pages;
+  long long kpage, krow, khead, vpage, vrow, vhead;
+};
+
+// Units of sequence b. In a paged batch with `cu`, one of other than one new token has none.
+template <bool PAGED>
+__device__ __forceinline__ int dec_units(const DecParams& p, int b) {
+  if (PAGED && p.pages.cu && p.pages.end(b) - p.pages.first(b) != 1) return 0;
+  return DecWork::units(p.work.len(b));
+}
+
 // Whole warp: units before sequence b, and those of all sequences in `total`.
-__device__ __forceinline__ int dec_units_before(const DecWork& w, int b, int& total) {
+template <bool PAGED>
+__device__ __forceinline__ int dec_units_before(const DecParams& p, int b, int& total) {
+  const DecWork& w = p.work;
   if (!w.lens) {
     const int n = DecWork::units(w.len_all);
     total = n * w.B;
@@ -97,7 +124,7 @@ __device__ __forceinline__ int dec_units_before(const DecWork& w, int b, int& to
   const int lane = threadIdx.x & 31;
   int before = 0, all = 0;
   for (int i = lane; i < w.B; i += 32) {
-    const int n = DecWork::units(w.len(i));
+    const int n = dec_units<PAGED>(p, i);
     all += n;
     if (i < b) before += n;
   }
@@ -108,18 +135,22 @@ __device__ __forceinline__ int dec_units_before(const DecWork& w, int b, int& to
 // A place in the order of the units of one KV head.
 struct DecAt {
   int b, blk, len, n;
-  __device__ __forceinline__ void next(const DecWork& w) {
+  template <bool PAGED>
+  __device__ __forceinline__ void next(const DecParams& p) {
     if (++blk < n) return;
     blk = 0;
-    if (++b < w.B) {
-      len = w.len(b);
-      n = DecWork::units(len);
+    while (++b < p.work.B) {
+      len = p.work.len(b);
+      n = dec_units<PAGED>(p, b);
+      if (!PAGED || n > 0) return;
     }
   }
 };
 
 // Whole warp: the place of unit u < total.
-__device__ __forceinline__ DecAt dec_find(const DecWork& w, int u) {
+template <bool PAGED>
+__device__ __forceinline__ DecAt dec_find(const DecParams& p, int u) {
+  const DecWork& w = p.work;
   DecAt at;
   if (!w.lens) {
     at.len = w.len_all;
@@ -130,7 +161,7 @@ __device__ __forceinline__ DecAt dec_find(const DecWork& w, int u) {
   }
   const int lane = threadIdx.x & 31;
   for (int base = 0, before = 0;; base += 32) {
-    const int n = base + lane < w.B ? DecWork::units(w.len(base + lane)) : 0;
+    const int n = base + lane < w.B ? dec_units<PAGED>(p, base + lane) : 0;
     int incl = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -149,24 +180,6 @@ __device__ __forceinline__ DecAt dec_find(const DecWork& w, int u) {
     before += __shfl_sync(0xffffffffu, incl, 31);
   }
 }
-
-struct DecParams {
-  DecWork work;
-  const __nv_bfloat16* q;       // [B, Hq * D], pitch ldq; with append: packed rows [Hq + 2 Hkv heads of D]
-  long long ldq;
-  __nv_bfloat16 *kc, *vc;       // [B, s_max, Hkv * D]
-  int Hq, G;                    // G = Hq / Hkv
-  float scale_log2;
-  float* part;                  // [slots][G heads][D sums, maximum, total]
-  __nv_bfloat16* out;
-  long long ldo;
-  // append (gf_llama_decode): the new token's k and v are row len - 1; q and k are rotated here with these rows of the tables
-  const float *cos_row, *sin_row;
-  int interleaved;
-  // pages (gf_paged_attn_one): kc and vc are pools, a block of 16 keys lies in one page. Strides of pages, rows and heads, in elements
-  PagedBatch pages;
-  long long kpage, krow, khead, vpage, vrow, vhead;
-};
 
 // Rotates packed pairs: lo holds dims d, d + 1 and hi their partners (half-split), or each word is a pair (interleaved); the
 // arithmetic and its rounding are the ones of rope_qkv_kernel.
@@ -212,25 +225,32 @@ attn_decode_kernel(const __grid_constant__ DecParams p) {
   int left_units;                  // of this CTA's part
   if constexpr (SHARES) {
     int total;
-    dec_units_before(w, 0, total);
-    const int parts = min(w.parts, total);                       // none is empty
+    dec_units_before<PAGED>(p, 0, total);
+    const int parts = PAGED ? max(1, min(w.parts, total)) : min(w.parts, total);    // none is empty
     const int u0 = (int)((long long)part * total / parts);
     left_units = part < parts ? (int)((long long)(part + 1) * total / parts) - u0 : 0;
-    if (left_units > 0) at = dec_find(w, u0);
+    if (left_units > 0) at = dec_find<PAGED>(p, u0);
   } else {
     at.b = part;
     if (w.splits > 1) at.b = part / w.splits;
     at.len = w.len(at.b);
-    at.n = left_units = DecWork::units(at.len);
+    at.n = left_units = dec_units<PAGED>(p, at.b);
     at.blk = 0;
-    if (w.splits > 1) {
+    if (w.splits > 1 && (!PAGED || at.n > 0)) {
       const unsigned sp = part - at.b * w.splits, splits = w.splits;             // sp n / splits in 32 bits: splits < 2^16
       const unsigned each = (unsigned)at.n / splits, rest = (unsigned)at.n - each * splits;
       at.blk = (int)(sp * each + sp * rest / splits);
       left_units = (int)((sp + 1) * each + (sp + 1) * rest / splits) - at.blk;
     }
   }
-  if (left_units <= 0) return;
+  // chained behind a kernel that this one does not depend on: the last CTA waits for it, so that whoever waits for this kernel has waited for both
+  auto behind = [&] {
+    if (PAGED && blockIdx.x == gridDim.x - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
+  };
+  if (left_units <= 0) {
+    behind();
+    return;
+  }
   const long long row_stride = (long long)w.Hkv * D, batch_stride = (long long)w.s_max * row_stride;
   const bool wide = ((reinterpret_cast<uintptr_t>(p.kc) | reinterpret_cast<uintptr_t>(p.vc)) & 15) == 0;   // rows are multiples of it
   const uint32_t my = smem_u32(ring) + warp * Cfg::WARP_BYTES;
@@ -290,7 +310,7 @@ attn_decode_kernel(const __grid_constant__ DecParams p) {
     --ahead_units;
     if constexpr (SHARES) {
       if (ahead_units > 0) {
-        ahead.next(w);
+        ahead.next<PAGED>(p);
         head = ahead.b * batch_stride + (long long)hk * D;
         if constexpr (PAGED) page_ahead = page_of(ahead, ahead.blk);
       }
@@ -315,7 +335,7 @@ attn_decode_kernel(const __grid_constant__ DecParams p) {
   auto begin = [&] {
     if (PAGED && threadIdx.x == 0 && hk == 0 && w.lens[at.b] != at.len) p.pages.bad();
     const unsigned short* qp = reinterpret_cast<const unsigned short*>(
-        p.q + at.b * p.ldq + (long long)(hk * G + min(r, G - 1)) * D + 2 * c);
+        p.q + (PAGED ? p.pages.first(at.b) : at.b) * p.ldq + (long long)(hk * G + min(r, G - 1)) * D + 2 * c);
 #pragma unroll
     for (int t = 0; t < D / 16; ++t) {
       qb[t][0] = r < G ? qp[16 * t] | ((uint32_t)qp[16 * t + 1] << 16) : 0u;
@@ -473,7 +493,7 @@ attn_decode_kernel(const __grid_constant__ DecParams p) {
     }
     __syncthreads();
     const int have = last ? DEC_WARPS : 1;
-    __nv_bfloat16* to = p.out + at.b * p.ldo + (long long)hk * G * D;
+    __nv_bfloat16* to = p.out + (PAGED ? p.pages.first(at.b) : at.b) * p.ldo + (long long)hk * G * D;
     float* slot = p.part + slot_of * G * (D + 2);
     for (int i = threadIdx.x; i < G * D; i += DEC_WARPS * 32) {
       const int g = i / D, d = i % D;
@@ -532,9 +552,10 @@ attn_decode_kernel(const __grid_constant__ DecParams p) {
         finish(left_units == 1, begins && ends, 2 * (long long)blockIdx.x + begins);
         __syncthreads();
       }
-      if (--left_units > 0) at.next(w);
+      if (--left_units > 0) at.next<PAGED>(p);
     }
   }
+  behind();
 }
 
 // One CTA of D threads for each query head: heads whose units all lay in one part are done, the others' pieces are added up,
@@ -548,14 +569,19 @@ __global__ void __launch_bounds__(D) attn_decode_merge_kernel(const __grid_const
   const float *first, *rest;                       // the first piece's sums, and where piece k > 0 is: rest + k * step
   long long step;
   int pieces;
-  const int n = DecWork::units(w.len(b));
+  const int n = dec_units<true>(p, b);
+  const long long at_row = p.pages.cu ? p.pages.first(b) : b;
+  if (n == 0) {                                    // not this kernel's; ends behind the ones in front all the same
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
   if (w.splits > 0) {
     pieces = min(n, w.splits);                     // with fewer units than parts some are empty
     step = w.Hkv * piece;
     first = rest = p.part + ((long long)b * w.splits * w.Hkv + hk) * piece + (long long)g * (D + 2);
   } else {
     int total;
-    const int s0 = dec_units_before(w, b, total), parts = min(w.parts, total);
+    const int s0 = dec_units_before<true>(p, b, total), parts = min(w.parts, total);
     const int c0 = DecWork::part_of(s0, parts, total), c1 = DecWork::part_of(s0 + n - 1, parts, total);
     pieces = c1 - c0 + 1;
     step = 2 * w.Hkv * piece;
@@ -588,7 +614,7 @@ __global__ void __launch_bounds__(D) attn_decode_merge_kernel(const __grid_const
       o += x[k] * e;
       t += l[k] * e;
     }
-    p.out[b * p.ldo + (long long)h * D + d] = __float2bfloat16(t > 0.f ? o / t : 0.f);
+    p.out[at_row * p.ldo + (long long)h * D + d] = __float2bfloat16(t > 0.f ? o / t : 0.f);
     return;
   }
   float mm = -INFINITY;
@@ -625,7 +651,7 @@ __global__ void __launch_bounds__(D) attn_decode_merge_kernel(const __grid_const
   l = 0.f;
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) l += share[i];
-  p.out[b * p.ldo + (long long)h * D + d] = __float2bfloat16(l > 0.f ? o / l : 0.f);
+  p.out[at_row * p.ldo + (long long)h * D + d] = __float2bfloat16(l > 0.f ? o / l : 0.f);
 }
 
 template <int D, int KIND>
@@ -695,26 +721,38 @@ GF_API int gf_attn_decode(const void* q, long long ldq, const void* kcache, cons
   return D == 128 ? launch_decode<128, DEC_SLICES>(p, 0, st) : launch_decode<64, DEC_SLICES>(p, 0, st);
 }
 
+namespace gf {
+
+bool attn_paged_one_ok(const PagedCall& c, int splits, const float* scratch) {
+  PagedBatch b;
+  return paged_batch(b, c) && c.H > 0 && c.Hk > 0 && c.H % c.Hk == 0 && c.H / c.Hk <= DEC_MAX_G && (c.D == 64 || c.D == 128) && splits != 0 &&
+         (scratch || splits == 1) && c.pages > 0;
+}
+
+int attn_paged_one(const PagedCall& c, float scale, int splits, float* scratch, int chained, cudaStream_t st) {
+  DecParams p{};
+  paged_batch(p.pages, c);
+  if (splits > 65535) splits = 65535;
+  const int D = (int)c.D;
+  p.work = {p.pages.lens, 0, (int)p.pages.capacity(), p.pages.B, (int)c.Hk, splits < 0 ? -splits : 0, splits > 0 ? splits : 0};
+  p.q = (const __nv_bfloat16*)c.x; p.ldq = c.ldx;
+  p.kc = (__nv_bfloat16*)c.kpages; p.vc = (__nv_bfloat16*)c.vpages;
+  p.Hq = (int)c.H; p.G = (int)(c.H / c.Hk);
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.part = scratch;
+  p.out = (__nv_bfloat16*)c.y; p.ldo = c.ldy;
+  p.kpage = c.strides[0]; p.krow = c.strides[1]; p.khead = c.strides[2];
+  p.vpage = c.strides[3]; p.vrow = c.strides[4]; p.vhead = c.strides[5];
+  if (splits < 0) return D == 128 ? launch_decode<128, DEC_PAGES_SHARES>(p, chained, st) : launch_decode<64, DEC_PAGES_SHARES>(p, chained, st);
+  return D == 128 ? launch_decode<128, DEC_PAGES>(p, chained, st) : launch_decode<64, DEC_PAGES>(p, chained, st);
+}
+
+}  // namespace gf
+
 // One new token of each sequence over pages (see paged.cuh): x [B, Hq, D] and y alike; splits and scratch as above, with at most
 // width * page keys. At most 8 query heads to a KV head.
 GF_API int gf_paged_attn_one(const PagedCall* c, float scale, int splits, float* scratch, void* stream) {
-  DecParams p{};
-  if (!c || c->cu || !paged_batch(p.pages, *c) || c->H <= 0 || c->Hk <= 0 || c->H % c->Hk || c->H / c->Hk > DEC_MAX_G ||
-      (c->D != 64 && c->D != 128) || splits == 0 || (!scratch && splits != 1) || c->pages == 0)
-    return GFH_BAD_ARG;
-  if (splits > 65535) splits = 65535;
+  if (!c || c->cu || !attn_paged_one_ok(*c, splits, scratch)) return GFH_BAD_ARG;
   gf::enter();
-  const int D = (int)c->D;
-  p.work = {p.pages.lens, 0, (int)p.pages.capacity(), p.pages.B, (int)c->Hk, splits < 0 ? -splits : 0, splits > 0 ? splits : 0};
-  p.q = (const __nv_bfloat16*)c->x; p.ldq = c->ldx;
-  p.kc = (__nv_bfloat16*)c->kpages; p.vc = (__nv_bfloat16*)c->vpages;
-  p.Hq = (int)c->H; p.G = (int)(c->H / c->Hk);
-  p.scale_log2 = scale * 1.4426950408889634f;
-  p.part = scratch;
-  p.out = (__nv_bfloat16*)c->y; p.ldo = c->ldy;
-  p.kpage = c->strides[0]; p.krow = c->strides[1]; p.khead = c->strides[2];
-  p.vpage = c->strides[3]; p.vrow = c->strides[4]; p.vhead = c->strides[5];
-  cudaStream_t st = (cudaStream_t)stream;
-  if (splits < 0) return D == 128 ? launch_decode<128, DEC_PAGES_SHARES>(p, 0, st) : launch_decode<64, DEC_PAGES_SHARES>(p, 0, st);
-  return D == 128 ? launch_decode<128, DEC_PAGES>(p, 0, st) : launch_decode<64, DEC_PAGES>(p, 0, st);
+  return attn_paged_one(*c, scale, splits, scratch, 0, (cudaStream_t)stream);
 }

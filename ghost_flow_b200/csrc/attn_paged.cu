@@ -33,6 +33,7 @@ struct PagedAttn {
   PagedBatch seqs;
   int Hq, Hkv, G, tq;            // G = Hq / Hkv, tq = 128 / G tokens of a tile
   int slots;                     // CTAs that run at a time; 0: no block is cut
+  int skip_ones;                 // sequences of one new token are not this kernel's
   float scale;
   __nv_bfloat16* out;            // [T, Hq, D], rows ldo apart
   long long ldo;
@@ -48,6 +49,7 @@ struct PgShape {                 // what a sequence is cut into
 __device__ __forceinline__ PgShape pg_shape(const PagedAttn& p, int b) {
   PgShape s;
   s.n = max(0, p.seqs.end(b) - p.seqs.first(b));
+  if (p.skip_ones && s.n == 1) s.n = 0;
   s.len = p.seqs.lens[b];
   s.keys = (int)min((long long)max(s.len, 0), p.seqs.capacity());
   s.blocks = (s.n + 2 * p.tq - 1) / (2 * p.tq);
@@ -56,39 +58,36 @@ __device__ __forceinline__ PgShape pg_shape(const PagedAttn& p, int b) {
 }
 
 // Whole warp: steps of a piece. All blocks uncut where they fill the machine; else the shortest pieces that run at one time, or, of cuts in 2, 3
-// and 4, the one whose waves of CTAs take the least (a piece costs about 3 steps of its own).
-__device__ __forceinline__ int paged_plan(const PagedAttn& p) {
+// and 4, the one whose waves of CTAs take the least (a piece costs about 3 steps of its own). `own`: the lane's sequence of the first 32.
+__device__ __forceinline__ int paged_plan(const PagedAttn& p, const PgShape& own) {
   constexpr int OWN = 3;
   if (p.slots == 0) return PG_WHOLE;
   const int lane = threadIdx.x & 31;
-  auto items = [&](int U) {
-    int n = 0;
-    for (int b = lane; b < p.seqs.B; b += 32) {
-      const PgShape s = pg_shape(p, b);
-      n += s.blocks * ((s.steps + U - 1) / U);
-    }
+  auto sum = [&](auto f) {
+    int n = f(own);
+    for (int b = lane + 32; b < p.seqs.B; b += 32) n += f(pg_shape(p, b));
     return __reduce_add_sync(0xffffffffu, n) * p.Hkv;
   };
-  int most = 0;
-  for (int b = lane; b < p.seqs.B; b += 32) {
+  auto items = [&](int U) { return sum([&](const PgShape& s) { return s.blocks * ((s.steps + U - 1) / U); }); };
+  const int whole = sum([](const PgShape& s) { return s.blocks; });
+  if (2 * whole <= p.slots) {
+    int U = max(1, (sum([](const PgShape& s) { return s.blocks * s.steps; }) + p.slots - 1) / p.slots);
+#pragma unroll 1
+    while (items(U) > p.slots) U += 1 + U / 16;    // ends: with whole blocks there are no more than half of them
+    return U;
+  }
+  int most = own.blocks > 0 ? own.steps : 0;
+  for (int b = lane + 32; b < p.seqs.B; b += 32) {
     const PgShape s = pg_shape(p, b);
-    if (s.n > 0) most = max(most, s.steps);
+    if (s.blocks > 0) most = max(most, s.steps);
   }
   most = __reduce_max_sync(0xffffffffu, most);
-  const int whole = items(PG_WHOLE);
-  if (2 * whole <= p.slots) {
-    int lo = 1, hi = max(1, most);                 // the least U with items(U) <= slots
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (items(mid) <= p.slots) hi = mid; else lo = mid + 1;
-    }
-    return lo;
-  }
   int best = PG_WHOLE, cost = (whole + p.slots - 1) / p.slots * (most + OWN);
-  for (int k = 2; k <= 4; ++k) {
+#pragma unroll 1
+  for (int k = 2; k <= 4 && most > 0; ++k) {
     const int U = (most + k - 1) / k, n = items(U);
     const int c = (n + p.slots - 1) / p.slots * (U + OWN);
-    if (U > 0 && n <= 2 * p.slots && c < cost) {
+    if (n <= 2 * p.slots && c < cost) {
       cost = c;
       best = U;
     }
@@ -98,7 +97,7 @@ __device__ __forceinline__ int paged_plan(const PagedAttn& p) {
 
 // A block of a sequence, and the keys of a piece of it.
 struct PgItem {
-  int b, hk, token, tokens, pos, keys, pieces, j0, j1;     // first token (row of q), how many, position of the first; steps j0 .. j1 - 1
+  int b, hk, token, tokens, pos, len, keys, pieces, j0, j1;     // first token (row of q), how many, position of the first; steps j0 .. j1 - 1
   __device__ __forceinline__ int visible(int upto) const {   // keys that the last of the first `upto` tokens sees
     return max(0, min(pos + min(upto, tokens), keys));
   }
@@ -109,21 +108,18 @@ __device__ __forceinline__ void pg_block(const PagedAttn& p, PgItem& it, const P
   it.token = p.seqs.first(b) + blk * 2 * p.tq;
   it.tokens = min(2 * p.tq, s.n - blk * 2 * p.tq);
   it.pos = s.len - s.n + blk * 2 * p.tq;
+  it.len = s.len;
   it.keys = s.keys;
 }
 
 // Whole warp: the item of a CTA; false behind the last. Inside a sequence the last block (the most keys) comes first, its heads and pieces
 // next to each other.
-__device__ __forceinline__ bool pg_find(const PagedAttn& p, int x, int U, PgItem& it) {
+__device__ __forceinline__ bool pg_find(const PagedAttn& p, const PgShape& own, int x, int U, PgItem& it) {
   const int lane = threadIdx.x & 31;
+#pragma unroll 1
   for (int base = 0, before = 0; base < p.seqs.B; base += 32) {
-    PgShape s{};
-    int pieces = 1, n = 0;
-    if (base + lane < p.seqs.B) {
-      s = pg_shape(p, base + lane);
-      pieces = (s.steps + U - 1) / U;
-      n = s.blocks * pieces * p.Hkv;
-    }
+    PgShape s = base == 0 ? own : base + lane < p.seqs.B ? pg_shape(p, base + lane) : PgShape{};
+    const int pieces = U == PG_WHOLE ? 1 : (s.steps + U - 1) / U, n = s.blocks * pieces * p.Hkv;
     int incl = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -207,74 +203,87 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  PgItem it{};
+  bool there = false, alternate, clears;
+  int n_j, tail, box;
+  auto derive = [&](const PgItem& o) {
+    alternate = o.tokens <= p.tq;
+    n_j = o.j1 - o.j0;
+    // the last step's V has rows behind the sequence inside a page
+    box = min(PG_TILE, 1 << p.seqs.page_shift);
+    tail = o.keys - (o.j1 - 1) * PG_TILE;                            // rows of the last step that are keys
+    clears = n_j > 0 && tail < PG_TILE && (tail & (box - 1)) != 0;
+  };
+  // A CTA of few steps is mostly this: the queries are on their way before the other warps have started. (Keys and values too was slower: the
+  // producer's code then stands twice, and the softmax warps spill.)
   if (warp == 0) {
-    const int U = paged_plan(p);
+    PgShape own{};
+    if (lane < p.seqs.B) own = pg_shape(p, lane);
+    if (lane == 0) {
+      mbar_init(q_full, 1);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&k_full[i], 1);
+        mbar_init(&k_empty[i], 1);
+        mbar_init(&v_full[i], 1);
+        mbar_init(&v_empty[i], 1);
+        mbar_init(&s_full[i], 1);
+        for (int c = 0; c < PG_PARTS; ++c) mbar_init(&p_full[i * PG_PARTS + c], 4);
+        mbar_init(&o_done[i], 1);
+      }
+      mbar_init(v_tail, 1);
+      mbar_fence_init();
+    }
+    const int U = paged_plan(p, own);
     if (p.plan && blockIdx.x == 0 && lane == 0) *p.plan = U;
-    PgItem it;
-    const bool there = pg_find(p, blockIdx.x, U, it);
+    there = pg_find(p, own, blockIdx.x, U, it);
     if (lane == 0) {
       shared_there = there;
       if (there) shared_item = it;
     }
-  } else if (threadIdx.x == 32) {
-    mbar_init(q_full, 1);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&k_full[i], 1);
-      mbar_init(&k_empty[i], 1);
-      mbar_init(&v_full[i], 1);
-      mbar_init(&v_empty[i], 1);
-      mbar_init(&s_full[i], 1);
-      for (int c = 0; c < PG_PARTS; ++c) mbar_init(&p_full[i * PG_PARTS + c], 4);
-      mbar_init(&o_done[i], 1);
+    if (there) {
+      derive(it);
+      if (lane == 0) {
+        const int qtiles = alternate ? 1 : 2;
+        mbar_expect_tx(q_full, qtiles * p.tq * p.G * HD * 2);
+        for (int t = 0; t < qtiles; ++t)
+#pragma unroll
+          for (int c = 0; c < Cfg::CH; ++c)
+            tma_load_3d(sQ + t * Cfg::TILE_BYTES + c * (PG_TILE * 128), &tmQ, q_full, c * 64, it.hk * p.G, it.token + t * p.tq);
+        if (it.keys != it.len) p.seqs.bad();
+      }
+      __syncwarp();
     }
-    mbar_init(v_tail, 1);
-    mbar_fence_init();
+  } else if (warp == 1) {
+    tmem_alloc(tmem_slot, Cfg::TMEM_COLS);
+    tmem_relinquish();
+  } else if (threadIdx.x == 64) {
     tma_prefetch_desc(&tmQ);
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
-  }
-  __syncthreads();
-  if (!shared_there) return;
-  const PgItem it = shared_item;
-  if (warp == 1) {
-    tmem_alloc(tmem_slot, Cfg::TMEM_COLS);
-    tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-
-  // steps of the piece, and of each tile: one behind the other over its own keys (two tiles of rows), or every other (one)
-  const bool alternate = it.tokens <= p.tq;
-  const int n_j = it.j1 - it.j0;
+  if (!shared_there) {
+    if (warp == 1) tmem_dealloc(tmem_base, Cfg::TMEM_COLS);
+    return;
+  }
+  const PgItem& item = shared_item;                // read where it is needed: the softmax warps have no registers to keep it in
+  if (warp != 0) derive(item);
+  // steps of each tile: one behind the other over its own keys (two tiles of rows), or every other (one)
   int cnt[2];
-  cnt[0] = alternate ? (n_j + 1) >> 1 : max(0, min(it.j1, it.steps(p.tq)) - it.j0);
+  cnt[0] = alternate ? (n_j + 1) >> 1 : max(0, min(item.j1, item.steps(p.tq)) - item.j0);
   cnt[1] = alternate ? n_j >> 1 : n_j;
-  // the last step's V has rows behind the sequence inside a page
-  const int box = min(PG_TILE, 1 << p.seqs.page_shift);
-  const int tail = it.keys - (it.j1 - 1) * PG_TILE;                  // rows of the last step that are keys
-  const bool clears = n_j > 0 && tail < PG_TILE && (tail & (box - 1)) != 0;
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PG_REGS_CTRL));
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA producer: a lane has one box of a step
-    const int qtiles = alternate ? 1 : 2, qbox = p.tq * p.G * HD * 2;
-    if (lane == 0) {
-      mbar_expect_tx(q_full, qtiles * qbox);
-      for (int t = 0; t < qtiles; ++t)
-#pragma unroll
-        for (int c = 0; c < Cfg::CH; ++c)
-          tma_load_3d(sQ + t * Cfg::TILE_BYTES + c * (PG_TILE * 128), &tmQ, q_full, c * 64, it.hk * p.G, it.token + t * p.tq);
-      if (it.keys != p.seqs.lens[it.b]) p.seqs.bad();
-    }
-    const int boxes = PG_TILE / box;
-    const int* table = p.seqs.table + (long long)it.b * p.seqs.ld;
     auto page_of = [&](int j) {
       const int key = j * PG_TILE + lane * box;
-      if (lane >= boxes || j >= it.j1 || key >= it.keys) return p.seqs.pages;           // zeros
-      const int page = table[key >> p.seqs.page_shift];
+      if (lane * box >= PG_TILE || j >= it.j1 || key >= it.keys) return p.seqs.pages;       // zeros
+      const int page = p.seqs.table[(long long)it.b * p.seqs.ld + (key >> p.seqs.page_shift)];
       if (page >= 0 && page < p.seqs.pages) return page;
       p.seqs.bad();
       return p.seqs.pages;
@@ -282,9 +291,9 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     auto boxes_to = [&](uint8_t* dst, const CUtensorMap* m, uint64_t* bar, int j, int page) {
       if (lane == 0) mbar_expect_tx(bar, Cfg::TILE_BYTES);
       __syncwarp();
-      if (lane < boxes) {
+      if (lane * box < PG_TILE) {
         const int y = (j * PG_TILE + lane * box) & ((1 << p.seqs.page_shift) - 1);
-#pragma unroll
+  #pragma unroll
         for (int c = 0; c < Cfg::CH; ++c)
           tma_load_4d(dst + c * (PG_TILE * 128) + lane * box * 128, m, bar, c * 64, y, it.hk, page);
       }
@@ -424,12 +433,12 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const int lane_grp = warp & 3;
     const int r = lane_grp * 32 + lane;
     const int tile_token = alternate ? 0 : t * p.tq;                   // first token of the tile in the block
-    const int tile_rows = max(0, min(p.tq, it.tokens - tile_token)) * p.G;
-    const int tok = tile_token + r / p.G, head = it.hk * p.G + r % p.G;
+    const int tile_rows = max(0, min(p.tq, item.tokens - tile_token)) * p.G;
+    const int tok = tile_token + r / p.G, head = item.hk * p.G + r % p.G;
     const bool mine = r < tile_rows;                                   // the row is a token's
     const bool idle = lane_grp * 32 >= tile_rows;                      // no row of the warp is
-    const int lim = mine ? min(it.pos + tok, it.keys - 1) : -1;        // last key that the row sees
-    const int tile_lim = min(it.pos + tile_token, it.keys - 1);        // ... that all of them see
+    const int lim = mine ? min(item.pos + tok, item.keys - 1) : -1;        // last key that the row sees
+    const int tile_lim = min(item.pos + tile_token, item.keys - 1);        // ... that all of them see
     const uint32_t tlane = (uint32_t)(lane_grp * 32) << 16;
     const uint32_t ts = tmem_base + Cfg::TM_S + t * 128 + tlane;
     const uint32_t to = tmem_base + Cfg::TM_O + t * 128 + tlane;
@@ -449,7 +458,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         continue;
       }
       tc_fence_after();
-      const int kv0 = (it.j0 + (alternate ? 2 * j + t : j)) * PG_TILE;
+      const int kv0 = (item.j0 + (alternate ? 2 * j + t : j)) * PG_TILE;
       const bool need_mask = kv0 + PG_TILE - 1 > tile_lim;
       // ---- row maximum, 64 scores at a time (the exponential pass reads them from tensor memory again)
       float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -546,7 +555,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       done(0);
       if (t == 1 && !idle) {
         tc_fence_after();
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < HD / 32; ++c) {
           uint32_t rr[32];
           tmem_ld32(to + c * 32, rr);
@@ -571,14 +580,15 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         l = l * a0 + ml[PG_TILE + r] * a1;
         m_ref = mm;
       }
-      const bool whole = it.pieces == 1;
+      const bool whole = item.pieces == 1;
       const float inv = !whole ? 1.f : l > 0.f ? 1.f / l : 0.f;
       a0 *= inv;
       a1 *= inv;
-      __nv_bfloat16* orow = p.out + (long long)(it.token + tok) * p.ldo + head * HD;
+      __nv_bfloat16* orow = p.out + (long long)(item.token + tok) * p.ldo + head * HD;
       const long long row = (long long)blockIdx.x * p.rows + (alternate ? r : t * PG_TILE + r);
       float* prow = p.part + row * HD;
-#pragma unroll
+      // rolled up: code that runs once is waited for
+#pragma unroll 1
       for (int c = 0; c < HD / 32; ++c) {
         uint32_t rr[32];
         tmem_ld32(to + c * 32, rr);
@@ -732,13 +742,16 @@ static int launch_paged(PagedAttn& p, const void* q, long long ldq, const void* 
   if (!rc) rc = pg_map(&tv, vp, 4, dims, vs, box);
   if (rc) return rc;
   kern<<<items, PG_THREADS, Cfg::SMEM_BYTES, st>>>(tq, tk, tv, p);
-  if (cudaGetLastError() != cudaSuccess) return GFH_CUDA;
-  if (p.slots == 0) return GFH_OK;
+  return cudaGetLastError() == cudaSuccess ? GFH_OK : GFH_CUDA;
+}
+
+template <int HD>
+static int launch_join(const PagedAttn& p, cudaStream_t st) {
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)min(((long long)S.T * p.Hq + 7) / 8, 8ll * p.slots));
+  cfg.gridDim = dim3((unsigned)min(((long long)p.seqs.T * p.Hq + 7) / 8, 8ll * p.slots));
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cfg.attrs = at;
@@ -759,7 +772,7 @@ static bool pg_call(PgCall& c, int B, int T, bool one_each, int Hq, int Hkv, int
   const long long items = blocks * Hkv;
   if (items > 0x7fffffffll) return false;
   c.slots = items < 2 * sms ? sms : 0;
-  c.items = c.slots ? 2 * sms : (int)items;
+  c.items = !c.slots ? (int)items : 2 * items <= sms ? sms : 2 * sms;
   c.rows = one_each || T <= PG_TILE / G ? PG_TILE : 2 * PG_TILE;       // blocks of one tile, or of two
   c.ws = c.slots ? 256 + 4ll * c.items * c.rows * (D + 2) : 0;
   return true;
@@ -781,12 +794,15 @@ GF_API long long gf_paged_attn_workspace(int B, int T, int one_each, int Hq, int
   return c.ws;
 }
 
-// x [T, Hq, D] and y alike; ws: as many bytes as gf_paged_attn_workspace says, on a 16-byte boundary. scale > 0.
-GF_API int gf_paged_attn(const PagedCall* c, float scale, void* ws, long long ws_bytes, void* stream) {
+// x [T, Hq, D] and y alike; ws: as many bytes as gf_paged_attn_workspace says, on a 16-byte boundary. scale > 0. ones != 0: sequences of one new
+// token go to the decode kernel, with that many splits and its scratch (see gf_paged_attn_one), while this one's CTAs run out. Each kernel is
+// launched while the one in front of it runs, and none ends before that one has.
+GF_API int gf_paged_attn(const PagedCall* c, float scale, void* ws, long long ws_bytes, int ones, float* ones_scratch, void* stream) {
   PagedAttn p{};
   if (!c || !paged_batch(p.seqs, *c) || c->pages == 0 || c->H > 0x7fffffff || c->Hk > 65535) return GFH_BAD_ARG;
   const int B = p.seqs.B, T = p.seqs.T, Hq = (int)c->H, Hkv = (int)c->Hk, D = (int)c->D;
   if (!paged_sizes(B, T, Hq, Hkv, D) || !(scale > 0.f) || (reinterpret_cast<uintptr_t>(ws) & 15)) return GFH_BAD_ARG;
+  if (ones && !attn_paged_one_ok(*c, ones, ones_scratch)) return GFH_BAD_ARG;
   gf::bind();
   PgCall n;
   if (!pg_call(n, B, T, !p.seqs.cu, Hq, Hkv, D, sm_count())) return GFH_TOO_LARGE;
@@ -794,6 +810,7 @@ GF_API int gf_paged_attn(const PagedCall* c, float scale, void* ws, long long ws
   gf::enter();
   p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.tq = PG_TILE / p.G;
   p.slots = n.slots; p.scale = scale; p.rows = n.rows; p.items = n.items;
+  p.skip_ones = ones != 0;
   p.out = (__nv_bfloat16*)c->y; p.ldo = c->ldy;
   if (n.slots) {
     p.plan = (int*)ws;
@@ -801,6 +818,12 @@ GF_API int gf_paged_attn(const PagedCall* c, float scale, void* ws, long long ws
     p.part_ml = p.part + (long long)n.items * n.rows * D;
   }
   cudaStream_t st = (cudaStream_t)stream;
-  return D == 128 ? launch_paged<128>(p, c->x, c->ldx, c->kpages, c->vpages, c->strides, n.items, st)
-                  : launch_paged<64>(p, c->x, c->ldx, c->kpages, c->vpages, c->strides, n.items, st);
+  int rc = D == 128 ? launch_paged<128>(p, c->x, c->ldx, c->kpages, c->vpages, c->strides, n.items, st)
+                    : launch_paged<64>(p, c->x, c->ldx, c->kpages, c->vpages, c->strides, n.items, st);
+  if (!rc && ones) {
+    note_extra_launches(1);
+    rc = attn_paged_one(*c, scale, ones, ones_scratch, 1, st);
+  }
+  if (!rc && n.slots) rc = D == 128 ? launch_join<128>(p, st) : launch_join<64>(p, st);
+  return rc;
 }

@@ -69,4 +69,9 @@ inline bool paged_batch(PagedBatch& s, const PagedCall& c) {
   return true;
 }
 
+// attn_decode.cu: one new token of each sequence of a call (with cu: of those that have one), as gf_paged_attn_one. `chained`: behind a
+// kernel of the same call that it does not depend on; it starts under it and ends behind it.
+bool attn_paged_one_ok(const PagedCall& c, int splits, const float* scratch);
+int attn_paged_one(const PagedCall& c, float scale, int splits, float* scratch, int chained, cudaStream_t st);
+
 }  // namespace gf

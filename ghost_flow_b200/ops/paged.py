@@ -197,6 +197,11 @@ def rope_qkv_to_pages(qkv, num_heads: int, num_kv_heads: int, cos, sin, kpages, 
 
 
 # ------------------------------------------------------------------------------------------ attention
+# A batch of this many sequences may be a server's, most of which have one new token: those then go to the decode kernel, which reads keys
+# twice as fast as the tiles for prompts do.
+_MANY = 8
+
+
 @functools.lru_cache(maxsize=4096)
 def _attention_workspace(device: int, B: int, T: int, one_each: bool, H: int, Hk: int, D: int) -> int:
     """Bytes that a call leaves the results of pieces in (the number of SMs decides whether keys are cut)."""
@@ -300,14 +305,19 @@ def paged_attention(q, kpages, vpages, page_table, lens, cu=None, scale: float |
         o, ldo = torch.empty_like(x) if ld == H * D else q.new_empty((T, H, D)), H * D
     call = _CALL(at, ld, o.data_ptr(), ldo, *pools, page_table.data_ptr(), page_table.stride(0), width, lens.data_ptr(),
                  0 if cu is None else cu.data_ptr(), B, T, H, Hk, D, page, P, _lib.status_ptr(device))
-    if one:
+    parts, few = 0, None
+    if one or (cu is not None and B >= _MANY and H // Hk <= 8):
         parts = _decode_parts(B, Hk, width * page, D, _sm_count(q.device), True)
-        ws = None if parts == 1 else torch.empty((B * parts if parts > 0 else -2 * parts) * H * (D + 2), dtype=torch.float32, device=q.device)
-        _rc(_lib.cuda_lib().gf_paged_attn_one(call, scale, parts, None if ws is None else ws.data_ptr(), stream), "gf_paged_attn_one")
+        if parts != 1:
+            few = torch.empty((B * parts if parts > 0 else -2 * parts) * H * (D + 2), dtype=torch.float32, device=q.device)
+    few_at = None if few is None else few.data_ptr()
+    if one:
+        _rc(_lib.cuda_lib().gf_paged_attn_one(call, scale, parts, few_at, stream), "gf_paged_attn_one")
     else:
         nbytes = _attention_workspace(device, B, T, cu is None, H, Hk, D)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-        _rc(_lib.cuda_lib().gf_paged_attn(call, scale, None if ws is None else ws.data_ptr(), nbytes, stream), "gf_paged_attn")
+        _rc(_lib.cuda_lib().gf_paged_attn(call, scale, None if ws is None else ws.data_ptr(), nbytes, parts, few_at, stream),
+            "gf_paged_attn")
     if out is not None:
         _increment_version(out)
     return o

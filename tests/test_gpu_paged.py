@@ -53,6 +53,25 @@ def test_attention_of_one_token_each(H, Hk, D, scale, kernel_status):
     oracle.close(_attend(s, cu=False, scale=scale), want, off)
 
 
+@pytest.mark.parametrize("parts", [1, 3, 16, -1, -5, -300])
+@pytest.mark.parametrize("H,Hk,D", [(4, 2, 64), (8, 1, 128)])
+def test_attention_of_some_with_one_token(parts, H, Hk, D, monkeypatch, kernel_status):
+    """Sequences of one token beside others, however their keys are cut; also where there is none of them, or nothing but them."""
+    from ghost_flow_b200.ops import paged
+
+    monkeypatch.setattr(paged, "_decode_parts", lambda *a: parts)
+    lens = [900, 40, 64, 0, 1, 200, 333, 70, 5, 1200]
+    for new in ([1, 40, 1, 1, 1, 2, 1, 33, 0, 1], [2, 40, 3, 2, 0, 2, 7, 33, 5, 0], [1] * 10, [0, 0, 0, 0, 0, 0, 0, 0, 1, 0]):
+        s = oracle.batch(lens, new, H, Hk, D, 16, device="cuda", behind=1)
+        want, off = oracle.attention(s)
+        out = torch.full_like(s["q"], 7.0)
+        for _ in range(2):
+            _attend(s, out=out)
+        n = sum(new)
+        oracle.close(out[:n], want[:n], off[:n])
+        assert (out[n:] == 7).all()
+
+
 @pytest.mark.parametrize("lens,new", [([9000], [1]), ([5000, 3], [1, 1]), ([4000, 700], [40, 300]), ([20000], [3])])
 @pytest.mark.parametrize("H,Hk,D", [(4, 1, 128), (4, 4, 64)])
 def test_attention_over_long_sequences(lens, new, H, Hk, D, kernel_status):
