@@ -112,7 +112,7 @@ __device__ __forceinline__ void pg_block(const PagedAttn& p, PgItem& it, const P
   it.keys = s.keys;
 }
 
-// Whole warp: the item of a CTA; false behind the last. Inside a sequence the last block (the most keys) comes first, its heads and pieces
+// Whole warp: item x; false behind the last one. Inside a sequence the last block (the most keys) comes first, its heads and pieces
 // next to each other.
 __device__ __forceinline__ bool pg_find(const PagedAttn& p, const PgShape& own, int x, int U, PgItem& it) {
   const int lane = threadIdx.x & 31;
@@ -141,7 +141,7 @@ __device__ __forceinline__ bool pg_find(const PagedAttn& p, const PgShape& own, 
       const int piece = in - it.hk * it.pieces, steps = it.steps(2 * p.tq);
       it.j0 = (int)((long long)steps * piece / it.pieces);
       it.j1 = (int)((long long)steps * (piece + 1) / it.pieces);
-      return true;
+      return it.pieces == 1 || x < p.items;                  // (the plan makes no more pieces than there is room for)
     }
     before += __shfl_sync(0xffffffffu, incl, 31);
   }
@@ -199,10 +199,14 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   uint64_t* p_full = bars + 14;   // [2][PG_PARTS]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 14 + 2 * PG_PARTS);
   __shared__ PgItem shared_item;
-  __shared__ int shared_there;
+  __shared__ int shared_there, shared_failed;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  auto fail = [&](int code) {                      // a wait that ran out
+    if (p.seqs.status) atomicCAS(p.seqs.status, 0, code);
+    shared_failed = 1;
+  };
   PgItem it{};
   bool there = false, alternate, clears;
   int n_j, tail, box;
@@ -232,6 +236,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       }
       mbar_init(v_tail, 1);
       mbar_fence_init();
+      shared_failed = 0;
     }
     const int U = paged_plan(p, own);
     if (p.plan && blockIdx.x == 0 && lane == 0) *p.plan = U;
@@ -305,12 +310,12 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       const uint32_t ph = (i >> 1) & 1;
       next = page_of(j + 1);
       if (!mbar_wait_warp(&k_empty[st], ph ^ 1)) {
-        if (p.seqs.status && lane == 0) atomicCAS(p.seqs.status, 0, GF_ERR_WAIT_EMPTY);
+        if (lane == 0) fail(GF_ERR_WAIT_EMPTY);
         break;
       }
       boxes_to(sK + st * Cfg::TILE_BYTES, &tmK, &k_full[st], j, page);
       if (!mbar_wait_warp(&v_empty[st], ph ^ 1)) {
-        if (p.seqs.status && lane == 0) atomicCAS(p.seqs.status, 0, GF_ERR_WAIT_EMPTY);
+        if (lane == 0) fail(GF_ERR_WAIT_EMPTY);
         break;
       }
       boxes_to(sV + st * Cfg::TILE_BYTES, &tmV, clears && i == n_j - 1 ? v_tail : &v_full[st], j, page);
@@ -325,7 +330,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const uint64_t dv0 = umma_desc_sw128(smem_u32(sV), PG_TILE * 128, 1024);
     constexpr uint64_t TILE_D = Cfg::TILE_BYTES >> 4;
     bool ok = mbar_wait_warp_tight(q_full, 0);
-    if (!ok && p.seqs.status && leader) atomicCAS(p.seqs.status, 0, GF_ERR_WAIT_FULL);
+    if (!ok && leader) fail(GF_ERR_WAIT_FULL);
     const uint64_t second = alternate ? 0 : TILE_D;        // Q of tile 1
     // S_t = Q_t K(stage)^T, announced on s_full[t]
     auto issue_qk = [&](int t, int st) {
@@ -343,7 +348,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 #pragma unroll
       for (int c = 0; c < PG_PARTS; ++c) {
         if (ok && !mbar_wait_warp_tight(&p_full[t * PG_PARTS + c], n & 1)) {
-          if (p.seqs.status && leader) atomicCAS(p.seqs.status, 0, GF_ERR_WAIT_SOFTMAX);
+          if (leader) fail(GF_ERR_WAIT_SOFTMAX);
           ok = false;
         }
         if (ok) {
@@ -358,7 +363,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     };
     auto full = [&](uint64_t* bar, int i) {
       if (ok && !mbar_wait_warp_tight(&bar[i & 1], (i >> 1) & 1)) {
-        if (p.seqs.status && leader) atomicCAS(p.seqs.status, 0, GF_ERR_WAIT_FULL);
+        if (leader) fail(GF_ERR_WAIT_FULL);
         ok = false;
       }
     };
@@ -414,7 +419,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   } else if (warp == 2 && clears) {
     // ---------------------------------------------------------------- rows of the last V behind the sequence: zeros
     if (!mbar_wait_warp(v_tail, 0)) {
-      if (p.seqs.status && lane == 0) atomicCAS(p.seqs.status, 0, GF_ERR_WAIT_FULL);
+      if (lane == 0) fail(GF_ERR_WAIT_FULL);
     } else {
       const int st = (n_j - 1) & 1, end = (tail + box - 1) & ~(box - 1);       // what lies behind `end` came as zeros
       for (int c = 0; c < Cfg::CH; ++c) {
@@ -448,7 +453,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const int my_n = t ? cnt[1] : cnt[0];
     for (int j = 0; j < my_n && ok; ++j) {
       if (!mbar_wait_warp_tight(&s_full[t], j & 1)) {
-        if (p.seqs.status) atomicCAS(p.seqs.status, 0, GF_ERR_WAIT_TMEM_FULL);
+        fail(GF_ERR_WAIT_TMEM_FULL);
         ok = false;
         break;
       }
@@ -543,7 +548,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     // ---- end: all products into O have been done
     auto done = [&](int tile) {
       if (ok && (tile ? cnt[1] : cnt[0]) > 0 && !mbar_wait_warp_tight(&o_done[tile], 0)) {
-        if (p.seqs.status) atomicCAS(p.seqs.status, 0, GF_ERR_WAIT_TMEM_FULL);
+        fail(GF_ERR_WAIT_TMEM_FULL);
         ok = false;
       }
     };
@@ -618,9 +623,9 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     }
   }
 
-  if (p.seqs.status && *reinterpret_cast<volatile int*>(p.seqs.status) != 0) error_drain_pause();
   tc_fence_before();
   __syncthreads();
+  if (shared_failed) error_drain_pause();
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
@@ -772,7 +777,7 @@ static bool pg_call(PgCall& c, int B, int T, bool one_each, int Hq, int Hkv, int
   const long long items = blocks * Hkv;
   if (items > 0x7fffffffll) return false;
   c.slots = items < 2 * sms ? sms : 0;
-  c.items = !c.slots ? (int)items : 2 * items <= sms ? sms : 2 * sms;
+  c.items = c.slots ? 2 * sms : (int)items;
   c.rows = one_each || T <= PG_TILE / G ? PG_TILE : 2 * PG_TILE;       // blocks of one tile, or of two
   c.ws = c.slots ? 256 + 4ll * c.items * c.rows * (D + 2) : 0;
   return true;
