@@ -725,8 +725,9 @@ namespace gf {
 
 bool attn_paged_one_ok(const PagedCall& c, int splits, const float* scratch) {
   PagedBatch b;
-  return paged_batch(b, c) && c.H > 0 && c.Hk > 0 && c.H % c.Hk == 0 && c.H / c.Hk <= DEC_MAX_G && (c.D == 64 || c.D == 128) && splits != 0 &&
-         (scratch || splits == 1) && c.pages > 0;
+  const long long parts = splits > 0 ? c.B * min(splits, 65535) : -(long long)splits;
+  return paged_batch(b, c) && c.H > 0 && c.Hk > 0 && c.H <= 65535 && parts * c.Hk <= 0x7fffffff && c.H % c.Hk == 0 && c.H / c.Hk <= DEC_MAX_G &&
+         (c.D == 64 || c.D == 128) && splits != 0 && (scratch || splits == 1) && c.pages > 0;
 }
 
 int attn_paged_one(const PagedCall& c, float scale, int splits, float* scratch, int chained, cudaStream_t st) {

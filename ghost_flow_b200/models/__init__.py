@@ -2,6 +2,7 @@
 from .configs import BertConfig, GPTConfig, LLaMAConfig, MixtralConfig, T5Config, ViTConfig  # noqa: F401
 from .gpt import GPTForCausalLM, GPTForSequenceClassification, GPTModel  # noqa: F401
 from .llama import LLaMAForCausalLM, LLaMAModel  # noqa: F401
+from .paged import PagedBatch, PagedKVCache  # noqa: F401
 from .encoders import (  # noqa: F401
     BertForMaskedLM, BertForSequenceClassification, BertForTokenClassification, BertModel, BertOutput,
     MixtralForCausalLM, PatchEmbedding, T5ForConditionalGeneration, T5Embeddings, T5ForSequenceClassification, T5Model, T5Output,

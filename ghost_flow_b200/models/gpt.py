@@ -138,7 +138,8 @@ class GPTForCausalLM(Module):
         return ops.cross_entropy(logits.view(-1, logits.shape[-1]), labels.reshape(-1)), logits
 
     @torch.no_grad()
-    def generate(self, ids, max_new_tokens: int, temperature: float = 0.0):
+    def generate(self, ids, max_new_tokens: int, temperature: float = 0.0, **choice):
+        """``choice``: penalties, bias and mask of :func:`~ghost_flow_b200.ops.sampling.next_tokens`."""
         was_training = self.training
         self.eval()
         t = self.transformer
@@ -151,10 +152,7 @@ class GPTForCausalLM(Module):
         out = [ids]
         pos = ids.shape[1]
         for _ in range(max_new_tokens):
-            if temperature and temperature > 0:
-                nxt = torch.multinomial(torch.softmax(logits.float() / temperature, -1), 1)
-            else:
-                nxt = logits.argmax(-1, keepdim=True)
+            nxt = ops.next_tokens(logits, temperature, torch.cat(out, 1) if choice else None, prompt=ids.shape[1], **choice)
             out.append(nxt)
             if pos >= self.cfg.n_positions:
                 break

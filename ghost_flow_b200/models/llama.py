@@ -16,6 +16,7 @@ from ..ops import raw
 from ..nn.layers import Embedding, Linear, RMSNorm, SwiGLU
 from ..nn.module import Module, ModuleList, plain_modules
 from .configs import LLaMAConfig
+from .paged import PagedKVCache
 
 
 class LLaMAAttention(Module):
@@ -63,6 +64,15 @@ class LLaMAAttention(Module):
             q, k, v = ops.rope_qkv(qkv, H, Hk, cos, sin, c.rope_interleaved, start_pos)
             o = ops.flash_attention(q, k, v, causal=True)
         return self.wo(o.reshape(B, S, H * D), residual)
+
+    def forward_pages(self, x, cos, sin, pools, batch, residual=None):
+        """New tokens ``[T, hidden]`` of the sequences of a :class:`~.paged.PagedBatch`, whose keys are in this layer's ``pools``."""
+        c = self.cfg
+        H, Hk, D = c.num_attention_heads, c.num_key_value_heads, c.head_dim
+        qkv = self.wqkv(x).view(x.shape[0], H + 2 * Hk, D)
+        q = ops.rope_qkv_to_pages(qkv, H, Hk, cos, sin, *pools, batch.table, batch.lens, batch.cu, c.rope_interleaved)
+        o = ops.paged_attention(q, *pools, batch.table, batch.lens, batch.cu)
+        return self.wo(o.reshape(x.shape[0], H * D), residual)
 
 
 def _weight(module):
@@ -124,6 +134,10 @@ class LLaMADecoderLayer(Module):
         x = self.attn(self.attn_norm(x), cos, sin, residual=x, cache=cache, start_pos=start_pos)
         return self.mlp(self.ffn_norm(x), residual=x)
 
+    def forward_pages(self, x, cos, sin, pools, batch):
+        x = self.attn.forward_pages(self.attn_norm(x), cos, sin, pools, batch, residual=x)
+        return self.mlp(self.ffn_norm(x), residual=x)
+
 
 class LLaMAModel(Module):
     def __init__(self, cfg: LLaMAConfig, device=None, dtype=None):
@@ -150,6 +164,16 @@ class LLaMAModel(Module):
 
     def forward(self, ids, caches=None, start_pos: int = 0):
         return self.norm(self._before_norm(ids, caches, start_pos))
+
+    def forward_pages(self, ids, cache, batch, rows=None):
+        """Hidden states of the new tokens ``ids [T]`` of a batch over a :class:`~.paged.PagedKVCache`, or of those in ``rows`` (indices)."""
+        cos, sin = self.rope(batch.longest, ids.device)
+        x = self.embed_tokens(ids)
+        for layer, pools in zip(self.layers, cache.pools):
+            x = layer.forward_pages(x, cos, sin, pools, batch)
+        if rows is not None:
+            x = x[rows]
+        return self.norm(x) if x.shape[0] else x
 
 
 class LLaMAForCausalLM(Module):
@@ -202,6 +226,18 @@ class LLaMAForCausalLM(Module):
             return logits
         return ops.cross_entropy(logits.view(-1, logits.shape[-1]), labels.reshape(-1)), logits
 
+    @torch.no_grad()
+    def forward_pages(self, ids, cache, batch, rows=None):
+        """Logits ``[T, vocab]`` of new tokens ``ids [T]`` of the sequences of ``batch``, one behind the other, over a
+        :class:`~.paged.PagedKVCache`, or of those in ``rows``. Inference only."""
+        h = self.model.forward_pages(ids, cache, batch, rows)
+        return self.lm_head(h) if h.shape[0] else h.new_empty(0, self.lm_head.weight.shape[0])
+
+    def new_paged_cache(self, num_pages: int, page_size: int = 64, device=None, dtype=None):
+        c, p = self.cfg, next(self.parameters())
+        return PagedKVCache(c.num_hidden_layers, num_pages, page_size, c.num_key_value_heads, c.head_dim, device or p.device,
+                            dtype or p.dtype)
+
     def new_caches(self, batch: int, max_len: int, device=None, dtype=None):
         c = self.cfg
         p = next(self.parameters())
@@ -211,22 +247,73 @@ class LLaMAForCausalLM(Module):
                 for _ in range(c.num_hidden_layers)]
 
     @torch.no_grad()
-    def generate(self, ids, max_new_tokens: int, temperature: float = 0.0):
-        """Greedy (temperature 0) or sampled continuation with a KV cache."""
+    def generate(self, ids, max_new_tokens: int, temperature: float = 0.0, **choice):
+        """Greedy (temperature 0) or sampled continuation with a KV cache. ``choice``: penalties, bias and mask of
+        :func:`~ghost_flow_b200.ops.sampling.next_tokens`."""
         B, S = ids.shape
         caches = self.new_caches(B, S + max_new_tokens)
         logits = self.forward(ids, caches=caches, start_pos=0)[:, -1]
         out = [ids]
         pos = S
         for _ in range(max_new_tokens):
-            if temperature and temperature > 0:
-                nxt = torch.multinomial(torch.softmax(logits.float() / temperature, -1), 1)
-            else:
-                nxt = logits.argmax(-1, keepdim=True)
+            nxt = ops.next_tokens(logits, temperature, torch.cat(out, 1) if choice else None, prompt=S, **choice)
             out.append(nxt)
             logits = self.forward(nxt, caches=caches, start_pos=pos)[:, -1]
             pos += 1
         return torch.cat(out, dim=1)
+
+    @torch.no_grad()
+    def generate_batch(self, prompts, max_new_tokens: int, temperature: float = 0.0, page_size: int = 64, chunk_tokens: int = 4096,
+                       **choice):
+        """Continuations of prompts (1-D token tensors) of any lengths in one batch over a paged cache; a list of prompts with their
+        ``max_new_tokens`` new tokens. Prompts go through the model at most ``chunk_tokens`` tokens at a time. ``choice`` as for
+        :meth:`generate`."""
+        p = next(self.parameters())
+        prompts = [t.to(p.device).long().reshape(-1) for t in prompts]
+        if not prompts or max_new_tokens <= 0:
+            return prompts
+        if any(t.numel() == 0 for t in prompts) or chunk_tokens < 1:
+            raise ValueError("generate_batch continues prompts of one token or more, in chunks of one or more")
+        B, lens = len(prompts), [t.numel() for t in prompts]
+        cache = self.new_paged_cache(sum(-(-(n + max_new_tokens) // page_size) for n in lens), page_size)
+        for b, n in enumerate(lens):
+            cache.reserve(b, n + max_new_tokens)
+        # the prompts, in chunks: logits are wanted of their last tokens only
+        done, logits = [0] * B, [None] * B
+        while done != lens:
+            room, take = chunk_tokens, {}
+            for b in range(B):
+                n = min(room, lens[b] - done[b])
+                if n > 0:
+                    take[b] = n
+                    room -= n
+            batch = cache.batch(take, [done[b] + n for b, n in take.items()], take.values())
+            ids = torch.cat([prompts[b][done[b]:done[b] + n] for b, n in take.items()])
+            ends, at = {}, 0
+            for b, n in take.items():
+                at += n
+                done[b] += n
+                if done[b] == lens[b]:
+                    ends[b] = at - 1
+            out = self.forward_pages(ids, cache, batch, torch.tensor(list(ends.values()), dtype=torch.long, device=p.device))
+            for row, b in zip(out, ends):
+                logits[b] = row
+        logits = torch.stack(logits)
+        # then all sequences, token by token; what is appended is told to the device by the lengths it holds
+        tokens = torch.zeros(B, max(lens) + max_new_tokens, dtype=torch.long, device=p.device)
+        for b, t in enumerate(prompts):
+            tokens[b, :lens[b]] = t
+        count = torch.tensor(lens, dtype=torch.int32, device=p.device)
+        first = count.clone()
+        batch = cache.batch(range(B), [n + 1 for n in lens])
+        for i in range(max_new_tokens):
+            nxt = ops.next_tokens(logits, temperature, tokens if choice else None, count, first, **choice)
+            tokens.scatter_(1, count.long()[:, None], nxt)
+            count += 1
+            if i + 1 < max_new_tokens:
+                logits = self.forward_pages(nxt.view(-1), cache, batch)
+                batch.advance()
+        return [tokens[b, :n + max_new_tokens] for b, n in enumerate(lens)]
 
     # names used by the ZeRO engine's state_dict
     def load_engine_state(self, sd: dict):

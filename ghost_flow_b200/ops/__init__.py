@@ -6,4 +6,4 @@ from .fused import (  # noqa: F401
     cross_entropy, decode_cache_ok, embedding_rows, flash_attention, attention_ref, split_qkv, observed, gpt_block, gpt_block_ok,
 )
 from .paged import paged_attention, rope_qkv_to_pages  # noqa: F401
-from .sampling import pack_allowed, process_logits  # noqa: F401
+from .sampling import next_tokens, pack_allowed, process_logits  # noqa: F401

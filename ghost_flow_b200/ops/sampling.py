@@ -175,3 +175,18 @@ def process_logits(logits, tokens=None, token_lens=None, generated_from=None, re
     if out is not None:
         torch.autograd.graph.increment_version(out)
     return y
+
+
+def next_tokens(logits, temperature: float = 0.0, tokens=None, token_lens=None, generated_from=None, prompt: int | None = None,
+                repetition=1.0, presence=0.0, frequency=0.0, bias=None, allowed=None):
+    """The next token ``[B, 1]`` of every row of ``logits [B, V]``: the likeliest (temperature 0) or a sampled one, after
+    :func:`process_logits` where ``tokens``, a bias or a mask are given. ``prompt``: the number of tokens of every row that are its prompt,
+    in place of ``generated_from``."""
+    if tokens is not None or bias is not None or allowed is not None:
+        if tokens is not None and generated_from is None and prompt is not None:
+            generated_from = torch.full((logits.shape[0],), prompt, dtype=torch.int32, device=logits.device)
+        logits = process_logits(logits, tokens, token_lens if tokens is not None else None, generated_from if tokens is not None else None,
+                                repetition, presence, frequency, bias, allowed)
+    if temperature and temperature > 0:
+        return torch.multinomial(torch.softmax(logits.float() / temperature, -1), 1)
+    return logits.argmax(-1, keepdim=True)

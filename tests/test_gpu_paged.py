@@ -9,7 +9,9 @@ pytestmark = pytest.mark.gpu
 BATCHES = {"one": ([1], [1]), "two keys": ([2], [1]), "one each": ([1, 63, 64, 65, 128, 129, 300], [1] * 7),
            "empty slots": ([0, 17, 0, 130], [1, 1, 0, 1]), "prompt": ([130], [130]), "prompts": ([5, 128, 257, 31], [5, 128, 257, 31]),
            "chunk": ([385], [100]), "chunk behind a page": ([272], [16]), "mixed": ([300, 1, 77, 400, 0, 200], [1, 1, 30, 129, 0, 1]),
-           "fewer keys than tokens": ([3, 20, 0], [9, 4, 2]), "more than 32 sequences": ([*range(1, 40)], [1 + b % 3 for b in range(39)])}
+           "fewer keys than tokens": ([3, 20, 0], [9, 4, 2]),
+           "server": ([300, 700, 1, 64, 0, 129, 500, 17, 90, 0, 33, 250], [120, 1, 1, 1, 1, 1, 300, 1, 2, 0, 1, 1]),
+           "nobody has one token": ([30, 40, 50, 60, 70, 80, 90, 200], [2, 3, 0, 60, 5, 2, 90, 7]), "more than 32 sequences": ([*range(1, 40)], [1 + b % 3 for b in range(39)])}
 HEADS = [(1, 1, 64), (4, 2, 64), (6, 2, 128), (5, 1, 128), (8, 1, 64), (16, 1, 128), (12, 12, 64), (3, 1, 128)]
 
 
@@ -123,7 +125,7 @@ def test_append(name, H, Hk, D, layout, interleaved, kernel_status):
 
     lens, new = BATCHES[name]
     s = oracle.batch(lens, new, H, Hk, D, 16 if D == 64 else 32, device="cuda", layout=layout, behind=2)
-    cos, sin = ops.rope_tables(512, D, 1e4, "cuda")
+    cos, sin = ops.rope_tables(1024, D, 1e4, "cuda")
     q, qo, k, ko, v = oracle.append(s, H, Hk, cos, sin, interleaved)
     with torch.no_grad():
         got = ops.rope_qkv_to_pages(s["qkv"], H, Hk, cos, sin, s["kp"], s["vp"], s["table"], s["lens"], s["cu"], interleaved)
@@ -265,3 +267,60 @@ def test_writes_are_visible_to_autograd_and_to_dispatch_modes():
     with torch.no_grad(), Mode():
         got = ops.paged_attention(s["q"], kp, vp, *args)
     assert "aten::_softmax" in seen and (got.float() - want.float()).abs().max() < 2 ** -4
+
+
+@pytest.mark.parametrize("which", ["append", "one each", "chunk", "prompts", "server", "logits"])
+def test_count_is_the_kernels_of_a_call(which, kernel_status):
+    from ghost_flow_b200 import ops
+    from ghost_flow_b200.ops import _lib
+    from test_gpu_launch_count import _kernels
+
+    lens, new = {"one each": ([3000, 5], [1, 1]), "chunk": ([2000], [33]), "prompts": ([4100] * 2, [4100] * 2),
+                 "server": BATCHES["server"]}.get(which, ([20, 30], [3, 1]))
+    H, Hk = (32, 8) if which == "prompts" else (8, 2)
+    s = oracle.batch(lens, new, H, Hk, 128, 64, device="cuda")
+    cos, sin = ops.rope_tables(64, 128, 1e4, "cuda")
+    x = torch.randn(4, 100, device="cuda")
+    f = {"append": lambda: ops.rope_qkv_to_pages(s["qkv"], 8, 2, cos, sin, s["kp"], s["vp"], s["table"], s["lens"], s["cu"]),
+         "logits": lambda: ops.process_logits(x, repetition=1.5)}.get(which, lambda: _attend(s, cu=which != "one each"))
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.no_grad():
+        f()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            n = _lib.launch_count()
+            f()
+            n = _lib.launch_count() - n
+    assert n == _kernels(graph) > 0
+
+
+def test_tensors_on_another_stream_and_calls_from_two_threads(kernel_status):
+    import threading
+
+    batches = [oracle.batch([700, 40, 300], [1, 33, 129], 8, 2, 64, 16, device="cuda", seed=i) for i in range(4)]
+    want = [_attend(s) for s in batches]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                if not torch.equal(_attend(batches[i]), want[i]):
+                    wrong.append(i)
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not wrong
+
+
+def test_results_do_not_depend_on_what_scratch_memory_held(kernel_status):
+    """NaN in the allocator's free blocks, which workspaces and results are made of."""
+    for lens, new in (([3000], [40]), ([5000, 70], [1, 1]), BATCHES["server"], BATCHES["empty slots"]):
+        s = oracle.batch(lens, new, 8, 2, 128, 32, device="cuda")
+        one = set(new) == {1}
+        want = _attend(s, cu=not one)
+        for _ in range(2):
+            torch.full((64 << 20,), float("nan"), device="cuda")
+            assert torch.equal(_attend(s, cu=not one), want)
