@@ -766,17 +766,19 @@ static int launch_join(const PagedAttn& p, cudaStream_t st) {
   return GFH_OK;
 }
 
-// Items of a call at most, rows of one that are tokens' at most, and whether blocks may be cut: what decides the grid and the workspace.
+// Items of a call at most, rows of one that are tokens' at most, and whether blocks may be cut: what decides the grid and the workspace. They are
+// not where there are two for every SM, nor where no sequence has more than four steps of keys: those four (6 us) take as long as one and the
+// second kernel.
 struct PgCall {
   int items, rows, slots;
   long long ws;
 };
-static bool pg_call(PgCall& c, int B, int T, bool one_each, int Hq, int Hkv, int D, int sms) {
+static bool pg_call(PgCall& c, int B, int T, bool one_each, long long keys, int Hq, int Hkv, int D, int sms) {
   const int G = Hq / Hkv, w = 2 * (PG_TILE / G);
   const long long blocks = one_each ? B : min((long long)T, ((long long)T + (long long)B * (w - 1)) / w);
   const long long items = blocks * Hkv;
   if (items > 0x7fffffffll) return false;
-  c.slots = items < 2 * sms ? sms : 0;
+  c.slots = items < 2 * sms && keys > 4 * PG_TILE ? sms : 0;
   c.items = c.slots ? 2 * sms : (int)items;
   c.rows = one_each || T <= PG_TILE / G ? PG_TILE : 2 * PG_TILE;       // blocks of one tile, or of two
   c.ws = c.slots ? 256 + 4ll * c.items * c.rows * (D + 2) : 0;
@@ -791,11 +793,11 @@ static bool paged_sizes(int B, int T, int Hq, int Hkv, int D) {
   return B > 0 && T > 0 && Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && Hq / Hkv <= PG_TILE && (D == 64 || D == 128) && Hkv <= 65535;
 }
 
-// Bytes of workspace of a call, -1 for sizes that are not taken.
-GF_API long long gf_paged_attn_workspace(int B, int T, int one_each, int Hq, int Hkv, int D) {
+// Bytes of workspace of a call, -1 for sizes that are not taken. one_each: there is no `cu`; keys: width * page.
+GF_API long long gf_paged_attn_workspace(int B, int T, int one_each, long long keys, int Hq, int Hkv, int D) {
   gf::bind();
   PgCall c;
-  if (!paged_sizes(B, T, Hq, Hkv, D) || !pg_call(c, B, T, one_each != 0, Hq, Hkv, D, sm_count())) return -1;
+  if (!paged_sizes(B, T, Hq, Hkv, D) || !pg_call(c, B, T, one_each != 0, keys, Hq, Hkv, D, sm_count())) return -1;
   return c.ws;
 }
 
@@ -810,7 +812,7 @@ GF_API int gf_paged_attn(const PagedCall* c, float scale, void* ws, long long ws
   if (ones && !attn_paged_one_ok(*c, ones, ones_scratch)) return GFH_BAD_ARG;
   gf::bind();
   PgCall n;
-  if (!pg_call(n, B, T, !p.seqs.cu, Hq, Hkv, D, sm_count())) return GFH_TOO_LARGE;
+  if (!pg_call(n, B, T, !p.seqs.cu, p.seqs.capacity(), Hq, Hkv, D, sm_count())) return GFH_TOO_LARGE;
   if (ws_bytes < n.ws || (n.ws && !ws)) return GFH_BAD_ARG;
   gf::enter();
   p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.tq = PG_TILE / p.G;

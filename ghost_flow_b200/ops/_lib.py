@@ -73,7 +73,7 @@ _SIGS = {
     "gf_llama_decode_layer": [P, P, F, P, P, P, F, P, P, P, P, P, P, I, P, P, I, I, I, I, I, I, I, I, I, P, P],
     "gf_attn_decode": [P, L, P, P, I, P, I, P, L, I, I, I, I, F, I, P, P],
     "gf_paged_append": [P, P, P, I, I, P],
-    "gf_paged_attn_workspace": [I, I, I, I, I, I],
+    "gf_paged_attn_workspace": [I, I, I, L, I, I, I],
     "gf_paged_attn": [P, F, P, L, I, P, P],
     "gf_paged_attn_one": [P, F, I, P, P],
     "gf_process_logits": [P, P],
@@ -183,10 +183,15 @@ def stream_on(device: int):
 _STATUS = {}
 
 
+_STATUS_AT = {}
+
+
 def status_ptr(device: int) -> int:
     """Address of :func:`status_word` of a device's index."""
-    t = _STATUS.get(device)
-    return (status_word(torch.device("cuda", device)) if t is None else t).data_ptr()
+    at = _STATUS_AT.get(device)
+    if at is None:
+        at = _STATUS_AT[device] = status_word(torch.device("cuda", device)).data_ptr()
+    return at
 
 
 def status_word(device=None) -> torch.Tensor:

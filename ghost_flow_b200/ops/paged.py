@@ -20,7 +20,7 @@ import torch
 
 from . import _lib
 from .fused import _observed, _rc, _rope_tables_fit_kernel, _rows_apart
-from .gemm import _sm_count
+from .gemm import _SMS, _sm_count
 from .raw import _decode_parts
 
 _INT32, _BF16 = torch.int32, torch.bfloat16
@@ -71,18 +71,20 @@ def _for_kernels(x, kpages, vpages, page_table, lens, cu):
     see :func:`_check_batch` for why."""
     dev = x.get_device()
     if dev < 0 or x.dtype is not _BF16 or kpages.dtype is not _BF16 or vpages.dtype is not _BF16 or page_table.dtype is not _INT32 \
-            or lens.dtype is not _INT32 or not dev == kpages.get_device() == vpages.get_device() == page_table.get_device() == lens.get_device() \
-            or x.dim() != 3 or lens.dim() != 1 or page_table.dim() != 2 or kpages.dim() != 4:
+            or lens.dtype is not _INT32 or not dev == kpages.get_device() == vpages.get_device() == page_table.get_device() == lens.get_device():
         return None
-    shape, B, (Bt, width) = kpages.shape, lens.shape[0], page_table.shape
-    if vpages.shape != shape or Bt != B or B == 0 or not page_table.stride(1) == 1 == lens.stride(0):
+    shape = kpages.shape
+    try:
+        (P, page, Hk, D), (B,), (Bt, width) = shape, lens.shape, page_table.shape
+    except ValueError:
+        return None
+    if vpages.shape != shape or Bt != B or B == 0 or not page_table.stride(1) == 1 == lens.stride(0) or x.dim() != 3:
         return None
     if cu is None:
         if x.shape[0] != B:
             return None
     elif cu.dtype is not _INT32 or cu.get_device() != dev or cu.dim() != 1 or cu.shape[0] != B + 1 or cu.stride(0) != 1:
         return None
-    P, page, Hk, D = shape
     a0, a1, a2, a3 = kpages.stride()
     b0, b1, b2, b3 = vpages.stride()
     if P == 0 or Hk == 0 or page < 16 or page & (page - 1) or P * page > _MOST or width > _MOST // page or not a3 == 1 == b3 \
@@ -203,9 +205,9 @@ _MANY = 8
 
 
 @functools.lru_cache(maxsize=4096)
-def _attention_workspace(device: int, B: int, T: int, one_each: bool, H: int, Hk: int, D: int) -> int:
-    """Bytes that a call leaves the results of pieces in (the number of SMs decides whether keys are cut)."""
-    return _lib.cuda_lib().gf_paged_attn_workspace(B, T, 1 if one_each else 0, H, Hk, D)
+def _attention_workspace(device: int, B: int, T: int, one_each: bool, keys: int, H: int, Hk: int, D: int) -> int:
+    """Bytes that a call leaves the results of pieces in (the number of SMs decides whether keys, ``keys`` of a sequence at most, are cut)."""
+    return _lib.cuda_lib().gf_paged_attn_workspace(B, T, 1 if one_each else 0, keys, H, Hk, D)
 
 
 def _attention_ref(q, kpages, vpages, page_table, lens, cu, scale, out):
@@ -307,14 +309,14 @@ def paged_attention(q, kpages, vpages, page_table, lens, cu=None, scale: float |
                  0 if cu is None else cu.data_ptr(), B, T, H, Hk, D, page, P, _lib.status_ptr(device))
     parts, few = 0, None
     if one or (cu is not None and B >= _MANY and H // Hk <= 8):
-        parts = _decode_parts(B, Hk, width * page, D, _sm_count(q.device), True)
+        parts = _decode_parts(B, Hk, width * page, D, _SMS.get(device) or _sm_count(q.device), True)
         if parts != 1:
             few = torch.empty((B * parts if parts > 0 else -2 * parts) * H * (D + 2), dtype=torch.float32, device=q.device)
     few_at = None if few is None else few.data_ptr()
     if one:
         _rc(_lib.cuda_lib().gf_paged_attn_one(call, scale, parts, few_at, stream), "gf_paged_attn_one")
     else:
-        nbytes = _attention_workspace(device, B, T, cu is None, H, Hk, D)
+        nbytes = _attention_workspace(device, B, T, cu is None, width * page, H, Hk, D)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
         _rc(_lib.cuda_lib().gf_paged_attn(call, scale, None if ws is None else ws.data_ptr(), nbytes, parts, few_at, stream),
             "gf_paged_attn")

@@ -42,13 +42,13 @@ def test_attention(kw):
 
 def test_attention_scales_workspaces_and_splits():
     lib = _lib.cuda_lib()
-    need = lib.gf_paged_attn_workspace(2, 5, 0, 4, 2, 64)
-    assert need > 0 and lib.gf_paged_attn_workspace(2, 5, 0, 5, 2, 64) == lib.gf_paged_attn_workspace(2, 5, 0, 4, 2, 96) == -1
+    need = lib.gf_paged_attn_workspace(2, 5, 0, 64 * 16, 4, 2, 64)
+    assert need > 0 and lib.gf_paged_attn_workspace(2, 5, 0, 1024, 5, 2, 64) == lib.gf_paged_attn_workspace(2, 5, 0, 1024, 4, 2, 96) == -1
     for scale in (0.0, -0.1, float("nan")):
         assert lib.gf_paged_attn(_call(), scale, P, need, 0, None, None) == BAD_ARG
     for ws, n in ((P, need - 1), (None, need), (P + 8, need)):
-        assert lib.gf_paged_attn(_call(), 0.1, ws, n, 0, None, None) == BAD_ARG
-    assert lib.gf_paged_attn(_call(), 0.1, P, need, 2, None, None) == BAD_ARG             # no scratch for the splits
+        assert lib.gf_paged_attn(_call(width=64), 0.1, ws, n, 0, None, None) == BAD_ARG
+    assert lib.gf_paged_attn(_call(width=64), 0.1, P, need, 2, None, None) == BAD_ARG             # no scratch for the splits
     assert lib.gf_paged_attn(_call(H=32, Hk=2), 0.1, P, 1 << 40, 2, P, None) == BAD_ARG   # sixteen query heads to a KV head
     one = dict(cu=0, T=2)
     assert lib.gf_paged_attn_one(_call(**one), 0.1, 0, P, None) == lib.gf_paged_attn_one(_call(**one), 0.1, 2, None, None) == BAD_ARG
