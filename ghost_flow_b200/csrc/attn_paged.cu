@@ -15,8 +15,6 @@
 //  * Rows behind a sequence's last key may hold anything. Scores there are set to -inf, but a product takes 0 * V too, so an idle warp clears those
 //    rows of V in shared memory before the tile is handed on. Pages that are not there, and those behind the last, are zeros from TMA (a
 //    coordinate outside of the pool).
-#include <type_traits>
-
 #include "paged.cuh"
 
 namespace gf {
@@ -40,7 +38,7 @@ struct PagedAttn {
   int* plan;                     // keys (in steps) of a piece, for the kernel that joins pieces
   float* part;                   // [item][rows][D], then [item][rows][maximum, sum]
   float* part_ml;
-  int rows, items;               // rows of an item in `part`, and CTAs
+  int rows, items, blocks;       // rows of an item in `part`, items and blocks (of all KV heads) at most
 };
 
 struct PgShape {                 // what a sequence is cut into
@@ -591,7 +589,8 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       a1 *= inv;
       __nv_bfloat16* orow = p.out + (long long)(item.token + tok) * p.ldo + head * HD;
       const long long row = (long long)blockIdx.x * p.rows + (alternate ? r : t * PG_TILE + r);
-      float* prow = p.part + row * HD;
+      // left for the other kernel four columns of 32 rows at a time: a warp's rows lie next to each other
+      float* prow = p.part + (row - lane) * HD + lane * 4;
       // rolled up: code that runs once is waited for
 #pragma unroll 1
       for (int c = 0; c < HD / 32; ++c) {
@@ -616,7 +615,8 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           }
         } else if (n_j > 0) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(prow + c * 32 + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<float4*>(prow + (c * 32 + i) * 32) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
         }
       }
       if (mine && !whole && n_j > 0) *reinterpret_cast<float2*>(p.part_ml + 2 * row) = make_float2(m_ref * sl2, l);
@@ -633,82 +633,84 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   }
 }
 
-// Adds up the pieces of blocks that were cut: a warp takes one token's row (a query head) after the other, a lane D / 32 columns of it. What the
-// rows belong to is found before the first kernel has ended.
+constexpr int PG_COLS = 8, PG_AHEAD = 4;
+// Adds up the pieces of blocks that were cut: a CTA has 8 columns of one block, a warp 32 of its rows, a lane one of them. Which block that is is
+// found before the first kernel has ended. Two or three pieces of many rows want warps on an SM, many pieces of few rows loads of a warp on
+// their way together: the whole call, us, with 2 / 4 (64 registers) / 8 pieces at a time, 512 new tokens over 7681 keys, 2 pieces 72 / 72 to 75 / 76, 5 over
+// 30000, 17 pieces 39.2 / 37.6 / 37.0, 16 over 2000, 16 pieces 14.2 / 12.5 / 12.3.
 template <int HD>
-__global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ PagedAttn p) {
-  constexpr int E = HD / 32;
-  using Vec = typename std::conditional<E == 4, float4, float2>::type;
-  const int lane = threadIdx.x & 31;
-  const long long rows = (long long)p.seqs.T * p.Hq;
-  int U = 0;
-  for (long long x = blockIdx.x * 8ll + (threadIdx.x >> 5); x < rows; x += gridDim.x * 8ll) {
-    const int t = (int)(x / p.Hq), h = (int)(x - (long long)t * p.Hq), hk = h / p.G;
-    const int b = paged_seq_of(p.seqs, t);
-    PgShape s{};
-    int first = 0;
-    if (b < p.seqs.B) {
-      s = pg_shape(p, b);
-      first = p.seqs.first(b);
+__global__ void __launch_bounds__(256, 4) paged_join_kernel(const __grid_constant__ PagedAttn p) {
+  constexpr int GROUPS = HD / PG_COLS;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = (blockIdx.x % GROUPS) * PG_COLS;
+  PgShape own{};
+  if (lane < p.seqs.B) own = pg_shape(p, lane);
+  PgItem it{};
+  const bool there = pg_find(p, own, blockIdx.x / GROUPS, PG_WHOLE, it);
+  const int t = warp >> 2, r = (warp & 3) * 32 + lane;                 // tile and row in it
+  const int rows = max(0, min(p.tq, it.tokens - t * p.tq)) * p.G;      // of the tile
+  const bool mine = there && r < rows;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int U = *p.plan;
+  if (!__any_sync(0xffffffffu, mine) || U == PG_WHOLE) return;
+  const PgShape s = pg_shape(p, it.b);
+  const int pieces = (s.steps + U - 1) / U, blk = (it.token - p.seqs.first(it.b)) / (2 * p.tq);
+  if (pieces == 1) return;
+  int before = 0;                  // items of the sequences in front
+  for (int i = lane; i < it.b; i += 32) {
+    const PgShape o = pg_shape(p, i);
+    before += o.blocks * ((o.steps + U - 1) / U);
+  }
+  before = __reduce_add_sync(0xffffffffu, before) * p.Hkv;
+  const int steps = it.steps(2 * p.tq);
+  const long long item = before + ((long long)(s.blocks - 1 - blk) * p.Hkv + it.hk) * pieces;
+  if (item + pieces > p.items || !mine) return;            // sequences that overlap in `cu`: not all items were run
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + item * p.rows + t * PG_TILE + r;
+  const float* part = p.part + (item * p.rows + t * PG_TILE + r - lane) * HD + col * 32 + lane * 4;
+  // a piece that has no keys was not run; there are such where a block has fewer steps than pieces
+  auto run = [&](int k) { return steps >= pieces || steps * k / pieces < steps * (k + 1) / pieces; };
+  float m = -INFINITY, l = 0.f, o[PG_COLS];
+#pragma unroll
+  for (int e = 0; e < PG_COLS; ++e) o[e] = 0.f;
+#pragma unroll 1
+  for (int k0 = 0; k0 < pieces; k0 += PG_AHEAD) {           // what PG_AHEAD pieces left is on its way together
+    float2 x[PG_AHEAD];
+    float4 v[PG_AHEAD][PG_COLS / 4];
+#pragma unroll
+    for (int i = 0; i < PG_AHEAD; ++i) {
+      const int k = k0 + i;
+      x[i] = make_float2(-INFINITY, 0.f);
+      if (k >= pieces || !run(k)) continue;
+      x[i] = ml[(long long)k * p.rows];
+#pragma unroll
+      for (int e = 0; e < PG_COLS / 4; ++e) v[i][e] = *reinterpret_cast<const float4*>(part + (long long)k * p.rows * HD + e * 128);
     }
-    if (U == 0) {
-      asm volatile("griddepcontrol.wait;" ::: "memory");
-      U = *p.plan;
-    }
-    if (U == PG_WHOLE || b >= p.seqs.B) return;
-    const int pieces = (s.steps + U - 1) / U;
-    if (pieces == 1 || t < first || t >= first + s.n) continue;
-    int before = 0;                // items of the sequences in front
-    for (int i = lane; i < b; i += 32) {
-      const PgShape o = pg_shape(p, i);
-      before += o.blocks * ((o.steps + U - 1) / U);
-    }
-    before = __reduce_add_sync(0xffffffffu, before) * p.Hkv;
-    const int blk = (t - first) / (2 * p.tq);
-    PgItem it;
-    pg_block(p, it, s, b, blk);
-    const int in = t - it.token, steps = it.steps(2 * p.tq);
-    const long long item = before + ((long long)(s.blocks - 1 - blk) * p.Hkv + hk) * pieces;
-    if (item + pieces > p.items) return;                   // sequences that overlap in `cu`: not all items were run
-    const long long row = item * p.rows + (in / p.tq) * PG_TILE + (in % p.tq) * p.G + (h - hk * p.G);
-    float m = -INFINITY, l = 0.f, o[E];
+    float mm = m;
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = 0.f;
-    for (int k0 = 0; k0 < pieces; k0 += 32) {              // a lane has a piece's maximum and sum
-      const int k = k0 + lane;
-      const bool there = k < pieces && (long long)steps * k / pieces < (long long)steps * (k + 1) / pieces;
-      const float2 ml = there ? *reinterpret_cast<const float2*>(p.part_ml + 2 * (row + (long long)k * p.rows)) : make_float2(-INFINITY, 0.f);
-      float mm = ml.x;
+    for (int i = 0; i < PG_AHEAD; ++i) mm = fmaxf(mm, x[i].x);
+    const float use = mm == -INFINITY ? 0.f : mm, old = ex2_approx(m - use);
+    m = mm;
+    l *= old;
 #pragma unroll
-      for (int i = 16; i; i >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, i));
-      mm = fmaxf(mm, m);
-      const float use = mm == -INFINITY ? 0.f : mm, old = ex2_approx(m - use), w = ml.y > 0.f ? ex2_approx(ml.x - use) : 0.f;
-      m = mm;
-      float sum = ml.y * w;
+    for (int e = 0; e < PG_COLS; ++e) o[e] *= old;
 #pragma unroll
-      for (int i = 16; i; i >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
-      l = l * old + sum;
+    for (int i = 0; i < PG_AHEAD; ++i) {
+      if (!(x[i].y > 0.f)) continue;                       // 0 times what may be anything
+      const float w = ex2_approx(x[i].x - use);
+      l += x[i].y * w;
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[e] *= old;
-      const int n = min(32, pieces - k0);
-      const float* part = p.part + (row + (long long)k0 * p.rows) * HD + lane * E;
-#pragma unroll 4
-      for (int i = 0; i < n; ++i) {
-        const float wi = __shfl_sync(0xffffffffu, w, i);
-        const Vec v = *reinterpret_cast<const Vec*>(part + (long long)i * p.rows * HD);
-        const float* f = reinterpret_cast<const float*>(&v);
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] += wi > 0.f ? f[e] * wi : 0.f;      // what no piece has written may be anything
+      for (int e = 0; e < PG_COLS / 4; ++e) {
+        o[4 * e] += v[i][e].x * w;
+        o[4 * e + 1] += v[i][e].y * w;
+        o[4 * e + 2] += v[i][e].z * w;
+        o[4 * e + 3] += v[i][e].w * w;
       }
     }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    uint32_t u[E / 2];
-#pragma unroll
-    for (int e = 0; e < E; e += 2) u[e / 2] = pack_bf16x2(o[e] * inv, o[e + 1] * inv);
-    uint32_t* to = reinterpret_cast<uint32_t*>(p.out + t * p.ldo + h * HD + lane * E);
-#pragma unroll
-    for (int e = 0; e < E / 2; ++e) to[e] = u[e];
   }
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  uint4 u;
+  u.x = pack_bf16x2(o[0] * inv, o[1] * inv); u.y = pack_bf16x2(o[2] * inv, o[3] * inv);
+  u.z = pack_bf16x2(o[4] * inv, o[5] * inv); u.w = pack_bf16x2(o[6] * inv, o[7] * inv);
+  *reinterpret_cast<uint4*>(p.out + (long long)(it.token + t * p.tq + r / p.G) * p.ldo + (it.hk * p.G + r % p.G) * HD + col) = u;
 }
 
 static int pg_map(CUtensorMap* out, const void* base, int rank, const cuuint64_t* dims, const long long* strides, const cuuint32_t* box) {
@@ -756,7 +758,7 @@ static int launch_join(const PagedAttn& p, cudaStream_t st) {
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)min(((long long)p.seqs.T * p.Hq + 7) / 8, 8ll * p.slots));
+  cfg.gridDim = dim3((unsigned)(p.blocks * (HD / PG_COLS)));
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cfg.attrs = at;
@@ -770,7 +772,7 @@ static int launch_join(const PagedAttn& p, cudaStream_t st) {
 // not where there are two for every SM, nor where no sequence has more than four steps of keys: those four (6 us) take as long as one and the
 // second kernel.
 struct PgCall {
-  int items, rows, slots;
+  int items, rows, slots, blocks;
   long long ws;
 };
 static bool pg_call(PgCall& c, int B, int T, bool one_each, long long keys, int Hq, int Hkv, int D, int sms) {
@@ -779,6 +781,7 @@ static bool pg_call(PgCall& c, int B, int T, bool one_each, long long keys, int 
   const long long items = blocks * Hkv;
   if (items > 0x7fffffffll) return false;
   c.slots = items < 2 * sms && keys > 4 * PG_TILE ? sms : 0;
+  c.blocks = (int)items;
   c.items = c.slots ? 2 * sms : (int)items;
   c.rows = one_each || T <= PG_TILE / G ? PG_TILE : 2 * PG_TILE;       // blocks of one tile, or of two
   c.ws = c.slots ? 256 + 4ll * c.items * c.rows * (D + 2) : 0;
@@ -816,7 +819,7 @@ GF_API int gf_paged_attn(const PagedCall* c, float scale, void* ws, long long ws
   if (ws_bytes < n.ws || (n.ws && !ws)) return GFH_BAD_ARG;
   gf::enter();
   p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.tq = PG_TILE / p.G;
-  p.slots = n.slots; p.scale = scale; p.rows = n.rows; p.items = n.items;
+  p.slots = n.slots; p.scale = scale; p.rows = n.rows; p.items = n.items; p.blocks = n.blocks;
   p.skip_ones = ones != 0;
   p.out = (__nv_bfloat16*)c->y; p.ldo = c->ldy;
   if (n.slots) {

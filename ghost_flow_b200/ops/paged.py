@@ -293,7 +293,9 @@ def paged_attention(q, kpages, vpages, page_table, lens, cu=None, scale: float |
     if stream is None:
         with torch.cuda.device(device):
             return paged_attention(q, kpages, vpages, page_table, lens, cu, scale, out)
-    one = cu is None and H // Hk <= 8
+    G = H // Hk
+    groups = 1 if G <= 8 else 2 if G <= 16 and G % 2 == 0 else 0        # of heads that the decode kernel takes at a time; 0: not its
+    one = cu is None and groups > 0
     x = q
     if not scale > 0 and not one:            # this kernel takes the largest score before it scales
         x, scale = q * (-1 if scale < 0 else 0), -scale if scale < 0 else 1.0
@@ -308,8 +310,8 @@ def paged_attention(q, kpages, vpages, page_table, lens, cu=None, scale: float |
     call = _CALL(at, ld, o.data_ptr(), ldo, *pools, page_table.data_ptr(), page_table.stride(0), width, lens.data_ptr(),
                  0 if cu is None else cu.data_ptr(), B, T, H, Hk, D, page, P, _lib.status_ptr(device))
     parts, few = 0, None
-    if one or (cu is not None and B >= _MANY and H // Hk <= 8):
-        parts = _decode_parts(B, Hk, width * page, D, _SMS.get(device) or _sm_count(q.device), True)
+    if one or (cu is not None and B >= _MANY and groups):
+        parts = _decode_parts(B, Hk * groups, width * page, D, _SMS.get(device) or _sm_count(q.device), True)
         if parts != 1:
             few = torch.empty((B * parts if parts > 0 else -2 * parts) * H * (D + 2), dtype=torch.float32, device=q.device)
     few_at = None if few is None else few.data_ptr()

@@ -46,7 +46,7 @@ def test_attention_pages_and_layouts(page, layout, H, Hk, D, kernel_status):
     oracle.close(_attend(s), want, off)
 
 
-@pytest.mark.parametrize("H,Hk,D", [(4, 2, 64), (8, 1, 128), (16, 1, 64)])
+@pytest.mark.parametrize("H,Hk,D", [(4, 2, 64), (8, 1, 128), (16, 1, 64), (20, 2, 128), (11, 1, 64), (40, 1, 128)])
 @pytest.mark.parametrize("scale", [None, 0.02, -0.3])
 def test_attention_of_one_token_each(H, Hk, D, scale, kernel_status):
     lens = [1, 16, 17, 0, 64, 1000, 515]
@@ -56,7 +56,7 @@ def test_attention_of_one_token_each(H, Hk, D, scale, kernel_status):
 
 
 @pytest.mark.parametrize("parts", [1, 3, 16, -1, -5, -300])
-@pytest.mark.parametrize("H,Hk,D", [(4, 2, 64), (8, 1, 128)])
+@pytest.mark.parametrize("H,Hk,D", [(4, 2, 64), (8, 1, 128), (24, 2, 64), (16, 1, 128)])
 def test_attention_of_some_with_one_token(parts, H, Hk, D, monkeypatch, kernel_status):
     """Sequences of one token beside others, however their keys are cut; also where there is none of them, or nothing but them."""
     from ghost_flow_b200.ops import paged

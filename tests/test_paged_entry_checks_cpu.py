@@ -49,7 +49,7 @@ def test_attention_scales_workspaces_and_splits():
     for ws, n in ((P, need - 1), (None, need), (P + 8, need)):
         assert lib.gf_paged_attn(_call(width=64), 0.1, ws, n, 0, None, None) == BAD_ARG
     assert lib.gf_paged_attn(_call(width=64), 0.1, P, need, 2, None, None) == BAD_ARG             # no scratch for the splits
-    assert lib.gf_paged_attn(_call(H=32, Hk=2), 0.1, P, 1 << 40, 2, P, None) == BAD_ARG   # sixteen query heads to a KV head
+    assert lib.gf_paged_attn(_call(H=26, Hk=2), 0.1, P, 1 << 40, 2, P, None) == BAD_ARG   # thirteen query heads to a KV head
     one = dict(cu=0, T=2)
     assert lib.gf_paged_attn_one(_call(**one), 0.1, 0, P, None) == lib.gf_paged_attn_one(_call(**one), 0.1, 2, None, None) == BAD_ARG
     assert lib.gf_paged_attn_one(_call(T=2), 0.1, 1, P, None) == lib.gf_paged_attn_one(None, 0.1, 1, P, None) == BAD_ARG
