@@ -178,8 +178,8 @@ def rope_qkv_to_pages(qkv, num_heads: int, num_kv_heads: int, cos, sin, kpages, 
         if not (cos.dim() == 2 and cos.shape == sin.shape and 2 * cos.shape[1] == D and cos.device == sin.device == qkv.device):
             raise ValueError(f"{what}: rope tables must be [positions, {D // 2}] on {qkv.device}, got {list(cos.shape)} on {cos.device} and "
                              f"{list(sin.shape)} on {sin.device}")
-        if T == 0:
-            return qkv.new_empty(0, H, D)
+        if T == 0 or lens.shape[0] == 0:
+            return qkv.new_zeros(T, H, D)
         return _append_ref(qkv, H, Hk, cos, sin, kpages, vpages, page_table, lens, cu, interleaved)
     stream = _lib.stream_on(device)
     if stream is None:
@@ -267,7 +267,7 @@ def paged_attention(q, kpages, vpages, page_table, lens, cu=None, scale: float |
         elif out is not None:
             st = out.stride()
             if out.shape != q.shape or out.dtype is not _BF16 or out.device != q.device or st[2] != 1 or st[1] != D or st[0] % 8 \
-                    or st[0] < H * D or out.data_ptr() % 16:
+                    or st[0] < H * D or out.data_ptr() % 16 or (out.requires_grad and torch.is_grad_enabled()):
                 fits = None
     what = "paged_attention"
     if fits is None:

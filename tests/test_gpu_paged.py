@@ -324,3 +324,42 @@ def test_results_do_not_depend_on_what_scratch_memory_held(kernel_status):
         for _ in range(2):
             torch.full((64 << 20,), float("nan"), device="cuda")
             assert torch.equal(_attend(s, cu=not one), want)
+
+
+def test_batches_of_nothing_and_tensors_that_autograd_does_not_follow(kernel_status):
+    from ghost_flow_b200 import ops
+
+    cos, sin = ops.rope_tables(64, 64, 1e4, "cuda")
+    s = oracle.batch([], [], 4, 2, 64, 16, device="cuda", behind=3)
+    assert _attend(s).shape == (3, 4, 64)
+    assert ops.rope_qkv_to_pages(s["qkv"], 4, 2, cos, sin, s["kp"], s["vp"], s["table"], s["lens"], s["cu"]).shape == (3, 4, 64)
+    s = oracle.batch([7, 20], [1, 2], 4, 2, 64, 16, device="cuda")
+    args = s["table"], s["lens"], s["cu"]
+    want = _attend(s)
+    with torch.inference_mode():
+        pools = s["kp"].clone(), s["vp"].clone()
+        assert torch.equal(ops.paged_attention(s["q"].clone(), *pools, *args), want)
+        ops.rope_qkv_to_pages(s["qkv"], 4, 2, cos, sin, *pools, *args)
+    leaf = torch.zeros_like(s["q"], requires_grad=True)
+    with pytest.raises(RuntimeError):                       # as a write to a leaf is
+        _attend(s, out=leaf)
+    with torch.no_grad():
+        _attend(s, out=leaf)
+    assert torch.equal(leaf.detach(), want)
+
+
+def test_gradients_of_shared_heads_on_the_device():
+    """A call with a gradient to record takes PyTorch's operations, in the type of its tensors."""
+    s = oracle.batch([40, 9], [7, 9], 4, 2, 64, 16, device="cuda")
+    s = {k: v.nan_to_num(0, 0, 0) if k in ("kp", "vp") else v for k, v in s.items()}
+    t = [s[n].float().requires_grad_() for n in ("q", "kp", "vp")]
+    d = [s[n].double().requires_grad_() for n in ("q", "kp", "vp")]
+    b = [s[n].clone().requires_grad_() for n in ("q", "kp", "vp")]
+    from ghost_flow_b200 import ops
+
+    w = torch.randn(16, 4, 64, device="cuda")
+    grads = [torch.autograd.grad((ops.paged_attention(*x, s["table"], s["lens"], s["cu"]) * w.to(x[0].dtype)).sum(), x) for x in (d, t, b)]
+    for exact, single, half in zip(*grads):
+        # 32 bits: sums of at most 40 products of numbers of this size; bf16: the products' inputs and results are rounded, and grads once more
+        assert (single.double() - exact).norm() <= 64 * 2 ** -24 * 16 * exact.norm()
+        assert (half.double() - exact).norm() <= 8 * 2 ** -8 * exact.norm()

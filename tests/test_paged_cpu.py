@@ -48,6 +48,19 @@ def test_one_token_of_each_sequence_needs_no_cu():
     assert torch.equal(*q) and all(torch.equal(x.nan_to_num(3), y.nan_to_num(3)) for x, y in zip(*pools)) and not q[0][1].any()
 
 
+def test_batches_of_nothing():
+    s = oracle.batch([], [], 4, 2, 16, 16, torch.float32, behind=3)
+    cos, sin = ops.rope_tables(8, 16, 1e4)
+    assert ops.paged_attention(s["q"], s["kp"], s["vp"], s["table"], s["lens"], s["cu"]).shape == (3, 4, 16)
+    assert ops.rope_qkv_to_pages(s["qkv"], 4, 2, cos, sin, s["kp"], s["vp"], s["table"], s["lens"], s["cu"]).shape == (3, 4, 16)
+    s = oracle.batch([7], [0], 4, 2, 16, 16, torch.float32)
+    out = torch.zeros(0, 4, 16)
+    assert ops.paged_attention(s["q"], s["kp"], s["vp"], s["table"], s["lens"], s["cu"], out=out) is out
+    assert ops.rope_qkv_to_pages(s["qkv"], 4, 2, cos, sin, s["kp"], s["vp"], s["table"], s["lens"], s["cu"]).shape == (0, 4, 16)
+    x = torch.zeros(0, 7)
+    assert ops.process_logits(x).shape == (0, 7) and ops.process_logits(x, out=x) is x
+
+
 def test_gradient_of_attention_is_that_of_its_formula():
     s = oracle.batch([4, 9], [2, 5], 4, 2, 8, 16, torch.float64)
     for n in ("kp", "vp"):
