@@ -85,6 +85,31 @@ def build(args, dev):
         kc = torch.randn(B, S, Hkv * D, device=dev, dtype=bf)
         vc = torch.randn(B, S, Hkv * D, device=dev, dtype=bf)
         return (lambda: raw.attn_decode(q, kc, vc, S, B, H, Hkv, D)), 4.0 * B * H * S * D, 4.0 * B * S * Hkv * D
+    if k in ("paged_attn", "paged_append"):
+        # --batch sequences of --seq keys in pages of --page rows, --new new tokens each
+        from ghost_flow_b200 import ops
+        B, S, H, Hkv, D, n, page = args.batch, args.seq, args.heads, args.kv_heads or args.heads, args.dim, args.new, args.page
+        width = -(-S // page)
+        kp, vp = (torch.randn(B * width, page, Hkv, D, device=dev, dtype=bf) for _ in range(2))
+        table = torch.randperm(B * width, device=dev).int().view(B, width)
+        lens = torch.full((B,), S, dtype=torch.int32, device=dev)
+        cu = None if n == 1 else (n * torch.arange(B + 1, device=dev)).int()
+        if k == "paged_append":
+            qkv = torch.randn(B * n, H + 2 * Hkv, D, device=dev, dtype=bf)
+            cos, sin = ops.rope_tables(S, D, 10000.0, dev)
+            return (lambda: ops.rope_qkv_to_pages(qkv, H, Hkv, cos, sin, kp, vp, table, lens, cu)), 0.0, 4.0 * qkv.numel() + 4.0 * B * n * D
+        q = torch.randn(B * n, H, D, device=dev, dtype=bf)
+        return (lambda: ops.paged_attention(q, kp, vp, table, lens, cu)), 4.0 * B * H * D * (n * S - n * (n - 1) / 2), \
+            4.0 * (q.numel() + B * S * Hkv * D)
+    if k == "process_logits":
+        # --rows rows of --cols entries in bf16, --seq tokens each, all penalties and a mask
+        from ghost_flow_b200 import ops
+        R, V = args.rows, args.cols
+        x = torch.randn(R, V, device=dev, dtype=bf)
+        tokens = (V * torch.rand(R, args.seq, device=dev) ** 4).int()
+        allowed = ops.pack_allowed(torch.rand(R, V, device=dev) < 0.5)
+        return (lambda: ops.process_logits(x, tokens, repetition=1.2, presence=0.5, frequency=0.2, allowed=allowed)), 0.0, \
+            4.0 * R * V + R * V / 8 + 4.0 * R * args.seq
     if k in ("attn_fwd", "attn_bwd"):
         B, S, H, Hkv, D = args.batch, args.seq, args.heads, args.kv_heads or args.heads, args.dim
         q = torch.randn(B * S, H * D, device=dev, dtype=bf)
@@ -200,6 +225,8 @@ def main():
     ap.add_argument("--heads", type=int, default=32)
     ap.add_argument("--kv-heads", type=int, default=0)
     ap.add_argument("--dim", type=int, default=128)
+    ap.add_argument("--new", type=int, default=1)
+    ap.add_argument("--page", type=int, default=64)
     ap.add_argument("--rows", type=int, default=32768)
     ap.add_argument("--cols", type=int, default=4096)
     ap.add_argument("--iters", type=int, default=20)
