@@ -78,6 +78,7 @@ __device__ __forceinline__ int paged_plan(const PagedAttn& p, const PgShape& own
   };
   auto items = [&](int U) { return sum([&](const PgShape& s) { return s.blocks * ((s.steps + U - 1) / U); }); };
   const int whole = sum([](const PgShape& s) { return s.blocks; });
+  if (whole == 0) return PG_WHOLE;
   if (2 * whole <= p.slots) {
     int U = max(1, (sum([](const PgShape& s) { return s.blocks * s.steps; }) + p.slots - 1) / p.slots);
 #pragma unroll 1
@@ -779,18 +780,21 @@ static int launch_join(const PagedAttn& p, cudaStream_t st) {
 }
 
 // Items of a call at most, rows of one that are tokens' at most, and whether blocks may be cut: what decides the grid and the workspace. They are
-// not where there are two for every SM, nor where no sequence has more than four steps of keys: those four (6 us) take as long as one and the
-// second kernel.
+// not where there are two for every SM, nor where no sequence has more than four steps of keys (those four take 6 us, as long as one and the
+// second kernel), nor beside the decode kernel (`ones`) when that has more to do: a step of keys of all KV heads of all sequences takes it as long
+// as a step takes here, 2 us, with 1.25 of them for every SM. 31 sequences of up to 2048 keys with one token and one with 4 / 30 / 481, 32 / 8 heads, cut / not: 60
+// / 46, 62 / 47, 56 / 56 us.
 struct PgCall {
   int items, rows, slots, blocks;
   long long ws;
 };
-static bool pg_call(PgCall& c, int B, int T, bool one_each, long long keys, int Hq, int Hkv, int D, int sms) {
+static bool pg_call(PgCall& c, int B, int T, bool one_each, bool ones, long long keys, int Hq, int Hkv, int D, int sms) {
   const int G = Hq / Hkv, w = 2 * (PG_TILE / G);
   const long long blocks = one_each ? B : min((long long)T, ((long long)T + (long long)B * (w - 1)) / w);
   const long long items = blocks * Hkv;
   if (items > 0x7fffffffll) return false;
-  c.slots = items < 2 * sms && keys > 4 * PG_TILE ? sms : 0;
+  const bool beside = ones && 4ll * B * Hkv >= 5ll * sms;
+  c.slots = items < 2 * sms && keys > 4 * PG_TILE && !beside ? sms : 0;
   c.blocks = (int)items;
   c.items = c.slots ? 2 * sms : (int)items;
   c.rows = one_each || T <= PG_TILE / G ? PG_TILE : 2 * PG_TILE;       // blocks of one tile, or of two
@@ -806,11 +810,11 @@ static bool paged_sizes(int B, int T, int Hq, int Hkv, int D) {
   return B > 0 && T > 0 && Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && Hq / Hkv <= PG_TILE && (D == 64 || D == 128) && Hkv <= 65535;
 }
 
-// Bytes of workspace of a call, -1 for sizes that are not taken. one_each: there is no `cu`; keys: width * page.
-GF_API long long gf_paged_attn_workspace(int B, int T, int one_each, long long keys, int Hq, int Hkv, int D) {
+// Bytes of workspace of a call, -1 for sizes that are not taken. one_each: there is no `cu`; ones: as for gf_paged_attn; keys: width * page.
+GF_API long long gf_paged_attn_workspace(int B, int T, int one_each, int ones, long long keys, int Hq, int Hkv, int D) {
   gf::bind();
   PgCall c;
-  if (!paged_sizes(B, T, Hq, Hkv, D) || !pg_call(c, B, T, one_each != 0, keys, Hq, Hkv, D, sm_count())) return -1;
+  if (!paged_sizes(B, T, Hq, Hkv, D) || !pg_call(c, B, T, one_each != 0, ones != 0, keys, Hq, Hkv, D, sm_count())) return -1;
   return c.ws;
 }
 
@@ -825,7 +829,7 @@ GF_API int gf_paged_attn(const PagedCall* c, float scale, void* ws, long long ws
   if (ones && !attn_paged_one_ok(*c, ones, ones_scratch)) return GFH_BAD_ARG;
   gf::bind();
   PgCall n;
-  if (!pg_call(n, B, T, !p.seqs.cu, p.seqs.capacity(), Hq, Hkv, D, sm_count())) return GFH_TOO_LARGE;
+  if (!pg_call(n, B, T, !p.seqs.cu, ones != 0, p.seqs.capacity(), Hq, Hkv, D, sm_count())) return GFH_TOO_LARGE;
   if (ws_bytes < n.ws || (n.ws && !ws)) return GFH_BAD_ARG;
   gf::enter();
   p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.tq = PG_TILE / p.G;

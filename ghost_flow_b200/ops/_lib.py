@@ -73,7 +73,7 @@ _SIGS = {
     "gf_llama_decode_layer": [P, P, F, P, P, P, F, P, P, P, P, P, P, I, P, P, I, I, I, I, I, I, I, I, I, P, P],
     "gf_attn_decode": [P, L, P, P, I, P, I, P, L, I, I, I, I, F, I, P, P],
     "gf_paged_append": [P, P, P, I, I, P],
-    "gf_paged_attn_workspace": [I, I, I, L, I, I, I],
+    "gf_paged_attn_workspace": [I, I, I, I, L, I, I, I],
     "gf_paged_attn": [P, F, P, L, I, P, P],
     "gf_paged_attn_one": [P, F, I, P, P],
     "gf_process_logits": [P, P],

@@ -21,7 +21,7 @@ import torch
 from . import _lib
 from .fused import _observed, _rc, _rope_tables_fit_kernel, _rows_apart
 from .gemm import _SMS, _sm_count
-from .raw import _decode_parts
+from .raw import _SLICES, _decode_parts
 
 _INT32, _BF16 = torch.int32, torch.bfloat16
 _MOST = 2 ** 31 - 1
@@ -204,10 +204,18 @@ def rope_qkv_to_pages(qkv, num_heads: int, num_kv_heads: int, cos, sin, kpages, 
 _MANY = 8
 
 
+def _parts_beside(heads: int, sms: int) -> int:
+    """How the decode kernel cuts keys (see ``raw._decode_parts``) beside a kernel that holds SMs for as long as it takes: into so few parts of
+    each sequence that they are 1.5 for an SM. Equal shares of all keys, one for every place on the machine, then wait for their places: 64
+    sequences of up to 2000 keys, one of them with 16 new tokens, 32 / 8 heads of 128, us with shares / 1 / 2 / 4 parts 90 / 64 / 67 / 72, 32 of up to
+    4096, one with 256 90 / 83 / 91 / 87, 16 of up to 8000, one with 64 89 / 132 / 96 / 98."""
+    return next((s for s in _SLICES if 2 * heads * s >= 3 * sms), _SLICES[-1])
+
+
 @functools.lru_cache(maxsize=4096)
-def _attention_workspace(device: int, B: int, T: int, one_each: bool, keys: int, H: int, Hk: int, D: int) -> int:
+def _attention_workspace(device: int, B: int, T: int, one_each: bool, ones: bool, keys: int, H: int, Hk: int, D: int) -> int:
     """Bytes that a call leaves the results of pieces in (the number of SMs decides whether keys, ``keys`` of a sequence at most, are cut)."""
-    return _lib.cuda_lib().gf_paged_attn_workspace(B, T, 1 if one_each else 0, keys, H, Hk, D)
+    return _lib.cuda_lib().gf_paged_attn_workspace(B, T, 1 if one_each else 0, 1 if ones else 0, keys, H, Hk, D)
 
 
 def _attention_ref(q, kpages, vpages, page_table, lens, cu, scale, out):
@@ -311,14 +319,15 @@ def paged_attention(q, kpages, vpages, page_table, lens, cu=None, scale: float |
                  0 if cu is None else cu.data_ptr(), B, T, H, Hk, D, page, P, _lib.status_ptr(device))
     parts, few = 0, None
     if one or (cu is not None and B >= _MANY and groups):
-        parts = _decode_parts(B, Hk * groups, width * page, D, _SMS.get(device) or _sm_count(q.device), True)
+        sms = _SMS.get(device) or _sm_count(q.device)
+        parts = _decode_parts(B, Hk * groups, width * page, D, sms, True) if one else _parts_beside(B * Hk * groups, sms)
         if parts != 1:
             few = torch.empty((B * parts if parts > 0 else -2 * parts) * H * (D + 2), dtype=torch.float32, device=q.device)
     few_at = None if few is None else few.data_ptr()
     if one:
         _rc(_lib.cuda_lib().gf_paged_attn_one(call, scale, parts, few_at, stream), "gf_paged_attn_one")
     else:
-        nbytes = _attention_workspace(device, B, T, cu is None, width * page, H, Hk, D)
+        nbytes = _attention_workspace(device, B, T, cu is None, parts != 0, width * page, H, Hk, D)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
         _rc(_lib.cuda_lib().gf_paged_attn(call, scale, None if ws is None else ws.data_ptr(), nbytes, parts, few_at, stream),
             "gf_paged_attn")

@@ -61,7 +61,7 @@ def test_attention_of_some_with_one_token(parts, H, Hk, D, monkeypatch, kernel_s
     """Sequences of one token beside others, however their keys are cut; also where there is none of them, or nothing but them."""
     from ghost_flow_b200.ops import paged
 
-    monkeypatch.setattr(paged, "_decode_parts", lambda *a: parts)
+    monkeypatch.setattr(paged, "_parts_beside", lambda *a: parts)
     lens = [900, 40, 64, 0, 1, 200, 333, 70, 5, 1200]
     for new in ([1, 40, 1, 1, 1, 2, 1, 33, 0, 1], [2, 40, 3, 2, 0, 2, 7, 33, 5, 0], [1] * 10, [0, 0, 0, 0, 0, 0, 0, 0, 1, 0]):
         s = oracle.batch(lens, new, H, Hk, D, 16, device="cuda", behind=1)

@@ -207,3 +207,9 @@ def test_out_that_overlaps_the_logits_is_refused():
     t = torch.zeros(40)
     with pytest.raises(ValueError, match="shares memory"):
         ops.process_logits(t[:16].view(2, 8), out=t[8:24].view(2, 8))
+
+
+def test_parts_beside_another_kernel():
+    from ghost_flow_b200.ops.paged import _parts_beside
+
+    assert [_parts_beside(n, 148) for n in (8, 32, 64, 128, 256, 259, 4000)] == [16, 7, 4, 2, 1, 1, 1]

@@ -42,8 +42,8 @@ def test_attention(kw):
 
 def test_attention_scales_workspaces_and_splits():
     lib = _lib.cuda_lib()
-    need = lib.gf_paged_attn_workspace(2, 5, 0, 64 * 16, 4, 2, 64)
-    assert need > 0 and lib.gf_paged_attn_workspace(2, 5, 0, 1024, 5, 2, 64) == lib.gf_paged_attn_workspace(2, 5, 0, 1024, 4, 2, 96) == -1
+    need = lib.gf_paged_attn_workspace(2, 5, 0, 0, 64 * 16, 4, 2, 64)
+    assert need > 0 and lib.gf_paged_attn_workspace(2, 5, 0, 0, 1024, 5, 2, 64) == lib.gf_paged_attn_workspace(2, 5, 0, 0, 1024, 4, 2, 96) == -1
     for scale in (0.0, -0.1, float("nan")):
         assert lib.gf_paged_attn(_call(), scale, P, need, 0, None, None) == BAD_ARG
     for ws, n in ((P, need - 1), (None, need), (P + 8, need)):
