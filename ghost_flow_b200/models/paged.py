@@ -55,15 +55,21 @@ class PagedKVCache:
         """The batch of ``sequences`` with ``lens`` keys each, of which the last ``new`` (one, without it) are new tokens. Their pages have to be
         reserved."""
         sequences, lens = list(sequences), [int(n) for n in lens]
-        for s, n in zip(sequences, lens):
-            if n > len(self._pages.get(s, ())) * self.page_size:
-                raise ValueError(f"sequence {s!r} has {len(self._pages.get(s, ()))} pages of {self.page_size} rows, not room for {n} keys")
-        B, width = len(lens), max((len(self._pages[s]) for s in sequences), default=0)
-        ints = [p for s in sequences for p in (*self._pages[s], *[-1] * (width - len(self._pages[s])))] + lens
+        new = None if new is None else [int(n) for n in new]
+        if len(sequences) != len(lens) or (new is not None and len(new) != len(lens)):
+            raise ValueError(f"{len(sequences)} sequences, {len(lens)} lengths and {None if new is None else len(new)} numbers of new tokens")
+        pages = [self._pages.get(s, []) for s in sequences]
+        for s, n, m, have in zip(sequences, lens, new or lens, pages):
+            if n > len(have) * self.page_size:
+                raise ValueError(f"sequence {s!r} has {len(have)} pages of {self.page_size} rows, not room for {n} keys")
+            if not 0 <= m <= n:
+                raise ValueError(f"sequence {s!r} has {n} keys, {m} of them new")
+        B, width = len(lens), max(map(len, pages), default=0)
+        ints = [p for have in pages for p in (*have, *[-1] * (width - len(have)))] + lens
         if new is not None:
             ints.append(0)
             for n in new:
-                ints.append(ints[-1] + int(n))
+                ints.append(ints[-1] + n)
         t = torch.tensor(ints, dtype=torch.int32, device=self.device)            # one copy
         return PagedBatch(t[:B * width].view(B, width), t[B * width:B * width + B], t[B * width + B:] if new is not None else None,
                           max(lens, default=0))

@@ -61,6 +61,11 @@ def test_account_of_pages():
     for who, n in (("a", 13), ("c", 1)):
         with pytest.raises(ValueError, match="not room"):
             c.batch([who], [n])
+    for who, lens, new in ((["a"], [3, 4], None), (["a"], [3], [1, 1]), (["a"], [3], [4]), (["a"], [3], [-1]), (["a"], [-1], None)):
+        with pytest.raises(ValueError):
+            c.batch(who, lens, new)
+    empty = c.batch(["nobody", "b"], [0, 8])                  # an empty slot
+    assert empty.lens.tolist() == [0, 8] and empty.table[0].tolist() == [-1, -1]
     c.release("a")
     assert c.free_pages == 3
     one = c.batch(["b"], [4])
