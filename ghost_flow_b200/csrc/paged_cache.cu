@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const __grid_c
 
 using namespace gf;
 
-// x [T, H + 2 Hk, D], y [T, H, D] dense. Tables fp32 [positions, D / 2] dense, on 16-byte boundaries.
+// x [T, H + 2 Hk, D], y [T, H, D] dense. GFH_OVERLAP where x shares memory with the pools. Tables fp32 [positions, D / 2] dense, on 16-byte boundaries.
 GF_API int gf_paged_append(const PagedCall* c, const float* cos, const float* sin, int positions, int interleaved, void* stream) {
   PagedAppend p;
   if (!c || !paged_batch(p.seqs, *c)) return GFH_BAD_ARG;
@@ -126,6 +126,13 @@ GF_API int gf_paged_append(const PagedCall* c, const float* cos, const float* si
   if (H <= 0 || Hk <= 0 || H > 65535 || Hk > 65535 || D < 16 || D % 16 || D / 16 > PA_THREADS || positions < 0 || c->ldy != H * D ||
       !cos || !sin || ((reinterpret_cast<uintptr_t>(cos) | reinterpret_cast<uintptr_t>(sin)) & 15))
     return GFH_BAD_ARG;
+  // new tokens are read while others are written to the pages
+  const char *x0 = (const char*)c->x, *x1 = x0 + 2 * ((c->T - 1) * c->ldx + (H + 2 * Hk) * D);
+  for (int i = 0; i < 2; ++i) {
+    const long long* st = c->strides + 3 * i;
+    const char* pool = (const char*)(i ? c->vpages : c->kpages);
+    if (c->pages > 0 && x0 < pool + 2 * ((c->pages - 1) * st[0] + (c->page - 1) * st[1] + (Hk - 1) * st[2] + D) && pool < x1) return GFH_OVERLAP;
+  }
   gf::enter();
   p.qkv = (const __nv_bfloat16*)c->x; p.ldx = c->ldx;
   p.q = (__nv_bfloat16*)c->y; p.kp = (__nv_bfloat16*)c->kpages; p.vp = (__nv_bfloat16*)c->vpages;

@@ -25,6 +25,7 @@ from .raw import _SLICES, _decode_parts
 
 _INT32, _BF16 = torch.int32, torch.bfloat16
 _MOST = 2 ** 31 - 1
+_OVERLAP = -5      # GFH_OVERLAP of csrc/gf_host.h
 _increment_version = torch.autograd.graph.increment_version
 
 
@@ -180,6 +181,8 @@ def rope_qkv_to_pages(qkv, num_heads: int, num_kv_heads: int, cos, sin, kpages, 
                              f"{list(sin.shape)} on {sin.device}")
         if T == 0 or lens.shape[0] == 0:
             return qkv.new_zeros(T, H, D)
+        if kpages.numel() and not _observed() and (_ranges_overlap(qkv, kpages) or _ranges_overlap(qkv, vpages)):
+            raise ValueError(f"{what}: qkv shares memory with the pages")
         return _append_ref(qkv, H, Hk, cos, sin, kpages, vpages, page_table, lens, cu, interleaved)
     stream = _lib.stream_on(device)
     if stream is None:
@@ -190,10 +193,13 @@ def rope_qkv_to_pages(qkv, num_heads: int, num_kv_heads: int, cos, sin, kpages, 
         x = qkv.clone(memory_format=torch.contiguous_format)
         ld, at = G * D, x.data_ptr()
     q = qkv.new_empty((T, H, D))
-    _rc(_lib.cuda_lib().gf_paged_append(
+    rc = _lib.cuda_lib().gf_paged_append(
         _CALL(at, ld, q.data_ptr(), H * D, *pools, page_table.data_ptr(), page_table.stride(0), width, lens.data_ptr(),
               0 if cu is None else cu.data_ptr(), B, T, H, Hk, D, page, P, _lib.status_ptr(device)),
-        cos.data_ptr(), sin.data_ptr(), n, 1 if interleaved else 0, stream), "gf_paged_append")
+        cos.data_ptr(), sin.data_ptr(), n, 1 if interleaved else 0, stream)
+    if rc == _OVERLAP:
+        raise ValueError("rope_qkv_to_pages: qkv shares memory with the pages")
+    _rc(rc, "gf_paged_append")
     _increment_version((kpages, vpages))     # a graph that saved the pools has to notice the write
     return q
 
@@ -262,7 +268,8 @@ def _ranges_overlap(a, b) -> bool:
 def paged_attention(q, kpages, vpages, page_table, lens, cu=None, scale: float | None = None, out=None):
     """Causal attention of new tokens ``q [T, Hq, D]`` over the keys of their sequences in the pages (see the module), which hold the new
     tokens' own already: a token at position ``p`` sees the keys ``0 .. p``. A token that sees none gives zeros; tokens behind
-    the last sequence are not written. What the pages hold behind a sequence's last key does not matter. ``out [T, Hq, D]``, where given, is
+    the last sequence are not written. What the pages hold behind a sequence's last key does not matter; a value of a new token
+    that is not finite may reach those in front of it as well. ``out [T, Hq, D]``, where given, is
     written and returned. A page that is not in the pools reads as zeros, keys behind the page table do not exist, and
     ``_lib.check_status`` raises for both. Head sizes 64 and 128 with pages of a power of two from 16 rows take the kernels.
     Inference only: a call with a gradient to record takes PyTorch's operations."""

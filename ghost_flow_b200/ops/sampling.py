@@ -88,6 +88,9 @@ def _check(logits, tokens, token_lens, generated_from, repetition, presence, fre
         inplace = out is logits or (out.data_ptr() == logits.data_ptr() and out.stride() == logits.stride())
         if not inplace and logits.numel() and _ranges_overlap(out, logits):
             raise ValueError(f"{what}: out shares memory with logits and is not logits")
+        for name, t in (("bias", bias), ("allowed", allowed), ("tokens", tokens)):
+            if t is not None and t.numel() and out.numel() and _ranges_overlap(out, t):
+                raise ValueError(f"{what}: out shares memory with {name}")
 
 
 def _row(t, B, device, dtype) -> bool:
@@ -129,6 +132,9 @@ def _for_kernel(x, tokens, token_lens, generated_from, repetition, presence, fre
             return None
         if not (out.data_ptr() == x.data_ptr() and out.stride(0) == ld) and _ranges_overlap(out, x):
             return None
+        for t in (bias, allowed, tokens):
+            if t is not None and t.numel() and _ranges_overlap(out, t):
+                return None
     return device, B, V, ld
 
 

@@ -117,6 +117,14 @@ def test_projections_and_tables_that_are_refused(kw):
         ops.rope_qkv_to_pages(s["qkv"], a["H"], a["Hk"], a["cos"], a["sin"], s["kp"], s["vp"], s["table"], s["lens"], s["cu"])
 
 
+def test_projections_in_the_pages_are_refused():
+    s = oracle.batch([7, 20], [1, 2], 4, 2, 16, 16, torch.float32)
+    cos, sin = ops.rope_tables(64, 16, 1e4)
+    for pool in (s["kp"], s["vp"]):
+        with pytest.raises(ValueError, match="shares memory"):
+            ops.rope_qkv_to_pages(pool.reshape(-1)[:3 * 8 * 16].view(3, 8, 16), 4, 2, cos, sin, s["kp"], s["vp"], s["table"], s["lens"], s["cu"])
+
+
 @pytest.mark.parametrize("change", [lambda s: s["table"].__setitem__((1, 1), 99), lambda s: s["table"].__setitem__((1, 1), -1),
                                     lambda s: s["lens"].__setitem__(1, 60)], ids=["page behind", "page below", "length behind the table"])
 def test_pages_and_positions_that_are_not_there(change):
@@ -207,6 +215,12 @@ def test_out_that_overlaps_the_logits_is_refused():
     t = torch.zeros(40)
     with pytest.raises(ValueError, match="shares memory"):
         ops.process_logits(t[:16].view(2, 8), out=t[8:24].view(2, 8))
+
+
+def test_out_that_overlaps_what_else_is_read_is_refused():
+    t = torch.zeros(2, 8)
+    with pytest.raises(ValueError, match="shares memory with bias"):
+        ops.process_logits(torch.zeros(2, 8), bias=t, out=t)
 
 
 def test_parts_beside_another_kernel():

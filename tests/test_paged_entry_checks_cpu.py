@@ -26,6 +26,12 @@ def test_append(kw):
     assert _lib.cuda_lib().gf_paged_append(_call(**kw), P, P, 100, 0, None) == BAD_ARG
 
 
+# x: 5 rows 512 apart, the last of 8 x 64; the pools: 9 pages of 16 rows of 128
+@pytest.mark.parametrize("kw", [dict(), dict(kp=P + 2 * 2560 - 16, vp=1 << 30), dict(vp=P - 2 * 18432 + 16, kp=1 << 30)], ids=str)
+def test_append_of_tokens_that_lie_in_the_pools(kw):
+    assert _lib.cuda_lib().gf_paged_append(_call(**kw), P, P, 100, 0, None) == -5
+
+
 @pytest.mark.parametrize("cos,sin,n", [(None, P, 9), (P, None, 9), (P + 4, P, 9), (P, P + 8, 9), (P, P, -1)])
 def test_append_tables(cos, sin, n):
     assert _lib.cuda_lib().gf_paged_append(_call(), cos, sin, n, 0, None) == BAD_ARG
