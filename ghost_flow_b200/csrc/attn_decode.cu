@@ -516,7 +516,7 @@ attn_decode_kernel(const __grid_constant__ DecParams p) {
         }
       }
       if (whole) {
-        to[i] = __float2bfloat16(ll > 0.f ? ov / ll : 0.f);
+        to[i] = __float2bfloat16(ll > 0.f || (PAGED && ll != ll) ? ov / ll : 0.f);       // over pages what is not a number stays so
       } else {
         slot[g * (D + 2) + d] = ov;
         if (d == 0) {
@@ -616,7 +616,7 @@ __global__ void __launch_bounds__(D) attn_decode_merge_kernel(const __grid_const
       o += x[k] * e;
       t += l[k] * e;
     }
-    p.out[at_row * p.ldo + (long long)h * D + d] = __float2bfloat16(t > 0.f ? o / t : 0.f);
+    p.out[at_row * p.ldo + (long long)h * D + d] = __float2bfloat16(t > 0.f || (p.pages.lens && t != t) ? o / t : 0.f);
     return;
   }
   float mm = -INFINITY;
@@ -653,7 +653,7 @@ __global__ void __launch_bounds__(D) attn_decode_merge_kernel(const __grid_const
   l = 0.f;
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) l += share[i];
-  p.out[at_row * p.ldo + (long long)h * D + d] = __float2bfloat16(l > 0.f ? o / l : 0.f);
+  p.out[at_row * p.ldo + (long long)h * D + d] = __float2bfloat16(l > 0.f || (p.pages.lens && l != l) ? o / l : 0.f);
 }
 
 template <int D, int KIND>

@@ -705,7 +705,7 @@ __global__ void __launch_bounds__(256, 4) paged_join_kernel(const __grid_constan
     for (int e = 0; e < PG_COLS; ++e) o[e] *= old;
 #pragma unroll
     for (int i = 0; i < PG_AHEAD; ++i) {
-      if (!(x[i].y > 0.f)) continue;                       // 0 times what may be anything
+      if (x[i].y == 0.f) continue;                         // 0 times what may be anything
       const float w = ex2_approx(x[i].x - use);
       l += x[i].y * w;
 #pragma unroll

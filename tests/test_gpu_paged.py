@@ -363,3 +363,41 @@ def test_gradients_of_shared_heads_on_the_device():
         # 32 bits: sums of at most 40 products of numbers of this size; bf16: the products' inputs and results are rounded, and grads once more
         assert (single.double() - exact).norm() <= 64 * 2 ** -24 * 16 * exact.norm()
         assert (half.double() - exact).norm() <= 8 * 2 ** -8 * exact.norm()
+
+
+@pytest.mark.parametrize("H,Hk,D", [(4, 2, 64), (16, 1, 128), (20, 1, 128)])
+@pytest.mark.parametrize("lens,new", [([40, 90], [1, 1]), ([3000, 70], [1, 1]), ([300] * 40, [1] * 40), ([130, 70], [130, 70]), ([5000, 300], [3, 100]),
+                                      ([2000, 30, 50, 60, 64, 5, 80, 90, 700], [200, 1, 1, 1, 1, 1, 1, 1, 2])], ids=str)
+def test_what_is_not_a_number_stays_so_and_where_it_is(lens, new, H, Hk, D, kernel_status):
+    """A query that is not a number gives a row that is not, one of the keys every row that sees it; all other rows are as they were."""
+    s = oracle.batch(lens, new, H, Hk, D, 16, device="cuda")
+    one = set(new) == {1}
+    want = _attend(s, cu=not one)
+    t = sum(new[:2]) - 1                                 # the last token of the second sequence
+    q = s["q"].clone()
+    s["q"][t, H - 1, 5] = float("nan")
+    got = _attend(s, cu=not one)
+    assert got[t, H - 1].isnan().all()
+    got[t, H - 1] = want[t, H - 1]
+    assert torch.equal(got, want)
+    s["q"] = q
+    at = lens[0] // 2                                    # a key of the first sequence
+    s["kp"][int(s["table"][0, at // 16]), at % 16, 0, 7] = float("nan")
+    got = _attend(s, cu=not one)
+    sees = torch.zeros(len(want), H, dtype=torch.bool, device="cuda")
+    sees[max(0, at - (lens[0] - new[0])):new[0], :H // Hk] = True
+    assert got[sees].isnan().all()
+    got[sees] = want[sees]
+    assert torch.equal(got, want)
+
+
+def test_projections_in_the_pages_are_refused(kernel_status):
+    from ghost_flow_b200 import ops
+
+    s = oracle.batch([7, 20], [1, 2], 4, 2, 64, 16, device="cuda")
+    cos, sin = ops.rope_tables(64, 64, 1e4, "cuda")
+    for pool in (s["kp"], s["vp"]):
+        before = pool.nan_to_num(1, 2, 3)
+        with pytest.raises(ValueError, match="shares memory"):
+            ops.rope_qkv_to_pages(pool.view(-1)[:3 * 8 * 64].view(3, 8, 64), 4, 2, cos, sin, s["kp"], s["vp"], s["table"], s["lens"], s["cu"])
+        assert torch.equal(pool.nan_to_num(1, 2, 3), before)
