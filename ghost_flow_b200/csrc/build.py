@@ -3,6 +3,7 @@
 ``libgfb200.so``   - every CUDA kernel (sm_100a only) behind a C ABI, loaded with ctypes.
 ``libghostflow.so`` - the C ABI of the reference's ``ghostflow.h`` plus the checkpoint
                       readers/writers (host C++ only, no CUDA needed to load it).
+``_gf_calls.so``    - Python module through which operators of short calls reach ``libgfb200.so``.
 
 Usage: ``python -m ghost_flow_b200.csrc.build [--force] [--verbose]``.
 """
@@ -14,6 +15,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
@@ -57,6 +59,7 @@ CUDA_SOURCES = [
     "runtime.cu",
 ]
 
+PYTHON_SOURCES = ["calls.cpp"]
 HOST_SOURCES = ["cabi.cpp", "formats.cpp", "cpu_ref.cpp", "symm_alloc.cpp"]
 
 
@@ -101,7 +104,7 @@ def build(force: bool = False, verbose: bool = False, checked: bool = True) -> d
     OBJ_DIR.mkdir(exist_ok=True)
     nvcc = _nvcc()
     jobs = []
-    cuda_objs, host_objs, checked_objs = [], [], []
+    cuda_objs, host_objs, checked_objs, python_objs = [], [], [], []
     for name in CUDA_SOURCES:
         src = HERE / name
         if not src.exists():
@@ -128,6 +131,11 @@ def build(force: bool = False, verbose: bool = False, checked: bool = True) -> d
                "-c", str(src), "-o", str(obj)]
         jobs.append((cmd, src, obj))
         host_objs.append(obj)
+    for name in PYTHON_SOURCES:
+        src, obj = HERE / name, OBJ_DIR / (name + ".o")
+        jobs.append((["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-I", str(HERE), "-I", sysconfig.get_paths()["include"],
+                      "-c", str(src), "-o", str(obj)], src, obj))
+        python_objs.append(obj)
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 2)) as ex:
         futs = []
         for cmd, src, obj in jobs:
@@ -168,6 +176,12 @@ def build(force: bool = False, verbose: bool = False, checked: bool = True) -> d
             if r.returncode != 0:
                 raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
         out["host"] = lib
+    lib = LIB_DIR / "_gf_calls.so"
+    if force or not lib.exists() or lib.stat().st_mtime < max(o.stat().st_mtime for o in python_objs):
+        r = subprocess.run(["g++", "-shared", "-o", str(lib), *map(str, python_objs)], capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    out["python"] = lib
     return out
 
 

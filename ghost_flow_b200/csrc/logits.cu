@@ -20,6 +20,7 @@
 // of a thread at a time, without the ring, took 95; two CTAs of 512 threads on an SM and longer rings 57. Small batches: 64 rows 11 us, two or three 4.
 #include <cuda_fp16.h>
 
+#include "calls.h"
 #include "gf_host.h"
 #include "gf_ptx.cuh"
 
@@ -266,23 +267,6 @@ static int launch_logits(LogitsParams& p, long long B, cudaStream_t st) {
 }  // namespace gf
 
 using namespace gf;
-
-// 8 bytes each, as in PagedCall.
-struct LogitsCall {
-  const void* x;                 // [B, V] of dtype (0 fp32, 1 bf16, 2 fp16), rows ldx apart
-  long long ldx;
-  void* y;                       // alike; may be x
-  long long ldy, dtype, B, V;
-  const void* tokens;
-  long long ldt, tokens64, L;
-  const int *token_lens, *generated_from;
-  const float *repetition, *presence, *frequency;
-  double repetition0, presence0, frequency0;
-  const float* bias;
-  long long ldb;
-  const unsigned* allowed;
-  long long lda;
-};
 
 GF_API int gf_process_logits(const LogitsCall* c, void* stream) {
   constexpr long long MOST = 0x7fffffff;

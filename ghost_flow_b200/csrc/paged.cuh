@@ -5,6 +5,7 @@
 // table[b, p / page]. Everything that comes out of device memory is bounded before it is used as an address: page numbers and positions
 // that are not there are reported in the status word (GF_ERR_BAD_ARG), never read or written.
 #pragma once
+#include "calls.h"
 #include "gf_host.h"
 #include "gf_ptx.cuh"
 
@@ -37,21 +38,6 @@ __device__ __forceinline__ int paged_seq_of(const PagedBatch& s, int t) {
   }
   return b;
 }
-
-// What the entry points take: tensors as addresses, sizes and strides in elements, 8 bytes each so that a caller in any language can pack them.
-struct PagedCall {
-  const void* x;                 // new tokens: [T, heads, D], heads packed, rows ldx apart
-  long long ldx;
-  void* y;                       // result: [T, H, D], rows ldy apart
-  long long ldy;
-  void *kpages, *vpages;         // [pages, page, Hk, D]
-  long long strides[6];          // pages, rows and heads of kpages, then of vpages
-  const int* table;
-  long long ld_table, width;
-  const int *lens, *cu;
-  long long B, T, H, Hk, D, page, pages;
-  int* status;
-};
 
 // Host: the batch of a call; false where the kernels do not take it: sizes, pages of other than a power of two from 16 rows, and rows of x, y
 // and the pools that are not on 16-byte boundaries.

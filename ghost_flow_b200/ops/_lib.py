@@ -6,6 +6,8 @@ silently falling back, so a missing or stale build can never hide behind PyTorch
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 import threading
 from ctypes import c_float, c_int, c_longlong, c_void_p
@@ -125,6 +127,30 @@ def cuda_lib():
             )
         _CUDA_LIB = _bind(ctypes.CDLL(str(path), mode=ctypes.RTLD_GLOBAL), _SIGS)
     return _CUDA_LIB
+
+
+_CALLS = None
+
+
+def calls():
+    """The Python module that looks at an operator's tensors and launches on ``libgfb200.so`` (``csrc/calls.cpp``); both are built if missing."""
+    global _CALLS
+    if _CALLS is None:
+        lib, path = cuda_lib(), _PKG / "lib" / "_gf_calls.so"
+        if not path.exists():
+            from ..csrc.build import build
+
+            build()
+        exchange = getattr(torch.Tensor, "__dlpack_c_exchange_api__", None)
+        if exchange is None:
+            raise RuntimeError("this PyTorch has no DLPack C exchange interface (version 2.10 and later have it)")
+        loader = importlib.machinery.ExtensionFileLoader("_gf_calls", str(path))
+        module = importlib.util.module_from_spec(importlib.util.spec_from_file_location("_gf_calls", str(path), loader=loader))
+        loader.exec_module(module)
+        module.bind(exchange, *(ctypes.cast(getattr(lib, name), c_void_p).value for name in (
+            "gf_paged_append", "gf_paged_attn", "gf_paged_attn_one", "gf_process_logits")))
+        _CALLS = module
+    return _CALLS
 
 
 def launch_count() -> int:

@@ -14,17 +14,15 @@ from __future__ import annotations
 
 import functools
 import math
-import struct
 
 import torch
 
 from . import _lib
-from .fused import _observed, _rc, _rope_tables_fit_kernel, _rows_apart
+from .fused import _observed, _rc, _rows_apart
 from .gemm import _SMS, _sm_count
 from .raw import _SLICES, _decode_parts
 
 _INT32, _BF16 = torch.int32, torch.bfloat16
-_MOST = 2 ** 31 - 1
 _OVERLAP = -5      # GFH_OVERLAP of csrc/gf_host.h
 _increment_version = torch.autograd.graph.increment_version
 
@@ -62,40 +60,10 @@ def _pages_apart(P, page, Hk, D, pools) -> bool:
     return all(_rows_apart(D, d) for d in dims) and ends[0][1] <= ends[1][0]
 
 
-# the PagedCall of csrc/paged.cuh
-_CALL = struct.Struct("25q").pack
-
-
-def _for_kernels(x, kpages, vpages, page_table, lens, cu):
-    """What a kernel call needs to know of a batch that the kernels take, in few looks at the tensors (a call for one token of a small
-    model is all host time): its device, the sizes of the batch and the pools, and the pools' addresses and strides. ``None``:
-    see :func:`_check_batch` for why."""
-    dev = x.get_device()
-    if dev < 0 or x.dtype is not _BF16 or kpages.dtype is not _BF16 or vpages.dtype is not _BF16 or page_table.dtype is not _INT32 \
-            or lens.dtype is not _INT32 or not dev == kpages.get_device() == vpages.get_device() == page_table.get_device() == lens.get_device():
-        return None
-    shape = kpages.shape
-    try:
-        (P, page, Hk, D), (B,), (Bt, width) = shape, lens.shape, page_table.shape
-    except ValueError:
-        return None
-    if vpages.shape != shape or Bt != B or B == 0 or not page_table.stride(1) == 1 == lens.stride(0) or x.dim() != 3:
-        return None
-    if cu is None:
-        if x.shape[0] != B:
-            return None
-    elif cu.dtype is not _INT32 or cu.get_device() != dev or cu.dim() != 1 or cu.shape[0] != B + 1 or cu.stride(0) != 1:
-        return None
-    a0, a1, a2, a3 = kpages.stride()
-    b0, b1, b2, b3 = vpages.stride()
-    if P == 0 or Hk == 0 or page < 16 or page & (page - 1) or P * page > _MOST or width > _MOST // page or not a3 == 1 == b3 \
-            or (a0 | a1 | a2 | b0 | b1 | b2) & 7 or _observed() \
-            or (torch.is_grad_enabled() and (x.requires_grad or kpages.requires_grad or vpages.requires_grad)):
-        return None
-    k, v = kpages.data_ptr(), vpages.data_ptr()        # behind _observed: transformed tensors have no memory
-    if (k | v) & 15:
-        return None
-    return dev, B, width, P, page, Hk, D, (k, v, a0, a1, a2, b0, b1, b2)
+def _launches(x, kpages, vpages) -> bool:
+    """Whether a call on these may be a kernel's: CUDA tensors, and nothing that follows it."""
+    return x.get_device() >= 0 and not _observed() and not (
+        torch.is_grad_enabled() and (x.requires_grad or kpages.requires_grad or vpages.requires_grad))
 
 
 def _report(device, bad, what: str) -> None:
@@ -159,16 +127,12 @@ def rope_qkv_to_pages(qkv, num_heads: int, num_kv_heads: int, cos, sin, kpages, 
     or a position that is not in the tables or behind the page table, is left out too, and ``_lib.check_status`` raises.
     Inference only: a call with a gradient to record takes PyTorch's operations."""
     H, Hk = num_heads, num_kv_heads
-    fits = _for_kernels(qkv, kpages, vpages, page_table, lens, cu)
-    if fits is not None:
-        device, B, width, P, page, heads, D, pools = fits
-        T, G, Dx = qkv.shape
-        tables = cos.shape
-        n = tables[0] if len(tables) == 2 and tables[1] * 2 == D and sin.shape == tables and device == cos.get_device() == sin.get_device() else -1
-        if not (heads == Hk > 0 < H and G == H + 2 * Hk and Dx == D and D % 16 == 0 and D <= 4096 and T > 0 and n >= 0
-                and _rope_tables_fit_kernel(cos, sin) and _pages_apart(P, page, Hk, D, pools)):
-            fits = None
-    if fits is None:
+    call = None
+    if _launches(qkv, kpages, vpages):
+        call = _lib.calls().append(qkv, H, Hk, kpages, vpages, page_table, lens, cu, cos, sin)
+        if call is not None and call[5] is not None and not _pages_apart(*kpages.shape, call[5]):
+            call = None
+    if call is None:
         what = "rope_qkv_to_pages"
         if qkv.dim() != 3 or qkv.shape[1] != H + 2 * Hk or H < 1 or Hk < 1:
             raise ValueError(f"{what}: a packed projection of {H} + 2 x {Hk} heads is [tokens, {H + 2 * Hk}, head size], not {list(qkv.shape)}")
@@ -184,19 +148,16 @@ def rope_qkv_to_pages(qkv, num_heads: int, num_kv_heads: int, cos, sin, kpages, 
         if kpages.numel() and not _observed() and (_ranges_overlap(qkv, kpages) or _ranges_overlap(qkv, vpages)):
             raise ValueError(f"{what}: qkv shares memory with the pages")
         return _append_ref(qkv, H, Hk, cos, sin, kpages, vpages, page_table, lens, cu, interleaved)
+    at, device, T, D, packed, _ = call
     stream = _lib.stream_on(device)
     if stream is None:
         with torch.cuda.device(device):
             return rope_qkv_to_pages(qkv, H, Hk, cos, sin, kpages, vpages, page_table, lens, cu, interleaved)
-    x, (ld, sh, se), at = qkv, qkv.stride(), qkv.data_ptr()
-    if se != 1 or sh != D or ld % 8 or at % 16:
-        x = qkv.clone(memory_format=torch.contiguous_format)
-        ld, at = G * D, x.data_ptr()
+    if not packed:
+        qkv = qkv.clone(memory_format=torch.contiguous_format)
+        at = _lib.calls().append(qkv, H, Hk, kpages, vpages, page_table, lens, cu, cos, sin)[0]
     q = qkv.new_empty((T, H, D))
-    rc = _lib.cuda_lib().gf_paged_append(
-        _CALL(at, ld, q.data_ptr(), H * D, *pools, page_table.data_ptr(), page_table.stride(0), width, lens.data_ptr(),
-              0 if cu is None else cu.data_ptr(), B, T, H, Hk, D, page, P, _lib.status_ptr(device)),
-        cos.data_ptr(), sin.data_ptr(), n, 1 if interleaved else 0, stream)
+    rc = _lib.calls().run_append(at, q, interleaved, _lib.status_ptr(device), stream)
     if rc == _OVERLAP:
         raise ValueError("rope_qkv_to_pages: qkv shares memory with the pages")
     _rc(rc, "gf_paged_append")
@@ -273,19 +234,15 @@ def paged_attention(q, kpages, vpages, page_table, lens, cu=None, scale: float |
     written and returned. A page that is not in the pools reads as zeros, keys behind the page table do not exist, and
     ``_lib.check_status`` raises for both. Head sizes 64 and 128 with pages of a power of two from 16 rows take the kernels.
     Inference only: a call with a gradient to record takes PyTorch's operations."""
-    fits = _for_kernels(q, kpages, vpages, page_table, lens, cu)
-    if fits is not None:
-        device, B, width, P, page, Hk, D, pools = fits
-        T, H, Dx = q.shape
-        if not (T > 0 and Dx == D and (D == 128 or D == 64) and H > 0 and H % Hk == 0 and H // Hk <= 128 and 0 not in pools[2:]):
-            fits = None
-        elif out is not None:
-            st = out.stride()
+    call, what = None, "paged_attention"
+    if _launches(q, kpages, vpages):
+        call = _lib.calls().attention(q, kpages, vpages, page_table, lens, cu)
+        if call is not None and out is not None:
+            H, D, st = call[4], call[6], out.stride()
             if out.shape != q.shape or out.dtype is not _BF16 or out.device != q.device or st[2] != 1 or st[1] != D or st[0] % 8 \
                     or st[0] < H * D or out.data_ptr() % 16 or (out.requires_grad and torch.is_grad_enabled()):
-                fits = None
-    what = "paged_attention"
-    if fits is None:
+                call = None
+    if call is None:
         if q.dim() != 3:
             raise ValueError(f"{what}: q is [tokens, heads, head size], not {list(q.shape)}")
         _check_batch(what, q, kpages, vpages, page_table, lens, cu)
@@ -297,12 +254,14 @@ def paged_attention(q, kpages, vpages, page_table, lens, cu=None, scale: float |
             raise ValueError(f"{what}: out is {list(q.shape)} of {q.dtype} on {q.device}, not {list(out.shape)} of {out.dtype} on {out.device}")
         if T == 0:
             return torch.empty_like(q) if out is None else out
+    else:
+        at, device, B, T, H, Hk, D, keys, packed = call
     if out is not None and (_ranges_overlap(out, q) or _ranges_overlap(out, kpages) or _ranges_overlap(out, vpages)):
         raise ValueError(f"{what}: out shares memory with q or the pages")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not math.isfinite(scale):
         raise ValueError(f"{what}: a scale of {scale}")
-    if fits is None:
+    if call is None:
         return _attention_ref(q, kpages, vpages, page_table, lens, cu, scale, out)
     stream = _lib.stream_on(device)
     if stream is None:
@@ -313,31 +272,23 @@ def paged_attention(q, kpages, vpages, page_table, lens, cu=None, scale: float |
     one = cu is None and groups > 0
     x = q
     if not scale > 0 and not one:            # this kernel takes the largest score before it scales
-        x, scale = q * (-1 if scale < 0 else 0), -scale if scale < 0 else 1.0
-    (ld, sh, se), at = x.stride(), x.data_ptr()
-    if se != 1 or sh != D or ld % 8 or at % 16 or ld < H * D:
-        x = x.clone(memory_format=torch.contiguous_format)
-        ld, at = H * D, x.data_ptr()
-    if out is not None:
-        o, ldo = out, out.stride(0)
-    else:
-        o, ldo = torch.empty_like(x) if ld == H * D else q.new_empty((T, H, D)), H * D
-    call = _CALL(at, ld, o.data_ptr(), ldo, *pools, page_table.data_ptr(), page_table.stride(0), width, lens.data_ptr(),
-                 0 if cu is None else cu.data_ptr(), B, T, H, Hk, D, page, P, _lib.status_ptr(device))
-    parts, few = 0, None
+        x, scale = (q * (-1 if scale < 0 else 0)).contiguous(), -scale if scale < 0 else 1.0
+    elif not packed:
+        x = q.clone(memory_format=torch.contiguous_format)
+    if x is not q:
+        at = _lib.calls().attention(x, kpages, vpages, page_table, lens, cu)[0]
+    o = out if out is not None else torch.empty_like(x) if x.is_contiguous() else q.new_empty((T, H, D))
+    parts, few, ws = 0, None, None
     if one or (cu is not None and B >= _MANY and groups):
         sms = _SMS.get(device) or _sm_count(q.device)
-        parts = _decode_parts(B, Hk * groups, width * page, D, sms, True) if one else _parts_beside(B * Hk * groups, sms)
+        parts = _decode_parts(B, Hk * groups, keys, D, sms, True) if one else _parts_beside(B * Hk * groups, sms)
         if parts != 1:
             few = torch.empty((B * parts if parts > 0 else -2 * parts) * H * (D + 2), dtype=torch.float32, device=q.device)
-    few_at = None if few is None else few.data_ptr()
-    if one:
-        _rc(_lib.cuda_lib().gf_paged_attn_one(call, scale, parts, few_at, stream), "gf_paged_attn_one")
-    else:
-        nbytes = _attention_workspace(device, B, T, cu is None, parts != 0, width * page, H, Hk, D)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-        _rc(_lib.cuda_lib().gf_paged_attn(call, scale, None if ws is None else ws.data_ptr(), nbytes, parts, few_at, stream),
-            "gf_paged_attn")
+    if not one:
+        nbytes = _attention_workspace(device, B, T, cu is None, parts != 0, keys, H, Hk, D)
+        if nbytes:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    _rc(_lib.calls().run_attention(at, o, scale, one, ws, parts, few, _lib.status_ptr(device), stream), "gf_paged_attn")
     if out is not None:
         _increment_version(out)
     return o

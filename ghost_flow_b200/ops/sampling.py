@@ -5,17 +5,11 @@ CUDA logits of fp32, bf16 or fp16 take the kernel of ``csrc/logits.cu``; CPU ten
 gradient, tracing, transforms, modes) plain PyTorch."""
 from __future__ import annotations
 
-import struct
-
 import torch
 
 from . import _lib
 from .fused import _observed, _rc
 from .paged import _ranges_overlap
-
-_CALL = struct.Struct("16q3d4q").pack      # the LogitsCall of csrc/logits.cu
-_WHOLE = (torch.int32, torch.int64)
-_KINDS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
 def pack_allowed(mask):
@@ -93,49 +87,18 @@ def _check(logits, tokens, token_lens, generated_from, repetition, presence, fre
                 raise ValueError(f"{what}: out shares memory with {name}")
 
 
-def _row(t, B, device, dtype) -> bool:
-    return t.dtype is dtype and t.get_device() == device and t.dim() == 1 and t.shape[0] == B and t.stride(0) == 1
-
-
-def _for_kernel(x, tokens, token_lens, generated_from, repetition, presence, frequency, bias, allowed, out):
-    """Device, rows, vocabulary and distance of rows of a call that the kernel takes, in few looks at the tensors. ``None``: see :func:`_check`."""
-    device = x.get_device()
-    if device < 0 or x.dim() != 2 or x.dtype not in _KINDS or _observed():
-        return None
-    (B, V), (ld, one) = x.shape, x.stride()
-    if B == 0 or V == 0 or one != 1:
-        return None
-    if tokens is not None:
-        if tokens.dim() != 2 or tokens.shape[0] != B or tokens.dtype not in _WHOLE or tokens.get_device() != device or tokens.stride(1) != 1 \
-                or not (token_lens is None or _row(token_lens, B, device, torch.int32)) \
-                or not (generated_from is None or _row(generated_from, B, device, torch.int32)):
-            return None
-    elif token_lens is not None or generated_from is not None:
-        return None
-    grad = torch.is_grad_enabled()
-    if grad and x.requires_grad:
-        return None
-    for t in (repetition, presence, frequency):
-        if type(t) is not float and torch.is_tensor(t) and (not _row(t, B, device, torch.float32) or (grad and t.requires_grad)):
-            return None
-    if not torch.is_tensor(repetition) and not repetition > 0:
-        return None
-    if bias is not None and (bias.dtype is not torch.float32 or bias.get_device() != device or bias.shape not in ((V,), (B, V))
-                             or bias.stride(-1) != 1 or (grad and bias.requires_grad)):
-        return None
-    if allowed is not None and (allowed.dtype is not torch.int32 or allowed.get_device() != device or allowed.stride(-1) != 1
-                                or allowed.shape not in (((V + 31) // 32,), (B, (V + 31) // 32))):
-        return None
-    if out is not None:
-        if out.shape != x.shape or out.dtype is not x.dtype or out.get_device() != device or out.stride(1) != 1 \
-                or (B > 1 and out.stride(0) < V) or (grad and out.requires_grad):
-            return None
-        if not (out.data_ptr() == x.data_ptr() and out.stride(0) == ld) and _ranges_overlap(out, x):
-            return None
-        for t in (bias, allowed, tokens):
-            if t is not None and t.numel() and _ranges_overlap(out, t):
-                return None
-    return device, B, V, ld
+def _launches(x, out, others) -> bool:
+    """Whether a call on these may be the kernel's: CUDA tensors, nothing that follows it, and a place for the result that the kernel takes."""
+    if x.get_device() < 0 or x.dim() != 2 or _observed():
+        return False
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, out, *others) if t is not None and type(t) is not float and torch.is_tensor(t)):
+        return False
+    if out is None:
+        return True
+    return (out.shape == x.shape and out.dtype is x.dtype and out.device == x.device and out.stride(1) == 1
+            and (x.shape[0] <= 1 or out.stride(0) >= x.shape[1])
+            and ((out.data_ptr() == x.data_ptr() and out.stride() == x.stride()) or not _ranges_overlap(out, x))
+            and not any(torch.is_tensor(t) and t.numel() and _ranges_overlap(out, t) for t in others))
 
 
 def process_logits(logits, tokens=None, token_lens=None, generated_from=None, repetition=1.0, presence=0.0, frequency=0.0, bias=None,
@@ -148,14 +111,16 @@ def process_logits(logits, tokens=None, token_lens=None, generated_from=None, re
     (int32 ``[B]``; 0) are generated ones, those before them the prompt; a token outside the vocabulary (padding) is passed over. The
     three penalties are numbers or fp32 ``[B]``. ``bias``: fp32 ``[V]`` or ``[B, V]``. ``allowed``: int32 bits ``[words]`` or ``[B, words]``
     (:func:`pack_allowed`). ``out`` may be ``logits`` itself. A row of which nothing is allowed is all ``-inf``."""
-    call = _for_kernel(logits, tokens, token_lens, generated_from, repetition, presence, frequency, bias, allowed, out)
+    call = None
+    if _launches(logits, out, (repetition, presence, frequency, bias, tokens, allowed)):
+        call = _lib.calls().logits(logits, tokens, token_lens, generated_from, repetition, presence, frequency, bias, allowed)
     if call is None:
         _check(logits, tokens, token_lens, generated_from, repetition, presence, frequency, bias, allowed, out)
         if logits.numel() == 0:
             return torch.empty_like(logits) if out is None else out
         y = _logits_ref(logits, tokens, token_lens, generated_from, repetition, presence, frequency, bias, allowed)
         return y if out is None else out.copy_(y)
-    device, B, V, ld = call
+    at, device, B, V, ld = call
     stream = _lib.stream_on(device)
     if stream is None:
         with torch.cuda.device(device):
@@ -166,18 +131,7 @@ def process_logits(logits, tokens=None, token_lens=None, generated_from=None, re
         # rows as far apart as they are, where they are apart: they then begin on the same boundaries
         ldy = ld if V <= ld < V + 64 else V
         y = torch.empty_strided((B, V), (ldy, 1), dtype=logits.dtype, device=logits.device)
-    r, p, f = (t if type(t) is float else None if torch.is_tensor(t) else float(t) for t in (repetition, presence, frequency))
-    if tokens is None:
-        t, ldt, wide, L = 0, 0, 0, 0
-    else:
-        t, ldt, wide, L = tokens.data_ptr(), tokens.stride(0), tokens.dtype is torch.int64, tokens.shape[1]
-    _rc(_lib.cuda_lib().gf_process_logits(_CALL(
-        logits.data_ptr(), ld, y.data_ptr(), ldy, _KINDS[logits.dtype], B, V, t, ldt, wide, L,
-        0 if token_lens is None else token_lens.data_ptr(), 0 if generated_from is None else generated_from.data_ptr(),
-        repetition.data_ptr() if r is None else 0, presence.data_ptr() if p is None else 0, frequency.data_ptr() if f is None else 0,
-        r or 0.0, p or 0.0, f or 0.0, 0 if bias is None else bias.data_ptr(), 0 if bias is None or bias.dim() == 1 else bias.stride(0),
-        0 if allowed is None else allowed.data_ptr(), 0 if allowed is None or allowed.dim() == 1 else allowed.stride(0)), stream),
-        "gf_process_logits")
+    _rc(_lib.calls().run_logits(at, y, ldy, stream), "gf_process_logits")
     if out is not None:
         torch.autograd.graph.increment_version(out)
     return y
