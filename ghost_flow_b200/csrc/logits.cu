@@ -9,15 +9,15 @@
 //   x = x + bias[v]
 //   x = allowed ? x : -inf                                   all in 32 bits, rounded once
 //
-// One CTA has a slice of one row. The row's tokens, each with a thread, set a bit for the entry that they hold and count themselves; then a pass
-// over the slice, 16 bytes at a time, does the arithmetic, whose first vectors were asked for before the tokens were looked at. An
-// entry's counter, later what is taken off it, lies at its rank among the set bits (those of the words in front, counted once, and of its own word):
-// there are no more of them than tokens, so that a slice may be long, and a CTA looks at all tokens of its row whatever its slice is; entries
-// of one vector have ranks one behind the other. Counters are whole numbers: the order of the threads does not matter.
+// One CTA has a slice of one row. The row's tokens, each with a thread, count themselves at the entry that they hold; then a pass over the slice, 16
+// bytes at a time, does the arithmetic, whose first vectors were asked for before the tokens were looked at. Counters are whole numbers:
+// the order of the threads does not matter. They lie in shared memory, 16 bits to an entry (32 where a row has 2^15 tokens or more), so that a
+// vector's are one load; bits, with a counter at each set one's rank, are a third of that, but took 11.4 / 51 us for 64 / 512 rows instead of 8.0 / 47: two
+// rounds over the tokens, ranks between them, and three looks for each vector.
 //
-// What bounds it: issue slots, 73 % of them taken with fp32. 512 rows of 50257 with 2048 to 4096 tokens, a bias for all and a mask each take 52 us
-// (4.1 TB/s); a pass without any of them 33 (6.2), the mask adds less than 1, the bias, from L2 once more for every row, 7 to 10, the tokens 7. One vector
-// of a thread at a time, without the ring, took 95; two CTAs of 512 threads on an SM and longer rings 57. Small batches: 64 rows 11 us, two or three 4.
+// What bounds it: 512 rows of 50257 in fp32, 2048 to 4096 tokens, a bias for all and a mask each, take 47 us (4.5 TB/s); a pass without any of them 33 (6.2), with
+// the mask 35, and the bias 43 (from L2 once more for every row; it comes by the same way as the tokens, 50 MB for three slices of a row), the mask and the
+// tokens 44. One vector of a thread at a time, without the ring, took 95. Small batches: 64 rows 8.0 us, two or three 3.3.
 #include <cuda_fp16.h>
 
 #include "calls.h"
@@ -28,9 +28,8 @@ namespace gf {
 
 constexpr int LG_THREADS = 512;
 constexpr int LG_CTAS = 3;       // on an SM
-constexpr int LG_STAGES = 4;     // vectors of a thread on their way together
-constexpr int LG_TOKENS = 8;     // tokens of a thread that it looks up once
-constexpr int LG_SLICE_MIN = 4096, LG_SLICE_MAX = 25600;
+constexpr int LG_TOKENS = 8;     // tokens of a thread on their way together
+constexpr int LG_SLICE_MIN = 4096, LG_SLICE_MAX = 17408;
 
 struct LogitsParams {
   const void* x;
@@ -55,21 +54,39 @@ __device__ __forceinline__ void from_f(float& y, float x) { y = x; }
 __device__ __forceinline__ void from_f(__nv_bfloat16& y, float x) { y = __float2bfloat16(x); }
 __device__ __forceinline__ void from_f(__half& y, float x) { y = __float2half(x); }
 
-template <typename T>
+// Words of a slice's mask, which may begin up to 7 entries into the first: a multiple of 16 bytes.
+__host__ __device__ constexpr int lg_words(int slice) { return (slice / 32 + 4) & ~3; }
+
+// What the tokens say of an entry: that they hold it, in the highest bit (of a token of the prompt) or by the count below it (of generated ones).
+// 16 bits to an entry where rows have fewer than 2^15 tokens; no bits where there are none.
+template <int BITS>
+struct LgCount {
+  static constexpr int PER = BITS == 32 ? 1 : 2;                 // entries of a word
+  static constexpr unsigned HELD = BITS == 32 ? 0x80000000u : 0x8000u;
+  __device__ __forceinline__ static float number(unsigned c) {
+    return BITS == 32 ? (float)c : __uint_as_float(0x4b000000u | c) - 8388608.f;        // 2^23 + c
+  }
+};
+// Vectors of a thread on their way together. With counters in shared memory a fourth leaves the L1 too little: us, 3 / 4, 512 rows of 50257 with all
+// there is 47 / 54, without tokens, bf16, 22 / 20.
+__host__ __device__ constexpr int lg_stages(int bits) { return bits ? 3 : 4; }
+
+template <typename T, int BITS>
 __global__ void __launch_bounds__(LG_THREADS, LG_CTAS) logits_kernel(const __grid_constant__ LogitsParams p) {
-  constexpr int VEC = 16 / sizeof(T);
+  using Count = LgCount<BITS>;
+  constexpr int VEC = 16 / sizeof(T), PER = Count::PER, WORDS = VEC / PER, STAGES = lg_stages(BITS);      // WORDS: counters' words of a vector
+  constexpr unsigned FIELD = PER == 1 ? 0xffffffffu : 0xffffu;
   extern __shared__ __align__(16) unsigned shared[];
-  __shared__ int warp_sum[LG_THREADS / 32];
-  const int row = blockIdx.x / p.slices, v0 = (blockIdx.x - row * p.slices) * p.slice, size = min(p.slice, p.V - v0), n_words = p.slice / 32;
-  uint4* ring = reinterpret_cast<uint4*>(shared);  // [LG_STAGES][LG_THREADS]: a thread reads what it asked for itself
-  unsigned* open = shared + 4 * LG_STAGES * LG_THREADS;          // [n_words]: allowed
-  uint2* seen = reinterpret_cast<uint2*>(open + n_words);        // [n_words]: bits, and set bits of the words in front
-  int* count = (int*)(seen + n_words);             // [min(L, slice)]
+  const int row = blockIdx.x / p.slices, v0 = (blockIdx.x - row * p.slices) * p.slice, size = min(p.slice, p.V - v0);
+  uint4* ring = reinterpret_cast<uint4*>(shared);  // [STAGES][LG_THREADS]: a thread reads what it asked for itself
+  unsigned* open = shared + 4 * STAGES * LG_THREADS;          // allowed, 32 entries to a word
+  unsigned* count = open + lg_words(p.slice);      // PER entries to a word
   const T* x = (const T*)p.x + row * p.ldx + v0;   // entry 0 of the slice
   T* y = (T*)p.y + row * p.ldy + v0;
   // whole vectors: `vectors` from entry `head` on, on 16-byte boundaries of x and y; none where the two begin on different ones
   const int head = min((int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) % 16 / sizeof(T)), size);
   const int vectors = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(y)) & 15) ? 0 : (size - head) / VEC;
+  const int shift = (VEC - head % VEC) % VEC;      // entry v is v + shift in shared memory, where vectors begin on their boundaries
   const T* xv = x + head + threadIdx.x * VEC;
   const uint32_t slot = smem_u32(ring + threadIdx.x);
   auto ask = [&](int k, int st) {                  // vector k of the slice; one group each, empty ones behind the last
@@ -81,98 +98,72 @@ __global__ void __launch_bounds__(LG_THREADS, LG_CTAS) logits_kernel(const __gri
   const float* bias = p.bias ? p.bias + row * p.ldb + v0 : nullptr;
   auto begin = [&] {                               // what the pass needs first, on its way while the tokens are counted
 #pragma unroll
-    for (int i = 0; i < LG_STAGES; ++i) ask(threadIdx.x + i * LG_THREADS, i);
-    if (p.allowed)
-      for (int i = threadIdx.x; i < (size + 31) / 32; i += LG_THREADS) open[i] = __ldg(p.allowed + row * p.lda + (v0 >> 5) + i);
-  };
-  auto rank = [&](int v) {                         // of entry v if its bit is set, else of the next one whose is
-    const uint2 w = seen[v >> 5];
-    return (int)w.y + __popc(w.x & ~(0xffffffffu << (v & 31)));
+    for (int i = 0; i < STAGES; ++i) ask(threadIdx.x + i * LG_THREADS, i);
+    if (p.allowed) {
+      const unsigned* from = p.allowed + row * p.lda + (v0 >> 5);
+      const int words = (size + 31) / 32;
+      for (int i = threadIdx.x; i < (size + shift + 31) / 32; i += LG_THREADS)
+        open[i] = __funnelshift_l(i > 0 ? __ldg(from + i - 1) : 0u, i < words ? __ldg(from + i) : 0u, shift);
+    }
   };
   int n = 0;
-  const float rep = p.repetition ? p.repetition[row] : p.repetition0, less = 1.f / rep;
-  auto penalised = [&](float a, int r) { return (a > 0.f ? a * less : a * rep) - __int_as_float(count[r]); };
-  if (p.tokens) {
-    const float pres = p.presence ? p.presence[row] : p.presence0, freq = p.frequency ? p.frequency[row] : p.frequency0;
-    const int from = p.generated_from ? p.generated_from[row] : 0;
-    n = p.token_lens ? max(0, min(p.token_lens[row], p.L)) : p.L;
-    // LG_TOKENS tokens of a thread from i0 on: their entries, -1 for one that is not in the slice (or not there)
-    auto tokens = [&](int i0, int (&v)[LG_TOKENS]) {
+  float rep = 1.f, less = 1.f, pres = 0.f, freq = 0.f;
+  if (BITS && p.tokens) {                          // (there are, with BITS; without the test the pass is compiled to spill, 53 us for 47)
+    int t[LG_TOKENS];                              // LG_TOKENS tokens of the thread from i0 on: their entries, -1 for what is not in the slice
+    auto tokens = [&](int i0) {
 #pragma unroll
       for (int j = 0; j < LG_TOKENS; ++j) {
         const int i = i0 + j * LG_THREADS;
-        long long t = -1;
-        if (i < p.L) t = p.tokens64 ? ((const long long*)p.tokens)[row * p.ldt + i] : ((const int*)p.tokens)[row * p.ldt + i];
-        t -= v0;
-        v[j] = t >= 0 && t < size ? (int)t : -1;
+        long long v = -1;
+        if (i < p.L) v = p.tokens64 ? ((const long long*)p.tokens)[row * p.ldt + i] : ((const int*)p.tokens)[row * p.ldt + i];
+        v -= v0;
+        t[j] = v >= 0 && v < size ? (int)v + shift : -1;
       }
-#pragma unroll
-      for (int j = 0; j < LG_TOKENS; ++j)
-        if (i0 + j * LG_THREADS >= n) v[j] = -1;
     };
-    int mine[LG_TOKENS];                           // the first of them, for every round
-    tokens(threadIdx.x, mine);
+    tokens(threadIdx.x);
     begin();                                       // behind the tokens, which everything waits for
-    auto each = [&](auto f) {
+    rep = p.repetition ? p.repetition[row] : p.repetition0;
+    less = 1.f / rep;
+    pres = p.presence ? p.presence[row] : p.presence0;
+    freq = p.frequency ? p.frequency[row] : p.frequency0;
+    const int from = p.generated_from ? p.generated_from[row] : 0;
+    n = p.token_lens ? max(0, min(p.token_lens[row], p.L)) : p.L;
+    for (int i = threadIdx.x; i < (p.slice + 8) / PER / 4; i += LG_THREADS) reinterpret_cast<uint4*>(count)[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    for (int i0 = threadIdx.x; i0 < n;) {
 #pragma unroll
-      for (int j = 0; j < LG_TOKENS; ++j)
-        if (mine[j] >= 0) f(mine[j], (int)threadIdx.x + j * LG_THREADS);
-      for (int i0 = threadIdx.x + LG_TOKENS * LG_THREADS; i0 < n; i0 += LG_TOKENS * LG_THREADS) {
-        int v[LG_TOKENS];
-        tokens(i0, v);
-#pragma unroll
-        for (int j = 0; j < LG_TOKENS; ++j)
-          if (v[j] >= 0) f(v[j], i0 + j * LG_THREADS);
+      for (int j = 0; j < LG_TOKENS; ++j) {
+        const int i = i0 + j * LG_THREADS;
+        if (t[j] < 0 || i >= n) continue;
+        unsigned* word = count + t[j] / PER;
+        const int at = t[j] % PER * 16;
+        if (i >= from)
+          atomicAdd(word, 1u << at);
+        else
+          atomicOr(word, Count::HELD << at);
       }
-    };
-    for (int i = threadIdx.x; i < n_words; i += LG_THREADS) seen[i].x = 0;
-    __syncthreads();
-    each([&](int v, int) { atomicOr(&seen[v >> 5].x, 1u << (v & 31)); });
-    __syncthreads();
-    // ranks: a thread sums up the words that are its own, one behind the other, then the threads' sums
-    const int per = (n_words + LG_THREADS - 1) / LG_THREADS, w0 = min(threadIdx.x * per, n_words), w1 = min(w0 + per, n_words);
-    int own = 0;
-    for (int i = w0; i < w1; ++i) own += __popc(seen[i].x);
-    int incl = own;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, incl, o);
-      if ((threadIdx.x & 31) >= o) incl += u;
-    }
-    if ((threadIdx.x & 31) == 31) warp_sum[threadIdx.x >> 5] = incl;
-    __syncthreads();
-    int at = incl - own, held = 0;                 // entries that the tokens hold
-#pragma unroll
-    for (int i = 0; i < LG_THREADS / 32; ++i) {
-      if (i < (threadIdx.x >> 5)) at += warp_sum[i];
-      held += warp_sum[i];
-    }
-    for (int i = threadIdx.x; i < held; i += LG_THREADS) count[i] = 0;
-    for (int i = w0; i < w1; ++i) {
-      seen[i].y = at;
-      at += __popc(seen[i].x);
-    }
-    __syncthreads();
-    each([&](int v, int i) {
-      if (i >= from) atomicAdd(&count[rank(v)], 1);
-    });
-    __syncthreads();
-    for (int i = threadIdx.x; i < held; i += LG_THREADS) {
-      const int c = count[i];
-      count[i] = __float_as_int(c * freq + (c > 0 ? pres : 0.f));
+      i0 += LG_TOKENS * LG_THREADS;
+      if (i0 < n) tokens(i0);
     }
   } else {
     begin();
   }
-  __syncthreads();                                 // `open` and what is taken off
+  __syncthreads();                                 // `open` and `count`
+  auto penalised = [&](float a, unsigned held) {   // held: not 0
+    const unsigned c = held & (Count::HELD - 1);
+    return (a > 0.f ? a * less : a * rep) - (Count::number(c) * freq + (c ? pres : 0.f));
+  };
   // ---- the entries in front of the vectors and behind them, or all
   const int behind = head + vectors * VEC;
   for (int i = threadIdx.x; i < head + size - behind; i += LG_THREADS) {
-    const int v = i < head ? i : i - head + behind;
+    const int v = i < head ? i : i - head + behind, l = v + shift;
     float a = to_f(x[v]);
-    if (n > 0 && ((seen[v >> 5].x >> (v & 31)) & 1)) a = penalised(a, rank(v));
+    if (BITS && n > 0) {
+      const unsigned held = (count[l / PER] >> (l % PER * 16)) & FIELD;
+      if (held) a = penalised(a, held);
+    }
     if (bias) a += bias[v];
-    if (p.allowed && !((open[v >> 5] >> (v & 31)) & 1)) a = -INFINITY;
+    if (p.allowed && !((open[l >> 5] >> (l & 31)) & 1)) a = -INFINITY;
     from_f(y[v], a);
   }
   // ---- the vectors
@@ -193,33 +184,41 @@ __global__ void __launch_bounds__(LG_THREADS, LG_CTAS) logits_kernel(const __gri
       for (int j = 0; j < VEC; ++j) add[j] = __ldg(from + j);
     }
   };
-  const bool apart = head % VEC != 0;              // the bits of a vector may go on into the next word
-  auto bits = [&](int l, auto word) {              // of the VEC entries from l on
-    unsigned w = word(l >> 5) >> (l & 31);
-    if (apart && (l & 31) + VEC > 32) w |= word((l >> 5) + 1) << (32 - (l & 31));
-    return w & ((1u << VEC) - 1);
-  };
   bias_of(threadIdx.x);
   T* to = y + head + threadIdx.x * VEC;
-  for (int k0 = threadIdx.x; k0 < vectors; k0 += LG_STAGES * LG_THREADS) {
+  const int first = head + shift;                  // of the vectors' entries in shared memory
+  for (int k0 = threadIdx.x; k0 < vectors; k0 += STAGES * LG_THREADS) {
 #pragma unroll
-    for (int st = 0; st < LG_STAGES; ++st) {
+    for (int st = 0; st < STAGES; ++st) {
       const int k = k0 + st * LG_THREADS;
       if (k >= vectors) break;
-      asm volatile("cp.async.wait_group %0;" ::"n"(LG_STAGES - 1) : "memory");
+      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
       const uint4 in = ring[st * LG_THREADS + threadIdx.x];
       const T* have = reinterpret_cast<const T*>(&in);
-      const int l = head + k * VEC;
+      const int l = first + k * VEC;
       float a[VEC];
 #pragma unroll
       for (int j = 0; j < VEC; ++j) a[j] = to_f(have[j]);
-      if (n > 0) {
-        const unsigned hit = bits(l, [&](int w) { return seen[w].x; });
-        if (hit) {
-          int r = rank(l);
+      if (BITS && n > 0) {
+        unsigned held[WORDS], any = 0;
+        if constexpr (WORDS == 2) {
+          const uint2 u = reinterpret_cast<const uint2*>(count)[l / VEC];
+          held[0] = u.x; held[1] = u.y;
+        } else {
 #pragma unroll
-          for (int j = 0; j < VEC; ++j)
-            if ((hit >> j) & 1) a[j] = penalised(a[j], r++);
+          for (int w = 0; w < WORDS; w += 4) {
+            const uint4 u = reinterpret_cast<const uint4*>(count)[(l / PER + w) / 4];
+            held[w] = u.x; held[w + 1] = u.y; held[w + 2] = u.z; held[w + 3] = u.w;
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < WORDS; ++w) any |= held[w];
+        if (any) {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            const unsigned f = (held[j / PER] >> (j % PER * 16)) & FIELD;
+            if (f) a[j] = penalised(a[j], f);
+          }
         }
       }
       if (bias) {
@@ -228,7 +227,7 @@ __global__ void __launch_bounds__(LG_THREADS, LG_CTAS) logits_kernel(const __gri
         bias_of(k + LG_THREADS);
       }
       if (p.allowed) {
-        const unsigned ok = bits(l, [&](int w) { return open[w]; });
+        const unsigned ok = open[l >> 5] >> (l & 31);
 #pragma unroll
         for (int j = 0; j < VEC; ++j)
           if (!((ok >> j) & 1)) a[j] = -INFINITY;
@@ -238,27 +237,29 @@ __global__ void __launch_bounds__(LG_THREADS, LG_CTAS) logits_kernel(const __gri
 #pragma unroll
       for (int j = 0; j < VEC; ++j) from_f(left[j], a[j]);
       *reinterpret_cast<uint4*>(to + (k - (int)threadIdx.x) * VEC) = u;
-      ask(k + LG_STAGES * LG_THREADS, st);
+      ask(k + STAGES * LG_THREADS, st);
     }
   }
 }
 
-// Rows are cut into as many slices as run at one time, of LG_SLICE_MIN entries or more; more rows than that into slices of at most LG_SLICE_MAX (a CTA
-// spends about half as long on its row's tokens as on such a slice: half as long ones took 62 us for 512 rows instead of 52, whole rows 61, because
-// a fourth round of CTAs then has little to do).
+// Rows are cut into two slices for every SM (with three 64 rows took 8.8 us instead of 8.0: every CTA looks at all tokens of its row), of LG_SLICE_MIN entries or
+// more; many rows into slices of at most LG_SLICE_MAX, which leave the L1 room beside three CTAs' counters: 512 rows took 49 us with a quarter less, 54
+// with half more. Without counters half more, with wide ones half of it.
 template <typename T>
 static int launch_logits(LogitsParams& p, long long B, cudaStream_t st) {
-  const long long most = (p.V + LG_SLICE_MIN - 1) / LG_SLICE_MIN, least = (p.V + LG_SLICE_MAX - 1) / LG_SLICE_MAX;
-  const long long slices = max(least, min(most, (long long)LG_CTAS * sm_count() / B));
+  const int bits = !p.tokens ? 0 : p.L < 1 << 15 ? 16 : 32;
+  const long long longest = bits == 0 ? LG_SLICE_MAX * 3 / 2 : bits == 16 ? LG_SLICE_MAX : LG_SLICE_MAX / 2;
+  const long long most = (p.V + LG_SLICE_MIN - 1) / LG_SLICE_MIN, least = (p.V + longest - 1) / longest;
+  const long long slices = max(least, min(most, 2ll * sm_count() / B));
   p.slice = (int)(((p.V + slices - 1) / slices + 63) / 64 * 64);
   p.slices = (p.V + p.slice - 1) / p.slice;
   if (B * p.slices > 0x7fffffffll) return GFH_TOO_LARGE;
-  const size_t smem = 16 * LG_STAGES * LG_THREADS + p.slice / 8 + (p.tokens ? p.slice / 4 + 4ll * min(p.L, p.slice) : 0);
-  static gf::DeviceMax granted;
-  auto kern = logits_kernel<T>;
-  if (smem > 48 * 1024 && granted.get() < smem) {
+  const size_t smem = 16 * lg_stages(bits) * LG_THREADS + 4 * lg_words(p.slice) + (p.slice + 8) * bits / 8;
+  static gf::DeviceMax granted[3];
+  auto kern = bits == 0 ? logits_kernel<T, 0> : bits == 16 ? logits_kernel<T, 16> : logits_kernel<T, 32>;
+  if (smem > 48 * 1024 && granted[bits / 16].get() < smem) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return GFH_CUDA;
-    granted.set(smem);
+    granted[bits / 16].set(smem);
   }
   kern<<<(unsigned)(B * p.slices), LG_THREADS, smem, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? GFH_OK : GFH_CUDA;

@@ -96,3 +96,19 @@ def test_replayed_and_on_another_stream():
         z = ops.process_logits(x, **kw)
     torch.cuda.synchronize()
     assert torch.equal(y, z)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("L", [32767, 32768, 70001])
+@pytest.mark.parametrize("pitch", [0, 3])
+def test_long_histories_of_few_tokens(dtype, L, pitch):
+    """Counts up to the whole history: one token all along, and one only in the prompt."""
+    B, V = 3, 20011
+    x = (3 * torch.randn(B, V + pitch, device="cuda")).to(dtype)[:, :V]
+    tokens = 500 * torch.randint(0, 41, (B, L), device="cuda")
+    tokens[0] = 7                                        # c = L
+    tokens[1, :L // 2], tokens[1, L // 2:] = 20010, 6
+    first = torch.tensor([0, L // 2, L - 3], dtype=torch.int32, device="cuda")
+    kw = dict(tokens=tokens, generated_from=first, repetition=1.3, presence=0.5, frequency=2 ** -14)
+    _check(x, **kw)
+    _check(x, **kw, bias=torch.randn(V, device="cuda"), allowed=torch.rand(B, V, device="cuda") < 0.5)
