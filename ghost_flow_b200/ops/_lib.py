@@ -147,8 +147,10 @@ def calls():
         loader = importlib.machinery.ExtensionFileLoader("_gf_calls", str(path))
         module = importlib.util.module_from_spec(importlib.util.spec_from_file_location("_gf_calls", str(path), loader=loader))
         loader.exec_module(module)
+        from .fused import follows
+
         module.bind(exchange, *(ctypes.cast(getattr(lib, name), c_void_p).value for name in (
-            "gf_paged_append", "gf_paged_attn", "gf_paged_attn_one", "gf_process_logits")))
+            "gf_paged_append", "gf_paged_attn", "gf_paged_attn_one", "gf_process_logits")), *follows())
         _CALLS = module
     return _CALLS
 

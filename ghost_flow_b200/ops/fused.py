@@ -455,6 +455,12 @@ def _observed() -> bool:
 observed = _observed
 
 
+def follows() -> tuple:
+    """What :func:`_observed` asks, and whether gradients are recorded, for ``csrc/calls.cpp`` (which a call reaches only outside of compilation)."""
+    tracing, transforms, dispatch_modes, function_modes = _PROBES if None not in _PROBES else (lambda: 1,) * 4
+    return tracing, transforms, dispatch_modes, function_modes, _only_device_contexts, forward_ad, torch.is_grad_enabled
+
+
 def decode_cache_ok(kcache, vcache, cos, sin, heads, device, pos: int) -> bool:
     """Whether a decoding kernel may write row ``pos`` of the caches ``[B, n, Hk, D]`` (``heads`` = B, Hk, D) and rotate with these
     tables; positions that are not in the tables are an error. For calls that nothing follows (:func:`observed`)."""

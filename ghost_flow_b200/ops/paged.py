@@ -25,6 +25,7 @@ from .raw import _SLICES, _decode_parts
 _INT32, _BF16 = torch.int32, torch.bfloat16
 _OVERLAP = -5      # GFH_OVERLAP of csrc/gf_host.h
 _increment_version = torch.autograd.graph.increment_version
+_is_compiling = torch.compiler.is_compiling
 
 
 def _check_batch(what, x, kpages, vpages, page_table, lens, cu) -> None:
@@ -60,12 +61,6 @@ def _pages_apart(P, page, Hk, D, pools) -> bool:
     return all(_rows_apart(D, d) for d in dims) and ends[0][1] <= ends[1][0]
 
 
-def _launches(x, kpages, vpages) -> bool:
-    """Whether a call on these may be a kernel's: CUDA tensors, and nothing that follows it."""
-    return x.get_device() >= 0 and not _observed() and not (
-        torch.is_grad_enabled() and (x.requires_grad or kpages.requires_grad or vpages.requires_grad))
-
-
 def _report(device, bad, what: str) -> None:
     """A batch that names pages or positions that are not there: an error on the CPU, else the status word's (see ``_lib.check_status``)."""
     if device.type != "cuda":
@@ -85,7 +80,7 @@ def _places(T, lens, cu):
     c = cu.long().clamp(0, T)
     b = torch.searchsorted(c[1:].contiguous(), t, right=True)
     inside = (b < B) & (t >= c[0])
-    b = b.clamp(max=max(B - 1, 0))
+    b = b.clamp(max=max(int(B) - 1, 0))        # (a number under tracing too)
     return b, lens.long()[b] - c[b + 1] + t, inside
 
 
@@ -128,7 +123,7 @@ def rope_qkv_to_pages(qkv, num_heads: int, num_kv_heads: int, cos, sin, kpages, 
     Inference only: a call with a gradient to record takes PyTorch's operations."""
     H, Hk = num_heads, num_kv_heads
     call = None
-    if _launches(qkv, kpages, vpages):
+    if qkv.get_device() >= 0 and not _is_compiling():
         call = _lib.calls().append(qkv, H, Hk, kpages, vpages, page_table, lens, cu, cos, sin)
         if call is not None and call[5] is not None and not _pages_apart(*kpages.shape, call[5]):
             call = None
@@ -156,7 +151,7 @@ def rope_qkv_to_pages(qkv, num_heads: int, num_kv_heads: int, cos, sin, kpages, 
     if not packed:
         qkv = qkv.clone(memory_format=torch.contiguous_format)
         at = _lib.calls().append(qkv, H, Hk, kpages, vpages, page_table, lens, cu, cos, sin)[0]
-    q = qkv.new_empty((T, H, D))
+    q = qkv.new_empty(T, H, D)
     rc = _lib.calls().run_append(at, q, interleaved, _lib.status_ptr(device), stream)
     if rc == _OVERLAP:
         raise ValueError("rope_qkv_to_pages: qkv shares memory with the pages")
@@ -235,7 +230,7 @@ def paged_attention(q, kpages, vpages, page_table, lens, cu=None, scale: float |
     ``_lib.check_status`` raises for both. Head sizes 64 and 128 with pages of a power of two from 16 rows take the kernels.
     Inference only: a call with a gradient to record takes PyTorch's operations."""
     call, what = None, "paged_attention"
-    if _launches(q, kpages, vpages):
+    if q.get_device() >= 0 and not _is_compiling():
         call = _lib.calls().attention(q, kpages, vpages, page_table, lens, cu)
         if call is not None and out is not None:
             H, D, st = call[4], call[6], out.stride()
@@ -277,7 +272,7 @@ def paged_attention(q, kpages, vpages, page_table, lens, cu=None, scale: float |
         x = q.clone(memory_format=torch.contiguous_format)
     if x is not q:
         at = _lib.calls().attention(x, kpages, vpages, page_table, lens, cu)[0]
-    o = out if out is not None else torch.empty_like(x) if x.is_contiguous() else q.new_empty((T, H, D))
+    o = out if out is not None else torch.empty_like(x) if x.is_contiguous() else q.new_empty(T, H, D)
     parts, few, ws = 0, None, None
     if one or (cu is not None and B >= _MANY and groups):
         sms = _SMS.get(device) or _sm_count(q.device)

@@ -8,8 +8,8 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .fused import _observed, _rc
-from .paged import _ranges_overlap
+from .fused import _rc
+from .paged import _is_compiling, _ranges_overlap
 
 
 def pack_allowed(mask):
@@ -87,16 +87,10 @@ def _check(logits, tokens, token_lens, generated_from, repetition, presence, fre
                 raise ValueError(f"{what}: out shares memory with {name}")
 
 
-def _launches(x, out, others) -> bool:
-    """Whether a call on these may be the kernel's: CUDA tensors, nothing that follows it, and a place for the result that the kernel takes."""
-    if x.get_device() < 0 or x.dim() != 2 or _observed():
-        return False
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, out, *others) if t is not None and type(t) is not float and torch.is_tensor(t)):
-        return False
-    if out is None:
-        return True
+def _takes(out, x, others) -> bool:
+    """Whether the kernel may write there."""
     return (out.shape == x.shape and out.dtype is x.dtype and out.device == x.device and out.stride(1) == 1
-            and (x.shape[0] <= 1 or out.stride(0) >= x.shape[1])
+            and (x.shape[0] <= 1 or out.stride(0) >= x.shape[1]) and not (out.requires_grad and torch.is_grad_enabled())
             and ((out.data_ptr() == x.data_ptr() and out.stride() == x.stride()) or not _ranges_overlap(out, x))
             and not any(torch.is_tensor(t) and t.numel() and _ranges_overlap(out, t) for t in others))
 
@@ -112,8 +106,10 @@ def process_logits(logits, tokens=None, token_lens=None, generated_from=None, re
     three penalties are numbers or fp32 ``[B]``. ``bias``: fp32 ``[V]`` or ``[B, V]``. ``allowed``: int32 bits ``[words]`` or ``[B, words]``
     (:func:`pack_allowed`). ``out`` may be ``logits`` itself. A row of which nothing is allowed is all ``-inf``."""
     call = None
-    if _launches(logits, out, (repetition, presence, frequency, bias, tokens, allowed)):
+    if logits.get_device() >= 0 and not _is_compiling():
         call = _lib.calls().logits(logits, tokens, token_lens, generated_from, repetition, presence, frequency, bias, allowed)
+        if call is not None and out is not None and not _takes(out, logits, (repetition, presence, frequency, bias, tokens, allowed)):
+            call = None
     if call is None:
         _check(logits, tokens, token_lens, generated_from, repetition, presence, frequency, bias, allowed, out)
         if logits.numel() == 0:
@@ -130,7 +126,7 @@ def process_logits(logits, tokens=None, token_lens=None, generated_from=None, re
     else:
         # rows as far apart as they are, where they are apart: they then begin on the same boundaries
         ldy = ld if V <= ld < V + 64 else V
-        y = torch.empty_strided((B, V), (ldy, 1), dtype=logits.dtype, device=logits.device)
+        y = logits.new_empty_strided((B, V), (ldy, 1))
     _rc(_lib.calls().run_logits(at, y, ldy, stream), "gf_process_logits")
     if out is not None:
         torch.autograd.graph.increment_version(out)

@@ -6,6 +6,7 @@ import torch
 
 import _paged_oracle as oracle
 from ghost_flow_b200.ops import _lib
+from ghost_flow_b200.ops.fused import follows
 
 
 def _args():
@@ -47,6 +48,6 @@ def test_other_versions_of_the_exchange_interface_are_refused():
     new.restype, new.argtypes = ctypes.py_object, [ctypes.c_void_p, ctypes.c_char_p, ctypes.c_void_p]
     table = (ctypes.c_uint32 * 16)(2, 0)
     with pytest.raises(RuntimeError, match="version 2"):
-        _lib.calls().bind(new(ctypes.addressof(table), b"dlpack_exchange_api", None), 1, 1, 1, 1)
+        _lib.calls().bind(new(ctypes.addressof(table), b"dlpack_exchange_api", None), 1, 1, 1, 1, *follows())
     with pytest.raises(ValueError):
-        _lib.calls().bind(new(ctypes.addressof(table), b"another", None), 1, 1, 1, 1)
+        _lib.calls().bind(new(ctypes.addressof(table), b"another", None), 1, 1, 1, 1, *follows())

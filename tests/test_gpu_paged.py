@@ -401,3 +401,41 @@ def test_projections_in_the_pages_are_refused(kernel_status):
         with pytest.raises(ValueError, match="shares memory"):
             ops.rope_qkv_to_pages(pool.view(-1)[:3 * 8 * 64].view(3, 8, 64), 4, 2, cos, sin, s["kp"], s["vp"], s["table"], s["lens"], s["cu"])
         assert torch.equal(pool.nan_to_num(1, 2, 3), before)
+
+
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+@pytest.mark.parametrize("inside,kernels", [("nothing", True), ("a device", True), ("a function mode", False), ("a dispatch mode", False),
+                                            ("forward mode", False), ("a gradient", False), ("no gradients", True), ("tracing", False)])
+def test_kernels_run_where_nothing_follows(inside, kernels, kernel_status):
+    import contextlib
+
+    from torch.overrides import TorchFunctionMode
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    from ghost_flow_b200 import ops
+    from ghost_flow_b200.ops import _lib
+
+    class Function(TorchFunctionMode):
+        def __torch_function__(self, func, types, a=(), kw=None):
+            return func(*a, **(kw or {}))
+
+    class Dispatch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, a=(), kw=None):
+            return func(*a, **(kw or {}))
+
+    s = oracle.batch([7, 20], [1, 2], 4, 2, 64, 16, device="cuda")
+    s["kp"], s["vp"] = s["kp"].nan_to_num(0, 0, 0), s["vp"].nan_to_num(0, 0, 0)
+    cos, sin = ops.rope_tables(64, 64, 1e4, "cuda")
+    x = torch.randn(2, 90, device="cuda")
+    around = {"a device": torch.device("cuda"), "a function mode": Function(), "a dispatch mode": Dispatch(),
+              "forward mode": torch.autograd.forward_ad.dual_level(), "no gradients": torch.no_grad()}.get(inside, contextlib.nullcontext())
+    if "gradient" in inside:
+        s["q"].requires_grad_(), s["qkv"].requires_grad_(), x.requires_grad_()
+    calls = [lambda: _attend(s), lambda: ops.process_logits(x, bias=torch.ones(90, device="cuda"))]
+    if inside != "a gradient":                               # to pools that are no leaves
+        calls.append(lambda: ops.rope_qkv_to_pages(s["qkv"], 4, 2, cos, sin, s["kp"], s["vp"], s["table"], s["lens"], s["cu"]))
+    for f in calls:
+        n = _lib.launch_count()
+        with around:
+            torch.jit.trace(lambda _: f(), (torch.ones(1),), check_trace=False) if inside == "tracing" else f()
+        assert (_lib.launch_count() > n) == kernels
