@@ -7,7 +7,7 @@ sequence ``b`` in their order. New tokens of all sequences lie one behind the ot
 ``i`` of ``n`` stands at position ``lens[b] - n + i``. All of these stay on the device and nothing here waits for them: a captured call goes by
 what they hold when it is replayed. A sequence of no new tokens, or of no keys (an empty slot of a batch), is allowed.
 
-bf16 CUDA tensors take the kernels of ``csrc/paged_cache.cu`` and ``csrc/attn_paged.cu``; other types, layouts and CPU tensors, and calls that
+bf16 CUDA tensors take the kernels of ``csrc/paged_cache.cu`` and ``csrc/attn_paged.cu`` (through ``csrc/calls.cpp``); other types, layouts and CPU tensors, and calls that
 something follows (a gradient, tracing, transforms, modes), plain PyTorch. The reference has no cache (ghostflow-nn/src/gpt.rs:402-422).
 """
 from __future__ import annotations
