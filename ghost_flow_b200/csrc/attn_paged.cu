@@ -21,10 +21,11 @@
 // memory bounds, takes P in two terms.)
 //
 // What bounds it. Whole prompts: as attn_fwd3.cu, tensor pipe and exponentials, 1.9 us for a step of 256 rows; us, dense / pages of 64 / 16:
-// [1, 4096] with 32 / 8 heads of 128 133 / 137 / 137 (1000 TFLOP/s), [4, 2987] with 32 / 32 heads 325 / 327 / 327, [8, 1024] with 12 / 12 heads of 64 44 /
-// 49 / 49 (a CTA has 8 steps at most there, and finds its block, pages and queries in 3 us). The next 512 tokens over 7681 keys, 32 / 8 heads: 72 us
-// (860 TFLOP/s), two pieces of 64 blocks on 128 of 148 SMs, 60 of it in steps. Few rows: keys come at 6 TB/s while steps run, and the ends of it, 5 us
-// in front and 8 behind with the second kernel, are what is left: 5 tokens over 30000 keys 37 us (3.3 TB/s), 16 over 2000 12.5.
+// [1, 4096] with 32 / 8 heads of 128 133 / 135 / 136 (1000 TFLOP/s), [4, 2987] with 32 / 32 heads 325 / 327 / 327, [8, 1024] with 12 / 12 heads of 64 44 /
+// 49 / 49 (a CTA has 8 steps at most there, and finds its block, pages and queries in 3 us). The next 512 tokens over 7681 keys, 32 / 8 heads: 71 us
+// (870 TFLOP/s), two pieces of 64 blocks on 128 of 148 SMs, 60 of it in steps. A block of one tile takes half as long and is cut into half as many pieces: 284
+// tokens over 5983 keys, 25 / 25 heads of 64, 40 us, with as many as the others 53. Few rows: keys come at 6 TB/s while steps run, and the ends of it, 5 us
+// in front and 6 behind with the second kernel, are what is left: 5 tokens over 30000 keys 35 us (3.5 TB/s), 16 over 2000 12.
 #include "paged.cuh"
 
 namespace gf {
@@ -35,7 +36,6 @@ constexpr int PG_REGS_CTRL = 104; // 128 x 104 + 256 x 200 = 64512, the block's 
 constexpr int PG_REGS_SOFTMAX = 200;
 constexpr int PG_PARTS = 2;       // P V of a tile is issued in this many parts of the keys
 constexpr float PG_RESCALE = 8.0f;  // log2 units
-constexpr int PG_WHOLE = 1 << 30;   // steps of a piece where no block is cut
 
 struct PagedAttn {
   PagedBatch seqs;
@@ -45,14 +45,25 @@ struct PagedAttn {
   float scale;
   __nv_bfloat16* out;            // [T, Hq, D], rows ldo apart
   long long ldo;
-  int* plan;                     // keys (in steps) of a piece, for the kernel that joins pieces
+  int* cut;                      // how many blocks were cut into pieces (all, or 0)
+  int4* where;                   // for each of them, what the kernel that joins pieces wants to know (see there)
   float* part;                   // [item][rows][D], then [item][rows][maximum, sum]
   float* part_ml;
   int rows, items, blocks;       // rows of an item in `part`, items and blocks (of all KV heads) at most
 };
 
+constexpr int PG_WHOLE = 1 << 30;   // no block is cut
 struct PgShape {                 // what a sequence is cut into
   int n, len, keys, blocks, steps;
+  bool short_end;                // its last block has rows for one tile alone (see `alternate` below), and takes half as long
+  // pieces of a block, none longer than U steps of two tiles
+  __device__ __forceinline__ int pieces(bool end, int U) const {
+    if (U == PG_WHOLE) return 1;
+    if (end && short_end) U *= 2;
+    return (unsigned)(steps + U - 1) / (unsigned)U;
+  }
+  __device__ __forceinline__ int items(int U) const { return blocks == 0 ? 0 : (blocks - 1) * pieces(false, U) + pieces(true, U); }
+  __device__ __forceinline__ int longest() const { return blocks == 0 ? 0 : blocks == 1 && short_end ? (steps + 1) / 2 : steps; }     // block, uncut
 };
 __device__ __forceinline__ PgShape pg_shape(const PagedAttn& p, int b) {
   PgShape s;
@@ -62,12 +73,13 @@ __device__ __forceinline__ PgShape pg_shape(const PagedAttn& p, int b) {
   s.keys = (int)min((long long)max(s.len, 0), p.seqs.capacity());
   s.blocks = (s.n + 2 * p.tq - 1) / (2 * p.tq);
   s.steps = max(1, (s.keys + PG_TILE - 1) / PG_TILE);
+  s.short_end = s.n - (s.blocks - 1) * 2 * p.tq <= p.tq;
   return s;
 }
 
 // Whole warp: steps of a piece. All blocks uncut where they fill the machine; else the shortest pieces that run at one time, or, of cuts in 2, 3
 // and 4, the one whose waves of CTAs take the least (a piece costs about 3 steps of its own). `own`: the lane's sequence of the first 32.
-__device__ __forceinline__ int paged_plan(const PagedAttn& p, const PgShape& own) {
+__device__ __forceinline__ int paged_plan(const PagedAttn& p, const PgShape& own, int& whole) {
   constexpr int OWN = 3;
   if (p.slots == 0) return PG_WHOLE;
   const int lane = threadIdx.x & 31;
@@ -76,20 +88,17 @@ __device__ __forceinline__ int paged_plan(const PagedAttn& p, const PgShape& own
     for (int b = lane + 32; b < p.seqs.B; b += 32) n += f(pg_shape(p, b));
     return __reduce_add_sync(0xffffffffu, n) * p.Hkv;
   };
-  auto items = [&](int U) { return sum([&](const PgShape& s) { return s.blocks * ((s.steps + U - 1) / U); }); };
-  const int whole = sum([](const PgShape& s) { return s.blocks; });
+  auto items = [&](int U) { return sum([&](const PgShape& s) { return s.items(U); }); };
+  whole = sum([](const PgShape& s) { return s.blocks; });
   if (whole == 0) return PG_WHOLE;
   if (2 * whole <= p.slots) {
-    int U = max(1, (sum([](const PgShape& s) { return s.blocks * s.steps; }) + p.slots - 1) / p.slots);
+    int U = max(1, (sum([](const PgShape& s) { return max(0, s.blocks - 1) * s.steps + (s.blocks == 0 ? 0 : s.short_end ? (s.steps + 1) / 2 : s.steps); }) + p.slots - 1) / p.slots);
 #pragma unroll 1
     while (items(U) > p.slots) U += 1 + U / 16;    // ends: with whole blocks there are no more than half of them
     return U;
   }
-  int most = own.blocks > 0 ? own.steps : 0;
-  for (int b = lane + 32; b < p.seqs.B; b += 32) {
-    const PgShape s = pg_shape(p, b);
-    if (s.blocks > 0) most = max(most, s.steps);
-  }
+  int most = own.longest();
+  for (int b = lane + 32; b < p.seqs.B; b += 32) most = max(most, pg_shape(p, b).longest());
   most = __reduce_max_sync(0xffffffffu, most);
   int best = PG_WHOLE, cost = (whole + p.slots - 1) / p.slots * (most + OWN);
 #pragma unroll 1
@@ -107,6 +116,7 @@ __device__ __forceinline__ int paged_plan(const PagedAttn& p, const PgShape& own
 // A block of a sequence, and the keys of a piece of it.
 struct PgItem {
   int b, hk, token, tokens, pos, len, keys, pieces, j0, j1;     // first token (row of q), how many, position of the first; steps j0 .. j1 - 1
+  int piece, block;              // which one, of which block
   __device__ __forceinline__ int visible(int upto) const {   // keys that the last of the first `upto` tokens sees
     return max(0, min(pos + min(upto, tokens), keys));
   }
@@ -125,32 +135,52 @@ __device__ __forceinline__ void pg_block(const PagedAttn& p, PgItem& it, const P
 // next to each other.
 __device__ __forceinline__ bool pg_find(const PagedAttn& p, const PgShape& own, int x, int U, PgItem& it) {
   const int lane = threadIdx.x & 31;
+  const bool cuts = p.slots != 0;
+  const int mask = cuts ? 0xffff : -1;
 #pragma unroll 1
   for (int base = 0, before = 0; base < p.seqs.B; base += 32) {
     PgShape s = base == 0 ? own : base + lane < p.seqs.B ? pg_shape(p, base + lane) : PgShape{};
-    const int pieces = U == PG_WHOLE ? 1 : (s.steps + U - 1) / U, n = s.blocks * pieces * p.Hkv;
-    int incl = n;
+    int each = s.pieces(false, U), at_end = s.pieces(true, U);
+    const int n = s.blocks == 0 ? 0 : ((s.blocks - 1) * each + at_end) * p.Hkv;
+    const int both = cuts ? n | (s.blocks * p.Hkv) << 16 : n;          // items, and blocks: both are less than 2^16 where any may be cut
+    int incl = both;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int v = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += v;
     }
-    const unsigned hit = __ballot_sync(0xffffffffu, before + incl > x);
+    const unsigned hit = __ballot_sync(0xffffffffu, ((before + incl) & mask) > x);
     if (hit) {
-      const int l = __ffs(hit) - 1;
-      const int rem = x - before - (__shfl_sync(0xffffffffu, incl, l) - __shfl_sync(0xffffffffu, n, l));
+      const int l = __ffs(hit) - 1, front = before + __shfl_sync(0xffffffffu, incl - both, l), rem = x - (front & mask);
       s.n = __shfl_sync(0xffffffffu, s.n, l);
       s.len = __shfl_sync(0xffffffffu, s.len, l);
       s.keys = __shfl_sync(0xffffffffu, s.keys, l);
       s.blocks = __shfl_sync(0xffffffffu, s.blocks, l);
-      it.pieces = __shfl_sync(0xffffffffu, pieces, l);
-      const int per = p.Hkv * it.pieces, blk = s.blocks - 1 - rem / per, in = rem % per;
-      it.hk = in / it.pieces;
+      each = __shfl_sync(0xffffffffu, each, l);
+      at_end = __shfl_sync(0xffffffffu, at_end, l);
+      const int behind = rem - at_end * p.Hkv;               // the items of the last block
+      int blk = s.blocks - 1, in = rem;
+      it.pieces = at_end;
+      if (behind >= 0) {
+        const int q = behind / (each * p.Hkv);
+        in = behind - q * each * p.Hkv;
+        blk -= 1 + q;
+        it.pieces = each;
+      }
       pg_block(p, it, s, base + l, blk);
-      const int piece = in - it.hk * it.pieces, steps = it.steps(2 * p.tq);
-      it.j0 = (int)((long long)steps * piece / it.pieces);
-      it.j1 = (int)((long long)steps * (piece + 1) / it.pieces);
-      return it.pieces == 1 || x < p.items;                  // (the plan makes no more pieces than there is room for)
+      const int steps = it.steps(2 * p.tq);
+      it.hk = in;
+      it.piece = it.j0 = 0;
+      it.j1 = steps;
+      if (it.pieces > 1) {                                   // steps piece / pieces and steps (piece + 1) / pieces, in 32 bits
+        const unsigned pieces = it.pieces, piece = in % pieces, part = steps / pieces, rest = steps - part * pieces;
+        it.hk = in / pieces;
+        it.piece = piece;
+        it.j0 = piece * part + piece * rest / pieces;
+        it.j1 = (piece + 1) * part + (piece + 1) * rest / pieces;
+      }
+      it.block = (front >> 16) + (s.blocks - 1 - blk) * p.Hkv + it.hk;       // (where blocks may be cut)
+      return it.pieces == 1 || x < p.items;                  // (no more pieces are made than there is room for)
     }
     before += __shfl_sync(0xffffffffu, incl, 31);
   }
@@ -247,12 +277,17 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       mbar_fence_init();
       shared_failed = 0;
     }
-    const int U = paged_plan(p, own);
-    if (p.plan && blockIdx.x == 0 && lane == 0) *p.plan = U;
+    int whole = 0;                 // blocks
+    const int U = paged_plan(p, own, whole);
     there = pg_find(p, own, blockIdx.x, U, it);
     if (lane == 0) {
       shared_there = there;
       if (there) shared_item = it;
+      if (p.slots && blockIdx.x == 0) *p.cut = U == PG_WHOLE || !there ? 0 : whole;
+      if (U != PG_WHOLE && there && it.piece == 0 && it.block < p.blocks) {
+        p.where[2 * it.block] = make_int4(blockIdx.x, it.pieces, it.steps(2 * p.tq), it.token);
+        p.where[2 * it.block + 1] = make_int4(it.tokens, it.hk, 0, 0);
+      }
     }
     if (there) {
       derive(it);
@@ -645,36 +680,22 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 }
 
 constexpr int PG_COLS = 8, PG_AHEAD = 4;
-// Adds up the pieces of blocks that were cut: a CTA has 8 columns of one block, a warp 32 of its rows, a lane one of them. Which block that is is
-// found before the first kernel has ended. Two or three pieces of many rows want warps on an SM, many pieces of few rows loads of a warp on
+// Adds up the pieces of blocks that were cut: a CTA has 8 columns of one block, a warp 32 of its rows, a lane one of them. Where a block's pieces are is
+// left in memory by the CTA that has the first: most CTAs here begin when the first kernel's registers are free, at its end, so that what they do to
+// find out would be waited for. Two or three pieces of many rows want warps on an SM, many pieces of few rows loads of a warp on
 // their way together: the whole call, us, with 2 / 4 (64 registers) / 8 pieces at a time, 512 new tokens over 7681 keys, 2 pieces 72 / 72 to 75 / 76, 5 over
 // 30000, 17 pieces 39.2 / 37.6 / 37.0, 16 over 2000, 16 pieces 14.2 / 12.5 / 12.3.
 template <int HD>
 __global__ void __launch_bounds__(256, 4) paged_join_kernel(const __grid_constant__ PagedAttn p) {
   constexpr int GROUPS = HD / PG_COLS;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = (blockIdx.x % GROUPS) * PG_COLS;
-  PgShape own{};
-  if (lane < p.seqs.B) own = pg_shape(p, lane);
-  PgItem it{};
-  const bool there = pg_find(p, own, blockIdx.x / GROUPS, PG_WHOLE, it);
-  const int t = warp >> 2, r = (warp & 3) * 32 + lane;                 // tile and row in it
-  const int rows = max(0, min(p.tq, it.tokens - t * p.tq)) * p.G;      // of the tile
-  const bool mine = there && r < rows;
+  const int block = blockIdx.x / GROUPS, t = warp >> 2, r = (warp & 3) * 32 + lane;       // block, tile and row in it
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int U = *p.plan;
-  if (!__any_sync(0xffffffffu, mine) || U == PG_WHOLE) return;
-  const PgShape s = pg_shape(p, it.b);
-  const int pieces = (s.steps + U - 1) / U, blk = (it.token - p.seqs.first(it.b)) / (2 * p.tq);
-  if (pieces == 1) return;
-  int before = 0;                  // items of the sequences in front
-  for (int i = lane; i < it.b; i += 32) {
-    const PgShape o = pg_shape(p, i);
-    before += o.blocks * ((o.steps + U - 1) / U);
-  }
-  before = __reduce_add_sync(0xffffffffu, before) * p.Hkv;
-  const int steps = it.steps(2 * p.tq);
-  const long long item = before + ((long long)(s.blocks - 1 - blk) * p.Hkv + it.hk) * pieces;
-  if (item + pieces > p.items || !mine) return;            // sequences that overlap in `cu`: not all items were run
+  const int cut = *p.cut;
+  const int4 a = p.where[2 * block], b = p.where[2 * block + 1];     // items of the block from a.x on, how many, its steps of keys, its first token; tokens, KV head
+  const int pieces = a.y, steps = a.z, rows = max(0, min(p.tq, b.x - t * p.tq)) * p.G;         // rows of the tile
+  const long long item = a.x;
+  if (block >= cut || pieces == 1 || item + pieces > p.items || r >= rows) return;
   const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + item * p.rows + t * PG_TILE + r;
   const float* part = p.part + (item * p.rows + t * PG_TILE + r - lane) * HD + col * 32 + lane * 4;
   // a piece that has no keys was not run; there are such where a block has fewer steps than pieces
@@ -721,7 +742,7 @@ __global__ void __launch_bounds__(256, 4) paged_join_kernel(const __grid_constan
   uint4 u;
   u.x = pack_bf16x2(o[0] * inv, o[1] * inv); u.y = pack_bf16x2(o[2] * inv, o[3] * inv);
   u.z = pack_bf16x2(o[4] * inv, o[5] * inv); u.w = pack_bf16x2(o[6] * inv, o[7] * inv);
-  *reinterpret_cast<uint4*>(p.out + (long long)(it.token + t * p.tq + r / p.G) * p.ldo + (it.hk * p.G + r % p.G) * HD + col) = u;
+  *reinterpret_cast<uint4*>(p.out + (long long)(a.w + t * p.tq + r / p.G) * p.ldo + (b.y * p.G + r % p.G) * HD + col) = u;
 }
 
 static int pg_map(CUtensorMap* out, const void* base, int rank, const cuuint64_t* dims, const long long* strides, const cuuint32_t* box) {
@@ -798,7 +819,7 @@ static bool pg_call(PgCall& c, int B, int T, bool one_each, bool ones, long long
   c.blocks = (int)items;
   c.items = c.slots ? 2 * sms : (int)items;
   c.rows = one_each || T <= PG_TILE / G ? PG_TILE : 2 * PG_TILE;       // blocks of one tile, or of two
-  c.ws = c.slots ? 256 + 4ll * c.items * c.rows * (D + 2) : 0;
+  c.ws = c.slots ? 256 + 32ll * c.blocks + 4ll * c.items * c.rows * (D + 2) : 0;
   return true;
 }
 
@@ -837,8 +858,9 @@ GF_API int gf_paged_attn(const PagedCall* c, float scale, void* ws, long long ws
   p.skip_ones = ones != 0;
   p.out = (__nv_bfloat16*)c->y; p.ldo = c->ldy;
   if (n.slots) {
-    p.plan = (int*)ws;
-    p.part = (float*)((char*)ws + 256);
+    p.cut = (int*)ws;
+    p.where = (int4*)((char*)ws + 256);
+    p.part = (float*)((char*)ws + 256 + 32ll * n.blocks);
     p.part_ml = p.part + (long long)n.items * n.rows * D;
   }
   cudaStream_t st = (cudaStream_t)stream;
