@@ -39,7 +39,7 @@ constexpr float PG_RESCALE = 8.0f;  // log2 units
 
 struct PagedAttn {
   PagedBatch seqs;
-  int Hq, Hkv, G, tq;            // G = Hq / Hkv, tq = 128 / G tokens of a tile
+  int Hq, Hkv, G, tq, tb;        // G = Hq / Hkv, tq = 128 / G tokens of a tile, tb of a block: tq or two times that
   int slots;                     // CTAs that run at a time; 0: no block is cut
   int skip_ones;                 // sequences of one new token are not this kernel's
   float scale;
@@ -71,9 +71,9 @@ __device__ __forceinline__ PgShape pg_shape(const PagedAttn& p, int b) {
   if (p.skip_ones && s.n == 1) s.n = 0;
   s.len = p.seqs.lens[b];
   s.keys = (int)min((long long)max(s.len, 0), p.seqs.capacity());
-  s.blocks = (s.n + 2 * p.tq - 1) / (2 * p.tq);
+  s.blocks = (s.n + p.tb - 1) / p.tb;
   s.steps = max(1, (s.keys + PG_TILE - 1) / PG_TILE);
-  s.short_end = s.n - (s.blocks - 1) * 2 * p.tq <= p.tq;
+  s.short_end = s.n - (s.blocks - 1) * p.tb <= p.tq;
   return s;
 }
 
@@ -124,9 +124,9 @@ struct PgItem {
 };
 __device__ __forceinline__ void pg_block(const PagedAttn& p, PgItem& it, const PgShape& s, int b, int blk) {
   it.b = b;
-  it.token = p.seqs.first(b) + blk * 2 * p.tq;
-  it.tokens = min(2 * p.tq, s.n - blk * 2 * p.tq);
-  it.pos = s.len - s.n + blk * 2 * p.tq;
+  it.token = p.seqs.first(b) + blk * p.tb;
+  it.tokens = min(p.tb, s.n - blk * p.tb);
+  it.pos = s.len - s.n + blk * p.tb;
   it.len = s.len;
   it.keys = s.keys;
 }
@@ -168,7 +168,7 @@ __device__ __forceinline__ bool pg_find(const PagedAttn& p, const PgShape& own, 
         it.pieces = each;
       }
       pg_block(p, it, s, base + l, blk);
-      const int steps = it.steps(2 * p.tq);
+      const int steps = it.steps(p.tb);
       it.hk = in;
       it.piece = it.j0 = 0;
       it.j1 = steps;
@@ -285,7 +285,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       if (there) shared_item = it;
       if (p.slots && blockIdx.x == 0) *p.cut = U == PG_WHOLE || !there ? 0 : whole;
       if (U != PG_WHOLE && there && it.piece == 0 && it.block < p.blocks) {
-        p.where[2 * it.block] = make_int4(blockIdx.x, it.pieces, it.steps(2 * p.tq), it.token);
+        p.where[2 * it.block] = make_int4(blockIdx.x, it.pieces, it.steps(p.tb), it.token);
         p.where[2 * it.block + 1] = make_int4(it.tokens, it.hk, 0, 0);
       }
     }
@@ -805,20 +805,24 @@ static int launch_join(const PagedAttn& p, cudaStream_t st) {
 // second kernel), nor beside the decode kernel (`ones`) when that has more to do: a step of keys of all KV heads of all sequences takes it as long
 // as a step takes here, 2 us, with 1.25 of them for every SM. 31 sequences of up to 2048 keys with one token and one with 4 / 30 / 481, 32 / 8 heads, cut / not: 60
 // / 46, 62 / 47, 56 / 56 us.
+//
+// Over those few steps blocks have one tile's rows where as many run at one time, half of the SMs' beside the decode kernel: each takes half as long. us, two
+// tiles / one: 61 tokens over 414 keys, 32 / 8 heads of 128 16.7 / 12.0, a prompt of 469, 16 / 1 heads 16.4 / 12.7, of 200, 32 / 8 heads 12.6 / 10.1.
 struct PgCall {
-  int items, rows, slots, blocks;
+  int items, rows, slots, blocks, tb;
   long long ws;
 };
 static bool pg_call(PgCall& c, int B, int T, bool one_each, bool ones, long long keys, int Hq, int Hkv, int D, int sms) {
-  const int G = Hq / Hkv, w = 2 * (PG_TILE / G);
-  const long long blocks = one_each ? B : min((long long)T, ((long long)T + (long long)B * (w - 1)) / w);
-  const long long items = blocks * Hkv;
+  const int tq = PG_TILE / (Hq / Hkv);
+  auto blocks_of = [&](int tb) { return one_each ? (long long)B : min((long long)T, ((long long)T + (long long)B * (tb - 1)) / tb); };
+  c.tb = keys <= 4 * PG_TILE && blocks_of(tq) * Hkv <= (ones ? sms / 2 : sms) ? tq : 2 * tq;
+  const long long items = blocks_of(c.tb) * Hkv;
   if (items > 0x7fffffffll) return false;
   const bool beside = ones && 4ll * B * Hkv >= 5ll * sms;
   c.slots = items < 2 * sms && keys > 4 * PG_TILE && !beside ? sms : 0;
   c.blocks = (int)items;
   c.items = c.slots ? 2 * sms : (int)items;
-  c.rows = one_each || T <= PG_TILE / G ? PG_TILE : 2 * PG_TILE;       // blocks of one tile, or of two
+  c.rows = one_each || T <= tq ? PG_TILE : 2 * PG_TILE;       // blocks of one tile, or of two
   c.ws = c.slots ? 256 + 32ll * c.blocks + 4ll * c.items * c.rows * (D + 2) : 0;
   return true;
 }
@@ -853,7 +857,7 @@ GF_API int gf_paged_attn(const PagedCall* c, float scale, void* ws, long long ws
   if (!pg_call(n, B, T, !p.seqs.cu, ones != 0, p.seqs.capacity(), Hq, Hkv, D, sm_count())) return GFH_TOO_LARGE;
   if (ws_bytes < n.ws || (n.ws && !ws)) return GFH_BAD_ARG;
   gf::enter();
-  p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.tq = PG_TILE / p.G;
+  p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.tq = PG_TILE / p.G; p.tb = n.tb;
   p.slots = n.slots; p.scale = scale; p.rows = n.rows; p.items = n.items; p.blocks = n.blocks;
   p.skip_ones = ones != 0;
   p.out = (__nv_bfloat16*)c->y; p.ldo = c->ldy;
