@@ -15,7 +15,7 @@
 // vector's are one load; bits, with a counter at each set one's rank, are a third of that, but took 11.4 / 51 us for 64 / 512 rows instead of 8.0 / 47: two
 // rounds over the tokens, ranks between them, and three looks for each vector.
 //
-// What bounds it: 512 rows of 50257 in fp32, 2048 to 4096 tokens, a bias for all and a mask each, take 47 us (4.5 TB/s); a pass without any of them 33 (6.2), with
+// What bounds it: issue slots, 79 % of them taken: 512 rows of 50257 in fp32, 2048 to 4096 tokens, a bias for all and a mask each, take 47 us (4.5 TB/s); a pass without any of them 33 (6.2), with
 // the mask 35, and the bias 43 (from L2 once more for every row; it comes by the same way as the tokens, 50 MB for three slices of a row), the mask and the
 // tokens 44. One vector of a thread at a time, without the ring, took 95. Small batches: 64 rows 8.0 us, two or three 3.3.
 #include <cuda_fp16.h>
