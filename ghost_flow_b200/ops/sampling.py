@@ -136,13 +136,19 @@ def process_logits(logits, tokens=None, token_lens=None, generated_from=None, re
 def next_tokens(logits, temperature: float = 0.0, tokens=None, token_lens=None, generated_from=None, prompt: int | None = None,
                 repetition=1.0, presence=0.0, frequency=0.0, bias=None, allowed=None):
     """The next token ``[B, 1]`` of every row of ``logits [B, V]``: the likeliest (temperature 0) or a sampled one, after
-    :func:`process_logits` where ``tokens``, a bias or a mask are given. ``prompt``: the number of tokens of every row that are its prompt,
-    in place of ``generated_from``."""
-    if tokens is not None or bias is not None or allowed is not None:
+    :func:`process_logits` where ``tokens``, a bias or a mask are given: -1 then for a row that they leave nothing of (all ``-inf``), for which
+    an embedding has zeros and :func:`process_logits` no penalty. Sampling takes the likeliest token of a row that has no probabilities (it
+    holds what is not a number, or infinity). ``prompt``: the number of tokens of every row that are its prompt, in place of ``generated_from``."""
+    processed = tokens is not None or bias is not None or allowed is not None
+    if processed:
         if tokens is not None and generated_from is None and prompt is not None:
             generated_from = torch.full((logits.shape[0],), prompt, dtype=torch.int32, device=logits.device)
         logits = process_logits(logits, tokens, token_lens if tokens is not None else None, generated_from if tokens is not None else None,
                                 repetition, presence, frequency, bias, allowed)
+    likeliest = chosen = logits.argmax(-1, keepdim=True)
     if temperature and temperature > 0:
-        return torch.multinomial(torch.softmax(logits.float() / temperature, -1), 1)
-    return logits.argmax(-1, keepdim=True)
+        # multinomial stops the device at a row that is no distribution; softmax leaves nothing but NaN of one
+        p = torch.softmax(logits.float() / temperature, -1)
+        none = p[:, :1].isnan()
+        chosen = torch.where(none, likeliest, torch.multinomial(p.masked_fill(none, 1.0), 1))
+    return torch.where(logits.gather(-1, likeliest) == float("-inf"), -1, chosen) if processed else chosen
