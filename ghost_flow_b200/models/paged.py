@@ -53,17 +53,22 @@ class PagedKVCache:
 
     def batch(self, sequences, lens, new=None) -> PagedBatch:
         """The batch of ``sequences`` with ``lens`` keys each, of which the last ``new`` (one, without it) are new tokens. Their pages have to be
-        reserved."""
+        reserved. A sequence may come more than once (parts of a prompt; any number of empty slots), but no position of it be new twice."""
         sequences, lens = list(sequences), [int(n) for n in lens]
         new = None if new is None else [int(n) for n in new]
         if len(sequences) != len(lens) or (new is not None and len(new) != len(lens)):
             raise ValueError(f"{len(sequences)} sequences, {len(lens)} lengths and {None if new is None else len(new)} numbers of new tokens")
-        pages = [self._pages.get(s, []) for s in sequences]
-        for s, n, m, have in zip(sequences, lens, new or lens, pages):
+        pages, written = [self._pages.get(s, []) for s in sequences], {}
+        for s, n, m, have in zip(sequences, lens, [min(n, 1) for n in lens] if new is None else new, pages):
             if n > len(have) * self.page_size:
                 raise ValueError(f"sequence {s!r} has {len(have)} pages of {self.page_size} rows, not room for {n} keys")
             if not 0 <= m <= n:
                 raise ValueError(f"sequence {s!r} has {n} keys, {m} of them new")
+            if m > 0:
+                spans = written.setdefault(s, [])
+                if any(n - m < end and start < n for start, end in spans):
+                    raise ValueError(f"sequence {s!r} is there more than once with new tokens at the same positions")
+                spans.append((n - m, n))
         B, width = len(lens), max(map(len, pages), default=0)
         ints = [p for have in pages for p in (*have, *[-1] * (width - len(have)))] + lens
         if new is not None:
