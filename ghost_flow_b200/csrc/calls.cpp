@@ -296,7 +296,7 @@ PyObject* logits(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Py_RETURN_NONE;
   }
   if (!penalty(a[4], B, device, c.repetition0, c.repetition) || !penalty(a[5], B, device, c.presence0, c.presence) ||
-      !penalty(a[6], B, device, c.frequency0, c.frequency) || !(c.repetition || c.repetition0 > 0))
+      !penalty(a[6], B, device, c.frequency0, c.frequency) || !(c.repetition || (c.repetition0 >= 0x1p-126 && c.repetition0 <= 0x1p126)))
     Py_RETURN_NONE;
   // [V] for all rows or [B, V]
   auto rows = [&](PyObject* o, int code, long long wide, const void*& data, long long& ld) {

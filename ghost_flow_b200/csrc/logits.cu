@@ -8,6 +8,8 @@
 //   x = x - (c frequency + (c > 0) presence)
 //   x = x + bias[v]
 //   x = allowed ? x : -inf                                   all in 32 bits, rounded once
+// x / repetition is x (1 / repetition), one rounding more: with a quotient the pass spills, 61 us for 55 (512 rows of 50257 in fp32, 4096 tokens, bias and
+// mask). Callers bound the repetition so that the reciprocal is a normal number.
 //
 // One CTA has a slice of one row. The row's tokens, each with a thread, count themselves at the entry that they hold; then a pass over the slice, 16
 // bytes at a time, does the arithmetic, whose first vectors were asked for before the tokens were looked at. Counters are whole numbers:

@@ -67,8 +67,8 @@ def _check(logits, tokens, token_lens, generated_from, repetition, presence, fre
         if torch.is_tensor(t):
             if t.shape != (B,) or t.dtype is not torch.float32 or t.device != dev:
                 raise ValueError(f"{what}: {name} is a number or fp32 [{B}] on {dev}, not {t.dtype} {list(t.shape)} on {t.device}")
-    if not torch.is_tensor(repetition) and not repetition > 0:
-        raise ValueError(f"{what}: repetition is above 0, not {repetition}")
+    if not torch.is_tensor(repetition) and not 2.0 ** -126 <= repetition <= 2.0 ** 126:
+        raise ValueError(f"{what}: repetition is above 0, from 2^-126 to 2^126, not {repetition}")
     if bias is not None and (bias.shape not in ((V,), (B, V)) or bias.dtype is not torch.float32 or bias.device != dev):
         raise ValueError(f"{what}: bias is fp32 [{V}] or [{B}, {V}] on {dev}, not {bias.dtype} {list(bias.shape)} on {bias.device}")
     words = (V + 31) // 32
@@ -99,11 +99,12 @@ def process_logits(logits, tokens=None, token_lens=None, generated_from=None, re
                    allowed=None, out=None):
     """Logits ``[B, V]`` ready for the choice of a token. For an entry that stands ``c`` times among the row's generated tokens, in this order:
     if the row's ``tokens`` hold it at all, ``x / repetition`` where ``x > 0`` and ``x * repetition`` elsewhere, and then
-    ``x - (c * frequency + presence where c > 0)``; ``x + bias``; ``-inf`` unless ``allowed``. Computed in 32 bits and rounded once.
+    ``x - (c * frequency + presence where c > 0)``; ``x + bias``; ``-inf`` unless ``allowed``. Computed in 32 bits (the kernel multiplies by
+    ``1 / repetition``) and rounded once.
 
     ``tokens [B, L]``, int32 or int64, holds ``token_lens[b]`` tokens (int32 ``[B]``; all ``L``) of which those from ``generated_from[b]``
     (int32 ``[B]``; 0) are generated ones, those before them the prompt; a token outside the vocabulary (padding) is passed over. The
-    three penalties are numbers or fp32 ``[B]``. ``bias``: fp32 ``[V]`` or ``[B, V]``. ``allowed``: int32 bits ``[words]`` or ``[B, words]``
+    three penalties are numbers or fp32 ``[B]``, ``repetition`` from 2^-126 to 2^126, where it and its reciprocal have all their bits. ``bias``: fp32 ``[V]`` or ``[B, V]``. ``allowed``: int32 bits ``[words]`` or ``[B, words]``
     (:func:`pack_allowed`). ``out`` may be ``logits`` itself. A row of which nothing is allowed is all ``-inf``."""
     call = None
     if logits.get_device() >= 0 and not _is_compiling():

@@ -1,0 +1,20 @@
+"""Arguments of what stands between logits and a token: ranges, and what goes with what."""
+import pytest
+import torch
+
+import _paged_oracle as oracle
+from ghost_flow_b200 import ops
+
+
+@pytest.mark.parametrize("r", [1e-39, 2.0 ** -127, 2.0 ** 127, float("inf"), float("nan"), 0.0, -2.0])
+def test_a_repetition_whose_reciprocal_has_fewer_bits_is_refused(r):
+    with pytest.raises(ValueError, match="repetition"):
+        ops.process_logits(torch.zeros(2, 8), torch.zeros(2, 4, dtype=torch.int32), repetition=r)
+
+
+@pytest.mark.parametrize("r", [2.0 ** -126, 3e-38, 2.0 ** 126, 5e37])
+def test_the_ends_of_the_range(r):
+    x = torch.tensor([[1e-3, -1e-3, 0.0, 5.0]])
+    t = torch.tensor([[0, 1, 2]], dtype=torch.int32)
+    want, off = oracle.logits(x, t, r=r)
+    oracle.close(ops.process_logits(x, t, repetition=r), want, off)
