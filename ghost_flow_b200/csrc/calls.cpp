@@ -160,7 +160,7 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   long long heads;
   bool packed;
   View cs, sn;
-  if (followed({a[0], a[3], a[4]})) Py_RETURN_NONE;
+  if (followed({a[0], a[3], a[4], a[8], a[9]})) Py_RETURN_NONE;
   if (!paged(a, a[3], a[4], a[5], a[6], a[7], r.c, device, heads, packed) || H <= 0 || H > MOST || r.c.Hk != Hk || heads != H + 2 * Hk ||
       r.c.D % 16 || r.c.D > 4096 || !cs.of(a[8]) || !sn.of(a[9]))
     Py_RETURN_NONE;
