@@ -3,6 +3,7 @@
 // and the C error codes of the library.
 #pragma once
 #include <atomic>
+#include <mutex>
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -55,12 +56,22 @@ struct DeviceOnce {
   bool todo() { return done[device()].load(std::memory_order_acquire) == 0; }
   void mark() { done[device()].store(1, std::memory_order_release); }
 };
-// The same for attributes that only ever grow (dynamic shared-memory limit raised to the largest request so far).
-struct DeviceMax {
+// The limit of a kernel's dynamic shared memory, which only ever grows, per device. One thread at a time raises it: of two that both see the old limit the
+// one with less to ask for could set its own last, and the other's be what is remembered.
+struct SharedLimit {
   std::atomic<size_t> value[64];
-  DeviceMax() { for (auto& v : value) v.store(0); }
-  size_t get() { return value[DeviceOnce::device()].load(std::memory_order_acquire); }
-  void set(size_t v) { value[DeviceOnce::device()].store(v, std::memory_order_release); }
+  std::mutex raising;
+  SharedLimit() { for (auto& v : value) v.store(0); }
+  template <typename Kernel>
+  bool raise(Kernel* kernel, size_t bytes) {
+    auto& limit = value[DeviceOnce::device()];
+    if (bytes <= limit.load(std::memory_order_acquire)) return true;
+    std::lock_guard<std::mutex> one(raising);
+    if (bytes <= limit.load(std::memory_order_relaxed)) return true;
+    if (cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) return false;
+    limit.store(bytes, std::memory_order_release);
+    return true;
+  }
 };
 // Checked build: the 8-int status buffer of the current device (registered with gf_set_check_buffer), for kernels
 // whose exported signature has no status pointer. Null when none was registered.

@@ -257,12 +257,9 @@ static int launch_logits(LogitsParams& p, long long B, cudaStream_t st) {
   p.slices = (p.V + p.slice - 1) / p.slice;
   if (B * p.slices > 0x7fffffffll) return GFH_TOO_LARGE;
   const size_t smem = 16 * lg_stages(bits) * LG_THREADS + 4 * lg_words(p.slice) + (p.slice + 8) * bits / 8;
-  static gf::DeviceMax granted[3];
+  static gf::SharedLimit limit[3];
   auto kern = bits == 0 ? logits_kernel<T, 0> : bits == 16 ? logits_kernel<T, 16> : logits_kernel<T, 32>;
-  if (smem > 48 * 1024 && granted[bits / 16].get() < smem) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return GFH_CUDA;
-    granted[bits / 16].set(smem);
-  }
+  if (smem > 48 * 1024 && !limit[bits / 16].raise(kern, smem)) return GFH_CUDA;
   kern<<<(unsigned)(B * p.slices), LG_THREADS, smem, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? GFH_OK : GFH_CUDA;
 }

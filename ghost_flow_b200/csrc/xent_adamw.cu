@@ -374,12 +374,8 @@ GF_API int gf_xent_fused(const void* logits, const long long* targets, float* lo
   if ((reinterpret_cast<uintptr_t>(logits) & 15) || (reinterpret_cast<uintptr_t>(dlogits) & 15)) return GFH_BAD_ARG;
   const size_t smem = (size_t)v8 * 2;
   if (smem > 200 * 1024) return GFH_TOO_LARGE;
-  static gf::DeviceMax configured;
-  if (smem > configured.get()) {
-    if (cudaFuncSetAttribute(xent_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-      return GFH_CUDA;
-    configured.set(smem);
-  }
+  static gf::SharedLimit limit;
+  if (!limit.raise(xent_kernel, smem)) return GFH_CUDA;
   long long per_sm = (long long)(XENT_SMEM / (smem + 2048));   // 1 KB of static and reserved shared memory each, rounded up
   per_sm = per_sm < 1 ? 1 : per_sm > XENT_CTAS ? XENT_CTAS : per_sm;
   const long long most = per_sm * sm_count();
