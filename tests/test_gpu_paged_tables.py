@@ -33,3 +33,15 @@ def test_a_gradient_of_the_tables_alone_is_recorded(learned, kernel_status):
         assert ((t.grad - want).abs() <= off).all()
     with torch.no_grad():
         assert torch.equal(ops.rope_qkv_to_pages(s["qkv"], H, Hk, *tables, s["kp"], s["vp"], *args), plain)
+
+
+@pytest.mark.parametrize("lens,new", [([40, 9], [1, 1]), ([300, 70, 9], [33, 70, 1])])
+@pytest.mark.parametrize("scale", [1e-50, -1e-50, 2e-46, 0.0])
+def test_a_scale_below_all_numbers_of_32_bits(scale, lens, new, kernel_status):
+    from ghost_flow_b200 import ops
+
+    s = oracle.batch(lens, new, 8, 2, 64, 16, device="cuda")
+    args = s["q"], s["kp"], s["vp"], s["table"], s["lens"], None if set(new) == {1} else s["cu"]
+    oracle.close(ops.paged_attention(*args, scale=scale), *oracle.attention(s, scale))
+    with pytest.raises(ValueError, match="scale"):
+        ops.paged_attention(*args, scale=2.0 ** 127)
