@@ -105,7 +105,7 @@ def process_logits(logits, tokens=None, token_lens=None, generated_from=None, re
     ``tokens [B, L]``, int32 or int64, holds ``token_lens[b]`` tokens (int32 ``[B]``; all ``L``) of which those from ``generated_from[b]``
     (int32 ``[B]``; 0) are generated ones, those before them the prompt; a token outside the vocabulary (padding) is passed over. The
     three penalties are numbers or fp32 ``[B]``, ``repetition`` from 2^-126 to 2^126, where it and its reciprocal have all their bits. ``bias``: fp32 ``[V]`` or ``[B, V]``. ``allowed``: int32 bits ``[words]`` or ``[B, words]``
-    (:func:`pack_allowed`). ``out`` may be ``logits`` itself. A row of which nothing is allowed is all ``-inf``."""
+    (:func:`pack_allowed`). Without ``tokens`` there is nothing that a penalty is for. ``out`` may be ``logits`` itself. A row of which nothing is allowed is all ``-inf``."""
     call = None
     if logits.get_device() >= 0 and not _is_compiling():
         call = _lib.calls().logits(logits, tokens, token_lens, generated_from, repetition, presence, frequency, bias, allowed)
@@ -140,6 +140,8 @@ def next_tokens(logits, temperature: float = 0.0, tokens=None, token_lens=None, 
     :func:`process_logits` where ``tokens``, a bias or a mask are given: -1 then for a row that they leave nothing of (all ``-inf``), for which
     an embedding has zeros and :func:`process_logits` no penalty. Sampling takes the likeliest token of a row that has no probabilities (it
     holds what is not a number, or infinity). ``prompt``: the number of tokens of every row that are its prompt, in place of ``generated_from``."""
+    if tokens is None and any(torch.is_tensor(t) or t != none for t, none in ((repetition, 1), (presence, 0), (frequency, 0))):
+        raise ValueError("next_tokens: penalties go with the tokens that they count")
     processed = tokens is not None or bias is not None or allowed is not None
     if processed:
         if tokens is not None and generated_from is None and prompt is not None:

@@ -18,3 +18,11 @@ def test_the_ends_of_the_range(r):
     t = torch.tensor([[0, 1, 2]], dtype=torch.int32)
     want, off = oracle.logits(x, t, r=r)
     oracle.close(ops.process_logits(x, t, repetition=r), want, off)
+
+
+@pytest.mark.parametrize("kw", [dict(repetition=1.5), dict(presence=0.1), dict(frequency=-0.1), dict(repetition=torch.ones(2)),
+                                dict(presence=torch.zeros(2), bias=torch.zeros(8))], ids=lambda k: "-".join(k))
+def test_a_choice_with_penalties_and_nothing_to_count_is_refused(kw):
+    with pytest.raises(ValueError, match="next_tokens"):
+        ops.next_tokens(torch.zeros(2, 8), **kw)
+    ops.next_tokens(torch.zeros(2, 8), repetition=1.0, presence=0, frequency=0.0)
