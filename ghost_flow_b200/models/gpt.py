@@ -149,10 +149,10 @@ class GPTForCausalLM(Module):
             x, c = blk.forward_cached(x, (None, None))
             caches.append(c)
         logits = self.lm_head(t.ln_f(x))[:, -1]
-        out = [ids]
+        out, counted = [ids], ops.sampling.counts_tokens(choice)
         pos = ids.shape[1]
         for _ in range(max_new_tokens):
-            nxt = ops.next_tokens(logits, temperature, torch.cat(out, 1) if choice else None, prompt=ids.shape[1], **choice)
+            nxt = ops.next_tokens(logits, temperature, torch.cat(out, 1) if counted else None, prompt=ids.shape[1], **choice)
             out.append(nxt)
             if pos >= self.cfg.n_positions:
                 break

@@ -253,10 +253,10 @@ class LLaMAForCausalLM(Module):
         B, S = ids.shape
         caches = self.new_caches(B, S + max_new_tokens)
         logits = self.forward(ids, caches=caches, start_pos=0)[:, -1]
-        out = [ids]
+        out, counted = [ids], ops.sampling.counts_tokens(choice)
         pos = S
         for _ in range(max_new_tokens):
-            nxt = ops.next_tokens(logits, temperature, torch.cat(out, 1) if choice else None, prompt=S, **choice)
+            nxt = ops.next_tokens(logits, temperature, torch.cat(out, 1) if counted else None, prompt=S, **choice)
             out.append(nxt)
             logits = self.forward(nxt, caches=caches, start_pos=pos)[:, -1]
             pos += 1
@@ -305,9 +305,9 @@ class LLaMAForCausalLM(Module):
             tokens[b, :lens[b]] = t
         count = torch.tensor(lens, dtype=torch.int32, device=p.device)
         first = count.clone()
-        batch = cache.batch(range(B), [n + 1 for n in lens])
+        batch, counted = cache.batch(range(B), [n + 1 for n in lens]), ops.sampling.counts_tokens(choice)
         for i in range(max_new_tokens):
-            nxt = ops.next_tokens(logits, temperature, tokens if choice else None, count, first, **choice)
+            nxt = ops.next_tokens(logits, temperature, tokens if counted else None, count, first, **choice)
             tokens.scatter_(1, count.long()[:, None], nxt)
             count += 1
             if i + 1 < max_new_tokens:

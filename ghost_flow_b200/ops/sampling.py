@@ -134,6 +134,11 @@ def process_logits(logits, tokens=None, token_lens=None, generated_from=None, re
     return y
 
 
+def counts_tokens(choice) -> bool:
+    """Whether keyword arguments of :func:`next_tokens` have a penalty, which wants to know the tokens so far."""
+    return not choice.keys().isdisjoint(("repetition", "presence", "frequency"))
+
+
 def next_tokens(logits, temperature: float = 0.0, tokens=None, token_lens=None, generated_from=None, prompt: int | None = None,
                 repetition=1.0, presence=0.0, frequency=0.0, bias=None, allowed=None):
     """The next token ``[B, 1]`` of every row of ``logits [B, V]``: the likeliest (temperature 0) or a sampled one, after

@@ -66,3 +66,26 @@ def test_generation_goes_on_beside_a_row_that_nothing_is_left_of(kind, temperatu
     assert live.min() >= 0 and live.max() < 97
     if not temperature:
         assert torch.equal(got[[0, 2]], make(ids[[0, 2]], ops.pack_allowed(ok[[0, 2]])))
+
+
+@pytest.mark.parametrize("kind", ["llama", "gpt", "llama pages"])
+def test_tokens_are_counted_for_penalties_only(kind, monkeypatch):
+    torch.manual_seed(0)
+    if kind == "gpt":
+        m = GPTForCausalLM(GPTConfig(vocab_size=97, n_positions=64, n_embd=32, n_layer=1, n_head=2, n_inner=64, dropout=0.0)).eval()
+    else:
+        m = LLaMAForCausalLM(LLaMAConfig(vocab_size=97, hidden_size=64, intermediate_size=96, num_hidden_layers=1, num_attention_heads=4,
+                                         num_key_value_heads=2, max_position_embeddings=32), dtype=torch.float32).eval()
+    seen, plain = [], ops.sampling.process_logits
+
+    def process(logits, tokens=None, *a, **kw):
+        seen.append(tokens is not None)
+        return plain(logits, tokens, *a, **kw)
+
+    monkeypatch.setattr(ops.sampling, "process_logits", process)
+    ids = torch.randint(0, 97, (2, 5))
+    for choice, counted in ((dict(bias=torch.zeros(97)), False), (dict(allowed=ops.pack_allowed(torch.ones(97))), False),
+                            (dict(bias=torch.zeros(97), presence=0.1), True), (dict(repetition=1.5), True), (dict(frequency=0.5), True)):
+        seen.clear()
+        m.generate_batch(list(ids), 3, **choice) if kind == "llama pages" else m.generate(ids, 3, **choice)
+        assert seen == [counted] * 3
