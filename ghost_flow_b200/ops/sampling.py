@@ -25,8 +25,8 @@ def _logits_ref(x, tokens, token_lens, generated_from, repetition, presence, fre
     B, V = x.shape
     y = x.to(torch.promote_types(x.dtype, torch.float32))
 
-    def column(a):
-        return a[:, None] if torch.is_tensor(a) else a
+    def column(a):         # (a number beside whole numbers would be of the default type)
+        return a[:, None] if torch.is_tensor(a) else torch.full((), a, dtype=y.dtype, device=y.device)
 
     if tokens is not None and tokens.shape[1] > 0:
         t, j = tokens.long(), torch.arange(tokens.shape[1], device=x.device)

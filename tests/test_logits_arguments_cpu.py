@@ -26,3 +26,21 @@ def test_a_choice_with_penalties_and_nothing_to_count_is_refused(kw):
     with pytest.raises(ValueError, match="next_tokens"):
         ops.next_tokens(torch.zeros(2, 8), **kw)
     ops.next_tokens(torch.zeros(2, 8), repetition=1.0, presence=0, frequency=0.0)
+
+
+@pytest.mark.parametrize("default", [torch.float16, torch.bfloat16, torch.float64])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float64])
+def test_numbers_keep_their_bits_whatever_the_default_type(default, dtype):
+    x = torch.randn(3, 40, dtype=torch.float64).to(dtype)
+    t = torch.randint(0, 40, (3, 30), dtype=torch.int32)
+    kw = dict(r=1.2345678, p=0.3333333, f=0.1234567)
+    want, off = oracle.logits(x, t, **kw)
+    if dtype is torch.float64:             # 64 bits throughout: six operations, each off by half a step of what it works on
+        off = 6 * 2.0 ** -53 * (x.abs() + 30)
+    torch.set_default_dtype(default)
+    try:
+        got = ops.process_logits(x, t, repetition=kw["r"], presence=kw["p"], frequency=kw["f"])
+    finally:
+        torch.set_default_dtype(torch.float32)
+    assert got.dtype is dtype
+    oracle.close(got, want, off)
