@@ -13,10 +13,10 @@ from .paged import _is_compiling, _ranges_overlap
 
 
 def pack_allowed(mask):
-    """Bits of a truth-valued mask ``[..., V]`` for :func:`process_logits`: int32 ``[..., ceil(V / 32)]``, entry ``v`` is bit ``v % 32`` of word
-    ``v // 32``."""
+    """Bits of a mask ``[..., V]`` (truth values; numbers that are not 0) for :func:`process_logits`: int32 ``[..., ceil(V / 32)]``, entry ``v``
+    is bit ``v % 32`` of word ``v // 32``."""
     V = mask.shape[-1]
-    m = torch.nn.functional.pad(mask.to(torch.int64), (0, -V % 32)).unflatten(-1, (-1, 32))
+    m = torch.nn.functional.pad((mask != 0).long(), (0, -V % 32)).unflatten(-1, (-1, 32))
     words = (m << torch.arange(32, device=mask.device)).sum(-1)
     return torch.where(words >= 2 ** 31, words - 2 ** 32, words).to(torch.int32)
 

@@ -44,3 +44,11 @@ def test_numbers_keep_their_bits_whatever_the_default_type(default, dtype):
         torch.set_default_dtype(torch.float32)
     assert got.dtype is dtype
     oracle.close(got, want, off)
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.uint8, torch.float32])
+def test_masks_of_numbers(dtype):
+    mask = torch.tensor([[0, 2, 1, 0, 3] * 9, [5, 0, 0, 0, 0] * 9], dtype=dtype)
+    if dtype.is_floating_point:
+        mask[0, 1] = 0.5
+    assert torch.equal(ops.pack_allowed(mask), ops.pack_allowed(mask != 0))
