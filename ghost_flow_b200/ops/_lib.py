@@ -143,7 +143,7 @@ def calls():
             build()
         exchange = getattr(torch.Tensor, "__dlpack_c_exchange_api__", None)
         if exchange is None:
-            raise RuntimeError("this PyTorch has no DLPack C exchange interface (version 2.10 and later have it)")
+            raise RuntimeError(f"PyTorch {torch.__version__} has no DLPack C exchange interface; 2.11 has it")
         loader = importlib.machinery.ExtensionFileLoader("_gf_calls", str(path))
         module = importlib.util.module_from_spec(importlib.util.spec_from_file_location("_gf_calls", str(path), loader=loader))
         loader.exec_module(module)
