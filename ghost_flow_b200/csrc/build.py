@@ -137,15 +137,21 @@ def build(force: bool = False, verbose: bool = False, checked: bool = True) -> d
                       "-c", str(src), "-o", str(obj)], src, obj))
         python_objs.append(obj)
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 2)) as ex:
-        futs = []
+        futs, python_error = [], None
         for cmd, src, obj in jobs:
             stamp = obj.with_suffix(".stamp")
             digest = _digest(src, " ".join(cmd))
             if force and stamp.exists():
                 stamp.unlink()
-            futs.append(ex.submit(_compile_one, cmd, src, obj, stamp, digest, verbose))
-        for f in futs:
-            msg = f.result()
+            futs.append((ex.submit(_compile_one, cmd, src, obj, stamp, digest, verbose), obj))
+        for f, obj in futs:
+            try:
+                msg = f.result()
+            except RuntimeError as e:
+                if obj not in python_objs:
+                    raise
+                python_error = e       # (without Python's headers) the libraries do not need it
+                continue
             if verbose:
                 print(msg)
     out = {}
@@ -176,6 +182,8 @@ def build(force: bool = False, verbose: bool = False, checked: bool = True) -> d
             if r.returncode != 0:
                 raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
         out["host"] = lib
+    if python_error is not None:
+        raise python_error
     lib = LIB_DIR / "_gf_calls.so"
     if force or not lib.exists() or lib.stat().st_mtime < max(o.stat().st_mtime for o in python_objs):
         r = subprocess.run(["g++", "-shared", "-o", str(lib), *map(str, python_objs)], capture_output=True, text=True)
