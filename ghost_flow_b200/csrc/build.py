@@ -3,7 +3,8 @@
 ``libgfb200.so``   - every CUDA kernel (sm_100a only) behind a C ABI, loaded with ctypes.
 ``libghostflow.so`` - the C ABI of the reference's ``ghostflow.h`` plus the checkpoint
                       readers/writers (host C++ only, no CUDA needed to load it).
-``_gf_calls.so``    - Python module through which operators of short calls reach ``libgfb200.so``.
+``_gf_calls.*.so``  - Python module through which operators of short calls reach ``libgfb200.so``, with the interpreter that it was
+                      built for in its name.
 
 Usage: ``python -m ghost_flow_b200.csrc.build [--force] [--verbose]``.
 """
@@ -11,6 +12,7 @@ from __future__ import annotations
 
 import concurrent.futures as cf
 import hashlib
+import importlib.machinery
 import os
 import shutil
 import subprocess
@@ -60,6 +62,7 @@ CUDA_SOURCES = [
 ]
 
 PYTHON_SOURCES = ["calls.cpp"]
+CALLS_NAME = "_gf_calls" + importlib.machinery.EXTENSION_SUFFIXES[0]
 HOST_SOURCES = ["cabi.cpp", "formats.cpp", "cpu_ref.cpp", "symm_alloc.cpp"]
 
 
@@ -184,7 +187,7 @@ def build(force: bool = False, verbose: bool = False, checked: bool = True) -> d
         out["host"] = lib
     if python_error is not None:
         raise python_error
-    lib = LIB_DIR / "_gf_calls.so"
+    lib = LIB_DIR / CALLS_NAME
     if force or not lib.exists() or lib.stat().st_mtime < max(o.stat().st_mtime for o in python_objs):
         r = subprocess.run(["g++", "-shared", "-o", str(lib), *map(str, python_objs)], capture_output=True, text=True)
         if r.returncode != 0:

@@ -136,14 +136,14 @@ def calls():
     """The Python module that looks at an operator's tensors and launches on ``libgfb200.so`` (``csrc/calls.cpp``); both are built if missing."""
     global _CALLS
     if _CALLS is None:
-        lib, path = cuda_lib(), _PKG / "lib" / "_gf_calls.so"
-        if not path.exists():
-            from ..csrc.build import build
+        from ..csrc.build import CALLS_NAME, build
 
-            build()
         exchange = getattr(torch.Tensor, "__dlpack_c_exchange_api__", None)
         if exchange is None:
             raise RuntimeError(f"PyTorch {torch.__version__} has no DLPack C exchange interface; 2.11 has it")
+        lib, path = cuda_lib(), _PKG / "lib" / CALLS_NAME
+        if not path.exists():
+            build()
         loader = importlib.machinery.ExtensionFileLoader("_gf_calls", str(path))
         module = importlib.util.module_from_spec(importlib.util.spec_from_file_location("_gf_calls", str(path), loader=loader))
         loader.exec_module(module)

@@ -1,4 +1,5 @@
 """What is built, for which interpreter, and what does not need what."""
+import importlib.machinery
 import re
 from pathlib import Path
 
@@ -6,6 +7,13 @@ import pytest
 import torch
 
 from ghost_flow_b200.csrc import build as b
+from ghost_flow_b200.ops import _lib
+
+
+def test_the_module_is_this_interpreters():
+    suffix = importlib.machinery.EXTENSION_SUFFIXES[0]
+    path = Path(_lib.calls().__file__)
+    assert path.name == "_gf_calls" + suffix and suffix.count(".") == 2 and path.parent == b.LIB_DIR
 
 
 def test_the_declared_pytorch_has_the_interface_that_operators_go_through():
@@ -22,7 +30,7 @@ def test_the_libraries_are_linked_where_the_module_cannot_be_compiled(tmp_path, 
         monkeypatch.setattr(b, name, value)
     with pytest.raises(RuntimeError, match="module.cpp"):
         b.build(checked=False)
-    assert (tmp_path / "lib" / "libghostflow.so").exists() and not (tmp_path / "lib" / "_gf_calls.so").exists()
+    assert (tmp_path / "lib" / "libghostflow.so").exists() and not (tmp_path / "lib" / b.CALLS_NAME).exists()
     (tmp_path / "host.cpp").write_text("no c++")
     with pytest.raises(RuntimeError, match="host.cpp"):
         b.build(checked=False)
