@@ -167,7 +167,7 @@ def layer_norm(x, w, b=None, eps: float = 1e-5):
 
 
 # ------------------------------------------------------------------------------------------ RoPE
-_ROPE_CACHE = {}
+_ROPE_CACHE = {}      # kept for good: a captured step goes on reading the tables of its time when a model has taken longer ones
 
 
 def rope_tables(seq_len: int, head_dim: int, theta: float = 10000.0, device="cpu"):
