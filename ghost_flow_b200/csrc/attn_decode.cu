@@ -727,7 +727,7 @@ namespace gf {
 
 // Groups of at most 8 query heads to a KV head; 0 where they are not equal, or more than two: the keys are read again for every group, and the
 // tiles for prompts are then as fast. With two, us here / there: 2 sequences of 300 .. 3000 keys, 16 / 1 heads of 128 9.6 / 15.5, 16 of them
-// 12.7 / 16.4, 32 of them with 32 / 2 heads 28.0 / 26.7.
+// 12.7 / 16.4; with much to read the tiles come level, 32 of them with 32 / 2 heads 28.0 / 26.7, which no rule is made for.
 static int head_groups(long long H, long long Hk) {
   if (H <= 0 || Hk <= 0 || H % Hk) return 0;
   const long long G = H / Hk;

@@ -20,9 +20,10 @@
 // result is of P before that: a result is 0.0020 to 0.0023 of its norm off, of which its own rounding to bf16 is 0.0017. (The decode kernel, which
 // memory bounds, takes P in two terms.)
 //
-// What bounds it. Whole prompts: as attn_fwd3.cu, tensor pipe and exponentials, 1.9 us for a step of 256 rows; us, dense / pages of 64 / 16:
-// [1, 4096] with 32 / 8 heads of 128 133 / 135 / 136 (1000 TFLOP/s), [4, 2987] with 32 / 32 heads 325 / 327 / 327, [8, 1024] with 12 / 12 heads of 64 44 /
-// 49 / 49 (a CTA has 8 steps at most there, and finds its block, pages and queries in 3 us). The next 512 tokens over 7681 keys, 32 / 8 heads: 71 us
+// What bounds it. Whole prompts: a step of 256 rows takes 1.9 us, 0.8 of the tensor rate (exponentials share it, as in attn_fwd3.cu), and every CTA some 7 us
+// beside its steps (first scores after 5.2 us, results 5.3 us behind the last step), which nothing covers: a CTA has its SM to itself. 15712 steps of
+// 1344 blocks on 148 SMs are 202 us without the second and 271 with it, measured 269. us, dense / pages of 64 / 16: [1, 4096] with 32 / 8 heads of 128 133 / 135 /
+// 136 (1000 TFLOP/s), [4, 2987] with 32 / 32 heads 325 / 327 / 327, [8, 1024] with 12 / 12 heads of 64 44 / 49 / 49 (8 steps of a CTA at most). The next 512 tokens over 7681 keys, 32 / 8 heads: 71 us
 // (870 TFLOP/s), two pieces of 64 blocks on 128 of 148 SMs, 60 of it in steps. A block of one tile takes half as long and is cut into half as many pieces: 284
 // tokens over 5983 keys, 25 / 25 heads of 64, 40 us, with as many as the others 53. Few rows: keys come at 6 TB/s while steps run, and the ends of it, 5 us
 // in front and 6 behind with the second kernel, are what is left: 5 tokens over 30000 keys 35 us (3.5 TB/s), 16 over 2000 12.
@@ -808,6 +809,10 @@ static int launch_join(const PagedAttn& p, cudaStream_t st) {
 //
 // Over those few steps blocks have one tile's rows where as many run at one time, half of the SMs' beside the decode kernel: each takes half as long. us, two
 // tiles / one: 61 tokens over 414 keys, 32 / 8 heads of 128 16.7 / 12.0, a prompt of 469, 16 / 1 heads 16.4 / 12.7, of 200, 32 / 8 heads 12.6 / 10.1.
+//
+// `keys` is what the page table has room for: the host knows no lengths. A table that is wider than its sequences (a captured step's) gives up the
+// last two rules: a prompt of 200, 32 / 8 heads, its own table / one for 4096 keys 16.4 / 22.5, four of them 20.5 / 26.6 (L2 flushed). Every sequence counts
+// as if it had part of a block, those of one token too, which have none beside the decode kernel: the CTAs without a block leave.
 struct PgCall {
   int items, rows, slots, blocks, tb;
   long long ws;

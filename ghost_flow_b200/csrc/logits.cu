@@ -19,7 +19,8 @@
 //
 // What bounds it: issue slots, 79 % of them taken: 512 rows of 50257 in fp32, 2048 to 4096 tokens, a bias for all and a mask each, take 47 us (4.5 TB/s); a pass without any of them 33 (6.2), with
 // the mask 35, and the bias 43 (from L2 once more for every row; it comes by the same way as the tokens, 50 MB for three slices of a row), the mask and the
-// tokens 44. One vector of a thread at a time, without the ring, took 95. Small batches: 64 rows 8.0 us, two or three 3.3.
+// tokens 44. One vector of a thread at a time, without the ring, took 95. Small batches: 64 rows 8.0 us, two or three 3.3. Three CTAs on an SM leave a thread
+// 40 registers: enough for fp32 with 16-bit counters (36); the 16-bit types spill 28 bytes with counters and 8 without, fp32 with 32-bit counters 44.
 #include <cuda_fp16.h>
 
 #include "calls.h"
@@ -110,7 +111,7 @@ __global__ void __launch_bounds__(LG_THREADS, LG_CTAS) logits_kernel(const __gri
   };
   int n = 0;
   float rep = 1.f, less = 1.f, pres = 0.f, freq = 0.f;
-  if (BITS && p.tokens) {                          // (there are, with BITS; without the test the pass is compiled to spill, 53 us for 47)
+  if (BITS && p.tokens) {                          // (there are, with BITS; without the test the pass of fp32 is compiled to spill, 53 us for 47)
     int t[LG_TOKENS];                              // LG_TOKENS tokens of the thread from i0 on: their entries, -1 for what is not in the slice
     auto tokens = [&](int i0) {
 #pragma unroll

@@ -162,7 +162,9 @@ def rope_qkv_to_pages(qkv, num_heads: int, num_kv_heads: int, cos, sin, kpages, 
 
 # ------------------------------------------------------------------------------------------ attention
 # A batch of this many sequences may be a server's, most of which have one new token: those then go to the decode kernel, which reads keys
-# twice as fast as the tiles for prompts do.
+# twice as fast as the tiles for prompts do, for one or two launches more. us, tiles alone / decode kernel beside them, 32 / 8 heads of 128, one chunk and the
+# others one token over up to so many keys: 2 sequences, 64 new tokens over 500 18 / 23, 512 over 8000 53 / 68; 7 sequences, 64 over 500 18 / 27, 64 over 2000
+# 31 / 35, 512 over 2000 43 / 47, 64 over 8000 68 / 74, but 512 over 8000 129 / 96.
 _MANY = 8
 
 
