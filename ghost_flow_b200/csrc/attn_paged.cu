@@ -23,8 +23,8 @@
 // What bounds it. Whole prompts: a step of 256 rows takes 1.9 us, 0.8 of the tensor rate (exponentials share it, as in attn_fwd3.cu), and every CTA some 7 us
 // beside its steps (first scores after 5.2 us, results 5.3 us behind the last step), which nothing covers: a CTA has its SM to itself. 15712 steps of
 // 1344 blocks on 148 SMs are 202 us without the second and 271 with it, measured 269. us, dense / pages of 64 / 16: [1, 4096] with 32 / 8 heads of 128 133 / 135 /
-// 136 (1000 TFLOP/s), [4, 2987] with 32 / 32 heads 325 / 327 / 327, [8, 1024] with 12 / 12 heads of 64 44 / 49 / 49 (8 steps of a CTA at most). The next 512 tokens over 7681 keys, 32 / 8 heads: 71 us
-// (870 TFLOP/s), two pieces of 64 blocks on 128 of 148 SMs, 60 of it in steps. A block of one tile takes half as long and is cut into half as many pieces: 284
+// 136 (1000 TFLOP/s), [4, 2987] with 32 / 32 heads 325 / 327 / 327, [8, 1024] with 12 / 12 heads of 64 44 / 49 / 49 (8 steps of a CTA at most).
+// The next 512 tokens over 7681 keys, 32 / 8 heads: 71 us (870 TFLOP/s), two pieces of 64 blocks on 128 of 148 SMs, 60 of it in steps. A block of one tile takes half as long and is cut into half as many pieces: 284
 // tokens over 5983 keys, 25 / 25 heads of 64, 40 us, with as many as the others 53. Few rows: keys come at 6 TB/s while steps run, and the ends of it, 5 us
 // in front and 6 behind with the second kernel, are what is left: 5 tokens over 30000 keys 35 us (3.5 TB/s), 16 over 2000 12.
 #include "paged.cuh"

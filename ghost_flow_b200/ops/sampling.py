@@ -104,8 +104,9 @@ def process_logits(logits, tokens=None, token_lens=None, generated_from=None, re
 
     ``tokens [B, L]``, int32 or int64, holds ``token_lens[b]`` tokens (int32 ``[B]``; all ``L``) of which those from ``generated_from[b]``
     (int32 ``[B]``; 0) are generated ones, those before them the prompt; a token outside the vocabulary (padding) is passed over. The
-    three penalties are numbers or fp32 ``[B]``, ``repetition`` from 2^-126 to 2^126, where it and its reciprocal have all their bits. ``bias``: fp32 ``[V]`` or ``[B, V]``. ``allowed``: int32 bits ``[words]`` or ``[B, words]``
-    (:func:`pack_allowed`). Without ``tokens`` there is nothing that a penalty is for. ``out`` may be ``logits`` itself. A row of which nothing is allowed is all ``-inf``."""
+    three penalties are numbers or fp32 ``[B]``, ``repetition`` from 2^-126 to 2^126, where it and its reciprocal have all their bits. Without
+    ``tokens`` there is nothing that a penalty is for. ``bias``: fp32 ``[V]`` or ``[B, V]``. ``allowed``: int32 bits ``[words]`` or ``[B, words]``
+    (:func:`pack_allowed`). ``out`` may be ``logits`` itself. A row of which nothing is allowed is all ``-inf``."""
     call = None
     if logits.get_device() >= 0 and not _is_compiling():
         call = _lib.calls().logits(logits, tokens, token_lens, generated_from, repetition, presence, frequency, bias, allowed)
@@ -157,6 +158,6 @@ def next_tokens(logits, temperature: float = 0.0, tokens=None, token_lens=None, 
     if temperature and temperature > 0:
         # multinomial stops the device at a row that is no distribution; softmax leaves nothing but NaN of one
         p = torch.softmax(logits.float() / temperature, -1)
-        none = p[:, :1].isnan()
+        none = p[..., :1].isnan()
         chosen = torch.where(none, likeliest, torch.multinomial(p.masked_fill(none, 1.0), 1))
     return torch.where(logits.gather(-1, likeliest) == float("-inf"), -1, chosen) if processed else chosen

@@ -89,3 +89,10 @@ def test_tokens_are_counted_for_penalties_only(kind, monkeypatch):
         seen.clear()
         m.generate_batch(list(ids), 3, **choice) if kind == "llama pages" else m.generate(ids, 3, **choice)
         assert seen == [counted] * 3
+
+
+def test_logits_of_one_row_alone():
+    x = torch.tensor([0.0, 4.0, NAN])
+    for temperature in (0.0, 0.5):
+        assert ops.next_tokens(x[:2] * 100, temperature).tolist() == [1] and ops.next_tokens(x, temperature).tolist() == [2]
+        assert ops.next_tokens(torch.zeros(0, 5), temperature).shape == (0, 1)
