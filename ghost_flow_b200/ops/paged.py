@@ -255,10 +255,11 @@ def paged_attention(q, kpages, vpages, page_table, lens, cu=None, scale: float |
         at, device, B, T, H, Hk, D, keys, packed = call
     if out is not None and (_ranges_overlap(out, q) or _ranges_overlap(out, kpages) or _ranges_overlap(out, vpages)):
         raise ValueError(f"{what}: out shares memory with q or the pages")
-    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if not abs(scale) <= 2.0 ** 126:         # (in units of log 2 it is a number of 32 bits too)
-        raise ValueError(f"{what}: a scale of {scale}")
-    if abs(scale) < 2.0 ** -149:             # no number of 32 bits
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    elif not 2.0 ** -149 <= abs(scale := float(scale)) <= 2.0 ** 126:
+        if not abs(scale) < 1.0:             # in units of log 2 it is no number of 32 bits
+            raise ValueError(f"{what}: a scale of {scale}")
         scale = 0.0
     if call is None:
         return _attention_ref(q, kpages, vpages, page_table, lens, cu, scale, out)
