@@ -52,6 +52,7 @@ CUDA_SOURCES = [
     "paged_cache.cu",
     "attn_paged.cu",
     "logits.cu",
+    "sample.cu",
     "transformer_block.cu",
     "comm_kernels.cu",
     "moe_kernels.cu",

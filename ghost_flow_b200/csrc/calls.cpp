@@ -40,6 +40,7 @@ int (*f_append)(const gf::PagedCall*, const float*, const float*, int, int, void
 int (*f_attn)(const gf::PagedCall*, float, void*, long long, int, float*, void*);
 int (*f_attn_one)(const gf::PagedCall*, float, int, float*, void*);
 int (*f_logits)(const gf::LogitsCall*, void*);
+int (*f_sample)(const gf::SampleCall*, void*);
 // what the operators' `_observed` asks (ops/fused.py), here without its Python frames (0.15 us instead of 0.6), and whether gradients are recorded
 PyObject *tracing, *transforms, *dispatch_modes, *function_modes, *only_device_contexts, *forward_ad, *grad_enabled, *requires_grad, *current_level;
 
@@ -331,6 +332,73 @@ PyObject* run_logits(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return PyLong_FromLong(rc);
 }
 
+// A choice: a number from `least` to `most`, or one of 32 bits of every row.
+bool choice(PyObject* o, long long B, int device, int code, double least, double most, double& number, const void*& rows) {
+  View v;
+  if (PyFloat_Check(o) || PyLong_Check(o) || !v.of(o)) {
+    number = PyFloat_AsDouble(o);
+    if (!PyErr_Occurred()) return number >= least && number <= most && (code != INT || number == (double)(long long)number);
+    PyErr_Clear();
+    return false;
+  }
+  if (!v.is(code, 32, 1, device) || v.shape[0] != B || v.stride(0, 1) != 1) return false;
+  rows = v.data;
+  return true;
+}
+
+// sample(logits, u, temperature, top_k, top_p, min_p): (call, device, B), None as above
+PyObject* sample(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!arguments("sample", n, 6)) return nullptr;
+  gf::SampleCall c{};
+  View x, u;
+  if (followed({a[0], a[1], a[2], a[4], a[5]}) || !x.of(a[0]) || x.ndim != 2) Py_RETURN_NONE;
+  const int device = x.device;
+  c.dtype = x.is(FLOAT, 32, 2, device) ? 0 : x.is(BFLOAT, 16, 2, device) ? 1 : x.is(FLOAT, 16, 2, device) ? 2 : 3;
+  c.B = x.shape[0];
+  c.V = x.shape[1];
+  if (c.dtype == 3 || c.B == 0 || c.V == 0 || c.V > 1 << 20 || x.stride(1, 1) != 1 || !u.floats(a[1], c.B, device)) Py_RETURN_NONE;
+  c.x = x.data;
+  c.ldx = x.stride(0, c.V);
+  c.u = (const float*)u.data;
+  const void *t = nullptr, *k = nullptr, *p = nullptr, *least = nullptr;
+  double top_k = 0;
+  constexpr double TINY = 0x1p-149;                // (a share of 0 is none)
+  if (!choice(a[2], c.B, device, FLOAT, 0, 0x1p127, c.temperature0, t) || !choice(a[3], c.B, device, INT, 0, MOST, top_k, k) ||
+      !choice(a[4], c.B, device, FLOAT, TINY, 1, c.top_p0, p) || !choice(a[5], c.B, device, FLOAT, 0, 1, c.min_p0, least))
+    Py_RETURN_NONE;
+  c.temperature = (const float*)t;
+  c.top_k = (const int*)k;
+  c.top_k0 = (long long)top_k;
+  c.top_p = (const float*)p;
+  c.min_p = (const float*)least;
+  return Py_BuildValue("(y#iL)", (const char*)&c, (Py_ssize_t)sizeof c, device, c.B);
+}
+
+// run_sample(call, out, stream)
+PyObject* run_sample(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  gf::SampleCall c;
+  View y;
+  if (!arguments("run_sample", n, 3) || !call_of(a[0], c) || !memory_of(a[1], y)) return nullptr;
+  c.out = (long long*)y.data;
+  void* stream = PyLong_AsVoidPtr(a[2]);
+  if (PyErr_Occurred()) return nullptr;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = f_sample(&c, stream);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(rc);
+}
+
+// bind_more(addresses of gf_sample_tokens)
+PyObject* bind_more(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!arguments("bind_more", n, 1)) return nullptr;
+  void* f[1];
+  for (int i = 0; i < 1; ++i) f[i] = PyLong_AsVoidPtr(a[i]);
+  if (PyErr_Occurred()) return nullptr;
+  f_sample = (decltype(f_sample))f[0];
+  Py_RETURN_NONE;
+}
+
 // bind(exchange interface, addresses of gf_paged_append, gf_paged_attn, gf_paged_attn_one, gf_process_logits, the functions and the module that `followed`
 // asks)
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -364,7 +432,8 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 #define FN(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {FN(bind), FN(append), FN(run_append), FN(attention), FN(run_attention), FN(logits), FN(run_logits), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {FN(bind), FN(append), FN(run_append), FN(attention), FN(run_attention), FN(logits), FN(run_logits), FN(sample), FN(run_sample),
+                         FN(bind_more), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_gf_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -34,4 +34,15 @@ struct LogitsCall {
   long long lda;
 };
 
+struct SampleCall {
+  const void* x;                 // [B, V] of dtype (0 fp32, 1 bf16, 2 fp16), rows ldx apart
+  long long ldx, dtype, B, V;
+  const float* u;                // [B]; the rest as in SampleParams of sample.cu
+  const float *temperature, *top_p, *min_p;
+  const int* top_k;
+  double temperature0, top_p0, min_p0;
+  long long top_k0;
+  long long* out;                // [B]
+};
+
 }  // namespace gf

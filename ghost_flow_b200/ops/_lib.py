@@ -79,6 +79,7 @@ _SIGS = {
     "gf_paged_attn": [P, F, P, L, I, P, P],
     "gf_paged_attn_one": [P, F, I, P, P],
     "gf_process_logits": [P, P],
+    "gf_sample_tokens": [P, P],
     "gf_flash_attn_bwd": [P, P, P, P, P, P, P, P, P, I, I, I, I, I, L, L, L, L, L, L, F, I, P, P],
     "gf_attn_bwd_prep": [P, P, P, P, I, I, I, I, L, L, P],
     "gf_flash_attn_bwd3": [P, P, P, P, P, P, P, P, P, I, I, I, I, I, L, L, L, L, L, L, F, I, P, P],
@@ -151,6 +152,7 @@ def calls():
 
         module.bind(exchange, *(ctypes.cast(getattr(lib, name), c_void_p).value for name in (
             "gf_paged_append", "gf_paged_attn", "gf_paged_attn_one", "gf_process_logits")), *follows())
+        module.bind_more(*(ctypes.cast(getattr(lib, name), c_void_p).value for name in ("gf_sample_tokens",)))
         _CALLS = module
     return _CALLS
 

@@ -1,7 +1,7 @@
 """What stands between a model's logits and the choice of a token: penalties for tokens that are there already, biases, and masks of the
 tokens that a grammar allows. The reference picks the largest logit (ghostflow-nn/src/gpt.rs:402-422).
 
-CUDA logits of fp32, bf16 or fp16 take the kernel of ``csrc/logits.cu``; CPU tensors, other layouts, and calls that something follows (a
+CUDA logits of fp32, bf16 or fp16 take the kernels of ``csrc/logits.cu`` and ``csrc/sample.cu``; CPU tensors, other layouts, and calls that something follows (a
 gradient, tracing, transforms, modes) plain PyTorch."""
 from __future__ import annotations
 
@@ -135,17 +135,78 @@ def process_logits(logits, tokens=None, token_lens=None, generated_from=None, re
     return y
 
 
+def _sample_ref(x, u, temperature, top_k, top_p, min_p):
+    B, V = x.shape
+
+    def column(a, dtype=torch.float64):
+        return a.to(dtype)[:, None] if torch.is_tensor(a) else torch.full((B, 1), a, dtype=dtype, device=x.device)
+
+    likeliest = x.argmax(-1, keepdim=True)               # what is not a number before all others
+    top = x.gather(-1, likeliest).double()
+    t, k, p, least = column(temperature), column(top_k, torch.int64), column(top_p), column(min_p).nan_to_num(1.0).clamp(max=1.0)
+    share = column(u).nan_to_num(0.0).clamp(0.0, 1.0 - 2.0 ** -24)
+    sampled = (t > 0) & (k != 1) & ~(p <= 0) & top.isfinite()
+    y, order = torch.sort(torch.where(sampled, x.double(), 0.0), dim=-1, descending=True, stable=True)
+    w = torch.exp((y - y[:, :1]) / torch.where(sampled, t, 1.0))
+    w = torch.where((k <= 0) | (torch.arange(V, device=x.device) < k), w, 0.0)
+    upto = w.cumsum(-1)
+    stays = (~(p < 1) | (upto - w < p * upto[:, -1:])) & (w >= least)
+    upto = torch.zeros_like(w).scatter_(1, order, torch.where(stays, w, 0.0)).cumsum(-1)
+    chosen = (upto <= share * upto[:, -1:]).sum(-1, keepdim=True)
+    return torch.where(top == float("-inf"), -1, torch.where(sampled, chosen, likeliest))
+
+
+def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """A token ``[B, 1]`` for every row of ``logits [B, V]`` from one random number each, ``u`` fp32 ``[B]`` from 0 up to, but not, 1 (``torch.rand``).
+    With ``w = exp((x - max x) / temperature)`` and the row's tokens in the order of their logits, equal ones in that of the vocabulary: the first ``top_k`` stay
+    (0: all), of these each in front of which less than ``top_p`` of their weights' sum stands (1: all), of these those with ``w >= min_p``, the first
+    one in any case. The result is the first token, in the order of the vocabulary, up to which the weights of those that stay exceed ``u`` of their
+    sum. Weights, sums and shares are of 64 bits.
+
+    The four choices are numbers or one of each row: fp32 ``[B]``, ``top_k`` int32 ``[B]``. A temperature that is not above 0 takes the likeliest token, as do ``top_k`` 1 and
+    rows that have no probabilities (that hold what is not a number, or infinity); a row of all ``-inf`` gives -1."""
+    call = None
+    if logits.get_device() >= 0 and not _is_compiling():
+        call = _lib.calls().sample(logits, u, temperature, top_k, top_p, min_p)
+    if call is None:
+        what = "sample_tokens"
+        if logits.dim() != 2 or not logits.is_floating_point() or logits.shape[1] == 0:
+            raise ValueError(f"{what}: logits are [rows, vocabulary], not {logits.dtype} {list(logits.shape)}")
+        B, dev = logits.shape[0], logits.device
+        for name, t, dtype in (("u", u, torch.float32), ("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
+                               ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+            if torch.is_tensor(t) and (t.shape != (B,) or t.dtype is not dtype or t.device != dev):
+                raise ValueError(f"{what}: {name} is of each row {dtype} [{B}] on {dev}, not {t.dtype} {list(t.shape)} on {t.device}")
+        if not torch.is_tensor(u):
+            raise ValueError(f"{what}: u is fp32 [{B}], a random number for each row, not {u!r}")
+        for name, t, ok in (("temperature", temperature, lambda t: t >= 0), ("top_k", top_k, lambda t: t >= 0 and t == int(t)),
+                            ("top_p", top_p, lambda t: 0 < t <= 1), ("min_p", min_p, lambda t: 0 <= t <= 1)):
+            if not torch.is_tensor(t) and not ok(t):
+                raise ValueError(f"{what}: a {name} of {t}")
+        return _sample_ref(logits, u, temperature, top_k, top_p, min_p)
+    at, device, B = call
+    stream = _lib.stream_on(device)
+    if stream is None:
+        with torch.cuda.device(device):
+            return sample_tokens(logits, u, temperature, top_k, top_p, min_p)
+    out = torch.empty((B, 1), dtype=torch.int64, device=logits.device)
+    _rc(_lib.calls().run_sample(at, out, stream), "gf_sample_tokens")
+    return out
+
+
 def counts_tokens(choice) -> bool:
     """Whether keyword arguments of :func:`next_tokens` have a penalty, which wants to know the tokens so far."""
     return not choice.keys().isdisjoint(("repetition", "presence", "frequency"))
 
 
 def next_tokens(logits, temperature: float = 0.0, tokens=None, token_lens=None, generated_from=None, prompt: int | None = None,
-                repetition=1.0, presence=0.0, frequency=0.0, bias=None, allowed=None):
+                repetition=1.0, presence=0.0, frequency=0.0, bias=None, allowed=None, top_k=0, top_p=1.0, min_p=0.0, u=None):
     """The next token ``[B, 1]`` of every row of ``logits [B, V]``: the likeliest (temperature 0) or a sampled one, after
     :func:`process_logits` where ``tokens``, a bias or a mask are given: -1 then for a row that they leave nothing of (all ``-inf``), for which
     an embedding has zeros and :func:`process_logits` no penalty. Sampling takes the likeliest token of a row that has no probabilities (it
-    holds what is not a number, or infinity). ``prompt``: the number of tokens of every row that are its prompt, in place of ``generated_from``."""
+    holds what is not a number, or infinity). ``prompt``: the number of tokens of every row that are its prompt, in place of ``generated_from``. With
+    ``top_k``, ``top_p``, ``min_p``, a temperature of each row or the random numbers ``u`` themselves it is :func:`sample_tokens` that chooses, from
+    ``torch.rand`` where ``u`` is not given."""
     if tokens is None and any(torch.is_tensor(t) or t != none for t, none in ((repetition, 1), (presence, 0), (frequency, 0))):
         raise ValueError("next_tokens: penalties go with the tokens that they count")
     processed = tokens is not None or bias is not None or allowed is not None
@@ -154,6 +215,8 @@ def next_tokens(logits, temperature: float = 0.0, tokens=None, token_lens=None, 
             generated_from = torch.full((logits.shape[0],), prompt, dtype=torch.int32, device=logits.device)
         logits = process_logits(logits, tokens, token_lens if tokens is not None else None, generated_from if tokens is not None else None,
                                 repetition, presence, frequency, bias, allowed)
+    if u is not None or any(torch.is_tensor(t) or t != none for t, none in ((temperature, temperature), (top_k, 0), (top_p, 1), (min_p, 0))):
+        return sample_tokens(logits, torch.rand(logits.shape[0], device=logits.device) if u is None else u, temperature, top_k, top_p, min_p)
     likeliest = chosen = logits.argmax(-1, keepdim=True)
     if temperature and temperature > 0:
         # multinomial stops the device at a row that is no distribution; softmax leaves nothing but NaN of one

@@ -1,0 +1,109 @@
+"""sample_tokens on the device against the definition: sizes, layouts, rows whose order has many equal entries, captured calls, other streams."""
+import pytest
+import torch
+
+import _sample_oracle as oracle
+
+pytestmark = pytest.mark.gpu
+INF, NAN = float("inf"), float("nan")
+
+
+def _rows(kind, B, V, dtype, lead=0, pad=0):
+    r = torch.randn(B, V, device="cuda")
+    r = {"random": 3 * r, "flat": 0.01 * r, "equal": torch.zeros_like(r), "two": (r > 1).float(), "far": 1e4 * r, "narrow": 100 + 0.1 * r,
+         "masked": torch.where(torch.rand_like(r) < 0.9, -INF, 2 * r), "lowest": torch.where(torch.rand_like(r) < 0.9, torch.finfo(dtype).min, 2 * r)}[kind]
+    x = torch.full((B, lead + V + pad), NAN, device="cuda").to(dtype)                # nothing beside a row is looked at
+    x[:, lead:lead + V] = r.to(dtype)
+    x[:, lead + V // 2] = 0.0
+    return x[:, lead:lead + V]
+
+
+def _check(x, u, **c):
+    from ghost_flow_b200 import ops
+    from ghost_flow_b200.ops import _lib
+
+    n = _lib.launch_count()
+    got = ops.sample_tokens(x, u, **c)
+    assert _lib.launch_count() == n + 1 and got.shape == (x.shape[0], 1) and got.dtype is torch.int64
+    assert got.flatten().tolist() == oracle.tokens(x, u, **c)
+
+
+CHOICES = [{}, dict(top_k=50), dict(top_p=0.9), dict(min_p=0.05), dict(top_k=2000, top_p=0.5), dict(top_k=20, top_p=0.75, min_p=0.125, temperature=0.5),
+           dict(top_p=0.999, temperature=4.0)]
+
+
+@pytest.mark.parametrize("kind", ["random", "flat", "equal", "two", "far", "narrow", "masked", "lowest"])
+@pytest.mark.parametrize("choice", CHOICES, ids=str)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_kinds_of_rows(kind, choice, dtype, kernel_status):
+    _check(_rows(kind, 3, 5003, dtype, 3, 5), torch.rand(3, device="cuda"), **choice)
+
+
+@pytest.mark.parametrize("V", [1, 2, 7, 8, 9, 511, 512, 513, 2048, 4095, 4097, 50257])
+@pytest.mark.parametrize("lead", [0, 1, 4])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_sizes(V, lead, dtype):
+    x, u = _rows("random", 2, V, dtype, lead, 3), torch.rand(2, device="cuda")
+    for c in ({}, dict(top_k=3), dict(top_k=max(2, V - 1)), dict(top_p=0.6)):
+        _check(x, u, **c)
+
+
+def test_the_largest_vocabulary_and_a_larger_one():
+    from ghost_flow_b200 import ops
+    from ghost_flow_b200.ops import sampling
+
+    for V in (1 << 20, (1 << 20) + 1):
+        x, u = torch.randn(2, V, device="cuda"), torch.rand(2, device="cuda")
+        assert torch.equal(ops.sample_tokens(x, u, top_p=0.8), sampling._sample_ref(x, u, 1.0, 0, 0.8, 0.0))
+
+
+def test_choices_of_each_row_and_rows_without_probabilities():
+    x = _rows("random", 9, 700, torch.bfloat16)
+    x[1, [5, 60]], x[2, [8, 9]], x[3] = NAN, INF, -INF
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    t = lambda v: torch.tensor(v, device="cuda")  # noqa: E731
+    _check(x, t([0.0, 0.5, 0.5, 0.5, 0.25, 1 - 2.0 ** -24, 0.5, 0.75, 0.125]),
+           temperature=t([1.0, 1.0, 1.0, 1.0, 0.0, 0.5, 2.0, 1e-3, 0.75]), top_k=ints([0, 0, 9, 3, 2, 600, 1, 800, 30]),
+           top_p=t([1.0, 0.5, 1.0, 0.5, 0.5, 0.75, 0.5, 1.0, 0.25]), min_p=t([0.0, 0.0, 0.5, 0.0, 0.0, 2.0 ** -10, 0.5, 1.0, 0.0]))
+
+
+def test_rows_behind_32_bit_offsets():
+    free = torch.cuda.mem_get_info()[0]
+    if free < 12 << 30:
+        pytest.skip("not enough memory")
+    x = torch.empty(3, (1 << 30) + 64, dtype=torch.bfloat16, device="cuda")[:, :1000]
+    x.copy_(torch.randn(3, 1000, device="cuda"))
+    _check(x, torch.rand(3, device="cuda"), top_p=0.9)
+
+
+def test_captured_on_another_stream_and_twice_at_once():
+    from ghost_flow_b200 import ops
+
+    x, u, k = _rows("random", 4, 3001, torch.float32), torch.rand(4, device="cuda"), torch.full((4,), 40, dtype=torch.int32, device="cuda")
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        a, b = ops.sample_tokens(x, u, top_k=k), ops.sample_tokens(x, u, top_p=0.5)
+    other = ops.sample_tokens(x, u, 0.5)
+    torch.cuda.synchronize()
+    assert a.flatten().tolist() == oracle.tokens(x, u, top_k=k) and b.flatten().tolist() == oracle.tokens(x, u, top_p=0.5)
+    assert other.flatten().tolist() == oracle.tokens(x, u, 0.5)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        a, b = ops.sample_tokens(x, u, top_k=k), ops.next_tokens(x, 0.7, top_p=0.9)
+    x.copy_(_rows("random", 4, 3001, torch.float32))
+    u.uniform_()
+    k.fill_(7)
+    g.replay()
+    assert a.flatten().tolist() == oracle.tokens(x, u, top_k=k) and ((b >= 0) & (b < 3001)).all()
+
+
+def test_what_a_gradient_or_a_trace_follows_takes_other_operations():
+    from ghost_flow_b200 import ops
+    from ghost_flow_b200.ops import _lib
+
+    x, u = torch.randn(2, 90, device="cuda", requires_grad=True), torch.rand(2, device="cuda")
+    n = _lib.launch_count()
+    assert ops.sample_tokens(x, u, 0.5, 10).flatten().tolist() == oracle.tokens(x, u, 0.5, 10)
+    assert ops.sample_tokens(x.detach().t().contiguous().t(), u, 0.5).flatten().tolist() == oracle.tokens(x, u, 0.5)
+    assert _lib.launch_count() == n
