@@ -5,7 +5,7 @@
 // <= 8 query heads that share the KV head are processed together, so each cache row is read once, and softmax is kept online.
 // The pieces of a sequence are merged by a second kernel, which is on the machine before the first one ends. The cache read is
 // the only traffic that matters, and what bounds the kernel is how much of it is in flight, and where: every warp has its own
-// ring of DEC_STAGES blocks of 16 keys (K and V) filled by cp.async two blocks ahead, 128 KB on an SM, and neighbouring CTAs
+// ring of three blocks of 16 keys (K and V) filled by cp.async two blocks ahead, 128 KB on an SM, and neighbouring CTAs
 // read the same keys of neighbouring heads, which are one piece of memory (a head's row is 256 bytes; with the CTAs of a
 // sequence at different keys, 32 sequences of 4096 keys took 98 us instead of 86). A CTA that goes from one sequence to the
 // next loses about 4 us of its own.
@@ -35,7 +35,6 @@ namespace gf {
 constexpr int DEC_WARPS = 4;
 constexpr int DEC_MAX_G = 8;
 constexpr int DEC_KEYS = 16;     // keys of a block
-constexpr int DEC_STAGES = 3;
 constexpr int DEC_P_TERMS = 2;   // bf16 numbers that stand for a probability
 
 __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
@@ -45,6 +44,22 @@ __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
 __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// two e4m3 numbers of a word (the lower or the upper ones) as f16: exact
+template <int UPPER>
+__device__ __forceinline__ uint32_t f16x2_of_e4m3(uint32_t four) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((unsigned short)(UPPER ? four >> 16 : four)));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
   uint32_t r;
@@ -56,18 +71,20 @@ __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, uint3
   asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
-template <int D, bool SHARES>
+template <int D, bool SHARES, bool BYTES = false>
 struct DecCfg {
-  static constexpr int ROW = D * 2;
+  static constexpr int STAGES = BYTES ? 6 : 3;
+  static constexpr int ROW = BYTES ? D : D * 2;
   static constexpr int TILE = DEC_KEYS * ROW;          // K or V of a block
-  static constexpr int WARP_BYTES = DEC_STAGES * 2 * TILE;
+  static constexpr int STAGE = 2 * TILE + (BYTES ? 2 * DEC_KEYS : 0);      // and the rows' scales
+  static constexpr int WARP_BYTES = STAGES * STAGE;
   static constexpr int RING = DEC_WARPS * WARP_BYTES;
   static constexpr int PITCH = D + 4;                  // a head's sums, maximum and total; the pitch spreads a lane's heads over the banks
   static constexpr int SMEM = RING + (SHARES ? 2 * DEC_MAX_G * PITCH * 4 : 0);
   static constexpr int CTAS = D > 64 ? 2 : 4;          // on an SM
   static_assert(DEC_WARPS * DEC_MAX_G * PITCH * 4 <= RING, "results fit in the ring");
-  // 16-byte chunk c of row r lies at chunk c ^ (r % 8): ldmatrix meets every bank once, and rows fill whole lines
-  __device__ __forceinline__ static int chunk(int row, int col) { return (col ^ (row & 7)) << 4; }
+  // 16-byte chunk c of row r lies at chunk c ^ (r % 8), in rows of 64 bytes at c ^ (r / 2 % 4): ldmatrix meets every bank once, and rows fill whole lines
+  __device__ __forceinline__ static int chunk(int row, int col) { return (col ^ (ROW == 64 ? (row >> 1) & 3 : row & 7)) << 4; }
 };
 
 // How the keys are dealt out. A unit is 64 keys of one KV head (16 for each warp); an empty sequence has one. Neighbouring CTAs
@@ -104,6 +121,7 @@ struct DecParams {
   PagedBatch pages;
   int share;                    // more than 8 query heads to a KV head: in this many groups, each as if it had a KV head of its own
   long long kpage, krow, khead, vpage, vrow, vhead;
+  const unsigned char *kscales, *vscales;          // of pages of 8 bits (strides in bytes)
 };
 
 // Units of sequence b. In a paged batch with `cu`, one of other than one new token has none.
@@ -203,18 +221,23 @@ enum DecKind : int {
   DEC_SHARES = 2,    // splits == 0
   DEC_PAGES = 3,     // splits > 0, keys in pages
   DEC_PAGES_SHARES = 4,
+  DEC_PAGES8 = 5,    // the two over pages of 8 bits
+  DEC_PAGES8_SHARES = 6,
 };
-__host__ __device__ constexpr bool dec_shares(int kind) { return kind == DEC_SHARES || kind == DEC_PAGES_SHARES; }
+__host__ __device__ constexpr bool dec_shares(int kind) { return kind == DEC_SHARES || kind == DEC_PAGES_SHARES || kind == DEC_PAGES8_SHARES; }
+__host__ __device__ constexpr bool dec_bytes(int kind) { return kind == DEC_PAGES8 || kind == DEC_PAGES8_SHARES; }
 
 // Kinds of one piece to a CTA are compiled without what goes from one sequence to the next. With it, calls that the memory does
 // not bound took 5 to 25 % longer: us with / without it, 4 sequences of 64 keys, 64 / 8 heads of 64 3.8 / 3.1, 32 of 800, 32 /
 // 8 heads of 64 13.7 / 11.4, 32 of 200, 32 / 32 heads of 128 32.7 / 26.5. (Padded rows instead of the exchange of chunks are 10
 // % slower where memory bounds it: 32 of 4096 keys, 32 / 8 heads of 128 93 / 82: cp.async then fills lines in two parts.)
 template <int D, int KIND>
-__global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, dec_shares(KIND)>::CTAS)
+__global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, dec_shares(KIND), dec_bytes(KIND)>::CTAS)
 attn_decode_kernel(const __grid_constant__ DecParams p) {
-  constexpr bool SHARES = dec_shares(KIND), APPEND = KIND == DEC_APPEND, PAGED = KIND == DEC_PAGES || KIND == DEC_PAGES_SHARES;
-  using Cfg = DecCfg<D, SHARES>;
+  constexpr bool SHARES = dec_shares(KIND), APPEND = KIND == DEC_APPEND, BYTES = dec_bytes(KIND);
+  constexpr bool PAGED = KIND == DEC_PAGES || KIND == DEC_PAGES_SHARES || BYTES;
+  using Cfg = DecCfg<D, SHARES, BYTES>;
+  constexpr int STAGES = Cfg::STAGES;
   extern __shared__ __align__(128) uint8_t ring[];
   const DecWork& w = p.work;
   const int G = p.G;
@@ -273,8 +296,26 @@ attn_decode_kernel(const __grid_constant__ DecParams p) {
   auto load = [&](int st) {
     const int k0 = ahead.blk * 64 + warp * DEC_KEYS;
     if (ahead_units > 0 && k0 < ahead.len) {
-      const uint32_t dst = my + st * (2 * Cfg::TILE);
-      if constexpr (PAGED) {
+      const uint32_t dst = my + st * Cfg::STAGE;
+      if constexpr (BYTES) {
+        const bool there = page_ahead >= 0 && page_ahead < p.pages.pages;
+        if (!there && lane == 0) p.pages.bad();
+        const int r0 = k0 & ((1 << p.pages.page_shift) - 1);
+        const long long page = there ? page_ahead : 0;
+        const uint8_t* kb = reinterpret_cast<const uint8_t*>(p.kc) + page * p.kpage + r0 * p.krow + kv_head * p.khead;
+        const uint8_t* vb = reinterpret_cast<const uint8_t*>(p.vc) + page * p.vpage + r0 * p.vrow + kv_head * p.vhead;
+#pragma unroll
+        for (int n = 0; n < DEC_KEYS * D / 16 / 32; ++n) {
+          const int id = lane + n * 32, row = id / (D / 16), col = id % (D / 16);
+          const uint32_t to = dst + row * Cfg::ROW + Cfg::chunk(row, col), bytes = there && k0 + row < ahead.len ? 16u : 0u;
+          cp_async_16(to, kb + row * p.krow + col * 16, bytes);
+          cp_async_16(to + Cfg::TILE, vb + row * p.vrow + col * 16, bytes);
+        }
+        // 16 keys' scales: of rows behind the last key too, which no result depends on
+        if (lane < 2)
+          cp_async_16(dst + 2 * Cfg::TILE + lane * DEC_KEYS,
+                      (lane ? p.vscales : p.kscales) + ((page * (w.Hkv / p.share) + kv_head) << p.pages.page_shift) + r0, there ? 16u : 0u);
+      } else if constexpr (PAGED) {
         const bool there = page_ahead >= 0 && page_ahead < p.pages.pages;
         if (!there && lane == 0) p.pages.bad();
         const int r0 = k0 & ((1 << p.pages.page_shift) - 1);
@@ -326,22 +367,51 @@ attn_decode_kernel(const __grid_constant__ DecParams p) {
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll
-  for (int i = 0; i < DEC_STAGES - 1; ++i) load(i);
+  for (int i = 0; i < STAGES - 1; ++i) load(i);
   if (APPEND) asm volatile("griddepcontrol.wait;" ::: "memory");
 
   uint32_t qb[D / 16][2];          // Q^T as the 8-column operand: head r, dims 16 t + 2c, + 1 and + 8, + 9
   float o[D / 16][4];              // O^T: dims 16 j + r (+ 8), heads 2c, 2c + 1
   float m[2], l[2];
+  float mv[2], qf[2];              // BYTES: see `unit`
   uint4 k_new, v_new;              // append: chunk `lane` of the new token's rows, in the warp whose keys it belongs to
   // ---- start of a piece
   auto begin = [&] {
     if (PAGED && threadIdx.x == 0 && hk == 0 && w.lens[at.b] != at.len) p.pages.bad();
     const unsigned short* qp = reinterpret_cast<const unsigned short*>(
         p.q + (PAGED ? p.pages.first(at.b) : at.b) * p.ldq + (long long)(hk * G + min(r, G - 1)) * D + 2 * c);
+    if constexpr (BYTES) {
+      // head r, dims 16 t + 4c .. 4c + 3 (a word of K is four dims), as f16 in a unit of its own, which leaves them 11 bits down to 2^-14 of the largest
+      qp += 2 * c;
+      unsigned largest = 0;
+#pragma unroll
+      for (int t = 0; t < D / 16; ++t) {
+        qb[t][0] = r < G ? qp[16 * t] | ((uint32_t)qp[16 * t + 1] << 16) : 0u;
+        qb[t][1] = r < G ? qp[16 * t + 2] | ((uint32_t)qp[16 * t + 3] << 16) : 0u;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) largest = max(largest, max(qb[t][h] & 0x7fffu, (qb[t][h] >> 16) & 0x7fffu));
+      }
+      largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+      largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+      unsigned e = largest >> 7;
+      e = e == 255 ? 127 : min(max(e, 1u), 253u);
+      const float inv = __uint_as_float((254u - e) << 23);
+#pragma unroll
+      for (int t = 0; t < D / 16; ++t)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float2 f = unpack_bf16x2(qb[t][h]);
+          qb[t][h] = pack_f16x2(f.x * inv, f.y * inv);
+        }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) qf[i] = __uint_as_float(__shfl_sync(0xffffffffu, e, (2 * c + i) * 4) << 23) * p.scale_log2;
+      mv[0] = mv[1] = -INFINITY;
+    } else {
 #pragma unroll
     for (int t = 0; t < D / 16; ++t) {
       qb[t][0] = r < G ? qp[16 * t] | ((uint32_t)qp[16 * t + 1] << 16) : 0u;
       qb[t][1] = r < G ? qp[16 * t + 8] | ((uint32_t)qp[16 * t + 9] << 16) : 0u;
+    }
     }
     if (APPEND) {
       if (lane < D / 8) {
@@ -369,13 +439,13 @@ attn_decode_kernel(const __grid_constant__ DecParams p) {
   };
   // ---- the unit at `at`, in stage st
   auto unit = [&](int st) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(DEC_STAGES - 1) : "memory");
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
     __syncwarp();
     const int left = at.len - (at.blk * 64 + warp * DEC_KEYS);    // valid keys of the block
     if (APPEND && left > 0 && left <= DEC_KEYS) {                 // the new token is the last valid key: into the ring and the caches
       if (lane < D / 8) {
         const int row = left - 1;
-        uint8_t* to = ring + (my - smem_u32(ring)) + st * (2 * Cfg::TILE) + row * Cfg::ROW + Cfg::chunk(row, lane);
+        uint8_t* to = ring + (my - smem_u32(ring)) + st * Cfg::STAGE + row * Cfg::ROW + Cfg::chunk(row, lane);
         *reinterpret_cast<uint4*>(to) = k_new;
         *reinterpret_cast<uint4*>(to + Cfg::TILE) = v_new;
         const long long off = at.b * batch_stride + (long long)(at.len - 1) * row_stride + (long long)hk * D + lane * 8;
@@ -384,8 +454,66 @@ attn_decode_kernel(const __grid_constant__ DecParams p) {
       }
       __syncwarp();
     }
-    if (left > 0) {
-      const uint32_t tk = my + st * (2 * Cfg::TILE), tv = tk + Cfg::TILE;
+    if constexpr (BYTES) {
+      // Numbers of the cache become f16 as they are; their rows' powers of two go to the scores (K) and to the probabilities (V): with e the exponents of V,
+      // P' = 2^(score + e - mv + 14) of the largest score + e so far, so that the products with V have all of f16's bits whatever the rows' scales are. l, of P
+      // itself, goes by the largest score. 2^14: what is below 2^-39 of the largest is lost, not 2^-25. One f16 number stands for a P': half a step is 2^-12.
+      if (left > 0) {
+        const uint32_t tk = my + st * Cfg::STAGE, tv = tk + Cfg::TILE;
+        const uint8_t* scales = ring + (tv + Cfg::TILE - smem_u32(ring));
+        const unsigned k0 = scales[r], k1 = scales[r + 8], v0 = scales[DEC_KEYS + r], v1 = scales[DEC_KEYS + r + 8];
+        float sc[4] = {0.f, 0.f, 0.f, 0.f}, sd[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int t = 0; t < D / 16; t += 2) {
+          uint32_t a[4];
+          ldmatrix_x4(a, tk + (lane & 15) * Cfg::ROW + Cfg::chunk(lane & 15, t + (lane >> 4)));
+          mma_f16_16816(sc, f16x2_of_e4m3<0>(a[0]), f16x2_of_e4m3<0>(a[1]), f16x2_of_e4m3<1>(a[0]), f16x2_of_e4m3<1>(a[1]), qb[t][0], qb[t][1]);
+          mma_f16_16816(sd, f16x2_of_e4m3<0>(a[2]), f16x2_of_e4m3<0>(a[3]), f16x2_of_e4m3<1>(a[2]), f16x2_of_e4m3<1>(a[3]), qb[t + 1][0], qb[t + 1][1]);
+        }
+        const float f0 = __uint_as_float(k0 << 23), f1 = __uint_as_float(k1 << 23), e0 = (float)v0 - 127.f, e1 = (float)v1 - 127.f;
+        float corr[2], pr[4];
+        bool same = true;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float x0 = r < left ? (sc[e] + sd[e]) * f0 * qf[e] : -INFINITY;
+          const float x1 = r + 8 < left ? (sc[2 + e] + sd[2 + e]) * f1 * qf[e] : -INFINITY;
+          const float z0 = x0 + e0, z1 = x1 + e1;
+          float mx = fmaxf(x0, x1), mz = fmaxf(z0, z1);
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) {
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            mz = fmaxf(mz, __shfl_xor_sync(0xffffffffu, mz, o));
+          }
+          const float mn = fmaxf(m[e], mx), mzn = fmaxf(mv[e], mz);
+          const float ref = mn == -INFINITY ? 0.f : mn, refz = mzn == -INFINITY ? 0.f : mzn;
+          l[e] = l[e] * ex2_approx(m[e] - ref) + ex2_approx(x0 - ref) + ex2_approx(x1 - ref);
+          corr[e] = ex2_approx(mv[e] - refz);
+          same &= mv[e] == mzn;
+          m[e] = mn;
+          mv[e] = mzn;
+          pr[e] = ex2_approx(z0 - refz + 14.f);
+          pr[2 + e] = ex2_approx(z1 - refz + 14.f);
+        }
+        uint32_t pt[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) pt[h] = transpose_8x8(pack_f16x2(pr[2 * h], pr[2 * h + 1]));
+        if (!__all_sync(0xffffffffu, same)) {
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j) { o[j][0] *= corr[0]; o[j][1] *= corr[1]; o[j][2] *= corr[0]; o[j][3] *= corr[1]; }
+        }
+        // O^T += V^T P'^T: row r of a product is dim 2 r of the 16, row r + 8 dim 2 r + 1
+#pragma unroll
+        for (int j = 0; j < D / 16; j += 2) {
+          uint32_t a[4];
+          ldmatrix_x4_trans(a, tv + (lane & 15) * Cfg::ROW + Cfg::chunk(lane & 15, j + (lane >> 4)));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) a[i] = __byte_perm(a[i], 0, 0x3120);
+          mma_f16_16816(o[j], f16x2_of_e4m3<0>(a[0]), f16x2_of_e4m3<1>(a[0]), f16x2_of_e4m3<0>(a[1]), f16x2_of_e4m3<1>(a[1]), pt[0], pt[1]);
+          mma_f16_16816(o[j + 1], f16x2_of_e4m3<0>(a[2]), f16x2_of_e4m3<1>(a[2]), f16x2_of_e4m3<0>(a[3]), f16x2_of_e4m3<1>(a[3]), pt[0], pt[1]);
+        }
+      }
+    } else if (left > 0) {
+      const uint32_t tk = my + st * Cfg::STAGE, tv = tk + Cfg::TILE;
       // S^T: keys r, r + 8 by heads 2c, 2c + 1
       float sc[4] = {0.f, 0.f, 0.f, 0.f}, sd[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -445,6 +573,19 @@ attn_decode_kernel(const __grid_constant__ DecParams p) {
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], 8);
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], 16);
     }
+    if constexpr (BYTES) {       // from units of the largest score + e to those of the largest score
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float f = m[e] == -INFINITY ? 0.f : ex2_approx(mv[e] - m[e] - 14.f);
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) {
+          o[j][e] *= f;
+          o[j][2 + e] *= f;
+        }
+      }
+    }
+    // dims of o[j][0 .. 1] and o[j][2 .. 3]
+    auto dim = [&](int j, int half) { return BYTES ? 16 * j + 2 * r + half : 16 * j + 8 * half + r; };
     constexpr int BUF = DEC_MAX_G * Cfg::PITCH;
     float* buf = reinterpret_cast<float*>(ring + (last ? 0 : Cfg::RING));
     auto give = [&](float* to) {
@@ -453,8 +594,8 @@ attn_decode_kernel(const __grid_constant__ DecParams p) {
         float* g = to + (2 * c + e) * Cfg::PITCH;
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) {
-          g[16 * j + r] = o[j][e];
-          g[16 * j + 8 + r] = o[j][2 + e];
+          g[dim(j, 0)] = o[j][e];
+          g[dim(j, 1)] = o[j][2 + e];
         }
         if (r == 0) {
           g[D] = m[e];
@@ -477,8 +618,8 @@ attn_decode_kernel(const __grid_constant__ DecParams p) {
           l[e] = l[e] * ca + g[D + 1] * cb;
 #pragma unroll
           for (int j = 0; j < D / 16; ++j) {
-            o[j][e] = o[j][e] * ca + g[16 * j + r] * cb;
-            o[j][2 + e] = o[j][2 + e] * ca + g[16 * j + 8 + r] * cb;
+            o[j][e] = o[j][e] * ca + g[dim(j, 0)] * cb;
+            o[j][2 + e] = o[j][2 + e] * ca + g[dim(j, 1)] * cb;
           }
         }
         __syncwarp();              // read by all lanes before the buffer is written again
@@ -527,28 +668,28 @@ attn_decode_kernel(const __grid_constant__ DecParams p) {
     }
   };
 
-  int st = 0, st_load = DEC_STAGES - 1;
+  int st = 0, st_load = STAGES - 1;
   if constexpr (!SHARES) {
     const bool whole = left_units == at.n;
     begin();
     for (; left_units > 0; --left_units, ++at.blk) {
       load(st_load);
-      if (++st_load == DEC_STAGES) st_load = 0;
+      if (++st_load == STAGES) st_load = 0;
       unit(st);
-      if (++st == DEC_STAGES) st = 0;
+      if (++st == STAGES) st = 0;
     }
     finish(true, whole, blockIdx.x);
   } else {
     bool begins = false;           // the piece in work starts with its head's first unit
     for (bool first = true; left_units > 0; first = false) {
       load(st_load);
-      if (++st_load == DEC_STAGES) st_load = 0;
+      if (++st_load == STAGES) st_load = 0;
       if (first || at.blk == 0) {
         begins = at.blk == 0;
         begin();
       }
       unit(st);
-      if (++st == DEC_STAGES) st = 0;
+      if (++st == STAGES) st = 0;
       const bool ends = at.blk == at.n - 1;
       if (ends || left_units == 1) {
         finish(left_units == 1, begins && ends, 2 * (long long)blockIdx.x + begins);
@@ -659,7 +800,7 @@ __global__ void __launch_bounds__(D) attn_decode_merge_kernel(const __grid_const
 template <int D, int KIND>
 static int launch_decode(const DecParams& p, int chained, cudaStream_t st) {
   static gf::DeviceOnce configured;
-  constexpr int SMEM = DecCfg<D, dec_shares(KIND)>::SMEM;
+  constexpr int SMEM = DecCfg<D, dec_shares(KIND), dec_bytes(KIND)>::SMEM;
   auto kern = attn_decode_kernel<D, KIND>;
   if (configured.todo()) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess)
@@ -741,7 +882,8 @@ bool attn_paged_one_ok(const PagedCall& c, int splits, const float* scratch) {
          splits != 0 && (scratch || splits == 1) && c.pages > 0;
 }
 
-int attn_paged_one(const PagedCall& c, float scale, int splits, float* scratch, int chained, cudaStream_t st) {
+int attn_paged_one(const PagedCall& c, float scale, int splits, float* scratch, int chained, cudaStream_t st, const unsigned char* kscales,
+                   const unsigned char* vscales) {
   DecParams p{};
   paged_batch(p.pages, c);
   if (splits > 65535) splits = 65535;
@@ -756,6 +898,11 @@ int attn_paged_one(const PagedCall& c, float scale, int splits, float* scratch, 
   p.out = (__nv_bfloat16*)c.y; p.ldo = c.ldy;
   p.kpage = c.strides[0]; p.krow = c.strides[1]; p.khead = c.strides[2];
   p.vpage = c.strides[3]; p.vrow = c.strides[4]; p.vhead = c.strides[5];
+  p.kscales = kscales; p.vscales = vscales;
+  if (kscales) {
+    if (splits < 0) return D == 128 ? launch_decode<128, DEC_PAGES8_SHARES>(p, chained, st) : launch_decode<64, DEC_PAGES8_SHARES>(p, chained, st);
+    return D == 128 ? launch_decode<128, DEC_PAGES8>(p, chained, st) : launch_decode<64, DEC_PAGES8>(p, chained, st);
+  }
   if (splits < 0) return D == 128 ? launch_decode<128, DEC_PAGES_SHARES>(p, chained, st) : launch_decode<64, DEC_PAGES_SHARES>(p, chained, st);
   return D == 128 ? launch_decode<128, DEC_PAGES>(p, chained, st) : launch_decode<64, DEC_PAGES>(p, chained, st);
 }
@@ -768,4 +915,11 @@ GF_API int gf_paged_attn_one(const PagedCall* c, float scale, int splits, float*
   if (!c || c->cu || !attn_paged_one_ok(*c, splits, scratch)) return GFH_BAD_ARG;
   gf::enter();
   return attn_paged_one(*c, scale, splits, scratch, 0, (cudaStream_t)stream);
+}
+
+// The same over pages of 8 bits.
+GF_API int gf_paged_attn8_one(const PagedCall8* c8, float scale, int splits, float* scratch, void* stream) {
+  if (!c8 || c8->c.cu || !paged_scales(*c8) || !attn_paged_one_ok(c8->c, splits, scratch)) return GFH_BAD_ARG;
+  gf::enter();
+  return attn_paged_one(c8->c, scale, splits, scratch, 0, (cudaStream_t)stream, c8->kscales, c8->vscales);
 }

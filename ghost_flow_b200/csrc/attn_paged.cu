@@ -35,6 +35,9 @@ constexpr int PG_TILE = 128;      // rows of a tile, keys of a step
 constexpr int PG_THREADS = 384;   // warpgroup 0: TMA warp, MMA warp, warp that clears rows, an idle one; warpgroups 1 and 2: softmax of tile 0 / 1
 constexpr int PG_REGS_CTRL = 104; // 128 x 104 + 256 x 200 = 64512, the block's own at launch (384 x 168)
 constexpr int PG_REGS_SOFTMAX = 200;
+// With pages of 8 bits there is a fourth warpgroup, of warps that turn them into bf16: 128 x 56 + 256 x 200 + 128 x 56 = 65536, 512 x 128 at launch.
+constexpr int PG_THREADS8 = 512;
+constexpr int PG_REGS_CTRL8 = 56, PG_REGS_TURN = 56;
 constexpr int PG_PARTS = 2;       // P V of a tile is issued in this many parts of the keys
 constexpr float PG_RESCALE = 8.0f;  // log2 units
 
@@ -50,6 +53,7 @@ struct PagedAttn {
   int4* where;                   // for each of them, what the kernel that joins pieces wants to know (see there)
   float* part;                   // [item][rows][D], then [item][rows][maximum, sum]
   float* part_ml;
+  const unsigned char *kscales, *vscales;          // of pages of 8 bits
   int rows, items, blocks;       // rows of an item in `part`, items and blocks (of all KV heads) at most
 };
 
@@ -188,14 +192,17 @@ __device__ __forceinline__ bool pg_find(const PagedAttn& p, const PgShape& own, 
   return false;
 }
 
-template <int HD>
+template <int HD, bool BYTES>
 struct PgCfg {
+  static constexpr int THREADS = BYTES ? PG_THREADS8 : PG_THREADS;
   static constexpr int CH = HD / 64;
   static constexpr int TILE_BYTES = PG_TILE * HD * 2;
   static constexpr int OFF_Q = 0;                                   // 2 tiles
   static constexpr int OFF_K = OFF_Q + 2 * TILE_BYTES;              // 2 stages; at the end the sums of tile 1's keys
   static constexpr int OFF_V = OFF_K + 2 * TILE_BYTES;              // 2 stages
-  static constexpr int OFF_BAR = OFF_V + 2 * TILE_BYTES;
+  static constexpr int OFF_RAW = OFF_V + 2 * TILE_BYTES;            // BYTES: K and V of a step as they are in the pages
+  static constexpr int RAW_BYTES = PG_TILE * HD;
+  static constexpr int OFF_BAR = OFF_RAW + (BYTES ? 2 * RAW_BYTES : 0);
   static constexpr int OFF_ML = OFF_BAR + 256;                      // maxima and sums of tile 1's keys
   static constexpr int SMEM_BYTES = OFF_ML + 2 * PG_TILE * 4 + 1024;
   static constexpr int TM_S = 0;      // + t * 128; P (bf16 pairs) occupies the first 64 columns of the same region
@@ -217,11 +224,27 @@ __device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* m
       : "memory");
 }
 
-template <int HD>
-__global__ void __launch_bounds__(PG_THREADS, 1)
+// 16 numbers of the cache times their row's power of two, as bf16: exact
+__device__ __forceinline__ void bf16x16_of_e4m3(const uint4& in, float scale, uint4& lo, uint4& hi) {
+  const uint32_t* four = reinterpret_cast<const uint32_t*>(&in);
+  uint32_t out[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((unsigned short)(i & 1 ? four[i >> 1] >> 16 : four[i >> 1])));
+    float a, b;
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, h;\n\t}" : "=f"(a), "=f"(b) : "r"(h));
+    out[i] = pack_bf16x2(a * scale, b * scale);
+  }
+  lo = make_uint4(out[0], out[1], out[2], out[3]);
+  hi = make_uint4(out[4], out[5], out[6], out[7]);
+}
+
+template <int HD, bool BYTES>
+__global__ void __launch_bounds__(PgCfg<HD, BYTES>::THREADS, 1)
 paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                   const __grid_constant__ CUtensorMap tmV, const __grid_constant__ PagedAttn p) {
-  using Cfg = PgCfg<HD>;
+  using Cfg = PgCfg<HD, BYTES>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem + Cfg::OFF_Q;
@@ -237,7 +260,9 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   uint64_t* o_done = bars + 11;   // [2] per tile
   uint64_t* v_tail = bars + 13;   // the last V tile before its rows behind the sequence are cleared
   uint64_t* p_full = bars + 14;   // [2][PG_PARTS]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 14 + 2 * PG_PARTS);
+  uint64_t* raw_full = bars + 14 + 2 * PG_PARTS;   // [2] K, V
+  uint64_t* raw_empty = raw_full + 2;              // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(raw_empty + 2);
   __shared__ PgItem shared_item;
   __shared__ int shared_there, shared_failed;
 
@@ -256,7 +281,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     // the last step's V has rows behind the sequence inside a page
     box = min(PG_TILE, 1 << p.seqs.page_shift);
     tail = o.keys - (o.j1 - 1) * PG_TILE;                            // rows of the last step that are keys
-    clears = n_j > 0 && tail < PG_TILE && (tail & (box - 1)) != 0;
+    clears = !BYTES && n_j > 0 && tail < PG_TILE && (tail & (box - 1)) != 0;
   };
   // A CTA of few steps is mostly this: the queries are on their way before the other warps have started. (Keys and values too was slower: the
   // producer's code then stands twice, and the softmax warps spill.)
@@ -266,10 +291,14 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     if (lane == 0) {
       mbar_init(q_full, 1);
       for (int i = 0; i < 2; ++i) {
-        mbar_init(&k_full[i], 1);
+        mbar_init(&k_full[i], BYTES ? 4 : 1);
         mbar_init(&k_empty[i], 1);
-        mbar_init(&v_full[i], 1);
+        mbar_init(&v_full[i], BYTES ? 4 : 1);
         mbar_init(&v_empty[i], 1);
+        if (BYTES) {
+          mbar_init(&raw_full[i], 1);
+          mbar_init(&raw_empty[i], 4);
+        }
         mbar_init(&s_full[i], 1);
         for (int c = 0; c < PG_PARTS; ++c) mbar_init(&p_full[i * PG_PARTS + c], 4);
         mbar_init(&o_done[i], 1);
@@ -327,7 +356,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   cnt[1] = alternate ? n_j >> 1 : n_j;
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PG_REGS_CTRL));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(BYTES ? PG_REGS_CTRL8 : PG_REGS_CTRL));
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA producer: a lane has one box of a step
     auto page_of = [&](int j) {
@@ -349,11 +378,31 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       }
       __syncwarp();
     };
+    auto bytes_to = [&](uint8_t* dst, const CUtensorMap* m, uint64_t* bar, int j, int page) {
+      if (lane == 0) mbar_expect_tx(bar, Cfg::RAW_BYTES);
+      __syncwarp();
+      if (lane * box < PG_TILE)
+        tma_load_4d(dst + lane * box * HD, m, bar, 0, (j * PG_TILE + lane * box) & ((1 << p.seqs.page_shift) - 1), it.hk, page);
+      __syncwarp();
+    };
     int next = page_of(it.j0);
     for (int i = 0; i < n_j; ++i) {
       const int j = it.j0 + i, st = i & 1, page = next;
       const uint32_t ph = (i >> 1) & 1;
       next = page_of(j + 1);
+      if constexpr (BYTES) {
+        if (!mbar_wait_warp(&raw_empty[0], (i & 1) ^ 1)) {
+          if (lane == 0) fail(GF_ERR_WAIT_EMPTY);
+          break;
+        }
+        bytes_to(smem + Cfg::OFF_RAW, &tmK, &raw_full[0], j, page);
+        if (!mbar_wait_warp(&raw_empty[1], (i & 1) ^ 1)) {
+          if (lane == 0) fail(GF_ERR_WAIT_EMPTY);
+          break;
+        }
+        bytes_to(smem + Cfg::OFF_RAW + Cfg::RAW_BYTES, &tmV, &raw_full[1], j, page);
+        continue;
+      }
       if (!mbar_wait_warp(&k_empty[st], ph ^ 1)) {
         if (lane == 0) fail(GF_ERR_WAIT_EMPTY);
         break;
@@ -476,6 +525,61 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       if (lane == 0) mbar_arrive(&v_full[st]);
     }
   }
+  } else if (BYTES && warp >= 12) {
+    // ---------------------------------------------------------------- pages of 8 bits to bf16: a thread has a key
+    // Lanes of neighbouring rows begin at neighbouring chunks of 16 bytes, so that eight of them meet every bank once, here and in the swizzled tile.
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PG_REGS_TURN));
+    const int r = threadIdx.x & 127;
+    int ks = -1, vs = 0;                           // bytes of the row's powers of two; -1: there is no such key, zeros
+    auto look = [&](int i) {
+      ks = -1;
+      const int key = (item.j0 + i) * PG_TILE + r;
+      if (i >= n_j || key >= item.keys) return;
+      const int page = p.seqs.table[(long long)item.b * p.seqs.ld + (key >> p.seqs.page_shift)];
+      if (page < 0 || page >= p.seqs.pages) return;            // (reported by the producer)
+      const long long at = (((long long)page * p.Hkv + item.hk) << p.seqs.page_shift) + (key & ((1 << p.seqs.page_shift) - 1));
+      ks = p.kscales[at];
+      vs = p.vscales[at];
+    };
+    auto turn = [&](const uint8_t* raw, uint8_t* tile, int byte) {
+      constexpr int CHUNKS = HD / 16;
+      const float scale = __uint_as_float((unsigned)max(byte, 0) << 23);
+#pragma unroll 2
+      for (int k = 0; k < CHUNKS; ++k) {
+        const int q = (k + (HD == 64 ? r >> 1 : r)) & (CHUNKS - 1), u = 2 * q;
+        uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+        if (byte >= 0) bf16x16_of_e4m3(*reinterpret_cast<const uint4*>(raw + r * HD + q * 16), scale, lo, hi);
+        uint8_t* to = tile + (u >> 3) * (PG_TILE * 128) + r * 128;
+        *reinterpret_cast<uint4*>(to + (((u & 7) ^ (r & 7)) << 4)) = lo;
+        *reinterpret_cast<uint4*>(to + ((((u + 1) & 7) ^ (r & 7)) << 4)) = hi;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+    };
+    look(0);
+    for (int i = 0; i < n_j; ++i) {
+      const int st = i & 1, kb = ks, vb = ks < 0 ? -1 : vs;
+      const uint32_t ph = (i >> 1) & 1;
+      look(i + 1);
+      bool ok = mbar_wait_warp_tight(&raw_full[0], i & 1) && mbar_wait_warp_tight(&k_empty[st], ph ^ 1);
+      if (ok) {
+        turn(smem + Cfg::OFF_RAW, sK + st * Cfg::TILE_BYTES, kb);
+        if (lane == 0) {
+          mbar_arrive(&k_full[st]);
+          mbar_arrive(&raw_empty[0]);
+        }
+        ok = mbar_wait_warp_tight(&raw_full[1], i & 1) && mbar_wait_warp_tight(&v_empty[st], ph ^ 1);
+      }
+      if (!ok) {
+        if (lane == 0) fail(GF_ERR_WAIT_FULL);
+        break;
+      }
+      turn(smem + Cfg::OFF_RAW + Cfg::RAW_BYTES, sV + st * Cfg::TILE_BYTES, vb);
+      if (lane == 0) {
+        mbar_arrive(&v_full[st]);
+        mbar_arrive(&raw_empty[1]);
+      }
+    }
   } else {
     // ---------------------------------------------------------------- softmax warps: tile t = warp / 4 - 1
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PG_REGS_SOFTMAX));
@@ -746,24 +850,24 @@ __global__ void __launch_bounds__(256, 4) paged_join_kernel(const __grid_constan
   *reinterpret_cast<uint4*>(p.out + (long long)(a.w + t * p.tq + r / p.G) * p.ldo + (b.y * p.G + r % p.G) * HD + col) = u;
 }
 
-static int pg_map(CUtensorMap* out, const void* base, int rank, const cuuint64_t* dims, const long long* strides, const cuuint32_t* box) {
+static int pg_map(CUtensorMap* out, const void* base, int rank, const cuuint64_t* dims, const long long* strides, const cuuint32_t* box, bool bytes = false) {
   EncodeTiledFn fn = get_encode_fn();
   if (!fn) return GFH_TMAP;
-  cuuint64_t bytes[3];
-  for (int i = 0; i < rank - 1; ++i) bytes[i] = dims[i + 1] > 1 ? (cuuint64_t)strides[i] * 2 : dims[0] * 2;   // a stride that nothing goes by
+  cuuint64_t pitch[3];
+  for (int i = 0; i < rank - 1; ++i) pitch[i] = dims[i + 1] > 1 ? (cuuint64_t)strides[i] * (bytes ? 1 : 2) : dims[0] * (bytes ? 1 : 2);   // a stride that nothing goes by
   const cuuint32_t ones[4] = {1, 1, 1, 1};
-  const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, bytes, box, ones,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+  const CUresult r = fn(out, bytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, pitch, box, ones,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, bytes ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? GFH_OK : GFH_TMAP;
 }
 
-template <int HD>
+template <int HD, bool BYTES>
 static int launch_paged(PagedAttn& p, const void* q, long long ldq, const void* kp, const void* vp, const long long* strides, int items,
                         cudaStream_t st) {
-  using Cfg = PgCfg<HD>;
+  using Cfg = PgCfg<HD, BYTES>;
   static gf::DeviceOnce configured;
-  auto kern = paged_attn_kernel<HD>;
+  auto kern = paged_attn_kernel<HD, BYTES>;
   if (configured.todo()) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES) != cudaSuccess) return GFH_CUDA;
     configured.mark();
@@ -775,13 +879,13 @@ static int launch_paged(PagedAttn& p, const void* q, long long ldq, const void* 
   const cuuint32_t qbox[3] = {64, (cuuint32_t)p.G, (cuuint32_t)p.tq};
   const int page = 1 << S.page_shift;
   const cuuint64_t dims[4] = {HD, (cuuint64_t)page, (cuuint64_t)p.Hkv, (cuuint64_t)S.pages};
-  const cuuint32_t box[4] = {64, (cuuint32_t)(page < PG_TILE ? page : PG_TILE), 1, 1};
+  const cuuint32_t box[4] = {BYTES ? HD : 64, (cuuint32_t)(page < PG_TILE ? page : PG_TILE), 1, 1};
   const long long ks[3] = {strides[1], strides[2], strides[0]}, vs[3] = {strides[4], strides[5], strides[3]};
   int rc = pg_map(&tq, q, 3, qdims, qstrides, qbox);
-  if (!rc) rc = pg_map(&tk, kp, 4, dims, ks, box);
-  if (!rc) rc = pg_map(&tv, vp, 4, dims, vs, box);
+  if (!rc) rc = pg_map(&tk, kp, 4, dims, ks, box, BYTES);
+  if (!rc) rc = pg_map(&tv, vp, 4, dims, vs, box, BYTES);
   if (rc) return rc;
-  kern<<<items, PG_THREADS, Cfg::SMEM_BYTES, st>>>(tq, tk, tv, p);
+  kern<<<items, Cfg::THREADS, Cfg::SMEM_BYTES, st>>>(tq, tk, tv, p);
   return cudaGetLastError() == cudaSuccess ? GFH_OK : GFH_CUDA;
 }
 
@@ -848,10 +952,8 @@ GF_API long long gf_paged_attn_workspace(int B, int T, int one_each, int ones, l
   return c.ws;
 }
 
-// x [T, Hq, D] and y alike; ws: as many bytes as gf_paged_attn_workspace says, on a 16-byte boundary. scale > 0. ones != 0: sequences of one new
-// token go to the decode kernel, with that many splits and its scratch (see gf_paged_attn_one), while this one's CTAs run out. Each kernel is
-// launched while the one in front of it runs, and none ends before that one has.
-GF_API int gf_paged_attn(const PagedCall* c, float scale, void* ws, long long ws_bytes, int ones, float* ones_scratch, void* stream) {
+static int attn_paged(const PagedCall* c, const unsigned char* kscales, const unsigned char* vscales, float scale, void* ws, long long ws_bytes, int ones,
+                      float* ones_scratch, void* stream) {
   PagedAttn p{};
   if (!c || !paged_batch(p.seqs, *c) || c->pages == 0 || c->H > 0x7fffffff || c->Hk > 65535) return GFH_BAD_ARG;
   const int B = p.seqs.B, T = p.seqs.T, Hq = (int)c->H, Hkv = (int)c->Hk, D = (int)c->D;
@@ -872,13 +974,28 @@ GF_API int gf_paged_attn(const PagedCall* c, float scale, void* ws, long long ws
     p.part = (float*)((char*)ws + 256 + 32ll * n.blocks);
     p.part_ml = p.part + (long long)n.items * n.rows * D;
   }
+  p.kscales = kscales;
+  p.vscales = vscales;
   cudaStream_t st = (cudaStream_t)stream;
-  int rc = D == 128 ? launch_paged<128>(p, c->x, c->ldx, c->kpages, c->vpages, c->strides, n.items, st)
-                    : launch_paged<64>(p, c->x, c->ldx, c->kpages, c->vpages, c->strides, n.items, st);
+  auto launch = kscales ? (D == 128 ? launch_paged<128, true> : launch_paged<64, true>) : D == 128 ? launch_paged<128, false> : launch_paged<64, false>;
+  int rc = launch(p, c->x, c->ldx, c->kpages, c->vpages, c->strides, n.items, st);
   if (!rc && ones) {
     note_extra_launches(1);
-    rc = attn_paged_one(*c, scale, ones, ones_scratch, 1, st);
+    rc = attn_paged_one(*c, scale, ones, ones_scratch, 1, st, kscales, vscales);
   }
   if (!rc && n.slots) rc = D == 128 ? launch_join<128>(p, st) : launch_join<64>(p, st);
   return rc;
+}
+
+// x [T, Hq, D] and y alike; ws: as many bytes as gf_paged_attn_workspace says, on a 16-byte boundary. scale > 0. ones != 0: sequences of one new
+// token go to the decode kernel, with that many splits and its scratch (see gf_paged_attn_one), while this one's CTAs run out. Each kernel is
+// launched while the one in front of it runs, and none ends before that one has.
+GF_API int gf_paged_attn(const PagedCall* c, float scale, void* ws, long long ws_bytes, int ones, float* ones_scratch, void* stream) {
+  return attn_paged(c, nullptr, nullptr, scale, ws, ws_bytes, ones, ones_scratch, stream);
+}
+
+// The same over pages of 8 bits.
+GF_API int gf_paged_attn8(const PagedCall8* c8, float scale, void* ws, long long ws_bytes, int ones, float* ones_scratch, void* stream) {
+  if (!c8 || !paged_scales(*c8)) return GFH_BAD_ARG;
+  return attn_paged(&c8->c, c8->kscales, c8->vscales, scale, ws, ws_bytes, ones, ones_scratch, stream);
 }

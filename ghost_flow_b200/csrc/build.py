@@ -40,6 +40,7 @@ CUDA_SOURCES = [
     "gemm_skinny.cu",
     "gemm_rows.cu",
     "norm.cu",
+    "norm_rope.cu",
     "pointwise.cu",
     "xent_adamw.cu",
     "attn_fwd.cu",

@@ -32,7 +32,7 @@ struct DLPackExchangeAPI {
   int (*tensor_from_object)(void* object, DLTensor* out);
   int (*current_stream)(int32_t device_type, int32_t device, void** out);
 };
-enum { INT = 0, FLOAT = 2, BFLOAT = 4, CUDA = 2 };
+enum { INT = 0, FLOAT = 2, BFLOAT = 4, E4M3 = 10, E8M0 = 14, CUDA = 2 };
 constexpr long long MOST = 0x7fffffff;
 
 const DLPackExchangeAPI* api;
@@ -41,6 +41,10 @@ int (*f_attn)(const gf::PagedCall*, float, void*, long long, int, float*, void*)
 int (*f_attn_one)(const gf::PagedCall*, float, int, float*, void*);
 int (*f_logits)(const gf::LogitsCall*, void*);
 int (*f_sample)(const gf::SampleCall*, void*);
+int (*f_append_heads)(const gf::PagedCall8*, const float*, const float*, int, int, int, const void*, const void*, float, void*);
+int (*f_attn8)(const gf::PagedCall8*, float, void*, long long, int, float*, void*);
+int (*f_attn8_one)(const gf::PagedCall8*, float, int, float*, void*);
+int (*f_read)(const gf::PagedCall8*, void*, void*, void*);
 // what the operators' `_observed` asks (ops/fused.py), here without its Python frames (0.15 us instead of 0.6), and whether gradients are recorded
 PyObject *tracing, *transforms, *dispatch_modes, *function_modes, *only_device_contexts, *forward_ad, *grad_enabled, *requires_grad, *current_level;
 
@@ -100,18 +104,15 @@ struct View : DLTensor {
   uintptr_t at() const { return reinterpret_cast<uintptr_t>(data); }
 };
 
-// x [T, heads, D], kpages, vpages, page_table, lens, cu or None: the call but for H and what is only known at its launch. `packed`: rows of x are dense and
-// lie on 16-byte boundaries.
-bool paged(PyObject* const* a, PyObject* pages_k, PyObject* pages_v, PyObject* table, PyObject* lens_, PyObject* cu_, gf::PagedCall& c, int& device,
-           long long& heads, bool& packed) {
-  View x, k, v, t, n, cu;
-  if (!x.of(a[0])) return false;
-  device = x.device;
-  if (!x.is(BFLOAT, 16, 3, device) || !k.of(pages_k) || !k.is(BFLOAT, 16, 4, device) || !v.of(pages_v) || !v.is(BFLOAT, 16, 4, device) ||
-      !t.of(table) || !t.is(INT, 32, 2, device) || std::memcmp(k.shape, v.shape, 4 * sizeof(int64_t)))
+// kpages, vpages, page_table, lens, cu or None of T tokens on a device: what a call says of them. `bytes`: pages of 8 bits.
+bool pools(PyObject* pages_k, PyObject* pages_v, PyObject* table, PyObject* lens_, PyObject* cu_, long long T, int device, bool bytes, gf::PagedCall& c) {
+  View k, v, t, n, cu;
+  const int code = bytes ? E4M3 : BFLOAT, bits = bytes ? 8 : 16, vec = 128 / bits;
+  if (!k.of(pages_k) || !k.is(code, bits, 4, device) || !v.of(pages_v) || !v.is(code, bits, 4, device) || !t.of(table) || !t.is(INT, 32, 2, device) ||
+      std::memcmp(k.shape, v.shape, 4 * sizeof(int64_t)))
     return false;
-  const long long P = k.shape[0], page = k.shape[1], Hk = k.shape[2], D = k.shape[3], B = t.shape[0], width = t.shape[1], T = x.shape[0];
-  if (!n.ints(lens_, B, device) || B == 0 || T == 0 || x.shape[2] != D || D % 8 || D == 0 || t.stride(1, 1) != 1) return false;
+  const long long P = k.shape[0], page = k.shape[1], Hk = k.shape[2], D = k.shape[3], B = t.shape[0], width = t.shape[1];
+  if (!n.ints(lens_, B, device) || B == 0 || T == 0 || D % vec || D == 0 || t.stride(1, 1) != 1) return false;
   if (cu_ == Py_None ? T != B : !cu.ints(cu_, B + 1, device)) return false;
   if (P == 0 || Hk == 0 || page < 16 || page & (page - 1) || page > MOST || P > MOST / page || width > MOST / page || k.stride(3, 1) != 1 ||
       v.stride(3, 1) != 1 || ((k.at() | v.at()) & 15))
@@ -121,13 +122,9 @@ bool paged(PyObject* const* a, PyObject* pages_k, PyObject* pages_v, PyObject* t
     st[2] = w->stride(2, D);
     st[1] = w->stride(1, Hk * D);
     st[0] = w->stride(0, page * st[1]);
-    if ((st[0] | st[1] | st[2]) & 7) return false;
+    if ((st[0] | st[1] | st[2]) & (vec - 1)) return false;
     st += 3;
   }
-  heads = x.shape[1];
-  c.x = x.data;
-  c.ldx = x.stride(0, heads * D);
-  packed = x.stride(2, 1) == 1 && x.stride(1, D) == D && c.ldx % 8 == 0 && c.ldx >= heads * D && (x.at() & 15) == 0;
   c.kpages = k.data;
   c.vpages = v.data;
   c.table = (const int*)t.data;
@@ -139,6 +136,35 @@ bool paged(PyObject* const* a, PyObject* pages_k, PyObject* pages_v, PyObject* t
   return true;
 }
 
+// The same with x [T, heads, D] in front: the call but for H and what is only known at its launch. `packed`: rows of x are dense and
+// lie on 16-byte boundaries.
+bool paged(PyObject* const* a, PyObject* pages_k, PyObject* pages_v, PyObject* table, PyObject* lens_, PyObject* cu_, gf::PagedCall& c, int& device,
+           long long& heads, bool& packed, bool bytes = false) {
+  View x;
+  if (!x.of(a[0])) return false;
+  device = x.device;
+  if (!x.is(BFLOAT, 16, 3, device) || !pools(pages_k, pages_v, table, lens_, cu_, x.shape[0], device, bytes, c) || x.shape[2] != c.D) return false;
+  heads = x.shape[1];
+  c.x = x.data;
+  c.ldx = x.stride(0, heads * c.D);
+  packed = x.stride(2, 1) == 1 && x.stride(1, c.D) == c.D && c.ldx % 8 == 0 && c.ldx >= heads * c.D && (x.at() & 15) == 0;
+  return true;
+}
+
+// Scales [pages, Hk, page] of pages of 8 bits, dense and apart from each other; none (None) where pages are bf16.
+bool scales(PyObject* of_k, PyObject* of_v, const gf::PagedCall& c, int device, const unsigned char*& ks, const unsigned char*& vs) {
+  const unsigned char** to[2] = {&ks, &vs};
+  for (int i = 0; i < 2; ++i) {
+    View t;
+    if (!t.of(i ? of_v : of_k) || !t.is(E8M0, 8, 3, device) || t.shape[0] != c.pages || t.shape[1] != c.Hk || t.shape[2] != c.page || t.stride(2, 1) != 1 ||
+        t.stride(1, c.page) != c.page || t.stride(0, c.Hk * c.page) != c.Hk * c.page || (t.at() & 15))
+      return false;
+    *to[i] = (const unsigned char*)t.data;
+  }
+  const uintptr_t a = reinterpret_cast<uintptr_t>(ks), b = reinterpret_cast<uintptr_t>(vs);
+  return (a > b ? a - b : b - a) >= (uintptr_t)(c.pages * c.Hk * c.page);
+}
+
 struct Append {
   gf::PagedCall c;
   const float *cos, *sin;
@@ -148,6 +174,16 @@ struct Append {
 bool arguments(const char* what, Py_ssize_t got, Py_ssize_t want) {
   if (got != want) PyErr_Format(PyExc_TypeError, "%s takes %zd arguments, not %zd", what, want, got);
   return got == want;
+}
+
+// The pools' addresses and strides where they are not simply dense and apart, else None.
+PyObject* where_pools(const gf::PagedCall& c, int size) {
+  const long long *k = c.strides, *v = k + 3, row = c.Hk * c.D, all = c.pages * c.page * row;
+  const uintptr_t k0 = reinterpret_cast<uintptr_t>(c.kpages), v0 = reinterpret_cast<uintptr_t>(c.vpages);
+  const bool apart = k[2] == c.D && v[2] == c.D && k[1] == row && v[1] == row && k[0] == c.page * row && v[0] == k[0] &&
+                     (k0 > v0 ? k0 - v0 : v0 - k0) >= (uintptr_t)(size * all);
+  return apart ? Py_NewRef(Py_None)
+               : Py_BuildValue("(KKLLLLLL)", (unsigned long long)k0, (unsigned long long)v0, k[0], k[1], k[2], v[0], v[1], v[2]);
 }
 
 // append(qkv, H, Hk, kpages, vpages, page_table, lens, cu, cos, sin): (call, device, T, D, whether qkv is packed, the pools where they are not simply
@@ -173,13 +209,70 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   r.cos = (const float*)cs.data;
   r.sin = (const float*)sn.data;
   r.positions = (int)cs.shape[0];
-  const long long *k = r.c.strides, *v = k + 3, row = Hk * r.c.D, all = r.c.pages * r.c.page * row;
-  const uintptr_t k0 = reinterpret_cast<uintptr_t>(r.c.kpages), v0 = reinterpret_cast<uintptr_t>(r.c.vpages);
-  const bool apart = k[2] == r.c.D && v[2] == r.c.D && k[1] == row && v[1] == row && k[0] == r.c.page * row && v[0] == k[0] &&
-                     (k0 > v0 ? k0 - v0 : v0 - k0) >= (uintptr_t)(2 * all);
-  PyObject* pools = apart ? Py_NewRef(Py_None)
-                          : Py_BuildValue("(KKLLLLLL)", (unsigned long long)k0, (unsigned long long)v0, k[0], k[1], k[2], v[0], v[1], v[2]);
-  return pools ? Py_BuildValue("(y#iLLON)", (const char*)&r, (Py_ssize_t)sizeof r, device, r.c.T, r.c.D, packed ? Py_True : Py_False, pools) : nullptr;
+  PyObject* where = where_pools(r.c, 2);
+  return where ? Py_BuildValue("(y#iLLON)", (const char*)&r, (Py_ssize_t)sizeof r, device, r.c.T, r.c.D, packed ? Py_True : Py_False, where) : nullptr;
+}
+
+struct AppendHeads {
+  gf::PagedCall8 c8;
+  const float *cos, *sin;
+  const void *qw, *kw;
+  int positions, rotary;
+};
+
+// append_heads(qkv, H, Hk, kpages, vpages, page_table, lens, cu, cos, sin, kscales, vscales, q_weight, k_weight): as append
+PyObject* append_heads(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!arguments("append_heads", n, 14)) return nullptr;
+  const long long H = PyLong_AsLongLong(a[1]), Hk = PyLong_AsLongLong(a[2]);
+  if (PyErr_Occurred()) return nullptr;
+  AppendHeads r{};
+  gf::PagedCall& c = r.c8.c;
+  int device;
+  long long heads;
+  bool packed;
+  View cs, sn, w;
+  const bool bytes = a[10] != Py_None;
+  if (followed({a[0], a[3], a[4], a[8], a[9], a[12], a[13]})) Py_RETURN_NONE;
+  if (!paged(a, a[3], a[4], a[5], a[6], a[7], c, device, heads, packed, bytes) || H <= 0 || H > 65535 || c.Hk != Hk || Hk > 65535 || heads != H + 2 * Hk ||
+      (c.D != 32 && c.D != 64 && c.D != 128 && c.D != 256) || !cs.of(a[8]) || !sn.of(a[9]) || (a[11] != Py_None) != bytes ||
+      (bytes && !scales(a[10], a[11], c, device, r.c8.kscales, r.c8.vscales)) || (a[12] == Py_None) != (a[13] == Py_None))
+    Py_RETURN_NONE;
+  for (const View* t : {&cs, &sn})
+    if (!t->is(FLOAT, 32, 2, device) || t->shape[1] % 8 || 2 * t->shape[1] > c.D || t->shape[1] != cs.shape[1] || t->shape[0] != cs.shape[0] ||
+        t->shape[0] > MOST || (t->shape[1] && (t->stride(1, 1) != 1 || t->stride(0, t->shape[1]) != t->shape[1] || (t->at() & 15) || !t->data)))
+      Py_RETURN_NONE;
+  for (int i = 12; i < 14; ++i) {
+    if (a[i] == Py_None) continue;
+    if (!w.of(a[i]) || !w.is(BFLOAT, 16, 1, device) || w.shape[0] != c.D || w.stride(0, 1) != 1 || (w.at() & 15)) Py_RETURN_NONE;
+    (i == 12 ? r.qw : r.kw) = w.data;
+  }
+  c.H = H;
+  r.cos = cs.shape[1] ? (const float*)cs.data : nullptr;
+  r.sin = cs.shape[1] ? (const float*)sn.data : nullptr;
+  r.positions = (int)cs.shape[0];
+  r.rotary = (int)(2 * cs.shape[1]);
+  PyObject* where = where_pools(c, bytes ? 1 : 2);
+  return where ? Py_BuildValue("(y#iLLON)", (const char*)&r, (Py_ssize_t)sizeof r, device, c.T, c.D, packed ? Py_True : Py_False, where) : nullptr;
+}
+
+// read(rows, kpages, vpages, page_table, lens, cu, kscales, vscales): (call, device, Hk, D), None as above
+PyObject* read(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!arguments("read", n, 8)) return nullptr;
+  const long long T = PyLong_AsLongLong(a[0]);
+  if (PyErr_Occurred()) return nullptr;
+  gf::PagedCall8 r{};
+  View k;
+  const bool bytes = a[6] != Py_None;
+  if (followed({a[1], a[2]}) || !k.of(a[1]) || T <= 0 || T > MOST || !pools(a[1], a[2], a[3], a[4], a[5], T, k.device, bytes, r.c) || r.c.D % 16 ||
+      r.c.D > 4096 || r.c.Hk > 65535 || (a[7] != Py_None) != bytes || (bytes && !scales(a[6], a[7], r.c, k.device, r.kscales, r.vscales)))
+    Py_RETURN_NONE;
+  return Py_BuildValue("(y#iLL)", (const char*)&r, (Py_ssize_t)sizeof r, k.device, r.c.Hk, r.c.D);
+}
+
+bool attends(const gf::PagedCall& c) {
+  for (long long st : c.strides)
+    if (st == 0) return false;
+  return (c.D == 64 || c.D == 128) && c.H > 0 && c.H <= MOST && c.H % c.Hk == 0 && c.H / c.Hk <= 128;
 }
 
 // attention(q, kpages, vpages, page_table, lens, cu): (call, device, B, T, H, Hk, D, keys of a sequence at most, whether q is packed), None as above
@@ -189,12 +282,21 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   int device;
   bool packed;
   if (followed({a[0], a[1], a[2]})) Py_RETURN_NONE;
-  if (!paged(a, a[1], a[2], a[3], a[4], a[5], c, device, c.H, packed) || (c.D != 64 && c.D != 128) || c.H == 0 || c.H > MOST || c.H % c.Hk ||
-      c.H / c.Hk > 128)
-    Py_RETURN_NONE;
-  for (long long st : c.strides)
-    if (st == 0) Py_RETURN_NONE;
+  if (!paged(a, a[1], a[2], a[3], a[4], a[5], c, device, c.H, packed) || !attends(c)) Py_RETURN_NONE;
   return Py_BuildValue("(y#iLLLLLLO)", (const char*)&c, (Py_ssize_t)sizeof c, device, c.B, c.T, c.H, c.Hk, c.D, c.width * c.page,
+                       packed ? Py_True : Py_False);
+}
+
+// attention8(q, kpages, vpages, page_table, lens, cu, kscales, vscales): the same over pages of 8 bits
+PyObject* attention8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!arguments("attention8", n, 8)) return nullptr;
+  gf::PagedCall8 r{};
+  gf::PagedCall& c = r.c;
+  int device;
+  bool packed;
+  if (followed({a[0], a[1], a[2]})) Py_RETURN_NONE;
+  if (!paged(a, a[1], a[2], a[3], a[4], a[5], c, device, c.H, packed, true) || !attends(c) || !scales(a[6], a[7], c, device, r.kscales, r.vscales)) Py_RETURN_NONE;
+  return Py_BuildValue("(y#iLLLLLLO)", (const char*)&r, (Py_ssize_t)sizeof r, device, c.B, c.T, c.H, c.Hk, c.D, c.width * c.page,
                        packed ? Py_True : Py_False);
 }
 
@@ -236,11 +338,47 @@ PyObject* run_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return PyLong_FromLong(rc);
 }
 
+// run_append_heads(call, q, interleaved, eps, status, stream)
+PyObject* run_append_heads(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  AppendHeads r;
+  View y;
+  if (!arguments("run_append_heads", n, 6) || !call_of(a[0], r) || !memory_of(a[1], y)) return nullptr;
+  r.c8.c.y = y.data;
+  r.c8.c.ldy = r.c8.c.H * r.c8.c.D;
+  const int interleaved = PyObject_IsTrue(a[2]);
+  const float eps = (float)PyFloat_AsDouble(a[3]);
+  r.c8.c.status = (int*)PyLong_AsVoidPtr(a[4]);
+  void* stream = PyLong_AsVoidPtr(a[5]);
+  if (PyErr_Occurred()) return nullptr;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = f_append_heads(&r.c8, r.cos, r.sin, r.positions, r.rotary, interleaved, r.qw, r.kw, eps, stream);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(rc);
+}
+
+// run_read(call, k, v, status, stream)
+PyObject* run_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  gf::PagedCall8 r;
+  View k, v;
+  if (!arguments("run_read", n, 5) || !call_of(a[0], r) || !memory_of(a[1], k) || !memory_of(a[2], v)) return nullptr;
+  r.c.status = (int*)PyLong_AsVoidPtr(a[3]);
+  void* stream = PyLong_AsVoidPtr(a[4]);
+  if (PyErr_Occurred()) return nullptr;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = f_read(&r, k.data, v.data, stream);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(rc);
+}
+
 // run_attention(call, out, scale, one, workspace, parts, scratch, status, stream): gf_paged_attn_one where `one`, else gf_paged_attn
-PyObject* run_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  gf::PagedCall c;
+template <typename Call, typename Attn, typename One>
+PyObject* launch_attention(const char* what, PyObject* const* a, Py_ssize_t n, gf::PagedCall& (*of)(Call&), Attn attn, One attn_one) {
+  Call r;
   View y, ws, few;
-  if (!arguments("run_attention", n, 9) || !call_of(a[0], c) || !memory_of(a[1], y) || !memory_of(a[4], ws) || !memory_of(a[6], few)) return nullptr;
+  if (!arguments(what, n, 9) || !call_of(a[0], r) || !memory_of(a[1], y) || !memory_of(a[4], ws) || !memory_of(a[6], few)) return nullptr;
+  gf::PagedCall& c = of(r);
   c.y = y.data;
   c.ldy = y.ndim == 3 ? y.stride(0, c.H * c.D) : 0;
   const float scale = (float)PyFloat_AsDouble(a[2]);
@@ -251,10 +389,16 @@ PyObject* run_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (PyErr_Occurred()) return nullptr;
   int rc;
   Py_BEGIN_ALLOW_THREADS
-  rc = one ? f_attn_one(&c, scale, (int)parts, (float*)few.data, stream)
-           : f_attn(&c, scale, ws.data, ws.data ? ws.shape[0] : 0, (int)parts, (float*)few.data, stream);
+  rc = one ? attn_one(&r, scale, (int)parts, (float*)few.data, stream)
+           : attn(&r, scale, ws.data, ws.data ? ws.shape[0] : 0, (int)parts, (float*)few.data, stream);
   Py_END_ALLOW_THREADS
   return PyLong_FromLong(rc);
+}
+PyObject* run_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return launch_attention<gf::PagedCall>("run_attention", a, n, [](gf::PagedCall& c) -> gf::PagedCall& { return c; }, f_attn, f_attn_one);
+}
+PyObject* run_attention8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return launch_attention<gf::PagedCall8>("run_attention8", a, n, [](gf::PagedCall8& r) -> gf::PagedCall& { return r.c; }, f_attn8, f_attn8_one);
 }
 
 // A penalty: a number, or 32-bit numbers of every row.
@@ -389,13 +533,18 @@ PyObject* run_sample(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return PyLong_FromLong(rc);
 }
 
-// bind_more(addresses of gf_sample_tokens)
+// bind_more(addresses of gf_sample_tokens, gf_paged_append_heads, gf_paged_read, gf_paged_attn8, gf_paged_attn8_one)
 PyObject* bind_more(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (!arguments("bind_more", n, 1)) return nullptr;
-  void* f[1];
-  for (int i = 0; i < 1; ++i) f[i] = PyLong_AsVoidPtr(a[i]);
+  constexpr int N = 5;
+  if (!arguments("bind_more", n, N)) return nullptr;
+  void* f[N];
+  for (int i = 0; i < N; ++i) f[i] = PyLong_AsVoidPtr(a[i]);
   if (PyErr_Occurred()) return nullptr;
   f_sample = (decltype(f_sample))f[0];
+  f_append_heads = (decltype(f_append_heads))f[1];
+  f_read = (decltype(f_read))f[2];
+  f_attn8 = (decltype(f_attn8))f[3];
+  f_attn8_one = (decltype(f_attn8_one))f[4];
   Py_RETURN_NONE;
 }
 
@@ -433,7 +582,8 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 #define FN(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FN(bind), FN(append), FN(run_append), FN(attention), FN(run_attention), FN(logits), FN(run_logits), FN(sample), FN(run_sample),
-                         FN(bind_more), {nullptr, nullptr, 0, nullptr}};
+                         FN(bind_more), FN(append_heads), FN(run_append_heads), FN(read), FN(run_read),
+                         FN(attention8), FN(run_attention8), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_gf_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -18,6 +18,12 @@ struct PagedCall {
   int* status;
 };
 
+// The same with pages of 8 bits, whose strides are of 16 bytes then: kscales and vscales [pages, Hk, page] dense, null where pages are bf16.
+struct PagedCall8 {
+  PagedCall c;
+  const unsigned char *kscales, *vscales;
+};
+
 struct LogitsCall {
   const void* x;                 // [B, V] of dtype (0 fp32, 1 bf16, 2 fp16), rows ldx apart
   long long ldx;

@@ -55,9 +55,23 @@ inline bool paged_batch(PagedBatch& s, const PagedCall& c) {
   return true;
 }
 
+// Pages of 8 bits. A row of a head is numbers of type e4m3 times 2^(b - 127), b the row's byte in the scales: the smallest power of two that leaves none of them
+// above 448, the type's largest, so that none is cut off; and at least 2^-126. A power of two loses no bits in what it is multiplied with: a number of the
+// cache has 4 bits, and is one of bf16 too. (A scale that brings the largest number to 448 itself gains nothing: the type's steps are
+// relative.) Scales of a head lie one behind the other, so that 16 keys' are 16 bytes.
+inline bool paged_scales(const PagedCall8& c8) {
+  const PagedCall& c = c8.c;
+  for (const void* p : {(const void*)c8.kscales, (const void*)c8.vscales})
+    if (!p || (reinterpret_cast<uintptr_t>(p) & 15)) return false;
+  for (long long st : c.strides)
+    if (st % 16) return false;
+  return c.D % 16 == 0;
+}
+
 // attn_decode.cu: one new token of each sequence of a call (with cu: of those that have one), as gf_paged_attn_one. `chained`: behind a
 // kernel of the same call that it does not depend on; it starts under it and ends behind it.
 bool attn_paged_one_ok(const PagedCall& c, int splits, const float* scratch);
-int attn_paged_one(const PagedCall& c, float scale, int splits, float* scratch, int chained, cudaStream_t st);
+int attn_paged_one(const PagedCall& c, float scale, int splits, float* scratch, int chained, cudaStream_t st, const unsigned char* kscales = nullptr,
+                   const unsigned char* vscales = nullptr);      // scales: pages of 8 bits
 
 }  // namespace gf

@@ -8,6 +8,13 @@
 // head it works on (8 pairs, two vectors), so it reads its part of the tables once, and all its loads are on their way before it knows where
 // the token goes. 4500 tokens of five prompts, 32 / 32 heads of 128: 39 us, 5.9 TB/s; one token of each of 64 sequences 2.6 us, three looks into memory
 // one behind the other (lengths, page, table rows). What a call costs is then its launch.
+//
+// Heads that are normed or rotated in part, and pages of 8 bits, have a kernel of their own (the one without them is as it was): the same CTA to a token, with
+// D / 16 neighbouring lanes to a head (norm_rope.cuh), whose sum of squares, and largest number, are shuffles. Rows read back are written out as bf16, which
+// has all of their bits.
+#include <type_traits>
+
+#include "norm_rope.cuh"
 #include "paged.cuh"
 
 namespace gf {
@@ -114,6 +121,208 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const __grid_c
   }
 }
 
+struct PagedHeads {
+  PagedAppend a;                 // pools and strides are of bytes where there are scales
+  const __nv_bfloat16 *qw, *kw;  // [D]; null: no norms
+  unsigned char *kscales, *vscales;
+  float eps;
+  int rotary;
+};
+
+// Where a new token's row is.
+struct PagedRow {
+  long long page;
+  int pos, r;                    // position, row of the page
+  bool there, stored;            // the token has a position; its row is in the pools
+};
+// Whole CTA; false for tokens behind the last sequence. `positions`: those that there are tables for.
+__device__ __forceinline__ bool paged_row(const PagedBatch& S, int t, int positions, PagedRow& row) {
+  const int b = paged_seq_of(S, t);
+  if (b >= S.B) return false;
+  const int first = S.first(b), end = S.end(b);
+  if (t < first || t >= end) return false;
+  row.pos = S.lens[b] - (end - first) + (t - first);
+  row.there = row.pos >= 0;
+  bool bad = row.there && (row.pos >= S.capacity() || row.pos >= positions);
+  if (bad) row.there = false;
+  row.page = row.there ? S.table[(long long)b * S.ld + (row.pos >> S.page_shift)] : 0;
+  row.stored = row.there && row.page >= 0 && row.page < S.pages;
+  bad |= row.there && !row.stored;
+  if (bad && threadIdx.x == 0) S.bad();
+  row.r = row.pos & ((1 << S.page_shift) - 1);
+  return true;
+}
+
+__device__ __forceinline__ unsigned short e4m3x2(float lo, float hi) {
+  unsigned short r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// 8 numbers in a unit of `inv`^-1.
+__device__ __forceinline__ uint2 e4m3x8(const float (&f)[8], float inv) {
+  unsigned short h[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = e4m3x2(f[2 * i] * inv, f[2 * i + 1] * inv);
+  return make_uint2(h[0] | (unsigned)h[1] << 16, h[2] | (unsigned)h[3] << 16);
+}
+template <int LANES>
+__device__ __forceinline__ unsigned group_max(unsigned v) {
+#pragma unroll
+  for (int o = LANES / 2; o; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+// Whole warp: the byte of a row's power of two. What is not finite becomes NaN, which the type has, and counts for nothing.
+template <int LANES>
+__device__ __forceinline__ unsigned scale_byte(Head16& v) {
+  constexpr unsigned INF = 0x7f800000u;
+  auto largest = [&](bool finite) {
+    unsigned m = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+#pragma unroll
+      for (unsigned u : {__float_as_uint(v.a[e]) & 0x7fffffffu, __float_as_uint(v.b[e]) & 0x7fffffffu}) m = max(m, finite && u >= INF ? 0 : u);
+    return group_max<LANES>(m);
+  };
+  unsigned m = largest(false);
+  if (__any_sync(0xffffffffu, m >= INF)) {
+    m = largest(true);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v.a[e] += v.a[e] - v.a[e];
+      v.b[e] += v.b[e] - v.b[e];
+    }
+  }
+  // m = 1.f 2^(E - 127), 448 = 1.75 2^8
+  return (unsigned)max(1, (int)(m >> 23) - 8 + ((m & 0x7fffffu) > 0x600000u));
+}
+
+template <int LANES, bool BYTES>
+__global__ void __launch_bounds__(PA_THREADS) paged_append_heads_kernel(const __grid_constant__ PagedHeads p) {
+  constexpr int D = 16 * LANES, STEP = PA_THREADS / LANES;
+  const PagedAppend& A = p.a;
+  const int t = blockIdx.x, head0 = threadIdx.x / LANES, i = threadIdx.x % LANES, heads = A.H + 2 * A.Hk;
+  const HeadLane at(i, p.rotary, A.interleaved);
+  const __nv_bfloat16* from = A.qkv + (long long)t * A.ldx;
+  uint4 x[PA_AHEAD], y[PA_AHEAD];
+  auto load = [&](int h0) {
+#pragma unroll
+    for (int n = 0; n < PA_AHEAD; ++n) {
+      const int h = h0 + n * STEP;
+      x[n] = y[n] = make_uint4(0, 0, 0, 0);
+      if (h < heads) {
+        x[n] = *reinterpret_cast<const uint4*>(from + (long long)h * D + at.x);
+        y[n] = *reinterpret_cast<const uint4*>(from + (long long)h * D + at.y);
+      }
+    }
+  };
+  load(head0);
+  PagedRow row;
+  if (!paged_row(A.seqs, t, A.positions, row)) return;
+  float c[8], s[8];
+  const long long off = (long long)row.pos * (p.rotary / 2) + at.t;
+  table8(A.cos + off, row.there && at.turns, c);
+  table8(A.sin + off, row.there && at.turns, s);
+  for (int base = 0; base < heads; base += PA_AHEAD * STEP) {              // (the same for all lanes of a warp)
+    if (base) load(base + head0);
+#pragma unroll
+    for (int n = 0; n < PA_AHEAD; ++n) {
+      const int h = base + head0 + n * STEP;
+      const bool query = h < A.H, key = !query && h < A.H + A.Hk;
+      if (!__any_sync(0xffffffffu, h < heads)) break;
+      Head16 v;
+      v.of(x[n], y[n]);
+      if (p.qw) {
+        const float r = rsqrtf(group_sum<LANES>(v.dot(v)) * (1.f / D) + p.eps);
+        if (query || key) {
+          Head16 w;
+          const __nv_bfloat16* weight = query ? p.qw : p.kw;
+          w.of(__ldg(reinterpret_cast<const uint4*>(weight + at.x)), __ldg(reinterpret_cast<const uint4*>(weight + at.y)));
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            v.a[e] *= r * w.a[e];
+            v.b[e] *= r * w.b[e];
+          }
+        }
+      }
+      if ((query || key) && at.turns) v.turn<1>(c, s, A.interleaved);
+      unsigned byte = 0;
+      if constexpr (BYTES) byte = scale_byte<LANES>(v);
+      if (query) {
+        v.to(x[n], y[n]);
+        if (!row.there) x[n] = y[n] = make_uint4(0, 0, 0, 0);              // not the products of what stands there
+        __nv_bfloat16* to = A.q + ((long long)t * A.H + h) * D;
+        *reinterpret_cast<uint4*>(to + at.x) = x[n];
+        *reinterpret_cast<uint4*>(to + at.y) = y[n];
+        continue;
+      }
+      if (!row.stored || h >= heads) continue;
+      const int hk = h - A.H - (key ? 0 : A.Hk);
+      const long long to = key ? row.page * A.kpage + row.r * A.krow + hk * A.khead : row.page * A.vpage + row.r * A.vrow + hk * A.vhead;
+      if constexpr (BYTES) {
+        unsigned char* pool = reinterpret_cast<unsigned char*>(key ? A.kp : A.vp) + to;
+        const float inv = __uint_as_float((254u - byte) << 23);
+        *reinterpret_cast<uint2*>(pool + at.x) = e4m3x8(v.a, inv);
+        *reinterpret_cast<uint2*>(pool + at.y) = e4m3x8(v.b, inv);
+        if (i == 0) (key ? p.kscales : p.vscales)[((row.page * A.Hk + hk) << A.seqs.page_shift) + row.r] = (unsigned char)byte;
+      } else {
+        __nv_bfloat16* pool = (key ? A.kp : A.vp) + to;
+        v.to(x[n], y[n]);
+        *reinterpret_cast<uint4*>(pool + at.x) = x[n];
+        *reinterpret_cast<uint4*>(pool + at.y) = y[n];
+      }
+    }
+  }
+}
+
+struct PagedRead {
+  PagedBatch seqs;
+  const void *kp, *vp;
+  const unsigned char *kscales, *vscales;
+  __nv_bfloat16 *k, *v;          // [T, Hk, D] dense
+  long long kpage, krow, khead, vpage, vrow, vhead;
+  int Hk, D;
+};
+
+__device__ __forceinline__ uint32_t bf16x2_of_e4m3(unsigned short two, float scale) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(two));
+  float lo, hi;
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, h;\n\t}" : "=f"(lo), "=f"(hi) : "r"(h));
+  return pack_bf16x2(lo * scale, hi * scale);
+}
+
+template <bool BYTES>
+__global__ void __launch_bounds__(PA_THREADS) paged_read_kernel(const __grid_constant__ PagedRead p) {
+  const int t = blockIdx.x, per = p.D / 16, all = 2 * p.Hk * per;
+  PagedRow row{};
+  if (!paged_row(p.seqs, t, 0x7fffffff, row)) row.stored = false;
+  for (int id = threadIdx.x; id < all; id += PA_THREADS) {
+    const int i = id % per, head = id / per;
+    const bool key = head < p.Hk;
+    const int hk = key ? head : head - p.Hk;
+    const long long from = key ? row.page * p.kpage + row.r * p.krow + hk * p.khead : row.page * p.vpage + row.r * p.vrow + hk * p.vhead;
+    uint4 x[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+    if (row.stored) {
+      if constexpr (BYTES) {
+        const uint4 in = *reinterpret_cast<const uint4*>((const unsigned char*)(key ? p.kp : p.vp) + from + 16 * i);
+        const unsigned byte = (key ? p.kscales : p.vscales)[((row.page * p.Hk + hk) << p.seqs.page_shift) + row.r];
+        const float scale = __uint_as_float(byte << 23);
+        const unsigned short* two = reinterpret_cast<const unsigned short*>(&in);
+        uint32_t* u = reinterpret_cast<uint32_t*>(x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u[e] = bf16x2_of_e4m3(two[e], scale);
+      } else {
+        const uint4* in = reinterpret_cast<const uint4*>((const __nv_bfloat16*)(key ? p.kp : p.vp) + from + 16 * i);
+        x[0] = in[0];
+        x[1] = in[1];
+      }
+    }
+    uint4* to = reinterpret_cast<uint4*>((key ? p.k : p.v) + ((long long)t * p.Hk + hk) * p.D + 16 * i);
+    to[0] = x[0];
+    to[1] = x[1];
+  }
+}
+
 }  // namespace gf
 
 using namespace gf;
@@ -141,5 +350,66 @@ GF_API int gf_paged_append(const PagedCall* c, const float* cos, const float* si
   p.cos = cos; p.sin = sin;
   p.H = (int)H; p.Hk = (int)Hk; p.D = (int)D; p.positions = positions; p.interleaved = interleaved;
   paged_append_kernel<<<p.seqs.T, PA_THREADS, 0, (cudaStream_t)stream>>>(p);
+  return cudaGetLastError() == cudaSuccess ? GFH_OK : GFH_CUDA;
+}
+
+// The same with heads that are normed (qw, kw [D]; null: not) and of which `rotary` dims are rotated (tables [positions, rotary / 2]), into pages of bf16 (no
+// scales) or of 8 bits. GFH_OVERLAP where x shares memory with the pools or scales. D of 32, 64, 128 or 256.
+GF_API int gf_paged_append_heads(const PagedCall8* c8, const float* cos, const float* sin, int positions, int rotary, int interleaved, const void* qw,
+                                 const void* kw, float eps, void* stream) {
+  PagedHeads p{};
+  if (!c8 || !paged_batch(p.a.seqs, c8->c) || !c8->kscales != !c8->vscales || (c8->kscales && !paged_scales(*c8))) return GFH_BAD_ARG;
+  const PagedCall* c = &c8->c;
+  const long long H = c->H, Hk = c->Hk, D = c->D, size = c8->kscales ? 1 : 2;
+  if (H <= 0 || Hk <= 0 || H > 65535 || Hk > 65535 || (D != 32 && D != 64 && D != 128 && D != 256) || positions < 0 || c->ldy != H * D || rotary < 0 ||
+      rotary > D || rotary % 16 || !qw != !kw || ((reinterpret_cast<uintptr_t>(qw) | reinterpret_cast<uintptr_t>(kw)) & 15) ||
+      (rotary && (!cos || !sin)) || ((reinterpret_cast<uintptr_t>(cos) | reinterpret_cast<uintptr_t>(sin)) & 15))
+    return GFH_BAD_ARG;
+  // new tokens are read while others are written to the pages
+  const char *x0 = (const char*)c->x, *x1 = x0 + 2 * ((c->T - 1) * c->ldx + (H + 2 * Hk) * D);
+  for (int i = 0; i < 2; ++i) {
+    const long long* st = c->strides + 3 * i;
+    const char *pool = (const char*)(i ? c->vpages : c->kpages), *scales = (const char*)(i ? c8->vscales : c8->kscales);
+    if (c->pages > 0 && x0 < pool + size * ((c->pages - 1) * st[0] + (c->page - 1) * st[1] + (Hk - 1) * st[2] + D) && pool < x1) return GFH_OVERLAP;
+    if (scales && x0 < scales + c->pages * c->page * Hk && scales < x1) return GFH_OVERLAP;
+  }
+  gf::enter();
+  PagedAppend& a = p.a;
+  a.qkv = (const __nv_bfloat16*)c->x; a.ldx = c->ldx;
+  a.q = (__nv_bfloat16*)c->y; a.kp = (__nv_bfloat16*)c->kpages; a.vp = (__nv_bfloat16*)c->vpages;
+  a.kpage = c->strides[0]; a.krow = c->strides[1]; a.khead = c->strides[2];
+  a.vpage = c->strides[3]; a.vrow = c->strides[4]; a.vhead = c->strides[5];
+  a.cos = cos; a.sin = sin;
+  a.H = (int)H; a.Hk = (int)Hk; a.D = (int)D; a.positions = positions; a.interleaved = interleaved;
+  p.qw = (const __nv_bfloat16*)qw; p.kw = (const __nv_bfloat16*)kw; p.eps = eps; p.rotary = rotary;
+  p.kscales = (unsigned char*)c8->kscales; p.vscales = (unsigned char*)c8->vscales;
+  auto of = [&](auto bytes) {
+    constexpr bool B = decltype(bytes)::value;
+    return D == 32 ? paged_append_heads_kernel<2, B> : D == 64 ? paged_append_heads_kernel<4, B> : D == 128 ? paged_append_heads_kernel<8, B>
+                                                                                                           : paged_append_heads_kernel<16, B>;
+  };
+  auto kern = c8->kscales ? of(std::true_type{}) : of(std::false_type{});
+  kern<<<a.seqs.T, PA_THREADS, 0, (cudaStream_t)stream>>>(p);
+  return cudaGetLastError() == cudaSuccess ? GFH_OK : GFH_CUDA;
+}
+
+// Rows of the new tokens out of the pages: k, v [T, Hk, D] dense bf16, zeros for tokens that have none. x and y of the call are not looked at.
+GF_API int gf_paged_read(const PagedCall8* c8, void* k, void* v, void* stream) {
+  PagedRead p{};
+  if (!c8 || !k || !v || ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15)) return GFH_BAD_ARG;
+  PagedCall c = c8->c;
+  c.x = c.y = k;
+  c.ldx = c.ldy = 0;
+  if (!paged_batch(p.seqs, c) || !c8->kscales != !c8->vscales || (c8->kscales && !paged_scales(*c8)) || c.Hk <= 0 || c.Hk > 65535 || c.D < 16 || c.D % 16 ||
+      c.D > 4096)
+    return GFH_BAD_ARG;
+  gf::enter();
+  p.kp = c.kpages; p.vp = c.vpages; p.kscales = c8->kscales; p.vscales = c8->vscales;
+  p.k = (__nv_bfloat16*)k; p.v = (__nv_bfloat16*)v;
+  p.kpage = c.strides[0]; p.krow = c.strides[1]; p.khead = c.strides[2];
+  p.vpage = c.strides[3]; p.vrow = c.strides[4]; p.vhead = c.strides[5];
+  p.Hk = (int)c.Hk; p.D = (int)c.D;
+  auto kern = c8->kscales ? paged_read_kernel<true> : paged_read_kernel<false>;
+  kern<<<p.seqs.T, PA_THREADS, 0, (cudaStream_t)stream>>>(p);
   return cudaGetLastError() == cudaSuccess ? GFH_OK : GFH_CUDA;
 }

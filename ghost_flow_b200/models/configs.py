@@ -7,7 +7,7 @@ GQA fields (llama.rs:28) with its MoE defaults (ghostflow-nn/src/mixture_of_expe
 """
 from __future__ import annotations
 
-from dataclasses import dataclass, replace
+from dataclasses import dataclass, field, replace
 
 
 @dataclass
@@ -24,10 +24,17 @@ class LLaMAConfig:
     rope_interleaved: bool = False
     initializer_range: float = 0.02
     tie_word_embeddings: bool = False
+    qk_norm: bool = field(default=False, kw_only=True)             # RMS norms of every query and key head, in front of the rotation
+    rotary_dim: int | None = field(default=None, kw_only=True)     # dims of a head that are rotated; None: all
 
     @property
     def head_dim(self) -> int:
         return self.hidden_size // self.num_attention_heads
+
+    @property
+    def plain_heads(self) -> bool:
+        """Whether heads are rotated as a whole and not normed: what the layers' fused forms and the parallel engines take."""
+        return not self.qk_norm and self.rotary_dim in (None, self.head_dim)
 
     @classmethod
     def llama_7b(cls): return cls()
@@ -54,7 +61,7 @@ class LLaMAConfig:
     def num_parameters(self) -> int:
         d, f, v = self.hidden_size, self.intermediate_size, self.vocab_size
         kv = self.num_key_value_heads * self.head_dim
-        per_layer = 2 * d + d * (d + 2 * kv) + d * d + 3 * d * f
+        per_layer = 2 * d + d * (d + 2 * kv) + d * d + 3 * d * f + (2 * self.head_dim if self.qk_norm else 0)
         head = 0 if self.tie_word_embeddings else v * d
         return self.num_hidden_layers * per_layer + v * d + d + head
 

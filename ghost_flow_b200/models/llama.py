@@ -27,6 +27,29 @@ class LLaMAAttention(Module):
         self.wqkv = Linear(cfg.hidden_size, (cfg.num_attention_heads + 2 * cfg.num_key_value_heads) * hd, False,
                            device, dtype)
         self.wo = Linear(cfg.num_attention_heads * hd, cfg.hidden_size, False, device, dtype)
+        if cfg.qk_norm:
+            self.q_norm = RMSNorm(hd, cfg.rms_norm_eps, device, dtype)
+            self.k_norm = RMSNorm(hd, cfg.rms_norm_eps, device, dtype)
+
+    def _weights(self):
+        """Weights of the heads' norms, if there are any."""
+        return (self.q_norm.weight, self.k_norm.weight) if self.cfg.qk_norm else (None, None)
+
+    def _heads(self, qkv, cos, sin, start_pos):
+        c = self.cfg
+        H, Hk = c.num_attention_heads, c.num_key_value_heads
+        if c.plain_heads:
+            return ops.rope_qkv(qkv, H, Hk, cos, sin, c.rope_interleaved, start_pos)
+        return ops.norm_rope_qkv(qkv, H, Hk, *self._weights(), cos, sin, c.rms_norm_eps, c.rope_interleaved, start_pos)
+
+    def _heads_to_cache(self, qkv, cos, sin, kc, vc, start_pos):
+        c = self.cfg
+        if c.plain_heads:
+            return ops.rope_qkv_to_cache(qkv, c.num_attention_heads, c.num_key_value_heads, cos, sin, kc, vc, c.rope_interleaved, start_pos)
+        q, k, v = self._heads(qkv, cos, sin, start_pos)
+        kc[:, start_pos:start_pos + q.shape[1]] = k
+        vc[:, start_pos:start_pos + q.shape[1]] = v
+        return q
 
     def forward(self, x, cos, sin, residual=None, cache=None, start_pos: int = 0):
         c = self.cfg
@@ -39,17 +62,17 @@ class LLaMAAttention(Module):
             kernels = x.is_cuda and x.dtype == torch.bfloat16 and D in (64, 128) and not torch.is_grad_enabled()
             if kernels and start_pos == 0 and S > 1:
                 # prompt: nothing older than itself to attend to
-                q, k, v = ops.rope_qkv(qkv, H, Hk, cos, sin, c.rope_interleaved, start_pos)
+                q, k, v = self._heads(qkv, cos, sin, start_pos)
                 kc[:, :S] = k
                 vc[:, :S] = v
                 o = ops.flash_attention(q, k, v, causal=True)
             elif kernels and S == 1:
-                q = ops.rope_qkv_to_cache(qkv, H, Hk, cos, sin, kc, vc, c.rope_interleaved, start_pos)
+                q = self._heads_to_cache(qkv, cos, sin, kc, vc, start_pos)
                 # one new token per sequence: the decode kernel streams the cache once (GQA groups share the reads)
                 o = raw.attn_decode(q.reshape(B, H * D), kc.view(B, kc.shape[1], Hk * D), vc.view(B, vc.shape[1], Hk * D),
                                     start_pos + 1, B, H, Hk, D).view(B, 1, H, D)
             else:
-                q = ops.rope_qkv_to_cache(qkv, H, Hk, cos, sin, kc, vc, c.rope_interleaved, start_pos)
+                q = self._heads_to_cache(qkv, cos, sin, kc, vc, start_pos)
                 kk, vv = kc[:, :start_pos + S], vc[:, :start_pos + S]
                 G = H // Hk
                 qf = q.transpose(1, 2).float()
@@ -61,7 +84,7 @@ class LLaMAAttention(Module):
                 s = s.masked_fill(~mask, float("-inf"))
                 o = (torch.softmax(s, -1) @ vf).transpose(1, 2).to(x.dtype)
         else:
-            q, k, v = ops.rope_qkv(qkv, H, Hk, cos, sin, c.rope_interleaved, start_pos)
+            q, k, v = self._heads(qkv, cos, sin, start_pos)
             o = ops.flash_attention(q, k, v, causal=True)
         return self.wo(o.reshape(B, S, H * D), residual)
 
@@ -70,8 +93,11 @@ class LLaMAAttention(Module):
         c = self.cfg
         H, Hk, D = c.num_attention_heads, c.num_key_value_heads, c.head_dim
         qkv = self.wqkv(x).view(x.shape[0], H + 2 * Hk, D)
-        q = ops.rope_qkv_to_pages(qkv, H, Hk, cos, sin, *pools, batch.table, batch.lens, batch.cu, c.rope_interleaved)
-        o = ops.paged_attention(q, *pools, batch.table, batch.lens, batch.cu)
+        k, v, *scales = pools
+        scales = dict(zip(("kscales", "vscales"), scales))
+        norms = dict(q_weight=self.q_norm.weight, k_weight=self.k_norm.weight, eps=c.rms_norm_eps) if c.qk_norm else {}
+        q = ops.rope_qkv_to_pages(qkv, H, Hk, cos, sin, k, v, batch.table, batch.lens, batch.cu, c.rope_interleaved, **scales, **norms)
+        o = ops.paged_attention(q, k, v, batch.table, batch.lens, batch.cu, **scales)
         return self.wo(o.reshape(x.shape[0], H * D), residual)
 
 
@@ -108,6 +134,8 @@ class LLaMADecoderLayer(Module):
         if not plain_modules(an, at, fn, mlp, *lin):
             return None
         c, (kc, vc), (B, _, hidden), dev = at.cfg, cache, x.shape, x.device
+        if not c.plain_heads:
+            return None
         H, Hk, D = c.num_attention_heads, c.num_key_value_heads, c.head_dim
         w = [_weight(n) for n in (an, lin[0], lin[1], fn, lin[2], lin[3])]
         inner = w[5].shape[1] if w[5].dim() == 2 else 0
@@ -151,7 +179,7 @@ class LLaMAModel(Module):
     def rope(self, length, device):
         if self._rope is None or self._rope[0].shape[0] < length or self._rope[0].device != torch.device(device):
             n = max(length, self.cfg.max_position_embeddings)
-            self._rope = ops.rope_tables(n, self.cfg.head_dim, self.cfg.rope_theta, device)
+            self._rope = ops.rope_tables(n, self.cfg.rotary_dim or self.cfg.head_dim, self.cfg.rope_theta, device)
         return self._rope
 
     def _before_norm(self, ids, caches, start_pos):
@@ -248,7 +276,7 @@ class LLaMAForCausalLM(Module):
 
     @torch.no_grad()
     def generate(self, ids, max_new_tokens: int, temperature: float = 0.0, **choice):
-        """Greedy (temperature 0) or sampled continuation with a KV cache. ``choice``: penalties, bias and mask of
+        """Greedy (temperature 0) or sampled continuation with a KV cache. ``choice``: penalties, bias, mask, top-k, top-p and min-p of
         :func:`~ghost_flow_b200.ops.sampling.next_tokens`."""
         B, S = ids.shape
         caches = self.new_caches(B, S + max_new_tokens)
@@ -264,10 +292,10 @@ class LLaMAForCausalLM(Module):
 
     @torch.no_grad()
     def generate_batch(self, prompts, max_new_tokens: int, temperature: float = 0.0, page_size: int = 64, chunk_tokens: int = 4096,
-                       **choice):
+                       cache_dtype=None, **choice):
         """Continuations of prompts (1-D token tensors) of any lengths in one batch over a paged cache; a list of prompts with their
-        ``max_new_tokens`` new tokens. Prompts go through the model at most ``chunk_tokens`` tokens at a time. ``choice`` as for
-        :meth:`generate`."""
+        ``max_new_tokens`` new tokens. Prompts go through the model at most ``chunk_tokens`` tokens at a time. ``cache_dtype``: of the cache, the
+        model's or ``torch.float8_e4m3fn``. ``choice`` as for :meth:`generate`."""
         p = next(self.parameters())
         prompts = [t.to(p.device).long().reshape(-1) for t in prompts]
         if not prompts or max_new_tokens <= 0:
@@ -275,7 +303,7 @@ class LLaMAForCausalLM(Module):
         if any(t.numel() == 0 for t in prompts) or chunk_tokens < 1:
             raise ValueError("generate_batch continues prompts of one token or more, in chunks of one or more")
         B, lens = len(prompts), [t.numel() for t in prompts]
-        cache = self.new_paged_cache(sum(-(-(n + max_new_tokens) // page_size) for n in lens), page_size)
+        cache = self.new_paged_cache(sum(-(-(n + max_new_tokens) // page_size) for n in lens), page_size, dtype=cache_dtype)
         for b, n in enumerate(lens):
             cache.reserve(b, n + max_new_tokens)
         # the prompts, in chunks: logits are wanted of their last tokens only

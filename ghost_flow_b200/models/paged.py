@@ -9,6 +9,8 @@ from dataclasses import dataclass
 
 import torch
 
+from ..ops import read_pages
+
 
 @dataclass
 class PagedBatch:
@@ -25,12 +27,22 @@ class PagedBatch:
 
 
 class PagedKVCache:
-    """``num_pages`` pages of ``page_size`` rows (a power of two from 16 for the kernels) for the keys and values of ``layers`` layers."""
+    """``num_pages`` pages of ``page_size`` rows (a power of two from 16 for the kernels) for the keys and values of ``layers`` layers. ``pools``: of each
+    layer keys and values, and with the type ``torch.float8_e4m3fn``, which takes half the memory, their scales (see ``ops/paged.py``)."""
 
     def __init__(self, layers: int, num_pages: int, page_size: int, kv_heads: int, head_dim: int, device=None, dtype=None):
         shape = (num_pages, page_size, kv_heads, head_dim)
         self.page_size = page_size
-        self.pools = [(torch.zeros(shape, device=device, dtype=dtype), torch.zeros(shape, device=device, dtype=dtype)) for _ in range(layers)]
+        kinds = [(shape, dtype)] * 2
+        if dtype is torch.float8_e4m3fn:
+            kinds += [((num_pages, kv_heads, page_size), torch.float8_e8m0fnu)] * 2
+
+        def pool(shape, dtype):
+            if dtype is None or not str(dtype).startswith("torch.float8"):
+                return torch.zeros(shape, device=device, dtype=dtype)
+            return torch.zeros(shape, device=device, dtype=torch.uint8).view(dtype)
+
+        self.pools = [tuple(pool(*k) for k in kinds) for _ in range(layers)]
         self.device = self.pools[0][0].device if layers else torch.device(device or "cpu")
         self._free = list(range(num_pages - 1, -1, -1))
         self._pages: dict = {}
@@ -50,6 +62,13 @@ class PagedKVCache:
     def release(self, sequence) -> None:
         """Gives a sequence's pages back."""
         self._free.extend(reversed(self._pages.pop(sequence)))
+
+    def read(self, sequence, length: int, layer: int = 0):
+        """Keys and values ``[length, KV heads, head size]`` of the first ``length`` positions of a sequence, as they stand in a layer's pools (of pools of 8 bits
+        as bf16)."""
+        batch = self.batch([sequence], [length], [length])
+        k, v, *scales = self.pools[layer]
+        return read_pages(length, k, v, batch.table, batch.lens, batch.cu, *scales)
 
     def batch(self, sequences, lens, new=None) -> PagedBatch:
         """The batch of ``sequences`` with ``lens`` keys each, of which the last ``new`` (one, without it) are new tokens. Their pages have to be

@@ -46,6 +46,9 @@ _SIGS = {
     "gf_rope": [P, P, P, I, I, I, L, L, I, I, I, I, P],
     "gf_embedding_rows": [P, I, P, P, L, L, I, P],
     "gf_rope_qkv": [P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, P],
+    "gf_norm_rope_qkv": [P, L, P, P, P, P, P, P, L, I, I, I, I, I, I, I, F, P],
+    "gf_norm_rope_scratch": [I],
+    "gf_norm_rope_qkv_bwd": [P, L, P, P, P, P, P, P, P, P, P, P, P, P, L, I, I, I, I, I, I, I, F, P],
     "gf_swiglu_fwd": [P, P, L, I, P],
     "gf_scale_by_dev_scalar": [P, L, P, P],
     "gf_swiglu_bwd": [P, P, P, L, I, P],
@@ -75,9 +78,13 @@ _SIGS = {
     "gf_llama_decode_layer": [P, P, F, P, P, P, F, P, P, P, P, P, P, I, P, P, I, I, I, I, I, I, I, I, I, P, P],
     "gf_attn_decode": [P, L, P, P, I, P, I, P, L, I, I, I, I, F, I, P, P],
     "gf_paged_append": [P, P, P, I, I, P],
+    "gf_paged_append_heads": [P, P, P, I, I, I, P, P, F, P],
+    "gf_paged_read": [P, P, P, P],
     "gf_paged_attn_workspace": [I, I, I, I, L, I, I, I],
     "gf_paged_attn": [P, F, P, L, I, P, P],
     "gf_paged_attn_one": [P, F, I, P, P],
+    "gf_paged_attn8": [P, F, P, L, I, P, P],
+    "gf_paged_attn8_one": [P, F, I, P, P],
     "gf_process_logits": [P, P],
     "gf_sample_tokens": [P, P],
     "gf_flash_attn_bwd": [P, P, P, P, P, P, P, P, P, I, I, I, I, I, L, L, L, L, L, L, F, I, P, P],
@@ -152,7 +159,8 @@ def calls():
 
         module.bind(exchange, *(ctypes.cast(getattr(lib, name), c_void_p).value for name in (
             "gf_paged_append", "gf_paged_attn", "gf_paged_attn_one", "gf_process_logits")), *follows())
-        module.bind_more(*(ctypes.cast(getattr(lib, name), c_void_p).value for name in ("gf_sample_tokens",)))
+        module.bind_more(*(ctypes.cast(getattr(lib, name), c_void_p).value for name in (
+            "gf_sample_tokens", "gf_paged_append_heads", "gf_paged_read", "gf_paged_attn8", "gf_paged_attn8_one")))
         _CALLS = module
     return _CALLS
 

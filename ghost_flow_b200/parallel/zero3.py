@@ -148,6 +148,8 @@ class Zero3LlamaEngine:
         self.world, self.rank = self.comm.world, self.comm.rank
         self.streams = _Streams(self.device)
         self.step_count = 0
+        if not cfg.plain_heads:
+            raise NotImplementedError("heads that are normed or rotated in part are not wired into this engine")
         d, f, v = cfg.hidden_size, cfg.intermediate_size, cfg.vocab_size
         hd = cfg.head_dim
         self.qkv_out = (cfg.num_attention_heads + 2 * cfg.num_key_value_heads) * hd

@@ -85,7 +85,7 @@ def _llama_config_from_state(state: dict, extra: dict | None = None):
     qkv_out = state["model.layers.0.attn.wqkv.weight"].shape[0]
     inter = state["model.layers.0.mlp.w_gate_up.weight"].shape[0] // 2 if "model.layers.0.mlp.w_gate_up.weight" in state \
         else state["model.layers.0.mlp.gate_up.weight"].shape[0] // 2
-    ex = dict(extra or {})
+    ex = {"qk_norm": "model.layers.0.attn.q_norm.weight" in state, **(extra or {})}
     heads = int(ex.pop("num_attention_heads", hidden // (128 if hidden % 128 == 0 and hidden >= 512 else 64)))
     hd = hidden // heads
     kv = int(ex.pop("num_key_value_heads", (qkv_out // hd - heads) // 2))

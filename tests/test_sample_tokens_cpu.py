@@ -61,7 +61,7 @@ def test_shares_follow_the_weights():
                                 dict(u=torch.rand(3, device="meta")), dict(temperature=torch.ones(2)), dict(temperature=torch.ones(3, 1)),
                                 dict(top_k=torch.ones(3)), dict(top_k=torch.ones(3, dtype=torch.int64)), dict(top_p=torch.ones(3).bfloat16()),
                                 dict(min_p=torch.ones(())), dict(logits=torch.randn(9)), dict(logits=torch.ones(3, 9, dtype=torch.int64)),
-                                dict(logits=torch.randn(3, 0))], ids=str)
+                                dict(logits=torch.randn(3, 0))], ids=lambda k: "-".join(k))
 def test_refusals(kw):
     with pytest.raises(ValueError, match="sample_tokens"):
         ops.sample_tokens(**{"logits": torch.randn(3, 9), "u": torch.rand(3), **kw})
