@@ -12,11 +12,12 @@
 // neighbour (a vocabulary of 50257 has that many borders, each off by some 2^-25). A weight below the last bit counts as one of it: u = 0 still takes the
 // first token that stays.
 //
-// One CTA has a row, and reads it from L2 in every pass but the first: the largest entry; a histogram over bins of equal width of m - x, of numbers or of weights,
-// that says in which bin the k-th entry or the share p ends; the entries of that bin, which are ranked among each other in shared memory (each thread has one
-// and looks at all others). Bins of too many entries are cut further by the entries' bits, and entries that are all equal counted off in the order of
-// the vocabulary. A last pass leaves the sums of every warp's pieces, among which u is looked up. Where all of the first k entries fit into shared memory the
-// rest happens there, without that pass.
+// One CTA has a row, and reads it from L2 in every pass but the first: the largest entry; a histogram over bins of equal width of m - x, which says in which bin the k-th
+// entry lies, or about where the share p ends; then, with top-k, all entries up to that bin go to shared memory, are put in order there, and the rest is done
+// among them. Without it a pass adds up the weights: all, those in front of the bins around the place where the share may end, the latter by 32 parts of
+// the vocabulary too, and leaves the entries of those bins in shared memory, among which the last one that stays is found. u then tells the part, and the
+// token in it. What does not fit (more than 1024 entries, as with equal ones) takes as many histograms as it wants, by weights and then by the entries' bits, and
+// entries that are all equal are counted off in the order of the vocabulary.
 #include <cuda_fp16.h>
 
 #include "calls.h"
@@ -25,9 +26,7 @@
 
 namespace gf {
 
-constexpr int SM_THREADS = 512, SM_WARPS = SM_THREADS / 32;
 constexpr int SM_BINS = 2048;
-constexpr int SM_LIST = SM_THREADS;      // entries that are ranked in shared memory
 constexpr int SM_MOST = 1 << 20;         // entries of a row
 
 typedef unsigned long long u64;
@@ -42,25 +41,38 @@ struct SampleParams {
   int top_k0;
   long long* out;                                   // [B]
   int V, bits;                                      // a weight of 1 is 2^bits
+  double series[5];                                 // (log(2) / 16)^n / n!, n from 1: operands that an instruction takes from here, not from registers
 };
 
+constexpr int SM_LIST = 1024;    // entries that are ordered in shared memory
+constexpr int SM_PARTS = 32;     // of the vocabulary, whose sums lead to the token
+
 struct SampleShared {
-  unsigned bin[2][SM_BINS];        // low and high words
-  u64 entry[SM_LIST], weight[SM_LIST];
-  u64 part[SM_WARPS];
+  unsigned bin[2][SM_BINS];        // low and high words of sums; or numbers, and how many there are in front
+  u64 entry[SM_LIST], sorted[SM_LIST];
+  u64 part[SM_PARTS];
+  unsigned kept[2][SM_PARTS];
+  double power[16];                // 2^(i / 16) 2^bits
   unsigned lo, hi;
   int n, first;
   u64 cut, above, total;
   unsigned critical;
+  int b1;
 };
 
 __device__ __forceinline__ float sm_f(float x) { return x; }
 __device__ __forceinline__ float sm_f(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float sm_f(__half x) { return __half2float(x); }
+// The larger one; what is not a number before all others.
+__device__ __forceinline__ float sm_max(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 
-// Numbers in the order of the floats (zeros are one: -0 was made 0).
+// Numbers in the order of the floats (zeros are one).
 __device__ __forceinline__ unsigned sm_key(float x) {
-  const unsigned b = __float_as_uint(x);
+  const unsigned b = __float_as_uint(x + 0.f);
   return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
 }
 // An entry's place in the order by (x down, index up): the larger, the further in front.
@@ -88,6 +100,7 @@ __device__ __forceinline__ u64 sm_warp_before(u64 v) {
   return s - v;
 }
 // Whole CTA: the sum of the threads in front, and of all. `part` is free again behind the next barrier.
+template <int THREADS>
 __device__ __forceinline__ u64 sm_before(u64 v, u64* part, u64& all) {
   const u64 in_warp = sm_warp_before(v), last = __shfl_sync(0xffffffffu, in_warp + v, 31);
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = last;
@@ -95,135 +108,195 @@ __device__ __forceinline__ u64 sm_before(u64 v, u64* part, u64& all) {
   u64 before = 0;
   all = 0;
 #pragma unroll
-  for (int i = 0; i < SM_WARPS; ++i) {
+  for (int i = 0; i < THREADS / 32; ++i) {
     if (i < (int)(threadIdx.x >> 5)) before += part[i];
     all += part[i];
   }
   return before + in_warp;
 }
 
-template <typename T>
+template <typename T, int THREADS>
 struct SampleRow {
   static constexpr int VEC = 16 / sizeof(T);
-  static constexpr int TILE = SM_THREADS * VEC;    // a vector to a thread
-  static constexpr int AHEAD = sizeof(T) == 4 ? 4 : 2;         // vectors of a thread on their way together
   const T* x;
-  int V, off, tiles;             // vector 0 begins `off` entries in front of the row, on a 16-byte boundary
+  int V, head, vectors;          // whole vectors from entry `head` on, on 16-byte boundaries; the few entries around them are threads' own
   float m, per_bin;
-  double per_t;                  // log2(e) / T
-  double one;                    // 2^bits
+  double per16;                  // 16 log2(e) / T
+  float low, zero;               // entries from which on weights are 2^-48 of the largest, and nothing
+  const double* power;
+  const SampleParams& p;
 
-  __device__ __forceinline__ void vector(int i, float (&a)[VEC]) const {
-    const int v0 = i * VEC - off;
-    if (v0 >= 0 && v0 + VEC <= V) {
-      const uint4 in = __ldg(reinterpret_cast<const uint4*>(x + v0));
-      const T* have = reinterpret_cast<const T*>(&in);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) a[j] = sm_f(have[j]) + 0.f;
-    } else {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) a[j] = v0 + j >= 0 && v0 + j < V ? sm_f(x[v0 + j]) + 0.f : -INFINITY;
-    }
+  __device__ __forceinline__ SampleRow(const SampleParams& p_) : p(p_) {}
+
+  __device__ __forceinline__ void begin(const T* x_, int V_) {
+    x = x_;
+    V = V_;
+    head = min((int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) % 16 / sizeof(T)), V);
+    vectors = (V - head) / VEC;
   }
-  // f(entry, index) for all of them and, at the row's ends, for -inf at indices that are not there
+  __device__ __forceinline__ int edges() const { return V - vectors * VEC; }
+  __device__ __forceinline__ int edge(int i) const { return i < head ? i : i + vectors * VEC; }
+  // f(entries, index of the first): an array of VEC of them, or of one at the row's ends
   template <typename F>
-  __device__ __forceinline__ void each(F f) const {
+  __device__ __forceinline__ void one(int v, F f) const {
+    const float a[1] = {sm_f(x[v])};
+    f(a, v);
+  }
+  __device__ __forceinline__ uint4 raw(int i) const { return __ldg(reinterpret_cast<const uint4*>(x + head) + i); }
+  template <typename F>
+  __device__ __forceinline__ void vector(const uint4& in, int i, F f) const {
+    const T* have = reinterpret_cast<const T*>(&in);
+    float a[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) a[j] = sm_f(have[j]);
+    f(a, head + i * VEC);
+  }
+  // ... for vectors first, first + step .. below `end`, so many of a thread on their way together; of much work, the next one
+  template <int TOGETHER, typename F>
+  __device__ __forceinline__ void range(int first, int step, int end, F f) const {
+    if constexpr (TOGETHER == 1) {
+      uint4 next = make_uint4(0, 0, 0, 0);
+      if (first < end) next = raw(first);
 #pragma unroll 1
-    for (int t = 0; t < tiles; t += AHEAD) {
-      float a[AHEAD][VEC];
+      for (int i = first; i < end; i += step) {
+        const uint4 in = next;
+        if (i + step < end) next = raw(i + step);
+        vector(in, i, f);
+      }
+    } else {
+#pragma unroll 1
+      for (int i = first; i < end; i += TOGETHER * step) {
+        uint4 in[TOGETHER];
 #pragma unroll
-      for (int k = 0; k < AHEAD; ++k) vector((t + k) * SM_THREADS + threadIdx.x, a[k]);
+        for (int k = 0; k < TOGETHER; ++k)
+          if (i + k * step < end) in[k] = raw(i + k * step);
 #pragma unroll
-      for (int k = 0; k < AHEAD; ++k) {
-        const int v0 = ((t + k) * SM_THREADS + threadIdx.x) * VEC - off;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) f(a[k][j], v0 + j);
+        for (int k = 0; k < TOGETHER; ++k)
+          if (i + k * step < end) vector(in[k], i + k * step, f);
       }
     }
   }
-  __device__ __forceinline__ bool there(int v) const { return (unsigned)v < (unsigned)V; }
-  __device__ __forceinline__ int bin(float a) const { return min(SM_BINS - 1, __float2int_rz((m - a) * per_bin)); }
-  __device__ __forceinline__ double weight(float a) const { return exp2(((double)a - (double)m) * per_t); }
-  __device__ __forceinline__ u64 whole(double w) const {
-    const u64 n = __double2ull_rn(w * one);
-    return n == 0 && w > 0.0 ? 1 : n;
+  // ... for all entries
+  template <int TOGETHER, typename F>
+  __device__ __forceinline__ void each(F f) const {
+    range<TOGETHER>(threadIdx.x, THREADS, vectors, f);
+    if ((int)threadIdx.x < edges()) one(edge(threadIdx.x), f);
+  }
+  // bins of equal width, the further from the largest entry the higher
+  __device__ __forceinline__ int bin(float a) const {
+    const float t = fminf(fmaf(m - a, per_bin, 8388608.f), 8388608.f + (SM_BINS - 1));     // 2^23 + a whole number
+    return __float_as_uint(t) & (SM_BINS - 1);
+  }
+  // w 2^bits, w = 2^((a - m) log2(e) / T), of entries from `zero` on: sixteenths of the exponent from a table, what is left of it, at most 2^-5, by the series of
+  // the exponential function up to its fifth power (the sixth is 2^-42 of it), rounded up: what is above 0 counts as 1 at least. Without branches: a chain of
+  // a dozen operations of 64 bits is hidden by the other entries of a vector.
+  __device__ __forceinline__ u64 weight(float a) const {
+    constexpr double MAGIC = 6755399441055744.0;               // 1.5 2^52: what is added to it is a whole number in the low bits
+    const double t = ((double)fmaxf(a, low) - (double)m) * per16;          // (0 of the largest, whose weight is 2^bits)
+    const double n = t + MAGIC;
+    const int i = __double2loint(n);
+    const double r = t - (n - MAGIC);
+    const double e = fma(fma(fma(fma(fma(p.series[4], r, p.series[3]), r, p.series[2]), r, p.series[1]), r, p.series[0]), r, 1.0) * power[i & 15];
+    const double w = __dadd_ru(__hiloint2double(__double2hiint(e) + ((i & ~15) << 16), __double2loint(e)), 4503599627370496.0);       // 2^52
+    return __double_as_longlong(w) & 0xfffffffffffffull;
+  }
+  // The least entry with w >= p.
+  __device__ __forceinline__ float least(float p, float temperature) const {
+    return p > 0.f ? __double2float_ru((double)m + (double)temperature * log((double)p)) : -INFINITY;
   }
 };
 
-// Where the order ends: the last entry (see sm_entry) that stays of those from `from` on, by numbers (the first `share` ones) or by weights (up to a `share` of
-// their sum). `all_in_list`: by numbers, and the list has all entries from the first on, n of them, of which the first `share` are what stays.
-template <bool WEIGHTS, typename T>
-__device__ u64 sm_cut(const SampleRow<T>& row, SampleShared& s, u64 from, double share, bool& all_in_list) {
+// Where the order ends: the last entry (see sm_entry) that stays of those from `from` on (0: of all), by numbers (the first `share` ones) or by weights (up
+// to a `share` of their sum).
+template <bool WEIGHTS, typename T, int THREADS>
+__device__ u64 sm_cut(const SampleRow<T, THREADS>& row, SampleShared& s, u64 from, double share) {
+  constexpr int LIST = 256;                        // each of these is compared with all others
   const int tid = threadIdx.x;
-  all_in_list = false;
   unsigned lo = 0, hi = 0xffffffffu;               // keys that are looked at
   int bin0 = -1;                                   // and, behind the first level, the bin
   unsigned top = 0;
   int shift = 0;
   u64 above = 0;
   double target = share;
+  // what an earlier choice has left out, or has no weight
+  const float from_value = fmaxf(from ? sm_value(from) : -INFINITY, WEIGHTS ? row.zero : -INFINITY);
+  const int from_index = from && sm_value(from) == from_value ? sm_index(from) : 0x7fffffff;
+  auto behind = [&](float a, int v) { return a <= from_value && (a < from_value || v > from_index); };
   auto looked_at = [&](float a, int v) {
-    if (!row.there(v) || sm_entry(a, v) < from) return false;
-    if (bin0 < 0) return true;
     const unsigned k = sm_key(a);
-    return row.bin(a) == bin0 && k >= lo && k <= hi;
+    return !behind(a, v) && row.bin(a) == bin0 && k >= lo && k <= hi;
   };
   while (true) {
     // ---- the bins
-    for (int i = tid; i < 2 * SM_BINS; i += SM_THREADS) s.bin[0][i] = 0;
+    for (int i = tid; i < 2 * SM_BINS; i += THREADS) s.bin[0][i] = 0;
     if (tid == 0) s.n = 0;
     __syncthreads();
-    row.each([&](float a, int v) {
-      if (!looked_at(a, v)) return;
-      const unsigned b = bin0 < 0 ? row.bin(a) : (top - sm_key(a)) >> shift;
-      if (!WEIGHTS) {
-        atomicAdd(&s.bin[0][b], 1u);
-      } else {
-        const u64 w = row.whole(row.weight(a));
-        const unsigned low = (unsigned)w, old = atomicAdd(&s.bin[0][b], low), high = (unsigned)(w >> 32) + (old + low < old);
-        if (high) atomicAdd(&s.bin[1][b], high);
-      }
-    });
+    auto count = [&](unsigned b, u64 w) {
+      const unsigned low = (unsigned)w, old = atomicAdd(&s.bin[0][b], low), high = (unsigned)(w >> 32) + (old + low < old);
+      if (high) atomicAdd(&s.bin[1][b], high);
+    };
+    if (bin0 < 0) {
+      row.template each<WEIGHTS ? 1 : 2>([&](auto& a, int v0) {
+        constexpr int N = sizeof(a) / sizeof(float);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const unsigned b = row.bin(a[j]);
+          if constexpr (WEIGHTS) {
+            const u64 w = row.weight(a[j]);
+            if (!behind(a[j], v0 + j)) count(b, w);
+          } else {
+            if (b < SM_BINS - 1) atomicAdd(&s.bin[0][b], 1u);              // (those in the last bin are what is left)
+          }
+        }
+      });
+    } else {
+      row.template each<1>([&](auto& a, int v0) {
+#pragma unroll
+        for (int j = 0; j < (int)(sizeof(a) / sizeof(float)); ++j)
+          if (looked_at(a[j], v0 + j)) count((top - sm_key(a[j])) >> shift, WEIGHTS ? row.weight(a[j]) : 1);
+      });
+    }
     __syncthreads();
-    constexpr int OWN = SM_BINS / SM_THREADS;
+    constexpr int OWN = SM_BINS / THREADS;
     u64 own[OWN], sum = 0, total;
 #pragma unroll
     for (int i = 0; i < OWN; ++i) sum += own[i] = (u64)s.bin[1][tid * OWN + i] << 32 | s.bin[0][tid * OWN + i];
-    u64 before = sm_before(sum, s.part, total) + above;
+    u64 before = sm_before<THREADS>(sum, s.part, total) + above;
+    if (!WEIGHTS && bin0 < 0 && tid == THREADS - 1) own[OWN - 1] = row.V - total;
     if (WEIGHTS && bin0 < 0) target = share * (double)total;
 #pragma unroll
     for (int i = 0; i < OWN; ++i) {
       if ((double)before < target && (double)(before + own[i]) >= target) {
         s.critical = tid * OWN + i;
         s.above = before;
-        s.total = before + own[i];
       }
       before += own[i];
     }
     __syncthreads();
     const unsigned b = s.critical;
-    const u64 up_to = s.total;
     above = s.above;
-    // ---- its entries, or all up to it
-    all_in_list = !WEIGHTS && bin0 < 0 && up_to <= SM_LIST;
+    // ---- its entries
     if (bin0 < 0) {
       bin0 = (int)b;
     } else {
       hi = top - (b << shift);
       lo = hi - ((1u << shift) - 1);
     }
-    row.each([&](float a, int v) {
-      if (all_in_list ? row.there(v) && row.bin(a) <= bin0 : looked_at(a, v)) {
-        const int at = atomicAdd(&s.n, 1);
-        if (at < SM_LIST) s.entry[at] = sm_entry(a, v);
+    row.template each<2>([&](auto& a, int v0) {
+#pragma unroll
+      for (int j = 0; j < (int)(sizeof(a) / sizeof(float)); ++j) {
+        const int bin = row.bin(a[j]);
+        if (bin == bin0 && looked_at(a[j], v0 + j)) {
+          const int at = atomicAdd(&s.n, 1);
+          if (at < LIST) s.entry[at] = sm_entry(a[j], v0 + j);
+        }
       }
     });
     __syncthreads();
     const int n = s.n;
-    if (n <= SM_LIST) {
-      if (all_in_list) return 0;
+    if (n <= LIST) {
       if (WEIGHTS) {
-        if (tid < n) s.weight[tid] = row.whole(row.weight(sm_value(s.entry[tid])));
+        if (tid < n) s.sorted[tid] = row.weight(sm_value(s.entry[tid]));
         __syncthreads();
       }
       if (tid < n) {
@@ -231,8 +304,8 @@ __device__ u64 sm_cut(const SampleRow<T>& row, SampleShared& s, u64 from, double
         u64 front = above;
 #pragma unroll 4
         for (int j = 0; j < n; ++j)
-          if (s.entry[j] > e) front += WEIGHTS ? s.weight[j] : 1;
-        if ((double)front < target && (double)(front + (WEIGHTS ? s.weight[tid] : 1)) >= target) s.cut = e;
+          if (s.entry[j] > e) front += WEIGHTS ? s.sorted[j] : 1;
+        if ((double)front < target && (double)(front + (WEIGHTS ? s.sorted[tid] : 1)) >= target) s.cut = e;
       }
       __syncthreads();
       return s.cut;
@@ -244,10 +317,13 @@ __device__ u64 sm_cut(const SampleRow<T>& row, SampleShared& s, u64 from, double
     }
     __syncthreads();
     unsigned least = 0xffffffffu, most = 0;
-    row.each([&](float a, int v) {
-      if (!looked_at(a, v)) return;
-      least = min(least, sm_key(a));
-      most = max(most, sm_key(a));
+    row.template each<2>([&](auto& a, int v0) {
+#pragma unroll
+      for (int j = 0; j < (int)(sizeof(a) / sizeof(float)); ++j) {
+        if (!looked_at(a[j], v0 + j)) continue;
+        least = min(least, sm_key(a[j]));
+        most = max(most, sm_key(a[j]));
+      }
     });
     least = __reduce_min_sync(0xffffffffu, least);
     most = __reduce_max_sync(0xffffffffu, most);
@@ -263,38 +339,110 @@ __device__ u64 sm_cut(const SampleRow<T>& row, SampleShared& s, u64 from, double
     __syncthreads();
   }
   // ---- equal entries: as many of them as it takes, in the order of the vocabulary
-  const u64 w = WEIGHTS ? row.whole(row.weight(sm_value((u64)hi << 32))) : 1;
-  u64 take = (u64)fmax(1.0, ceil((target - (double)above) / (double)w));
-  while (take > 1 && (double)(above + (take - 1) * w) >= target) --take;
-  while ((double)(above + take * w) < target) ++take;
+  const float value = sm_value((u64)hi << 32);
+  const u64 each = WEIGHTS ? row.weight(value) : 1;
+  u64 take = (u64)fmax(1.0, ceil((target - (double)above) / (double)each));
+  while (take > 1 && (double)(above + (take - 1) * each) >= target) --take;
+  while ((double)(above + take * each) < target) ++take;
+  // those in front of the vectors, then a vector to a thread at a time, then those behind
   u64 seen = 0;
-  for (int t = 0; t < row.tiles; ++t) {            // a tile's entries stand in the threads' order
-    float a[SampleRow<T>::VEC];
-    const int v0 = (t * SM_THREADS + tid) * SampleRow<T>::VEC - row.off;
-    row.vector(t * SM_THREADS + tid, a);
+  const int rounds = (row.vectors + THREADS - 1) / THREADS;
+  for (int t = -1; t <= rounds && seen < take; ++t) {
     unsigned hit = 0;
+    int first = 0;
+    auto look = [&](auto& a, int v0) {
+      first = v0;
 #pragma unroll
-    for (int j = 0; j < SampleRow<T>::VEC; ++j)
-      if (row.there(v0 + j) && sm_entry(a[j], v0 + j) >= from && sm_key(a[j]) == hi) hit |= 1u << j;
-    u64 all, before = seen + sm_before(__popc(hit), s.part, all);
-#pragma unroll
-    for (int j = 0; j < SampleRow<T>::VEC; ++j)
-      if (hit >> j & 1 && ++before == take) s.cut = sm_entry(a[j], v0 + j);
+      for (int j = 0; j < (int)(sizeof(a) / sizeof(float)); ++j)
+        if (a[j] == value && !behind(a[j], v0 + j)) hit |= 1u << j;
+    };
+    if (t < 0) {
+      if (tid < row.head) row.one(tid, look);
+    } else if (t == rounds) {
+      if (row.head + tid < row.edges()) row.one(row.edge(row.head + tid), look);
+    } else if (t * THREADS + tid < row.vectors) {
+      row.vector(row.raw(t * THREADS + tid), t * THREADS + tid, look);
+    }
+    u64 all, before = seen + sm_before<THREADS>(__popc(hit), s.part, all);
+    for (; hit; hit &= hit - 1)
+      if (++before == take) s.cut = sm_entry(value, first + __ffs(hit) - 1);
     seen += all;
     __syncthreads();
-    if (seen >= take) break;
   }
   return s.cut;
 }
 
+// Whole warp: the part of the vocabulary that holds u of the sum of all parts, that number, and the sums in front of the part.
+struct SamplePart {
+  int part;
+  u64 target, front;
+  __device__ __forceinline__ SamplePart(const SampleShared& s, float u) {
+    const int lane = threadIdx.x & 31;
+    const u64 own = (u64)s.kept[1][lane] << 32 | s.kept[0][lane], before = sm_warp_before(own);
+    target = (u64)((double)u * (double)__shfl_sync(0xffffffffu, before + own, 31));
+    part = __ffs(__ballot_sync(0xffffffffu, before <= target && target < before + own)) - 1;
+    front = __shfl_sync(0xffffffffu, before, part);
+  }
+};
+static_assert(SM_PARTS == 32, "a lane has a part");
+
+// Numbers of entries in every bin, and of those in front; the last bin, which reaches to the least entry, is not counted.
+template <typename T, int THREADS>
+__device__ void sm_count(const SampleRow<T, THREADS>& row, SampleShared& s) {
+  constexpr int OWN = SM_BINS / THREADS;
+  const int tid = threadIdx.x;
+  for (int i = tid; i < SM_BINS; i += THREADS) s.bin[0][i] = 0;
+  __syncthreads();
+  row.template each<2>([&](auto& a, int) {
+#pragma unroll
+    for (int j = 0; j < (int)(sizeof(a) / sizeof(float)); ++j) {
+      const int b = row.bin(a[j]);
+      if (b < SM_BINS - 1) atomicAdd(&s.bin[0][b], 1u);
+    }
+  });
+  __syncthreads();
+  unsigned own[OWN], sum = 0;
+#pragma unroll
+  for (int i = 0; i < OWN; ++i) sum += own[i] = s.bin[0][tid * OWN + i];
+  u64 all;
+  unsigned before = (unsigned)sm_before<THREADS>(sum, s.part, all);
+#pragma unroll
+  for (int i = 0; i < OWN; ++i) {
+    s.bin[1][tid * OWN + i] = before;
+    before += own[i];
+  }
+  __syncthreads();
+}
+
+// An entry of bins b0 .. b1, which have at most SM_LIST, into the list behind those of the bins in front.
+template <typename T, int THREADS>
+__device__ __forceinline__ void sm_keep(const SampleRow<T, THREADS>& row, SampleShared& s, float a, int v, int bin, int b0) {
+  s.entry[s.bin[1][bin] - s.bin[1][b0] + atomicSub(&s.bin[0][bin], 1u) - 1] = sm_entry(a, v);
+}
+// Whole CTA: the list's n entries, from bin b0 on, in their order: an entry is compared with those of its bin.
+template <typename T, int THREADS>
+__device__ void sm_sort(const SampleRow<T, THREADS>& row, SampleShared& s, int n, int b0) {
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += THREADS) {
+    const u64 e = s.entry[i];
+    const int b = row.bin(sm_value(e)), first = s.bin[1][b] - s.bin[1][b0], end = min(n, (int)(s.bin[1][b + 1] - s.bin[1][b0]));
+    int rank = first;
+    for (int j = first; j < end; ++j) rank += s.entry[j] > e;
+    s.sorted[rank] = e;
+  }
+  __syncthreads();
+}
+
 // Whole CTA: the smallest index for which `f(entry)`; -1 where there is none.
-template <typename T, typename F>
-__device__ int sm_first(const SampleRow<T>& row, SampleShared& s, F f) {
+template <typename T, int THREADS, typename F>
+__device__ int sm_first(const SampleRow<T, THREADS>& row, SampleShared& s, F f) {
   if (threadIdx.x == 0) s.first = 0x7fffffff;
   __syncthreads();
   int best = 0x7fffffff;
-  row.each([&](float a, int v) {
-    if (row.there(v) && f(a)) best = min(best, v);
+  row.template each<2>([&](auto& a, int v0) {
+#pragma unroll
+    for (int j = 0; j < (int)(sizeof(a) / sizeof(float)); ++j)
+      if (f(a[j])) best = min(best, v0 + j);
   });
   best = __reduce_min_sync(0xffffffffu, best);
   if ((threadIdx.x & 31) == 0) atomicMin(&s.first, best);
@@ -302,171 +450,314 @@ __device__ int sm_first(const SampleRow<T>& row, SampleShared& s, F f) {
   return s.first == 0x7fffffff ? -1 : s.first;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(const __grid_constant__ SampleParams p) {
-  extern __shared__ __align__(16) uint8_t raw[];
-  SampleShared& s = *reinterpret_cast<SampleShared*>(raw);
-  u64* pieces = reinterpret_cast<u64*>(raw + sizeof(SampleShared));          // [tiles][warps]
-  using Row = SampleRow<T>;
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const __grid_constant__ SampleParams p) {
+  constexpr int WARPS = THREADS / 32;
+  using Row = SampleRow<T, THREADS>;
+  __shared__ SampleShared s;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const long long b = blockIdx.x;
-  Row row;
-  row.x = (const T*)p.x + b * p.ldx;
-  row.V = p.V;
-  row.off = (int)((reinterpret_cast<uintptr_t>(row.x) & 15) / sizeof(T));
-  row.tiles = (p.V + row.off + Row::TILE - 1) / Row::TILE;
+  Row row(p);
+  row.begin((const T*)p.x + b * p.ldx, p.V);
   const float temperature = p.temperature ? p.temperature[b] : p.temperature0;
   const float top_p = p.top_p ? p.top_p[b] : p.top_p0;
   const float min_p = fminf(p.min_p ? p.min_p[b] : p.min_p0, 1.f);
   const int top_k = p.top_k ? p.top_k[b] : p.top_k0;
   const float u = fminf(fmaxf(p.u[b], 0.f), 0x1.fffffep-1f);
+  if (tid < 16) s.power[tid] = exp2(tid / 16.0) * (double)(1ull << p.bits);
 
-  // ---- the largest entry, and the mean of those that are numbers
+  // ---- the largest entry, and the mean of some that are numbers
   float most = -INFINITY, sum = 0.f;
-  int numbers = 0, none = 0;
-  row.each([&](float a, int v) {
-    none |= a != a;
-    most = fmaxf(most, a);
-    const bool number = fabsf(a) < 0x1p100f;
-    sum += number ? a : 0.f;
-    numbers += number;
+  int numbers = 0;
+  row.template each<4>([&](auto& a, int) {
+#pragma unroll
+    for (int j = 0; j < (int)(sizeof(a) / sizeof(float)); ++j) most = sm_max(most, a[j]);
+  });
+  if (tid < row.vectors) row.vector(row.raw(tid), tid, [&](auto& a, int) {
+#pragma unroll
+    for (int j = 0; j < (int)(sizeof(a) / sizeof(float)); ++j) {
+      const bool number = fabsf(a[j]) < 0x1p100f;
+      sum += number ? a[j] : 0.f;
+      numbers += number;
+    }
   });
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
-    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    most = sm_max(most, __shfl_xor_sync(0xffffffffu, most, o));
     sum += __shfl_xor_sync(0xffffffffu, sum, o);
   }
   numbers = __reduce_add_sync(0xffffffffu, numbers);
-  none = __any_sync(0xffffffffu, none);
   float* f = reinterpret_cast<float*>(s.entry);
-  int* n = reinterpret_cast<int*>(s.weight);
+  int* n = reinterpret_cast<int*>(s.sorted);
   if (lane == 0) {
     f[warp] = most;
-    f[SM_WARPS + warp] = sum;
+    f[WARPS + warp] = sum;
     n[warp] = numbers;
-    n[SM_WARPS + warp] = none;
   }
   __syncthreads();
-  most = -INFINITY, sum = 0.f, numbers = none = 0;
+  most = -INFINITY, sum = 0.f, numbers = 0;
 #pragma unroll
-  for (int i = 0; i < SM_WARPS; ++i) {
-    most = fmaxf(most, f[i]);
-    sum += f[SM_WARPS + i];
+  for (int i = 0; i < WARPS; ++i) {
+    most = sm_max(most, f[i]);
+    sum += f[WARPS + i];
     numbers += n[i];
-    none |= n[SM_WARPS + i];
   }
   // ---- rows without probabilities, and those whose likeliest entry is asked for
-  if (none || !(temperature > 0.f) || top_k == 1 || top_p <= 0.f || fabsf(most) == INFINITY) {
-    const int v = none                ? sm_first(row, s, [](float a) { return a != a; })
-                  : most == -INFINITY ? -1
-                                      : sm_first(row, s, [&](float a) { return a == most; });
+  if (!(fabsf(most) < INFINITY) || !(temperature > 0.f) || top_k == 1 || top_p <= 0.f) {
+    const bool none = most != most;
+    const int v = most == -INFINITY ? -1 : sm_first(row, s, [&](float a) { return none ? a != a : a == most; });
     if (tid == 0) p.out[b] = v;
     return;
   }
   row.m = most;
-  row.per_t = 1.4426950408889634 / (double)temperature;
-  row.one = (double)(1ull << p.bits);
-  // bins that reach twice as far as the mean; what is further away lies in the last
-  const float reach = 2.f * (most - sum / (float)max(numbers, 1));
-  row.per_bin = reach > 0x1p-60f && reach < 0x1p100f ? (float)SM_BINS / reach : 1.f;
+  row.per16 = 16.0 * 1.4426950408889634 / (double)temperature;
+  row.low = most - 33.271065f * temperature;       // 48 log(2)
+  row.zero = most - 744.44009f * temperature;      // 1074 log(2)
+  row.power = s.power;
+  // Bins of numbers reach three quarters of the way to the mean, which some of the first entries stand for; those of weights twice as far. What is further away lies in
+  // the last.
+  const float reach = most - sum / (float)max(numbers, 1);
+  const float per = reach > 0x1p-60f && reach < 0x1p100f ? (float)(SM_BINS - 1) / reach : 1.f;
   __syncthreads();
 
   u64 cut = 0;
-  bool all_in_list;
+  const int per_part = (row.vectors + SM_PARTS - 1) / SM_PARTS;          // vectors; what is in front of them is the first part's, what is behind the last one's
+  auto part_of = [&](int v) {
+    const int i = (v - row.head) / Row::VEC;
+    return v < row.head ? 0 : i >= row.vectors ? SM_PARTS - 1 : (int)((unsigned)i / (unsigned)per_part);
+  };
+  const float least_p = row.least(min_p, temperature);
   if (top_k > 0 && top_k < p.V) {
-    cut = sm_cut<false>(row, s, 0, (double)top_k, all_in_list);
-    if (all_in_list) {                             // the rest among these entries: a thread has one
-      const int n = s.n;
-      const u64 e = tid < n ? s.entry[tid] : 0;
-      int rank = 0;
-      if (tid < n) {
-#pragma unroll 4
-        for (int j = 0; j < n; ++j) rank += s.entry[j] > e;
+    row.per_bin = per * (4.f / 3.f);
+    sm_count(row, s);
+    // ---- the bin that the k-th entry lies in
+    for (int i = tid; i < SM_BINS - 1; i += THREADS)
+      if (s.bin[1][i] < (unsigned)top_k && s.bin[1][i + 1] >= (unsigned)top_k) s.b1 = i;
+    if (tid < SM_PARTS) s.kept[0][tid] = s.kept[1][tid] = 0;
+    if (tid == 0 && s.bin[1][SM_BINS - 1] < (unsigned)top_k) s.b1 = SM_BINS - 1;
+    __syncthreads();
+    const int b1 = s.b1, n = b1 < SM_BINS - 1 ? (int)s.bin[1][b1 + 1] : SM_LIST + 1;
+    if (n <= SM_LIST) {
+      // ---- all of them into the list; the rest happens there
+      row.template each<2>([&](auto& a, int v0) {
+#pragma unroll
+        for (int j = 0; j < (int)(sizeof(a) / sizeof(float)); ++j) {
+          const int bin = row.bin(a[j]);
+          if (bin <= b1) sm_keep(row, s, a[j], v0 + j, bin, 0);
+        }
+      });
+      sm_sort(row, s, n, 0);
+      constexpr int OWN = SM_LIST / THREADS;       // a thread's entries, next to each other
+      u64 e[OWN], w[OWN], sum = 0, total;
+#pragma unroll
+      for (int i = 0; i < OWN; ++i) {
+        const int at = tid * OWN + i;
+        e[i] = at < top_k && at < n ? s.sorted[at] : 0;
+        w[i] = e[i] && sm_value(e[i]) >= row.zero ? row.weight(sm_value(e[i])) : 0;
+        sum += w[i];
       }
-      const double w = tid < n && rank < top_k ? row.weight(sm_value(e)) : 0.0;
-      const u64 mine = w > 0.0 ? row.whole(w) : 0;
-      if (tid < n) s.weight[tid] = mine;
-      u64 total;
-      sm_before(mine, s.part, total);              // (its barrier is the one behind the weights too)
-      u64 front = 0;
-      if (top_p < 1.f && tid < n) {
-#pragma unroll 4
-        for (int j = 0; j < n; ++j) front += s.entry[j] > e ? s.weight[j] : 0;
+      u64 before = sm_before<THREADS>(sum, s.part, total);
+      const double target = (double)top_p * (double)total;
+#pragma unroll
+      for (int i = 0; i < OWN; ++i) {
+        const u64 front = before;
+        before += w[i];
+        if (w[i] == 0) continue;
+        if ((top_p < 1.f && !((double)front < target)) || sm_value(e[i]) < least_p) {
+          w[i] = 0;
+          continue;
+        }
+        const int part = part_of(sm_index(e[i]));
+        const unsigned low = (unsigned)w[i], old = atomicAdd(&s.kept[0][part], low), high = (unsigned)(w[i] >> 32) + (old + low < old);
+        if (high) atomicAdd(&s.kept[1][part], high);
       }
-      const u64 stays = (!(top_p < 1.f) || (double)front < (double)top_p * (double)total) && !(w < (double)min_p) ? mine : 0;
+      if (tid == 0) s.n = 0;
       __syncthreads();
-      if (tid < n) s.weight[tid] = stays;
-      sm_before(stays, s.part, total);
-      if (stays) {
-        const u64 target = (u64)((double)u * (double)total);
-        u64 before = 0;
-#pragma unroll 4
-        for (int j = 0; j < n; ++j) before += (unsigned)s.entry[j] > (unsigned)e ? s.weight[j] : 0;      // of smaller indices
-        if (before <= target && target < before + stays) p.out[b] = sm_index(e);
+      const SamplePart at(s, u);
+      // ---- the part's own: each is compared with all of them
+#pragma unroll
+      for (int i = 0; i < OWN; ++i) {
+        if (w[i] == 0 || part_of(sm_index(e[i])) != at.part) continue;
+        const int to = atomicAdd(&s.n, 1);
+        s.entry[to] = e[i];
+        s.sorted[to] = w[i];
+      }
+      __syncthreads();
+      for (int i = tid; i < s.n; i += THREADS) {
+        const int v = sm_index(s.entry[i]);
+        u64 front = at.front;
+        for (int j = 0; j < s.n; ++j) front += sm_index(s.entry[j]) < v ? s.sorted[j] : 0;
+        if (front <= at.target && at.target < front + s.sorted[i]) p.out[b] = v;
       }
       return;
     }
+    cut = sm_cut<false>(row, s, 0, (double)top_k);
     __syncthreads();
   }
+  u64 mine = 0;                                    // of this warp's part
+  bool summed = false;
   if (top_p < 1.f) {
-    cut = sm_cut<true>(row, s, cut, (double)top_p, all_in_list);
+    row.per_bin = per * 0.5f;
+    if (cut == 0) {
+      // ---- by the bins' numbers and middles, about where the share ends
+      sm_count(row, s);
+      constexpr int OWN = SM_BINS / THREADS;
+      float own[OWN], sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < OWN; ++i) {
+        const int at = tid * OWN + i;
+        const float middle = row.m - at / row.per_bin;
+        own[i] = at < SM_BINS - 1 ? (float)(s.bin[1][at + 1] - s.bin[1][at]) * exp2f((middle - row.m) * (float)(row.per16 / 16.0)) : 0.f;
+        sum += own[i];
+      }
+      // (as whole numbers, of which the scan is)
+      u64 all, before = sm_before<THREADS>((u64)(sum * 0x1p20f), s.part, all);
+      const u64 target = (u64)((double)top_p * (double)all);
+      if (tid == 0) s.critical = 0;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < OWN; ++i) {
+        const u64 upto = before + (u64)(own[i] * 0x1p20f);
+        if (before <= target && target < upto) s.critical = tid * OWN + i;
+        before = upto;
+      }
+      __syncthreads();
+      // as many of them around it as there is room for, 31 on both sides at most (it is hardly ever that far off)
+      const int about = min((int)s.critical, SM_BINS - 2), b0_ = max(about - lane, 0), b1_ = min(about + lane, SM_BINS - 2);
+      const unsigned fits = __ballot_sync(0xffffffffu, s.bin[1][b1_ + 1] - s.bin[1][b0_] <= SM_LIST);
+      const int wide = 31 - __clz(fits), b0 = max(about - wide, 0), b1 = fits ? min(about + wide, SM_BINS - 2) : -1;
+      if (b1 >= 0) {
+        // ---- all weights, those in front of the list, those of each part; the list
+        const int n = (int)(s.bin[1][b1 + 1] - s.bin[1][b0]);
+        u64 everything = 0, in_front = 0;
+        auto take = [&](auto& a, int v0) {
+#pragma unroll 4
+          for (int j = 0; j < (int)(sizeof(a) / sizeof(float)); ++j) {
+            const u64 w = row.weight(a[j]);
+            const int bin = row.bin(a[j]);
+            if (a[j] >= row.zero) everything += w;
+            if (bin < b0) {
+              in_front += w;
+              if (a[j] >= least_p) mine += w;
+            } else if (bin <= b1) {
+              sm_keep(row, s, a[j], v0 + j, bin, b0);
+            }
+          }
+        };
+        for (int part = warp; part < SM_PARTS; part += WARPS) {
+          mine = 0;
+          row.template range<1>(part * per_part + lane, 32, min((part + 1) * per_part, row.vectors), take);
+          if (part == 0 && lane < row.head) row.one(lane, take);
+          if (part == SM_PARTS - 1 && row.head + lane < row.edges()) row.one(row.edge(row.head + lane), take);
+          mine = sm_warp_sum(mine);
+          if (lane == 0) {
+            s.kept[0][part] = (unsigned)mine;
+            s.kept[1][part] = (unsigned)(mine >> 32);
+          }
+        }
+        u64 total, front;
+        sm_before<THREADS>(everything, s.part, total);
+        __syncthreads();
+        sm_before<THREADS>(in_front, s.part, front);
+        sm_sort(row, s, n, b0);
+        // ---- the entry of the list at which the share ends
+        constexpr int OWN_LIST = SM_LIST / THREADS;
+        u64 w[OWN_LIST], sum = 0, list;
+#pragma unroll
+        for (int i = 0; i < OWN_LIST; ++i) {
+          const int at = tid * OWN_LIST + i;
+          w[i] = at < n && sm_value(s.sorted[at]) >= row.zero ? row.weight(sm_value(s.sorted[at])) : 0;
+          sum += w[i];
+        }
+        u64 before = front + sm_before<THREADS>(sum, s.part, list);
+        const double share = (double)top_p * (double)total;
+        if ((double)front < share && (double)(front + list) >= share) {      // else it lies elsewhere, and is looked for in another way
+#pragma unroll
+          for (int i = 0; i < OWN_LIST; ++i) {
+            if (w[i] && (double)before < share) {
+              const u64 e = s.sorted[tid * OWN_LIST + i];
+              if ((double)(before + w[i]) >= share) s.cut = e;
+              if (sm_value(e) >= least_p) {
+                const int part = part_of(sm_index(e));
+                const unsigned low = (unsigned)w[i], old = atomicAdd(&s.kept[0][part], low), high = (unsigned)(w[i] >> 32) + (old + low < old);
+                if (high) atomicAdd(&s.kept[1][part], high);
+              }
+            }
+            before += w[i];
+          }
+          summed = true;
+        }
+        __syncthreads();
+        if (summed) cut = s.cut;
+      }
+    }
+    if (!summed) {
+      cut = sm_cut<true>(row, s, cut, (double)top_p);
+      __syncthreads();
+    }
+  }
+  // ---- sums of what stays, of every part
+  const float cut_value = cut ? sm_value(cut) : -INFINITY, least = fmaxf(fmaxf(cut_value, row.zero), least_p);
+  const int cut_index = cut && cut_value == least ? sm_index(cut) : 0x7fffffff;             // of entries as large as the last one, the last that stays
+  const float next = sm_value((u64)(sm_key(least) + 1) << 32);
+  auto from = [&](int v) { return v > cut_index ? next : least; };         // the least that stays
+  auto add = [&](auto& a, int v0) {
+    constexpr int N = sizeof(a) / sizeof(float);
+    float largest = a[0];
+#pragma unroll
+    for (int j = 1; j < N; ++j) largest = fmaxf(largest, a[j]);
+    if (largest < least) return;
+#pragma unroll 4
+    for (int j = 0; j < N; ++j) {
+      const u64 w = row.weight(a[j]);
+      if (a[j] >= from(v0 + j)) mine += w;
+    }
+  };
+  if (!summed) {
+    for (int part = warp; part < SM_PARTS; part += WARPS) {
+      mine = 0;
+      row.template range<1>(part * per_part + lane, 32, min((part + 1) * per_part, row.vectors), add);
+      if (part == 0 && lane < row.head) row.one(lane, add);
+      if (part == SM_PARTS - 1 && row.head + lane < row.edges()) row.one(row.edge(row.head + lane), add);
+      mine = sm_warp_sum(mine);
+      if (lane == 0) {
+        s.kept[0][part] = (unsigned)mine;
+        s.kept[1][part] = (unsigned)(mine >> 32);
+      }
+    }
     __syncthreads();
   }
-  // ---- sums of what stays, of every warp's vectors of a tile
-  auto stays = [&](float a, int v) -> u64 {
-    if (!row.there(v) || sm_entry(a, v) < cut) return 0;
-    const double w = row.weight(a);
-    return w < (double)min_p ? 0 : row.whole(w);
+  const SamplePart here(s, u);
+  // ---- the part in which u lies, cut among all threads: vectors next to each other, the first thread with those in front of all vectors, the last with those
+  // behind
+  const int part = here.part, first = part * per_part, end = max(first, min(first + per_part, row.vectors)), own = (end - first + THREADS - 1) / THREADS;
+  const int i0 = min(first + tid * own, end), i1 = min(i0 + own, end);
+  auto walk = [&](auto f) {
+    if (part == 0 && tid == 0)
+      for (int v = 0; v < row.head; ++v) row.one(v, f);
+    for (int i = i0; i < i1; ++i) row.vector(row.raw(i), i, f);
+    if (part == SM_PARTS - 1 && tid == THREADS - 1)
+      for (int i = row.head; i < row.edges(); ++i) row.one(row.edge(i), f);
   };
+  mine = 0;
+  walk(add);
+  u64 all, before = here.front + sm_before<THREADS>(mine, s.part, all);
+  if (before <= here.target && here.target < before + mine)
+    walk([&](auto& a, int v0) {
 #pragma unroll 1
-  for (int t = 0; t < row.tiles; ++t) {
-    float a[Row::VEC];
-    row.vector(t * SM_THREADS + tid, a);
-    u64 w = 0;
-#pragma unroll
-    for (int j = 0; j < Row::VEC; ++j) w += stays(a[j], (t * SM_THREADS + tid) * Row::VEC - row.off + j);
-    w = sm_warp_sum(w);
-    if (lane == 0) pieces[t * SM_WARPS + warp] = w;
-  }
-  __syncthreads();
-  // ---- the piece in which u lies: a thread has some of them
-  const int count = row.tiles * SM_WARPS, own = (count + SM_THREADS - 1) / SM_THREADS;
-  u64 mine = 0, total;
-  for (int i = 0; i < own; ++i) mine += tid * own + i < count ? pieces[tid * own + i] : 0;
-  u64 before = sm_before(mine, s.part, total);
-  const u64 target = (u64)((double)u * (double)total);
-  for (int i = 0; i < own && tid * own + i < count; ++i) {
-    const u64 w = pieces[tid * own + i];
-    if (before <= target && target < before + w) {
-      s.first = tid * own + i;
-      s.above = before;
-    }
-    before += w;
-  }
-  __syncthreads();
-  if (warp == 0) {
-    float a[Row::VEC];
-    const int i = s.first * 32 + lane;             // vectors of a tile stand in the threads' order
-    row.vector(i, a);
-    u64 w[Row::VEC], all = 0;
-#pragma unroll
-    for (int j = 0; j < Row::VEC; ++j) all += w[j] = stays(a[j], i * Row::VEC - row.off + j);
-    u64 at = s.above + sm_warp_before(all);
-#pragma unroll
-    for (int j = 0; j < Row::VEC; ++j) {
-      if (at <= target && target < at + w[j]) p.out[b] = i * Row::VEC - row.off + j;
-      at += w[j];
-    }
-  }
+      for (int j = 0; j < (int)(sizeof(a) / sizeof(float)); ++j) {
+        const u64 x = a[j] >= from(v0 + j) ? row.weight(a[j]) : 0;
+        if (before <= here.target && here.target < before + x) p.out[b] = v0 + j;
+        before += x;
+      }
+    });
 }
 
 template <typename T>
 static int launch_sample(const SampleParams& p, long long B, cudaStream_t st) {
-  constexpr int TILE = SampleRow<T>::TILE;
-  const size_t smem = sizeof(SampleShared) + (size_t)((p.V + 16 + TILE - 1) / TILE) * SM_WARPS * sizeof(u64);
-  static gf::SharedLimit limit;
-  if (smem > 48 * 1024 && !limit.raise(sample_kernel<T>, smem)) return GFH_CUDA;
-  sample_kernel<T><<<(unsigned)B, SM_THREADS, smem, st>>>(p);
+  // one CTA to an SM where there are no more rows
+  if (B <= sm_count()) sample_kernel<T, 1024><<<(unsigned)B, 1024, 0, st>>>(p);
+  else sample_kernel<T, 512><<<(unsigned)B, 512, 0, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? GFH_OK : GFH_CUDA;
 }
 
@@ -479,8 +770,9 @@ GF_API int gf_sample_tokens(const SampleCall* c, void* stream) {
   gf::enter();
   int bits = 62;                                   // sums of V weights are below 2^62
   while (bits > 46 || (c->V >> (62 - bits)) > 0) --bits;
+  constexpr double C1 = 0.69314718055994530942 / 16;
   const SampleParams p{c->x, c->ldx, c->u, c->temperature, c->top_p, c->min_p, c->top_k, (float)c->temperature0, (float)c->top_p0, (float)c->min_p0,
-                       (int)c->top_k0, c->out, (int)c->V, bits};
+                       (int)c->top_k0, c->out, (int)c->V, bits, {C1, C1 * C1 / 2, C1 * C1 * C1 / 6, C1 * C1 * C1 * C1 / 24, C1 * C1 * C1 * C1 * C1 / 120}};
   cudaStream_t st = (cudaStream_t)stream;
   return c->dtype == 0 ? launch_sample<float>(p, c->B, st) : c->dtype == 1 ? launch_sample<__nv_bfloat16>(p, c->B, st) : launch_sample<__half>(p, c->B, st);
 }
