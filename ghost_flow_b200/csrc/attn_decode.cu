@@ -36,6 +36,7 @@ constexpr int DEC_WARPS = 4;
 constexpr int DEC_MAX_G = 8;
 constexpr int DEC_KEYS = 16;     // keys of a block
 constexpr int DEC_P_TERMS = 2;   // bf16 numbers that stand for a probability
+constexpr float LAZY = 7.f;      // see `unit`, pages of 8 bits
 
 __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -73,16 +74,17 @@ __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, uint3
 
 template <int D, bool SHARES, bool BYTES = false>
 struct DecCfg {
-  static constexpr int STAGES = BYTES ? 6 : 3;
+  static constexpr int STAGES = BYTES && D == 64 ? 6 : 3;
   static constexpr int ROW = BYTES ? D : D * 2;
   static constexpr int TILE = DEC_KEYS * ROW;          // K or V of a block
-  static constexpr int STAGE = 2 * TILE + (BYTES ? 2 * DEC_KEYS : 0);      // and the rows' scales
+  static constexpr int STAGE = 2 * TILE;
   static constexpr int WARP_BYTES = STAGES * STAGE;
-  static constexpr int RING = DEC_WARPS * WARP_BYTES;
+  static constexpr int SCALES = BYTES ? STAGES * 2 * DEC_KEYS : 0;         // of a warp's stages, behind all warps' rings
+  static constexpr int RING = DEC_WARPS * (WARP_BYTES + SCALES);
   static constexpr int PITCH = D + 4;                  // a head's sums, maximum and total; the pitch spreads a lane's heads over the banks
-  static constexpr int SMEM = RING + (SHARES ? 2 * DEC_MAX_G * PITCH * 4 : 0);
-  static constexpr int CTAS = D > 64 ? 2 : 4;          // on an SM
-  static_assert(DEC_WARPS * DEC_MAX_G * PITCH * 4 <= RING, "results fit in the ring");
+  static constexpr int SMEM = RING + (SHARES && !BYTES ? 2 * DEC_MAX_G * PITCH * 4 : 0);
+  static constexpr int CTAS = D > 64 && !BYTES ? 2 : 4;          // on an SM
+  static_assert(BYTES ? DEC_MAX_G * D * 4 <= STAGE : DEC_WARPS * DEC_MAX_G * PITCH * 4 <= RING, "results fit in the ring, or in a stage");
   // 16-byte chunk c of row r lies at chunk c ^ (r % 8), in rows of 64 bytes at c ^ (r / 2 % 4): ldmatrix meets every bank once, and rows fill whole lines
   __device__ __forceinline__ static int chunk(int row, int col) { return (col ^ (ROW == 64 ? (row >> 1) & 3 : row & 7)) << 4; }
 };
@@ -121,7 +123,8 @@ struct DecParams {
   PagedBatch pages;
   int share;                    // more than 8 query heads to a KV head: in this many groups, each as if it had a KV head of its own
   long long kpage, krow, khead, vpage, vrow, vhead;
-  const unsigned char *kscales, *vscales;          // of pages of 8 bits (strides in bytes)
+  const unsigned char *kscales, *vscales;          // of pages of 8 bits
+  unsigned step[5];              // their strides in bytes, from page to page and row to row of K, then of V, and KV heads: 32 bits each
 };
 
 // Units of sequence b. In a paged batch with `cu`, one of other than one new token has none.
@@ -239,6 +242,7 @@ attn_decode_kernel(const __grid_constant__ DecParams p) {
   using Cfg = DecCfg<D, SHARES, BYTES>;
   constexpr int STAGES = Cfg::STAGES;
   extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ float piece_totals[BYTES ? DEC_WARPS * DEC_MAX_G * 2 : 1];
   const DecWork& w = p.work;
   const int G = p.G;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -287,8 +291,15 @@ attn_decode_kernel(const __grid_constant__ DecParams p) {
     return k0 < a.len ? p.pages.table[(long long)a.b * p.pages.ld + (k0 >> p.pages.page_shift)] : 0;
   };
   int page_ahead = 0, page_next = 0, kv_head = 0;
+  const uint8_t *k_lane = nullptr, *v_lane = nullptr;
+  uint32_t scale_lane = 0;
   if constexpr (PAGED) {
     kv_head = p.share > 1 ? hk / p.share : hk;
+    if constexpr (BYTES) {         // what is a lane's own of an address
+      k_lane = reinterpret_cast<const uint8_t*>(p.kc) + kv_head * p.khead + lane / (D / 16) * p.krow + lane % (D / 16) * 16;
+      v_lane = reinterpret_cast<const uint8_t*>(p.vc) + kv_head * p.vhead + lane / (D / 16) * p.vrow + lane % (D / 16) * 16;
+      scale_lane = smem_u32(ring) + DEC_WARPS * Cfg::WARP_BYTES + warp * Cfg::SCALES + lane * DEC_KEYS;
+    }
     page_ahead = page_of(ahead, ahead.blk);
     if constexpr (!SHARES) page_next = page_of(ahead, ahead.blk + 1);
   }
@@ -300,21 +311,24 @@ attn_decode_kernel(const __grid_constant__ DecParams p) {
       if constexpr (BYTES) {
         const bool there = page_ahead >= 0 && page_ahead < p.pages.pages;
         if (!there && lane == 0) p.pages.bad();
-        const int r0 = k0 & ((1 << p.pages.page_shift) - 1);
-        const long long page = there ? page_ahead : 0;
-        const uint8_t* kb = reinterpret_cast<const uint8_t*>(p.kc) + page * p.kpage + r0 * p.krow + kv_head * p.khead;
-        const uint8_t* vb = reinterpret_cast<const uint8_t*>(p.vc) + page * p.vpage + r0 * p.vrow + kv_head * p.vhead;
+        constexpr int PER = D / 16, ROWS = 32 / PER;             // lanes to a row, rows of a step
+        const unsigned page = there ? page_ahead : 0, r0 = k0 & ((1 << p.pages.page_shift) - 1);
+        const int row = lane / PER, rows = there ? ahead.len - k0 - row : 0;
+        const uint8_t* kb = k_lane + ((unsigned long long)page * p.step[0] + r0 * p.step[1]);
+        const uint8_t* vb = v_lane + ((unsigned long long)page * p.step[2] + r0 * p.step[3]);
+        const uint32_t to = dst + row * Cfg::ROW + Cfg::chunk(row, lane % PER);
 #pragma unroll
-        for (int n = 0; n < DEC_KEYS * D / 16 / 32; ++n) {
-          const int id = lane + n * 32, row = id / (D / 16), col = id % (D / 16);
-          const uint32_t to = dst + row * Cfg::ROW + Cfg::chunk(row, col), bytes = there && k0 + row < ahead.len ? 16u : 0u;
-          cp_async_16(to, kb + row * p.krow + col * 16, bytes);
-          cp_async_16(to + Cfg::TILE, vb + row * p.vrow + col * 16, bytes);
+        for (int n = 0; n < DEC_KEYS / ROWS; ++n) {
+          const uint32_t at_n = (to ^ (Cfg::chunk(ROWS * n, 0))) + n * ROWS * Cfg::ROW, bytes = n * ROWS < rows ? 16u : 0u;
+          cp_async_16(at_n, kb, bytes);
+          cp_async_16(at_n + Cfg::TILE, vb, bytes);
+          kb += ROWS * p.step[1];
+          vb += ROWS * p.step[3];
         }
         // 16 keys' scales: of rows behind the last key too, which no result depends on
         if (lane < 2)
-          cp_async_16(dst + 2 * Cfg::TILE + lane * DEC_KEYS,
-                      (lane ? p.vscales : p.kscales) + ((page * (w.Hkv / p.share) + kv_head) << p.pages.page_shift) + r0, there ? 16u : 0u);
+          cp_async_16(scale_lane + st * (2 * DEC_KEYS), (lane ? p.vscales : p.kscales) +
+                      ((((unsigned long long)page * p.step[4] + kv_head) << p.pages.page_shift) + r0), there ? 16u : 0u);
       } else if constexpr (PAGED) {
         const bool there = page_ahead >= 0 && page_ahead < p.pages.pages;
         if (!there && lane == 0) p.pages.bad();
@@ -386,8 +400,9 @@ attn_decode_kernel(const __grid_constant__ DecParams p) {
       unsigned largest = 0;
 #pragma unroll
       for (int t = 0; t < D / 16; ++t) {
-        qb[t][0] = r < G ? qp[16 * t] | ((uint32_t)qp[16 * t + 1] << 16) : 0u;
-        qb[t][1] = r < G ? qp[16 * t + 2] | ((uint32_t)qp[16 * t + 3] << 16) : 0u;
+        const uint2 four = r < G ? *reinterpret_cast<const uint2*>(qp + 16 * t) : make_uint2(0, 0);
+        qb[t][0] = four.x;
+        qb[t][1] = four.y;
 #pragma unroll
         for (int h = 0; h < 2; ++h) largest = max(largest, max(qb[t][h] & 0x7fffu, (qb[t][h] >> 16) & 0x7fffu));
       }
@@ -456,12 +471,13 @@ attn_decode_kernel(const __grid_constant__ DecParams p) {
     }
     if constexpr (BYTES) {
       // Numbers of the cache become f16 as they are; their rows' powers of two go to the scores (K) and to the probabilities (V): with e the exponents of V,
-      // P' = 2^(score + e - mv + 14) of the largest score + e so far, so that the products with V have all of f16's bits whatever the rows' scales are. l, of P
-      // itself, goes by the largest score. 2^14: what is below 2^-39 of the largest is lost, not 2^-25. One f16 number stands for a P': half a step is 2^-12.
+      // P' = 2^(score + e - mv + 8), mv about the largest score + e so far, so that the products with V have all of f16's bits whatever the rows' scales are. l, of P
+      // itself, goes by the largest score. 2^8: what is below 2^-33 of the largest is lost, not 2^-25. One f16 number stands for a P': half a step is 2^-12.
       if (left > 0) {
         const uint32_t tk = my + st * Cfg::STAGE, tv = tk + Cfg::TILE;
-        const uint8_t* scales = ring + (tv + Cfg::TILE - smem_u32(ring));
+        const uint8_t* scales = ring + DEC_WARPS * Cfg::WARP_BYTES + warp * Cfg::SCALES + st * (2 * DEC_KEYS);
         const unsigned k0 = scales[r], k1 = scales[r + 8], v0 = scales[DEC_KEYS + r], v1 = scales[DEC_KEYS + r + 8];
+        // S^T: keys r, r + 8 by heads 2c, 2c + 1
         float sc[4] = {0.f, 0.f, 0.f, 0.f}, sd[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int t = 0; t < D / 16; t += 2) {
@@ -471,36 +487,45 @@ attn_decode_kernel(const __grid_constant__ DecParams p) {
           mma_f16_16816(sd, f16x2_of_e4m3<0>(a[2]), f16x2_of_e4m3<0>(a[3]), f16x2_of_e4m3<1>(a[2]), f16x2_of_e4m3<1>(a[3]), qb[t + 1][0], qb[t + 1][1]);
         }
         const float f0 = __uint_as_float(k0 << 23), f1 = __uint_as_float(k1 << 23), e0 = (float)v0 - 127.f, e1 = (float)v1 - 127.f;
-        float corr[2], pr[4];
-        bool same = true;
+        float x[4], z[4], pr[4];
+        bool grows = false;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {                            // key r (+ 8), head 2c (+ 1)
+          x[i] = r + 4 * (i & 2) < left ? (sc[i] + sd[i]) * ((i & 2) ? f1 : f0) * qf[i & 1] : -INFINITY;
+          z[i] = x[i] + ((i & 2) ? e1 : e0);
+          grows |= x[i] - m[i & 1] > LAZY || z[i] - mv[i & 1] > LAZY;
+        }
+        // The references are moved only when a score has grown by 2^7: what is 2^15 then still is a number of f16
+        if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float mx = fmaxf(fmaxf(x[e], x[2 + e]), m[e]), mz = fmaxf(fmaxf(z[e], z[2 + e]), mv[e]);
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+              mz = fmaxf(mz, __shfl_xor_sync(0xffffffffu, mz, o));
+            }
+            l[e] *= ex2_approx(m[e] - (mx == -INFINITY ? 0.f : mx));
+            const float corr = ex2_approx(mv[e] - (mz == -INFINITY ? 0.f : mz));
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j) {
+              o[j][e] *= corr;
+              o[j][2 + e] *= corr;
+            }
+            m[e] = mx;
+            mv[e] = mz;
+          }
+        }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float x0 = r < left ? (sc[e] + sd[e]) * f0 * qf[e] : -INFINITY;
-          const float x1 = r + 8 < left ? (sc[2 + e] + sd[2 + e]) * f1 * qf[e] : -INFINITY;
-          const float z0 = x0 + e0, z1 = x1 + e1;
-          float mx = fmaxf(x0, x1), mz = fmaxf(z0, z1);
-#pragma unroll
-          for (int o = 4; o < 32; o <<= 1) {
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-            mz = fmaxf(mz, __shfl_xor_sync(0xffffffffu, mz, o));
-          }
-          const float mn = fmaxf(m[e], mx), mzn = fmaxf(mv[e], mz);
-          const float ref = mn == -INFINITY ? 0.f : mn, refz = mzn == -INFINITY ? 0.f : mzn;
-          l[e] = l[e] * ex2_approx(m[e] - ref) + ex2_approx(x0 - ref) + ex2_approx(x1 - ref);
-          corr[e] = ex2_approx(mv[e] - refz);
-          same &= mv[e] == mzn;
-          m[e] = mn;
-          mv[e] = mzn;
-          pr[e] = ex2_approx(z0 - refz + 14.f);
-          pr[2 + e] = ex2_approx(z1 - refz + 14.f);
+          const float ref = m[e] == -INFINITY ? 0.f : m[e], refz = (mv[e] == -INFINITY ? 0.f : mv[e]) - 8.f;
+          l[e] += ex2_approx(x[e] - ref) + ex2_approx(x[2 + e] - ref);
+          pr[e] = ex2_approx(z[e] - refz);
+          pr[2 + e] = ex2_approx(z[2 + e] - refz);
         }
         uint32_t pt[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) pt[h] = transpose_8x8(pack_f16x2(pr[2 * h], pr[2 * h + 1]));
-        if (!__all_sync(0xffffffffu, same)) {
-#pragma unroll
-          for (int j = 0; j < D / 16; ++j) { o[j][0] *= corr[0]; o[j][1] *= corr[1]; o[j][2] *= corr[0]; o[j][3] *= corr[1]; }
-        }
         // O^T += V^T P'^T: row r of a product is dim 2 r of the 16, row r + 8 dim 2 r + 1
 #pragma unroll
         for (int j = 0; j < D / 16; j += 2) {
@@ -565,8 +590,9 @@ attn_decode_kernel(const __grid_constant__ DecParams p) {
     __syncwarp();                  // the stage is filled again two units on
   };
   // ---- end of a piece: the warps' results meet, in the ring behind the CTA's last piece, else in two buffers of their own, in two
-  // steps (2 and 3 give theirs to 0 and 1, then 1 to 0) while the ring fills with the next sequence. whole: the piece is a sequence
-  auto finish = [&](const bool last, const bool whole, const long long slot_of) {
+  // steps (2 and 3 give theirs to 0 and 1, then 1 to 0) while the ring fills with the next sequence. BYTES: each warp's lie in the stage that its last unit has
+  // left. whole: the piece is a sequence
+  auto finish = [&](const bool last, const bool whole, const long long slot_of, const int left_stage) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], 4);
@@ -576,7 +602,7 @@ attn_decode_kernel(const __grid_constant__ DecParams p) {
     if constexpr (BYTES) {       // from units of the largest score + e to those of the largest score
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float f = m[e] == -INFINITY ? 0.f : ex2_approx(mv[e] - m[e] - 14.f);
+        const float f = m[e] == -INFINITY ? 0.f : ex2_approx(mv[e] - m[e] - 8.f);
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) {
           o[j][e] *= f;
@@ -586,24 +612,29 @@ attn_decode_kernel(const __grid_constant__ DecParams p) {
     }
     // dims of o[j][0 .. 1] and o[j][2 .. 3]
     auto dim = [&](int j, int half) { return BYTES ? 16 * j + 2 * r + half : 16 * j + 8 * half + r; };
-    constexpr int BUF = DEC_MAX_G * Cfg::PITCH;
-    float* buf = reinterpret_cast<float*>(ring + (last ? 0 : Cfg::RING));
+    constexpr int PITCH = BYTES ? D : Cfg::PITCH, BUF = BYTES ? Cfg::WARP_BYTES / 4 : DEC_MAX_G * PITCH;
+    constexpr int TOTALS = BYTES ? 2 * DEC_MAX_G : BUF;          // from one warp's maxima and totals to the next one's
+    float* buf = reinterpret_cast<float*>(ring + (BYTES ? left_stage * Cfg::STAGE : last ? 0 : Cfg::RING));
+    auto totals = [&](float* of, int g) { return BYTES ? piece_totals + (of - buf) / BUF * TOTALS + 2 * g : of + g * PITCH + D; };      // of a head
     auto give = [&](float* to) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float* g = to + (2 * c + e) * Cfg::PITCH;
+        float* g = to + (2 * c + e) * PITCH;
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) {
           g[dim(j, 0)] = o[j][e];
           g[dim(j, 1)] = o[j][2 + e];
         }
         if (r == 0) {
-          g[D] = m[e];
-          g[D + 1] = l[e];
+          float* t = totals(to, 2 * c + e);
+          t[0] = m[e];
+          t[1] = l[e];
         }
       }
     };
-    if (last) {
+    if (BYTES) {
+      give(buf + warp * BUF);
+    } else if (last) {
       asm volatile("cp.async.wait_group 0;" ::: "memory");
       __syncthreads();
       give(buf + warp * BUF);
@@ -611,7 +642,7 @@ attn_decode_kernel(const __grid_constant__ DecParams p) {
       auto take = [&](const float* from) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float* g = from + (2 * c + e) * Cfg::PITCH;
+          const float* g = from + (2 * c + e) * PITCH;
           const float mo = g[D], mn = fmaxf(m[e], mo), ref = mn == -INFINITY ? 0.f : mn;
           const float ca = ex2_approx(m[e] - ref), cb = ex2_approx(mo - ref);
           m[e] = mn;
@@ -635,24 +666,24 @@ attn_decode_kernel(const __grid_constant__ DecParams p) {
       }
     }
     __syncthreads();
-    const int have = last ? DEC_WARPS : 1;
+    const int have = last || BYTES ? DEC_WARPS : 1;
     __nv_bfloat16* to = p.out + (PAGED ? p.pages.first(at.b) : at.b) * p.ldo + (long long)hk * G * D;
     float* slot = p.part + slot_of * G * (D + 2);
     for (int i = threadIdx.x; i < G * D; i += DEC_WARPS * 32) {
       const int g = i / D, d = i % D;
-      const float* x = buf + g * Cfg::PITCH;
-      float mm = x[D], ll = x[D + 1], ov = x[d];
+      const float *x = buf + g * PITCH, *t = totals(buf, g);
+      float mm = t[0], ll = t[1], ov = x[d];
       if (have > 1) {
 #pragma unroll
-        for (int k = 1; k < DEC_WARPS; ++k) mm = fmaxf(mm, x[k * BUF + D]);
+        for (int k = 1; k < DEC_WARPS; ++k) mm = fmaxf(mm, t[k * TOTALS]);
         const float ref = mm == -INFINITY ? 0.f : mm;
-        float e = ex2_approx(x[D] - ref);
+        float e = ex2_approx(t[0] - ref);
         ll *= e;
         ov *= e;
 #pragma unroll
         for (int k = 1; k < DEC_WARPS; ++k) {
-          e = ex2_approx(x[k * BUF + D] - ref);
-          ll += x[k * BUF + D + 1] * e;
+          e = ex2_approx(t[k * TOTALS] - ref);
+          ll += t[k * TOTALS + 1] * e;
           ov += x[k * BUF + d] * e;
         }
       }
@@ -678,7 +709,7 @@ attn_decode_kernel(const __grid_constant__ DecParams p) {
       unit(st);
       if (++st == STAGES) st = 0;
     }
-    finish(true, whole, blockIdx.x);
+    finish(true, whole, blockIdx.x, st == 0 ? STAGES - 1 : st - 1);
   } else {
     bool begins = false;           // the piece in work starts with its head's first unit
     for (bool first = true; left_units > 0; first = false) {
@@ -692,7 +723,7 @@ attn_decode_kernel(const __grid_constant__ DecParams p) {
       if (++st == STAGES) st = 0;
       const bool ends = at.blk == at.n - 1;
       if (ends || left_units == 1) {
-        finish(left_units == 1, begins && ends, 2 * (long long)blockIdx.x + begins);
+        finish(left_units == 1, begins && ends, 2 * (long long)blockIdx.x + begins, st == 0 ? STAGES - 1 : st - 1);
         __syncthreads();
       }
       if (--left_units > 0) at.next<PAGED>(p);
@@ -900,6 +931,8 @@ int attn_paged_one(const PagedCall& c, float scale, int splits, float* scratch, 
   p.vpage = c.strides[3]; p.vrow = c.strides[4]; p.vhead = c.strides[5];
   p.kscales = kscales; p.vscales = vscales;
   if (kscales) {
+    const long long steps[5] = {p.kpage, p.krow, p.vpage, p.vrow, c.Hk};
+    for (int i = 0; i < 5; ++i) p.step[i] = (unsigned)steps[i];
     if (splits < 0) return D == 128 ? launch_decode<128, DEC_PAGES8_SHARES>(p, chained, st) : launch_decode<64, DEC_PAGES8_SHARES>(p, chained, st);
     return D == 128 ? launch_decode<128, DEC_PAGES8>(p, chained, st) : launch_decode<64, DEC_PAGES8>(p, chained, st);
   }

@@ -123,6 +123,7 @@ bool pools(PyObject* pages_k, PyObject* pages_v, PyObject* table, PyObject* lens
     st[1] = w->stride(1, Hk * D);
     st[0] = w->stride(0, page * st[1]);
     if ((st[0] | st[1] | st[2]) & (vec - 1)) return false;
+    if (bytes && (st[0] > MOST || st[1] > MOST || st[2] > MOST)) return false;
     st += 3;
   }
   c.kpages = k.data;

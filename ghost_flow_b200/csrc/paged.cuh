@@ -64,7 +64,7 @@ inline bool paged_scales(const PagedCall8& c8) {
   for (const void* p : {(const void*)c8.kscales, (const void*)c8.vscales})
     if (!p || (reinterpret_cast<uintptr_t>(p) & 15)) return false;
   for (long long st : c.strides)
-    if (st % 16) return false;
+    if (st % 16 || st > 0x7fffffff) return false;
   return c.D % 16 == 0;
 }
 

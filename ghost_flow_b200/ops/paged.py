@@ -300,6 +300,26 @@ def _parts_beside(heads: int, sms: int) -> int:
 
 
 @functools.lru_cache(maxsize=4096)
+def _parts_of_8_bits(heads: int, keys: int, sms: int, kv_heads: int) -> int:
+    """The same over pages of 8 bits: parts of each of ``heads`` (sequences times KV heads) of at most ``keys`` keys, or, negative, the number of parts of all
+    sequences together. Four CTAs are on an SM. A unit of 64 keys takes a CTA .57 us alone and 1.55 on a full machine, waves that are not full count half as if
+    they were, and joining 3 us and .12 for each part. Shares of all sequences where there are 27 units to a CTA and sequences of 4096 keys. us with 1 / 2 / 4 / 8 / 16
+    parts / shares, heads of 128: 32 sequences of 100 .. 4096 keys, 32 / 8 heads 49 / 43 / 38 / 41 / 55 / 34 (shares), 4 of 20011 .. 30001, 64 / 8 heads 268 / 139 / 74 /
+    47 / 45 / 47 (16), 16 of 1000 .. 4000 45 / 31 / 28 / 31 / 42 / 31 (4), 16 of 2000, 32 / 32 heads 46 / 52 / 53 / 61 / 84 / 51 (1), 1 of 8000, 32 / 8 heads 72 / 40 /
+    23 / 14 / 12 / 19 (16)."""
+    slots, units = 4 * sms, (keys + 63) // 64
+    if units >= 64 and heads * units >= 27 * slots:
+        return -max(1, slots // kv_heads)
+
+    def cost(s):
+        full = heads * s / slots
+        waves = 1.0 if full <= 1 else (full + math.ceil(full)) / 2
+        return -(-units // s) * (.57 + .98 * min(1.0, full)) * waves + (3 + .12 * s if s > 1 else 0)
+
+    return min((s for s in _SLICES if s <= max(1, units)), key=cost)
+
+
+@functools.lru_cache(maxsize=4096)
 def _attention_workspace(device: int, B: int, T: int, one_each: bool, ones: bool, keys: int, H: int, Hk: int, D: int) -> int:
     """Bytes that a call leaves the results of pieces in (the number of SMs decides whether keys, ``keys`` of a sequence at most, are cut)."""
     return _lib.cuda_lib().gf_paged_attn_workspace(B, T, 1 if one_each else 0, 1 if ones else 0, keys, H, Hk, D)
@@ -409,7 +429,10 @@ def paged_attention(q, kpages, vpages, page_table, lens, cu=None, scale: float |
     parts, few, ws = 0, None, None
     if one or (cu is not None and B >= _MANY and groups):
         sms = _SMS.get(device) or _sm_count(q.device)
-        parts = _decode_parts(B, Hk * groups, keys, D, sms, True) if one else _parts_beside(B * Hk * groups, sms)
+        if not one:
+            parts = _parts_beside(B * Hk * groups, sms)
+        else:
+            parts = _decode_parts(B, Hk * groups, keys, D, sms, True) if kscales is None else _parts_of_8_bits(B * Hk * groups, keys, sms, Hk * groups)
         if parts != 1:
             few = torch.empty((B * parts if parts > 0 else -2 * parts) * H * (D + 2), dtype=torch.float32, device=q.device)
     if not one:
