@@ -35,9 +35,9 @@ constexpr int PG_TILE = 128;      // rows of a tile, keys of a step
 constexpr int PG_THREADS = 384;   // warpgroup 0: TMA warp, MMA warp, warp that clears rows, an idle one; warpgroups 1 and 2: softmax of tile 0 / 1
 constexpr int PG_REGS_CTRL = 104; // 128 x 104 + 256 x 200 = 64512, the block's own at launch (384 x 168)
 constexpr int PG_REGS_SOFTMAX = 200;
-// With pages of 8 bits there is a fourth warpgroup, of warps that turn them into bf16: 128 x 56 + 256 x 200 + 128 x 56 = 65536, 512 x 128 at launch.
+// With pages of 8 bits there is a fourth warpgroup, of warps that turn them into bf16: 128 x 80 + 256 x 176 + 128 x 80 = 65536, 512 x 128 at launch.
 constexpr int PG_THREADS8 = 512;
-constexpr int PG_REGS_CTRL8 = 56, PG_REGS_TURN = 56;
+constexpr int PG_REGS_CTRL8 = 80, PG_REGS_SOFTMAX8 = 176, PG_REGS_TURN = 80;
 constexpr int PG_PARTS = 2;       // P V of a tile is issued in this many parts of the keys
 constexpr float PG_RESCALE = 8.0f;  // log2 units
 
@@ -224,8 +224,8 @@ __device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* m
       : "memory");
 }
 
-// 16 numbers of the cache times their row's power of two, as bf16: exact
-__device__ __forceinline__ void bf16x16_of_e4m3(const uint4& in, float scale, uint4& lo, uint4& hi) {
+// 16 numbers of the cache times their row's power of two (twice, as f32x2), as bf16: exact
+__device__ __forceinline__ void bf16x16_of_e4m3(const uint4& in, uint64_t scale, uint4& lo, uint4& hi) {
   const uint32_t* four = reinterpret_cast<const uint32_t*>(&in);
   uint32_t out[8];
 #pragma unroll
@@ -234,7 +234,8 @@ __device__ __forceinline__ void bf16x16_of_e4m3(const uint4& in, float scale, ui
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((unsigned short)(i & 1 ? four[i >> 1] >> 16 : four[i >> 1])));
     float a, b;
     asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, h;\n\t}" : "=f"(a), "=f"(b) : "r"(h));
-    out[i] = pack_bf16x2(a * scale, b * scale);
+    const uint64_t x = f2_mul(pk2f(a, b), scale);
+    out[i] = pack_bf16x2(lo2(x), hi2(x));
   }
   lo = make_uint4(out[0], out[1], out[2], out[3]);
   hi = make_uint4(out[4], out[5], out[6], out[7]);
@@ -529,60 +530,72 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     // ---------------------------------------------------------------- pages of 8 bits to bf16: a thread has a key
     // Lanes of neighbouring rows begin at neighbouring chunks of 16 bytes, so that eight of them meet every bank once, here and in the swizzled tile.
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PG_REGS_TURN));
+    constexpr int SHIFT = HD == 64 ? 1 : 0;
     const int r = threadIdx.x & 127;
-    int ks = -1, vs = 0;                           // bytes of the row's powers of two; -1: there is no such key, zeros
-    auto look = [&](int i) {
-      ks = -1;
+    // the row's page of step i, -1 where there is no such key or page (which the producer reports), and its powers of two: asked for two steps ahead, and one
+    auto page_at = [&](int i) {
       const int key = (item.j0 + i) * PG_TILE + r;
-      if (i >= n_j || key >= item.keys) return;
+      if (i >= n_j || key >= item.keys) return -1;
       const int page = p.seqs.table[(long long)item.b * p.seqs.ld + (key >> p.seqs.page_shift)];
-      if (page < 0 || page >= p.seqs.pages) return;            // (reported by the producer)
-      const long long at = (((long long)page * p.Hkv + item.hk) << p.seqs.page_shift) + (key & ((1 << p.seqs.page_shift) - 1));
+      return page < p.seqs.pages ? page : -1;
+    };
+    int ks = 0, vs = 0;
+    auto scales_at = [&](int i, int page) {
+      ks = vs = 0;
+      if (page < 0) return;
+      const int row = ((item.j0 + i) * PG_TILE + r) & ((1 << p.seqs.page_shift) - 1);
+      const long long at = (((long long)page * p.Hkv + item.hk) << p.seqs.page_shift) + row;
       ks = p.kscales[at];
       vs = p.vscales[at];
     };
-    auto turn = [&](const uint8_t* raw, uint8_t* tile, int byte) {
-      constexpr int CHUNKS = HD / 16;
-      const float scale = __uint_as_float((unsigned)max(byte, 0) << 23);
-#pragma unroll 2
-      for (int k = 0; k < CHUNKS; ++k) {
-        const int q = (k + (HD == 64 ? r >> 1 : r)) & (CHUNKS - 1), u = 2 * q;
-        uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-        if (byte >= 0) bf16x16_of_e4m3(*reinterpret_cast<const uint4*>(raw + r * HD + q * 16), scale, lo, hi);
-        uint8_t* to = tile + (u >> 3) * (PG_TILE * 128) + r * 128;
-        *reinterpret_cast<uint4*>(to + (((u & 7) ^ (r & 7)) << 4)) = lo;
-        *reinterpret_cast<uint4*>(to + ((((u + 1) & 7) ^ (r & 7)) << 4)) = hi;
+    constexpr int CHUNKS = HD / 16, TOGETHER = 4;
+    auto turn = [&](const uint8_t* raw, uint8_t* tile, uint64_t* raw_full, uint64_t* raw_empty, uint64_t* full, uint64_t* empty, int i, bool there, int byte) {
+      if (!mbar_wait_warp_tight(raw_full, i & 1) || !mbar_wait_warp_tight(empty, ((i >> 1) & 1) ^ 1)) return false;
+      // where there is no key: zeros, whatever lies there (the tile's rows of pages that are there may be anything behind the last key)
+      const uint64_t scale = pk2((unsigned)byte << 23, (unsigned)byte << 23);
+      const uint32_t keep = there ? 0xffffffffu : 0u;
+#pragma unroll 1
+      for (int k0 = 0; k0 < CHUNKS; k0 += TOGETHER) {
+        uint4 in[TOGETHER];
+#pragma unroll
+        for (int k = 0; k < TOGETHER; ++k) in[k] = *reinterpret_cast<const uint4*>(raw + r * HD + (((k0 + k + (r >> SHIFT)) & (CHUNKS - 1)) << 4));
+#pragma unroll
+        for (int k = 0; k < TOGETHER; ++k) {
+          const int u = 2 * ((k0 + k + (r >> SHIFT)) & (CHUNKS - 1));
+          in[k].x &= keep; in[k].y &= keep; in[k].z &= keep; in[k].w &= keep;
+          uint4 lo, hi;
+          bf16x16_of_e4m3(in[k], scale, lo, hi);
+          uint8_t* to = tile + (u >> 3) * (PG_TILE * 128) + r * 128;
+          *reinterpret_cast<uint4*>(to + (((u & 7) ^ (r & 7)) << 4)) = lo;
+          *reinterpret_cast<uint4*>(to + ((((u + 1) & 7) ^ (r & 7)) << 4)) = hi;
+        }
       }
       fence_proxy_async_smem();
       __syncwarp();
-    };
-    look(0);
-    for (int i = 0; i < n_j; ++i) {
-      const int st = i & 1, kb = ks, vb = ks < 0 ? -1 : vs;
-      const uint32_t ph = (i >> 1) & 1;
-      look(i + 1);
-      bool ok = mbar_wait_warp_tight(&raw_full[0], i & 1) && mbar_wait_warp_tight(&k_empty[st], ph ^ 1);
-      if (ok) {
-        turn(smem + Cfg::OFF_RAW, sK + st * Cfg::TILE_BYTES, kb);
-        if (lane == 0) {
-          mbar_arrive(&k_full[st]);
-          mbar_arrive(&raw_empty[0]);
-        }
-        ok = mbar_wait_warp_tight(&raw_full[1], i & 1) && mbar_wait_warp_tight(&v_empty[st], ph ^ 1);
+      if (lane == 0) {
+        mbar_arrive(full);
+        mbar_arrive(raw_empty);
       }
-      if (!ok) {
+      return true;
+    };
+    int page = page_at(0), page_next = page_at(1);
+    scales_at(0, page);
+    for (int i = 0; i < n_j; ++i) {
+      const int st = i & 1, kb = ks, vb = vs;
+      const bool there = page >= 0;
+      page = page_next;
+      scales_at(i + 1, page);
+      page_next = page_at(i + 2);
+      const uint8_t* raw = smem + Cfg::OFF_RAW;
+      if (!turn(raw, sK + st * Cfg::TILE_BYTES, &raw_full[0], &raw_empty[0], &k_full[st], &k_empty[st], i, there, kb) ||
+          !turn(raw + Cfg::RAW_BYTES, sV + st * Cfg::TILE_BYTES, &raw_full[1], &raw_empty[1], &v_full[st], &v_empty[st], i, there, vb)) {
         if (lane == 0) fail(GF_ERR_WAIT_FULL);
         break;
-      }
-      turn(smem + Cfg::OFF_RAW + Cfg::RAW_BYTES, sV + st * Cfg::TILE_BYTES, vb);
-      if (lane == 0) {
-        mbar_arrive(&v_full[st]);
-        mbar_arrive(&raw_empty[1]);
       }
     }
   } else {
     // ---------------------------------------------------------------- softmax warps: tile t = warp / 4 - 1
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PG_REGS_SOFTMAX));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(BYTES ? PG_REGS_SOFTMAX8 : PG_REGS_SOFTMAX));
     const int t = (warp >> 2) - 1;
     const int lane_grp = warp & 3;
     const int r = lane_grp * 32 + lane;

@@ -44,6 +44,10 @@ int (*f_sample)(const gf::SampleCall*, void*);
 int (*f_append_heads)(const gf::PagedCall8*, const float*, const float*, int, int, int, const void*, const void*, float, void*);
 int (*f_attn8)(const gf::PagedCall8*, float, void*, long long, int, float*, void*);
 int (*f_attn8_one)(const gf::PagedCall8*, float, int, float*, void*);
+int (*f_norm_rope)(const void*, long long, const void*, const void*, const float*, const float*, void*, void*, long long, int, int, int, int, int, int, int,
+                   float, void*);
+int (*f_norm_rope_back)(const void*, long long, const void*, const void*, const float*, const float*, const void*, const void*, const void*, const long long*,
+                        void*, void*, void*, float*, long long, int, int, int, int, int, int, int, float, void*);
 int (*f_read)(const gf::PagedCall8*, void*, void*, void*);
 // what the operators' `_observed` asks (ops/fused.py), here without its Python frames (0.15 us instead of 0.6), and whether gradients are recorded
 PyObject *tracing, *transforms, *dispatch_modes, *function_modes, *only_device_contexts, *forward_ad, *grad_enabled, *requires_grad, *current_level;
@@ -477,6 +481,117 @@ PyObject* run_logits(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return PyLong_FromLong(rc);
 }
 
+// Rows [B, S, heads, D] of bf16, heads packed, as B * S of them that are equally far apart; false for other layouts.
+bool rows_of(const View& x, int device, long long heads, long long D, long long& ld) {
+  if (!x.is(BFLOAT, 16, 4, device) || x.shape[2] != heads || x.shape[3] != D || x.stride(3, 1) != 1 || x.stride(2, D) != D || (x.at() & 15)) return false;
+  const long long B = x.shape[0], S = x.shape[1];
+  ld = S > 1 ? x.stride(1, heads * D) : x.stride(0, heads * D);
+  return ld >= heads * D && ld % 8 == 0 && (B <= 1 || S <= 1 || x.stride(0, S * ld) == S * ld);
+}
+
+struct NormRope {
+  const void *x, *qw, *kw, *dq, *dk, *dv;
+  const float *cos, *sin;
+  long long ldx, lds[3], T, S, H, Hk, D, rotary, pos;
+};
+
+// What forward and backward pass look at alike: qkv, q_weight, k_weight, cos, sin.
+bool norm_rope_of(PyObject* const* a, PyObject* H, PyObject* Hk, PyObject* pos, NormRope& r, int& device) {
+  r.H = PyLong_AsLongLong(H);
+  r.Hk = PyLong_AsLongLong(Hk);
+  r.pos = PyLong_AsLongLong(pos);
+  View x, w, t;
+  if (PyErr_Occurred() || !x.of(a[0]) || x.ndim != 4 || r.H <= 0 || r.Hk <= 0 || r.H > 65535 || r.Hk > 65535 || r.pos < 0 || r.pos > MOST) return false;
+  device = x.device;
+  r.D = x.shape[3];
+  r.S = x.shape[1];
+  r.T = x.shape[0] * r.S;
+  if (r.T <= 0 || r.T > MOST || (r.D != 32 && r.D != 64 && r.D != 128 && r.D != 256) || !rows_of(x, device, r.H + 2 * r.Hk, r.D, r.ldx) ||
+      (a[1] == Py_None) != (a[2] == Py_None))
+    return false;
+  r.x = x.data;
+  for (int i = 1; i < 3; ++i) {
+    if (a[i] == Py_None) continue;
+    if (!w.of(a[i]) || !w.is(BFLOAT, 16, 1, device) || w.shape[0] != r.D || w.stride(0, 1) != 1 || (w.at() & 15)) return false;
+    (i == 1 ? r.qw : r.kw) = w.data;
+  }
+  for (int i = 3; i < 5; ++i) {
+    if (!t.of(a[i]) || !t.is(FLOAT, 32, 2, device) || t.shape[1] % 8 || 2 * t.shape[1] > r.D || (i == 4 && 2 * t.shape[1] != r.rotary) ||
+        t.shape[0] < r.S + r.pos || (t.shape[1] && (t.stride(1, 1) != 1 || t.stride(0, t.shape[1]) != t.shape[1] || (t.at() & 15))))
+      return false;
+    r.rotary = 2 * t.shape[1];
+    (i == 3 ? r.cos : r.sin) = r.rotary ? (const float*)t.data : nullptr;
+  }
+  return true;
+}
+
+// norm_rope(qkv, q_weight, k_weight, cos, sin, H, Hk, pos): (call, device, whether a gradient is to be recorded), None as above
+PyObject* norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!arguments("norm_rope", n, 8)) return nullptr;
+  NormRope r{};
+  int device;
+  if (followed({a[3], a[4]})) Py_RETURN_NONE;      // (gradients of the tables are not the kernel's)
+  if (!norm_rope_of(a, a[5], a[6], a[7], r, device)) {
+    if (PyErr_Occurred()) return nullptr;
+    Py_RETURN_NONE;
+  }
+  return Py_BuildValue("(y#iO)", (const char*)&r, (Py_ssize_t)sizeof r, device, followed({a[0], a[1], a[2]}) ? Py_True : Py_False);
+}
+
+// norm_rope_back(qkv, q_weight, k_weight, cos, sin, H, Hk, pos, dq, dk, dv): (call, device), None as above
+PyObject* norm_rope_back(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!arguments("norm_rope_back", n, 11)) return nullptr;
+  NormRope r{};
+  int device;
+  View g;
+  if (!norm_rope_of(a, a[5], a[6], a[7], r, device)) {
+    if (PyErr_Occurred()) return nullptr;
+    Py_RETURN_NONE;
+  }
+  const void** to[3] = {&r.dq, &r.dk, &r.dv};
+  for (int i = 0; i < 3; ++i) {
+    if (!g.of(a[8 + i]) || g.ndim != 4 || g.shape[1] != r.S || g.shape[0] * r.S != r.T || !rows_of(g, device, i ? r.Hk : r.H, r.D, r.lds[i])) Py_RETURN_NONE;
+    *to[i] = g.data;
+  }
+  return Py_BuildValue("(y#i)", (const char*)&r, (Py_ssize_t)sizeof r, device);
+}
+
+// run_norm_rope(call, q, k, eps, interleaved, stream)
+PyObject* run_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  NormRope r;
+  View q, k;
+  if (!arguments("run_norm_rope", n, 6) || !call_of(a[0], r) || !memory_of(a[1], q) || !memory_of(a[2], k)) return nullptr;
+  const float eps = (float)PyFloat_AsDouble(a[3]);
+  const int interleaved = PyObject_IsTrue(a[4]);
+  void* stream = PyLong_AsVoidPtr(a[5]);
+  if (PyErr_Occurred()) return nullptr;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = f_norm_rope(r.x, r.ldx, r.qw, r.kw, r.cos, r.sin, q.data, k.data, r.T, (int)r.S, (int)r.H, (int)r.Hk, (int)r.D, (int)r.rotary, (int)r.pos, interleaved,
+                   eps, stream);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(rc);
+}
+
+// run_norm_rope_back(call, dx, dq_weight, dk_weight, scratch, eps, interleaved, stream)
+PyObject* run_norm_rope_back(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  NormRope r;
+  View x, qw, kw, ws;
+  if (!arguments("run_norm_rope_back", n, 8) || !call_of(a[0], r) || !memory_of(a[1], x) || !memory_of(a[2], qw) || !memory_of(a[3], kw) ||
+      !memory_of(a[4], ws))
+    return nullptr;
+  const float eps = (float)PyFloat_AsDouble(a[5]);
+  const int interleaved = PyObject_IsTrue(a[6]);
+  void* stream = PyLong_AsVoidPtr(a[7]);
+  if (PyErr_Occurred()) return nullptr;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = f_norm_rope_back(r.x, r.ldx, r.qw, r.kw, r.cos, r.sin, r.dq, r.dk, r.dv, r.lds, x.data, qw.data, kw.data, (float*)ws.data, r.T, (int)r.S, (int)r.H,
+                        (int)r.Hk, (int)r.D, (int)r.rotary, (int)r.pos, interleaved, eps, stream);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(rc);
+}
+
 // A choice: a number from `least` to `most`, or one of 32 bits of every row.
 bool choice(PyObject* o, long long B, int device, int code, double least, double most, double& number, const void*& rows) {
   View v;
@@ -534,9 +649,10 @@ PyObject* run_sample(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return PyLong_FromLong(rc);
 }
 
-// bind_more(addresses of gf_sample_tokens, gf_paged_append_heads, gf_paged_read, gf_paged_attn8, gf_paged_attn8_one)
+// bind_more(addresses of gf_sample_tokens, gf_paged_append_heads, gf_paged_read, gf_paged_attn8, gf_paged_attn8_one,
+// gf_norm_rope_qkv, gf_norm_rope_qkv_bwd)
 PyObject* bind_more(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  constexpr int N = 5;
+  constexpr int N = 7;
   if (!arguments("bind_more", n, N)) return nullptr;
   void* f[N];
   for (int i = 0; i < N; ++i) f[i] = PyLong_AsVoidPtr(a[i]);
@@ -546,6 +662,8 @@ PyObject* bind_more(PyObject*, PyObject* const* a, Py_ssize_t n) {
   f_read = (decltype(f_read))f[2];
   f_attn8 = (decltype(f_attn8))f[3];
   f_attn8_one = (decltype(f_attn8_one))f[4];
+  f_norm_rope = (decltype(f_norm_rope))f[5];
+  f_norm_rope_back = (decltype(f_norm_rope_back))f[6];
   Py_RETURN_NONE;
 }
 
@@ -584,7 +702,8 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
 #define FN(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FN(bind), FN(append), FN(run_append), FN(attention), FN(run_attention), FN(logits), FN(run_logits), FN(sample), FN(run_sample),
                          FN(bind_more), FN(append_heads), FN(run_append_heads), FN(read), FN(run_read),
-                         FN(attention8), FN(run_attention8), {nullptr, nullptr, 0, nullptr}};
+                         FN(attention8), FN(run_attention8), FN(norm_rope), FN(norm_rope_back), FN(run_norm_rope),
+                         FN(run_norm_rope_back), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_gf_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

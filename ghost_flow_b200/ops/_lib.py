@@ -160,7 +160,8 @@ def calls():
         module.bind(exchange, *(ctypes.cast(getattr(lib, name), c_void_p).value for name in (
             "gf_paged_append", "gf_paged_attn", "gf_paged_attn_one", "gf_process_logits")), *follows())
         module.bind_more(*(ctypes.cast(getattr(lib, name), c_void_p).value for name in (
-            "gf_sample_tokens", "gf_paged_append_heads", "gf_paged_read", "gf_paged_attn8", "gf_paged_attn8_one")))
+            "gf_sample_tokens", "gf_paged_append_heads", "gf_paged_read", "gf_paged_attn8", "gf_paged_attn8_one",
+            "gf_norm_rope_qkv", "gf_norm_rope_qkv_bwd")))
         _CALLS = module
     return _CALLS
 

@@ -353,15 +353,10 @@ def head_norm_rope_ref(x, w, cos, sin, eps=1e-6, interleaved=False):
 
 class _NormRopeQKVFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, qkv, qw, kw, H, Hk, cos, sin, eps, interleaved, pos_offset):
+    def forward(ctx, qkv, qw, kw, H, Hk, cos, sin, eps, interleaved, pos_offset, call):
         B, S, _, D = qkv.shape
-        q = torch.empty((B, S, H, D), dtype=qkv.dtype, device=qkv.device)
-        k = torch.empty((B, S, Hk, D), dtype=qkv.dtype, device=qkv.device)
-        x, ld = _packed_rows(qkv)
-        weights = (None, None) if qw is None else (qw.data_ptr(), kw.data_ptr())
-        _rc(_lib.cuda_lib().gf_norm_rope_qkv(x.data_ptr(), ld, *weights, cos.data_ptr(), sin.data_ptr(), q.data_ptr(), k.data_ptr(),
-                                             B * S, S, H, Hk, D, 2 * cos.shape[1], pos_offset, interleaved, eps, _lib.stream_ptr()),
-            "gf_norm_rope_qkv")
+        q, k = qkv.new_empty((B, S, H, D)), qkv.new_empty((B, S, Hk, D))
+        _rc(_lib.calls().run_norm_rope(call, q, k, eps, interleaved, _lib.stream_ptr()), "gf_norm_rope_qkv")
         ctx.save_for_backward(qkv, qw, kw, cos, sin)
         ctx.args = H, Hk, eps, interleaved, pos_offset
         return q, k, qkv[:, :, H + Hk:]
@@ -371,21 +366,26 @@ class _NormRopeQKVFn(torch.autograd.Function):
     def backward(ctx, dq, dk, dv):
         qkv, qw, kw, cos, sin = ctx.saved_tensors
         H, Hk, eps, interleaved, pos_offset = ctx.args
-        B, S, G, D = qkv.shape
-        x, ld = _packed_rows(qkv)                       # (hooks on saved tensors may bring them back in another layout)
-        qw, kw, cos, sin = (None if t is None else _dense16(t) for t in (qw, kw, cos, sin))
-        packed = [_packed_rows(t) for t in (dq, dk, dv)]
-        dx, lib = torch.empty((B, S, G, D), dtype=qkv.dtype, device=qkv.device), _lib.cuda_lib()
-        dqw = dkw = None
-        weights = into = (None, None)
-        scratch = None
+        look, D = _lib.calls().norm_rope_back, qkv.shape[3]
+        call = look(qkv, qw, kw, cos, sin, H, Hk, pos_offset, dq, dk, dv)
+        if call is None:           # gradients of another layout, and saved tensors where hooks have brought them back in one
+            qkv, dq, dk, dv = (_packed_rows(t)[0] for t in (qkv, dq, dk, dv))
+            qw, kw, cos, sin = (None if t is None else _dense16(t) for t in (qw, kw, cos, sin))
+            call = look(qkv, qw, kw, cos, sin, H, Hk, pos_offset, dq, dk, dv)
+            if call is None:
+                raise RuntimeError("norm_rope_qkv: saved tensors or gradients that are not what they were made as")
+        dx = qkv.new_empty(qkv.shape)
+        dqw = dkw = scratch = None
         if qw is not None:
-            dqw, dkw, scratch = torch.empty_like(qw), torch.empty_like(kw), _scratch(qkv.device, lib.gf_norm_rope_scratch(D))
-            weights, into = (qw.data_ptr(), kw.data_ptr()), (dqw.data_ptr(), dkw.data_ptr())
-        _rc(lib.gf_norm_rope_qkv_bwd(x.data_ptr(), ld, *weights, cos.data_ptr(), sin.data_ptr(), *(t.data_ptr() for t, _ in packed),
-                                     (ctypes.c_longlong * 3)(*(n for _, n in packed)), dx.data_ptr(), *into,
-                                     None if scratch is None else scratch.data_ptr(), B * S, S, H, Hk, D, 2 * cos.shape[1], pos_offset, interleaved, eps, _lib.stream_ptr()), "gf_norm_rope_qkv_bwd")
-        return dx, dqw, dkw, None, None, None, None, None, None, None
+            dqw, dkw = torch.empty_like(qw), torch.empty_like(kw)
+            scratch = _scratch(qkv.device, _norm_rope_scratch(call[1], D))
+        _rc(_lib.calls().run_norm_rope_back(call[0], dx, dqw, dkw, scratch, eps, interleaved, _lib.stream_ptr()), "gf_norm_rope_qkv_bwd")
+        return dx, dqw, dkw, None, None, None, None, None, None, None, None
+
+
+@functools.lru_cache(maxsize=None)
+def _norm_rope_scratch(device: int, D: int) -> int:
+    return _lib.cuda_lib().gf_norm_rope_scratch(D)
 
 
 def _check_partial_tables(what: str, D: int, cos, sin, device) -> None:
@@ -401,27 +401,38 @@ def norm_rope_qkv(qkv, num_heads: int, num_kv_heads: int, q_weight, k_weight, co
     rotated (see :func:`rope`), in one launch per direction; v is a view. ``cos`` and ``sin`` ``[positions, n]`` rotate the first ``2 n`` dims of a
     head, the others stay as the norm leaves them. Without both weights (``None``) heads are rotated only. bf16 heads of 32, 64, 128 or 256 with a multiple of 16 dims rotated take the kernels."""
     what, H, Hk = "norm_rope_qkv", num_heads, num_kv_heads
-    if qkv.dim() != 4 or qkv.shape[2] != H + 2 * Hk or H < 1 or Hk < 1:
-        raise ValueError(f"{what}: a packed projection of {H} + 2 x {Hk} heads is [batch, sequence, {H + 2 * Hk}, head size], not {list(qkv.shape)}")
-    (_, S, _, D), dev = qkv.shape, qkv.device
-    if (q_weight is None) != (k_weight is None):
-        raise ValueError(f"{what}: the norms of q and k go together")
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None and (w.shape != (D,) or w.device != dev):
-            raise ValueError(f"{what}: {name} is [{D}] on {dev}, not {list(w.shape)} on {w.device}")
-    _check_partial_tables(what, D, cos, sin, dev)
-    if not 0 <= pos_offset <= cos.shape[0] - S:
-        raise ValueError(f"{what}: positions {pos_offset} .. {pos_offset + S - 1} are not in tables of {cos.shape[0]} rows")
-    fp32 = torch.float32
-    if _cuda_bf16(qkv, q_weight, k_weight) and D in (32, 64, 128, 256) and cos.shape[1] % 8 == 0 \
-            and cos.dtype is fp32 and sin.dtype is fp32 and not (cos.requires_grad or sin.requires_grad) and not _observed() and qkv.numel() > 0 \
-            and qkv.shape[0] * S < 2 ** 31 and H < 65536 and Hk < 65536:
-        if dev.index != torch.cuda.current_device():
-            with torch.cuda.device(dev):
+    call = None
+    if qkv.get_device() >= 0 and not torch.compiler.is_compiling():
+        look = _lib.calls().norm_rope
+        call = look(qkv, q_weight, k_weight, cos, sin, H, Hk, pos_offset)
+    if call is None:
+        if qkv.dim() != 4 or qkv.shape[2] != H + 2 * Hk or H < 1 or Hk < 1:
+            raise ValueError(f"{what}: a packed projection of {H} + 2 x {Hk} heads is [batch, sequence, {H + 2 * Hk}, head size], not {list(qkv.shape)}")
+        (_, S, _, D), dev = qkv.shape, qkv.device
+        if (q_weight is None) != (k_weight is None):
+            raise ValueError(f"{what}: the norms of q and k go together")
+        for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+            if w is not None and (w.shape != (D,) or w.device != dev):
+                raise ValueError(f"{what}: {name} is [{D}] on {dev}, not {list(w.shape)} on {w.device}")
+        _check_partial_tables(what, D, cos, sin, dev)
+        if not 0 <= pos_offset <= cos.shape[0] - S:
+            raise ValueError(f"{what}: positions {pos_offset} .. {pos_offset + S - 1} are not in tables of {cos.shape[0]} rows")
+        if qkv.is_cuda and not _observed() and qkv.numel() > 0:                # other layouts
+            qkv = _packed_rows(qkv)[0]
+            q_weight, k_weight, cos, sin = (None if t is None else _dense16(t) for t in (q_weight, k_weight, cos, sin))
+            call = look(qkv, q_weight, k_weight, cos, sin, H, Hk, pos_offset)
+    if call is not None:
+        at, device, graph = call
+        stream = _lib.stream_on(device)
+        if stream is None:
+            with torch.cuda.device(device):
                 return norm_rope_qkv(qkv, H, Hk, q_weight, k_weight, cos, sin, eps, interleaved, pos_offset)
-        qw, kw = (None if w is None else _dense16(w) for w in (q_weight, k_weight))
-        return _call(_NormRopeQKVFn, qkv, qw, kw, H, Hk, _dense16(cos), _dense16(sin), float(eps),
-                     1 if interleaved else 0, pos_offset)
+        if graph:
+            return _NormRopeQKVFn.apply(qkv, q_weight, k_weight, H, Hk, cos, sin, float(eps), interleaved, pos_offset, at)
+        B, S, _, D = qkv.shape
+        q, k = qkv.new_empty((B, S, H, D)), qkv.new_empty((B, S, Hk, D))
+        _rc(_lib.calls().run_norm_rope(at, q, k, float(eps), interleaved, stream), "gf_norm_rope_qkv")
+        return q, k, qkv[:, :, H + Hk:]
     c, s = (t[pos_offset:pos_offset + S].unsqueeze(1) for t in (cos, sin))
     q, k, v = split_qkv(qkv, H, Hk)
     return (head_norm_rope_ref(q, q_weight, c, s, eps, interleaved).to(qkv.dtype),
