@@ -486,7 +486,7 @@ bool rows_of(const View& x, int device, long long heads, long long D, long long&
   if (!x.is(BFLOAT, 16, 4, device) || x.shape[2] != heads || x.shape[3] != D || x.stride(3, 1) != 1 || x.stride(2, D) != D || (x.at() & 15)) return false;
   const long long B = x.shape[0], S = x.shape[1];
   ld = S > 1 ? x.stride(1, heads * D) : x.stride(0, heads * D);
-  return ld >= heads * D && ld % 8 == 0 && (B <= 1 || S <= 1 || x.stride(0, S * ld) == S * ld);
+  return ld >= heads * D && ld % 8 == 0 && ld <= MOST && (B <= 1 || S <= 1 || x.stride(0, S * ld) == S * ld);
 }
 
 struct NormRope {

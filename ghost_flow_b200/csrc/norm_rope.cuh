@@ -20,49 +20,73 @@ struct HeadLane {
   }
 };
 
+// Two neighbouring numbers to a register pair, whose products and sums are one instruction.
 struct Head16 {
-  float a[8], b[8];
-  __device__ __forceinline__ void of(const uint4& x, const uint4& y) {
-    const uint32_t *u = reinterpret_cast<const uint32_t*>(&x), *v = reinterpret_cast<const uint32_t*>(&y);
+  uint64_t x[8];                 // the first vector in 0 .. 3, the second in 4 .. 7
+  __device__ __forceinline__ void of(const uint4& first, const uint4& second) {
+    const uint32_t *u = reinterpret_cast<const uint32_t*>(&first), *v = reinterpret_cast<const uint32_t*>(&second);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 f = unpack_bf16x2(u[i]), g = unpack_bf16x2(v[i]);
-      a[2 * i] = f.x; a[2 * i + 1] = f.y;
-      b[2 * i] = g.x; b[2 * i + 1] = g.y;
+      x[i] = pk2(u[i] << 16, u[i] & 0xffff0000u);
+      x[4 + i] = pk2(v[i] << 16, v[i] & 0xffff0000u);
     }
   }
-  __device__ __forceinline__ void to(uint4& x, uint4& y) const {
-    uint32_t *u = reinterpret_cast<uint32_t*>(&x), *v = reinterpret_cast<uint32_t*>(&y);
+  __device__ __forceinline__ void to(uint4& first, uint4& second) const {
+    uint32_t *u = reinterpret_cast<uint32_t*>(&first), *v = reinterpret_cast<uint32_t*>(&second);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      u[i] = pack_bf16x2(a[2 * i], a[2 * i + 1]);
-      v[i] = pack_bf16x2(b[2 * i], b[2 * i + 1]);
+      u[i] = pack_bf16x2(lo2(x[i]), hi2(x[i]));
+      v[i] = pack_bf16x2(lo2(x[4 + i]), hi2(x[4 + i]));
     }
   }
   __device__ __forceinline__ float dot(const Head16& o) const {
-    float s = 0.f;
+    uint64_t s = f2_mul(x[0], o.x[0]), t = f2_mul(x[1], o.x[1]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s += a[i] * o.a[i] + b[i] * o.b[i];
-    return s;
+    for (int i = 2; i < 8; i += 2) {
+      s = f2_fma(x[i], o.x[i], s);
+      t = f2_fma(x[i + 1], o.x[i + 1], t);
+    }
+    s = f2_add(s, t);
+    return lo2(s) + hi2(s);
+  }
+  __device__ __forceinline__ void scale(const Head16& o) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = f2_mul(x[i], o.x[i]);
+  }
+  __device__ __forceinline__ void scale(float f) {
+    const uint64_t two = pk2f(f, f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = f2_mul(x[i], two);
+  }
+};
+
+// A lane's 8 entries of a row of the tables, and the turn by them.
+struct HeadTurn {
+  uint64_t c[4], s[4];
+  __device__ __forceinline__ void of(const float* cos, const float* sin, bool there) {
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+      const uint4 none = make_uint4(0, 0, 0, 0);
+      const uint4 u = there ? __ldg(reinterpret_cast<const uint4*>(cos) + i / 2) : none, v = there ? __ldg(reinterpret_cast<const uint4*>(sin) + i / 2) : none;
+      c[i] = pk2(u.x, u.y); c[i + 1] = pk2(u.z, u.w);
+      s[i] = pk2(v.x, v.y); s[i + 1] = pk2(v.z, v.w);
+    }
   }
   // a' = a c - b s, b' = b c + a s of every pair; SIGN -1: back
   template <int SIGN>
-  __device__ __forceinline__ void turn(const float (&c)[8], const float (&s)[8], int interleaved) {
+  __device__ __forceinline__ void turn(Head16& h, int interleaved) const {
     if (interleaved) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float p = a[2 * i], q = a[2 * i + 1], u = b[2 * i], v = b[2 * i + 1];
-        a[2 * i] = p * c[i] - SIGN * q * s[i];
-        a[2 * i + 1] = q * c[i] + SIGN * p * s[i];
-        b[2 * i] = u * c[i + 4] - SIGN * v * s[i + 4];
-        b[2 * i + 1] = v * c[i + 4] + SIGN * u * s[i + 4];
+      for (int i = 0; i < 8; ++i) {                // the i-th pair goes by the i-th entry
+        const float ci = i & 1 ? hi2(c[i >> 1]) : lo2(c[i >> 1]), si = i & 1 ? hi2(s[i >> 1]) : lo2(s[i >> 1]);
+        h.x[i] = f2_fma(pk2f(hi2(h.x[i]), lo2(h.x[i])), pk2f(-SIGN * si, SIGN * si), f2_mul(h.x[i], pk2f(ci, ci)));
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float p = a[i], q = b[i];
-        a[i] = p * c[i] - SIGN * q * s[i];
-        b[i] = q * c[i] + SIGN * p * s[i];
+      for (int i = 0; i < 4; ++i) {
+        const uint64_t minus = s[i] ^ 0x8000000080000000ull, a = h.x[i], b = h.x[4 + i];
+        h.x[i] = f2_fma(b, SIGN > 0 ? minus : s[i], f2_mul(a, c[i]));
+        h.x[4 + i] = f2_fma(a, SIGN > 0 ? s[i] : minus, f2_mul(b, c[i]));
       }
     }
   }
@@ -74,15 +98,6 @@ __device__ __forceinline__ float group_sum(float v) {
 #pragma unroll
   for (int o = LANES / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
-}
-
-// 8 entries of a row of the tables.
-__device__ __forceinline__ void table8(const float* row, bool there, float (&c)[8]) {
-#pragma unroll
-  for (int e = 0; e < 8; e += 4) {
-    const float4 u = there ? __ldg(reinterpret_cast<const float4*>(row + e)) : make_float4(0.f, 0.f, 0.f, 0.f);
-    c[e] = u.x; c[e + 1] = u.y; c[e + 2] = u.z; c[e + 3] = u.w;
-  }
 }
 
 }  // namespace gf

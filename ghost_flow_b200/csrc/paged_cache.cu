@@ -159,10 +159,14 @@ __device__ __forceinline__ unsigned short e4m3x2(float lo, float hi) {
   return r;
 }
 // 8 numbers in a unit of `inv`^-1.
-__device__ __forceinline__ uint2 e4m3x8(const float (&f)[8], float inv) {
+__device__ __forceinline__ uint2 e4m3x8(const uint64_t* x, float inv) {
+  const uint64_t two = pk2f(inv, inv);
   unsigned short h[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) h[i] = e4m3x2(f[2 * i] * inv, f[2 * i + 1] * inv);
+  for (int i = 0; i < 4; ++i) {
+    const uint64_t y = f2_mul(x[i], two);
+    h[i] = e4m3x2(lo2(y), hi2(y));
+  }
   return make_uint2(h[0] | (unsigned)h[1] << 16, h[2] | (unsigned)h[3] << 16);
 }
 template <int LANES>
@@ -180,7 +184,7 @@ __device__ __forceinline__ unsigned scale_byte(Head16& v) {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
 #pragma unroll
-      for (unsigned u : {__float_as_uint(v.a[e]) & 0x7fffffffu, __float_as_uint(v.b[e]) & 0x7fffffffu}) m = max(m, finite && u >= INF ? 0 : u);
+      for (unsigned u : {(unsigned)v.x[e] & 0x7fffffffu, (unsigned)(v.x[e] >> 32) & 0x7fffffffu}) m = max(m, finite && u >= INF ? 0 : u);
     return group_max<LANES>(m);
   };
   unsigned m = largest(false);
@@ -188,8 +192,8 @@ __device__ __forceinline__ unsigned scale_byte(Head16& v) {
     m = largest(true);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      v.a[e] += v.a[e] - v.a[e];
-      v.b[e] += v.b[e] - v.b[e];
+      const float a = lo2(v.x[e]), b = hi2(v.x[e]);
+      v.x[e] = pk2f(a + (a - a), b + (b - b));
     }
   }
   // m = 1.f 2^(E - 127), 448 = 1.75 2^8
@@ -218,10 +222,9 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_heads_kernel(const __
   load(head0);
   PagedRow row;
   if (!paged_row(A.seqs, t, A.positions, row)) return;
-  float c[8], s[8];
+  HeadTurn turn;
   const long long off = (long long)row.pos * (p.rotary / 2) + at.t;
-  table8(A.cos + off, row.there && at.turns, c);
-  table8(A.sin + off, row.there && at.turns, s);
+  turn.of(A.cos + off, A.sin + off, row.there && at.turns);
   for (int base = 0; base < heads; base += PA_AHEAD * STEP) {              // (the same for all lanes of a warp)
     if (base) load(base + head0);
 #pragma unroll
@@ -237,14 +240,11 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_heads_kernel(const __
           Head16 w;
           const __nv_bfloat16* weight = query ? p.qw : p.kw;
           w.of(__ldg(reinterpret_cast<const uint4*>(weight + at.x)), __ldg(reinterpret_cast<const uint4*>(weight + at.y)));
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            v.a[e] *= r * w.a[e];
-            v.b[e] *= r * w.b[e];
-          }
+          v.scale(r);
+          v.scale(w);
         }
       }
-      if ((query || key) && at.turns) v.turn<1>(c, s, A.interleaved);
+      if ((query || key) && at.turns) turn.turn<1>(v, A.interleaved);
       unsigned byte = 0;
       if constexpr (BYTES) byte = scale_byte<LANES>(v);
       if (query) {
@@ -261,8 +261,8 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_heads_kernel(const __
       if constexpr (BYTES) {
         unsigned char* pool = reinterpret_cast<unsigned char*>(key ? A.kp : A.vp) + to;
         const float inv = __uint_as_float((254u - byte) << 23);
-        *reinterpret_cast<uint2*>(pool + at.x) = e4m3x8(v.a, inv);
-        *reinterpret_cast<uint2*>(pool + at.y) = e4m3x8(v.b, inv);
+        *reinterpret_cast<uint2*>(pool + at.x) = e4m3x8(v.x, inv);
+        *reinterpret_cast<uint2*>(pool + at.y) = e4m3x8(v.x + 4, inv);
         if (i == 0) (key ? p.kscales : p.vscales)[((row.page * A.Hk + hk) << A.seqs.page_shift) + row.r] = (unsigned char)byte;
       } else {
         __nv_bfloat16* pool = (key ? A.kp : A.vp) + to;
