@@ -224,23 +224,6 @@ __device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* m
       : "memory");
 }
 
-// 16 numbers of the cache times their row's power of two (twice, as f32x2), as bf16: exact
-__device__ __forceinline__ void bf16x16_of_e4m3(const uint4& in, uint64_t scale, uint4& lo, uint4& hi) {
-  const uint32_t* four = reinterpret_cast<const uint32_t*>(&in);
-  uint32_t out[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    uint32_t h;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((unsigned short)(i & 1 ? four[i >> 1] >> 16 : four[i >> 1])));
-    float a, b;
-    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, h;\n\t}" : "=f"(a), "=f"(b) : "r"(h));
-    const uint64_t x = f2_mul(pk2f(a, b), scale);
-    out[i] = pack_bf16x2(lo2(x), hi2(x));
-  }
-  lo = make_uint4(out[0], out[1], out[2], out[3]);
-  hi = make_uint4(out[4], out[5], out[6], out[7]);
-}
-
 template <int HD, bool BYTES>
 __global__ void __launch_bounds__(PgCfg<HD, BYTES>::THREADS, 1)
 paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,

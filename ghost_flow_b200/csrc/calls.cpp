@@ -268,8 +268,8 @@ PyObject* read(PyObject*, PyObject* const* a, Py_ssize_t n) {
   gf::PagedCall8 r{};
   View k;
   const bool bytes = a[6] != Py_None;
-  if (followed({a[1], a[2]}) || !k.of(a[1]) || T <= 0 || T > MOST || !pools(a[1], a[2], a[3], a[4], a[5], T, k.device, bytes, r.c) || r.c.D % 16 ||
-      r.c.D > 4096 || r.c.Hk > 65535 || (a[7] != Py_None) != bytes || (bytes && !scales(a[6], a[7], r.c, k.device, r.kscales, r.vscales)))
+  if (followed({a[1], a[2]}) || !k.of(a[1]) || T <= 0 || T > MOST || !pools(a[1], a[2], a[3], a[4], a[5], T, k.device, bytes, r.c) || r.c.D < 16 ||
+      (r.c.D & (r.c.D - 1)) || r.c.D > 4096 || r.c.Hk > 65535 || (a[7] != Py_None) != bytes || (bytes && !scales(a[6], a[7], r.c, k.device, r.kscales, r.vscales)))
     Py_RETURN_NONE;
   return Py_BuildValue("(y#iLL)", (const char*)&r, (Py_ssize_t)sizeof r, k.device, r.c.Hk, r.c.D);
 }

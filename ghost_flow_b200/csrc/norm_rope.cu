@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(NR_THREADS, BACK ? NR_BWD_CTAS : NR_CTAS) norm
   extern __shared__ uint4 ring[];                  // [stages][vectors][threads]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = lane / LANES, heads = p.H + (BACK ? 2 : 1) * p.Hk;
   if (BACK && threadIdx.x == 0) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const HeadLane at(lane % LANES, p.rotary, p.interleaved);
+  const HeadLane at(lane % LANES, LANES, p.rotary, p.interleaved);
   const uint32_t mine = smem_u32(ring + threadIdx.x);
   NrAt now, ahead;
   now.begin(p, blockIdx.x * NR_WARPS + warp, heads);
@@ -112,8 +112,8 @@ __global__ void __launch_bounds__(NR_THREADS, BACK ? NR_BWD_CTAS : NR_CTAS) norm
   bool begins = true;
   for (int st = 0; now.u < p.units; st = st + 1 == NR_STAGES ? 0 : st + 1) {
     if (begins) {
-      const long long off = (long long)(now.pos + p.pos0) * (p.rotary / 2) + at.t;
-      turn.of(p.cos + off, p.sin + off, at.turns);
+      const long long off = (long long)(now.pos + p.pos0) * (p.rotary / 2);
+      turn.of(p.cos + off, p.sin + off, at, true);
     }
     ask(st == 0 ? NR_STAGES - 1 : st - 1);
     asm volatile("cp.async.wait_group %0;" ::"n"(NR_STAGES - 1) : "memory");
@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(NR_THREADS, BACK ? NR_BWD_CTAS : NR_CTAS) norm
         v.scale(rsqrtf(group_sum<LANES>(v.dot(v)) * (1.f / D) + p.eps));
         v.scale(w);
       }
-      if (at.turns) turn.turn<1>(v, p.interleaved);
+      turn.turn<1>(v, at, p.interleaved);
       v.to(x, y);
       if (there) {
         __nv_bfloat16* to = query ? p.q + ((unsigned long long)now.t * p.H + h) * D : p.k + ((unsigned long long)now.t * p.Hk + h - p.H) * D;
@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(NR_THREADS, BACK ? NR_BWD_CTAS : NR_CTAS) norm
       y = there ? in[3 * NR_THREADS] : none;
       Head16 g;
       g.of(x, y);
-      if (at.turns) turn.turn<-1>(g, p.interleaved);
+      turn.turn<-1>(g, at, p.interleaved);
       if (p.qw) {
         v.of(normed ? in[0] : none, normed ? in[NR_THREADS] : none);
         const float r = rsqrtf(group_sum<LANES>(v.dot(v)) * (1.f / D) + p.eps);
@@ -219,13 +219,13 @@ __global__ void __launch_bounds__(1024) norm_rope_fold_kernel(const float* part,
   }
 }
 
-// Units of a token: parts of its heads. A dozen for every warp, as those with one more than others are waited for, but of two rounds each at least (a unit's rows of the
+// Units of a token: parts of its heads. A dozen for every warp, as those with one more than others are waited for, but of four rounds each at least (a unit's rows of the
 // tables are not on their way before it begins) unless there are fewer units than warps.
 static void nr_cut(NormRope& p, long long T, int heads, int lanes, int ctas) {
   const int groups = 32 / lanes;
   const long long rounds = (heads + groups - 1) / groups, warps = (long long)sm_count() * ctas * NR_WARPS;
-  const long long room = 0x7fffffffll / T, many = (12 * warps + T - 1) / T, few = (warps + T - 1) / T, two = (rounds + 1) / 2;
-  const long long wanted = many < two ? many : few > two ? few : two, want = wanted < room ? wanted : room;
+  const long long room = 0x7fffffffll / T, many = (12 * warps + T - 1) / T, few = (warps + T - 1) / T, four = (rounds + 3) / 4;
+  const long long wanted = many < four ? many : few > four ? few : four, want = wanted < room ? wanted : room;
   p.chunks = (int)(want < 1 ? 1 : want < rounds ? want : rounds);
   p.per = (int)((rounds + p.chunks - 1) / p.chunks) * groups;
   p.chunks = (heads + p.per - 1) / p.per;

@@ -1,7 +1,8 @@
 // A row of a head in a group of D / 16 lanes: RMS norm and rotation of its first `rotary` dims.
 //
-// A lane has 16 numbers, two vectors of 8, chosen so that both numbers of every pair are its own: with halves apart lane i of the first rotary / 16 has dims
-// 8 i .. and rotary / 2 + 8 i .., with pairs side by side 16 i ..; lanes behind those have the dims that are not rotated.
+// A lane has 16 numbers, two vectors of 8, chosen so that both numbers of every pair are its own and neighbouring lanes' vectors are neighbours: with halves apart lane
+// i of the first n = rotary / 16 has dims 8 i .. and rotary / 2 + 8 i .., the m behind them, which are not rotated, vectors i - n and i - n + m of the rest;
+// with pairs side by side all have vectors i and i + D / 16. (Two vectors next to each other, 16 i .., fill half of every 32 bytes with an access: 28 us for 21.)
 #pragma once
 #include "gf_ptx.cuh"
 
@@ -9,14 +10,24 @@ namespace gf {
 
 struct HeadLane {
   int x, y;                      // first dims of the two vectors
-  int t;                         // first entry in a row of the tables
-  bool turns;
-  __device__ __forceinline__ HeadLane(int i, int rotary, int interleaved) {
-    turns = 16 * i < rotary;
-    t = 8 * i;
-    const bool apart = turns && !interleaved;
-    x = apart ? 8 * i : 16 * i;
-    y = apart ? rotary / 2 + 8 * i : 16 * i + 8;
+  int t0, t1;                    // entries in a row of the tables: four from here, and four from there
+  bool turns0, turns1;           // the vectors that those turn; with halves apart both together
+  __device__ __forceinline__ HeadLane(int i, int lanes, int rotary, int interleaved) {
+    const int n = rotary / 16, m = lanes - n;
+    if (interleaved) {
+      x = 8 * i;
+      y = 8 * (i + lanes);
+      turns0 = x < rotary;
+      turns1 = y < rotary;
+      t0 = x / 2;
+      t1 = y / 2;
+    } else {
+      turns0 = turns1 = i < n;
+      x = i < n ? 8 * i : rotary + 8 * (i - n);
+      y = i < n ? rotary / 2 + 8 * i : rotary + 8 * (i - n + m);
+      t0 = 8 * i;
+      t1 = 8 * i + 4;
+    }
   }
 };
 
@@ -63,25 +74,29 @@ struct Head16 {
 // A lane's 8 entries of a row of the tables, and the turn by them.
 struct HeadTurn {
   uint64_t c[4], s[4];
-  __device__ __forceinline__ void of(const float* cos, const float* sin, bool there) {
+  __device__ __forceinline__ void of(const float* cos, const float* sin, const HeadLane& at, bool there) {
 #pragma unroll
-    for (int i = 0; i < 4; i += 2) {
+    for (int i = 0; i < 2; ++i) {
+      const bool turns = there && (i ? at.turns1 : at.turns0);
+      const int t = i ? at.t1 : at.t0;
       const uint4 none = make_uint4(0, 0, 0, 0);
-      const uint4 u = there ? __ldg(reinterpret_cast<const uint4*>(cos) + i / 2) : none, v = there ? __ldg(reinterpret_cast<const uint4*>(sin) + i / 2) : none;
-      c[i] = pk2(u.x, u.y); c[i + 1] = pk2(u.z, u.w);
-      s[i] = pk2(v.x, v.y); s[i + 1] = pk2(v.z, v.w);
+      const uint4 u = turns ? __ldg(reinterpret_cast<const uint4*>(cos + t)) : none, v = turns ? __ldg(reinterpret_cast<const uint4*>(sin + t)) : none;
+      c[2 * i] = pk2(u.x, u.y); c[2 * i + 1] = pk2(u.z, u.w);
+      s[2 * i] = pk2(v.x, v.y); s[2 * i + 1] = pk2(v.z, v.w);
     }
   }
   // a' = a c - b s, b' = b c + a s of every pair; SIGN -1: back
   template <int SIGN>
-  __device__ __forceinline__ void turn(Head16& h, int interleaved) const {
+  __device__ __forceinline__ void turn(Head16& h, const HeadLane& at, int interleaved) const {
     if (interleaved) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {                // the i-th pair goes by the i-th entry
+        if (!(i < 4 ? at.turns0 : at.turns1)) continue;
         const float ci = i & 1 ? hi2(c[i >> 1]) : lo2(c[i >> 1]), si = i & 1 ? hi2(s[i >> 1]) : lo2(s[i >> 1]);
-        h.x[i] = f2_fma(pk2f(hi2(h.x[i]), lo2(h.x[i])), pk2f(-SIGN * si, SIGN * si), f2_mul(h.x[i], pk2f(ci, ci)));
+        const float a = lo2(h.x[i]), b = hi2(h.x[i]);          // (as pairs of their own they would have to be moved first)
+        h.x[i] = pk2f(a * ci - SIGN * b * si, b * ci + SIGN * a * si);
       }
-    } else {
+    } else if (at.turns0) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint64_t minus = s[i] ^ 0x8000000080000000ull, a = h.x[i], b = h.x[4 + i];

@@ -179,33 +179,30 @@ __device__ __forceinline__ unsigned group_max(unsigned v) {
 template <int LANES>
 __device__ __forceinline__ unsigned scale_byte(Head16& v) {
   constexpr unsigned INF = 0x7f800000u;
-  auto largest = [&](bool finite) {
-    unsigned m = 0;
+  float most = 0.f;                                // (what is not a number is passed over, and stays so in the conversion)
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-#pragma unroll
-      for (unsigned u : {(unsigned)v.x[e] & 0x7fffffffu, (unsigned)(v.x[e] >> 32) & 0x7fffffffu}) m = max(m, finite && u >= INF ? 0 : u);
-    return group_max<LANES>(m);
-  };
-  unsigned m = largest(false);
+  for (int e = 0; e < 8; ++e) most = fmaxf(most, fmaxf(fabsf(lo2(v.x[e])), fabsf(hi2(v.x[e]))));
+  unsigned m = group_max<LANES>(__float_as_uint(most));
   if (__any_sync(0xffffffffu, m >= INF)) {
-    m = largest(true);
+    most = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float a = lo2(v.x[e]), b = hi2(v.x[e]);
       v.x[e] = pk2f(a + (a - a), b + (b - b));
+      most = fmaxf(most, fmaxf(fabsf(lo2(v.x[e])), fabsf(hi2(v.x[e]))));
     }
+    m = group_max<LANES>(__float_as_uint(most));
   }
   // m = 1.f 2^(E - 127), 448 = 1.75 2^8
   return (unsigned)max(1, (int)(m >> 23) - 8 + ((m & 0x7fffffu) > 0x600000u));
 }
 
 template <int LANES, bool BYTES>
-__global__ void __launch_bounds__(PA_THREADS) paged_append_heads_kernel(const __grid_constant__ PagedHeads p) {
+__global__ void __launch_bounds__(PA_THREADS, 3) paged_append_heads_kernel(const __grid_constant__ PagedHeads p) {
   constexpr int D = 16 * LANES, STEP = PA_THREADS / LANES;
   const PagedAppend& A = p.a;
   const int t = blockIdx.x, head0 = threadIdx.x / LANES, i = threadIdx.x % LANES, heads = A.H + 2 * A.Hk;
-  const HeadLane at(i, p.rotary, A.interleaved);
+  const HeadLane at(i, LANES, p.rotary, A.interleaved);
   const __nv_bfloat16* from = A.qkv + (long long)t * A.ldx;
   uint4 x[PA_AHEAD], y[PA_AHEAD];
   auto load = [&](int h0) {
@@ -223,8 +220,8 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_heads_kernel(const __
   PagedRow row;
   if (!paged_row(A.seqs, t, A.positions, row)) return;
   HeadTurn turn;
-  const long long off = (long long)row.pos * (p.rotary / 2) + at.t;
-  turn.of(A.cos + off, A.sin + off, row.there && at.turns);
+  const long long off = (long long)row.pos * (p.rotary / 2);
+  turn.of(A.cos + off, A.sin + off, at, row.there);
   for (int base = 0; base < heads; base += PA_AHEAD * STEP) {              // (the same for all lanes of a warp)
     if (base) load(base + head0);
 #pragma unroll
@@ -244,7 +241,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_heads_kernel(const __
           v.scale(w);
         }
       }
-      if ((query || key) && at.turns) turn.turn<1>(v, A.interleaved);
+      if (query || key) turn.turn<1>(v, at, A.interleaved);
       unsigned byte = 0;
       if constexpr (BYTES) byte = scale_byte<LANES>(v);
       if (query) {
@@ -280,24 +277,16 @@ struct PagedRead {
   const unsigned char *kscales, *vscales;
   __nv_bfloat16 *k, *v;          // [T, Hk, D] dense
   long long kpage, krow, khead, vpage, vrow, vhead;
-  int Hk, D;
+  int Hk, D, shift;              // D = 16 << shift
 };
-
-__device__ __forceinline__ uint32_t bf16x2_of_e4m3(unsigned short two, float scale) {
-  uint32_t h;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(two));
-  float lo, hi;
-  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, h;\n\t}" : "=f"(lo), "=f"(hi) : "r"(h));
-  return pack_bf16x2(lo * scale, hi * scale);
-}
 
 template <bool BYTES>
 __global__ void __launch_bounds__(PA_THREADS) paged_read_kernel(const __grid_constant__ PagedRead p) {
-  const int t = blockIdx.x, per = p.D / 16, all = 2 * p.Hk * per;
+  const int t = blockIdx.x, all = 2 * p.Hk << p.shift;
   PagedRow row{};
   if (!paged_row(p.seqs, t, 0x7fffffff, row)) row.stored = false;
   for (int id = threadIdx.x; id < all; id += PA_THREADS) {
-    const int i = id % per, head = id / per;
+    const int i = id & ((1 << p.shift) - 1), head = id >> p.shift;
     const bool key = head < p.Hk;
     const int hk = key ? head : head - p.Hk;
     const long long from = key ? row.page * p.kpage + row.r * p.krow + hk * p.khead : row.page * p.vpage + row.r * p.vrow + hk * p.vhead;
@@ -306,11 +295,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_read_kernel(const __grid_con
       if constexpr (BYTES) {
         const uint4 in = *reinterpret_cast<const uint4*>((const unsigned char*)(key ? p.kp : p.vp) + from + 16 * i);
         const unsigned byte = (key ? p.kscales : p.vscales)[((row.page * p.Hk + hk) << p.seqs.page_shift) + row.r];
-        const float scale = __uint_as_float(byte << 23);
-        const unsigned short* two = reinterpret_cast<const unsigned short*>(&in);
-        uint32_t* u = reinterpret_cast<uint32_t*>(x);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) u[e] = bf16x2_of_e4m3(two[e], scale);
+        bf16x16_of_e4m3(in, pk2(byte << 23, byte << 23), x[0], x[1]);
       } else {
         const uint4* in = reinterpret_cast<const uint4*>((const __nv_bfloat16*)(key ? p.kp : p.vp) + from + 16 * i);
         x[0] = in[0];
@@ -400,7 +385,7 @@ GF_API int gf_paged_read(const PagedCall8* c8, void* k, void* v, void* stream) {
   PagedCall c = c8->c;
   c.x = c.y = k;
   c.ldx = c.ldy = 0;
-  if (!paged_batch(p.seqs, c) || !c8->kscales != !c8->vscales || (c8->kscales && !paged_scales(*c8)) || c.Hk <= 0 || c.Hk > 65535 || c.D < 16 || c.D % 16 ||
+  if (!paged_batch(p.seqs, c) || !c8->kscales != !c8->vscales || (c8->kscales && !paged_scales(*c8)) || c.Hk <= 0 || c.Hk > 65535 || c.D < 16 || (c.D & (c.D - 1)) ||
       c.D > 4096)
     return GFH_BAD_ARG;
   gf::enter();
@@ -408,7 +393,7 @@ GF_API int gf_paged_read(const PagedCall8* c8, void* k, void* v, void* stream) {
   p.k = (__nv_bfloat16*)k; p.v = (__nv_bfloat16*)v;
   p.kpage = c.strides[0]; p.krow = c.strides[1]; p.khead = c.strides[2];
   p.vpage = c.strides[3]; p.vrow = c.strides[4]; p.vhead = c.strides[5];
-  p.Hk = (int)c.Hk; p.D = (int)c.D;
+  p.Hk = (int)c.Hk; p.D = (int)c.D; p.shift = __builtin_ctz((unsigned)c.D) - 4;
   auto kern = c8->kscales ? paged_read_kernel<true> : paged_read_kernel<false>;
   kern<<<p.seqs.T, PA_THREADS, 0, (cudaStream_t)stream>>>(p);
   return cudaGetLastError() == cudaSuccess ? GFH_OK : GFH_CUDA;

@@ -141,7 +141,7 @@ def test_the_entry_points_refuse_before_they_launch():
     assert heads(None) == -1
     for n in "kp vp ks vs".split():                          # x among what is written
         assert heads(call(**{n: P + 2 * 2560 - 16})) == -5
-    for kw in (*pools, dict(D=8), dict(D=40), dict(D=8192)):
+    for kw in (*pools, dict(D=8), dict(D=40), dict(D=80), dict(D=8192)):
         assert lib.gf_paged_read(call(**kw), P, P, None) == -1, kw
     assert lib.gf_paged_read(None, P, P, None) == lib.gf_paged_read(call(), None, P, None) == lib.gf_paged_read(call(), P, P + 8, None) == -1
     for kw in (*pools, dict(ks=0), dict(ks=0, vs=0), dict(D=96), dict(H=5), dict(pages=0)):
