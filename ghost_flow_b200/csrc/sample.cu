@@ -12,12 +12,17 @@
 // neighbour (a vocabulary of 50257 has that many borders, each off by some 2^-25). A weight below the last bit counts as one of it: u = 0 still takes the
 // first token that stays.
 //
-// One CTA has a row, and reads it from L2 in every pass but the first: the largest entry; a histogram over bins of equal width of m - x, which says in which bin the k-th
+// One CTA has a row, or a cluster of them where there are few, and reads it from L2 in every pass but the first: the largest entry; a histogram over bins of equal width of m - x, which says in which bin the k-th
 // entry lies, or about where the share p ends; then, with top-k, all entries up to that bin go to shared memory, are put in order there, and the rest is done
 // among them. Without it a pass adds up the weights: all, those in front of the bins around the place where the share may end, the latter by 32 parts of
 // the vocabulary too, and leaves the entries of those bins in shared memory, among which the last one that stays is found. u then tells the part, and the
 // token in it. What does not fit (more than 1024 entries, as with equal ones) takes as many histograms as it wants, by weights and then by the entries' bits, and
 // entries that are all equal are counted off in the order of the vocabulary.
+//
+// What bounds it: the instructions of an entry's weight (a table of 16 powers and a series, 64 bits), of its bin and its atomic addition, not the 6.6 TB/s that
+// the first pass reaches. 512 rows of 50257 in bf16, of which memory wants 8 us: the likeliest 17 us, weights of all 59, k = 50 48, p = 0.9 126, p of the least
+// 35; 32 bits, 16 us: 22, 55, 50, 109, 31. 64 rows in bf16: 6, 19, 18, 38, 15; 3 rows of 32000: 5, 12, 14, 26, 12.
+#include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
 #include "calls.h"
@@ -46,6 +51,7 @@ struct SampleParams {
 
 constexpr int SM_LIST = 1024;    // entries that are ordered in shared memory
 constexpr int SM_PARTS = 32;     // of the vocabulary, whose sums lead to the token
+constexpr int SM_RANKS = 8;      // CTAs of a row
 
 struct SampleShared {
   unsigned bin[2][SM_BINS];        // low and high words of sums; or numbers, and how many there are in front
@@ -57,7 +63,12 @@ struct SampleShared {
   int n, first;
   u64 cut, above, total;
   unsigned critical;
-  int b1;
+  int b0, b1;
+  // of every CTA that has a part of the row: its largest entry, some entries' sum and number, and sums of weights
+  float most[SM_RANKS], sum[SM_RANKS];
+  int numbers[SM_RANKS];
+  u64 everything[SM_RANKS], in_front[SM_RANKS];
+  u64 own[32];                   // of this CTA's warps
 };
 
 __device__ __forceinline__ float sm_f(float x) { return x; }
@@ -115,11 +126,17 @@ __device__ __forceinline__ u64 sm_before(u64 v, u64* part, u64& all) {
   return before + in_warp;
 }
 
+// The CTAs of a row: all of them meet, and the shared memory of another one.
+__device__ __forceinline__ void sm_meet() { cooperative_groups::this_cluster().sync(); }
+__device__ __forceinline__ SampleShared& sm_of(SampleShared& s, int rank) { return *cooperative_groups::this_cluster().map_shared_rank(&s, rank); }
+
 template <typename T, int THREADS>
 struct SampleRow {
   static constexpr int VEC = 16 / sizeof(T);
   const T* x;
   int V, head, vectors;          // whole vectors from entry `head` on, on 16-byte boundaries; the few entries around them are threads' own
+  int per_part;                  // vectors of a part; what is in front of them is the first part's, what is behind the last one's
+  int part0, part1;              // parts of this CTA
   float m, per_bin;
   double per16;                  // 16 log2(e) / T
   float low, zero;               // entries from which on weights are 2^-48 of the largest, and nothing
@@ -133,6 +150,18 @@ struct SampleRow {
     V = V_;
     head = min((int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) % 16 / sizeof(T)), V);
     vectors = (V - head) / VEC;
+    per_part = (vectors + SM_PARTS - 1) / SM_PARTS;
+  }
+  __device__ __forceinline__ void share(int rank, int ranks) {
+    part0 = rank * (SM_PARTS / ranks);
+    part1 = part0 + SM_PARTS / ranks;
+  }
+  static constexpr bool ALONE = THREADS < 1024;    // a smaller CTA has the whole row always
+  __device__ __forceinline__ int first() const { return ALONE ? 0 : min(part0 * per_part, vectors); }
+  __device__ __forceinline__ int end() const { return ALONE ? vectors : min(part1 * per_part, vectors); }
+  __device__ __forceinline__ int part_of(int v) const {
+    const int i = (v - head) / VEC;
+    return v < head ? 0 : i >= vectors ? SM_PARTS - 1 : (int)((unsigned)i / (unsigned)per_part);
   }
   __device__ __forceinline__ int edges() const { return V - vectors * VEC; }
   __device__ __forceinline__ int edge(int i) const { return i < head ? i : i + vectors * VEC; }
@@ -176,11 +205,48 @@ struct SampleRow {
       }
     }
   }
-  // ... for all entries
+  // ... for all entries of this CTA
   template <int TOGETHER, typename F>
   __device__ __forceinline__ void each(F f) const {
-    range<TOGETHER>(threadIdx.x, THREADS, vectors, f);
-    if ((int)threadIdx.x < edges()) one(edge(threadIdx.x), f);
+    range<TOGETHER>(first() + threadIdx.x, THREADS, end(), f);
+    if ((int)threadIdx.x < edges() && (ALONE || ((int)threadIdx.x < head ? part0 == 0 : part1 == SM_PARTS))) one(edge(threadIdx.x), f);
+  }
+  // ... for those of a part, of which `warps` have as many each
+  template <typename F>
+  __device__ __forceinline__ void of_part(int part, int warp, int warps, F f) const {
+    const int lane = threadIdx.x & 31;
+    range<1>(part * per_part + warp * 32 + lane, 32 * warps, min((part + 1) * per_part, vectors), f);
+    if (warp) return;
+    if (part == 0 && lane < head) one(lane, f);
+    if (part == SM_PARTS - 1 && head + lane < edges()) one(edge(head + lane), f);
+  }
+  // Whole CTA: the sums of what `f` adds to `mine`, of each of its parts, into `to`. Behind the next barrier.
+  template <typename F>
+  __device__ __forceinline__ void sums(SampleShared& s, SampleShared& to, u64& mine, F f) const {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, parts = part1 - part0;
+    if (!ALONE && parts < SM_PARTS) {              // a cluster's CTA: several warps to a part
+      const int warps = THREADS / 32 / parts;
+      mine = 0;
+      of_part(part0 + warp / warps, warp % warps, warps, f);
+      mine = sm_warp_sum(mine);
+      if (lane == 0) s.own[warp] = mine;
+      __syncthreads();
+      if ((int)threadIdx.x >= parts) return;
+      mine = 0;
+      for (int i = 0; i < warps; ++i) mine += s.own[threadIdx.x * warps + i];
+      to.kept[0][part0 + threadIdx.x] = (unsigned)mine;
+      to.kept[1][part0 + threadIdx.x] = (unsigned)(mine >> 32);
+      return;
+    }
+    for (int part = warp; part < SM_PARTS; part += THREADS / 32) {
+      mine = 0;
+      of_part(part, 0, 1, f);
+      mine = sm_warp_sum(mine);
+      if (lane == 0) {
+        to.kept[0][part] = (unsigned)mine;
+        to.kept[1][part] = (unsigned)(mine >> 32);
+      }
+    }
   }
   // bins of equal width, the further from the largest entry the higher
   __device__ __forceinline__ int bin(float a) const {
@@ -386,9 +452,10 @@ struct SamplePart {
 };
 static_assert(SM_PARTS == 32, "a lane has a part");
 
-// Numbers of entries in every bin, and of those in front; the last bin, which reaches to the least entry, is not counted.
-template <typename T, int THREADS>
-__device__ void sm_count(const SampleRow<T, THREADS>& row, SampleShared& s) {
+// Numbers of entries in every bin, and of those in front; the last bin, which reaches to the least entry, is not counted. In the first CTA of the row; the
+// others have their own, and stay until the next barrier of all.
+template <bool MANY, typename T, int THREADS>
+__device__ void sm_count(const SampleRow<T, THREADS>& row, SampleShared& s, int rank, int ranks) {
   constexpr int OWN = SM_BINS / THREADS;
   const int tid = threadIdx.x;
   for (int i = tid; i < SM_BINS; i += THREADS) s.bin[0][i] = 0;
@@ -400,14 +467,23 @@ __device__ void sm_count(const SampleRow<T, THREADS>& row, SampleShared& s) {
       if (b < SM_BINS - 1) atomicAdd(&s.bin[0][b], 1u);
     }
   });
-  __syncthreads();
+  if (MANY && ranks > 1) sm_meet();
+  else __syncthreads();
+  if (MANY && rank) return;
   unsigned own[OWN], sum = 0;
 #pragma unroll
-  for (int i = 0; i < OWN; ++i) sum += own[i] = s.bin[0][tid * OWN + i];
+  for (int i = 0; i < OWN; ++i) own[i] = s.bin[0][tid * OWN + i];
+  for (int r = 1; MANY && r < ranks; ++r) {
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) own[i] += sm_of(s, r).bin[0][tid * OWN + i];
+  }
+#pragma unroll
+  for (int i = 0; i < OWN; ++i) sum += own[i];
   u64 all;
   unsigned before = (unsigned)sm_before<THREADS>(sum, s.part, all);
 #pragma unroll
   for (int i = 0; i < OWN; ++i) {
+    s.bin[0][tid * OWN + i] = own[i];
     s.bin[1][tid * OWN + i] = before;
     before += own[i];
   }
@@ -417,7 +493,7 @@ __device__ void sm_count(const SampleRow<T, THREADS>& row, SampleShared& s) {
 // An entry of bins b0 .. b1, which have at most SM_LIST, into the list behind those of the bins in front.
 template <typename T, int THREADS>
 __device__ __forceinline__ void sm_keep(const SampleRow<T, THREADS>& row, SampleShared& s, float a, int v, int bin, int b0) {
-  s.entry[s.bin[1][bin] - s.bin[1][b0] + atomicSub(&s.bin[0][bin], 1u) - 1] = sm_entry(a, v);
+  s.entry[s.bin[1][bin] - s.bin[1][b0] + atomicSub(&s.bin[0][bin], 1u) - 1] = sm_entry(a, v);        // (s: the first CTA's)
 }
 // Whole CTA: the list's n entries, from bin b0 on, in their order: an entry is compared with those of its bin.
 template <typename T, int THREADS>
@@ -450,21 +526,31 @@ __device__ int sm_first(const SampleRow<T, THREADS>& row, SampleShared& s, F f) 
   return s.first == 0x7fffffff ? -1 : s.first;
 }
 
-template <typename T, int THREADS>
+// A row has one CTA, or, where there are SMs for it, a cluster of them, each with as many of the row's parts: those help the first one with the passes over the
+// row, leave what they find in its shared memory, and are done; what follows, and what is seldom wanted, is the first one's alone. They meet (sm_meet) as often
+// as each other: what they go by is the same for all of them.
+template <typename T, int THREADS, bool MANY>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const __grid_constant__ SampleParams p) {
   constexpr int WARPS = THREADS / 32;
   using Row = SampleRow<T, THREADS>;
   __shared__ SampleShared s;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const long long b = blockIdx.x;
+  int rank = 0, ranks = 1;
+  if (MANY) {
+    rank = (int)cooperative_groups::this_cluster().block_rank();
+    ranks = (int)cooperative_groups::this_cluster().num_blocks();
+    cooperative_groups::this_cluster().barrier_arrive();
+  }
+  const long long b = blockIdx.x / ranks;
   Row row(p);
   row.begin((const T*)p.x + b * p.ldx, p.V);
+  row.share(rank, ranks);
   const float temperature = p.temperature ? p.temperature[b] : p.temperature0;
   const float top_p = p.top_p ? p.top_p[b] : p.top_p0;
   const float min_p = fminf(p.min_p ? p.min_p[b] : p.min_p0, 1.f);
   const int top_k = p.top_k ? p.top_k[b] : p.top_k0;
   const float u = fminf(fmaxf(p.u[b], 0.f), 0x1.fffffep-1f);
-  if (tid < 16) s.power[tid] = exp2(tid / 16.0) * (double)(1ull << p.bits);
+  if (warp == WARPS - 1 && lane < 16) s.power[lane] = exp2(lane / 16.0) * (double)(1ull << p.bits);
 
   // ---- the largest entry, and the mean of some that are numbers
   float most = -INFINITY, sum = 0.f;
@@ -473,7 +559,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const _
 #pragma unroll
     for (int j = 0; j < (int)(sizeof(a) / sizeof(float)); ++j) most = sm_max(most, a[j]);
   });
-  if (tid < row.vectors) row.vector(row.raw(tid), tid, [&](auto& a, int) {
+  if (row.first() + tid < row.end()) row.vector(row.raw(row.first() + tid), row.first() + tid, [&](auto& a, int) {
 #pragma unroll
     for (int j = 0; j < (int)(sizeof(a) / sizeof(float)); ++j) {
       const bool number = fabsf(a[j]) < 0x1p100f;
@@ -502,8 +588,27 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const _
     sum += f[WARPS + i];
     numbers += n[i];
   }
+  if (MANY) {
+    cooperative_groups::this_cluster().barrier_wait();               // (all of them run)
+    if (tid < ranks) {
+      SampleShared& to = sm_of(s, tid);
+      to.most[rank] = most;
+      to.sum[rank] = sum;
+      to.numbers[rank] = numbers;
+    }
+    sm_meet();
+    most = -INFINITY, sum = 0.f, numbers = 0;
+    for (int i = 0; i < ranks; ++i) {
+      most = sm_max(most, s.most[i]);
+      sum += s.sum[i];
+      numbers += s.numbers[i];
+    }
+  }
+  SampleShared& s0 = MANY ? sm_of(s, 0) : s;          // the first CTA's
   // ---- rows without probabilities, and those whose likeliest entry is asked for
   if (!(fabsf(most) < INFINITY) || !(temperature > 0.f) || top_k == 1 || top_p <= 0.f) {
+    if (MANY && rank) return;
+    row.share(0, 1);
     const bool none = most != most;
     const int v = most == -INFINITY ? -1 : sm_first(row, s, [&](float a) { return none ? a != a : a == most; });
     if (tid == 0) p.out[b] = v;
@@ -521,31 +626,33 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const _
   __syncthreads();
 
   u64 cut = 0;
-  const int per_part = (row.vectors + SM_PARTS - 1) / SM_PARTS;          // vectors; what is in front of them is the first part's, what is behind the last one's
-  auto part_of = [&](int v) {
-    const int i = (v - row.head) / Row::VEC;
-    return v < row.head ? 0 : i >= row.vectors ? SM_PARTS - 1 : (int)((unsigned)i / (unsigned)per_part);
-  };
   const float least_p = row.least(min_p, temperature);
   if (top_k > 0 && top_k < p.V) {
     row.per_bin = per * (4.f / 3.f);
-    sm_count(row, s);
-    // ---- the bin that the k-th entry lies in
-    for (int i = tid; i < SM_BINS - 1; i += THREADS)
-      if (s.bin[1][i] < (unsigned)top_k && s.bin[1][i + 1] >= (unsigned)top_k) s.b1 = i;
-    if (tid < SM_PARTS) s.kept[0][tid] = s.kept[1][tid] = 0;
-    if (tid == 0 && s.bin[1][SM_BINS - 1] < (unsigned)top_k) s.b1 = SM_BINS - 1;
-    __syncthreads();
-    const int b1 = s.b1, n = b1 < SM_BINS - 1 ? (int)s.bin[1][b1 + 1] : SM_LIST + 1;
-    if (n <= SM_LIST) {
+    sm_count<MANY>(row, s, rank, ranks);
+    // ---- the bin that the k-th entry lies in; -1 where there are more entries up to it than the list has room for
+    if (rank == 0) {
+      if (tid == 0) s.b1 = -1;
+      if (tid < SM_PARTS) s.kept[0][tid] = s.kept[1][tid] = 0;
+      __syncthreads();
+      for (int i = tid; i < SM_BINS - 1; i += THREADS)
+        if (s.bin[1][i] < (unsigned)top_k && s.bin[1][i + 1] >= (unsigned)top_k && s.bin[1][i + 1] <= SM_LIST) s.b1 = i;
+    }
+    if (MANY && ranks > 1) sm_meet();
+    else __syncthreads();
+    const int b1 = s0.b1;
+    if (b1 >= 0) {
       // ---- all of them into the list; the rest happens there
       row.template each<2>([&](auto& a, int v0) {
 #pragma unroll
         for (int j = 0; j < (int)(sizeof(a) / sizeof(float)); ++j) {
           const int bin = row.bin(a[j]);
-          if (bin <= b1) sm_keep(row, s, a[j], v0 + j, bin, 0);
+          if (bin <= b1) sm_keep(row, s0, a[j], v0 + j, bin, 0);
         }
       });
+      if (MANY && ranks > 1) sm_meet();
+      if (MANY && rank) return;
+      const int n = (int)s.bin[1][b1 + 1];
       sm_sort(row, s, n, 0);
       constexpr int OWN = SM_LIST / THREADS;       // a thread's entries, next to each other
       u64 e[OWN], w[OWN], sum = 0, total;
@@ -567,7 +674,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const _
           w[i] = 0;
           continue;
         }
-        const int part = part_of(sm_index(e[i]));
+        const int part = row.part_of(sm_index(e[i]));
         const unsigned low = (unsigned)w[i], old = atomicAdd(&s.kept[0][part], low), high = (unsigned)(w[i] >> 32) + (old + low < old);
         if (high) atomicAdd(&s.kept[1][part], high);
       }
@@ -577,7 +684,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const _
       // ---- the part's own: each is compared with all of them
 #pragma unroll
       for (int i = 0; i < OWN; ++i) {
-        if (w[i] == 0 || part_of(sm_index(e[i])) != at.part) continue;
+        if (w[i] == 0 || row.part_of(sm_index(e[i])) != at.part) continue;
         const int to = atomicAdd(&s.n, 1);
         s.entry[to] = e[i];
         s.sorted[to] = w[i];
@@ -591,6 +698,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const _
       }
       return;
     }
+    if (MANY && ranks > 1) sm_meet();                      // (its shared memory has been read)
+    if (MANY && rank) return;
+    row.share(0, 1);
+    ranks = 1;
     cut = sm_cut<false>(row, s, 0, (double)top_k);
     __syncthreads();
   }
@@ -600,35 +711,48 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const _
     row.per_bin = per * 0.5f;
     if (cut == 0) {
       // ---- by the bins' numbers and middles, about where the share ends
-      sm_count(row, s);
-      constexpr int OWN = SM_BINS / THREADS;
-      float own[OWN], sum = 0.f;
+      sm_count<MANY>(row, s, rank, ranks);
+      if (rank == 0) {
+        constexpr int OWN = SM_BINS / THREADS;
+        float own[OWN], sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < OWN; ++i) {
-        const int at = tid * OWN + i;
-        const float middle = row.m - at / row.per_bin;
-        own[i] = at < SM_BINS - 1 ? (float)(s.bin[1][at + 1] - s.bin[1][at]) * exp2f((middle - row.m) * (float)(row.per16 / 16.0)) : 0.f;
-        sum += own[i];
-      }
-      // (as whole numbers, of which the scan is)
-      u64 all, before = sm_before<THREADS>((u64)(sum * 0x1p20f), s.part, all);
-      const u64 target = (u64)((double)top_p * (double)all);
-      if (tid == 0) s.critical = 0;
-      __syncthreads();
+        for (int i = 0; i < OWN; ++i) {
+          const int at = tid * OWN + i;
+          const float middle = row.m - at / row.per_bin;
+          own[i] = at < SM_BINS - 1 ? (float)(s.bin[1][at + 1] - s.bin[1][at]) * exp2f((middle - row.m) * (float)(row.per16 / 16.0)) : 0.f;
+          sum += own[i];
+        }
+        // (as whole numbers, of which the scan is)
+        u64 all, before = sm_before<THREADS>((u64)(sum * 0x1p20f), s.part, all);
+        const u64 target = (u64)((double)top_p * (double)all);
+        if (tid == 0) s.critical = 0;
+        __syncthreads();
 #pragma unroll
-      for (int i = 0; i < OWN; ++i) {
-        const u64 upto = before + (u64)(own[i] * 0x1p20f);
-        if (before <= target && target < upto) s.critical = tid * OWN + i;
-        before = upto;
+        for (int i = 0; i < OWN; ++i) {
+          const u64 upto = before + (u64)(own[i] * 0x1p20f);
+          if (before <= target && target < upto) s.critical = tid * OWN + i;
+          before = upto;
+        }
+        __syncthreads();
+        // as many of them around it as there is room for, 31 on both sides at most (it is hardly ever that far off)
+        const int about = min((int)s.critical, SM_BINS - 2), b0_ = max(about - lane, 0), b1_ = min(about + lane, SM_BINS - 2);
+        const unsigned fits = __ballot_sync(0xffffffffu, s.bin[1][b1_ + 1] - s.bin[1][b0_] <= SM_LIST);
+        const int wide = 31 - __clz(fits);
+        if (tid == 0) {
+          s.b0 = max(about - wide, 0);
+          s.b1 = fits ? min(about + wide, SM_BINS - 2) : -1;
+        }
       }
-      __syncthreads();
-      // as many of them around it as there is room for, 31 on both sides at most (it is hardly ever that far off)
-      const int about = min((int)s.critical, SM_BINS - 2), b0_ = max(about - lane, 0), b1_ = min(about + lane, SM_BINS - 2);
-      const unsigned fits = __ballot_sync(0xffffffffu, s.bin[1][b1_ + 1] - s.bin[1][b0_] <= SM_LIST);
-      const int wide = 31 - __clz(fits), b0 = max(about - wide, 0), b1 = fits ? min(about + wide, SM_BINS - 2) : -1;
-      if (b1 >= 0) {
+      if (MANY && ranks > 1) sm_meet();
+      else __syncthreads();
+      const int b0 = s0.b0, b1 = s0.b1;
+      if (b1 < 0) {
+        if (MANY && ranks > 1) sm_meet();                  // (as above)
+        if (MANY && rank) return;
+        row.share(0, 1);
+        ranks = 1;
+      } else {
         // ---- all weights, those in front of the list, those of each part; the list
-        const int n = (int)(s.bin[1][b1 + 1] - s.bin[1][b0]);
         u64 everything = 0, in_front = 0;
         auto take = [&](auto& a, int v0) {
 #pragma unroll 4
@@ -640,25 +764,31 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const _
               in_front += w;
               if (a[j] >= least_p) mine += w;
             } else if (bin <= b1) {
-              sm_keep(row, s, a[j], v0 + j, bin, b0);
+              sm_keep(row, s0, a[j], v0 + j, bin, b0);
             }
           }
         };
-        for (int part = warp; part < SM_PARTS; part += WARPS) {
-          mine = 0;
-          row.template range<1>(part * per_part + lane, 32, min((part + 1) * per_part, row.vectors), take);
-          if (part == 0 && lane < row.head) row.one(lane, take);
-          if (part == SM_PARTS - 1 && row.head + lane < row.edges()) row.one(row.edge(row.head + lane), take);
-          mine = sm_warp_sum(mine);
-          if (lane == 0) {
-            s.kept[0][part] = (unsigned)mine;
-            s.kept[1][part] = (unsigned)(mine >> 32);
-          }
-        }
+        row.sums(s, s0, mine, take);
         u64 total, front;
         sm_before<THREADS>(everything, s.part, total);
         __syncthreads();
         sm_before<THREADS>(in_front, s.part, front);
+        if (MANY && ranks > 1) {
+          if (tid == 0) {
+            s0.everything[rank] = total;
+            s0.in_front[rank] = front;
+          }
+          sm_meet();
+          if (MANY && rank) return;
+          total = front = 0;
+          for (int i = 0; i < ranks; ++i) {
+            total += s.everything[i];
+            front += s.in_front[i];
+          }
+          row.share(0, 1);
+          ranks = 1;
+        }
+        const int n = (int)(s.bin[1][b1 + 1] - s.bin[1][b0]);
         sm_sort(row, s, n, b0);
         // ---- the entry of the list at which the share ends
         constexpr int OWN_LIST = SM_LIST / THREADS;
@@ -678,7 +808,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const _
               const u64 e = s.sorted[tid * OWN_LIST + i];
               if ((double)(before + w[i]) >= share) s.cut = e;
               if (sm_value(e) >= least_p) {
-                const int part = part_of(sm_index(e));
+                const int part = row.part_of(sm_index(e));
                 const unsigned low = (unsigned)w[i], old = atomicAdd(&s.kept[0][part], low), high = (unsigned)(w[i] >> 32) + (old + low < old);
                 if (high) atomicAdd(&s.kept[1][part], high);
               }
@@ -714,23 +844,15 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const _
     }
   };
   if (!summed) {
-    for (int part = warp; part < SM_PARTS; part += WARPS) {
-      mine = 0;
-      row.template range<1>(part * per_part + lane, 32, min((part + 1) * per_part, row.vectors), add);
-      if (part == 0 && lane < row.head) row.one(lane, add);
-      if (part == SM_PARTS - 1 && row.head + lane < row.edges()) row.one(row.edge(row.head + lane), add);
-      mine = sm_warp_sum(mine);
-      if (lane == 0) {
-        s.kept[0][part] = (unsigned)mine;
-        s.kept[1][part] = (unsigned)(mine >> 32);
-      }
-    }
-    __syncthreads();
+    row.sums(s, s0, mine, add);
+    if (MANY && ranks > 1) sm_meet();
+    else __syncthreads();
+    if (MANY && rank) return;
   }
   const SamplePart here(s, u);
   // ---- the part in which u lies, cut among all threads: vectors next to each other, the first thread with those in front of all vectors, the last with those
   // behind
-  const int part = here.part, first = part * per_part, end = max(first, min(first + per_part, row.vectors)), own = (end - first + THREADS - 1) / THREADS;
+  const int part = here.part, first = part * row.per_part, end = max(first, min(first + row.per_part, row.vectors)), own = (end - first + THREADS - 1) / THREADS;
   const int i0 = min(first + tid * own, end), i1 = min(i0 + own, end);
   auto walk = [&](auto f) {
     if (part == 0 && tid == 0)
@@ -755,9 +877,33 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const _
 
 template <typename T>
 static int launch_sample(const SampleParams& p, long long B, cudaStream_t st) {
-  // one CTA to an SM where there are no more rows
-  if (B <= sm_count()) sample_kernel<T, 1024><<<(unsigned)B, 1024, 0, st>>>(p);
-  else sample_kernel<T, 512><<<(unsigned)B, 512, 0, st>>>(p);
+  // Several CTAs to a row where it is long and there are SMs for them: clusters of 4 and 8 find room on seven and six of eight SMs. us with 1 / 2 / 4 / 8, the
+  // weights of all entries wanted and a share of 0.9: 3 rows of 32000 15, 33 / 14, 30 / 13, 26 / 12, 26; 8 of 128256 34, 71 / 25, 52 / 18, 40 / 15, 35; 64 of
+  // 50257 20, 43 / 18, 38; 4 of 16384 11, 23 / 13, 25 / 12, 25 / 12, 26. Where a cluster has to wait for another one: 16 of 128256 19, 40 with 4, 25, 54 with 8.
+  const int sms = sm_count();
+  if (B > sms) {
+    sample_kernel<T, 512, false><<<(unsigned)B, 512, 0, st>>>(p);
+    return cudaGetLastError() == cudaSuccess ? GFH_OK : GFH_CUDA;
+  }
+  // The likeliest entries alone, one pass, gain nothing: 8 of 128256 10 with one, 12 with 8.
+  const bool likeliest = !p.temperature && !(p.temperature0 > 0.f);
+  int ranks = 1;
+  while (!likeliest && ranks < SM_RANKS && p.V >= max(12000, 6000 * ranks) * 2 && 2 * ranks * B * 8 <= sms * (ranks == 4 ? 6 : ranks == 2 ? 7 : 8)) ranks *= 2;
+  if (ranks == 1) {
+    sample_kernel<T, 1024, false><<<(unsigned)B, 1024, 0, st>>>(p);
+    return cudaGetLastError() == cudaSuccess ? GFH_OK : GFH_CUDA;
+  }
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = ranks;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(B * ranks));
+  cfg.blockDim = dim3(1024);
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, sample_kernel<T, 1024, true>, p) != cudaSuccess) return GFH_CUDA;
   return cudaGetLastError() == cudaSuccess ? GFH_OK : GFH_CUDA;
 }
 

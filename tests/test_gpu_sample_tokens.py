@@ -107,3 +107,24 @@ def test_what_a_gradient_or_a_trace_follows_takes_other_operations():
     assert ops.sample_tokens(x, u, 0.5, 10).flatten().tolist() == oracle.tokens(x, u, 0.5, 10)
     assert ops.sample_tokens(x.detach().t().contiguous().t(), u, 0.5).flatten().tolist() == oracle.tokens(x, u, 0.5)
     assert _lib.launch_count() == n
+
+
+@pytest.mark.parametrize("V", [23999, 24000, 32003, 50257, 128256])
+@pytest.mark.parametrize("cuts", [{}, dict(top_k=50), dict(top_k=900), dict(top_k=5000), dict(top_p=0.9), dict(top_p=0.999), dict(top_k=64, top_p=0.5), dict(min_p=0.05),
+                                  dict(top_p=0.8, min_p=0.02)], ids=lambda k: "-".join(k) or "none")
+def test_a_row_has_one_token_however_many_rows_there_are(V, cuts):
+    """Rows of a few are read by several blocks each, rows of many by one: the same token of either, of rows without probabilities and of equal entries too."""
+    from ghost_flow_b200 import ops
+
+    x = _rows("random", 200, V, torch.bfloat16, 0, 5).clone()
+    x[3], x[5, 7], x[8, V - 1], x[11], x[14, V // 3:], x[17, : V // 2] = -INF, NAN, INF, 1.5, -INF, 20.0
+    x[20] *= 1e-3
+    x[23] *= 50
+    u = torch.rand(200, device="cuda")
+    u[:4] = torch.tensor([0.0, 1.0 - 2.0 ** -24, 0.5, 0.25])
+    all_ = ops.sample_tokens(x, u, 0.9, **cuts)
+    for n in (1, 5, 13, 30, 60, 120):
+        for at in (0, 2, 80):
+            assert torch.equal(ops.sample_tokens(x[at:at + n], u[at:at + n], 0.9, **cuts), all_[at:at + n]), (n, at)
+    for row in (0, 1, 3, 5, 8, 11, 14, 17, 20, 23, 30):
+        assert torch.equal(ops.sample_tokens(x[row:row + 1], u[row:row + 1], 0.9, **cuts), all_[row:row + 1]), row
