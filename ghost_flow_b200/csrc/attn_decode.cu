@@ -26,6 +26,8 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+#include <cfloat>
+
 #include "gf_host.h"
 #include "gf_ptx.cuh"
 #include "paged.cuh"
@@ -387,7 +389,7 @@ attn_decode_kernel(const __grid_constant__ DecParams p) {
   uint32_t qb[D / 16][2];          // Q^T as the 8-column operand: head r, dims 16 t + 2c, + 1 and + 8, + 9
   float o[D / 16][4];              // O^T: dims 16 j + r (+ 8), heads 2c, 2c + 1
   float m[2], l[2];
-  float mv[2], qf[2];              // BYTES: see `unit`
+  float ev[2], qf[2];              // BYTES: see `unit`
   uint4 k_new, v_new;              // append: chunk `lane` of the new token's rows, in the warp whose keys it belongs to
   // ---- start of a piece
   auto begin = [&] {
@@ -420,7 +422,6 @@ attn_decode_kernel(const __grid_constant__ DecParams p) {
         }
 #pragma unroll
       for (int i = 0; i < 2; ++i) qf[i] = __uint_as_float(__shfl_sync(0xffffffffu, e, (2 * c + i) * 4) << 23) * p.scale_log2;
-      mv[0] = mv[1] = -INFINITY;
     } else {
 #pragma unroll
     for (int t = 0; t < D / 16; ++t) {
@@ -449,7 +450,8 @@ attn_decode_kernel(const __grid_constant__ DecParams p) {
     }
 #pragma unroll
     for (int j = 0; j < D / 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-    m[0] = m[1] = -INFINITY;
+    m[0] = m[1] = BYTES ? 0.f : -INFINITY;
+    ev[0] = ev[1] = -FLT_MAX;      // nothing yet
     l[0] = l[1] = 0.f;
   };
   // ---- the unit at `at`, in stage st
@@ -471,8 +473,9 @@ attn_decode_kernel(const __grid_constant__ DecParams p) {
     }
     if constexpr (BYTES) {
       // Numbers of the cache become f16 as they are; their rows' powers of two go to the scores (K) and to the probabilities (V): with e the exponents of V,
-      // P' = 2^(score + e - mv + 8), mv about the largest score + e so far, so that the products with V have all of f16's bits whatever the rows' scales are. l, of P
-      // itself, goes by the largest score. 2^8: what is below 2^-33 of the largest is lost, not 2^-25. One f16 number stands for a P': half a step is 2^-12.
+      // P' = 2^((score - m) + e - ev), m about the largest score so far and ev about the largest (score - m) + e, less 8, so that the products with V have all of f16's
+      // bits whatever the rows' scales are, and scores of any size are only subtracted from each other. l, of P itself, goes by m. 8: what is below 2^-33 of
+      // the largest is lost, not 2^-25. One f16 number stands for a P': half a step is 2^-12.
       if (left > 0) {
         const uint32_t tk = my + st * Cfg::STAGE, tv = tk + Cfg::TILE;
         const uint8_t* scales = ring + DEC_WARPS * Cfg::WARP_BYTES + warp * Cfg::SCALES + st * (2 * DEC_KEYS);
@@ -487,41 +490,48 @@ attn_decode_kernel(const __grid_constant__ DecParams p) {
           mma_f16_16816(sd, f16x2_of_e4m3<0>(a[2]), f16x2_of_e4m3<0>(a[3]), f16x2_of_e4m3<1>(a[2]), f16x2_of_e4m3<1>(a[3]), qb[t + 1][0], qb[t + 1][1]);
         }
         const float f0 = __uint_as_float(k0 << 23), f1 = __uint_as_float(k1 << 23), e0 = (float)v0 - 127.f, e1 = (float)v1 - 127.f;
-        float x[4], z[4], pr[4];
+        float x[4], d[4], z[4], pr[4];
         bool grows = false;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {                            // key r (+ 8), head 2c (+ 1)
           x[i] = r + 4 * (i & 2) < left ? (sc[i] + sd[i]) * ((i & 2) ? f1 : f0) * qf[i & 1] : -INFINITY;
-          z[i] = x[i] + ((i & 2) ? e1 : e0);
-          grows |= x[i] - m[i & 1] > LAZY || z[i] - mv[i & 1] > LAZY;
+          d[i] = x[i] - m[i & 1];
+          z[i] = d[i] + ((i & 2) ? e1 : e0) - ev[i & 1];
+          grows |= d[i] > LAZY || z[i] > LAZY + 8;
         }
         // The references are moved only when a score has grown by 2^7: what is 2^15 then still is a number of f16
         if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float mx = fmaxf(fmaxf(x[e], x[2 + e]), m[e]), mz = fmaxf(fmaxf(z[e], z[2 + e]), mv[e]);
+            const bool none = ev[e] == -FLT_MAX;
+            float mx = fmaxf(fmaxf(x[e], x[2 + e]), none ? -INFINITY : m[e]);
 #pragma unroll
-            for (int o = 4; o < 32; o <<= 1) {
-              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-              mz = fmaxf(mz, __shfl_xor_sync(0xffffffffu, mz, o));
-            }
-            l[e] *= ex2_approx(m[e] - (mx == -INFINITY ? 0.f : mx));
-            const float corr = ex2_approx(mv[e] - (mz == -INFINITY ? 0.f : mz));
+            for (int s = 4; s < 32; s <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, s));
+            if (mx == -INFINITY) mx = 0.f;                       // (of a head that has no score yet)
+            const float by = none ? 0.f : m[e] - mx;
+            d[e] = x[e] - mx;
+            d[2 + e] = x[2 + e] - mx;
+            float mz = fmaxf(fmaxf(d[e] + e0, d[2 + e] + e1) - 8.f, ev[e] + by);
+#pragma unroll
+            for (int s = 4; s < 32; s <<= 1) mz = fmaxf(mz, __shfl_xor_sync(0xffffffffu, mz, s));
+            l[e] *= ex2_approx(by);
+            const float corr = ex2_approx(ev[e] + by - mz);
 #pragma unroll
             for (int j = 0; j < D / 16; ++j) {
               o[j][e] *= corr;
               o[j][2 + e] *= corr;
             }
+            z[e] = d[e] + e0 - mz;
+            z[2 + e] = d[2 + e] + e1 - mz;
             m[e] = mx;
-            mv[e] = mz;
+            ev[e] = mz;
           }
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float ref = m[e] == -INFINITY ? 0.f : m[e], refz = (mv[e] == -INFINITY ? 0.f : mv[e]) - 8.f;
-          l[e] += ex2_approx(x[e] - ref) + ex2_approx(x[2 + e] - ref);
-          pr[e] = ex2_approx(z[e] - refz);
-          pr[2 + e] = ex2_approx(z[2 + e] - refz);
+          l[e] += ex2_approx(d[e]) + ex2_approx(d[2 + e]);
+          pr[e] = ex2_approx(z[e]);
+          pr[2 + e] = ex2_approx(z[2 + e]);
         }
         uint32_t pt[2];
 #pragma unroll
@@ -599,10 +609,11 @@ attn_decode_kernel(const __grid_constant__ DecParams p) {
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], 8);
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], 16);
     }
-    if constexpr (BYTES) {       // from units of the largest score + e to those of the largest score
+    if constexpr (BYTES) {       // in units of m alone
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float f = m[e] == -INFINITY ? 0.f : ex2_approx(mv[e] - m[e] - 8.f);
+        const float f = ex2_approx(ev[e] + 8.f) * 0x1p-8f;      // (ev is -134 where V has the least scale)
+        if (ev[e] == -FLT_MAX) m[e] = -INFINITY;
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) {
           o[j][e] *= f;

@@ -314,3 +314,12 @@ def test_a_model_over_pages_of_8_bits(kw, kernel_status):
     assert 0 < (out[0] - out[2]).norm() < 0.2 * out[2].norm()
     tokens = m.generate_batch([ids[:9], ids[:20]], 5, page_size=16, cache_dtype=torch.float8_e4m3fn, temperature=0.9, top_k=20, top_p=0.9)
     assert [t.numel() for t in tokens] == [14, 25] and all(((t >= 0) & (t < 97)).all() for t in tokens)
+
+
+@pytest.mark.parametrize("H,Hk,D", [(8, 2, 128), (8, 8, 64), (16, 1, 64)])
+@pytest.mark.parametrize("spread", [10, 14, 18])
+def test_scores_far_beyond_the_powers_of_two(H, Hk, D, spread, kernel_status):
+    """One token each over rows of such sizes that a score's last bit is worth more than all powers of two: results stay finite."""
+    lens = [1, 2, 9, 33, 700, 1213]
+    s = oracle.batch(lens, [1] * len(lens), H, Hk, D, 16, device="cuda", spread=spread)
+    paged.close(_attend(s, cu=None), *oracle.attention(s))
