@@ -22,6 +22,7 @@
 // What bounds it: the instructions of an entry's weight (a table of 16 powers and a series, 64 bits), of its bin and its atomic addition, not the 6.6 TB/s that
 // the first pass reaches. 512 rows of 50257 in bf16, of which memory wants 8 us: the likeliest 17 us, weights of all 59, k = 50 48, p = 0.9 126, p of the least
 // 35; 32 bits, 16 us: 22, 55, 50, 109, 31. 64 rows in bf16: 6, 19, 18, 38, 15; 3 rows of 32000: 5, 12, 14, 26, 12.
+#include <cfloat>
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
@@ -42,7 +43,7 @@ struct SampleParams {
   const float* u;                                   // [B]
   const float *temperature, *top_p, *min_p;         // [B] or null: the numbers below
   const int* top_k;
-  float temperature0, top_p0, min_p0;
+  double temperature0, top_p0, min_p0;
   int top_k0;
   long long* out;                                   // [B]
   int V, bits;                                      // a weight of 1 is 2^bits
@@ -267,8 +268,8 @@ struct SampleRow {
     return __double_as_longlong(w) & 0xfffffffffffffull;
   }
   // The least entry with w >= p.
-  __device__ __forceinline__ float least(float p, float temperature) const {
-    return p > 0.f ? __double2float_ru((double)m + (double)temperature * log((double)p)) : -INFINITY;
+  __device__ __forceinline__ float least(double p, double temperature) const {
+    return p > 0 ? fmaxf(__double2float_ru((double)m + temperature * log(p)), -INFINITY) : -INFINITY;      // (all, of an infinite temperature)
   }
 };
 
@@ -545,9 +546,9 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const _
   Row row(p);
   row.begin((const T*)p.x + b * p.ldx, p.V);
   row.share(rank, ranks);
-  const float temperature = p.temperature ? p.temperature[b] : p.temperature0;
-  const float top_p = p.top_p ? p.top_p[b] : p.top_p0;
-  const float min_p = fminf(p.min_p ? p.min_p[b] : p.min_p0, 1.f);
+  const double temperature = p.temperature ? p.temperature[b] : p.temperature0;
+  const double top_p = p.top_p ? p.top_p[b] : p.top_p0;
+  const double min_p = fmin(p.min_p ? p.min_p[b] : p.min_p0, 1.0);
   const int top_k = p.top_k ? p.top_k[b] : p.top_k0;
   const float u = fminf(fmaxf(p.u[b], 0.f), 0x1.fffffep-1f);
   if (warp == WARPS - 1 && lane < 16) s.power[lane] = exp2(lane / 16.0) * (double)(1ull << p.bits);
@@ -606,7 +607,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const _
   }
   SampleShared& s0 = MANY ? sm_of(s, 0) : s;          // the first CTA's
   // ---- rows without probabilities, and those whose likeliest entry is asked for
-  if (!(fabsf(most) < INFINITY) || !(temperature > 0.f) || top_k == 1 || top_p <= 0.f) {
+  if (!(fabsf(most) < INFINITY) || !(temperature > 0) || top_k == 1 || top_p <= 0) {
     if (MANY && rank) return;
     row.share(0, 1);
     const bool none = most != most;
@@ -615,9 +616,9 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const _
     return;
   }
   row.m = most;
-  row.per16 = 16.0 * 1.4426950408889634 / (double)temperature;
-  row.low = most - 33.271065f * temperature;       // 48 log(2)
-  row.zero = most - 744.44009f * temperature;      // 1074 log(2)
+  row.per16 = 16.0 * 1.4426950408889634 / temperature;
+  row.low = fmaxf(most - 33.271065f * (float)temperature, -FLT_MAX);       // 48 log(2)
+  row.zero = fmaxf(most - 744.44009f * (float)temperature, -FLT_MAX);      // 1074 log(2); minus infinity has no weight at any temperature
   row.power = s.power;
   // Bins of numbers reach three quarters of the way to the mean, which some of the first entries stand for; those of weights twice as far. What is further away lies in
   // the last.
@@ -664,13 +665,13 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const _
         sum += w[i];
       }
       u64 before = sm_before<THREADS>(sum, s.part, total);
-      const double target = (double)top_p * (double)total;
+      const double target = top_p * (double)total;
 #pragma unroll
       for (int i = 0; i < OWN; ++i) {
         const u64 front = before;
         before += w[i];
         if (w[i] == 0) continue;
-        if ((top_p < 1.f && !((double)front < target)) || sm_value(e[i]) < least_p) {
+        if ((top_p < 1 && !((double)front < target)) || sm_value(e[i]) < least_p) {
           w[i] = 0;
           continue;
         }
@@ -707,7 +708,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const _
   }
   u64 mine = 0;                                    // of this warp's part
   bool summed = false;
-  if (top_p < 1.f) {
+  if (top_p < 1) {
     row.per_bin = per * 0.5f;
     if (cut == 0) {
       // ---- by the bins' numbers and middles, about where the share ends
@@ -724,7 +725,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const _
         }
         // (as whole numbers, of which the scan is)
         u64 all, before = sm_before<THREADS>((u64)(sum * 0x1p20f), s.part, all);
-        const u64 target = (u64)((double)top_p * (double)all);
+        const u64 target = (u64)(top_p * (double)all);
         if (tid == 0) s.critical = 0;
         __syncthreads();
 #pragma unroll
@@ -800,7 +801,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const _
           sum += w[i];
         }
         u64 before = front + sm_before<THREADS>(sum, s.part, list);
-        const double share = (double)top_p * (double)total;
+        const double share = top_p * (double)total;
         if ((double)front < share && (double)(front + list) >= share) {      // else it lies elsewhere, and is looked for in another way
 #pragma unroll
           for (int i = 0; i < OWN_LIST; ++i) {
@@ -886,7 +887,7 @@ static int launch_sample(const SampleParams& p, long long B, cudaStream_t st) {
     return cudaGetLastError() == cudaSuccess ? GFH_OK : GFH_CUDA;
   }
   // The likeliest entries alone, one pass, gain nothing: 8 of 128256 10 with one, 12 with 8.
-  const bool likeliest = !p.temperature && !(p.temperature0 > 0.f);
+  const bool likeliest = !p.temperature && !(p.temperature0 > 0);
   int ranks = 1;
   while (!likeliest && ranks < SM_RANKS && p.V >= max(12000, 6000 * ranks) * 2 && 2 * ranks * B * 8 <= sms * (ranks == 4 ? 6 : ranks == 2 ? 7 : 8)) ranks *= 2;
   if (ranks == 1) {
@@ -917,7 +918,7 @@ GF_API int gf_sample_tokens(const SampleCall* c, void* stream) {
   int bits = 62;                                   // sums of V weights are below 2^62
   while (bits > 46 || (c->V >> (62 - bits)) > 0) --bits;
   constexpr double C1 = 0.69314718055994530942 / 16;
-  const SampleParams p{c->x, c->ldx, c->u, c->temperature, c->top_p, c->min_p, c->top_k, (float)c->temperature0, (float)c->top_p0, (float)c->min_p0,
+  const SampleParams p{c->x, c->ldx, c->u, c->temperature, c->top_p, c->min_p, c->top_k, c->temperature0, c->top_p0, c->min_p0,
                        (int)c->top_k0, c->out, (int)c->V, bits, {C1, C1 * C1 / 2, C1 * C1 * C1 / 6, C1 * C1 * C1 * C1 / 24, C1 * C1 * C1 * C1 * C1 / 120}};
   cudaStream_t st = (cudaStream_t)stream;
   return c->dtype == 0 ? launch_sample<float>(p, c->B, st) : c->dtype == 1 ? launch_sample<__nv_bfloat16>(p, c->B, st) : launch_sample<__half>(p, c->B, st);

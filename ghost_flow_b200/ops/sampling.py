@@ -148,7 +148,7 @@ def _sample_ref(x, u, temperature, top_k, top_p, min_p):
     sampled = (t > 0) & (k != 1) & ~(p <= 0) & top.isfinite()
     y, order = torch.sort(torch.where(sampled, x.double(), 0.0), dim=-1, descending=True, stable=True)
     w = torch.exp((y - y[:, :1]) / torch.where(sampled, t, 1.0))
-    w = torch.where((k <= 0) | (torch.arange(V, device=x.device) < k), w, 0.0)
+    w = torch.where((y > float("-inf")) & ((k <= 0) | (torch.arange(V, device=x.device) < k)), w, 0.0)
     upto = w.cumsum(-1)
     stays = (~(p < 1) | (upto - w < p * upto[:, -1:])) & (w >= least)
     upto = torch.zeros_like(w).scatter_(1, order, torch.where(stays, w, 0.0)).cumsum(-1)

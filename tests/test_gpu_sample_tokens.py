@@ -128,3 +128,28 @@ def test_a_row_has_one_token_however_many_rows_there_are(V, cuts):
             assert torch.equal(ops.sample_tokens(x[at:at + n], u[at:at + n], 0.9, **cuts), all_[at:at + n]), (n, at)
     for row in (0, 1, 3, 5, 8, 11, 14, 17, 20, 23, 30):
         assert torch.equal(ops.sample_tokens(x[row:row + 1], u[row:row + 1], 0.9, **cuts), all_[row:row + 1]), row
+
+
+@pytest.mark.parametrize("kw", [{}, dict(top_k=5), dict(top_p=0.5), dict(min_p=0.9), dict(top_p=0.7, min_p=0.3)], ids=lambda k: "-".join(k) or "none")
+def test_temperatures_without_end_and_the_least(kw):
+    """At an infinite temperature what has a probability has the same; what has none still has none. At the least one the likeliest share it."""
+    from ghost_flow_b200 import ops
+
+    x = torch.tensor([[-INF, 2.0, -INF, 1.0, -3.0, -INF, 0.5, 7.0]], device="cuda").repeat(64, 1)
+    u = (torch.arange(64, device="cuda") + 0.5) / 64
+    order = [7, 1, 3, 6, 4]
+    kept = order[:3] if kw.get("top_p") == 0.5 else order[:4] if kw.get("top_p") == 0.7 else order
+    want = [sorted(kept)[int(v * len(kept))] for v in u.tolist()]
+    for t in (INF, torch.full((64,), INF, device="cuda"), 3e38, 1e38):
+        assert ops.sample_tokens(x, u, t, **kw).flatten().tolist() == want, t
+    for t in (1e-45, 1e-60, torch.full((64,), 1e-45, device="cuda")):
+        assert ops.sample_tokens(x, u, t, **kw).flatten().tolist() == [7] * 64
+
+
+def test_numbers_have_64_bits():
+    """A temperature or a share that is no number of 32 bits is taken as it is: the border of the second of two tokens lies between its neighbours."""
+    from ghost_flow_b200 import ops
+
+    x = torch.tensor([[0.0, 0.0, -INF]], device="cuda")
+    for p, want in ((0.5, 0), (0.5 + 2.0 ** -40, 1)):           # of 32 bits both are a half
+        assert ops.sample_tokens(x, torch.tensor([0.75], device="cuda"), 1.0, 0, p).item() == want

@@ -120,3 +120,15 @@ def test_generation_among_the_likeliest_alone_is_greedy(pages):
     a = run(temperature=5.0, top_k=40, top_p=0.9)
     torch.manual_seed(1)
     assert torch.equal(a, run(temperature=5.0, top_k=40, top_p=0.9))
+
+
+@pytest.mark.parametrize("kw", [{}, dict(top_k=5), dict(top_p=0.5), dict(min_p=0.9), dict(top_p=0.7, min_p=0.3)], ids=lambda k: "-".join(k) or "none")
+def test_temperatures_without_end(kw):
+    """At an infinite temperature what has a probability has the same; what has none still has none."""
+    x = torch.tensor([[-INF, 2.0, -INF, 1.0, -3.0, -INF, 0.5, 7.0]]).repeat(64, 1)
+    u = (torch.arange(64) + 0.5) / 64
+    order = [7, 1, 3, 6, 4]
+    kept = order[:3] if kw.get("top_p") == 0.5 else order[:4] if kw.get("top_p") == 0.7 else order
+    want = [sorted(kept)[int(v * len(kept))] for v in u.tolist()]
+    for t in (INF, torch.full((64,), INF), 3e38):
+        assert ops.sample_tokens(x, u, t, **kw).flatten().tolist() == want, t
