@@ -127,7 +127,7 @@ bool pools(PyObject* pages_k, PyObject* pages_v, PyObject* table, PyObject* lens
     st[1] = w->stride(1, Hk * D);
     st[0] = w->stride(0, page * st[1]);
     if ((st[0] | st[1] | st[2]) & (vec - 1)) return false;
-    if (bytes && (st[0] > MOST || st[1] > MOST || st[2] > MOST)) return false;
+    if (bytes && (st[0] > MOST || st[1] > MOST / page || st[2] > MOST)) return false;
     st += 3;
   }
   c.kpages = k.data;
@@ -624,7 +624,7 @@ PyObject* sample(PyObject*, PyObject* const* a, Py_ssize_t n) {
   double top_k = 0;
   constexpr double TINY = 0x1p-149;                // (a share of 0 is none)
   if (!choice(a[2], c.B, device, FLOAT, 0, 0x1p127, c.temperature0, t) || !choice(a[3], c.B, device, INT, 0, MOST, top_k, k) ||
-      !choice(a[4], c.B, device, FLOAT, TINY, 1, c.top_p0, p) || !choice(a[5], c.B, device, FLOAT, 0, 1, c.min_p0, least))
+      !choice(a[4], c.B, device, FLOAT, TINY, 1, c.top_p0, p) || !choice(a[5], c.B, device, FLOAT, 0, 1, c.min_p0, least) || (c.temperature0 > 0 && c.temperature0 < TINY))
     Py_RETURN_NONE;
   c.temperature = (const float*)t;
   c.top_k = (const int*)k;

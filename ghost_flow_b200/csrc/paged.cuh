@@ -82,6 +82,7 @@ inline bool paged_scales(const PagedCall8& c8) {
     if (!p || (reinterpret_cast<uintptr_t>(p) & 15)) return false;
   for (long long st : c.strides)
     if (st % 16 || st > 0x7fffffff) return false;
+  if (c.page <= 0 || c.strides[1] > 0x7fffffff / c.page || c.strides[4] > 0x7fffffff / c.page) return false;      // a page's rows are offsets of 32 bits
   return c.D % 16 == 0;
 }
 

@@ -188,7 +188,7 @@ def rope_qkv_to_pages(qkv, num_heads: int, num_kv_heads: int, cos, sin, kpages, 
     or a position that is not in the tables or behind the page table, is left out too, and ``_lib.check_status`` raises.
     Inference only: a call with a gradient to record takes PyTorch's operations."""
     H, Hk = num_heads, num_kv_heads
-    heads = kscales is not None or vscales is not None or q_weight is not None or k_weight is not None or 2 * cos.shape[-1] != qkv.shape[-1]
+    heads = kscales is not None or vscales is not None or q_weight is not None or k_weight is not None or cos.dim() != 2 or 2 * cos.shape[1] != qkv.shape[-1]
     more = (kscales, vscales, q_weight, k_weight) if heads else ()
     call = None
     if qkv.get_device() >= 0 and not _is_compiling():

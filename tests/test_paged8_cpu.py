@@ -198,3 +198,16 @@ def test_caches():
     assert k.shape == (20, 2, 32) and not k.any() and not v.any()
     with pytest.raises(ValueError, match="room"):
         c.read(0, 33)
+
+
+def test_rows_of_a_page_are_within_32_bits():
+    """The kernels add up rows of a page in 32 bits: pools whose rows are further apart are refused."""
+    import struct
+
+    lib, P = _lib.cuda_lib(), 1 << 20
+    far = 0x7fffffff // 16 // 16 * 16
+    call = lambda k1, v1: struct.pack("27q", P, 512, P, 256, 2 * P, 3 * P, 2048, k1, 64, 2048, v1, 64, P, 4, 4, P, P, 2, 5, 4, 2, 64, 16, 9, 0, 4 * P, 5 * P)  # noqa: E731
+    for k1, v1 in ((far + 16, 128), (128, far + 16), (1 << 31, 128)):
+        c = call(k1, v1)
+        assert lib.gf_paged_append_heads(c, P, P, 9, 64, 0, P, P, 1e-6, None) == lib.gf_paged_read(c, P, P, None) == -1
+        assert lib.gf_paged_attn8(c, 0.1, P, 1 << 40, 0, None, None) == lib.gf_paged_attn8_one(c, 0.1, 1, P, None) == -1
