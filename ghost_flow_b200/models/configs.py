@@ -32,9 +32,13 @@ class LLaMAConfig:
         return self.hidden_size // self.num_attention_heads
 
     @property
+    def rope_dims(self) -> int:
+        return self.head_dim if self.rotary_dim is None else self.rotary_dim
+
+    @property
     def plain_heads(self) -> bool:
         """Whether heads are rotated as a whole and not normed: what the layers' fused forms and the parallel engines take."""
-        return not self.qk_norm and self.rotary_dim in (None, self.head_dim)
+        return not self.qk_norm and self.rope_dims == self.head_dim
 
     @classmethod
     def llama_7b(cls): return cls()

@@ -362,7 +362,7 @@ class MixtralForCausalLM(Module):
 
     def forward(self, ids, labels=None):
         S = ids.shape[1]
-        cos, sin = ops.rope_tables(max(S, self.cfg.max_position_embeddings), self.cfg.head_dim, self.cfg.rope_theta,
+        cos, sin = ops.rope_tables(max(S, self.cfg.max_position_embeddings), self.cfg.rope_dims, self.cfg.rope_theta,
                                    ids.device)
         x = self.embed_tokens(ids)
         for layer in self.layers:

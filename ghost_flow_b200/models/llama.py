@@ -179,7 +179,7 @@ class LLaMAModel(Module):
     def rope(self, length, device):
         if self._rope is None or self._rope[0].shape[0] < length or self._rope[0].device != torch.device(device):
             n = max(length, self.cfg.max_position_embeddings)
-            self._rope = ops.rope_tables(n, self.cfg.rotary_dim or self.cfg.head_dim, self.cfg.rope_theta, device)
+            self._rope = ops.rope_tables(n, self.cfg.rope_dims, self.cfg.rope_theta, device)
         return self._rope
 
     def _before_norm(self, ids, caches, start_pos):

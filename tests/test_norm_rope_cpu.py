@@ -128,3 +128,19 @@ def test_a_served_checkpoint_with_norms_has_them():
     sd = _model(qk_norm=True).state_dict()
     assert _llama_config_from_state(sd, dict(num_attention_heads=4)).qk_norm
     assert not _llama_config_from_state(_model().state_dict(), dict(num_attention_heads=4)).qk_norm
+
+
+def test_no_dims_rotated_and_a_part_of_them_with_experts():
+    from ghost_flow_b200.models import MixtralConfig
+    from ghost_flow_b200.models.encoders import MixtralForCausalLM
+
+    m, ids = _model(rotary_dim=0), torch.randint(0, 97, (2, 6))
+    assert not m.cfg.plain_heads and torch.equal(torch.stack(m.generate_batch(list(ids), 5, page_size=16)), m.generate(ids, 5))
+    m(ids)
+    assert m.model.layers[0].attn.cfg.rope_dims == 0
+    seen = []
+    m = MixtralForCausalLM(MixtralConfig(vocab_size=97, hidden_size=64, intermediate_size=64, num_hidden_layers=1, num_attention_heads=4, num_key_value_heads=2,
+                                         num_local_experts=2, max_position_embeddings=16, rotary_dim=8, qk_norm=True), dtype=torch.float32)
+    m.layers[0].attn.register_forward_hook(lambda mod, args, out: seen.append(args[1].shape))
+    m(ids)
+    assert seen == [(16, 4)]
