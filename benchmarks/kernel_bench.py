@@ -110,6 +110,44 @@ def build(args, dev):
         allowed = ops.pack_allowed(torch.rand(R, V, device=dev) < 0.5)
         return (lambda: ops.process_logits(x, tokens, repetition=1.2, presence=0.5, frequency=0.2, allowed=allowed)), 0.0, \
             4.0 * R * V + R * V / 8 + 4.0 * R * args.seq
+    if k in ("paged_attn8", "paged_append8", "paged_read8"):
+        # as paged_attn, pages of 8 bits; the append norms the heads
+        from ghost_flow_b200 import ops
+        B, S, H, Hkv, D, n, page = args.batch, args.seq, args.heads, args.kv_heads or args.heads, args.dim, args.new, args.page
+        width = -(-S // page)
+        kp, vp = (torch.randn(B * width, page, Hkv, D, device=dev).to(torch.float8_e4m3fn) for _ in range(2))
+        ks, vs = (torch.full((B * width, Hkv, page), 127, device=dev, dtype=torch.uint8).view(torch.float8_e8m0fnu) for _ in range(2))
+        table = torch.randperm(B * width, device=dev).int().view(B, width)
+        lens = torch.full((B,), S, dtype=torch.int32, device=dev)
+        cu = None if n == 1 else (n * torch.arange(B + 1, device=dev)).int()
+        if k == "paged_read8":
+            return (lambda: ops.read_pages(B * n, kp, vp, table, lens, cu, ks, vs)), 0.0, 2.0 * B * n * Hkv * (3 * D + 1)
+        if k == "paged_append8":
+            qkv, w = torch.randn(B * n, H + 2 * Hkv, D, device=dev, dtype=bf), torch.ones(D, device=dev, dtype=bf)
+            cos, sin = ops.rope_tables(S, D, 10000.0, dev)
+            return (lambda: ops.rope_qkv_to_pages(qkv, H, Hkv, cos, sin, kp, vp, table, lens, cu, False, ks, vs, w, w)), 0.0, \
+                2.0 * qkv.numel() + 2.0 * B * n * H * D + 2.0 * B * n * Hkv * (D + 1) + 4.0 * B * n * D
+        q = torch.randn(B * n, H, D, device=dev, dtype=bf)
+        return (lambda: ops.paged_attention(q, kp, vp, table, lens, cu, kscales=ks, vscales=vs)), 4.0 * B * H * D * (n * S - n * (n - 1) / 2), \
+            4.0 * q.numel() + 2.0 * B * S * Hkv * (D + 1)
+    if k in ("norm_rope", "norm_rope_bwd"):
+        from ghost_flow_b200 import ops
+        B, S, H, Hkv, D = args.batch, args.seq, args.heads, args.kv_heads or args.heads, args.dim
+        qkv, (qw, kw) = torch.randn(B, S, H + 2 * Hkv, D, device=dev, dtype=bf), torch.ones(2, D, device=dev, dtype=bf).unbind()
+        cos, sin = ops.rope_tables(S, D, 10000.0, dev)
+        rows = 2.0 * B * S * D
+        if k == "norm_rope":
+            return (lambda: ops.norm_rope_qkv(qkv, H, Hkv, qw, kw, cos, sin)), 0.0, 2 * rows * (H + Hkv)
+        leaves = [t.requires_grad_() for t in (qkv, qw.clone(), kw.clone())]
+        out = ops.norm_rope_qkv(leaves[0], H, Hkv, *leaves[1:], cos, sin)
+        grads = [torch.randn_like(t) for t in out]
+        return (lambda: torch.autograd.grad(out, leaves, grads, retain_graph=True)), 0.0, rows * (3 * (H + Hkv) + 2 * Hkv)
+    if k == "sample_tokens":
+        # --rows rows of --cols entries in bf16, a share of 0.9
+        from ghost_flow_b200 import ops
+        x, u = 3 * torch.randn(args.rows, args.cols, device=dev), torch.rand(args.rows, device=dev)
+        x = x.to(bf)
+        return (lambda: ops.sample_tokens(x, u, 0.8, 0, 0.9)), 0.0, 2.0 * args.rows * args.cols
     if k in ("attn_fwd", "attn_bwd"):
         B, S, H, Hkv, D = args.batch, args.seq, args.heads, args.kv_heads or args.heads, args.dim
         q = torch.randn(B * S, H * D, device=dev, dtype=bf)

@@ -23,6 +23,10 @@
 // 44.9 / 41.1; one length: 32 of 4096, 32 / 8 heads 90.8 / 82.8 (6.5 TB/s), 8 of 1501, 32 / 32 heads 36.3 / 32.6, 8 of 4000, 40
 // / 40 heads 112.2 / 103.9, 32 of 4096, 12 / 12 heads of 64 72.7 / 60.7 (6.6 TB/s), 64 of 300, 16 / 2 heads of 64 5.9 / 5.9, 4
 // of 64, 64 / 8 heads of 64 3.1 / 3.2.
+//
+// Pages of 8 bits (see `unit`): the numbers become f16 operands, two to an instruction, without a product, and four CTAs are on an SM. 32 sequences of 100 .. 4096
+// keys, 32 / 8 heads of 128: 34 us (132 MB, 4 TB/s), pages of bf16 47; 4 of 20011 .. 30001, 64 / 8 heads 45 (4.7 TB/s), 71. Half of the issue slots are taken; the loads' path bounds it: without
+// them the second takes 37. Tried and taken back: the products of one unit beside the softmax of the one in front (slower, registers).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 

@@ -25,7 +25,9 @@
 // 1344 blocks on 148 SMs are 202 us without the second and 271 with it, measured 269. us, dense / pages of 64 / 16: [1, 4096] with 32 / 8 heads of 128 133 / 135 /
 // 136 (1000 TFLOP/s), [4, 2987] with 32 / 32 heads 325 / 327 / 327, [8, 1024] with 12 / 12 heads of 64 44 / 49 / 49 (8 steps of a CTA at most).
 // The next 512 tokens over 7681 keys, 32 / 8 heads: 71 us (870 TFLOP/s), two pieces of 64 blocks on 128 of 148 SMs, 60 of it in steps. A block of one tile takes half as long and is cut into half as many pieces: 284
-// tokens over 5983 keys, 25 / 25 heads of 64, 40 us, with as many as the others 53. Few rows: keys come at 6 TB/s while steps run, and the ends of it, 5 us
+// tokens over 5983 keys, 25 / 25 heads of 64, 40 us, with as many as the others 53. Over pages of 8 bits the same 512 tokens take 91: four more warps turn a
+// step's K and V into bf16 tiles in shared memory (exact), which bounds it: 82 with the conversion left out, 73 without its stores. With a branch for rows that are not
+// there 99, with rows turned in place 138, with a row unrolled as a whole, which spills, 199. Few rows: keys come at 6 TB/s while steps run, and the ends of it, 5 us
 // in front and 6 behind with the second kernel, are what is left: 5 tokens over 30000 keys 35 us (3.5 TB/s), 16 over 2000 12.
 #include "paged.cuh"
 

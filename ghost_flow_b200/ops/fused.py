@@ -362,8 +362,14 @@ class _NormRopeQKVFn(torch.autograd.Function):
         return q, k, qkv[:, :, H + Hk:]
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dq, dk, dv):
+    def backward(ctx, *grads):
+        back = _NormRopeQKVFn._back
+        if torch.is_grad_enabled():          # a graph of the gradients is wanted, which there is not; else the look at it takes a tenth of a small call
+            back = torch.autograd.function.once_differentiable(back)
+        return back(ctx, *grads)
+
+    @staticmethod
+    def _back(ctx, dq, dk, dv):
         qkv, qw, kw, cos, sin = ctx.saved_tensors
         H, Hk, eps, interleaved, pos_offset = ctx.args
         look, D = _lib.calls().norm_rope_back, qkv.shape[3]
