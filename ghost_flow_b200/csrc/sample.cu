@@ -140,7 +140,7 @@ struct SampleRow {
   int part0, part1;              // parts of this CTA
   float m, per_bin;
   double per16;                  // 16 log2(e) / T
-  float low, zero;               // entries from which on weights are 2^-48 of the largest, and nothing
+  float zero;                    // entries below have no weight
   const double* power;
   const SampleParams& p;
 
@@ -256,10 +256,12 @@ struct SampleRow {
   }
   // w 2^bits, w = 2^((a - m) log2(e) / T), of entries from `zero` on: sixteenths of the exponent from a table, what is left of it, at most 2^-5, by the series of
   // the exponential function up to its fifth power (the sixth is 2^-42 of it), rounded up: what is above 0 counts as 1 at least. Without branches: a chain of
-  // a dozen operations of 64 bits is hidden by the other entries of a vector.
+  // a dozen operations of 64 bits is hidden by the other entries of a vector. The exponent ends at -52 (by its upper word: it is never above 0), not the entry at one of 32 bits:
+  // at a small temperature numbers next to each other are further apart than that.
   __device__ __forceinline__ u64 weight(float a) const {
     constexpr double MAGIC = 6755399441055744.0;               // 1.5 2^52: what is added to it is a whole number in the low bits
-    const double t = ((double)fmaxf(a, low) - (double)m) * per16;          // (0 of the largest, whose weight is 2^bits)
+    const double far = ((double)a - (double)m) * per16;                    // (0 of the largest, whose weight is 2^bits)
+    const double t = __hiloint2double((int)min((unsigned)__double2hiint(far), 0xc08a0000u), __double2loint(far));       // -52 16 = -1.625 2^9
     const double n = t + MAGIC;
     const int i = __double2loint(n);
     const double r = t - (n - MAGIC);
@@ -616,8 +618,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const _
     return;
   }
   row.m = most;
-  row.per16 = 16.0 * 1.4426950408889634 / temperature;
-  row.low = fmaxf(most - 33.271065f * (float)temperature, -FLT_MAX);       // 48 log(2)
+  row.per16 = fmax(16.0 * 1.4426950408889634 / temperature, 1e-300);        // (of an infinite one too: minus infinity stays so)
   row.zero = fmaxf(most - 744.44009f * (float)temperature, -FLT_MAX);      // 1074 log(2); minus infinity has no weight at any temperature
   row.power = s.power;
   // Bins of numbers reach three quarters of the way to the mean, which some of the first entries stand for; those of weights twice as far. What is further away lies in
