@@ -7,10 +7,11 @@
 // their sum stands, of these those with w >= min_p. The result is the first v, in the order of the vocabulary, up to which the sum of what stays exceeds u
 // times all of it.
 //
-// Weights are whole numbers of 64 bits, w 2^46 rounded (2^42 at the largest vocabulary): their sums do not depend on an order, so threads add them up as they come,
-// and two runs agree to the bit. Exponentials are of 64 bits, as are shares and thresholds: with 32 the result of one row in some 10^4 would be another one's
-// neighbour (a vocabulary of 50257 has that many borders, each off by some 2^-25). A weight below the last bit counts as one of it: u = 0 still takes the
-// first token that stays.
+// Weights are whole numbers of 64 bits, w 2^46 rounded (2^45 from 2^17 entries on, 2^43 at the largest vocabulary): their sums do not depend on an order, so threads add
+// them up as they come, and two runs agree to the bit. A border, a sum of at most V weights, is off by V 2^-47 of the likeliest one's weight at most (2^-31 for 50257
+// entries, 2^-24 for 2^20), and by the series' 2^-42 of itself. Exponentials are of 64 bits, as are shares and thresholds: with 32 the result of one row in some 10^4 would be
+// another one's neighbour (a vocabulary of 50257 has that many borders, each off by some 2^-25). What is less than half of the last bit counts as nothing; u = 0, which takes the
+// first token that stays whatever its weight, looks for that one.
 //
 // One CTA has a row, or a cluster of them where there are few, and reads it from L2 in every pass but the first: the largest entry; a histogram over bins of equal width of m - x, which says in which bin the k-th
 // entry lies, or about where the share p ends; then, with top-k, all entries up to that bin go to shared memory, are put in order there, and the rest is done
@@ -255,7 +256,7 @@ struct SampleRow {
     return __float_as_uint(t) & (SM_BINS - 1);
   }
   // w 2^bits, w = 2^((a - m) log2(e) / T), of entries from `zero` on: sixteenths of the exponent from a table, what is left of it, at most 2^-5, by the series of
-  // the exponential function up to its fifth power (the sixth is 2^-42 of it), rounded up: what is above 0 counts as 1 at least. Without branches: a chain of
+  // the exponential function up to its fifth power (the sixth is 2^-42 of it), rounded to a whole number. Without branches: a chain of
   // a dozen operations of 64 bits is hidden by the other entries of a vector. The exponent ends at -52 (by its upper word: it is never above 0), not the entry at one of 32 bits:
   // at a small temperature numbers next to each other are further apart than that.
   __device__ __forceinline__ u64 weight(float a) const {
@@ -266,7 +267,7 @@ struct SampleRow {
     const int i = __double2loint(n);
     const double r = t - (n - MAGIC);
     const double e = fma(fma(fma(fma(fma(p.series[4], r, p.series[3]), r, p.series[2]), r, p.series[1]), r, p.series[0]), r, 1.0) * power[i & 15];
-    const double w = __dadd_ru(__hiloint2double(__double2hiint(e) + ((i & ~15) << 16), __double2loint(e)), 4503599627370496.0);       // 2^52
+    const double w = __hiloint2double(__double2hiint(e) + ((i & ~15) << 16), __double2loint(e)) + 4503599627370496.0;       // 2^52
     return __double_as_longlong(w) & 0xfffffffffffffull;
   }
   // The least entry with w >= p.
@@ -512,7 +513,7 @@ __device__ void sm_sort(const SampleRow<T, THREADS>& row, SampleShared& s, int n
   __syncthreads();
 }
 
-// Whole CTA: the smallest index for which `f(entry)`; -1 where there is none.
+// Whole CTA: the smallest index for which `f(entry, index)`; -1 where there is none.
 template <typename T, int THREADS, typename F>
 __device__ int sm_first(const SampleRow<T, THREADS>& row, SampleShared& s, F f) {
   if (threadIdx.x == 0) s.first = 0x7fffffff;
@@ -521,7 +522,7 @@ __device__ int sm_first(const SampleRow<T, THREADS>& row, SampleShared& s, F f) 
   row.template each<2>([&](auto& a, int v0) {
 #pragma unroll
     for (int j = 0; j < (int)(sizeof(a) / sizeof(float)); ++j)
-      if (f(a[j])) best = min(best, v0 + j);
+      if (f(a[j], v0 + j)) best = min(best, v0 + j);
   });
   best = __reduce_min_sync(0xffffffffu, best);
   if ((threadIdx.x & 31) == 0) atomicMin(&s.first, best);
@@ -613,13 +614,14 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const _
     if (MANY && rank) return;
     row.share(0, 1);
     const bool none = most != most;
-    const int v = most == -INFINITY ? -1 : sm_first(row, s, [&](float a) { return none ? a != a : a == most; });
+    const int v = most == -INFINITY ? -1 : sm_first(row, s, [&](float a, int) { return none ? a != a : a == most; });
     if (tid == 0) p.out[b] = v;
     return;
   }
   row.m = most;
   row.per16 = fmax(16.0 * 1.4426950408889634 / temperature, 1e-300);        // (of an infinite one too: minus infinity stays so)
-  row.zero = fmaxf(most - 744.44009f * (float)temperature, -FLT_MAX);      // 1074 log(2); minus infinity has no weight at any temperature
+  // half of 2^-1074, the least number of 64 bits, is none: 1075 log(2). Minus infinity has no weight at any temperature.
+  row.zero = fmaxf(__double2float_ru((double)most - 745.1332191019412 * temperature), -FLT_MAX);
   row.power = s.power;
   // Bins of numbers reach three quarters of the way to the mean, which some of the first entries stand for; those of weights twice as far. What is further away lies in
   // the last.
@@ -667,21 +669,29 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const _
       }
       u64 before = sm_before<THREADS>(sum, s.part, total);
       const double target = top_p * (double)total;
+      int lowest = 0x7fffffff;
 #pragma unroll
       for (int i = 0; i < OWN; ++i) {
         const u64 front = before;
         before += w[i];
+        if (!e[i] || sm_value(e[i]) < row.zero || (top_p < 1 && !((double)front < target)) || sm_value(e[i]) < least_p) w[i] = 0;
+        else lowest = min(lowest, sm_index(e[i]));
         if (w[i] == 0) continue;
-        if ((top_p < 1 && !((double)front < target)) || sm_value(e[i]) < least_p) {
-          w[i] = 0;
-          continue;
-        }
         const int part = row.part_of(sm_index(e[i]));
         const unsigned low = (unsigned)w[i], old = atomicAdd(&s.kept[0][part], low), high = (unsigned)(w[i] >> 32) + (old + low < old);
         if (high) atomicAdd(&s.kept[1][part], high);
       }
-      if (tid == 0) s.n = 0;
+      if (tid == 0) {
+        s.n = 0;
+        s.first = 0x7fffffff;
+      }
       __syncthreads();
+      if (u == 0.f) {                              // the first that stays
+        atomicMin(&s.first, lowest);
+        __syncthreads();
+        if (tid == 0) p.out[b] = s.first;
+        return;
+      }
       const SamplePart at(s, u);
       // ---- the part's own: each is compared with all of them
 #pragma unroll
@@ -851,6 +861,12 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const _
     else __syncthreads();
     if (MANY && rank) return;
   }
+  if (u == 0.f) {                                  // the first that stays
+    row.share(0, 1);
+    const int v = sm_first(row, s, [&](float a, int v) { return a >= from(v); });
+    if (tid == 0) p.out[b] = v;
+    return;
+  }
   const SamplePart here(s, u);
   // ---- the part in which u lies, cut among all threads: vectors next to each other, the first thread with those in front of all vectors, the last with those
   // behind
@@ -916,8 +932,8 @@ using namespace gf;
 GF_API int gf_sample_tokens(const SampleCall* c, void* stream) {
   if (!c || !c->x || !c->u || !c->out || c->B <= 0 || c->B > 0x7fffffff || c->V <= 0 || c->V > SM_MOST || c->dtype < 0 || c->dtype > 2) return GFH_BAD_ARG;
   gf::enter();
-  int bits = 62;                                   // sums of V weights are below 2^62
-  while (bits > 46 || (c->V >> (62 - bits)) > 0) --bits;
+  int bits = 46;                                   // sums of V weights are 2^63 at most
+  while (c->V > 1ll << (63 - bits)) --bits;
   constexpr double C1 = 0.69314718055994530942 / 16;
   const SampleParams p{c->x, c->ldx, c->u, c->temperature, c->top_p, c->min_p, c->top_k, c->temperature0, c->top_p0, c->min_p0,
                        (int)c->top_k0, c->out, (int)c->V, bits, {C1, C1 * C1 / 2, C1 * C1 * C1 / 6, C1 * C1 * C1 * C1 / 24, C1 * C1 * C1 * C1 * C1 / 120}};

@@ -161,7 +161,8 @@ def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     With ``w = exp((x - max x) / temperature)`` and the row's tokens in the order of their logits, equal ones in that of the vocabulary: the first ``top_k`` stay
     (0: all), of these each in front of which less than ``top_p`` of their weights' sum stands (1: all), of these those with ``w >= min_p``, the first
     one in any case. The result is the first token, in the order of the vocabulary, up to which the weights of those that stay exceed ``u`` of their
-    sum. Weights, sums and shares are of 64 bits.
+    sum. Weights, sums and shares are of 64 bits; those of the kernel are whole numbers, whose sums are off by ``V 2^-47`` of the likeliest token's weight (2^-31 for
+    50257 tokens, 2^-24 for 2^20) and by 2^-42 of themselves at most.
 
     The four choices are numbers or one of each row: fp32 ``[B]``, ``top_k`` int32 ``[B]``. A temperature that is not above 0 takes the likeliest token, as do ``top_k`` 1 and
     rows that have no probabilities (that hold what is not a number, or infinity); a row of all ``-inf`` gives -1."""
