@@ -8,7 +8,7 @@
 // times all of it.
 //
 // Weights are whole numbers of 64 bits, w 2^46 rounded (2^45 from 2^17 entries on, 2^43 at the largest vocabulary): their sums do not depend on an order, so threads add
-// them up as they come, and two runs agree to the bit. A border, a sum of at most V weights, is off by V 2^-47 of the likeliest one's weight at most (2^-31 for 50257
+// them up as they come, and two runs agree to the bit. A border, a sum of at most V weights, is off by V / 2 units at most (2^-31 of the likeliest one's weight for 50257
 // entries, 2^-24 for 2^20), and by the series' 2^-42 of itself. Exponentials are of 64 bits, as are shares and thresholds: with 32 the result of one row in some 10^4 would be
 // another one's neighbour (a vocabulary of 50257 has that many borders, each off by some 2^-25). What is less than half of the last bit counts as nothing; u = 0, which takes the
 // first token that stays whatever its weight, looks for that one.

@@ -161,10 +161,11 @@ def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     With ``w = exp((x - max x) / temperature)`` and the row's tokens in the order of their logits, equal ones in that of the vocabulary: the first ``top_k`` stay
     (0: all), of these each in front of which less than ``top_p`` of their weights' sum stands (1: all), of these those with ``w >= min_p``, the first
     one in any case. The result is the first token, in the order of the vocabulary, up to which the weights of those that stay exceed ``u`` of their
-    sum. Weights, sums and shares are of 64 bits; those of the kernel are whole numbers, whose sums are off by ``V 2^-47`` of the likeliest token's weight (2^-31 for
-    50257 tokens, 2^-24 for 2^20) and by 2^-42 of themselves at most.
+    sum. Weights, sums and shares are of 64 bits; those of the kernel are whole numbers, whose sums are off by ``V 2^-47`` of the likeliest token's weight at most (2^-31 for
+    50257 tokens; of more than 2^17 tokens by 2^-28 to 2^-24, that of 2^20) and by 2^-42 of themselves.
 
-    The four choices are numbers or one of each row: fp32 ``[B]``, ``top_k`` int32 ``[B]``. A temperature that is not above 0 takes the likeliest token, as do ``top_k`` 1 and
+    The four choices are numbers or one of each row: fp32 ``[B]``, ``top_k`` int32 ``[B]``. A temperature of 0, or one of a row that is not above 0, takes the likeliest token
+    (a number below 0, or NaN, is refused), as do ``top_k`` 1 and
     rows that have no probabilities (that hold what is not a number, or infinity); a row of all ``-inf`` gives -1."""
     call = None
     if logits.get_device() >= 0 and not _is_compiling():
@@ -206,8 +207,9 @@ def next_tokens(logits, temperature: float = 0.0, tokens=None, token_lens=None, 
     :func:`process_logits` where ``tokens``, a bias or a mask are given: -1 then for a row that they leave nothing of (all ``-inf``), for which
     an embedding has zeros and :func:`process_logits` no penalty. Sampling takes the likeliest token of a row that has no probabilities (it
     holds what is not a number, or infinity). ``prompt``: the number of tokens of every row that are its prompt, in place of ``generated_from``. With
-    ``top_k``, ``top_p``, ``min_p``, a temperature of each row or the random numbers ``u`` themselves it is :func:`sample_tokens` that chooses, from
-    ``torch.rand`` where ``u`` is not given."""
+    ``top_k``, ``top_p``, ``min_p``, a temperature of each row (fp32 ``[B]``) or the random numbers ``u`` themselves it is :func:`sample_tokens` that chooses, from
+    ``torch.rand`` where ``u`` is not given. A temperature alone draws by ``torch.multinomial``: what a seed has given stays. One that is not above 0 (or
+    no number) takes the likeliest token."""
     if tokens is None and any(torch.is_tensor(t) or t != none for t, none in ((repetition, 1), (presence, 0), (frequency, 0))):
         raise ValueError("next_tokens: penalties go with the tokens that they count")
     processed = tokens is not None or bias is not None or allowed is not None
@@ -216,7 +218,11 @@ def next_tokens(logits, temperature: float = 0.0, tokens=None, token_lens=None, 
             generated_from = torch.full((logits.shape[0],), prompt, dtype=torch.int32, device=logits.device)
         logits = process_logits(logits, tokens, token_lens if tokens is not None else None, generated_from if tokens is not None else None,
                                 repetition, presence, frequency, bias, allowed)
-    if u is not None or any(torch.is_tensor(t) or t != none for t, none in ((temperature, temperature), (top_k, 0), (top_p, 1), (min_p, 0))):
+    # one of each row, or the one of all rows in a tensor: that goes the way of a number
+    rows = torch.is_tensor(temperature) and (temperature.numel() != 1 or temperature.dtype is torch.float32 and temperature.shape == logits.shape[:1])
+    if u is not None or rows or any(torch.is_tensor(t) or t != none for t, none in ((top_k, 0), (top_p, 1), (min_p, 0))):
+        if not rows:
+            temperature = float(temperature) if temperature and temperature > 0 else 0.0
         return sample_tokens(logits, torch.rand(logits.shape[0], device=logits.device) if u is None else u, temperature, top_k, top_p, min_p)
     likeliest = chosen = logits.argmax(-1, keepdim=True)
     if temperature and temperature > 0:
