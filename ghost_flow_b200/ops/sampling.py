@@ -223,7 +223,7 @@ def next_tokens(logits, temperature: float = 0.0, tokens=None, token_lens=None, 
     if u is not None or rows or any(torch.is_tensor(t) or t != none for t, none in ((top_k, 0), (top_p, 1), (min_p, 0))):
         if not rows:
             temperature = float(temperature) if temperature and temperature > 0 else 0.0
-        return sample_tokens(logits, torch.rand(logits.shape[0], device=logits.device) if u is None else u, temperature, top_k, top_p, min_p)
+        return sample_tokens(logits, torch.rand(logits.shape[0], dtype=torch.float32, device=logits.device) if u is None else u, temperature, top_k, top_p, min_p)
     likeliest = chosen = logits.argmax(-1, keepdim=True)
     if temperature and temperature > 0:
         # multinomial stops the device at a row that is no distribution; softmax leaves nothing but NaN of one

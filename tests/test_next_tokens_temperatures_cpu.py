@@ -47,3 +47,15 @@ def test_a_temperature_of_each_row():
     for bad in (torch.ones(2), torch.ones(3, dtype=torch.float64), torch.ones(3, 1)):
         with pytest.raises(ValueError, match="temperature"):
             ops.next_tokens(x, bad)
+
+
+@pytest.mark.parametrize("dtype", [torch.float64, torch.bfloat16])
+def test_random_numbers_do_not_go_by_the_default_type(dtype):
+    x = torch.randn(4, 30, dtype=torch.float32)
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(dtype)
+    try:
+        got = ops.next_tokens(x, 0.8, top_k=5)
+    finally:
+        torch.set_default_dtype(before)
+    assert got.shape == (4, 1)
