@@ -243,17 +243,20 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_append_heads_kernel(const
         }
       }
       if (query || key) turn.turn<1>(v, at, A.interleaved);
-      unsigned byte = 0;
-      if constexpr (BYTES) byte = scale_byte<LANES>(v);
       if (query) {
         v.to(x[n], y[n]);
         if (!row.there) x[n] = y[n] = make_uint4(0, 0, 0, 0);              // not the products of what stands there
         __nv_bfloat16* to = A.q + ((long long)t * A.H + h) * D;
         *reinterpret_cast<uint4*>(to + at.x) = x[n];
         *reinterpret_cast<uint4*>(to + at.y) = y[n];
-        continue;
+        if constexpr (!BYTES) continue;
       }
-      if (!row.stored || h >= heads) continue;
+      unsigned byte = 0;
+      if constexpr (BYTES) {                       // (rows of queries have been written: what is not finite in them stays what it is)
+        if (!__any_sync(0xffffffffu, !query)) continue;
+        byte = scale_byte<LANES>(v);
+      }
+      if (query || !row.stored || h >= heads) continue;
       const int hk = h - A.H - (key ? 0 : A.Hk);
       const long long to = key ? row.page * A.kpage + row.r * A.krow + hk * A.khead : row.page * A.vpage + row.r * A.vrow + hk * A.vhead;
       if constexpr (BYTES) {

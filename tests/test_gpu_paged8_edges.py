@@ -1,0 +1,41 @@
+"""Pages of 8 bits at their edges: query heads that are not finite."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+INF, NAN = float("inf"), float("nan")
+E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+
+
+def _pools(pages, page, Hk, D, eight=True):
+    if not eight:
+        return [torch.zeros(pages, page, Hk, D, device="cuda", dtype=torch.bfloat16) for _ in range(2)]
+    return [torch.zeros(pages, page, Hk, D, device="cuda", dtype=torch.uint8).view(E4M3) for _ in range(2)] + [
+        torch.zeros(pages, Hk, page, device="cuda", dtype=torch.uint8).view(E8M0) for _ in range(2)]
+
+
+def _scales(pools):
+    return dict(zip(("kscales", "vscales"), pools[2:]))
+
+
+def _ints(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("H,Hk", [(4, 4), (8, 2), (3, 1)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_queries_that_are_not_finite_stay_what_they_are(H, Hk, D, kernel_status):
+    """Dims that are not rotated pass through: an infinity stays one, beside heads that are turned into 8 bits too."""
+    from ghost_flow_b200 import ops
+
+    T = 5
+    qkv = torch.randn(T, H + 2 * Hk, D, device="cuda").bfloat16()
+    qkv[0, 0, D - 1], qkv[1, H - 1, D - 2], qkv[2, 0, D - 3], qkv[3, H - 1, D - 4] = INF, -INF, NAN, INF
+    qkv[3, H, D - 1] = INF                                      # a key's becomes NaN
+    cos, sin = ops.rope_tables(16, D // 2, 1e4, "cuda")
+    got = {}
+    for eight in (False, True):
+        pools = _pools(2, 16, Hk, D, eight)
+        got[eight] = ops.rope_qkv_to_pages(qkv, H, Hk, cos, sin, *pools[:2], _ints([[1]]), _ints([T]), _ints([0, T]), **_scales(pools))
+    assert torch.equal(got[True].nan_to_num(7.0, 8.0, 9.0), got[False].nan_to_num(7.0, 8.0, 9.0))
+    assert torch.equal(got[True][:, :, D // 2:].nan_to_num(7.0, 8.0, 9.0), qkv[:, :H, D // 2:].nan_to_num(7.0, 8.0, 9.0))
