@@ -401,7 +401,7 @@ def paged_attention(q, kpages, vpages, page_table, lens, cu=None, scale: float |
             return torch.empty_like(q) if out is None else out
     else:
         at, device, B, T, H, Hk, D, keys, packed = call
-    if out is not None and (_ranges_overlap(out, q) or _ranges_overlap(out, kpages) or _ranges_overlap(out, vpages)):
+    if out is not None and any(t is not None and _ranges_overlap(out, t) for t in (q, kpages, vpages, kscales, vscales)):
         raise ValueError(f"{what}: out shares memory with q or the pages")
     if scale is None:
         scale = 1.0 / math.sqrt(D)
