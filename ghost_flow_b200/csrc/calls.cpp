@@ -240,7 +240,7 @@ PyObject* append_heads(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (followed({a[0], a[3], a[4], a[8], a[9], a[12], a[13]})) Py_RETURN_NONE;
   if (!paged(a, a[3], a[4], a[5], a[6], a[7], c, device, heads, packed, bytes) || H <= 0 || H > 65535 || c.Hk != Hk || Hk > 65535 || heads != H + 2 * Hk ||
       (c.D != 32 && c.D != 64 && c.D != 128 && c.D != 256) || !cs.of(a[8]) || !sn.of(a[9]) || (a[11] != Py_None) != bytes ||
-      (bytes && !scales(a[10], a[11], c, device, r.c8.kscales, r.c8.vscales)) || (a[12] == Py_None) != (a[13] == Py_None))
+      (bytes && (!scales(a[10], a[11], c, device, r.c8.kscales, r.c8.vscales) || !gf::paged_scales_apart(r.c8))) || (a[12] == Py_None) != (a[13] == Py_None))
     Py_RETURN_NONE;
   for (const View* t : {&cs, &sn})
     if (!t->is(FLOAT, 32, 2, device) || t->shape[1] % 8 || 2 * t->shape[1] > c.D || t->shape[1] != cs.shape[1] || t->shape[0] != cs.shape[0] ||

@@ -2,6 +2,8 @@
 // in any language can pack them.
 #pragma once
 
+#include <initializer_list>
+
 namespace gf {
 
 struct PagedCall {
@@ -23,6 +25,18 @@ struct PagedCall8 {
   PagedCall c;
   const unsigned char *kscales, *vscales;
 };
+
+// Whether the scales lie outside the pools, from the first row to the last.
+inline bool paged_scales_apart(const PagedCall8& r) {
+  const PagedCall& c = r.c;
+  for (int i = 0; i < 2; ++i) {
+    const char* pool = (const char*)(i ? c.vpages : c.kpages);
+    const char* end = pool + (c.pages - 1) * c.strides[3 * i] + (c.page - 1) * c.strides[3 * i + 1] + (c.Hk - 1) * c.strides[3 * i + 2] + c.D;
+    for (const unsigned char* s : {r.kscales, r.vscales})
+      if ((const char*)s < end && pool < (const char*)s + c.pages * c.Hk * c.page) return false;
+  }
+  return true;
+}
 
 struct LogitsCall {
   const void* x;                 // [B, V] of dtype (0 fp32, 1 bf16, 2 fp16), rows ldx apart

@@ -343,7 +343,7 @@ GF_API int gf_paged_append(const PagedCall* c, const float* cos, const float* si
 }
 
 // The same with heads that are normed (qw, kw [D]; null: not) and of which `rotary` dims are rotated (tables [positions, rotary / 2]), into pages of bf16 (no
-// scales) or of 8 bits. GFH_OVERLAP where x shares memory with the pools or scales. D of 32, 64, 128 or 256.
+// scales) or of 8 bits. GFH_OVERLAP where x shares memory with the pools or scales, or these with each other. D of 32, 64, 128 or 256.
 GF_API int gf_paged_append_heads(const PagedCall8* c8, const float* cos, const float* sin, int positions, int rotary, int interleaved, const void* qw,
                                  const void* kw, float eps, void* stream) {
   PagedHeads p{};
@@ -362,6 +362,7 @@ GF_API int gf_paged_append_heads(const PagedCall8* c8, const float* cos, const f
     if (c->pages > 0 && x0 < pool + size * ((c->pages - 1) * st[0] + (c->page - 1) * st[1] + (Hk - 1) * st[2] + D) && pool < x1) return GFH_OVERLAP;
     if (scales && x0 < scales + c->pages * c->page * Hk && scales < x1) return GFH_OVERLAP;
   }
+  if (c8->kscales && c->pages > 0 && !paged_scales_apart(*c8)) return GFH_OVERLAP;
   gf::enter();
   PagedAppend& a = p.a;
   a.qkv = (const __nv_bfloat16*)c->x; a.ldx = c->ldx;

@@ -214,6 +214,8 @@ def rope_qkv_to_pages(qkv, num_heads: int, num_kv_heads: int, cos, sin, kpages, 
             return qkv.new_zeros(T, H, D)
         if kpages.numel() and not _observed() and any(t is not None and _ranges_overlap(qkv, t) for t in (kpages, vpages, kscales, vscales)):
             raise ValueError(f"{what}: qkv shares memory with the pages")
+        if kscales is not None and kpages.numel() and not _observed() and any(_ranges_overlap(t, x) for t in (kscales, vscales) for x in (kpages, vpages)):
+            raise ValueError(f"{what}: the scales share memory with the pages")
         if heads:
             return _append_heads_ref(qkv, H, Hk, cos, sin, kpages, vpages, page_table, lens, cu, interleaved, *more, eps)
         return _append_ref(qkv, H, Hk, cos, sin, kpages, vpages, page_table, lens, cu, interleaved)

@@ -41,3 +41,31 @@ def test_results_over_the_scales_are_refused(device, which):
             ops.paged_attention(q, *pools, *_batch(device), out=out, **scales)
     else:
         assert ops.paged_attention(q, *pools, *_batch(device), out=out, **scales) is out
+
+
+def _append(device, pools, scales):
+    qkv = torch.randn(T, H + 2 * HK, D, device=device).bfloat16()
+    cos, sin = ops.rope_tables(64, D, 1e4, device)
+    return ops.rope_qkv_to_pages(qkv, H, HK, cos, sin, *pools, *_batch(device), **scales)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("scale", [0, 1])
+@pytest.mark.parametrize("pool", [0, 1])
+@pytest.mark.parametrize("where", ["first", "middle", "last"])
+def test_scales_within_the_pages_are_refused(device, scale, pool, where):
+    arena = torch.zeros(2 * POOL + 3 * SCALES, dtype=torch.uint8, device=device)
+    at = [2 * POOL + SCALES, 2 * POOL + 2 * SCALES]
+    at[scale] = pool * POOL + dict(first=0, middle=POOL // 2, last=POOL - 16)[where]
+    pools, scales = _tensors(arena, 0, POOL, *at)
+    with pytest.raises(ValueError, match="share"):
+        _append(device, pools, scales)
+    assert not arena.any()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_scales_behind_the_pages_are_written(device):
+    arena = torch.zeros(2 * POOL + 2 * SCALES, dtype=torch.uint8, device=device)
+    pools, scales = _tensors(arena, 0, POOL, 2 * POOL, 2 * POOL + SCALES)
+    _append(device, pools, scales)
+    assert all(t.view(torch.uint8).any() for t in (*pools, *scales.values()))
