@@ -9,7 +9,7 @@ what they hold when it is replayed. A sequence of no new tokens, or of no keys (
 
 Pools of ``torch.float8_e4m3fn`` hold a row of a head in 8 bits, as numbers times a power of two of its own: ``kscales`` and ``vscales``
 ``[pages, Hk, page]`` of ``torch.float8_e8m0fnu``, each the smallest from 2^-126 that leaves no number of the row above 448, so that none is cut off. What
-is not finite is kept as NaN. :func:`read_pages` gives rows back; such pools are written and read without gradients.
+is not finite is kept as NaN, as is a number of 64 bits that is above 448 times 2^127. :func:`read_pages` gives rows back; such pools are written and read without gradients.
 
 bf16 CUDA tensors take the kernels of ``csrc/paged_cache.cu`` and ``csrc/attn_paged.cu`` (through ``csrc/calls.cpp``); other types, layouts and CPU tensors, and calls that
 something follows (a gradient, tracing, transforms, modes), plain PyTorch. The reference has no cache (ghostflow-nn/src/gpt.rs:402-422).
@@ -110,7 +110,7 @@ def _in_8_bits(y):
     """Rows ``[.., D]`` of 32 or 64 bits as numbers of type e4m3, and the bytes ``[..]`` of their powers of two; both as bytes."""
     finite = y.isfinite()
     f, x = torch.frexp(torch.where(finite, y, 0).abs().amax(-1))                # 448 = 0.875 2^9
-    byte = (torch.where(f > 0, x + 118 + (f > 0.875).int(), 0)).clamp(min=1).to(torch.uint8)
+    byte = (torch.where(f > 0, x + 118 + (f > 0.875).int(), 0)).clamp(1, 254).to(torch.uint8)
     return torch.where(finite, y / _power_of(byte).unsqueeze(-1).to(y.dtype), float("nan")).to(_E4M3).view(torch.uint8), byte
 
 
