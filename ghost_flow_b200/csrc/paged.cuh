@@ -55,7 +55,7 @@ inline bool paged_batch(PagedBatch& s, const PagedCall& c) {
   return true;
 }
 
-// 16 numbers of the cache times their row's power of two (twice, as f32x2), as bf16: exact
+// 16 numbers of the cache times their row's power of two (twice, as f32x2), as bf16: exact but for what is below 2^-133, of rows of the two least units
 __device__ __forceinline__ void bf16x16_of_e4m3(const uint4& in, uint64_t scale, uint4& lo, uint4& hi) {
   const uint32_t* four = reinterpret_cast<const uint32_t*>(&in);
   uint32_t out[8];
@@ -74,7 +74,7 @@ __device__ __forceinline__ void bf16x16_of_e4m3(const uint4& in, uint64_t scale,
 
 // Pages of 8 bits. A row of a head is numbers of type e4m3 times 2^(b - 127), b the row's byte in the scales: the smallest power of two that leaves none of them
 // above 448, the type's largest, so that none is cut off; and at least 2^-126. A power of two loses no bits in what it is multiplied with: a number of the
-// cache has 4 bits, and is one of bf16 too. (A scale that brings the largest number to 448 itself gains nothing: the type's steps are
+// cache has 4 bits, and is one of bf16 too, where it is not below 2^-133. It is off by 2^-4 of itself or, from 2^-6 of the unit on down, by 2^-10 of the unit. (A scale that brings the largest number to 448 itself gains nothing: the type's steps are
 // relative.) Scales of a head lie one behind the other, so that 16 keys' are 16 bytes.
 inline bool paged_scales(const PagedCall8& c8) {
   const PagedCall& c = c8.c;

@@ -241,7 +241,7 @@ def rope_qkv_to_pages(qkv, num_heads: int, num_kv_heads: int, cos, sin, kpages, 
 
 def read_pages(rows: int, kpages, vpages, page_table, lens, cu=None, kscales=None, vscales=None):
     """Keys and values ``[rows, Hk, D]`` of the new tokens of a batch (see the module; a sequence's are all of its keys where ``cu`` says so), as they stand in
-    the pages: of pages of 8 bits the numbers that they stand for, as bf16, which has all of their bits. Tokens that have no row there, and those behind
+    the pages: of pages of 8 bits the numbers that they stand for, as bf16, which has all of their bits (from 2^-133 on). Tokens that have no row there, and those behind
     the last sequence, give zeros; a page that is not in the pools, or a position behind the page table, does too, and ``_lib.check_status`` raises."""
     call = None
     if kpages.get_device() >= 0 and not _is_compiling():

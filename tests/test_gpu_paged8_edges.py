@@ -1,4 +1,4 @@
-"""Pages of 8 bits at their edges: query heads that are not finite."""
+"""Pages of 8 bits at their edges: query heads that are not finite, rows of the least powers of two."""
 import pytest
 import torch
 
@@ -39,3 +39,26 @@ def test_queries_that_are_not_finite_stay_what_they_are(H, Hk, D, kernel_status)
         got[eight] = ops.rope_qkv_to_pages(qkv, H, Hk, cos, sin, *pools[:2], _ints([[1]]), _ints([T]), _ints([0, T]), **_scales(pools))
     assert torch.equal(got[True].nan_to_num(7.0, 8.0, 9.0), got[False].nan_to_num(7.0, 8.0, 9.0))
     assert torch.equal(got[True][:, :, D // 2:].nan_to_num(7.0, 8.0, 9.0), qkv[:, :H, D // 2:].nan_to_num(7.0, 8.0, 9.0))
+
+
+@pytest.mark.parametrize("byte", [1, 2, 3, 4, 9, 127, 246])
+def test_every_number_of_a_row_read_back(byte, kernel_status):
+    """bf16 has all bits of a number of the pages, but for those below 2^-133, of rows of the two least units: these are rounded to the nearest, by the kernel as by PyTorch."""
+    from ghost_flow_b200 import ops
+
+    pools = _pools(2, 16, 2, 128)
+    codes = torch.arange(256, dtype=torch.uint8, device="cuda").view(2, 128)
+    for pool, scale in zip(pools[:2], pools[2:]):
+        pool.view(torch.uint8)[1, 3] = codes
+        scale.view(torch.uint8)[1, :, 3] = byte
+    got = ops.read_pages(1, *pools[:2], _ints([[1]]), _ints([4]), **_scales(pools))
+    exact = codes.cpu().view(E4M3).double() * 2.0 ** (byte - 127)
+    for x in got:
+        x = x[0].cpu()
+        assert torch.equal(x.isnan(), exact.isnan()) and x.isnan().sum() == 2
+        assert torch.equal(x.nan_to_num(0.0), exact.bfloat16().nan_to_num(0.0))
+        if byte > 2:
+            assert torch.equal(x.double().nan_to_num(0.0), exact.nan_to_num(0.0))
+    cpu = ops.read_pages(1, *(t.cpu() for t in pools[:2]), _ints([[1]]).cpu(), _ints([4]).cpu(), **{n: t.cpu() for n, t in _scales(pools).items()})
+    for a, b in zip(got, cpu):
+        assert torch.equal(a.cpu().view(torch.int16), b.view(torch.int16)) or torch.equal(a.cpu().nan_to_num(0.0), b.nan_to_num(0.0))
