@@ -660,7 +660,23 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
       }
       const float mref_use = (m_ref == -INFINITY) ? 0.f : m_ref;  // row with no visible key yet
-      const float mneg = -mref_use * sl2;
+      float mneg = -mref_use * sl2;
+      // 2^(s sl2 - m sl2) in one operation has the rounding of m sl2 in the exponent, the same for the whole row: nothing up to 2^14, at 2^31 all of the range. Where a
+      // row is further up, m is taken off its warp's scores first. (The vote, us: 512 tokens over 7681 keys 73.6 / 74.0, 8 x 1024 of 12 heads of 64 49.1 / 49.9; looked at only
+      // where m moves, 73.3 and 50.9.)
+      if (__any_sync(0xffffffffu, fabsf(mneg) >= 0x1p14f)) {
+#pragma unroll 1
+        for (int c = 0; c < PG_TILE / 32; ++c) {
+          uint32_t far[32];
+          tmem_ld32(ts + c * 32, far);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) far[i] = __float_as_uint(__uint_as_float(far[i]) - mref_use);
+          tmem_st32(ts + c * 32, far);
+        }
+        tmem_st_wait();
+        mneg = 0.f;
+      }
       const uint64_t sl2x = pk2f(sl2, sl2), mnegx = pk2f(mneg, mneg);
       uint64_t rsa = 0, rsb = 0;
       uint32_t sa[32], sb[32];

@@ -1,4 +1,5 @@
-"""Pages of 8 bits at their edges: query heads that are not finite, rows of the least powers of two."""
+"""Pages of 8 bits at their edges: query heads that are not finite, rows of the least powers of two, scores of any size in prompts
+(of either type of pages)."""
 import pytest
 import torch
 
@@ -62,3 +63,42 @@ def test_every_number_of_a_row_read_back(byte, kernel_status):
     cpu = ops.read_pages(1, *(t.cpu() for t in pools[:2]), _ints([[1]]).cpu(), _ints([4]).cpu(), **{n: t.cpu() for n, t in _scales(pools).items()})
     for a, b in zip(got, cpu):
         assert torch.equal(a.cpu().view(torch.int16), b.view(torch.int16)) or torch.equal(a.cpu().nan_to_num(0.0), b.nan_to_num(0.0))
+
+
+# Keys are multiples of a row of ones by different numbers of at most 8 bits, so scores are exact in 32 bits and, at these sizes, thousands apart: a token's result is the value
+# of the largest key that it sees, of bf16 and of e4m3 numbers alike.
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("power", [10, 14, 18, 22, 26, 60, 100])
+@pytest.mark.parametrize("lens,new,H,Hk", [([300], [300], 4, 2), ([3000], [40], 8, 2), ([700, 5, 260], [130, 5, 2], 4, 4)])
+def test_scores_of_any_size_in_prompts(eight, D, power, lens, new, H, Hk, kernel_status):
+    from ghost_flow_b200 import ops
+
+    page, B = 64, len(lens)
+    width = -(-max(lens) // page)
+    table = torch.randperm(B * width, device="cuda").int().view(B, width)
+    pools = _pools(B * width, page, Hk, D, eight)
+    rank = torch.rand(B * width, page, Hk, device="cuda")
+    k = (rank * 15).floor() + 1                                 # of 4 bits; of equal ones any may stand in front
+    v = torch.randint(-8, 9, (B * width, page, Hk, D), device="cuda").float() / 8
+    sign = torch.where(torch.rand(D, device="cuda") < 0.5, -1.0, 1.0)
+    kk = k[..., None] * sign
+    for x, pool, scale in zip((kk, v), pools, pools[2:] if eight else (None, None)):
+        pool.view(torch.uint8 if eight else torch.bfloat16).copy_(x.to(E4M3).view(torch.uint8) if eight else x.bfloat16())
+        if eight:
+            scale.view(torch.uint8).fill_(127)
+    T = sum(new)
+    q = (sign * 2.0 ** power).expand(T, H, D).bfloat16().contiguous()
+    cu = _ints([0, *torch.tensor(new).cumsum(0).tolist()])
+    got = ops.paged_attention(q, *pools[:2], table, _ints(lens), cu, **_scales(pools))
+    at = 0
+    for b in range(B):
+        n, length = new[b], lens[b]
+        rows = [x[table[b].long()].flatten(0, 1)[:length].double() for x in (kk, v)]
+        s = torch.einsum("thgd,nhd->hgtn", q[at:at + n].double().unflatten(1, (Hk, H // Hk)), rows[0]) * D ** -0.5
+        hidden = torch.arange(length, device="cuda") > (length - n + torch.arange(n, device="cuda"))[:, None]
+        p = torch.softmax(s.masked_fill(hidden, -INF), -1)
+        want = torch.einsum("hgtn,nhd->thgd", p, rows[1]).flatten(1, 2)
+        # a weight is rounded to bf16, and the result, of values up to 1
+        assert (got[at:at + n].double() - want).abs().max().item() <= 2 * 2.0 ** -8
+        at += n
