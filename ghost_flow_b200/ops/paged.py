@@ -304,19 +304,22 @@ def _parts_beside(heads: int, sms: int) -> int:
 @functools.lru_cache(maxsize=4096)
 def _parts_of_8_bits(heads: int, keys: int, sms: int, kv_heads: int) -> int:
     """The same over pages of 8 bits: parts of each of ``heads`` (sequences times KV heads) of at most ``keys`` keys, or, negative, the number of parts of all
-    sequences together. Four CTAs are on an SM. A unit of 64 keys takes a CTA .57 us alone and 1.55 on a full machine, waves that are not full count half as if
-    they were, and joining 3 us and .12 for each part. Shares of all sequences where there are 27 units to a CTA and sequences of 4096 keys. us with 1 / 2 / 4 / 8 / 16
-    parts / shares, heads of 128: 32 sequences of 100 .. 4096 keys, 32 / 8 heads 49 / 43 / 38 / 41 / 55 / 34 (shares), 4 of 20011 .. 30001, 64 / 8 heads 268 / 139 / 74 /
-    47 / 45 / 47 (16), 16 of 1000 .. 4000 45 / 31 / 28 / 31 / 42 / 31 (4), 16 of 2000, 32 / 32 heads 46 / 52 / 53 / 61 / 84 / 51 (1), 1 of 8000, 32 / 8 heads 72 / 40 /
-    23 / 14 / 12 / 19 (16)."""
+    sequences together. Four CTAs are on an SM. us: a unit of 64 keys takes a CTA .4 alone and 1.2 on a full machine; of the CTAs beyond a wave each further wave .7 of the
+    first one (lengths differ) and 8 for its beginnings and ends; joining 1.5 and .2 for each part, 1 more for 16. Shares of all sequences, whose cost does not go by the longest one,
+    where there are 20 units to a CTA, 32 of a sequence, and 16 parts of each would be more than a wave: at their ends both ways take the same.
+
+    Over 2248 combinations of 1 to 159 sequences, 1 to 40 heads of 64 and 128 and 128 to 41000 keys, lengths all full / uniform / one in eight full and the others a 16th, the choice takes 4 / 2
+    / 3 % longer than the best of all on average, 51 % at most; what knows all but the lengths could have 2 %. us with 1 / 2 / 4 / 8 / 16 parts / shares, 32 / 8 heads of 128, uniform lengths:
+    31 sequences of up to 4096 keys 45 / 44 / 39 / 41 / 55 / 38 (shares), 4032 keys 45 / 37 / 36 / 37 / 49 / 34 (shares), 96 of 2048 47 / 51 / 57 / 72 / 107 / 51 (shares), 40 of 2048
+    27 / 29 / 30 / 36 / 52 / 29 (2), 16 of 4096 38 / 27 / 22 / 24 / 32 / 27 (5), 2 of 8000 42 / 26 / 16 / 12 / 12 / 18 (16)."""
     slots, units = 4 * sms, (keys + 63) // 64
-    if units >= 64 and heads * units >= 27 * slots:
+    if units >= 32 and heads * units >= 20 * slots and 16 * heads > slots:
         return -max(1, slots // kv_heads)
 
     def cost(s):
         full = heads * s / slots
-        waves = 1.0 if full <= 1 else (full + math.ceil(full)) / 2
-        return -(-units // s) * (.57 + .98 * min(1.0, full)) * waves + (3 + .12 * s if s > 1 else 0)
+        beyond = max(0.0, full - 1)
+        return -(-units // s) * (.4 + .8 * min(1.0, full)) * (1 + .7 * beyond) + 8 * beyond + (1.5 + .2 * s + (s > 8) if s > 1 else 0)
 
     return min((s for s in _SLICES if s <= max(1, units)), key=cost)
 
