@@ -25,8 +25,8 @@
 // of 64, 64 / 8 heads of 64 3.1 / 3.2.
 //
 // Pages of 8 bits (see `unit`): the numbers become f16 operands, two to an instruction, without a product, and four CTAs are on an SM. 32 sequences of 100 .. 4096
-// keys, 32 / 8 heads of 128: 34 us (132 MB, 4 TB/s), pages of bf16 47; 4 of 20011 .. 30001, 64 / 8 heads 45 (4.7 TB/s), 71. Half of the issue slots are taken; the loads' path bounds it: without
-// them the second takes 37. Tried and taken back: the products of one unit beside the softmax of the one in front (slower, registers).
+// keys, 32 / 8 heads of 128: 34 us (132 MB, 4 TB/s), pages of bf16 47; 4 of 20011 .. 30001, 64 / 8 heads 45 (4.7 TB/s), 71. Nothing is full (issue slots 52 %, DRAM 55 %, tensor pipe 13 %): a unit's
+// chain of copies, conversion, products and exponentials, of which four CTAs are on an SM; without its loads the second takes 37. Tried and taken back: the products of one unit beside the softmax of the one in front (slower, registers).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 

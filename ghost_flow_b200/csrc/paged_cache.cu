@@ -11,7 +11,7 @@
 //
 // Heads that are normed or rotated in part, and pages of 8 bits, have a kernel of their own (the one without them is as it was): the same CTA to a token, with
 // D / 16 neighbouring lanes to a head (norm_rope.cuh), whose sum of squares, and largest number, are shuffles. Rows read back are written out as bf16, which
-// has all of their bits. The same five prompts with norms into pages of 8 bits, and read back: 51 and 24 us (185 and 112 MB, of which 28 and 17; with the vectors of a lane far apart 81 together);
+// has all of their bits from 2^-133 on. The same five prompts with norms into pages of 8 bits, and read back: 49 and 24 us (185 and 112 MB, of which 28 and 17; with the vectors of a lane far apart 81 together);
 // 64 sequences of one token 3.0 and 2.5. Issue slots are 62 % taken: a number is normed, rotated, compared and rounded to 8 bits by itself.
 #include <type_traits>
 

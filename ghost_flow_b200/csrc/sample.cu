@@ -21,8 +21,8 @@
 // entries that are all equal are counted off in the order of the vocabulary.
 //
 // What bounds it: the instructions of an entry's weight (a table of 16 powers and a series, 64 bits), of its bin and its atomic addition, not the 6.6 TB/s that
-// the first pass reaches. 512 rows of 50257 in bf16, of which memory wants 8 us: the likeliest 17 us, weights of all 59, k = 50 48, p = 0.9 126, p of the least
-// 35; 32 bits, 16 us: 22, 55, 50, 109, 31. 64 rows in bf16: 6, 19, 18, 38, 15; 3 rows of 32000: 5, 12, 14, 26, 12.
+// the first pass reaches. 512 rows of 50257 in bf16, of which memory wants 8 us: the likeliest 17 us, weights of all 60, k = 50 48, p = 0.9 128, p of the least
+// 35; 32 bits, 16 us: 22, 54, 51, 109, 31. 64 rows in bf16: 6, 19, 18, 38, 15; 3 rows of 32000: 5, 12, 14, 26, 12.
 #include <cfloat>
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>

@@ -139,7 +139,7 @@ class GPTForCausalLM(Module):
 
     @torch.no_grad()
     def generate(self, ids, max_new_tokens: int, temperature: float = 0.0, **choice):
-        """``choice``: penalties, bias and mask of :func:`~ghost_flow_b200.ops.sampling.next_tokens`."""
+        """``choice``: penalties, bias, mask, top-k, top-p and min-p of :func:`~ghost_flow_b200.ops.sampling.next_tokens`."""
         was_training = self.training
         self.eval()
         t = self.transformer
